@@ -297,6 +297,96 @@ int vi_bin_gaussians(int P, int image_width, int image_height, const int* radii,
                      uint64_t scratch_bytes, uint32_t* point_list, uint32_t* tile_ids, uint32_t* ranges,
                      void* stream);
 
+/*
+ * ---- Per-pixel heads (extension) ----
+ * No counterpart in the reference, whose user code takes the rendered feature
+ * image [F_out, H, W] from here.  Dense layers on the pixels of such an image,
+ * and the loss of a linear classifier over a vocabulary of labels, both as one
+ * matrix product with its epilogue, in forward and backward.
+ *
+ * A vi_matrix is a 2D view: element (r, c) lies at data + r * row_stride +
+ * c * col_stride, strides in elements (0 and any order allowed for inputs).  A
+ * feature image [K, H*W] is the matrix of H*W rows and K columns with strides
+ * (1, H*W); results are best asked for in the same order.  data NULL in an
+ * optional argument means it is absent.  All matrices and vectors of a call
+ * share one element type (vi_dtype) unless stated otherwise; sums are float32.
+ *
+ * scratch is device memory, 256-byte aligned, of at least the bytes that the
+ * matching _scratch_bytes query returns for the same arguments (0 from a query
+ * means the arguments are invalid: see vi_last_error).  It may be reused by
+ * later work of the same stream as soon as the call returns.
+ */
+typedef enum vi_dtype { VI_F32 = 0, VI_F16 = 1, VI_BF16 = 2 } vi_dtype;
+typedef enum vi_activation {
+  VI_ACT_NONE = 0,
+  VI_ACT_RELU = 1,
+  VI_ACT_SILU = 2,   /* z / (1 + exp(-z)) */
+  VI_ACT_GELU = 3,   /* z * Phi(z), Phi the normal distribution function */
+  VI_ACT_SIGMOID = 4
+} vi_activation;
+typedef enum vi_reduction { VI_REDUCE_NONE = 0, VI_REDUCE_MEAN = 1, VI_REDUCE_SUM = 2 } vi_reduction;
+typedef struct vi_matrix {
+  void* data;
+  int64_t rows, cols, row_stride, col_stride;
+} vi_matrix;
+
+/*
+ * y = act(x weight^T + bias) + residual.  x [M,K], weight [N,K], bias [N] (or
+ * NULL), residual [M,N] (or NULL), y [M,N] with one of its strides 1 and rows
+ * or columns that do not overlap.  dact (or NULL; same shape and strides as y)
+ * receives act'(x weight^T + bias), which the backward needs unless the
+ * activation is VI_ACT_NONE.  K and N are at least 1, M may be 0.
+ */
+uint64_t vi_linear_act_forward_scratch_bytes(int dtype, int activation, const vi_matrix* x, const vi_matrix* weight,
+                                             const void* bias, const vi_matrix* residual, const vi_matrix* y,
+                                             const vi_matrix* dact);
+int vi_linear_act_forward(int dtype, int activation, const vi_matrix* x, const vi_matrix* weight, const void* bias,
+                          const vi_matrix* residual, const vi_matrix* y, const vi_matrix* dact, void* scratch,
+                          uint64_t scratch_bytes, void* stream);
+
+/*
+ * Gradients of vi_linear_act_forward for an incoming dy [M,N] (any strides):
+ * with s = dy * dact (dact NULL: s = dy), dx = s weight, dweight = s^T x, dbias
+ * = the column sums of s.  Each of dx, dweight, dbias may be NULL; dx and
+ * dweight have one of their strides 1.  The residual's gradient is dy itself.
+ */
+uint64_t vi_linear_act_backward_scratch_bytes(int dtype, const vi_matrix* dy, const vi_matrix* dact,
+                                              const vi_matrix* x, const vi_matrix* weight, const vi_matrix* dx,
+                                              const vi_matrix* dweight, const void* dbias);
+int vi_linear_act_backward(int dtype, const vi_matrix* dy, const vi_matrix* dact, const vi_matrix* x,
+                           const vi_matrix* weight, const vi_matrix* dx, const vi_matrix* dweight, void* dbias,
+                           void* scratch, uint64_t scratch_bytes, void* stream);
+
+/*
+ * Softmax cross entropy of the logits z = x weight^T + bias, which are never
+ * stored: loss_m = log(sum_v exp(z_mv)) - z_m,target[m].  x [M,K], weight
+ * [V,K], bias [V] (or NULL), target [M] int64.  Rows whose target equals
+ * ignore_index have loss 0 and no part in any gradient, whatever their features
+ * hold.  Any other target outside [0, V) makes its row's loss NaN.  loss
+ * (float32): [M] for VI_REDUCE_NONE, else one value, the sum over the rows or
+ * their mean over the rows not ignored (NaN when there are none).  lse [M]
+ * (float32) is what the backward needs.
+ */
+uint64_t vi_linear_ce_forward_scratch_bytes(int dtype, const vi_matrix* x, const vi_matrix* weight, const void* bias);
+int vi_linear_ce_forward(int dtype, const vi_matrix* x, const vi_matrix* weight, const void* bias,
+                         const int64_t* target, int64_t ignore_index, int reduction, float* loss, float* lse,
+                         void* scratch, uint64_t scratch_bytes, void* stream);
+
+/*
+ * Gradients of vi_linear_ce_forward: with g_m the incoming gradient of row m's
+ * loss (dloss float32, [M] for VI_REDUCE_NONE, else one value) and
+ * G = g_m (softmax(z_m) - onehot(target_m)): dx = G weight, dweight = G^T x,
+ * dbias = the column sums of G.  The logits are computed again, in pieces of
+ * the vocabulary.  Each of dx, dweight, dbias may be NULL; dx and dweight have
+ * one of their strides 1.
+ */
+uint64_t vi_linear_ce_backward_scratch_bytes(int dtype, const vi_matrix* x, const vi_matrix* weight, const void* bias,
+                                             const vi_matrix* dx, const vi_matrix* dweight, const void* dbias);
+int vi_linear_ce_backward(int dtype, const vi_matrix* x, const vi_matrix* weight, const void* bias,
+                          const int64_t* target, int64_t ignore_index, int reduction, const float* lse,
+                          const float* dloss, const vi_matrix* dx, const vi_matrix* dweight, void* dbias,
+                          void* scratch, uint64_t scratch_bytes, void* stream);
+
 /* Reads the status word a forward latched in its geometry buffer (blocks). */
 int vi_read_device_status(const char* geom_buffer, uint32_t* status, void* stream);
 

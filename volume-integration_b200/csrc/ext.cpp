@@ -355,6 +355,165 @@ std::tuple<Tensor, Tensor, Tensor> bin_gaussians(const Tensor& radii, const Tens
   return {point_list, tile_ids, ranges};
 }
 
+// ---- per-pixel heads ----
+namespace {
+
+int head_dtype(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return VI_F32;
+    case torch::kFloat16: return VI_F16;
+    case torch::kBFloat16: return VI_BF16;
+    default: TORCH_CHECK(false, name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
+  }
+}
+// What every tensor of a heads call must share with x.
+void head_like(const Tensor& t, const Tensor& x, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == x.device(), name, " must be on ", x.device(), ", got ", t.device());
+  TORCH_CHECK(t.scalar_type() == x.scalar_type(), name, " must be ", x.scalar_type(), ", got ", t.scalar_type());
+}
+vi_matrix head_matrix(const Tensor& t) { return {t.data_ptr(), t.size(0), t.size(1), t.stride(0), t.stride(1)}; }
+// The 2D matrix of an optional tensor; nullptr when there is none.
+struct OptMatrix {
+  vi_matrix m{};
+  bool on;
+  OptMatrix(const c10::optional<Tensor>& t, const Tensor& x, const char* name) : on(t.has_value()) {
+    if (!on) return;
+    head_like(*t, x, name);
+    TORCH_CHECK(t->dim() == 2, name, " must be 2D");
+    m = head_matrix(*t);
+  }
+  const vi_matrix* get() const { return on ? &m : nullptr; }
+};
+void head_check(const Tensor& x, const Tensor& weight) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  TORCH_CHECK(x.dim() == 2 && weight.dim() == 2, "x and weight must be 2D");
+  head_like(weight, x, "weight");
+}
+Tensor head_bias(const c10::optional<Tensor>& bias, const Tensor& x, const Tensor& weight) {
+  if (!bias.has_value()) return {};
+  head_like(*bias, x, "bias");
+  TORCH_CHECK(bias->dim() == 1 && bias->size(0) == weight.size(0), "bias must be [", weight.size(0), "]");
+  return bias->contiguous();
+}
+Tensor head_target(const Tensor& target, const Tensor& x) {
+  TORCH_CHECK(target.is_cuda() && target.device() == x.device(), "target must be on ", x.device());
+  TORCH_CHECK(target.scalar_type() == torch::kInt64 && target.dim() == 1 && target.size(0) == x.size(0),
+              "target must be int64 [", x.size(0), "]");
+  return target.contiguous();
+}
+void* head_ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// A new [rows, cols] in x's memory order: columns contiguous unless x is [K, rows] in memory.
+Tensor head_result(const Tensor& x, int64_t rows, int64_t cols) {
+  const bool image = x.stride(0) == 1 && x.stride(1) != 1;
+  return image ? torch::empty({cols, rows}, x.options()).t() : torch::empty({rows, cols}, x.options());
+}
+Tensor head_scratch(uint64_t bytes, const Tensor& x) {
+  TORCH_CHECK(bytes > 0, "volume_integration: ", vi_last_error());
+  return torch::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8));
+}
+
+// (y, act' or None)
+std::tuple<Tensor, c10::optional<Tensor>> linear_act_forward(const Tensor& x, const Tensor& weight,
+                                                             const c10::optional<Tensor>& bias,
+                                                             const c10::optional<Tensor>& residual, int64_t activation,
+                                                             bool want_dact) {
+  head_check(x, weight);
+  const at::cuda::OptionalCUDAGuard guard(x.device());
+  const int dt = head_dtype(x, "x");
+  const Tensor b = head_bias(bias, x, weight);
+  const OptMatrix r(residual, x, "residual");
+  const vi_matrix mx = head_matrix(x), mw = head_matrix(weight);
+  Tensor y = head_result(x, x.size(0), weight.size(0));
+  c10::optional<Tensor> dact;
+  vi_matrix my = head_matrix(y), md{};
+  if (want_dact) {
+    dact = torch::empty_like(y);
+    md = head_matrix(*dact);
+  }
+  const uint64_t n = vi_linear_act_forward_scratch_bytes(dt, (int)activation, &mx, &mw, head_ptr(b), r.get(), &my,
+                                                         want_dact ? &md : nullptr);
+  Tensor scratch = head_scratch(n, x);
+  ok(vi_linear_act_forward(dt, (int)activation, &mx, &mw, head_ptr(b), r.get(), &my, want_dact ? &md : nullptr,
+                           scratch.data_ptr(), n, at::cuda::getCurrentCUDAStream().stream()));
+  return {y, dact};
+}
+
+using Grads = std::tuple<c10::optional<Tensor>, c10::optional<Tensor>, c10::optional<Tensor>>;
+
+// Gradient tensors of x, weight and bias, those that are wanted.
+struct GradTensors {
+  c10::optional<Tensor> dx, dw, db;
+  vi_matrix mx{}, mw{};
+  GradTensors(const Tensor& x, const Tensor& weight, bool need_x, bool need_w, bool need_b) {
+    if (need_x) dx = head_result(x, x.size(0), x.size(1)), mx = head_matrix(*dx);
+    if (need_w) dw = torch::empty({weight.size(0), weight.size(1)}, x.options()), mw = head_matrix(*dw);
+    if (need_b) db = torch::empty({weight.size(0)}, x.options());
+  }
+  const vi_matrix* x() const { return dx.has_value() ? &mx : nullptr; }
+  const vi_matrix* w() const { return dw.has_value() ? &mw : nullptr; }
+  void* b() const { return db.has_value() ? db->data_ptr() : nullptr; }
+};
+
+// (dx, dweight, dbias), None where not wanted
+Grads linear_act_backward(const Tensor& dy, const c10::optional<Tensor>& dact, const Tensor& x, const Tensor& weight,
+                          bool need_x, bool need_w, bool need_b) {
+  head_check(x, weight);
+  head_like(dy, x, "dy");
+  TORCH_CHECK(dy.dim() == 2, "dy must be 2D");
+  const at::cuda::OptionalCUDAGuard guard(x.device());
+  const int dt = head_dtype(x, "x");
+  const OptMatrix d(dact, x, "dact");
+  const vi_matrix mdy = head_matrix(dy), mx = head_matrix(x), mw = head_matrix(weight);
+  GradTensors g(x, weight, need_x, need_w, need_b);
+  const uint64_t n = vi_linear_act_backward_scratch_bytes(dt, &mdy, d.get(), &mx, &mw, g.x(), g.w(), g.b());
+  Tensor scratch = head_scratch(n, x);
+  ok(vi_linear_act_backward(dt, &mdy, d.get(), &mx, &mw, g.x(), g.w(), g.b(), scratch.data_ptr(), n,
+                            at::cuda::getCurrentCUDAStream().stream()));
+  return {g.dx, g.dw, g.db};
+}
+
+// (loss, lse)
+std::tuple<Tensor, Tensor> linear_ce_forward(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias,
+                                             const Tensor& target, int64_t ignore_index, int64_t reduction) {
+  head_check(x, weight);
+  const at::cuda::OptionalCUDAGuard guard(x.device());
+  const int dt = head_dtype(x, "x");
+  const Tensor b = head_bias(bias, x, weight), t = head_target(target, x);
+  const vi_matrix mx = head_matrix(x), mw = head_matrix(weight);
+  const auto f32 = x.options().dtype(torch::kFloat32);
+  Tensor loss = reduction == VI_REDUCE_NONE ? torch::empty({x.size(0)}, f32) : torch::empty({}, f32);
+  Tensor lse = torch::empty({x.size(0)}, f32);
+  const uint64_t n = vi_linear_ce_forward_scratch_bytes(dt, &mx, &mw, head_ptr(b));
+  Tensor scratch = head_scratch(n, x);
+  ok(vi_linear_ce_forward(dt, &mx, &mw, head_ptr(b), t.data_ptr<int64_t>(), ignore_index, (int)reduction,
+                          loss.data_ptr<float>(), lse.data_ptr<float>(), scratch.data_ptr(), n,
+                          at::cuda::getCurrentCUDAStream().stream()));
+  return {loss, lse};
+}
+
+// (dx, dweight, dbias), None where not wanted
+Grads linear_ce_backward(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias, const Tensor& target,
+                         int64_t ignore_index, int64_t reduction, const Tensor& lse, const Tensor& dloss, bool need_x,
+                         bool need_w, bool need_b) {
+  head_check(x, weight);
+  const at::cuda::OptionalCUDAGuard guard(x.device());
+  const int dt = head_dtype(x, "x");
+  const Tensor b = head_bias(bias, x, weight), t = head_target(target, x);
+  Tensor l = cuda_f32(lse, "lse"), dl = cuda_f32(dloss, "dloss");
+  TORCH_CHECK(l.numel() == x.size(0), "lse must be [", x.size(0), "]");
+  TORCH_CHECK(dl.numel() == (reduction == VI_REDUCE_NONE ? x.size(0) : 1), "dloss does not fit the reduction");
+  const vi_matrix mx = head_matrix(x), mw = head_matrix(weight);
+  GradTensors g(x, weight, need_x, need_w, need_b);
+  const uint64_t n = vi_linear_ce_backward_scratch_bytes(dt, &mx, &mw, head_ptr(b), g.x(), g.w(), g.b());
+  Tensor scratch = head_scratch(n, x);
+  ok(vi_linear_ce_backward(dt, &mx, &mw, head_ptr(b), t.data_ptr<int64_t>(), ignore_index, (int)reduction,
+                           l.data_ptr<float>(), dl.data_ptr<float>(), g.x(), g.w(), g.b(), scratch.data_ptr(), n,
+                           at::cuda::getCurrentCUDAStream().stream()));
+  return {g.dx, g.dw, g.db};
+}
+
+}  // namespace
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("integrate_primitives", &integrate_primitives, "Integrate Primitives CUDA forward");
   m.def("integrate_primitives_backward", &integrate_primitives_backward, "Integrate Primitives CUDA backward");
@@ -369,6 +528,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("preprocess_gaussians_backward", &preprocess_gaussians_backward,
         "Exact derivative of the Gaussian-attribute preprocess (extension)");
   m.def("bin_gaussians", &bin_gaussians, "Tile binning of projected Gaussians (extension)");
+  m.def("linear_act_forward", &linear_act_forward, "act(x W^T + b) + residual (extension)");
+  m.def("linear_act_backward", &linear_act_backward, "Gradients of linear_act_forward (extension)");
+  m.def("linear_ce_forward", &linear_ce_forward, "Cross entropy of a linear classifier (extension)");
+  m.def("linear_ce_backward", &linear_ce_backward, "Gradients of linear_ce_forward (extension)");
   m.def("state_views", &state_views, "Integer state of a forward call in the reference's formats");
   m.def("sort_pairs", &sort_pairs, "Stable radix sort of (uint64 key, uint32 value) pairs");
   m.def("sort_end_bit", [](int64_t tiles) { return vi_sort_end_bit((uint32_t)tiles); });

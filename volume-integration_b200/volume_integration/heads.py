@@ -1,0 +1,159 @@
+"""Per-pixel heads on rendered feature images (extension; no counterpart in the
+reference, whose feature image goes to the user's own code: reference
+``volume_integration/__init__.py:365-389``).
+
+The renderer ends at ``out_features [F_out, H, W]``.  This module adds, on the
+same CUDA library, the two operators that feature and label fields put behind it:
+
+* ``linear_act``: a dense layer, ``act(x W^T + b) + residual``;
+* ``linear_cross_entropy``: the softmax cross entropy of a linear classifier over
+  a vocabulary of labels or codes, without ever storing the logits.
+
+Both take features of shape ``[..., K]`` in any strides, so the renderer's image
+goes in as ``out_features.flatten(1).t()`` (rows are pixels) without a copy by
+the caller, and ``linear_act`` answers in the same memory order.  float32,
+float16 and bfloat16; one type per call; sums in float32.  Gradients flow to every
+float input.
+
+Non-deterministic order: none.  Results of a call depend on its inputs and
+their strides alone.  There is no CPU fallback: without the CUDA library the import fails.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _C
+
+__all__ = ["ACTIVATIONS", "linear_act", "linear_cross_entropy"]
+
+ACTIVATIONS = ("none", "relu", "silu", "gelu", "sigmoid")
+REDUCTIONS = ("none", "mean", "sum")
+_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _check_operands(x, weight, bias, what, out_name):
+    if x.dim() < 1 or weight.dim() != 2:
+        raise ValueError(f"{what}: x must be [..., K] and weight [{out_name}, K], "
+                         f"got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"{what}: weight has {weight.shape[1]} columns but x has {x.shape[-1]}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"{what}: weight must have at least one row and one column, got {tuple(weight.shape)}")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f"{what}: bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{what}: x must be float32, float16 or bfloat16, got {x.dtype}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        _check_like(x, t, what, name)
+    if not x.is_cuda:
+        raise TypeError(f"{what}: x must be a CUDA tensor, but device is {x.device}")
+
+
+def _check_like(x, t, what, name):
+    if t is not None and t.dtype != x.dtype:
+        raise TypeError(f"{what}: {name} must be {x.dtype} like x, got {t.dtype}")
+    if t is not None and t.device != x.device:
+        raise ValueError(f"{what}: {name} is on {t.device} but x is on {x.device}")
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        # act' is kept rather than z: it is exact for relu, and the backward needs no transcendental
+        want = activation != 0 and any(ctx.needs_input_grad[:3])
+        y, dact = _C.linear_act_forward(x, weight, bias, residual, activation, want)
+        ctx.save_for_backward(x, weight, dact)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, dact = ctx.saved_tensors
+        nx, nw, nb, nr = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if nx or nw or nb:
+            dx, dw, db = _C.linear_act_backward(dy, dact, x, weight, nx, nw, nb)
+        return dx, dw, db, dy if nr else None, None
+
+
+def linear_act(x, weight, bias=None, residual=None, activation="none"):
+    """``act(x @ weight.T + bias) + residual`` in one pass over the output.
+
+    x: [..., K]; weight: [N, K]; bias: [N]; residual: [..., N]; ``activation`` one
+    of ``ACTIVATIONS`` (gelu is the exact form, with the normal distribution
+    function).  Returns [..., N] in x's type.  When x's rows lie next to each
+    other in memory (a channel-first image seen as [pixels, K]) so do the result's.
+
+    float16 and bfloat16 results are rounded once, from float32.  In the
+    backward the product of dy and act' is rounded to that type before the two
+    matrix products; act' itself is kept in it.
+    """
+    _check_operands(x, weight, bias, "linear_act", "N")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"linear_act: activation must be one of {ACTIVATIONS}, got {activation!r}")
+    n = weight.shape[0]
+    lead = x.shape[:-1]
+    if residual is not None:
+        if residual.shape != lead + (n,):
+            raise ValueError(f"linear_act: residual must be {tuple(lead + (n,))}, got {tuple(residual.shape)}")
+        _check_like(x, residual, "linear_act", "residual")
+    two_d = x.dim() == 2
+    x2 = x if two_d else x.reshape(-1, x.shape[-1])
+    r2 = residual if two_d or residual is None else residual.reshape(-1, n)
+    act = ACTIVATIONS.index(activation)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias, r2)):
+        y = _LinearAct.apply(x2, weight, bias, r2, act)
+    else:
+        y = _C.linear_act_forward(x2, weight, bias, r2, act, False)[0]
+    return y if two_d else y.reshape(lead + (n,))
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, reduction):
+        loss, lse = _C.linear_ce_forward(x, weight, bias, target, ignore_index, reduction)
+        ctx.save_for_backward(x, weight, bias, target, lse)
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        x, weight, bias, target, lse = ctx.saved_tensors
+        nx, nw, nb = ctx.needs_input_grad[:3]
+        dx = dw = db = None
+        if nx or nw or nb:
+            dx, dw, db = _C.linear_ce_backward(x, weight, bias, target, ctx.ignore_index, ctx.reduction, lse,
+                                               dloss, nx, nw, nb)
+        return dx, dw, db, None, None, None
+
+
+def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of the logits ``x @ weight.T + bias`` against ``target``.
+
+    x: [..., K]; weight: [V, K]; target: int64 [...], class indices; bias: [V].
+    Rows whose target is ``ignore_index`` have loss 0 and take no part in the mean or in any
+    gradient, whatever their features hold.  Any other target outside [0, V) makes its
+    row's loss, and what it is summed into, NaN.  Returns float32: [...] for
+    ``reduction="none"``, else a scalar (the mean over no row at all is NaN).
+
+    The logits exist only as tiles on the chip; the backward computes them again
+    in pieces of the vocabulary and keeps one piece of their gradient at a time,
+    in x's type.
+    """
+    _check_operands(x, weight, bias, "linear_cross_entropy", "V")
+    if reduction not in REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be one of {REDUCTIONS}, got {reduction!r}")
+    if target.dtype != torch.int64:
+        raise TypeError(f"linear_cross_entropy: target must be int64, got {target.dtype}")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: target must be {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    if target.device != x.device:
+        raise ValueError(f"linear_cross_entropy: target is on {target.device} but x is on {x.device}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    t1 = target.reshape(-1).contiguous()
+    red = REDUCTIONS.index(reduction)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias)):
+        loss = _LinearCrossEntropy.apply(x2, weight, bias, t1, int(ignore_index), red)
+    else:
+        loss = _C.linear_ce_forward(x2, weight, bias, t1, int(ignore_index), red)[0]
+    return loss.reshape(target.shape) if reduction == "none" else loss
