@@ -45,6 +45,7 @@ typedef enum vi_status {
  */
 #define VI_DEVICE_LOOKBACK_TIMEOUT 0x1u /* a sort's look-back gave up after its spin limit */
 #define VI_DEVICE_RECORD_OVERFLOW 0x2u  /* more records than grid points for a primitive */
+#define VI_DEVICE_HEAD_TIMEOUT 0x8u     /* a wait inside a matrix product of the heads gave up (vi_heads_status) */
 #define VI_DEVICE_STAGE_TIMEOUT 0x4u    /* a render tile's bulk-copy wait gave up; it read global memory instead */
 
 /* Grows the caller's byte buffer to at least nbytes and returns its device
@@ -334,8 +335,8 @@ typedef struct vi_matrix {
  * y = act(x weight^T + bias) + residual.  x [M,K], weight [N,K], bias [N] (or
  * NULL), residual [M,N] (or NULL), y [M,N] with one of its strides 1 and rows
  * or columns that do not overlap.  dact (or NULL; same shape and strides as y)
- * receives act'(x weight^T + bias), which the backward needs unless the
- * activation is VI_ACT_NONE.  K and N are at least 1, M may be 0.
+ * receives act'(x weight^T + bias) in a form of its own for the backward
+ * (float32, else a 16-bit code), which needs it unless the activation is VI_ACT_NONE.  K and N are at least 1, M may be 0.
  */
 uint64_t vi_linear_act_forward_scratch_bytes(int dtype, int activation, const vi_matrix* x, const vi_matrix* weight,
                                              const void* bias, const vi_matrix* residual, const vi_matrix* y,
@@ -386,6 +387,14 @@ int vi_linear_ce_backward(int dtype, const vi_matrix* x, const vi_matrix* weight
                           const int64_t* target, int64_t ignore_index, int reduction, const float* lse,
                           const float* dloss, const vi_matrix* dx, const vi_matrix* dweight, void* dbias,
                           void* scratch, uint64_t scratch_bytes, void* stream);
+
+/*
+ * The current device's status word of the heads' matrix products: 0, or
+ * VI_DEVICE_HEAD_TIMEOUT when a bounded wait gave up in one of them since the last
+ * reset (the results of that call are then unspecified).  Waits for `stream`; reset
+ * non-zero clears the word.
+ */
+int vi_heads_status(uint32_t* status, int reset, void* stream);
 
 /* Reads the status word a forward latched in its geometry buffer (blocks). */
 int vi_read_device_status(const char* geom_buffer, uint32_t* status, void* stream);

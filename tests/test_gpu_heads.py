@@ -258,6 +258,12 @@ def test_linear_cross_entropy(M, K, V, order, bias, ignored, reduction, dt):
     _ce_check(*_ce_inputs(M, K, V, dt, order, bias, ignored, M + V), reduction)
 
 
+@pytest.mark.parametrize("dt,V", [(F32, 4001), (F16, 9001), (BF16, 9001)], ids=["f32", "f16", "bf16"])
+def test_linear_cross_entropy_in_several_pieces(dt, V):
+    # the gradient of the logits of this many rows does not exist at once
+    _ce_check(*_ce_inputs(30000, 24, V, dt, "rows", True, 0.1, 31), "mean")
+
+
 @pytest.mark.parametrize("dt", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 def test_linear_cross_entropy_large_logits(dt):
     # spread of 40: probabilities of 1 beside ones far below float16's range
@@ -474,6 +480,20 @@ def test_offsets_beyond_32_bits():
     hl.assert_within("y", heads.linear_act(x, w, activation="silu"), hl.linear_act(x, w, None, None, "silu")[0])
     t = torch.randint(0, 48, (66,), generator=g, device="cuda")
     _ce_check(x, w, None, t, "none")
+
+
+def test_a_wait_that_runs_out_is_reported(monkeypatch):
+    # the first load is withheld and the waits are short: the kernel gives up and says so
+    import volume_integration.heads as heads
+    x, w, _, _, _ = _act_inputs(300, 200, 100, BF16, "rows", False, False, 28)
+    want = heads.linear_act(x, w)
+    assert heads.device_status(reset=True) == 0
+    monkeypatch.setenv("VI_HEADS_TEST_TIMEOUT", "1")
+    heads.linear_act(x, w)
+    assert heads.device_status(reset=True) == 8
+    monkeypatch.delenv("VI_HEADS_TEST_TIMEOUT")
+    assert torch.equal(heads.linear_act(x, w), want)  # and nothing is left behind
+    assert heads.device_status() == 0
 
 
 def test_gradients_reach_the_renderer():

@@ -79,6 +79,27 @@ def test_c_abi_refusals():
     assert lib.vi_linear_ce_backward_scratch_bytes(2, x, w, None, None, _m(5, 4, 2, 1), None) == 0
 
 
+def test_scratch_covers_every_layout_step():
+    # what a call lays out before its products has to be counted by its query: the masked
+    # copy of x (whenever dweight is wanted), and operands the copies cannot read in place
+    lib = ha.load()
+    M, K, V = 8192, 256, 16384  # as many tiles of dweight as SMs: no pieces of its sum beside
+    for dt, es in ((0, 6), (1, 2), (2, 2)):
+        x, w = _m(M, K, K, 1), _m(V, K, K, 1)
+        dx, dw = _m(M, K, K, 1), _m(V, K, K, 1)
+        q = lib.vi_linear_ce_backward_scratch_bytes
+        grad = M * V * es
+        assert q(dt, x, w, None, None, dw, None) >= min(grad, 256 << 20) + M * K * es
+        odd = _m(M, K, K + 1, 1)
+        assert q(dt, odd, w, None, None, None, None) >= min(grad, 256 << 20) + M * K * es
+        f = lib.vi_linear_act_forward_scratch_bytes
+        y = _m(M, V, V, 1)
+        assert f(dt, 0, odd, w, None, None, y, None) >= M * K * es
+        assert f(dt, 0, _m(M, K, K, 1, 264), w, None, None, y, None) >= M * K * es
+        b = lib.vi_linear_act_backward_scratch_bytes
+        assert b(dt, y, y, x, w, dx, dw, None) >= M * V * es
+
+
 @pytest.mark.parametrize("act", hl.ACTS)
 def test_float64_linear_act_against_autograd(act):
     g = torch.Generator().manual_seed(1)

@@ -512,6 +512,14 @@ Grads linear_ce_backward(const Tensor& x, const Tensor& weight, const c10::optio
   return {g.dx, g.dw, g.db};
 }
 
+// The heads' status word of a device (0 = no wait gave up).
+int64_t heads_status(int64_t device, bool reset) {
+  const at::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  uint32_t word = 0;
+  ok(vi_heads_status(&word, reset ? 1 : 0, at::cuda::getCurrentCUDAStream().stream()));
+  return word;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -532,6 +540,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_act_backward", &linear_act_backward, "Gradients of linear_act_forward (extension)");
   m.def("linear_ce_forward", &linear_ce_forward, "Cross entropy of a linear classifier (extension)");
   m.def("linear_ce_backward", &linear_ce_backward, "Gradients of linear_ce_forward (extension)");
+  m.def("heads_status", &heads_status, "Status word of the heads' kernels on a device (extension)");
   m.def("state_views", &state_views, "Integer state of a forward call in the reference's formats");
   m.def("sort_pairs", &sort_pairs, "Stable radix sort of (uint64 key, uint32 value) pairs");
   m.def("sort_end_bit", [](int64_t tiles) { return vi_sort_end_bit((uint32_t)tiles); });

@@ -8,165 +8,121 @@
 // Sums, the softmax's maximum and sum, and biases' gradients are float32; sums over
 // rows are split into pieces that are added in a fixed order, so results do not
 // depend on scheduling.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 #include <cstdio>
 
 #include "vi_heads.h"
+#include "vi_heads_math.cuh"
 #include "vi_internal.h"
 
 namespace vi {
 namespace heads {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float to_f(T v) { return (float)v; }
-template <>
-__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f(float v) { return (T)v; }
-template <>
-__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// One operand laid out for the tensor cores: 16-bit planes, rows of `inner`
+// elements `ld` apart, a multiple of 8.  value = src (* slope) (0 in rows whose coef is 0).
+struct PackJob {
+  View src;
+  View slope;         // act' beside it (float32, or the 16-bit code), p null = none
+  const float* coef;  // [rows] or null
+  int64_t rows, k;
+  void* dst;
+  int64_t ld, plane;
+  int k_major;
+};
+struct PackJobs {
+  PackJob j[2];
+};
 
-// act(z) and act'(z).  A NaN stays a NaN.
-__device__ __forceinline__ void activate(int act, float z, float& y, float& d) {
-  switch (act) {
-    case VI_ACT_RELU:
-      y = z <= 0.0f ? 0.0f : z;
-      d = z > 0.0f ? 1.0f : 0.0f;
-      break;
-    case VI_ACT_SILU: {
-      const float s = 1.0f / (1.0f + expf(-z)), c = 1.0f / (1.0f + expf(z));
-      y = z * s;
-      d = s * (1.0f + z * c);
-      break;
-    }
-    case VI_ACT_GELU: {
-      const float cdf = normcdff(z);
-      y = z * cdf;
-      d = cdf + z * 0.3989422804f * expf(-0.5f * z * z);
-      break;
-    }
-    case VI_ACT_SIGMOID: {
-      const float s = 1.0f / (1.0f + expf(-z)), c = 1.0f / (1.0f + expf(z));
-      y = s;
-      d = s * c;
-      break;
-    }
-    default:
-      y = z;
-      d = 1.0f;
-  }
+template <typename T>
+__device__ __forceinline__ float slope_at(const void* p, int64_t i) {
+  if constexpr (sizeof(T) == 4) return ((const float*)p)[i];
+  else return unpack_slope(((const uint16_t*)p)[i]);
 }
 
-constexpr int kTile = 64;  // output tile of one block, and of its 256 threads' 4x4 pieces
-constexpr int kDepth = 16;
-
-// acc(m, n) = sum_k A(m, k) B(n, k) on the FP32 cores, any strides; blockIdx.z
-// takes columns [z * ksplit, (z + 1) * ksplit) of the sum (kEpiPartial).
 template <typename T>
-__global__ void __launch_bounds__(256) gemm_kernel(View A, View B, int64_t M, int64_t N, int64_t K, int64_t ksplit,
-                                                   Epilogue e) {
-  __shared__ float sa[kDepth][kTile + 4], sb[kDepth][kTile + 4];
-  const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-  const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
-  const int64_t k_begin = blockIdx.z * ksplit, k_end = min(K, k_begin + ksplit);
-  const T* a = (const T*)A.p;
-  const T* b = (const T*)B.p;
-  float acc[4][4] = {};
-  for (int64_t k0 = k_begin; k0 < k_end; k0 += kDepth) {
-    for (int i = tid; i < kTile * kDepth; i += 256) {
-      // neighbouring threads along whichever axis is contiguous
-      const int ra = A.cs == 1 ? i / kDepth : i % kTile, ca = A.cs == 1 ? i % kDepth : i / kTile;
-      const int rb = B.cs == 1 ? i / kDepth : i % kTile, cb = B.cs == 1 ? i % kDepth : i / kTile;
-      sa[ca][ra] = m0 + ra < M && k0 + ca < k_end ? to_f(a[(m0 + ra) * A.rs + (k0 + ca) * A.cs]) : 0.0f;
-      sb[cb][rb] = n0 + rb < N && k0 + cb < k_end ? to_f(b[(n0 + rb) * B.rs + (k0 + cb) * B.cs]) : 0.0f;
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
+  const PackJob& q = jobs.j[blockIdx.y];
+  const int64_t inner = q.k_major ? q.k : q.rows, outer = q.k_major ? q.rows : q.k;
+  const uint32_t chunks = (uint32_t)((inner + 7) / 8);
+  const int64_t total = outer * chunks;
+  const int64_t si = q.k_major ? q.src.cs : q.src.rs, so = q.k_major ? q.src.rs : q.src.cs;
+  const int64_t di = q.k_major ? q.slope.cs : q.slope.rs, dn = q.k_major ? q.slope.rs : q.slope.cs;
+  const T* src = (const T*)q.src.p;
+  using B16 = typename std::conditional<std::is_same<T, __half>::value, __half, __nv_bfloat16>::type;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t o = i / chunks, c = (i - o * chunks) * 8;
+    float v[8];
+    const T* s = src + o * so + c * si;
+    if (si == 1 && c + 8 <= inner && ((uintptr_t)s & 15) == 0) {
+      uint4 w[sizeof(T) / 2];
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(T) / 2; j++) w[j] = ((const uint4*)s)[j];
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = to_f(((const T*)w)[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = c + j < inner ? to_f(s[j * si]) : 0.0f;
     }
-    __syncthreads();
+    if (q.slope.p) {
 #pragma unroll
-    for (int k = 0; k < kDepth; k++) {
-      float fa[4], fb[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) fa[i] = sa[k][ty * 4 + i], fb[i] = sb[k][tx * 4 + i];
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = fmaf(fa[i], fb[j], acc[i][j]);
+      for (int j = 0; j < 8; j++)
+        if (c + j < inner) v[j] *= slope_at<T>(q.slope.p, o * dn + (c + j) * di);
     }
-    __syncthreads();
-  }
-  const float alpha = e.alpha ? *e.alpha : 1.0f;
+    if (q.coef) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int64_t m = m0 + ty * 4 + i;
-    float top = -INFINITY;
+      for (int j = 0; j < 8; j++)
+        if (c + j < inner && q.coef[q.k_major ? o : c + j] == 0.0f) v[j] = 0.0f;
+    }
+    B16* d = (B16*)q.dst + o * q.ld + c;
+    if constexpr (sizeof(T) == 4) {
+      uint4 w[3];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int64_t n = n0 + tx * 4 + j;
-      if (m >= M || n >= N) continue;
-      float z = acc[i][j];
-      if (e.bias) z += to_f(((const T*)e.bias)[n]);
-      if (e.kind == kEpiAct) {
-        float y, d;
-        activate(e.act, z, y, d);
-        if (e.res.p) y += to_f(((const T*)e.res.p)[m * e.res.rs + n * e.res.cs]);
-        ((T*)e.out.p)[m * e.out.rs + n * e.out.cs] = from_f<T>(y);
-        if (e.dact.p) ((T*)e.dact.p)[m * e.dact.rs + n * e.dact.cs] = from_f<T>(d);
-      } else if (e.kind == kEpiStore) {
-        ((T*)e.out.p)[m * e.out.rs + n * e.out.cs] = from_f<T>(alpha * z);
-      } else if (e.kind == kEpiPartial) {
-        e.part[((int64_t)blockIdx.z * M + m) * N + n] = z;
-      } else if (e.kind == kEpiLse) {
-        acc[i][j] = z;
-        top = fmaxf(top, z);
-        if (n == e.target[m]) e.ztarget[m] = z;
-      } else {
-        const float c = e.coef[m];
-        const float p = c == 0.0f ? 0.0f : expf(z - e.lse[m]) - (n + e.col0 == e.target[m] ? 1.0f : 0.0f);
-        ((T*)e.out.p)[m * e.out.rs + n * e.out.cs] = from_f<T>(p * c);
+      for (int j = 0; j < 8; j++) {
+        __nv_bfloat16 p[3];
+        split3(v[j], p);
+#pragma unroll
+        for (int pl = 0; pl < 3; pl++) ((__nv_bfloat16*)&w[pl])[j] = p[pl];
       }
-    }
-    if (e.kind == kEpiLse) {  // the 16 threads of a row are 16 neighbouring lanes
-      for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      float sum = 0.0f;
-      for (int j = 0; j < 4; j++)
-        if (m < M && n0 + tx * 4 + j < N) sum += top == -INFINITY && acc[i][j] == top ? 0.0f : expf(acc[i][j] - top);
-      for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (tx == 0 && m < M) {
-        e.pmax[(int64_t)blockIdx.y * M + m] = top;
-        e.psum[(int64_t)blockIdx.y * M + m] = sum;
-      }
+#pragma unroll
+      for (int pl = 0; pl < 3; pl++) *(uint4*)(d + pl * q.plane) = w[pl];
+    } else {
+      uint4 w;
+#pragma unroll
+      for (int j = 0; j < 8; j++) ((B16*)&w)[j] = from_f<B16>(v[j]);
+      *(uint4*)d = w;
     }
   }
 }
 
-// s = dy * dact (dact null: a copy of dy), in dact's order; columns' sums in pieces.
+// part[piece][n] = sum of column n of src * slope over the piece's rows.
 template <typename T>
-__global__ void scale_kernel(View dy, View dact, View s, int64_t M, int64_t N) {
-  const int64_t total = M * N;
-  const bool by_col = s.cs == 1;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t m = by_col ? i / N : i % M, n = by_col ? i % N : i / M;
-    ((T*)s.p)[m * s.rs + n * s.cs] = from_f<T>(to_f(((const T*)dy.p)[m * dy.rs + n * dy.cs]) *
-                                               to_f(((const T*)dact.p)[m * dact.rs + n * dact.cs]));
-  }
-}
-
-// part[piece][n] = sum of column n over the piece's rows.
-template <typename T>
-__global__ void column_sums_kernel(View s, int64_t M, int64_t N, int64_t rows, float* part) {
+__global__ void __launch_bounds__(256) column_sums_kernel(View src, View slope, int64_t M, int64_t N, int64_t rows,
+                                                          float* part) {
   __shared__ float sh[8][33];
   const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
-  const int64_t n = (int64_t)blockIdx.x * 32 + lane, m_end = min(M, (blockIdx.y + 1) * rows);
+  const int64_t m0 = blockIdx.y * rows, m_end = min(M, m0 + rows);
+  auto value = [&](int64_t m, int64_t n) {
+    const float v = to_f(((const T*)src.p)[m * src.rs + n * src.cs]);
+    return slope.p ? v * slope_at<T>(slope.p, m * slope.rs + n * slope.cs) : v;
+  };
+  if (src.rs == 1 && src.cs != 1) {  // rows contiguous: a warp runs along a column
+    for (int c = w; c < 32; c += 8) {
+      const int64_t n = (int64_t)blockIdx.x * 32 + c;
+      float sum = 0.0f;
+      if (n < N)
+        for (int64_t m = m0 + lane; m < m_end; m += 32) sum += value(m, n);
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0 && n < N) part[(int64_t)blockIdx.y * N + n] = sum;
+    }
+    return;
+  }
+  const int64_t n = (int64_t)blockIdx.x * 32 + lane;
   float sum = 0.0f;
   if (n < N)
-    for (int64_t m = blockIdx.y * rows + w; m < m_end; m += 8) sum += to_f(((const T*)s.p)[m * s.rs + n * s.cs]);
+    for (int64_t m = m0 + w; m < m_end; m += 8) sum += value(m, n);
   sh[w][lane] = sum;
   __syncthreads();
   if (w == 0 && n < N) {
@@ -180,33 +136,35 @@ template <typename T>
 __global__ void sum_pieces_kernel(const float* part, int pieces, int64_t rows, int64_t cols, const float* alpha,
                                   View out) {
   const int64_t total = rows * cols;
+  const bool by_col = out.cs == 1;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = by_col ? i / cols : i % rows, c = by_col ? i % cols : i / rows;
     float sum = 0.0f;
-    for (int p = 0; p < pieces; p++) sum += part[(int64_t)p * total + i];
-    ((T*)out.p)[i / cols * out.rs + i % cols * out.cs] = from_f<T>(sum * (alpha ? *alpha : 1.0f));
+    for (int p = 0; p < pieces; p++) sum += part[(int64_t)p * total + r * cols + c];
+    ((T*)out.p)[r * out.rs + c * out.cs] = from_f<T>(sum * (alpha ? *alpha : 1.0f));
   }
 }
 
-// Rows' losses from the spans' maxima and sums; per block the sum of its rows' losses and their count.
+// Rows' losses from the parts' maxima and sums (maxima and lse2 in units of ln 2); per block the sum of its rows' losses and their count.
 __global__ void __launch_bounds__(256) loss_kernel(const float* pmax, const float* psum, const float* ztarget,
-                                                   int spans, int64_t M, int64_t V, const int64_t* target,
-                                                   int64_t ignore, float* rows, float* lse, float* bsum,
+                                                   int parts, int64_t M, int64_t V, const int64_t* target,
+                                                   int64_t ignore, float* rows, float* lse2, float* bsum,
                                                    float* bcount) {
   __shared__ float sh[2][8];
   const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
   float loss = 0.0f, live = 0.0f;
   if (m < M) {
     float top = -INFINITY, sum = 0.0f;
-    for (int i = 0; i < spans; i++) top = fmaxf(top, pmax[(int64_t)i * M + m]);
-    for (int i = 0; i < spans; i++) {
+    for (int i = 0; i < parts; i++) top = fmaxf(top, pmax[(int64_t)i * M + m]);
+    for (int i = 0; i < parts; i++) {
       const float p = pmax[(int64_t)i * M + m];
-      sum += psum[(int64_t)i * M + m] * (p == top ? 1.0f : expf(p - top));
+      sum += psum[(int64_t)i * M + m] * (p == top ? 1.0f : exp2f(p - top));
     }
-    const float l = top + logf(sum);
+    const float l = top + log2f(sum);
     const int64_t t = target[m];
     const bool ignored = t == ignore, bad = !ignored && (t < 0 || t >= V);
-    lse[m] = bad ? NAN : l;
-    loss = ignored ? 0.0f : bad ? NAN : l - ztarget[m];
+    lse2[m] = bad ? NAN : l;
+    loss = ignored ? 0.0f : bad ? NAN : l * 0.6931471806f - ztarget[m];
     live = ignored ? 0.0f : 1.0f;
     if (rows) rows[m] = loss;
   }
@@ -242,21 +200,42 @@ __global__ void __launch_bounds__(256) reduce_loss_kernel(const float* bsum, con
 }
 
 // Per-row factors of the logits' gradient.  Their common size goes to the
-// products' epilogue instead (alpha): G is kept in T, and float16 would lose
+// products' end instead (alpha): G is kept in 16 bits, and float16 would lose
 // probabilities divided by a pixel count.  lift (a power of two) moves float16's G
 // up further, so that a probability keeps float16's full precision down to 4e-9.
-// One block.
-__global__ void __launch_bounds__(1024) coef_kernel(const int64_t* target, int64_t ignore, int64_t M, int reduction,
-                                                    const float* dloss, float lift, float* coef, float* alpha) {
-  __shared__ float shm[32];
-  __shared__ unsigned long long shc[32];
+// First per block: the largest finite |dloss| and the number of rows not ignored.
+__global__ void __launch_bounds__(256) coef_parts_kernel(const int64_t* target, int64_t ignore, int64_t M,
+                                                         const float* dloss, float* bmax, uint32_t* bcount) {
+  __shared__ float shm[8];
+  __shared__ uint32_t shc[8];
   float top = 0.0f;
-  unsigned long long live = 0;
-  for (int64_t m = threadIdx.x; m < M; m += 1024) {
+  uint32_t live = 0;
+  for (int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x; m < M; m += (int64_t)gridDim.x * 256) {
     const bool on = target[m] != ignore;
     live += on;
-    if (reduction == VI_REDUCE_NONE && on && isfinite(dloss[m])) top = fmaxf(top, fabsf(dloss[m]));
+    if (dloss && on && isfinite(dloss[m])) top = fmaxf(top, fabsf(dloss[m]));
   }
+  for (int o = 16; o; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    live += __shfl_xor_sync(0xffffffffu, live, o);
+  }
+  if (threadIdx.x % 32 == 0) shm[threadIdx.x / 32] = top, shc[threadIdx.x / 32] = live;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; i++) top = fmaxf(top, shm[i]), live += shc[i];
+    bmax[blockIdx.x] = top;
+    bcount[blockIdx.x] = live;
+  }
+}
+
+// Then the factors themselves; every block adds the (at most 256) parts up again.
+__global__ void __launch_bounds__(256) coef_kernel(const int64_t* target, int64_t ignore, int64_t M, int reduction,
+                                                   const float* dloss, const float* bmax, const uint32_t* bcount,
+                                                   int parts, float lift, float* coef, float* alpha) {
+  __shared__ float shm[8];
+  __shared__ uint32_t shc[8];
+  float top = threadIdx.x < parts ? bmax[threadIdx.x] : 0.0f;
+  uint32_t live = threadIdx.x < parts ? bcount[threadIdx.x] : 0;
   for (int o = 16; o; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     live += __shfl_xor_sync(0xffffffffu, live, o);
@@ -265,30 +244,18 @@ __global__ void __launch_bounds__(1024) coef_kernel(const int64_t* target, int64
   __syncthreads();
   top = 0.0f;
   live = 0;
-  for (int i = 0; i < 32; i++) top = fmaxf(top, shm[i]), live += shc[i];
+  for (int i = 0; i < 8; i++) top = fmaxf(top, shm[i]), live += shc[i];
   int ex = 0;
   frexpf(top, &ex);
   ex = min(max(ex, -100), 100);  // a power of two at or above every finite |g|: the division is exact
-  if (threadIdx.x == 0)
-    *alpha = (reduction == VI_REDUCE_NONE ? ldexpf(1.0f, ex)
+  if (blockIdx.x == 0 && threadIdx.x == 0)
+    *alpha = (reduction == VI_REDUCE_NONE  ? ldexpf(1.0f, ex)
               : reduction == VI_REDUCE_SUM ? *dloss
               : live                       ? *dloss / (float)live
                                            : 0.0f) / lift;
-  for (int64_t m = threadIdx.x; m < M; m += 1024) {
+  for (int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x; m < M; m += (int64_t)gridDim.x * 256) {
     const float g = reduction == VI_REDUCE_NONE ? ldexpf(dloss[m], -ex) : 1.0f;
     coef[m] = target[m] != ignore ? g * lift : 0.0f;
-  }
-}
-
-// x with the rows of ignored targets set to zero: their zero gradient times a
-// NaN or an infinity would else reach the weights' gradient.  In x's own order.
-template <typename T>
-__global__ void live_rows_kernel(View x, const float* coef, View out, int64_t M, int64_t K) {
-  const int64_t total = M * K;
-  const bool by_col = out.cs == 1;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t m = by_col ? i / K : i % M, k = by_col ? i % K : i / M;
-    ((T*)out.p)[m * out.rs + k * out.cs] = coef[m] == 0.0f ? from_f<T>(0.0f) : ((const T*)x.p)[m * x.rs + k * x.cs];
   }
 }
 
@@ -296,29 +263,42 @@ __global__ void live_rows_kernel(View x, const float* coef, View out, int64_t M,
 // Host side.  One function per operator carves the scratch and launches; with
 // `dry` it only carves, which is how the _scratch_bytes queries count.
 // ---------------------------------------------------------------------------
+int sm_count() {
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 148;
+}
+
+// Bytes of the logits' gradient that exist at a time, if 256 columns fit.
+constexpr int64_t kPieceBytes = 256ll << 20;
+
 struct Run {
   char* base;
   cudaStream_t s;
   bool dry;
-  size_t cur = 0;
+  int sms = sm_count();
+  size_t cur = 0, peak = 0;
   int launches = 0;
   void* take(size_t bytes) {
     cur = align_up(cur);
     char* p = base + cur;
     cur += bytes;
+    peak = std::max(peak, cur);
     return p;
   }
+  // what was taken since `mark` may be taken again (by work that the stream runs later)
+  void release(size_t mark) { cur = mark; }
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int grid_for(int64_t n) { return (int)std::min<int64_t>(ceil_div(n, 256), 148 * 16); }
 size_t elem(int dtype) { return dtype == VI_F32 ? 4 : 2; }
 View view(const vi_matrix* m) { return m ? View{m->data, m->row_stride, m->col_stride} : View{nullptr, 0, 0}; }
-View transposed(View v) { return View{v.p, v.cs, v.rs}; }
-bool by_rows(const View& v) { return v.cs == 1; }
-// An [rows, cols] scratch matrix in the memory order of `like`.
-View scratch_like(void* p, const View& like, int64_t rows, int64_t cols) {
-  return by_rows(like) ? View{p, cols, 1} : View{p, 1, rows};
+Operand transposed(Operand o) {
+  std::swap(o.rows, o.k);
+  o.k_major = !o.k_major;
+  return o;
 }
 
 #define VI_DISPATCH(dtype, ...)                                    \
@@ -335,40 +315,113 @@ View scratch_like(void* p, const View& like, int64_t rows, int64_t cols) {
     }                                                              \
   } while (0)
 
-void gemm(Run& r, int dtype, View A, View B, int64_t M, int64_t N, int64_t K, int64_t ksplit, int splits,
-          const Epilogue& e) {
-  if (r.dry) return;
-  const dim3 grid((unsigned)ceil_div(M, kTile), (unsigned)ceil_div(N, kTile), splits);
-  VI_DISPATCH(dtype, (gemm_kernel<T><<<grid, 256, 0, r.s>>>(A, B, M, N, K, ksplit, e)));
-  r.launches++;
+// Whether the tensor cores' copies can read the matrix where it lies: 16-bit elements,
+// one axis contiguous, the other's stride and the address multiples of 16 bytes.
+bool direct(int dtype, const View& v, int64_t rows, int64_t k) {
+  if (dtype == VI_F32 || (uintptr_t)v.p % 16) return false;
+  if (v.cs == 1) return v.rs % 8 == 0 && v.rs >= k && v.rs < (1ll << 38);
+  return v.rs == 1 && v.cs % 8 == 0 && v.cs >= rows && v.cs < (1ll << 38);
 }
 
-// out = alpha * A B^T with a long sum: pieces of it in float32, added in order.
-void gemm_split(Run& r, int dtype, View A, View B, int64_t M, int64_t N, int64_t K, const float* alpha, View out) {
-  const int64_t tiles = ceil_div(M, kTile) * ceil_div(N, kTile);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(ceil_div(148 * 4, tiles), ceil_div(K, 512)));
-  const int64_t ksplit = ceil_div(ceil_div(K, want), kDepth) * kDepth;
-  const int splits = (int)ceil_div(K, ksplit);
-  float* part = (float*)r.take((size_t)splits * M * N * 4);
+// Operands of one call; those that have to be laid out first are collected and done by one launch.
+struct Packer {
+  Run& r;
+  int dtype;
+  PackJobs jobs{};
+  int n = 0;
+  int64_t chunks = 0;
+  Operand add(const View& v, int64_t rows, int64_t k, const View& slope = {}, const float* coef = nullptr) {
+    const bool k_major = v.cs == 1 || v.rs != 1;
+    if (!slope.p && !coef && direct(dtype, v, rows, k)) return Operand{v.p, rows, k, k_major ? v.rs : v.cs, 0, k_major};
+    const int64_t inner = k_major ? k : rows, outer = k_major ? rows : k;
+    const int64_t ld = ceil_div(inner, 8) * 8, plane = ld * outer;
+    void* dst = r.take((size_t)plane * 2 * (dtype == VI_F32 ? 3 : 1));
+    jobs.j[n++] = PackJob{v, slope, coef, rows, k, dst, ld, plane, k_major};
+    chunks = std::max(chunks, outer * (ld / 8));
+    if (n == 2) run();
+    return Operand{dst, rows, k, ld, plane, k_major};
+  }
+  void run() {
+    if (n && !r.dry) {
+      const dim3 grid((unsigned)std::min<int64_t>(ceil_div(chunks, 256), 148 * 16), n);
+      VI_DISPATCH(dtype, (pack_kernel<T><<<grid, 256, 0, r.s>>>(jobs)));
+      r.launches++;
+    }
+    n = 0;
+    chunks = 0;
+  }
+};
+
+// Tile width: the one whose waves of tiles take the least tensor-core time; narrow tiles
+// read their operands more often.
+int tile_width(int64_t M, int64_t N, int sms) {
+  const int64_t mt = ceil_div(M, 128);
+  int best = 64;
+  double cost = 1e300;
+  for (int bn : {256, 128, 64}) {
+    const double c = (double)ceil_div(mt * ceil_div(N, bn), sms) * (bn == 256 ? 256 : bn == 128 ? 150 : 90);
+    if (c < cost) cost = c, best = bn;
+  }
+  return best;
+}
+
+int gemm(Run& r, int dtype, int epi, const Operand& A, const Operand& B, const Epilogue& e) {
+  if (r.dry) return VI_OK;
+  Plan p{};
+  p.bn = tile_width(A.rows, B.rows, r.sms);
+  p.splits = 1;
+  p.kps = (int)ceil_div(A.k, 64);
+  return launch_gemm(dtype, epi, A, B, p, e, r.sms, r.s);
+}
+
+// Pieces of a long sum over k when there are few tiles.
+Plan split_plan(const Operand& A, const Operand& B, int sms) {
+  Plan p{};
+  p.bn = B.rows <= 64 ? 64 : B.rows <= 128 ? 128 : 256;
+  const int64_t tiles = ceil_div(A.rows, 128) * ceil_div(B.rows, p.bn), kb = ceil_div(A.k, 64);
+  // at least four blocks of k each, at most one piece per SM and tile
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(sms / std::min<int64_t>(tiles, sms), kb / 4));
+  p.kps = (int)ceil_div(kb, want);
+  p.splits = (int)ceil_div(kb, p.kps);
+  return p;
+}
+
+// out = alpha * A B^T; a long sum with few tiles in pieces, in float32, added in order.
+int gemm_out(Run& r, int dtype, const Operand& A, const Operand& B, const float* alpha, const View& out) {
+  const Plan p = split_plan(A, B, r.sms);
   Epilogue e{};
-  e.kind = kEpiPartial;
-  e.part = part;
-  gemm(r, dtype, A, B, M, N, K, ksplit, splits, e);
-  if (r.dry) return;
-  VI_DISPATCH(dtype, (sum_pieces_kernel<T><<<grid_for(M * N), 256, 0, r.s>>>(part, splits, M, N, alpha, out)));
+  if (p.splits == 1) {
+    e.out = out;
+    e.alpha = alpha;
+    return gemm(r, dtype, kEpiStore, A, B, e);
+  }
+  const size_t mark = r.cur;
+  e.part = (float*)r.take((size_t)p.splits * A.rows * B.rows * 4);
+  r.release(mark);
+  if (r.dry) return VI_OK;
+  if (int rc = launch_gemm(dtype, kEpiPartial, A, B, p, e, r.sms, r.s)) return rc;
+  VI_DISPATCH(dtype, (sum_pieces_kernel<T><<<grid_for(A.rows * B.rows), 256, 0, r.s>>>(e.part, p.splits, A.rows, B.rows, alpha, out)));
   r.launches++;
+  return VI_OK;
 }
 
-// out[n] = alpha * sum over rows of s.
-void column_sums(Run& r, int dtype, View s, int64_t M, int64_t N, const float* alpha, void* out) {
+// out[n] = alpha * sum over rows of src * slope.  planes: src is that many 16-bit matrices to add.
+void column_sums(Run& r, int dtype, const View& src, const View& slope, int planes, int64_t plane, int64_t M,
+                 int64_t N, const float* alpha, int out_dtype, void* out) {
   const int64_t blocks = ceil_div(N, 32);
   const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(ceil_div(148 * 8, blocks), ceil_div(M, 64)));
   const int64_t rows = ceil_div(M, pieces);
-  float* part = (float*)r.take((size_t)pieces * N * 4);
+  const size_t mark = r.cur;
+  float* part = (float*)r.take((size_t)planes * pieces * N * 4);
+  r.release(mark);
   if (r.dry) return;
-  VI_DISPATCH(dtype, (column_sums_kernel<T><<<dim3((unsigned)blocks, (unsigned)pieces), 256, 0, r.s>>>(s, M, N, rows, part)));
-  VI_DISPATCH(dtype, (sum_pieces_kernel<T><<<grid_for(N), 256, 0, r.s>>>(part, (int)pieces, 1, N, alpha, View{out, 0, 1})));
-  r.launches += 2;
+  const dim3 grid((unsigned)blocks, (unsigned)pieces);
+  for (int pl = 0; pl < planes; pl++) {
+    const View v{(char*)src.p + pl * plane * 2, src.rs, src.cs};
+    VI_DISPATCH(dtype, (column_sums_kernel<T><<<grid, 256, 0, r.s>>>(planes > 1 ? v : src, slope, M, N, rows, part + pl * pieces * N)));
+  }
+  VI_DISPATCH(out_dtype, (sum_pieces_kernel<T><<<grid_for(N), 256, 0, r.s>>>(part, (int)(pieces * planes), 1, N, alpha, View{out, 0, 1})));
+  r.launches += planes + 1;
 }
 
 // Gradients of the weights over no rows at all.
@@ -423,17 +476,20 @@ int finish(Run& r, const char* where) {
   return VI_OK;
 }
 
+// A dry run's base is not null, so that what it carves passes for given, as in the real run.
+char* dry_base() { return (char*)256; }
+
 template <class F>
 uint64_t count_bytes(F&& f) {
-  Run r{nullptr, nullptr, true};
-  return f(r) == VI_OK ? align_up(r.cur) + 256 : 0;
+  Run r{dry_base(), nullptr, true};
+  return f(r) == VI_OK ? align_up(r.peak) + 256 : 0;
 }
 template <class F>
 int execute(F&& f, void* scratch, uint64_t bytes, void* stream, const char* where) {
-  Run d{nullptr, nullptr, true};
+  Run d{scratch ? (char*)scratch : dry_base(), nullptr, true};  // exactly what the real run will take
   int rc = f(d);
   if (rc) return rc;
-  if (d.cur > bytes || (d.cur && (!scratch || (uintptr_t)scratch % 256)))
+  if (d.peak > bytes || (d.peak && (!scratch || (uintptr_t)scratch % 256)))
     return bad("heads: scratch is too small or not 256-byte aligned");
   Run r{(char*)scratch, (cudaStream_t)stream, false};
   rc = f(r);
@@ -454,14 +510,15 @@ int act_forward(Run& r, int dtype, int act, const vi_matrix* x, const vi_matrix*
     return bad("linear_act: dact must have y's strides");
   if (M == 0) return VI_OK;
   Epilogue e{};
-  e.kind = kEpiAct;
   e.act = act;
   e.bias = bias;
   e.res = view(res);
   e.out = view(y);
-  e.dact = view(dact);
-  gemm(r, dtype, view(x), view(w), M, N, K, K, 1, e);
-  return VI_OK;
+  e.dact = dact ? dact->data : nullptr;
+  Packer pk{r, dtype};
+  const Operand A = pk.add(view(x), M, K), B = pk.add(view(w), N, K);
+  pk.run();
+  return gemm(r, dtype, kEpiAct, A, B, e);
 }
 
 int act_backward(Run& r, int dtype, const vi_matrix* dy, const vi_matrix* dact, const vi_matrix* x,
@@ -478,22 +535,21 @@ int act_backward(Run& r, int dtype, const vi_matrix* dy, const vi_matrix* dact, 
     zero_gradients(r, dtype, N, K, dw, db);
     return VI_OK;
   }
-  View s = view(dy);
-  if (dact && dact->data) {
-    s = scratch_like(r.take((size_t)M * N * es), view(dact), M, N);
-    if (!r.dry) {
-      VI_DISPATCH(dtype, (scale_kernel<T><<<grid_for(M * N), 256, 0, r.s>>>(view(dy), view(dact), s, M, N)));
-      r.launches++;
-    }
+  const View slope = view(dact);
+  const bool need_dx = dx && dx->data, need_dw = dw && dw->data;
+  Packer pk{r, dtype};
+  if (need_dx || need_dw) {
+    const Operand S = pk.add(view(dy), M, N, slope);
+    Operand W{}, X{};
+    if (need_dx) W = pk.add(view(w), N, K);
+    if (need_dw) X = pk.add(view(x), M, K);
+    pk.run();
+    if (need_dx)
+      if (int rc = gemm_out(r, dtype, S, transposed(W), nullptr, view(dx))) return rc;
+    if (need_dw)
+      if (int rc = gemm_out(r, dtype, transposed(S), transposed(X), nullptr, view(dw))) return rc;
   }
-  if (dx && dx->data) {
-    Epilogue e{};
-    e.kind = kEpiStore;
-    e.out = view(dx);
-    gemm(r, dtype, s, transposed(view(w)), M, K, N, N, 1, e);
-  }
-  if (dw && dw->data) gemm_split(r, dtype, transposed(s), transposed(view(x)), N, K, M, nullptr, view(dw));
-  if (db) column_sums(r, dtype, s, M, N, nullptr, db);
+  if (db) column_sums(r, dtype, view(dy), slope, 1, 0, M, N, nullptr, dtype, db);
   return VI_OK;
 }
 
@@ -504,26 +560,39 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
   if (reduction < VI_REDUCE_NONE || reduction > VI_REDUCE_SUM) return bad("linear_ce: unknown reduction");
   const int64_t M = x->rows, K = x->cols, V = w->rows;
   if (!r.dry && M && (!target || !loss || !lse)) return bad("linear_ce: target, loss and lse are required");
-  const int spans = (int)ceil_div(V, kTile);
   const int64_t blocks = ceil_div(M, 256);
-  float* pmax = (float*)r.take((size_t)spans * M * 4);
-  float* psum = (float*)r.take((size_t)spans * M * 4);
+  Plan p{};
+  p.splits = 1;
+  p.kps = (int)ceil_div(K, 64);
+  p.bn = tile_width(M, V, r.sms);
+  // column tiles in runs, so that a block keeps a row's maximum and sum in registers over several of them
+  const int64_t nt = ceil_div(V, p.bn), mt = std::max<int64_t>(1, ceil_div(M, 128));
+  p.span = (int)ceil_div(nt, std::min(nt, ceil_div(4 * r.sms, mt)));
+  p.spans = (int)ceil_div(nt, p.span);
+  float* pmax = (float*)r.take((size_t)2 * p.spans * M * 4);
+  float* psum = (float*)r.take((size_t)2 * p.spans * M * 4);
   float* zt = (float*)r.take((size_t)M * 4);
   float* bsum = (float*)r.take((size_t)blocks * 4);
   float* bcount = (float*)r.take((size_t)blocks * 4);
+  Operand A{}, B{};
+  if (M) {
+    Packer pk{r, dtype};
+    A = pk.add(view(x), M, K);
+    B = pk.add(view(w), V, K);
+    pk.run();
+  }
   if (r.dry) return VI_OK;
   if (M) {
     Epilogue e{};
-    e.kind = kEpiLse;
     e.bias = bias;
     e.pmax = pmax;
     e.psum = psum;
     e.ztarget = zt;
     e.target = target;
-    gemm(r, dtype, view(x), view(w), M, V, K, K, 1, e);
+    if (int rc = launch_gemm(dtype, kEpiLse, A, B, p, e, r.sms, r.s)) return rc;
     const bool none = reduction == VI_REDUCE_NONE;
-    loss_kernel<<<(unsigned)blocks, 256, 0, r.s>>>(pmax, psum, zt, spans, M, V, target, ignore, none ? loss : nullptr,
-                                                   lse, none ? nullptr : bsum, bcount);
+    loss_kernel<<<(unsigned)blocks, 256, 0, r.s>>>(pmax, psum, zt, 2 * p.spans, M, V, target, ignore,
+                                                   none ? loss : nullptr, lse, none ? nullptr : bsum, bcount);
     r.launches++;
   }
   if (reduction != VI_REDUCE_NONE) {
@@ -548,36 +617,84 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
     zero_gradients(r, dtype, V, K, dw, db);
     return VI_OK;
   }
+  const bool need_dx = dx && dx->data, need_dw = dw && dw->data;
+  const int planes = dtype == VI_F32 ? 3 : 1;
   float* coef = (float*)r.take((size_t)M * 4);
   float* alpha = (float*)r.take(4);
-  View G{r.take((size_t)M * V * es), V, 1};
-  View xl = view(x);
-  if (dw && dw->data) xl = scratch_like(r.take((size_t)M * K * es), view(x), M, K);
+  const int parts = (int)std::min<int64_t>(ceil_div(M, 1024), 256);
+  float* bmax = (float*)r.take((size_t)parts * 4);
+  uint32_t* bcount = (uint32_t*)r.take((size_t)parts * 4);
   if (!r.dry) {
-    coef_kernel<<<1, 1024, 0, r.s>>>(target, ignore, M, reduction, dloss, dtype == VI_F16 ? 16384.0f : 1.0f, coef, alpha);
-    r.launches++;
-    if (dw && dw->data) {
-      VI_DISPATCH(dtype, (live_rows_kernel<T><<<grid_for(M * K), 256, 0, r.s>>>(view(x), coef, xl, M, K)));
-      r.launches++;
+    coef_parts_kernel<<<parts, 256, 0, r.s>>>(target, ignore, M, reduction == VI_REDUCE_NONE ? dloss : nullptr, bmax, bcount);
+    coef_kernel<<<parts, 256, 0, r.s>>>(target, ignore, M, reduction, dloss, bmax, bcount, parts,
+                                        dtype == VI_F16 ? 16384.0f : 1.0f, coef, alpha);
+    r.launches += 2;
+  }
+  // x without the rows of ignored targets: their zero gradient times a NaN or an
+  // infinity would else reach the weights' gradient
+  Packer pk{r, dtype};
+  const Operand X = pk.add(view(x), M, K, {}, need_dw ? coef : nullptr), W = pk.add(view(w), V, K);
+  pk.run();
+
+  // G in pieces of the vocabulary
+  const int64_t piece = std::min(V, std::max<int64_t>(256, kPieceBytes / (M * 2 * planes) / 256 * 256));
+  const int64_t ld = ceil_div(piece, 8) * 8;
+  void* grad = r.take((size_t)planes * M * ld * 2);
+  const bool several = piece < V;
+  float* acc = nullptr;  // dx over the pieces so far
+  Plan px{};
+  if (need_dx && several) {
+    px = split_plan(Operand{nullptr, M, piece}, Operand{nullptr, K, piece}, r.sms);
+    acc = (float*)r.take((size_t)px.splits * M * K * 4);
+  }
+  const size_t mark = r.cur;
+  for (int64_t c = 0; c < V; c += piece) {
+    const int64_t n = std::min(piece, V - c);
+    r.release(mark);
+    Operand Wc = W;
+    Wc.rows = n;
+    Wc.p = (const char*)W.p + c * (W.k_major ? W.ld : 1) * 2;
+    Epilogue e{};
+    e.bias = bias ? (const char*)bias + c * elem(dtype) : nullptr;
+    e.target = target;
+    e.lse2 = lse;
+    e.coef = coef;
+    e.col0 = c;
+    e.grad = grad;
+    e.grad_ld = ld;
+    e.grad_plane = M * ld;
+    if (int rc = gemm(r, dtype, kEpiGrad, X, Wc, e)) return rc;
+    const Operand G{grad, M, n, ld, M * ld, true};
+    if (need_dx) {
+      if (several) {
+        Epilogue d{};
+        d.part = acc;
+        d.add = c > 0;
+        Plan p = px;  // the last piece may be shorter: fewer blocks of k, some of px's splits empty
+        p.kps = (int)ceil_div(ceil_div(n, 64), px.splits);
+        p.splits = (int)ceil_div(ceil_div(n, 64), p.kps);
+        if (!r.dry)
+          if (int rc = launch_gemm(dtype, kEpiPartial, G, transposed(Wc), p, d, r.sms, r.s)) return rc;
+      } else if (int rc = gemm_out(r, dtype, G, transposed(Wc), alpha, view(dx))) {
+        return rc;
+      }
+    }
+    if (need_dw) {
+      View out = view(dw);
+      out.p = (char*)out.p + c * out.rs * elem(dtype);
+      if (int rc = gemm_out(r, dtype, transposed(G), transposed(X), alpha, out)) return rc;
+    }
+    if (db)
+      column_sums(r, dtype == VI_F16 ? VI_F16 : VI_BF16, View{grad, ld, 1}, View{}, planes, M * ld, M, n, alpha, dtype,
+                  (char*)db + c * elem(dtype));
+    if (r.dry && c + piece < V) {  // the last piece alone may be smaller: one more round counts it
+      c = (V - 1) / piece * piece - piece;
     }
   }
-  Epilogue e{};
-  e.kind = kEpiGrad;
-  e.bias = bias;
-  e.out = G;
-  e.target = target;
-  e.lse = lse;
-  e.coef = coef;
-  gemm(r, dtype, view(x), view(w), M, V, K, K, 1, e);
-  if (dx && dx->data) {
-    Epilogue d{};
-    d.kind = kEpiStore;
-    d.out = view(dx);
-    d.alpha = alpha;
-    gemm(r, dtype, G, transposed(view(w)), M, K, V, V, 1, d);
+  if (need_dx && several && !r.dry) {
+    VI_DISPATCH(dtype, (sum_pieces_kernel<T><<<grid_for(M * K), 256, 0, r.s>>>(acc, px.splits, M, K, alpha, view(dx))));
+    r.launches++;
   }
-  if (dw && dw->data) gemm_split(r, dtype, transposed(G), transposed(xl), V, K, M, alpha, view(dw));
-  if (db) column_sums(r, dtype, G, M, V, alpha, db);
   return VI_OK;
 }
 

@@ -16,29 +16,62 @@ struct View {
   int64_t rs, cs;
 };
 
-enum Epi { kEpiAct, kEpiStore, kEpiPartial, kEpiLse, kEpiGrad };
+// One operand of the product as the tensor cores read it: 16-bit elements, [rows][k]
+// with either axis contiguous, 16-byte aligned, in one plane or in three whose sum it
+// is (float32, see split3).
+struct Operand {
+  const void* p;
+  int64_t rows, k;       // extents
+  int64_t ld;            // elements from one row (k_major) or one k (else) to the next
+  int64_t plane;         // elements from one plane to the next
+  bool k_major;          // k is the contiguous axis
+};
+
+enum Epi {
+  kEpiAct,      // out = act(acc + bias) + res, dact = act'
+  kEpiStore,    // out = alpha * acc
+  kEpiPartial,  // part[split] = acc, or += acc (float32)
+  kEpiLse,      // per row the maximum and the sum of exponentials of the logits, the target's logit
+  kEpiGrad,     // G = coef * (softmax - onehot)
+  kEpiCount
+};
 
 // What happens to the product acc(m, n) = sum_k A(m, k) B(n, k).
 struct Epilogue {
-  int kind;
   int act;              // kEpiAct: vi_activation
   const void* bias;     // kEpiAct, kEpiLse, kEpiGrad: [N] or null
   View res;             // kEpiAct: residual, p null = none
-  View out;             // kEpiAct, kEpiStore, kEpiGrad: T
-  View dact;            // kEpiAct: act'(z), p null = not wanted
+  View out;             // kEpiAct, kEpiStore: T
+  void* dact;           // kEpiAct: act'(z) in out's strides (float32, or 16 bits: pack_slope), null = not wanted
   const float* alpha;   // kEpiStore: device scalar the product is multiplied with, null = 1
   float* part;          // kEpiPartial: [splits][M][N]
-  // kEpiLse: per (span of columns, row) the maximum of the logits and the sum of
-  // exp(z - maximum), [spans][M] each, and the target's logit [M]
+  int add;              // kEpiPartial: add to what part holds
+  // kEpiLse: [parts][M] maximum (in units of ln 2) and sum of exponentials, [M] the target's logit
   float* pmax;
   float* psum;
   float* ztarget;
   const int64_t* target;
-  // kEpiGrad: (exp(z - lse) - onehot) * coef per row, columns [col0, col0 + N) of the vocabulary
-  const float* lse;
-  const float* coef;
+  // kEpiGrad: columns [col0, col0 + N) of the vocabulary
+  const float* lse2;    // log2 of the sum of exponentials
+  const float* coef;    // per row
   int64_t col0;
+  void* grad;           // [planes][M][grad_ld], 16-bit
+  int64_t grad_ld, grad_plane;
 };
+
+// Tile shape and division of one product's work.
+struct Plan {
+  int bn;          // columns of a tile
+  int splits;      // pieces of the sum over k (kEpiPartial)
+  int kps;         // 64-wide blocks of k per piece
+  int span;        // column tiles one work item takes in turn (kEpiLse)
+  int spans;       // work items per row of tiles (kEpiLse); partial results per row: 2 * spans
+};
+
+// dtype: of outputs, bias and residual.  Planes: 1, or 3 for float32.
+// Returns a vi_status.
+int launch_gemm(int dtype, int epi, const Operand& a, const Operand& b, const Plan& p, const Epilogue& e, int sms,
+                cudaStream_t s);
 
 }  // namespace heads
 }  // namespace vi

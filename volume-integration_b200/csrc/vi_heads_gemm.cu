@@ -1,0 +1,707 @@
+// The heads' matrix product on the tensor cores, acc(m, n) = sum_k A(m, k) B(n, k),
+// with its epilogues.
+//
+// One persistent block per SM of ten warps.  Warp 8 copies 64-wide blocks of k of
+// both operands into a ring of shared-memory stages (cp.async.bulk.tensor, 128-byte
+// swizzle), warp 9 issues tcgen05.mma on them (128 x BN x 16, float32 accumulators
+// in tensor memory), warps 0-7 take finished accumulators out of tensor memory and
+// run the epilogue.  Two accumulators alternate, so the epilogue of one tile
+// overlaps the product of the next.  Either operand may have k or its rows
+// contiguous: both are layouts the tensor core reads, so a backward product
+// transposes nothing.
+//
+// float32 operands come as three bfloat16 planes, x = x0 + x1 + x2.  Of the nine
+// products of planes the six with i + j <= 2 are summed, smallest first; the others
+// are below 2^-24 of |x||w|.
+//
+// Every wait is bounded; one that runs out ends the block's work, drains what it
+// has in flight, and is latched in a status word (VI_DEVICE_HEAD_TIMEOUT).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdio>
+#include <cstdlib>
+
+#include "vi_heads.h"
+#include "vi_heads_math.cuh"
+#include "vi_internal.h"
+
+namespace vi {
+namespace heads {
+namespace {
+
+constexpr int kBM = 128, kBK = 64;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarps + 2) * 32;
+constexpr int kStageWarp = 4096;  // staging bytes per epilogue warp: 32 rows x 32 columns of float32
+constexpr uint32_t kSpinLimit = 1u << 24;
+
+__device__ uint32_t g_status;  // VI_DEVICE_HEAD_TIMEOUT when a wait ran out
+
+template <int BN>
+struct Shape {
+  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int kStage = (kBM + BN) * kBK * 2;  // bytes
+  static constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * kStageWarp;
+};
+
+struct Args {
+  int64_t M, N;
+  int m_tiles, n_tiles;  // n_tiles: column tiles
+  int kblocks;           // 64-wide blocks of the whole sum
+  int kps, splits;
+  int span, spans;
+  int pairs;             // products of planes: 1 or 6
+  uint32_t idesc;        // instruction descriptor
+  uint32_t a_lbo, b_lbo; // bytes >> 4
+  uint32_t a_step, b_step;  // bytes >> 4 from one 16-wide slice of k to the next
+  int a_k_major, b_k_major;
+  int64_t items;
+  uint32_t spin_limit;
+  int withhold;          // testing hook: the first load is never issued
+  Epilogue e;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+// Waits for the phase of `parity` to end.  False when the block has given up (*dead) or
+// the limit ran out, which sets *dead.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead, uint32_t limit) {
+  for (uint32_t i = 0; i < limit; i++) {
+    if (mbar_try(bar, parity)) return true;
+    if ((i & 63) == 63 && *dead) return false;
+  }
+  *dead = 1;
+  return false;
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          dst),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+// Shared-memory matrix descriptor: address, leading and stride byte offsets (>> 4),
+// version 1, 128-byte swizzle.  Stride: from one group of 8 rows (k contiguous) or of 8 k
+// (rows contiguous) to the next, 1024 bytes.  Leading (rows contiguous): from one
+// 64-row column of the tile to the next.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)lbo << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// 32 columns of this warp's 32 lanes of tensor memory.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, "
+      "%24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// Work item -> row tile, column tile (or span of them), piece of the sum.  Groups of 16 row
+// tiles run through all columns before the next group, so the blocks that run
+// together share operand tiles in L2.
+struct Item {
+  int mt, nt, nt_end, kb0, kb1, split, span;
+};
+template <int EPI>
+__device__ __forceinline__ Item item_of(const Args& a, int64_t i) {
+  Item t;
+  const int cols = EPI == kEpiLse ? a.spans : a.n_tiles;
+  t.split = 0;
+  if (EPI == kEpiPartial) {
+    const int64_t per = (int64_t)a.m_tiles * a.n_tiles;
+    t.split = (int)(i / per);
+    i -= t.split * per;
+  }
+  const int64_t group = i / (16ll * cols);
+  const int gm = min(16, a.m_tiles - (int)group * 16);
+  const int r = (int)(i - group * 16 * cols);
+  t.mt = (int)group * 16 + r % gm;
+  t.span = r / gm;
+  t.nt = EPI == kEpiLse ? t.span * a.span : t.span;
+  t.nt_end = EPI == kEpiLse ? min(a.n_tiles, t.nt + a.span) : t.nt + 1;
+  t.kb0 = t.split * a.kps;
+  t.kb1 = min(a.kblocks, t.kb0 + a.kps);
+  return t;
+}
+
+// ---- epilogue pieces ----
+// Each works on 32 rows (one per lane) x 32 columns in registers.
+
+template <typename T>
+__device__ __forceinline__ void load_bias(const void* bias, int64_t n0, int64_t N, float* b) {
+  const T* p = (const T*)bias + n0;
+  if (n0 + 32 <= N && ((uintptr_t)p & 15) == 0) {
+    constexpr int per = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 32 / per; i++) {
+      const uint4 q = __ldg((const uint4*)p + i);
+      const T* t = (const T*)&q;
+#pragma unroll
+      for (int j = 0; j < per; j++) b[i * per + j] = to_f(t[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j++) b[j] = n0 + j < N ? to_f(p[j]) : 0.0f;
+  }
+}
+
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void activate_row(float* v, float* d) {
+#pragma unroll
+  for (int j = 0; j < 32; j++) {
+    float y, s;
+    activate<ACT>(v[j], y, s);
+    v[j] = y;
+    if (SLOPE) d[j] = s;
+  }
+}
+template <bool SLOPE>
+__device__ __forceinline__ void activate_row(int act, float* v, float* d) {
+  switch (act) {
+    case VI_ACT_RELU: activate_row<VI_ACT_RELU, SLOPE>(v, d); break;
+    case VI_ACT_SILU: activate_row<VI_ACT_SILU, SLOPE>(v, d); break;
+    case VI_ACT_GELU: activate_row<VI_ACT_GELU, SLOPE>(v, d); break;
+    case VI_ACT_SIGMOID: activate_row<VI_ACT_SIGMOID, SLOPE>(v, d); break;
+    default: activate_row<VI_ACT_NONE, SLOPE>(v, d);
+  }
+}
+
+// Float32 staging of a warp, 32 rows x 32 columns: 16-byte pieces of a row are
+// exchanged by the row's number, so that both a lane writing its own row and lanes
+// reading along rows touch all banks once.
+__device__ __forceinline__ float4* staged(float* st, int row, int piece) {
+  return (float4*)(st + row * 32 + ((piece ^ (row & 7)) << 2));
+}
+__device__ __forceinline__ void stage_rows(float* st, int lane, const float* v) {
+#pragma unroll
+  for (int c = 0; c < 8; c++) *staged(st, lane, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+}
+
+// How a value goes to memory: as T, or as act' (16-bit code beside 16-bit types).
+template <typename T, bool SLOPE>
+struct Cell {
+  using type = T;
+  static __device__ __forceinline__ T make(float v) { return from_f<T>(v); }
+};
+template <>
+struct Cell<__half, true> {
+  using type = uint16_t;
+  static __device__ __forceinline__ uint16_t make(float v) { return pack_slope(v); }
+};
+template <>
+struct Cell<__nv_bfloat16, true> {
+  using type = uint16_t;
+  static __device__ __forceinline__ uint16_t make(float v) { return pack_slope(v); }
+};
+
+// Writes the lane-per-row values v of rows [m0, m0 + 32), columns [n0, n0 + 32) to
+// out, plus the residual.  Rows contiguous (rs == 1): a warp's store of one column is
+// contiguous as it is.  Columns contiguous: through the staging, 16 bytes a lane where
+// rows start on 16 bytes, else one row at a time.
+template <typename T, bool SLOPE>
+__device__ __forceinline__ void write_tile(const float* v, float* st, int lane, int64_t m0, int64_t n0, int64_t M,
+                                           int64_t N, const View& out, const View& res) {
+  using Z = typename Cell<T, SLOPE>::type;
+  Z* o = (Z*)out.p;
+  const T* r = (const T*)res.p;
+  if (out.rs == 1) {
+    const int64_t m = m0 + lane;
+    if (m >= M) return;
+    Z* om = o + m + n0 * out.cs;
+    const T* rm = r + m * res.rs + n0 * res.cs;
+    if (n0 + 32 <= N) {
+      float q[32];
+      if (r) {
+#pragma unroll
+        for (int j = 0; j < 32; j++) q[j] = to_f(rm[j * res.cs]);
+      }
+#pragma unroll
+      for (int j = 0; j < 32; j++) om[j * out.cs] = Cell<T, SLOPE>::make(r ? v[j] + q[j] : v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; j++)
+        if (n0 + j < N) om[j * out.cs] = Cell<T, SLOPE>::make(r ? v[j] + to_f(rm[j * res.cs]) : v[j]);
+    }
+    return;
+  }
+  __syncwarp();
+  stage_rows(st, lane, v);
+  __syncwarp();
+  constexpr int per = 16 / sizeof(Z), lanes = 32 / per, rows = 32 / lanes;  // elements a lane, lanes a row, rows a step
+  const bool vec = ((uintptr_t)o & 15) == 0 && out.rs % per == 0 && n0 + 32 <= N &&
+                   (!r || (res.cs == 1 && ((uintptr_t)r & 15) == 0 && res.rs % per == 0));
+  if (vec) {
+    const int c = (lane % lanes) * per;
+#pragma unroll
+    for (int i = 0; i < 32 / rows; i++) {
+      const int row = i * rows + lane / lanes;
+      const int64_t m = m0 + row;
+      if (m < M) {
+        float q[per];
+#pragma unroll
+        for (int h = 0; h < per / 4; h++) *(float4*)(q + 4 * h) = *staged(st, row, c / 4 + h);
+        if (r) {
+          const uint4 w = *(const uint4*)(r + m * res.rs + n0 + c);
+          const T* t = (const T*)&w;
+#pragma unroll
+          for (int j = 0; j < per; j++) q[j] += to_f(t[j]);
+        }
+        uint4 w;
+        Z* t = (Z*)&w;
+#pragma unroll
+        for (int j = 0; j < per; j++) t[j] = Cell<T, SLOPE>::make(q[j]);
+        *(uint4*)(o + m * out.rs + n0 + c) = w;
+      }
+    }
+  } else {
+    const int64_t n = n0 + lane;
+    for (int row = 0; row < 32 && m0 + row < M; row++) {
+      if (n >= N) continue;
+      float q = ((const float*)staged(st, row, lane / 4))[lane % 4];
+      if (r) q += to_f(r[(m0 + row) * res.rs + n * res.cs]);
+      o[(m0 + row) * out.rs + n] = Cell<T, SLOPE>::make(q);
+    }
+  }
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T, int BN, int EPI>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ Args a) {
+  constexpr int kStages = Shape<BN>::kStages, kStage = Shape<BN>::kStage;
+  constexpr uint32_t kCols = BN < 128 ? 2 * 64 : 2 * BN;  // tensor memory columns: two accumulators
+  extern __shared__ char smem_raw[];
+  __shared__ uint64_t bars[2 * kStages + 5];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int dead_flag;
+  char* smem = (char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  volatile int* dead = &dead_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16,
+                 drain = tempty + 16;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; i++) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(tfull + 8 * i, 1);
+      mbar_init(tempty + 8 * i, kEpiWarps);
+    }
+    mbar_init(drain, 1);
+    dead_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kEpiWarps + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == kEpiWarps) {
+    // ---- loads ----
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int64_t issued = 0;
+      bool on = true;
+      for (int64_t i = blockIdx.x; i < a.items && on; i += gridDim.x) {
+        const Item t = item_of<EPI>(a, i);
+        for (int nt = t.nt; nt < t.nt_end && on; nt++) {
+          for (int p = 0; p < a.pairs && on; p++) {
+            // planes of the pair, smallest products first: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+            const int pa = a.pairs == 1 ? 0 : p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
+            const int pb = a.pairs == 1 ? 0 : p == 2 ? 2 : p == 1 || p == 4 ? 1 : 0;
+            for (int kb = t.kb0; kb < t.kb1; kb++) {
+              if (!mbar_wait(empty + 8 * stage, phase ^ 1, dead, a.spin_limit)) {
+                on = false;
+                break;
+              }
+              const uint32_t bar = full + 8 * stage, sa = smem_u32(smem + stage * kStage), sb = sa + kBM * kBK * 2;
+              if (a.withhold && issued == 0) {  // this stage is never filled: its consumer's wait runs out
+                issued++;
+              } else {
+                mbar_expect(bar, kStage);
+                if (a.a_k_major) {
+                  tma_load(sa, &map_a, bar, kb * kBK, t.mt * kBM, pa);
+                } else {
+#pragma unroll
+                  for (int j = 0; j < kBM / 64; j++)
+                    tma_load(sa + j * 8192, &map_a, bar, t.mt * kBM + j * 64, kb * kBK, pa);
+                }
+                if (a.b_k_major) {
+                  tma_load(sb, &map_b, bar, kb * kBK, nt * BN, pb);
+                } else {
+#pragma unroll
+                  for (int j = 0; j < BN / 64; j++)
+                    tma_load(sb + j * 8192, &map_b, bar, nt * BN + j * 64, kb * kBK, pb);
+                }
+                issued++;
+              }
+              if (++stage == kStages) stage = 0, phase ^= 1;
+            }
+          }
+        }
+      }
+      if (*dead) {  // wait for the copies in flight: the last fill of every stage
+        for (int j = 0; j < kStages && j < issued; j++) {
+          const int64_t f = issued - 1 - j;  // fill number: stage f % kStages, phase (f / kStages) & 1
+          if (a.withhold && f == 0) continue;
+          for (uint32_t n = 0; n < a.spin_limit && !mbar_try(full + 8 * (uint32_t)(f % kStages), (uint32_t)(f / kStages) & 1); n++) {
+          }
+        }
+      }
+    }
+  } else if (warp == kEpiWarps + 1) {
+    // ---- products ----
+    if (lane == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool on = true;
+      for (int64_t i = blockIdx.x; i < a.items && on; i += gridDim.x) {
+        const Item t = item_of<EPI>(a, i);
+        const int steps = a.pairs * (t.kb1 - t.kb0);
+        for (int nt = t.nt; nt < t.nt_end && on; nt++) {
+          if (!mbar_wait(tempty + 8 * acc, acc_phase ^ 1, dead, a.spin_limit)) {
+            on = false;
+            break;
+          }
+          fence_after();
+          const uint32_t d = tmem + acc * BN;
+          for (int s = 0; s < steps; s++) {
+            if (!mbar_wait(full + 8 * stage, phase, dead, a.spin_limit)) {
+              on = false;
+              break;
+            }
+            fence_after();
+            const uint32_t sa = smem_u32(smem + stage * kStage);
+            const uint64_t da = smem_desc(sa, a.a_lbo), db = smem_desc(sa + kBM * kBK * 2, a.b_lbo);
+#pragma unroll
+            for (int k = 0; k < kBK / 16; k++)
+              mma_f16(d, da + k * a.a_step, db + k * a.b_step, a.idesc, s > 0 || k > 0);
+            mma_commit(empty + 8 * stage);
+            if (++stage == kStages) stage = 0, phase ^= 1;
+          }
+          if (!on) break;
+          mma_commit(tfull + 8 * acc);
+          if (++acc == 2) acc = 0, acc_phase ^= 1;
+        }
+      }
+      if (*dead) {
+        mma_commit(drain);
+        for (uint32_t n = 0; n < a.spin_limit && !mbar_try(drain, 0); n++) {
+        }
+      }
+    }
+  } else {
+    // ---- epilogue ----
+    const int quad = warp % 4, half = warp / 4;
+    float* st = (float*)(smem + kStages * kStage + warp * kStageWarp);
+    const Epilogue& e = a.e;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool on = true;
+    for (int64_t i = blockIdx.x; i < a.items && on; i += gridDim.x) {
+      const Item t = item_of<EPI>(a, i);
+      const int64_t m0 = (int64_t)t.mt * kBM + quad * 32, m = m0 + lane;
+      float top = -INFINITY, sum = 0.0f;
+      int64_t target = -1;
+      float lse2 = 0.0f, coef = 0.0f, alpha = 1.0f;
+      if (EPI == kEpiLse || EPI == kEpiGrad) {
+        if (m < a.M) target = e.target[m] - (EPI == kEpiGrad ? e.col0 : 0);
+      }
+      if (EPI == kEpiGrad && m < a.M) lse2 = e.lse2[m], coef = e.coef[m];
+      if (EPI == kEpiStore && e.alpha) alpha = *e.alpha;
+      for (int nt = t.nt; nt < t.nt_end; nt++) {
+        if (!mbar_wait(tfull + 8 * acc, acc_phase, dead, a.spin_limit)) on = false;
+        on = __all_sync(0xffffffffu, on);
+        if (!on) break;
+        fence_after();
+#pragma unroll 1
+        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+          const int64_t n0 = (int64_t)nt * BN + c;
+          float v[32];
+          __syncwarp();
+          tmem_load32(tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + c, v);
+          tmem_wait_load();
+          if (n0 >= a.N) continue;
+          if (EPI != kEpiPartial && EPI != kEpiStore) {
+            if (e.bias) {
+              float b[32];
+              load_bias<T>(e.bias, n0, a.N, b);
+#pragma unroll
+              for (int j = 0; j < 32; j++) v[j] += b[j];
+            }
+          }
+          if constexpr (EPI == kEpiAct) {
+            const View none{nullptr, 0, 0};
+            if (e.dact) {
+              float d[32];
+              activate_row<true>(e.act, v, d);
+              write_tile<T, true>(d, st, lane, m0, n0, a.M, a.N, View{e.dact, e.out.rs, e.out.cs}, none);
+            } else {
+              activate_row<false>(e.act, v, nullptr);
+            }
+            write_tile<T, false>(v, st, lane, m0, n0, a.M, a.N, e.out, e.res);
+          } else if constexpr (EPI == kEpiStore) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] *= alpha;
+            write_tile<T, false>(v, st, lane, m0, n0, a.M, a.N, e.out, View{nullptr, 0, 0});
+          } else if constexpr (EPI == kEpiPartial) {
+            write_tile<float, false>(v, st, lane, m0, n0, a.M, a.N, View{e.part + (int64_t)t.split * a.M * a.N, a.N, 1},
+                                     View{e.add ? e.part + (int64_t)t.split * a.M * a.N : nullptr, a.N, 1});
+          } else if constexpr (EPI == kEpiLse) {
+            if (__any_sync(0xffffffffu, target >= n0 && target < n0 + 32)) {
+#pragma unroll
+              for (int j = 0; j < 32; j++)
+                if (target == n0 + j && n0 + j < a.N) e.ztarget[m] = v[j];
+            }
+            float best = top;
+            if (n0 + 32 > a.N) {
+#pragma unroll
+              for (int j = 0; j < 32; j++)
+                if (n0 + j >= a.N) v[j] = -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              v[j] *= kLog2e;
+              best = fmaxf(best, v[j]);
+            }
+            // a row of -inf so far: leave the sum at zero, without -inf - -inf
+            const float ref = best == -INFINITY ? 0.0f : best;
+            float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              s0 += exp2_fast(v[j] - ref);
+              s1 += exp2_fast(v[j + 1] - ref);
+            }
+            sum = sum * exp2_fast(top - ref) + (s0 + s1);
+            top = best;
+          } else if constexpr (EPI == kEpiGrad) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = exp2_fast(v[j] * kLog2e - lse2);
+            if (__any_sync(0xffffffffu, target >= n0 && target < n0 + 32)) {
+#pragma unroll
+              for (int j = 0; j < 32; j++)
+                if (target == n0 + j) v[j] -= 1.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[j] = coef == 0.0f ? 0.0f : v[j] * coef;
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+              for (int pl = 0; pl < 3; pl++) {
+                float q[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                  __nv_bfloat16 s3[3];
+                  split3(v[j], s3);
+                  q[j] = __bfloat162float(s3[pl]);
+                }
+                write_tile<__nv_bfloat16, false>(q, st, lane, m0, n0, a.M, a.N,
+                                                 View{(__nv_bfloat16*)e.grad + pl * e.grad_plane, e.grad_ld, 1},
+                                                 View{nullptr, 0, 0});
+              }
+            } else {
+              write_tile<T, false>(v, st, lane, m0, n0, a.M, a.N, View{e.grad, e.grad_ld, 1}, View{nullptr, 0, 0});
+            }
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty + 8 * acc);
+        if (++acc == 2) acc = 0, acc_phase ^= 1;
+      }
+      if (EPI == kEpiLse && on && m < a.M) {
+        e.pmax[(int64_t)(2 * t.span + half) * a.M + m] = top;
+        e.psum[(int64_t)(2 * t.span + half) * a.M + m] = sum;
+      }
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == kEpiWarps + 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+  if (threadIdx.x == 0 && *dead) atomicOr(&g_status, VI_DEVICE_HEAD_TIMEOUT);
+}
+
+// ---- host ----
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (EncodeFn)p;
+  }();
+  return fn;
+}
+
+// The operand as [plane][outer][inner] with boxes of `box_rows` rows x 64 k.
+bool encode(CUtensorMap* map, const Operand& o, int planes, bool half, int box_rows) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t inner = (cuuint64_t)(o.k_major ? o.k : o.rows), outer = (cuuint64_t)(o.k_major ? o.rows : o.k);
+  const cuuint64_t dims[3] = {inner, outer, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(planes > 1 ? o.plane : o.ld) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)(o.k_major ? box_rows : kBK), 1};
+  const cuuint32_t unit[3] = {1, 1, 1};
+  return fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p), dims,
+            strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int BN, int EPI>
+cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
+  auto* k = gemm_tc_kernel<T, BN, EPI>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN>::kSmem);
+  if (e != cudaSuccess) return e;
+  k<<<(unsigned)std::min<int64_t>(a.items, sms), kThreads, Shape<BN>::kSmem, s>>>(ma, mb, a);
+  return cudaPeekAtLastError();
+}
+template <typename T, int EPI>
+cudaError_t run_bn(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
+  return bn == 256   ? run<T, 256, EPI>(ma, mb, a, sms, s)
+         : bn == 128 ? run<T, 128, EPI>(ma, mb, a, sms, s)
+                     : run<T, 64, EPI>(ma, mb, a, sms, s);
+}
+template <typename T>
+cudaError_t run_epi(int epi, int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms,
+                    cudaStream_t s) {
+  switch (epi) {
+    case kEpiAct: return run_bn<T, kEpiAct>(bn, ma, mb, a, sms, s);
+    case kEpiStore: return run_bn<T, kEpiStore>(bn, ma, mb, a, sms, s);
+    case kEpiLse: return run_bn<T, kEpiLse>(bn, ma, mb, a, sms, s);
+    default: return run_bn<T, kEpiGrad>(bn, ma, mb, a, sms, s);
+  }
+}
+
+}  // namespace
+
+int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Plan& p, const Epilogue& e, int sms,
+                cudaStream_t s) {
+  const int planes = dtype == VI_F32 ? 3 : 1;
+  const bool half = dtype == VI_F16;
+  CUtensorMap ma, mb;
+  if (!encode(&ma, A, planes, half, kBM) || !encode(&mb, B, planes, half, p.bn))
+    return set_error(VI_ERR_CUDA, "heads: a tensor map could not be encoded");
+  Args a{};
+  a.M = A.rows;
+  a.N = B.rows;
+  a.m_tiles = (int)((A.rows + kBM - 1) / kBM);
+  a.n_tiles = (int)((B.rows + p.bn - 1) / p.bn);
+  a.kblocks = (int)((A.k + kBK - 1) / kBK);
+  a.kps = p.kps;
+  a.splits = p.splits;
+  a.span = p.span;
+  a.spans = p.spans;
+  a.pairs = planes == 3 ? 6 : 1;
+  a.a_k_major = A.k_major;
+  a.b_k_major = B.k_major;
+  // k contiguous: 16 k are 32 bytes of a swizzled row.  Rows contiguous: 16 k are two groups of 1024 bytes.
+  a.a_lbo = A.k_major ? 1 : 8192 >> 4;
+  a.b_lbo = B.k_major ? 1 : 8192 >> 4;
+  a.a_step = A.k_major ? 32 >> 4 : 2048 >> 4;
+  a.b_step = B.k_major ? 32 >> 4 : 2048 >> 4;
+  const uint32_t type = half ? 0 : 1;
+  a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((A.k_major ? 0u : 1u) << 15) | ((B.k_major ? 0u : 1u) << 16) |
+            ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+  a.items = epi == kEpiLse ? (int64_t)a.m_tiles * p.spans : (int64_t)a.m_tiles * a.n_tiles * p.splits;
+  const char* test = getenv("VI_HEADS_TEST_TIMEOUT");
+  a.withhold = test && test[0] == '1';
+  a.spin_limit = a.withhold ? 1u << 12 : kSpinLimit;
+  a.e = e;
+  cudaError_t rc;
+  if (epi == kEpiPartial)
+    rc = run_bn<float, kEpiPartial>(p.bn, ma, mb, a, sms, s);
+  else if (dtype == VI_F32)
+    rc = run_epi<float>(epi, p.bn, ma, mb, a, sms, s);
+  else if (dtype == VI_F16)
+    rc = run_epi<__half>(epi, p.bn, ma, mb, a, sms, s);
+  else
+    rc = run_epi<__nv_bfloat16>(epi, p.bn, ma, mb, a, sms, s);
+  if (rc != cudaSuccess) {
+    char msg[256];
+    snprintf(msg, sizeof msg, "heads: %s", cudaGetErrorString(rc));
+    return set_error(VI_ERR_CUDA, msg);
+  }
+  note_launches(1);
+  return VI_OK;
+}
+
+}  // namespace heads
+}  // namespace vi
+
+extern "C" int vi_heads_status(uint32_t* status, int reset, void* stream) {
+  using namespace vi;
+  const cudaStream_t s = (cudaStream_t)stream;
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, heads::g_status);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(status, p, 4, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess && reset) e = cudaMemsetAsync(p, 0, 4, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess) return VI_OK;
+  char msg[256];
+  snprintf(msg, sizeof msg, "vi_heads_status: %s", cudaGetErrorString(e));
+  return set_error(VI_ERR_CUDA, msg);
+}

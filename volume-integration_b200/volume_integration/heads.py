@@ -15,15 +15,19 @@ the caller, and ``linear_act`` answers in the same memory order.  float32,
 float16 and bfloat16; one type per call; sums in float32.  Gradients flow to every
 float input.
 
-Non-deterministic order: none.  Results of a call depend on its inputs and
-their strides alone.  There is no CPU fallback: without the CUDA library the import fails.
+Sums are added in a fixed order: the same call gives the same bits.  There is no
+CPU fallback: without the CUDA library the import fails.
+
+The products run on the tensor cores; float32 operands as sums of three
+bfloat16 parts, which keeps float32's precision (an infinite feature or weight
+gives NaN where float32 arithmetic might give an infinity).
 """
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _C
 
-__all__ = ["ACTIVATIONS", "linear_act", "linear_cross_entropy"]
+__all__ = ["ACTIVATIONS", "device_status", "linear_act", "linear_cross_entropy"]
 
 ACTIVATIONS = ("none", "relu", "silu", "gelu", "sigmoid")
 REDUCTIONS = ("none", "mean", "sum")
@@ -83,9 +87,9 @@ def linear_act(x, weight, bias=None, residual=None, activation="none"):
     function).  Returns [..., N] in x's type.  When x's rows lie next to each
     other in memory (a channel-first image seen as [pixels, K]) so do the result's.
 
-    float16 and bfloat16 results are rounded once, from float32.  In the
-    backward the product of dy and act' is rounded to that type before the two
-    matrix products; act' itself is kept in it.
+    float16 and bfloat16 results are rounded once, from float32.  The backward
+    keeps act' (in 16 bits, to 2^-12 of its value) and rounds the product of dy and act' to
+    the operands' type before the two matrix products.
     """
     _check_operands(x, weight, bias, "linear_act", "N")
     if activation not in ACTIVATIONS:
@@ -157,3 +161,12 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     else:
         loss = _C.linear_ce_forward(x2, weight, bias, t1, int(ignore_index), red)[0]
     return loss.reshape(target.shape) if reduction == "none" else loss
+
+
+def device_status(device=None, reset=False):
+    """Status word of the heads' kernels on a device: 0, or ``VI_DEVICE_HEAD_TIMEOUT`` (8) when a
+    bounded wait gave up in one of them (that call's results are unspecified).  Waits
+    for the current stream; ``reset`` clears the word.
+    """
+    index = torch.device("cuda" if device is None else device).index
+    return _C.heads_status(torch.cuda.current_device() if index is None else index, reset)
