@@ -34,15 +34,20 @@ namespace {
 constexpr int kBM = 128, kBK = 64;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
-constexpr int kStageWarp = 4096;  // staging bytes per epilogue warp: 32 rows x 32 columns of float32
 constexpr uint32_t kSpinLimit = 1u << 24;
 
 __device__ uint32_t g_status;  // VI_DEVICE_HEAD_TIMEOUT when a wait ran out
 
-template <int BN>
+// Narrow tiles belong to products that memory bounds (few columns, short sums): two
+// blocks per SM, so that one's epilogue runs while the other waits for memory.  A
+// 256-wide tile takes all tensor memory (two accumulators) and the SM for itself.
+template <typename T, int BN, int EPI>
 struct Shape {
-  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  // float32's epilogue with act' needs more registers than half an SM has
+  static constexpr int kBlocks = BN == 256 || (EPI == kEpiAct && sizeof(T) == 4) ? 1 : 2;
+  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? (kBlocks == 2 ? 2 : 5) : (kBlocks == 2 ? 3 : 7);
   static constexpr int kStage = (kBM + BN) * kBK * 2;  // bytes
+  static constexpr int kStageWarp = EPI == kEpiLse ? 0 : 32 * 32 * (int)sizeof(T);  // an epilogue warp's staging
   static constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * kStageWarp;
 };
 
@@ -189,39 +194,7 @@ __device__ __forceinline__ void load_bias(const void* bias, int64_t n0, int64_t 
   }
 }
 
-template <int ACT, bool SLOPE>
-__device__ __forceinline__ void activate_row(float* v, float* d) {
-#pragma unroll
-  for (int j = 0; j < 32; j++) {
-    float y, s;
-    activate<ACT>(v[j], y, s);
-    v[j] = y;
-    if (SLOPE) d[j] = s;
-  }
-}
-template <bool SLOPE>
-__device__ __forceinline__ void activate_row(int act, float* v, float* d) {
-  switch (act) {
-    case VI_ACT_RELU: activate_row<VI_ACT_RELU, SLOPE>(v, d); break;
-    case VI_ACT_SILU: activate_row<VI_ACT_SILU, SLOPE>(v, d); break;
-    case VI_ACT_GELU: activate_row<VI_ACT_GELU, SLOPE>(v, d); break;
-    case VI_ACT_SIGMOID: activate_row<VI_ACT_SIGMOID, SLOPE>(v, d); break;
-    default: activate_row<VI_ACT_NONE, SLOPE>(v, d);
-  }
-}
-
-// Float32 staging of a warp, 32 rows x 32 columns: 16-byte pieces of a row are
-// exchanged by the row's number, so that both a lane writing its own row and lanes
-// reading along rows touch all banks once.
-__device__ __forceinline__ float4* staged(float* st, int row, int piece) {
-  return (float4*)(st + row * 32 + ((piece ^ (row & 7)) << 2));
-}
-__device__ __forceinline__ void stage_rows(float* st, int lane, const float* v) {
-#pragma unroll
-  for (int c = 0; c < 8; c++) *staged(st, lane, c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-}
-
-// How a value goes to memory: as T, or as act' (16-bit code beside 16-bit types).
+// How a value goes to memory: as T, or as act' (a 16-bit code beside 16-bit types).
 template <typename T, bool SLOPE>
 struct Cell {
   using type = T;
@@ -238,89 +211,139 @@ struct Cell<__nv_bfloat16, true> {
   static __device__ __forceinline__ uint16_t make(float v) { return pack_slope(v); }
 };
 
-// Writes the lane-per-row values v of rows [m0, m0 + 32), columns [n0, n0 + 32) to
-// out, plus the residual.  Rows contiguous (rs == 1): a warp's store of one column is
-// contiguous as it is.  Columns contiguous: through the staging, 16 bytes a lane where
-// rows start on 16 bytes, else one row at a time.
-template <typename T, bool SLOPE>
-__device__ __forceinline__ void write_tile(const float* v, float* st, int lane, int64_t m0, int64_t n0, int64_t M,
-                                           int64_t N, const View& out, const View& res) {
-  using Z = typename Cell<T, SLOPE>::type;
-  Z* o = (Z*)out.p;
-  const T* r = (const T*)res.p;
-  if (out.rs == 1) {
-    const int64_t m = m0 + lane;
-    if (m >= M) return;
-    Z* om = o + m + n0 * out.cs;
-    const T* rm = r + m * res.rs + n0 * res.cs;
+// 32 elements, one row of a warp's 32 x 32 tile.
+template <typename Z>
+union Row {
+  static constexpr int kPieces = 2 * sizeof(Z);  // of 16 bytes
+  uint4 q[kPieces];
+  Z z[32];
+  __device__ __forceinline__ Row() {}
+};
+
+// A warp's staging, 32 rows of 32 elements: the 16-byte pieces of a row are exchanged
+// by the row's number, so that lanes writing a row each and lanes reading along rows
+// both touch every bank once.
+template <typename Z>
+__device__ __forceinline__ uint4* staged(void* st, int row, int piece) {
+  constexpr int pieces = Row<Z>::kPieces;
+  return (uint4*)st + row * pieces + (piece ^ (sizeof(Z) == 4 ? row & 7 : (row >> 1) & 3));
+}
+
+enum Access { kNone, kImage, kVector, kScalar };
+// How a matrix is reached: rows contiguous, columns contiguous on 16-byte rows, or any strides.
+template <typename Z>
+__host__ __device__ __forceinline__ int access_of(const View& v) {
+  if (!v.p) return kNone;
+  if (v.rs == 1) return kImage;
+  return v.cs == 1 && ((uintptr_t)v.p & 15) == 0 && v.rs % (16 / (int)sizeof(Z)) == 0 ? kVector : kScalar;
+}
+
+// Loads 32 x 32 elements of v.  kVector leaves them as lanes along rows (see own_row); the
+// other ways give each lane its row.
+template <typename Z>
+__device__ __forceinline__ bool load_tile(Row<Z>& r, const View& v, int access, int lane, int64_t m0, int64_t n0,
+                                          int64_t M, int64_t N) {
+  const Z* p = (const Z*)v.p;
+  if (access == kVector && n0 + 32 <= N) {
+    constexpr int lanes = Row<Z>::kPieces, step = 32 / lanes;  // lanes a row, rows a step
+    const int row = lane / lanes, piece = lane % lanes;
+    const Z* q = p + (m0 + row) * v.rs + n0 + piece * (16 / (int)sizeof(Z));
+#pragma unroll
+    for (int i = 0; i < lanes; i++)
+      if (m0 + row + i * step < M) r.q[i] = *(const uint4*)(q + (int64_t)i * step * v.rs);
+    return true;
+  }
+  const int64_t m = m0 + lane;
+  if (m < M) {
+    const Z* q = p + m * v.rs + n0 * v.cs;
     if (n0 + 32 <= N) {
-      float q[32];
-      if (r) {
 #pragma unroll
-        for (int j = 0; j < 32; j++) q[j] = to_f(rm[j * res.cs]);
-      }
-#pragma unroll
-      for (int j = 0; j < 32; j++) om[j * out.cs] = Cell<T, SLOPE>::make(r ? v[j] + q[j] : v[j]);
+      for (int j = 0; j < 32; j++) r.z[j] = q[j * v.cs];
     } else {
 #pragma unroll
       for (int j = 0; j < 32; j++)
-        if (n0 + j < N) om[j * out.cs] = Cell<T, SLOPE>::make(r ? v[j] + to_f(rm[j * res.cs]) : v[j]);
+        if (n0 + j < N) r.z[j] = q[j * v.cs];
+    }
+  }
+  return false;
+}
+// From lanes along rows to a row each, through the staging.
+template <typename Z>
+__device__ __forceinline__ void own_row(Row<Z>& r, void* st, int lane) {
+  constexpr int lanes = Row<Z>::kPieces, step = 32 / lanes;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < lanes; i++) *staged<Z>(st, lane / lanes + i * step, lane % lanes) = r.q[i];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < lanes; i++) r.q[i] = *staged<Z>(st, lane, i);
+}
+
+// Writes each lane's row to rows [m0, m0 + 32), columns [n0, n0 + 32) of v, one of whose strides is 1.
+template <typename Z>
+__device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int access, void* st, int lane, int64_t m0,
+                                           int64_t n0, int64_t M, int64_t N) {
+  Z* p = (Z*)v.p;
+  if (access == kImage) {
+    const int64_t m = m0 + lane;
+    if (m >= M) return;
+    Z* q = p + m + n0 * v.cs;
+    if (n0 + 32 <= N) {
+#pragma unroll
+      for (int j = 0; j < 32; j++) q[j * v.cs] = r.z[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; j++)
+        if (n0 + j < N) q[j * v.cs] = r.z[j];
     }
     return;
   }
+  constexpr int lanes = Row<Z>::kPieces, step = 32 / lanes, per = 16 / (int)sizeof(Z);
   __syncwarp();
-  stage_rows(st, lane, v);
+#pragma unroll
+  for (int i = 0; i < lanes; i++) *staged<Z>(st, lane, i) = r.q[i];
   __syncwarp();
-  constexpr int per = 16 / sizeof(Z), lanes = 32 / per, rows = 32 / lanes;  // elements a lane, lanes a row, rows a step
-  const bool vec = ((uintptr_t)o & 15) == 0 && out.rs % per == 0 && n0 + 32 <= N &&
-                   (!r || (res.cs == 1 && ((uintptr_t)r & 15) == 0 && res.rs % per == 0));
-  if (vec) {
-    const int c = (lane % lanes) * per;
+  if (access == kVector && n0 + 32 <= N) {
+    const int row = lane / lanes, piece = lane % lanes;
+    Z* q = p + (m0 + row) * v.rs + n0 + piece * per;
 #pragma unroll
-    for (int i = 0; i < 32 / rows; i++) {
-      const int row = i * rows + lane / lanes;
-      const int64_t m = m0 + row;
-      if (m < M) {
-        float q[per];
-#pragma unroll
-        for (int h = 0; h < per / 4; h++) *(float4*)(q + 4 * h) = *staged(st, row, c / 4 + h);
-        if (r) {
-          const uint4 w = *(const uint4*)(r + m * res.rs + n0 + c);
-          const T* t = (const T*)&w;
-#pragma unroll
-          for (int j = 0; j < per; j++) q[j] += to_f(t[j]);
-        }
-        uint4 w;
-        Z* t = (Z*)&w;
-#pragma unroll
-        for (int j = 0; j < per; j++) t[j] = Cell<T, SLOPE>::make(q[j]);
-        *(uint4*)(o + m * out.rs + n0 + c) = w;
-      }
-    }
-  } else {
+    for (int i = 0; i < lanes; i++)
+      if (m0 + row + i * step < M) *(uint4*)(q + (int64_t)i * step * v.rs) = *staged<Z>(st, row + i * step, piece);
+  } else {  // a row at a time, each lane a column
     const int64_t n = n0 + lane;
-    for (int row = 0; row < 32 && m0 + row < M; row++) {
-      if (n >= N) continue;
-      float q = ((const float*)staged(st, row, lane / 4))[lane % 4];
-      if (r) q += to_f(r[(m0 + row) * res.rs + n * res.cs]);
-      o[(m0 + row) * out.rs + n] = Cell<T, SLOPE>::make(q);
-    }
+    for (int row = 0; row < 32 && m0 + row < M; row++)
+      if (n < N) p[(m0 + row) * v.rs + n] = ((const Z*)staged<Z>(st, row, lane / per))[lane % per];
   }
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// act over a row; the values stay in v, act' goes to d as stored.
+template <typename T, int ACT, bool SLOPE, typename Z>
+__device__ __forceinline__ void activate_row(float* v, Row<Z>& d) {
+#pragma unroll
+  for (int j = 0; j < 32; j++) {
+    float y, s;
+    activate<ACT, sizeof(T) == 4>(v[j], y, s);
+    v[j] = y;
+    if (SLOPE) d.z[j] = Cell<T, true>::make(s);
+  }
+}
+template <typename T, bool SLOPE, typename Z>
+__device__ __forceinline__ void activate_row(int act, float* v, Row<Z>& d) {
+  switch (act) {
+    case VI_ACT_RELU: activate_row<T, VI_ACT_RELU, SLOPE>(v, d); break;
+    case VI_ACT_SILU: activate_row<T, VI_ACT_SILU, SLOPE>(v, d); break;
+    case VI_ACT_GELU: activate_row<T, VI_ACT_GELU, SLOPE>(v, d); break;
+    case VI_ACT_SIGMOID: activate_row<T, VI_ACT_SIGMOID, SLOPE>(v, d); break;
+    default: activate_row<T, VI_ACT_NONE, SLOPE>(v, d);
+  }
 }
 
 template <typename T, int BN, int EPI>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, Shape<T, BN, EPI>::kBlocks)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ Args a) {
-  constexpr int kStages = Shape<BN>::kStages, kStage = Shape<BN>::kStage;
+  using S = Shape<T, BN, EPI>;
+  constexpr int kStages = S::kStages, kStage = S::kStage;
   constexpr uint32_t kCols = BN < 128 ? 2 * 64 : 2 * BN;  // tensor memory columns: two accumulators
   extern __shared__ char smem_raw[];
   __shared__ uint64_t bars[2 * kStages + 5];
@@ -453,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---- epilogue ----
     const int quad = warp % 4, half = warp / 4;
-    float* st = (float*)(smem + kStages * kStage + warp * kStageWarp);
+    void* st = smem + kStages * kStage + warp * S::kStageWarp;
     const Epilogue& e = a.e;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -470,18 +493,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (EPI == kEpiGrad && m < a.M) lse2 = e.lse2[m], coef = e.coef[m];
       if (EPI == kEpiStore && e.alpha) alpha = *e.alpha;
       for (int nt = t.nt; nt < t.nt_end; nt++) {
+        // what the epilogue adds is asked for before the product is waited for
+        constexpr bool kAdds = EPI == kEpiAct || EPI == kEpiPartial;
+        const int first = half * 32;
+        const int64_t col = (int64_t)nt * BN;
+        View add{nullptr, 0, 0};
+        if (EPI == kEpiAct) add = e.res;
+        if (EPI == kEpiPartial && e.add) add = View{e.part + (int64_t)t.split * a.M * a.N, a.N, 1};
+        Row<T> extra;
+        bool along = false;
+        if (kAdds && add.p && col + first < a.N)
+          along = load_tile<T>(extra, add, access_of<T>(add), lane, m0, col + first, a.M, a.N);
         if (!mbar_wait(tfull + 8 * acc, acc_phase, dead, a.spin_limit)) on = false;
         on = __all_sync(0xffffffffu, on);
         if (!on) break;
         fence_after();
 #pragma unroll 1
-        for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-          const int64_t n0 = (int64_t)nt * BN + c;
+        for (int c = first; c < BN && col + c < a.N; c += 64) {
+          const int64_t n0 = col + c;
+          if (kAdds && add.p && c != first)
+            along = load_tile<T>(extra, add, access_of<T>(add), lane, m0, n0, a.M, a.N);
           float v[32];
           __syncwarp();
           tmem_load32(tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + c, v);
           tmem_wait_load();
-          if (n0 >= a.N) continue;
           if (EPI != kEpiPartial && EPI != kEpiStore) {
             if (e.bias) {
               float b[32];
@@ -490,23 +525,27 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int j = 0; j < 32; j++) v[j] += b[j];
             }
           }
-          if constexpr (EPI == kEpiAct) {
-            const View none{nullptr, 0, 0};
-            if (e.dact) {
-              float d[32];
-              activate_row<true>(e.act, v, d);
-              write_tile<T, true>(d, st, lane, m0, n0, a.M, a.N, View{e.dact, e.out.rs, e.out.cs}, none);
-            } else {
-              activate_row<false>(e.act, v, nullptr);
+          if constexpr (EPI == kEpiAct || EPI == kEpiStore || EPI == kEpiPartial) {
+            if constexpr (EPI == kEpiAct) {
+              Row<typename Cell<T, true>::type> d;
+              if (e.dact) {
+                const View slope{e.dact, e.out.rs, e.out.cs};
+                activate_row<T, true>(e.act, v, d);
+                store_tile(d, slope, access_of<T>(slope), st, lane, m0, n0, a.M, a.N);
+              } else {
+                activate_row<T, false>(e.act, v, d);
+              }
             }
-            write_tile<T, false>(v, st, lane, m0, n0, a.M, a.N, e.out, e.res);
-          } else if constexpr (EPI == kEpiStore) {
+            if (kAdds && add.p) {
+              if (along) own_row<T>(extra, st, lane);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] *= alpha;
-            write_tile<T, false>(v, st, lane, m0, n0, a.M, a.N, e.out, View{nullptr, 0, 0});
-          } else if constexpr (EPI == kEpiPartial) {
-            write_tile<float, false>(v, st, lane, m0, n0, a.M, a.N, View{e.part + (int64_t)t.split * a.M * a.N, a.N, 1},
-                                     View{e.add ? e.part + (int64_t)t.split * a.M * a.N : nullptr, a.N, 1});
+              for (int j = 0; j < 32; j++) v[j] += to_f(extra.z[j]);
+            }
+            Row<T> y;
+#pragma unroll
+            for (int j = 0; j < 32; j++) y.z[j] = from_f<T>(EPI == kEpiStore ? v[j] * alpha : v[j]);
+            const View out = EPI == kEpiPartial ? View{e.part + (int64_t)t.split * a.M * a.N, a.N, 1} : e.out;
+            store_tile(y, out, access_of<T>(out), st, lane, m0, n0, a.M, a.N);
           } else if constexpr (EPI == kEpiLse) {
             if (__any_sync(0xffffffffu, target >= n0 && target < n0 + 32)) {
 #pragma unroll
@@ -547,19 +586,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
               for (int pl = 0; pl < 3; pl++) {
-                float q[32];
+                Row<__nv_bfloat16> g;
 #pragma unroll
                 for (int j = 0; j < 32; j++) {
                   __nv_bfloat16 s3[3];
                   split3(v[j], s3);
-                  q[j] = __bfloat162float(s3[pl]);
+                  g.z[j] = s3[pl];
                 }
-                write_tile<__nv_bfloat16, false>(q, st, lane, m0, n0, a.M, a.N,
-                                                 View{(__nv_bfloat16*)e.grad + pl * e.grad_plane, e.grad_ld, 1},
-                                                 View{nullptr, 0, 0});
+                const View out{(__nv_bfloat16*)e.grad + pl * e.grad_plane, e.grad_ld, 1};
+                store_tile(g, out, kVector, st, lane, m0, n0, a.M, a.N);
               }
             } else {
-              write_tile<T, false>(v, st, lane, m0, n0, a.M, a.N, View{e.grad, e.grad_ld, 1}, View{nullptr, 0, 0});
+              Row<T> g;
+#pragma unroll
+              for (int j = 0; j < 32; j++) g.z[j] = from_f<T>(v[j]);
+              store_tile(g, View{e.grad, e.grad_ld, 1}, kVector, st, lane, m0, n0, a.M, a.N);
             }
           }
         }
@@ -614,9 +655,9 @@ bool encode(CUtensorMap* map, const Operand& o, int planes, bool half, int box_r
 template <typename T, int BN, int EPI>
 cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
   auto* k = gemm_tc_kernel<T, BN, EPI>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN>::kSmem);
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, BN, EPI>::kSmem);
   if (e != cudaSuccess) return e;
-  k<<<(unsigned)std::min<int64_t>(a.items, sms), kThreads, Shape<BN>::kSmem, s>>>(ma, mb, a);
+  k<<<(unsigned)std::min<int64_t>(a.items, (int64_t)sms * Shape<T, BN, EPI>::kBlocks), kThreads, Shape<T, BN, EPI>::kSmem, s>>>(ma, mb, a);
   return cudaPeekAtLastError();
 }
 template <typename T, int EPI>
