@@ -287,6 +287,25 @@ def test_linear_cross_entropy_masked_classes(dt):
     assert float(db[100:].abs().max()) == 0.0
 
 
+@pytest.mark.parametrize("dt", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_linear_cross_entropy_every_class_at_the_lowest_value(dt):
+    # a row whose classes are all masked by the type's lowest value has them all equal
+    import volume_integration.heads as heads
+    V = 40
+    x = torch.zeros(130, 16, device="cuda", dtype=dt)
+    w = torch.ones(V, 16, device="cuda", dtype=dt)
+    b = torch.full((V,), torch.finfo(dt).min, device="cuda", dtype=dt).requires_grad_(True)
+    t = torch.arange(130, device="cuda") % V
+    loss = heads.linear_cross_entropy(x, w, t, b, reduction="none")
+    want = torch.full((130,), V, device="cuda", dtype=torch.float64).log()
+    hl.assert_within("loss", loss, (want, 64 * hl.E * want))
+    (db,) = torch.autograd.grad(loss.sum(), (b,))
+    counts = torch.bincount(t, minlength=V).double()
+    value = 130 / V - counts
+    bound = (130 + 64) * hl.E * (130 / V + counts) + hl.half_step(dt) * (130 / V + counts)
+    hl.assert_within("dbias", db, (value, bound + hl.last(dt, value.abs() + bound)))
+
+
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("dt", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 def test_linear_cross_entropy_ignored_rows_may_hold_anything(dt, reduction):

@@ -39,7 +39,7 @@ struct PackJobs {
 template <typename T>
 __device__ __forceinline__ float slope_at(const void* p, int64_t i) {
   if constexpr (sizeof(T) == 4) return ((const float*)p)[i];
-  else return unpack_slope(((const uint16_t*)p)[i]);
+  else return Slope<T>::unpack(((const uint16_t*)p)[i]);
 }
 
 template <typename T>
@@ -145,10 +145,10 @@ __global__ void sum_pieces_kernel(const float* part, int pieces, int64_t rows, i
   }
 }
 
-// Rows' losses from the parts' maxima and sums (maxima and lse2 in units of ln 2); per block the sum of its rows' losses and their count.
+// Rows' losses from the parts' maxima and sums; per block the sum of its rows' losses and their count.
 __global__ void __launch_bounds__(256) loss_kernel(const float* pmax, const float* psum, const float* ztarget,
                                                    int parts, int64_t M, int64_t V, const int64_t* target,
-                                                   int64_t ignore, float* rows, float* lse2, float* bsum,
+                                                   int64_t ignore, float* rows, float* lse, float* bsum,
                                                    float* bcount) {
   __shared__ float sh[2][8];
   const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -158,13 +158,14 @@ __global__ void __launch_bounds__(256) loss_kernel(const float* pmax, const floa
     for (int i = 0; i < parts; i++) top = fmaxf(top, pmax[(int64_t)i * M + m]);
     for (int i = 0; i < parts; i++) {
       const float p = pmax[(int64_t)i * M + m];
-      sum += psum[(int64_t)i * M + m] * (p == top ? 1.0f : exp2f(p - top));
+      sum += psum[(int64_t)i * M + m] * (p == top ? 1.0f : exp2f((p - top) * kLog2e));
     }
-    const float l = top + log2f(sum);
+    const float l = log2f(sum);
     const int64_t t = target[m];
     const bool ignored = t == ignore, bad = !ignored && (t < 0 || t >= V);
-    lse2[m] = bad ? NAN : l;
-    loss = ignored ? 0.0f : bad ? NAN : l * 0.6931471806f - ztarget[m];
+    lse[m] = top;
+    lse[M + m] = bad ? NAN : l;
+    loss = ignored ? 0.0f : bad ? NAN : fmaf(l, 0.6931471806f, top - ztarget[m]);
     live = ignored ? 0.0f : 1.0f;
     if (rows) rows[m] = loss;
   }
@@ -569,8 +570,9 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
   const int64_t nt = ceil_div(V, p.bn), mt = std::max<int64_t>(1, ceil_div(M, 128));
   p.span = (int)ceil_div(nt, std::min(nt, ceil_div(4 * r.sms, mt)));
   p.spans = (int)ceil_div(nt, p.span);
-  float* pmax = (float*)r.take((size_t)2 * p.spans * M * 4);
-  float* psum = (float*)r.take((size_t)2 * p.spans * M * 4);
+  const int parts = lse_parts(p.bn) * p.spans;
+  float* pmax = (float*)r.take((size_t)parts * M * 4);
+  float* psum = (float*)r.take((size_t)parts * M * 4);
   float* zt = (float*)r.take((size_t)M * 4);
   float* bsum = (float*)r.take((size_t)blocks * 4);
   float* bcount = (float*)r.take((size_t)blocks * 4);
@@ -591,7 +593,7 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
     e.target = target;
     if (int rc = launch_gemm(dtype, kEpiLse, A, B, p, e, r.sms, r.s)) return rc;
     const bool none = reduction == VI_REDUCE_NONE;
-    loss_kernel<<<(unsigned)blocks, 256, 0, r.s>>>(pmax, psum, zt, 2 * p.spans, M, V, target, ignore,
+    loss_kernel<<<(unsigned)blocks, 256, 0, r.s>>>(pmax, psum, zt, parts, M, V, target, ignore,
                                                    none ? loss : nullptr, lse, none ? nullptr : bsum, bcount);
     r.launches++;
   }
@@ -657,7 +659,7 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
     Epilogue e{};
     e.bias = bias ? (const char*)bias + c * elem(dtype) : nullptr;
     e.target = target;
-    e.lse2 = lse;
+    e.lse = lse;
     e.coef = coef;
     e.col0 = c;
     e.grad = grad;

@@ -46,13 +46,13 @@ struct Epilogue {
   const float* alpha;   // kEpiStore: device scalar the product is multiplied with, null = 1
   float* part;          // kEpiPartial: [splits][M][N]
   int add;              // kEpiPartial: add to what part holds
-  // kEpiLse: [parts][M] maximum (in units of ln 2) and sum of exponentials, [M] the target's logit
+  // kEpiLse: [parts][M] the largest logit and the sum of exp(z - largest), [M] the target's logit
   float* pmax;
   float* psum;
   float* ztarget;
   const int64_t* target;
   // kEpiGrad: columns [col0, col0 + N) of the vocabulary
-  const float* lse2;    // log2 of the sum of exponentials
+  const float* lse;     // [2][M]: the largest logit, and log2 of the sum of exp(z - largest)
   const float* coef;    // per row
   int64_t col0;
   void* grad;           // [planes][M][grad_ld], 16-bit
@@ -65,8 +65,11 @@ struct Plan {
   int splits;      // pieces of the sum over k (kEpiPartial)
   int kps;         // 64-wide blocks of k per piece
   int span;        // column tiles one work item takes in turn (kEpiLse)
-  int spans;       // work items per row of tiles (kEpiLse); partial results per row: 2 * spans
+  int spans;       // work items per row of tiles (kEpiLse); partial results per row: lse_parts(bn) each
 };
+
+// Partial results of kEpiLse per span.
+int lse_parts(int bn);
 
 // dtype: of outputs, bias and residual.  Planes: 1, or 3 for float32.
 // Returns a vi_status.

@@ -1,11 +1,10 @@
 // The heads' matrix product on the tensor cores, acc(m, n) = sum_k A(m, k) B(n, k),
 // with its epilogues.
 //
-// One persistent block per SM of ten warps.  Warp 8 copies 64-wide blocks of k of
-// both operands into a ring of shared-memory stages (cp.async.bulk.tensor, 128-byte
-// swizzle), warp 9 issues tcgen05.mma on them (128 x BN x 16, float32 accumulators
-// in tensor memory), warps 0-7 take finished accumulators out of tensor memory and
-// run the epilogue.  Two accumulators alternate, so the epilogue of one tile
+// Persistent blocks.  One warp copies 64-wide blocks of k of both operands into a ring
+// of shared-memory stages (cp.async.bulk.tensor, 128-byte swizzle), one issues
+// tcgen05.mma on them (128 x BN x 16, float32 accumulators in tensor memory), 8 or 16
+// take finished accumulators out of tensor memory and run the epilogue.  Two accumulators alternate, so the epilogue of one tile
 // overlaps the product of the next.  Either operand may have k or its rows
 // contiguous: both are layouts the tensor core reads, so a backward product
 // transposes nothing.
@@ -22,6 +21,7 @@
 #include <algorithm>
 #include <cstdio>
 #include <cstdlib>
+#include <type_traits>
 
 #include "vi_heads.h"
 #include "vi_heads_math.cuh"
@@ -32,8 +32,6 @@ namespace heads {
 namespace {
 
 constexpr int kBM = 128, kBK = 64;
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr uint32_t kSpinLimit = 1u << 24;
 
 __device__ uint32_t g_status;  // VI_DEVICE_HEAD_TIMEOUT when a wait ran out
@@ -45,10 +43,15 @@ template <typename T, int BN, int EPI>
 struct Shape {
   // float32's epilogue with act' needs more registers than half an SM has
   static constexpr int kBlocks = BN == 256 || (EPI == kEpiAct && sizeof(T) == 4) ? 1 : 2;
-  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? (kBlocks == 2 ? 2 : 5) : (kBlocks == 2 ? 3 : 7);
+  // Epilogue warps.  The softmax on a 256-wide tile has 16: with 8 its latency, not its
+  // instructions, bound it (K = 256: gradient 289 us with 8, 230 with 16; statistics 207, 159).
+  static constexpr int kWarps = BN == 256 && (EPI == kEpiLse || EPI == kEpiGrad) ? 16 : 8;
+  static constexpr int kParts = kWarps / 4;  // warps that share a tile's columns, 32 at a time
+  static constexpr int kThreads = (kWarps + 2) * 32;
+  static constexpr int kStages = BN == 256 ? (sizeof(T) == 4 && EPI == kEpiGrad ? 3 : 4) : BN == 128 ? (kBlocks == 2 ? 2 : 5) : (kBlocks == 2 ? 3 : 7);
   static constexpr int kStage = (kBM + BN) * kBK * 2;  // bytes
   static constexpr int kStageWarp = EPI == kEpiLse ? 0 : 32 * 32 * (int)sizeof(T);  // an epilogue warp's staging
-  static constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * kStageWarp;
+  static constexpr int kSmem = 1024 + kStages * kStage + kWarps * kStageWarp;
 };
 
 struct Args {
@@ -176,8 +179,9 @@ __device__ __forceinline__ Item item_of(const Args& a, int64_t i) {
 // ---- epilogue pieces ----
 // Each works on 32 rows (one per lane) x 32 columns in registers.
 
+// v += bias of columns [n0, n0 + 32).
 template <typename T>
-__device__ __forceinline__ void load_bias(const void* bias, int64_t n0, int64_t N, float* b) {
+__device__ __forceinline__ void add_bias(const void* bias, int64_t n0, int64_t N, float2* v) {
   const T* p = (const T*)bias + n0;
   if (n0 + 32 <= N && ((uintptr_t)p & 15) == 0) {
     constexpr int per = 16 / sizeof(T);
@@ -186,39 +190,43 @@ __device__ __forceinline__ void load_bias(const void* bias, int64_t n0, int64_t 
       const uint4 q = __ldg((const uint4*)p + i);
       const T* t = (const T*)&q;
 #pragma unroll
-      for (int j = 0; j < per; j++) b[i * per + j] = to_f(t[j]);
+      for (int j = 0; j < per / 2; j++)
+        v[i * (per / 2) + j] = __fadd2_rn(v[i * (per / 2) + j], make_float2(to_f(t[2 * j]), to_f(t[2 * j + 1])));
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; j++) b[j] = n0 + j < N ? to_f(p[j]) : 0.0f;
+    for (int j = 0; j < 32; j++)
+      if (n0 + j < N) ((float*)v)[j] += to_f(p[j]);
   }
 }
 
-// How a value goes to memory: as T, or as act' (a 16-bit code beside 16-bit types).
-template <typename T, bool SLOPE>
-struct Cell {
-  using type = T;
-  static __device__ __forceinline__ T make(float v) { return from_f<T>(v); }
-};
-template <>
-struct Cell<__half, true> {
-  using type = uint16_t;
-  static __device__ __forceinline__ uint16_t make(float v) { return pack_slope(v); }
-};
-template <>
-struct Cell<__nv_bfloat16, true> {
-  using type = uint16_t;
-  static __device__ __forceinline__ uint16_t make(float v) { return pack_slope(v); }
-};
+// The stored type of act' beside T.
+template <typename T>
+using SlopeCell = typename std::conditional<sizeof(T) == 4, float, uint16_t>::type;
 
 // 32 elements, one row of a warp's 32 x 32 tile.
 template <typename Z>
 union Row {
   static constexpr int kPieces = 2 * sizeof(Z);  // of 16 bytes
   uint4 q[kPieces];
+  uint32_t w[8 * sizeof(Z)];
   Z z[32];
   __device__ __forceinline__ Row() {}
 };
+
+// Values 2j and 2j + 1 of a row, rounded to T.
+__device__ __forceinline__ void set_pair(Row<float>& r, int j, float2 v) {
+  r.z[2 * j] = v.x;
+  r.z[2 * j + 1] = v.y;
+}
+template <typename T>
+__device__ __forceinline__ void set_pair(Row<T>& r, int j, float2 v) {
+  r.w[j] = pack2(v, T());
+}
+template <typename T>
+__device__ __forceinline__ float2 get_pair(const Row<T>& r, int j) {
+  return make_float2(to_f(r.z[2 * j]), to_f(r.z[2 * j + 1]));
+}
 
 // A warp's staging, 32 rows of 32 elements: the 16-byte pieces of a row are exchanged
 // by the row's number, so that lanes writing a row each and lanes reading along rows
@@ -317,18 +325,21 @@ __device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int a
 }
 
 // act over a row; the values stay in v, act' goes to d as stored.
-template <typename T, int ACT, bool SLOPE, typename Z>
-__device__ __forceinline__ void activate_row(float* v, Row<Z>& d) {
+template <typename T, int ACT, bool SLOPE>
+__device__ __forceinline__ void activate_row(float2* v, Row<SlopeCell<T>>& d) {
 #pragma unroll
-  for (int j = 0; j < 32; j++) {
-    float y, s;
+  for (int j = 0; j < 16; j++) {
+    float2 y, s;
     activate<ACT, sizeof(T) == 4>(v[j], y, s);
     v[j] = y;
-    if (SLOPE) d.z[j] = Cell<T, true>::make(s);
+    if constexpr (SLOPE) {
+      if constexpr (sizeof(T) == 4) set_pair(d, j, s);
+      else d.w[j] = Slope<T>::pack(s);
+    }
   }
 }
-template <typename T, bool SLOPE, typename Z>
-__device__ __forceinline__ void activate_row(int act, float* v, Row<Z>& d) {
+template <typename T, bool SLOPE>
+__device__ __forceinline__ void activate_row(int act, float2* v, Row<SlopeCell<T>>& d) {
   switch (act) {
     case VI_ACT_RELU: activate_row<T, VI_ACT_RELU, SLOPE>(v, d); break;
     case VI_ACT_SILU: activate_row<T, VI_ACT_SILU, SLOPE>(v, d); break;
@@ -339,11 +350,11 @@ __device__ __forceinline__ void activate_row(int act, float* v, Row<Z>& d) {
 }
 
 template <typename T, int BN, int EPI>
-__global__ void __launch_bounds__(kThreads, Shape<T, BN, EPI>::kBlocks)
+__global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>::kBlocks)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ Args a) {
   using S = Shape<T, BN, EPI>;
-  constexpr int kStages = S::kStages, kStage = S::kStage;
+  constexpr int kStages = S::kStages, kStage = S::kStage, kEpiWarps = S::kWarps;
   constexpr uint32_t kCols = BN < 128 ? 2 * 64 : 2 * BN;  // tensor memory columns: two accumulators
   extern __shared__ char smem_raw[];
   __shared__ uint64_t bars[2 * kStages + 5];
@@ -475,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, BN, EPI>::kBlocks)
     }
   } else {
     // ---- epilogue ----
-    const int quad = warp % 4, half = warp / 4;
+    const int quad = warp % 4, part = warp / 4;
     void* st = smem + kStages * kStage + warp * S::kStageWarp;
     const Epilogue& e = a.e;
     int acc = 0;
@@ -486,16 +497,16 @@ __global__ void __launch_bounds__(kThreads, Shape<T, BN, EPI>::kBlocks)
       const int64_t m0 = (int64_t)t.mt * kBM + quad * 32, m = m0 + lane;
       float top = -INFINITY, sum = 0.0f;
       int64_t target = -1;
-      float lse2 = 0.0f, coef = 0.0f, alpha = 1.0f;
+      float lsum = 0.0f, coef = 0.0f, alpha = 1.0f;
       if (EPI == kEpiLse || EPI == kEpiGrad) {
         if (m < a.M) target = e.target[m] - (EPI == kEpiGrad ? e.col0 : 0);
       }
-      if (EPI == kEpiGrad && m < a.M) lse2 = e.lse2[m], coef = e.coef[m];
+      if (EPI == kEpiGrad && m < a.M) top = e.lse[m], lsum = e.lse[a.M + m], coef = e.coef[m];
       if (EPI == kEpiStore && e.alpha) alpha = *e.alpha;
       for (int nt = t.nt; nt < t.nt_end; nt++) {
         // what the epilogue adds is asked for before the product is waited for
         constexpr bool kAdds = EPI == kEpiAct || EPI == kEpiPartial;
-        const int first = half * 32;
+        const int first = part * 32;
         const int64_t col = (int64_t)nt * BN;
         View add{nullptr, 0, 0};
         if (EPI == kEpiAct) add = e.res;
@@ -509,25 +520,19 @@ __global__ void __launch_bounds__(kThreads, Shape<T, BN, EPI>::kBlocks)
         if (!on) break;
         fence_after();
 #pragma unroll 1
-        for (int c = first; c < BN && col + c < a.N; c += 64) {
+        for (int c = first; c < BN && col + c < a.N; c += 32 * S::kParts) {
           const int64_t n0 = col + c;
           if (kAdds && add.p && c != first)
             along = load_tile<T>(extra, add, access_of<T>(add), lane, m0, n0, a.M, a.N);
-          float v[32];
+          float2 v[16];
           __syncwarp();
-          tmem_load32(tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + c, v);
+          tmem_load32(tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + c, (float*)v);
           tmem_wait_load();
-          if (EPI != kEpiPartial && EPI != kEpiStore) {
-            if (e.bias) {
-              float b[32];
-              load_bias<T>(e.bias, n0, a.N, b);
-#pragma unroll
-              for (int j = 0; j < 32; j++) v[j] += b[j];
-            }
-          }
+          if (EPI != kEpiPartial && EPI != kEpiStore)
+            if (e.bias) add_bias<T>(e.bias, n0, a.N, v);
           if constexpr (EPI == kEpiAct || EPI == kEpiStore || EPI == kEpiPartial) {
             if constexpr (EPI == kEpiAct) {
-              Row<typename Cell<T, true>::type> d;
+              Row<SlopeCell<T>> d;
               if (e.dact) {
                 const View slope{e.dact, e.out.rs, e.out.cs};
                 activate_row<T, true>(e.act, v, d);
@@ -539,50 +544,57 @@ __global__ void __launch_bounds__(kThreads, Shape<T, BN, EPI>::kBlocks)
             if (kAdds && add.p) {
               if (along) own_row<T>(extra, st, lane);
 #pragma unroll
-              for (int j = 0; j < 32; j++) v[j] += to_f(extra.z[j]);
+              for (int j = 0; j < 16; j++) v[j] = __fadd2_rn(v[j], get_pair(extra, j));
             }
             Row<T> y;
 #pragma unroll
-            for (int j = 0; j < 32; j++) y.z[j] = from_f<T>(EPI == kEpiStore ? v[j] * alpha : v[j]);
+            for (int j = 0; j < 16; j++) set_pair(y, j, EPI == kEpiStore ? __fmul2_rn(v[j], pair(alpha)) : v[j]);
             const View out = EPI == kEpiPartial ? View{e.part + (int64_t)t.split * a.M * a.N, a.N, 1} : e.out;
             store_tile(y, out, access_of<T>(out), st, lane, m0, n0, a.M, a.N);
           } else if constexpr (EPI == kEpiLse) {
+            float* z = (float*)v;
             if (__any_sync(0xffffffffu, target >= n0 && target < n0 + 32)) {
 #pragma unroll
               for (int j = 0; j < 32; j++)
-                if (target == n0 + j && n0 + j < a.N) e.ztarget[m] = v[j];
+                if (target == n0 + j && n0 + j < a.N) e.ztarget[m] = z[j];
             }
-            float best = top;
             if (n0 + 32 > a.N) {
 #pragma unroll
               for (int j = 0; j < 32; j++)
-                if (n0 + j >= a.N) v[j] = -INFINITY;
+                if (n0 + j >= a.N) z[j] = -INFINITY;
             }
+            float best = top;
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-              v[j] *= kLog2e;
-              best = fmaxf(best, v[j]);
-            }
+            for (int j = 0; j < 32; j++) best = fmaxf(best, z[j]);
             // a row of -inf so far: leave the sum at zero, without -inf - -inf
             const float ref = best == -INFINITY ? 0.0f : best;
-            float s0 = 0.0f, s1 = 0.0f;
+            float2 s2 = pair(0.0f);
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              s0 += exp2_fast(v[j] - ref);
-              s1 += exp2_fast(v[j + 1] - ref);
+            for (int j = 0; j < 16; j++) {
+              // the difference first: a logit of the type's lowest value times log2(e) would overflow
+              const float2 x = __fmul2_rn(__fadd2_rn(v[j], pair(-ref)), pair(kLog2e));
+              s2 = __fadd2_rn(s2, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
             }
-            sum = sum * exp2_fast(top - ref) + (s0 + s1);
+            sum = sum * exp2_fast((top - ref) * kLog2e) + (s2.x + s2.y);
             top = best;
           } else if constexpr (EPI == kEpiGrad) {
+            float* z = (float*)v;
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = exp2_fast(v[j] * kLog2e - lse2);
+            for (int j = 0; j < 16; j++) {
+              const float2 x = __ffma2_rn(__fadd2_rn(v[j], pair(-top)), pair(kLog2e), pair(-lsum));
+              v[j] = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+            }
             if (__any_sync(0xffffffffu, target >= n0 && target < n0 + 32)) {
 #pragma unroll
               for (int j = 0; j < 32; j++)
-                if (target == n0 + j) v[j] -= 1.0f;
+                if (target == n0 + j) z[j] -= 1.0f;
             }
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = coef == 0.0f ? 0.0f : v[j] * coef;
+            for (int j = 0; j < 16; j++) v[j] = __fmul2_rn(v[j], pair(coef));
+            if (__any_sync(0xffffffffu, coef == 0.0f)) {  // an ignored row's logits may be anything
+#pragma unroll
+              for (int j = 0; j < 32; j++) z[j] = coef == 0.0f ? 0.0f : z[j];
+            }
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
               for (int pl = 0; pl < 3; pl++) {
@@ -590,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, BN, EPI>::kBlocks)
 #pragma unroll
                 for (int j = 0; j < 32; j++) {
                   __nv_bfloat16 s3[3];
-                  split3(v[j], s3);
+                  split3(z[j], s3);
                   g.z[j] = s3[pl];
                 }
                 const View out{(__nv_bfloat16*)e.grad + pl * e.grad_plane, e.grad_ld, 1};
@@ -599,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, BN, EPI>::kBlocks)
             } else {
               Row<T> g;
 #pragma unroll
-              for (int j = 0; j < 32; j++) g.z[j] = from_f<T>(v[j]);
+              for (int j = 0; j < 16; j++) set_pair(g, j, v[j]);
               store_tile(g, View{e.grad, e.grad_ld, 1}, kVector, st, lane, m0, n0, a.M, a.N);
             }
           }
@@ -610,8 +622,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, BN, EPI>::kBlocks)
         if (++acc == 2) acc = 0, acc_phase ^= 1;
       }
       if (EPI == kEpiLse && on && m < a.M) {
-        e.pmax[(int64_t)(2 * t.span + half) * a.M + m] = top;
-        e.psum[(int64_t)(2 * t.span + half) * a.M + m] = sum;
+        e.pmax[(int64_t)(S::kParts * t.span + part) * a.M + m] = top;
+        e.psum[(int64_t)(S::kParts * t.span + part) * a.M + m] = sum;
       }
     }
   }
@@ -657,7 +669,7 @@ cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int
   auto* k = gemm_tc_kernel<T, BN, EPI>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, BN, EPI>::kSmem);
   if (e != cudaSuccess) return e;
-  k<<<(unsigned)std::min<int64_t>(a.items, (int64_t)sms * Shape<T, BN, EPI>::kBlocks), kThreads, Shape<T, BN, EPI>::kSmem, s>>>(ma, mb, a);
+  k<<<(unsigned)std::min<int64_t>(a.items, (int64_t)sms * Shape<T, BN, EPI>::kBlocks), Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>::kSmem, s>>>(ma, mb, a);
   return cudaPeekAtLastError();
 }
 template <typename T, int EPI>
@@ -678,6 +690,8 @@ cudaError_t run_epi(int epi, int bn, const CUtensorMap& ma, const CUtensorMap& m
 }
 
 }  // namespace
+
+int lse_parts(int bn) { return Shape<float, 256, kEpiLse>::kParts * (bn == 256) + Shape<float, 64, kEpiLse>::kParts * (bn != 256); }
 
 int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Plan& p, const Epilogue& e, int sms,
                 cudaStream_t s) {

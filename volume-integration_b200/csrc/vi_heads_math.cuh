@@ -28,81 +28,122 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// act(z) and act'(z) in float32.  A NaN stays a NaN.  EXACT: to a few float32 steps,
-// beside float32 outputs; else to 1e-6 of the value, beside 16-bit ones.
+// act(z) and act'(z) of two values in float32.  A NaN stays a NaN.  EXACT: to a few
+// float32 steps, beside float32 outputs; else to 1e-6 of the value, beside 16-bit ones.
 //
 // sigmoid: with e = exp(-z), s = 1 / (1 + e) and 1 - s = e s, without cancellation
 // for large z; e is kept finite, so e s tends to 1 and not to inf * 0.
-// gelu: Phi(-x) = exp(-x^2 / 2) r(t) for x >= 0, t = 1 / (1 + 0.265 x), r a polynomial of
-// degree 7 without constant term fitted here to Mills' ratio / sqrt(2 pi) by iteratively
-// reweighted least squares: 6.3e-7 of the value over [0, 14], where float32 ends.
-// One exponential serves Phi and the density.
+// gelu: with x = |z| and Q = Phi(-x), z Phi(z) = max(z, 0) - x Q.  Q = exp(-x^2 / 2) r(t),
+// t = 1 / (1 + 0.265 x), r a polynomial of degree 7 without constant term fitted
+// here to Mills' ratio / sqrt(2 pi) by iteratively reweighted least squares: 6.3e-7 of
+// the value over [0, 14], where float32 ends.  One exponential serves Q and the density.
+// Sums and products of pairs are one instruction each.
 template <int ACT, bool EXACT>
-__device__ __forceinline__ void activate(float z, float& y, float& d) {
+__device__ __forceinline__ void activate(float2 z, float2& y, float2& d) {
   if constexpr (ACT == VI_ACT_RELU) {
-    y = z <= 0.0f ? 0.0f : z;
-    d = z > 0.0f ? 1.0f : 0.0f;
+    y = make_float2(z.x <= 0.0f ? 0.0f : z.x, z.y <= 0.0f ? 0.0f : z.y);
+    d = make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
   } else if constexpr (ACT == VI_ACT_SILU || ACT == VI_ACT_SIGMOID) {
-    float e, s;
+    float2 e, s;
     if constexpr (EXACT) {
-      e = expf(fminf(-z, 87.0f));
-      s = 1.0f / (1.0f + e);
+      e = make_float2(expf(min_nan(-z.x, 87.0f)), expf(min_nan(-z.y, 87.0f)));
+      s = make_float2(1.0f / (1.0f + e.x), 1.0f / (1.0f + e.y));
     } else {
-      e = exp2_fast(fminf(-z * kLog2e, 126.0f));
-      s = __fdividef(1.0f, 1.0f + e);
+      const float2 t = __fmul2_rn(z, pair(-kLog2e));
+      e = make_float2(exp2_fast(min_nan(t.x, 126.0f)), exp2_fast(min_nan(t.y, 126.0f)));
+      const float2 q = __fadd2_rn(e, pair(1.0f));
+      s = make_float2(rcp_fast(q.x), rcp_fast(q.y));
     }
-    if (z != z) s = z;
-    const float c = e * s;
+    const float2 c = __fmul2_rn(e, s);
     if constexpr (ACT == VI_ACT_SILU) {
-      y = z * s;
-      d = s * fmaf(z, c, 1.0f);
+      y = __fmul2_rn(z, s);
+      d = __fmul2_rn(s, __ffma2_rn(z, c, pair(1.0f)));
     } else {
       y = s;
-      d = s * c;
+      d = __fmul2_rn(s, c);
     }
   } else if constexpr (ACT == VI_ACT_GELU) {
     if constexpr (EXACT) {
-      const float cdf = normcdff(z);
-      y = z * cdf;
-      d = cdf + z * 0.3989422804f * expf(-0.5f * z * z);
+      const float2 cdf = make_float2(normcdff(z.x), normcdff(z.y));
+      y = __fmul2_rn(z, cdf);
+      const float2 g = make_float2(expf(-0.5f * z.x * z.x), expf(-0.5f * z.y * z.y));
+      d = __ffma2_rn(__fmul2_rn(z, pair(0.3989422804f)), g, cdf);
     } else {
-      const float x = fabsf(z), t = __fdividef(1.0f, fmaf(0.265f, x, 1.0f));
-      float r = -0.0677848929f;
-      r = fmaf(r, t, 0.195265483f);
-      r = fmaf(r, t, -0.0663519581f);
-      r = fmaf(r, t, 0.142485184f);
-      r = fmaf(r, t, 0.0829498892f);
-      r = fmaf(r, t, 0.107836094f);
-      r = fmaf(r, t, 0.105599892f);
-      const float g = exp2_fast(z * z * (-0.5f * kLog2e)), q = g * (r * t);
-      const float cdf = z < 0.0f ? q : 1.0f - q;
-      y = z * cdf;
-      d = fmaf(z * 0.3989422804f, g, cdf);
+      const float2 x = make_float2(fminf(fabsf(z.x), 40.0f), fminf(fabsf(z.y), 40.0f));  // Q(40) is 0: no inf * 0
+      const float2 u = __ffma2_rn(x, pair(0.265f), pair(1.0f));
+      const float2 t = make_float2(rcp_fast(u.x), rcp_fast(u.y));
+      float2 r = __ffma2_rn(t, pair(-0.0677848929f), pair(0.195265483f));
+      r = __ffma2_rn(r, t, pair(-0.0663519581f));
+      r = __ffma2_rn(r, t, pair(0.142485184f));
+      r = __ffma2_rn(r, t, pair(0.0829498892f));
+      r = __ffma2_rn(r, t, pair(0.107836094f));
+      r = __ffma2_rn(r, t, pair(0.105599892f));
+      r = __fmul2_rn(r, t);
+      const float2 a = __fmul2_rn(__fmul2_rn(z, pair(-0.5f * kLog2e)), z);
+      const float2 g = make_float2(exp2_fast(a.x), exp2_fast(a.y)), q = __fmul2_rn(g, r);
+      const float2 top = make_float2(fmaxf(z.x, 0.0f), fmaxf(z.y, 0.0f));
+      y = __ffma2_rn(make_float2(-x.x, -x.y), q, top);
+      const float2 cdf = make_float2(z.x < 0.0f ? q.x : 1.0f - q.x, z.y < 0.0f ? q.y : 1.0f - q.y);
+      d = __ffma2_rn(__fmul2_rn(z, pair(0.3989422804f)), g, cdf);
     }
   } else {
     y = z;
-    d = 1.0f;
+    d = pair(1.0f);
   }
 }
 
-// act' lies in (-0.2, 1.2).  Beside 16-bit outputs it is kept in 16 bits, with a sign, 4
-// bits of exponent and 11 of mantissa: half a step is 2^-12 of the value (down to
-// 2^-14, 2^-26 absolute below), a half of float16's and an eighth of bfloat16's, so
-// the product dy * act' is off by its own rounding and little else.
-// The float scaled by 2^-112 has its exponent in the low 4 bits of the field.
-__device__ __forceinline__ uint16_t pack_slope(float d) {
-  const uint32_t f = __float_as_uint(d);
-  uint32_t u = __float_as_uint(__fmul_rn(__uint_as_float(f & 0x7fffffffu), 0x1p-112f));
-  u = (u + 0x7ffu + ((u >> 12) & 1u)) >> 12;
-  // a NaN (and nothing else) is beyond the 15 bits: keep it as the largest code
-  return (uint16_t)((u > 0x7fffu ? 0x7fffu : u) | ((f >> 16) & 0x8000u));
+// act' lies in (-0.2, 1.2) and is kept in 16 bits beside 16-bit types, more precisely
+// than they hold values, so that the product dy * act' is off by its own rounding
+// and little else: beside bfloat16 as float16 (half a step 2^-11 of the value, a quarter
+// of bfloat16's), beside float16 with a sign, 4 bits of exponent and 11 of mantissa (2^-12,
+// half of float16's, down to 2^-14; 2^-26 absolute below).  For the latter the float
+// scaled by 2^-112 has its exponent in the low 4 bits of the field.
+template <typename T>
+struct Slope;
+template <>
+struct Slope<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float2 d) {
+    const __half2 h = __float22half2_rn(d);
+    return *(const uint32_t*)&h;
+  }
+  static __device__ __forceinline__ float unpack(uint16_t v) { return __half2float(__ushort_as_half(v)); }
+};
+template <>
+struct Slope<__half> {
+  static __device__ __forceinline__ uint32_t pack(float2 d) {
+    const float2 s = __fmul2_rn(d, pair(0x1p-112f));
+    const uint32_t a = __float_as_uint(s.x) + 0x800u, b = __float_as_uint(s.y) + 0x800u;
+    const uint32_t m = ((a >> 12) & 0x7fffu) | ((b << 4) & 0x7fff0000u);
+    return m | ((a >> 16) & 0x8000u) | (b & 0x80000000u);
+  }
+  static __device__ __forceinline__ float unpack(uint16_t v) {
+    const float m = __uint_as_float((uint32_t)(v & 0x7fffu) << 12) * 0x1p112f;
+    return v & 0x8000u ? -m : m;
+  }
+};
+
+// Two float32 values rounded to T, packed.
+__device__ __forceinline__ uint32_t pack2(float2 v, __half) {
+  const __half2 h = __float22half2_rn(v);
+  return *(const uint32_t*)&h;
 }
-__device__ __forceinline__ float unpack_slope(uint16_t v) {
-  const float m = (v & 0x7fffu) == 0x7fffu ? NAN : __fmul_rn(__uint_as_float((uint32_t)(v & 0x7fffu) << 12), 0x1p112f);
-  return v & 0x8000u ? -m : m;
+__device__ __forceinline__ uint32_t pack2(float2 v, __nv_bfloat16) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(v);
+  return *(const uint32_t*)&h;
 }
 
 // x = p0 + p1 + p2 with bfloat16 parts: 24 bits in all.  p0 is cut, not rounded, so that
