@@ -10,7 +10,8 @@ torch.finfo(t).eps / 2; e = 2^-23, a truncated float32 step):
   16-bit parts (dropped products, 3 * 2^-24) and the bias;
 * act has slope at most 1.13 and act' slope at most 1 (relu's act' jumps: there an
   error of 1 is allowed where |z| <= dz); act and act' are evaluated to 32 e
-  relative plus 1e-7 absolute;
+  relative plus 1e-7 absolute, beside 16-bit types to 64 e (7.6e-6: gelu's polynomial is
+  6.1e-6 off in float32, and act' = Q + x phi cancels, so its error counts against Q <= 1/2);
 * y is rounded once: u |y|; float16 adds half its smallest step, 2^-25;
 * s = dy act': act' is kept in T and the product rounded to T: 2u + u^2 relative
   (float16: 2^-25 absolute each);
@@ -78,7 +79,8 @@ def linear_act(x, w, b, r, act, dy=None):
     dt = x.dtype
     z, dz = product(x, w, b)
     y, d = act64(act, z)
-    by = 1.13 * dz + 32 * E * y.abs() + 1e-7
+    rel = (32 if dt in (torch.float32, torch.float64) else 64) * E
+    by = 1.13 * dz + rel * y.abs() + 1e-7
     if r is not None:
         y = y + r.double()
         by = by + E * (y.abs() + r.double().abs())
@@ -88,7 +90,7 @@ def linear_act(x, w, b, r, act, dy=None):
     g = dy.double()
     s = g * d
     u = half_step(dt)
-    bd = dz + 32 * E * d.abs() + 1e-7
+    bd = dz + rel * (d.abs() if rel == 32 * E else d.abs().clamp(min=0.5)) + 1e-7
     if act == "relu":
         bd = (z.abs() <= dz).double()
     if act == "none":

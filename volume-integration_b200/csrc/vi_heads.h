@@ -40,8 +40,9 @@ enum Epi {
 struct Epilogue {
   int act;              // kEpiAct: vi_activation
   const void* bias;     // kEpiAct, kEpiLse, kEpiGrad: [N] or null
+  int bias_rows;        // kEpiAct: bias is [M], one value per row
   View res;             // kEpiAct: residual, p null = none
-  View out;             // kEpiAct, kEpiStore: T
+  View out;             // kEpiAct, kEpiStore: T, one stride 1
   void* dact;           // kEpiAct: act'(z) in out's strides (float32, or 16 bits: pack_slope), null = not wanted
   const float* alpha;   // kEpiStore: device scalar the product is multiplied with, null = 1
   float* part;          // kEpiPartial: [splits][M][N]

@@ -51,11 +51,25 @@ struct Shape {
   static constexpr int kStages = BN == 256 ? (sizeof(T) == 4 && EPI == kEpiGrad ? 3 : 4) : BN == 128 ? (kBlocks == 2 ? 2 : 5) : (kBlocks == 2 ? 3 : 7);
   static constexpr int kStage = (kBM + BN) * kBK * 2;  // bytes
   static constexpr int kStageWarp = EPI == kEpiLse ? 0 : 32 * 32 * (int)sizeof(T);  // an epilogue warp's staging
-  static constexpr int kSmem = 1024 + kStages * kStage + kWarps * kStageWarp;
+  // beside the stages each epilogue warp has its staging and 32 float32 of bias
+  static constexpr int kBars = kStages * kStage + kWarps * (kStageWarp + 128);
+  static constexpr int kSmem = kBars + (2 * kStages + 5) * 8 + 8;
+};
+
+// n / d for 0 <= n < 2^31 by a multiplication: mul = ceil(2^(31 + s) / d), s = ceil(log2 d).
+// The rounding of mul adds less than n / 2^31 / d to the quotient, which changes no floor.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  static FastDiv of(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) s++;
+    return FastDiv{d, d == 1 ? 0u : (uint32_t)(((1ull << (31 + s)) + d - 1) / d), s ? s - 1 : 0};
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return d == 1 ? n : __umulhi(n, mul) >> shift; }
 };
 
 struct Args {
-  int64_t M, N;
+  int M, N;
   int m_tiles, n_tiles;  // n_tiles: column tiles
   int kblocks;           // 64-wide blocks of the whole sum
   int kps, splits;
@@ -65,7 +79,9 @@ struct Args {
   uint32_t a_lbo, b_lbo; // bytes >> 4
   uint32_t a_step, b_step;  // bytes >> 4 from one 16-wide slice of k to the next
   int a_k_major, b_k_major;
-  int64_t items;
+  int items;
+  FastDiv per_split, per_group;  // items of one piece of the sum; of 16 row tiles
+  FastDiv last_rows;             // row tiles of the last group
   uint32_t spin_limit;
   int withhold;          // testing hook: the first load is never issued
   Epilogue e;
@@ -86,7 +102,7 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 0x989680;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
@@ -110,6 +126,32 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, u
           dst),
       "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
+}
+
+// Shared memory by its 32-bit address: a generic pointer would cost 64-bit arithmetic per access.
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_cell(uint32_t a, uint32_t) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint16_t lds_cell(uint32_t a, uint16_t) {
+  uint16_t v;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts_cell(uint32_t a, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+__device__ __forceinline__ void sts_cell(uint32_t a, uint16_t v) {
+  asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"(v) : "memory");
 }
 
 // Shared-memory matrix descriptor: address, leading and stride byte offsets (>> 4),
@@ -144,6 +186,15 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float* v) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -155,20 +206,29 @@ struct Item {
   int mt, nt, nt_end, kb0, kb1, split, span;
 };
 template <int EPI>
-__device__ __forceinline__ Item item_of(const Args& a, int64_t i) {
+__device__ __forceinline__ Item item_of(const Args& a, int i) {
   Item t;
-  const int cols = EPI == kEpiLse ? a.spans : a.n_tiles;
   t.split = 0;
   if (EPI == kEpiPartial) {
-    const int64_t per = (int64_t)a.m_tiles * a.n_tiles;
-    t.split = (int)(i / per);
-    i -= t.split * per;
+    t.split = (int)a.per_split.div(i);
+    i -= t.split * (int)a.per_split.d;
   }
-  const int64_t group = i / (16ll * cols);
-  const int gm = min(16, a.m_tiles - (int)group * 16);
-  const int r = (int)(i - group * 16 * cols);
-  t.mt = (int)group * 16 + r % gm;
-  t.span = r / gm;
+  if (EPI != kEpiLse && a.n_tiles == 1) {
+    t.mt = i;
+    t.span = t.nt = 0;
+    t.nt_end = 1;
+    t.kb0 = t.split * a.kps;
+    t.kb1 = min(a.kblocks, t.kb0 + a.kps);
+    return t;
+  }
+  const int group = (int)a.per_group.div(i), r = i - group * (int)a.per_group.d;
+  if (group * 16 + 16 <= a.m_tiles) {
+    t.mt = group * 16 + (r & 15);
+    t.span = r >> 4;
+  } else {
+    t.span = (int)a.last_rows.div(r);
+    t.mt = group * 16 + r - t.span * (int)a.last_rows.d;
+  }
   t.nt = EPI == kEpiLse ? t.span * a.span : t.span;
   t.nt_end = EPI == kEpiLse ? min(a.n_tiles, t.nt + a.span) : t.nt + 1;
   t.kb0 = t.split * a.kps;
@@ -179,27 +239,6 @@ __device__ __forceinline__ Item item_of(const Args& a, int64_t i) {
 // ---- epilogue pieces ----
 // Each works on 32 rows (one per lane) x 32 columns in registers.
 
-// v += bias of columns [n0, n0 + 32).
-template <typename T>
-__device__ __forceinline__ void add_bias(const void* bias, int64_t n0, int64_t N, float2* v) {
-  const T* p = (const T*)bias + n0;
-  if (n0 + 32 <= N && ((uintptr_t)p & 15) == 0) {
-    constexpr int per = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 32 / per; i++) {
-      const uint4 q = __ldg((const uint4*)p + i);
-      const T* t = (const T*)&q;
-#pragma unroll
-      for (int j = 0; j < per / 2; j++)
-        v[i * (per / 2) + j] = __fadd2_rn(v[i * (per / 2) + j], make_float2(to_f(t[2 * j]), to_f(t[2 * j + 1])));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; j++)
-      if (n0 + j < N) ((float*)v)[j] += to_f(p[j]);
-  }
-}
-
 // The stored type of act' beside T.
 template <typename T>
 using SlopeCell = typename std::conditional<sizeof(T) == 4, float, uint16_t>::type;
@@ -208,8 +247,10 @@ using SlopeCell = typename std::conditional<sizeof(T) == 4, float, uint16_t>::ty
 template <typename Z>
 union Row {
   static constexpr int kPieces = 2 * sizeof(Z);  // of 16 bytes
+  using Bits = typename std::conditional<sizeof(Z) == 4, uint32_t, uint16_t>::type;
   uint4 q[kPieces];
   uint32_t w[8 * sizeof(Z)];
+  Bits b[32];
   Z z[32];
   __device__ __forceinline__ Row() {}
 };
@@ -228,140 +269,206 @@ __device__ __forceinline__ float2 get_pair(const Row<T>& r, int j) {
   return make_float2(to_f(r.z[2 * j]), to_f(r.z[2 * j + 1]));
 }
 
-// A warp's staging, 32 rows of 32 elements: the 16-byte pieces of a row are exchanged
-// by the row's number, so that lanes writing a row each and lanes reading along rows
-// both touch every bank once.
+// A lane's places in its warp's staging, 32 lines of 32 elements.  The 16-byte pieces of a
+// line are exchanged by the line's number, so that lanes writing a line each and lanes
+// reading along lines both touch every bank once.
 template <typename Z>
-__device__ __forceinline__ uint4* staged(void* st, int row, int piece) {
-  constexpr int pieces = Row<Z>::kPieces;
-  return (uint4*)st + row * pieces + (piece ^ (sizeof(Z) == 4 ? row & 7 : (row >> 1) & 3));
-}
+struct Stage {
+  static constexpr int kLanes = Row<Z>::kPieces, kStep = 32 / kLanes, kPer = 16 / (int)sizeof(Z);  // lanes a line, lines a step
+  static constexpr uint32_t kLine = 32 * sizeof(Z);
+  static __device__ __forceinline__ uint32_t key(int line) { return (uint32_t)(sizeof(Z) == 4 ? line & 7 : (line >> 1) & 3) << 4; }
+  // piece i of the lane's own line
+  static __device__ __forceinline__ uint32_t own(uint32_t st, int lane, int i) {
+    return st + lane * kLine + ((uint32_t)(i << 4) ^ key(lane));
+  }
+  // the lane's piece of its line of step i
+  static __device__ __forceinline__ uint32_t along(uint32_t st, int lane, int i) {
+    const int line = lane / kLanes + i * kStep;
+    return st + line * kLine + ((uint32_t)((lane % kLanes) << 4) ^ key(line));
+  }
+};
 
-enum Access { kNone, kImage, kVector, kScalar };
-// How a matrix is reached: rows contiguous, columns contiguous on 16-byte rows, or any strides.
+// An image's tile: the column of the lane's line in step i.  16-bit elements are staged
+// in pairs of columns, 4 bytes a row, so that a lane's 8 rows of a pair are two 16-byte
+// pieces; odd pairs have them exchanged, so that 8 lanes touch every bank once.
 template <typename Z>
-__host__ __device__ __forceinline__ int access_of(const View& v) {
+__device__ __forceinline__ int image_column(int line, int i) {
+  return sizeof(Z) == 4 ? line + i * 4 : 2 * (line + (i >> 1) * 8) + (i & 1);
+}
+__device__ __forceinline__ uint32_t image_line(int lane, int i) { return (lane / 4 + i * 8) * 128 + (lane % 4) * 32; }
+__device__ __forceinline__ uint32_t image_half(int lane) { return (lane & 4) << 2; }
+
+enum Access { kNone, kVector, kImage, kScalar };
+// How a matrix is reached: columns contiguous on 16-byte rows, rows contiguous on 16-byte
+// columns (an image), or any strides.
+template <typename Z>
+__device__ __forceinline__ int access_of(const View& v) {
   if (!v.p) return kNone;
-  if (v.rs == 1) return kImage;
-  return v.cs == 1 && ((uintptr_t)v.p & 15) == 0 && v.rs % (16 / (int)sizeof(Z)) == 0 ? kVector : kScalar;
+  constexpr int per = 16 / (int)sizeof(Z);
+  if ((uintptr_t)v.p & 15) return kScalar;
+  return v.cs == 1 && v.rs % per == 0 ? kVector : v.rs == 1 && v.cs % per == 0 ? kImage : kScalar;
 }
 
-// Loads 32 x 32 elements of v.  kVector leaves them as lanes along rows (see own_row); the
-// other ways give each lane its row.
+// A 32 x 32 tile of a matrix: its first element's row and column, and how many of its rows and
+// columns exist (at least one each).
+struct Place {
+  int m0, n0;
+  int rows, cols;
+};
+
+// Loads a tile of v, 16 bytes a lane: along rows (kVector), along columns (kImage), to be
+// handed to their rows' lanes by own_row; or else each lane its row.  Returns the way.
 template <typename Z>
-__device__ __forceinline__ bool load_tile(Row<Z>& r, const View& v, int access, int lane, int64_t m0, int64_t n0,
-                                          int64_t M, int64_t N) {
+__device__ __forceinline__ int load_tile(Row<Z>& r, const View& v, int access, int lane, const Place& t) {
+  using G = Stage<Z>;
   const Z* p = (const Z*)v.p;
-  if (access == kVector && n0 + 32 <= N) {
-    constexpr int lanes = Row<Z>::kPieces, step = 32 / lanes;  // lanes a row, rows a step
-    const int row = lane / lanes, piece = lane % lanes;
-    const Z* q = p + (m0 + row) * v.rs + n0 + piece * (16 / (int)sizeof(Z));
+  const int line = lane / G::kLanes, piece = lane % G::kLanes;
+  if (access == kVector && t.cols >= 32) {
+    const Z* q = p + (int64_t)(t.m0 + line) * v.rs + t.n0 + piece * G::kPer;
+    const int64_t step = G::kStep * v.rs;
 #pragma unroll
-    for (int i = 0; i < lanes; i++)
-      if (m0 + row + i * step < M) r.q[i] = *(const uint4*)(q + (int64_t)i * step * v.rs);
-    return true;
+    for (int i = 0; i < G::kLanes; i++, q += step)
+      if (line + i * G::kStep < t.rows) r.q[i] = *(const uint4*)q;
+    return kVector;
   }
-  const int64_t m = m0 + lane;
-  if (m < M) {
-    const Z* q = p + m * v.rs + n0 * v.cs;
-    if (n0 + 32 <= N) {
+  if (access == kImage && t.rows >= 32) {
+    const Z* q = p + (int64_t)t.n0 * v.cs + t.m0 + piece * G::kPer;
 #pragma unroll
-      for (int j = 0; j < 32; j++) r.z[j] = q[j * v.cs];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; j++)
-        if (n0 + j < N) r.z[j] = q[j * v.cs];
+    for (int i = 0; i < G::kLanes; i++) {
+      const int c = image_column<Z>(line, i);
+      if (c < t.cols) r.q[i] = *(const uint4*)(q + c * v.cs);
     }
+    return kImage;
   }
-  return false;
+  if (lane < t.rows) {
+    const Z* q = p + (int64_t)(t.m0 + lane) * v.rs + (int64_t)t.n0 * v.cs;
+#pragma unroll
+    for (int j = 0; j < 32; j++, q += v.cs)
+      if (j < t.cols) r.z[j] = *q;
+  }
+  return kScalar;
 }
-// From lanes along rows to a row each, through the staging.
+// What load_tile left along lines, to a row each, through the staging.
 template <typename Z>
-__device__ __forceinline__ void own_row(Row<Z>& r, void* st, int lane) {
-  constexpr int lanes = Row<Z>::kPieces, step = 32 / lanes;
+__device__ __forceinline__ void own_row(Row<Z>& r, int way, uint32_t st, int lane) {
+  using G = Stage<Z>;
+  if (way == kScalar) return;
   __syncwarp();
+  if (way == kVector) {
 #pragma unroll
-  for (int i = 0; i < lanes; i++) *staged<Z>(st, lane / lanes + i * step, lane % lanes) = r.q[i];
-  __syncwarp();
+    for (int i = 0; i < G::kLanes; i++) sts128(G::along(st, lane, i), r.q[i]);
+    __syncwarp();
 #pragma unroll
-  for (int i = 0; i < lanes; i++) r.q[i] = *staged<Z>(st, lane, i);
+    for (int i = 0; i < G::kLanes; i++) r.q[i] = lds128(G::own(st, lane, i));
+  } else if constexpr (sizeof(Z) == 4) {  // staged as columns of 32 rows; neighbouring lanes read neighbouring elements
+#pragma unroll
+    for (int i = 0; i < G::kLanes; i++) sts128(st + lane * 16 + i * 512, r.q[i]);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; j++) r.b[j] = lds_cell(st + lane * 4 + j * 128, 0u);
+  } else {  // staged as pairs of columns of 32 rows
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const uint4 a = r.q[2 * i], b = r.q[2 * i + 1];
+      const uint32_t at = st + image_line(lane, i);
+      sts128(at + image_half(lane), make_uint4(__byte_perm(a.x, b.x, 0x5410), __byte_perm(a.x, b.x, 0x7632),
+                                               __byte_perm(a.y, b.y, 0x5410), __byte_perm(a.y, b.y, 0x7632)));
+      sts128(at + (image_half(lane) ^ 16), make_uint4(__byte_perm(a.z, b.z, 0x5410), __byte_perm(a.z, b.z, 0x7632),
+                                                      __byte_perm(a.w, b.w, 0x5410), __byte_perm(a.w, b.w, 0x7632)));
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; j++) r.w[j] = lds_cell(st + j * 128 + ((lane * 4) ^ ((j & 1) << 4)), 0u);
+  }
 }
 
-// Writes each lane's row to rows [m0, m0 + 32), columns [n0, n0 + 32) of v, one of whose strides is 1.
+// Writes each lane's row to a tile of v, one of whose strides is 1.
 template <typename Z>
-__device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int access, void* st, int lane, int64_t m0,
-                                           int64_t n0, int64_t M, int64_t N) {
+__device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int access, uint32_t st, int lane,
+                                           const Place& t) {
+  using G = Stage<Z>;
   Z* p = (Z*)v.p;
-  if (access == kImage) {
-    const int64_t m = m0 + lane;
-    if (m >= M) return;
-    Z* q = p + m + n0 * v.cs;
-    if (n0 + 32 <= N) {
+  const int line = lane / G::kLanes, piece = lane % G::kLanes;
+  __syncwarp();
+  if (access == kImage && t.rows >= 32) {
+    Z* q = p + (int64_t)t.n0 * v.cs + t.m0 + piece * G::kPer;
+    if constexpr (sizeof(Z) == 4) {
 #pragma unroll
-      for (int j = 0; j < 32; j++) q[j * v.cs] = r.z[j];
+      for (int j = 0; j < 32; j++) sts_cell(st + lane * 4 + j * 128, r.w[j]);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < G::kLanes; i++) {
+        const int c = image_column<Z>(line, i);
+        if (c < t.cols) *(uint4*)(q + c * v.cs) = lds128(st + lane * 16 + i * 512);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 32; j++)
-        if (n0 + j < N) q[j * v.cs] = r.z[j];
+      for (int j = 0; j < 16; j++) sts_cell(st + j * 128 + ((lane * 4) ^ ((j & 1) << 4)), r.w[j]);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const uint32_t at = st + image_line(lane, i);
+        const uint4 a = lds128(at + image_half(lane)), b = lds128(at + (image_half(lane) ^ 16));
+        const int c = image_column<Z>(line, 2 * i);
+        if (c < t.cols)
+          *(uint4*)(q + c * v.cs) = make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410),
+                                               __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410));
+        if (c + 1 < t.cols)
+          *(uint4*)(q + (c + 1) * v.cs) = make_uint4(__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632),
+                                                     __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632));
+      }
     }
     return;
   }
-  constexpr int lanes = Row<Z>::kPieces, step = 32 / lanes, per = 16 / (int)sizeof(Z);
-  __syncwarp();
+  if (v.rs == 1 && v.cs != 1) {  // an image off 16 bytes, or its ragged end: lanes along the rows
+    if (lane < t.rows) {
+      Z* q = p + t.m0 + lane + (int64_t)t.n0 * v.cs;
 #pragma unroll
-  for (int i = 0; i < lanes; i++) *staged<Z>(st, lane, i) = r.q[i];
-  __syncwarp();
-  if (access == kVector && n0 + 32 <= N) {
-    const int row = lane / lanes, piece = lane % lanes;
-    Z* q = p + (m0 + row) * v.rs + n0 + piece * per;
-#pragma unroll
-    for (int i = 0; i < lanes; i++)
-      if (m0 + row + i * step < M) *(uint4*)(q + (int64_t)i * step * v.rs) = *staged<Z>(st, row + i * step, piece);
-  } else {  // a row at a time, each lane a column
-    const int64_t n = n0 + lane;
-    for (int row = 0; row < 32 && m0 + row < M; row++)
-      if (n < N) p[(m0 + row) * v.rs + n] = ((const Z*)staged<Z>(st, row, lane / per))[lane % per];
-  }
-}
-
-// act over a row; the values stay in v, act' goes to d as stored.
-template <typename T, int ACT, bool SLOPE>
-__device__ __forceinline__ void activate_row(float2* v, Row<SlopeCell<T>>& d) {
-#pragma unroll
-  for (int j = 0; j < 16; j++) {
-    float2 y, s;
-    activate<ACT, sizeof(T) == 4>(v[j], y, s);
-    v[j] = y;
-    if constexpr (SLOPE) {
-      if constexpr (sizeof(T) == 4) set_pair(d, j, s);
-      else d.w[j] = Slope<T>::pack(s);
+      for (int j = 0; j < 32; j++, q += v.cs)
+        if (j < t.cols) *q = r.z[j];
     }
+    return;
   }
-}
-template <typename T, bool SLOPE>
-__device__ __forceinline__ void activate_row(int act, float2* v, Row<SlopeCell<T>>& d) {
-  switch (act) {
-    case VI_ACT_RELU: activate_row<T, VI_ACT_RELU, SLOPE>(v, d); break;
-    case VI_ACT_SILU: activate_row<T, VI_ACT_SILU, SLOPE>(v, d); break;
-    case VI_ACT_GELU: activate_row<T, VI_ACT_GELU, SLOPE>(v, d); break;
-    case VI_ACT_SIGMOID: activate_row<T, VI_ACT_SIGMOID, SLOPE>(v, d); break;
-    default: activate_row<T, VI_ACT_NONE, SLOPE>(v, d);
+#pragma unroll
+  for (int i = 0; i < G::kLanes; i++) sts128(G::own(st, lane, i), r.q[i]);
+  __syncwarp();
+  if (access == kVector && t.cols >= 32) {
+    Z* q = p + (int64_t)(t.m0 + line) * v.rs + t.n0 + piece * G::kPer;
+    const int64_t step = G::kStep * v.rs;
+#pragma unroll
+    for (int i = 0; i < G::kLanes; i++, q += step)
+      if (line + i * G::kStep < t.rows) *(uint4*)q = lds128(G::along(st, lane, i));
+  } else {  // a row at a time, each lane a column
+    typename Row<Z>::Bits* q = (typename Row<Z>::Bits*)p + (int64_t)t.m0 * v.rs + (int64_t)(t.n0 + lane) * v.cs;
+    for (int row = 0; row < min(32, t.rows); row++, q += v.rs)
+      if (lane < t.cols)
+        *q = lds_cell(st + row * G::kLine + ((uint32_t)(lane / G::kPer << 4) ^ G::key(row)) + lane % G::kPer * (int)sizeof(Z),
+                      typename Row<Z>::Bits());
   }
 }
 
-template <typename T, int BN, int EPI>
+// v += COLS values of a bias slot.
+template <int COLS>
+__device__ __forceinline__ void add_bias(uint32_t slot, float2* v) {
+#pragma unroll
+  for (int i = 0; i < COLS / 4; i++) {
+    const uint4 q = lds128(slot + i * 16);
+    v[2 * i] = __fadd2_rn(v[2 * i], make_float2(__uint_as_float(q.x), __uint_as_float(q.y)));
+    v[2 * i + 1] = __fadd2_rn(v[2 * i + 1], make_float2(__uint_as_float(q.z), __uint_as_float(q.w)));
+  }
+}
+
+template <typename T, int BN, int EPI, int ACT>
 __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>::kBlocks)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ Args a) {
   using S = Shape<T, BN, EPI>;
   constexpr int kStages = S::kStages, kStage = S::kStage, kEpiWarps = S::kWarps;
   constexpr uint32_t kCols = BN < 128 ? 2 * 64 : 2 * BN;  // tensor memory columns: two accumulators
-  extern __shared__ char smem_raw[];
-  __shared__ uint64_t bars[2 * kStages + 5];
-  __shared__ uint32_t tmem_slot;
-  __shared__ int dead_flag;
-  char* smem = (char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  volatile int* dead = &dead_flag;
+  extern __shared__ __align__(1024) char smem[];
+  uint64_t* bars = (uint64_t*)(smem + S::kBars);
+  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * kStages + 5);
+  volatile int* dead = (int*)(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t full = smem_u32(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages, tempty = tfull + 16,
                  drain = tempty + 16;
@@ -376,18 +483,18 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
       mbar_init(tempty + 8 * i, kEpiWarps);
     }
     mbar_init(drain, 1);
-    dead_flag = 0;
+    *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kEpiWarps + 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kCols)
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = *tmem_slot;
 
   if (warp == kEpiWarps) {
     // ---- loads ----
@@ -396,7 +503,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
       uint32_t phase = 0;
       int64_t issued = 0;
       bool on = true;
-      for (int64_t i = blockIdx.x; i < a.items && on; i += gridDim.x) {
+      for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
         const Item t = item_of<EPI>(a, i);
         for (int nt = t.nt; nt < t.nt_end && on; nt++) {
           for (int p = 0; p < a.pairs && on; p++) {
@@ -449,7 +556,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool on = true;
-      for (int64_t i = blockIdx.x; i < a.items && on; i += gridDim.x) {
+      for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
         const Item t = item_of<EPI>(a, i);
         const int steps = a.pairs * (t.kb1 - t.kb0);
         for (int nt = t.nt; nt < t.nt_end && on; nt++) {
@@ -487,14 +594,19 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
   } else {
     // ---- epilogue ----
     const int quad = warp % 4, part = warp / 4;
-    void* st = smem + kStages * kStage + warp * S::kStageWarp;
+    const uint32_t st = smem_u32(smem + kStages * kStage) + warp * S::kStageWarp;
+    const uint32_t bias_slot = smem_u32(smem + kStages * kStage) + kEpiWarps * S::kStageWarp + warp * 128;
+    int bias_at = -1;  // column the slot holds
     const Epilogue& e = a.e;
+    const int out_access = access_of<T>(e.out), res_access = access_of<T>(e.res);
     int acc = 0;
     uint32_t acc_phase = 0;
     bool on = true;
-    for (int64_t i = blockIdx.x; i < a.items && on; i += gridDim.x) {
+    for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
       const Item t = item_of<EPI>(a, i);
-      const int64_t m0 = (int64_t)t.mt * kBM + quad * 32, m = m0 + lane;
+      const int m0 = t.mt * kBM + quad * 32, m = m0 + lane;
+      const int rows = min(32, a.M - m0);
+      auto place = [&](int n0) { return Place{m0, n0, rows, min(32, a.N - n0)}; };
       float top = -INFINITY, sum = 0.0f;
       int64_t target = -1;
       float lsum = 0.0f, coef = 0.0f, alpha = 1.0f;
@@ -503,55 +615,96 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
       }
       if (EPI == kEpiGrad && m < a.M) top = e.lse[m], lsum = e.lse[a.M + m], coef = e.coef[m];
       if (EPI == kEpiStore && e.alpha) alpha = *e.alpha;
+      float row_bias = 0.0f;
+      if (EPI == kEpiAct && e.bias_rows && m < a.M) row_bias = to_f(((const T*)e.bias)[m]);
       for (int nt = t.nt; nt < t.nt_end; nt++) {
         // what the epilogue adds is asked for before the product is waited for
         constexpr bool kAdds = EPI == kEpiAct || EPI == kEpiPartial;
         const int first = part * 32;
-        const int64_t col = (int64_t)nt * BN;
+        const int col = nt * BN;
         View add{nullptr, 0, 0};
         if (EPI == kEpiAct) add = e.res;
         if (EPI == kEpiPartial && e.add) add = View{e.part + (int64_t)t.split * a.M * a.N, a.N, 1};
         Row<T> extra;
-        bool along = false;
-        if (kAdds && add.p && col + first < a.N)
-          along = load_tile<T>(extra, add, access_of<T>(add), lane, m0, col + first, a.M, a.N);
+        int way = kNone;
+        if (kAdds && add.p && col + first < a.N && m0 < a.M)
+          way = load_tile<T>(extra, add, EPI == kEpiAct ? res_access : access_of<T>(add), lane, place(col + first));
         if (!mbar_wait(tfull + 8 * acc, acc_phase, dead, a.spin_limit)) on = false;
         on = __all_sync(0xffffffffu, on);
         if (!on) break;
         fence_after();
 #pragma unroll 1
-        for (int c = first; c < BN && col + c < a.N; c += 32 * S::kParts) {
-          const int64_t n0 = col + c;
+        for (int c = first; c < BN && col + c < a.N && m0 < a.M; c += 32 * S::kParts) {
+          const int n0 = col + c;
+          const Place here = place(n0);
           if (kAdds && add.p && c != first)
-            along = load_tile<T>(extra, add, access_of<T>(add), lane, m0, n0, a.M, a.N);
-          float2 v[16];
+            way = load_tile<T>(extra, add, EPI == kEpiAct ? res_access : access_of<T>(add), lane, here);
+          const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + c;
+          if (EPI != kEpiPartial && EPI != kEpiStore) {
+            if (e.bias && !e.bias_rows && bias_at != n0) {  // a lane a column, then every lane all of them
+              __syncwarp();
+              sts_cell(bias_slot + lane * 4, __float_as_uint(lane < here.cols ? to_f(((const T*)e.bias)[n0 + lane]) : 0.0f));
+              bias_at = n0;
+            }
+          }
           __syncwarp();
-          tmem_load32(tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + c, (float*)v);
-          tmem_wait_load();
-          if (EPI != kEpiPartial && EPI != kEpiStore)
-            if (e.bias) add_bias<T>(e.bias, n0, a.N, v);
           if constexpr (EPI == kEpiAct || EPI == kEpiStore || EPI == kEpiPartial) {
-            if constexpr (EPI == kEpiAct) {
-              Row<SlopeCell<T>> d;
-              if (e.dact) {
-                const View slope{e.dact, e.out.rs, e.out.cs};
-                activate_row<T, true>(e.act, v, d);
-                store_tile(d, slope, access_of<T>(slope), st, lane, m0, n0, a.M, a.N);
-              } else {
-                activate_row<T, false>(e.act, v, d);
-              }
-            }
-            if (kAdds && add.p) {
-              if (along) own_row<T>(extra, st, lane);
-#pragma unroll
-              for (int j = 0; j < 16; j++) v[j] = __fadd2_rn(v[j], get_pair(extra, j));
-            }
+            if (kAdds && add.p) own_row<T>(extra, way, st, lane);
             Row<T> y;
+            auto columns = [&](auto with_slope, Row<SlopeCell<T>>& d) {
+              constexpr bool kSlope = decltype(with_slope)::value;
 #pragma unroll
-            for (int j = 0; j < 16; j++) set_pair(y, j, EPI == kEpiStore ? __fmul2_rn(v[j], pair(alpha)) : v[j]);
+              for (int h = 0; h < 2; h++) {  // 16 columns at a time: with 32 the activations spill
+                float2 v[8];
+                tmem_load16(src + h * 16, (float*)v);
+                tmem_wait_load();
+                if constexpr (EPI == kEpiAct) {
+                  if (e.bias_rows) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = __fadd2_rn(v[j], pair(row_bias));
+                  } else if (e.bias) {
+                    add_bias<16>(bias_slot + h * 64, v);
+                  }
+#pragma unroll
+                  for (int j = 0; j < 8; j++) {
+                    float2 w, s;
+                    activate<ACT, sizeof(T) == 4, kSlope>(v[j], w, s);
+                    v[j] = w;
+                    if constexpr (kSlope) {
+                      if constexpr (sizeof(T) == 4) set_pair(d, h * 8 + j, s);
+                      else d.w[h * 8 + j] = Slope<T>::pack(s);
+                    }
+                  }
+                }
+                if (kAdds && add.p) {
+#pragma unroll
+                  for (int j = 0; j < 8; j++) v[j] = __fadd2_rn(v[j], get_pair(extra, h * 8 + j));
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                  set_pair(y, h * 8 + j, EPI == kEpiStore ? __fmul2_rn(v[j], pair(alpha)) : v[j]);
+                // the half is finished before the next one starts, or their registers add up
+#pragma unroll
+                for (int j = 0; j < 4 * (int)sizeof(T); j++) {
+                  asm volatile("" : "+r"(y.w[h * 4 * sizeof(T) + j]));
+                  if constexpr (kSlope) asm volatile("" : "+r"(d.w[h * 4 * sizeof(T) + j]));
+                }
+              }
+            };
+            Row<SlopeCell<T>> d;
+            if (ACT != VI_ACT_NONE && e.dact) {
+              columns(std::true_type(), d);
+              store_tile(d, View{e.dact, e.out.rs, e.out.cs}, (uintptr_t)e.dact & 15 ? kScalar : out_access, st, lane, here);
+            } else {
+              columns(std::false_type(), d);
+            }
             const View out = EPI == kEpiPartial ? View{e.part + (int64_t)t.split * a.M * a.N, a.N, 1} : e.out;
-            store_tile(y, out, access_of<T>(out), st, lane, m0, n0, a.M, a.N);
+            store_tile(y, out, EPI == kEpiPartial ? access_of<T>(out) : out_access, st, lane, here);
           } else if constexpr (EPI == kEpiLse) {
+            float2 v[16];
+            tmem_load32(src, (float*)v);
+            tmem_wait_load();
+            if (e.bias) add_bias<32>(bias_slot, v);
             float* z = (float*)v;
             if (__any_sync(0xffffffffu, target >= n0 && target < n0 + 32)) {
 #pragma unroll
@@ -578,6 +731,10 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
             sum = sum * exp2_fast((top - ref) * kLog2e) + (s2.x + s2.y);
             top = best;
           } else if constexpr (EPI == kEpiGrad) {
+            float2 v[16];
+            tmem_load32(src, (float*)v);
+            tmem_wait_load();
+            if (e.bias) add_bias<32>(bias_slot, v);
             float* z = (float*)v;
 #pragma unroll
             for (int j = 0; j < 16; j++) {
@@ -606,13 +763,13 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
                   g.z[j] = s3[pl];
                 }
                 const View out{(__nv_bfloat16*)e.grad + pl * e.grad_plane, e.grad_ld, 1};
-                store_tile(g, out, kVector, st, lane, m0, n0, a.M, a.N);
+                store_tile(g, out, kVector, st, lane, here);
               }
             } else {
               Row<T> g;
 #pragma unroll
               for (int j = 0; j < 16; j++) set_pair(g, j, v[j]);
-              store_tile(g, View{e.grad, e.grad_ld, 1}, kVector, st, lane, m0, n0, a.M, a.N);
+              store_tile(g, View{e.grad, e.grad_ld, 1}, kVector, st, lane, here);
             }
           }
         }
@@ -664,25 +821,32 @@ bool encode(CUtensorMap* map, const Operand& o, int planes, bool half, int box_r
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int BN, int EPI>
+template <typename T, int BN, int EPI, int ACT>
 cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
-  auto* k = gemm_tc_kernel<T, BN, EPI>;
+  auto* k = gemm_tc_kernel<T, BN, EPI, ACT>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, BN, EPI>::kSmem);
   if (e != cudaSuccess) return e;
   k<<<(unsigned)std::min<int64_t>(a.items, (int64_t)sms * Shape<T, BN, EPI>::kBlocks), Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>::kSmem, s>>>(ma, mb, a);
   return cudaPeekAtLastError();
 }
-template <typename T, int EPI>
+template <typename T, int EPI, int ACT = VI_ACT_NONE>
 cudaError_t run_bn(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
-  return bn == 256   ? run<T, 256, EPI>(ma, mb, a, sms, s)
-         : bn == 128 ? run<T, 128, EPI>(ma, mb, a, sms, s)
-                     : run<T, 64, EPI>(ma, mb, a, sms, s);
+  return bn == 256   ? run<T, 256, EPI, ACT>(ma, mb, a, sms, s)
+         : bn == 128 ? run<T, 128, EPI, ACT>(ma, mb, a, sms, s)
+                     : run<T, 64, EPI, ACT>(ma, mb, a, sms, s);
 }
 template <typename T>
 cudaError_t run_epi(int epi, int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms,
                     cudaStream_t s) {
   switch (epi) {
-    case kEpiAct: return run_bn<T, kEpiAct>(bn, ma, mb, a, sms, s);
+    case kEpiAct:
+      switch (a.e.act) {
+        case VI_ACT_RELU: return run_bn<T, kEpiAct, VI_ACT_RELU>(bn, ma, mb, a, sms, s);
+        case VI_ACT_SILU: return run_bn<T, kEpiAct, VI_ACT_SILU>(bn, ma, mb, a, sms, s);
+        case VI_ACT_GELU: return run_bn<T, kEpiAct, VI_ACT_GELU>(bn, ma, mb, a, sms, s);
+        case VI_ACT_SIGMOID: return run_bn<T, kEpiAct, VI_ACT_SIGMOID>(bn, ma, mb, a, sms, s);
+        default: return run_bn<T, kEpiAct>(bn, ma, mb, a, sms, s);
+      }
     case kEpiStore: return run_bn<T, kEpiStore>(bn, ma, mb, a, sms, s);
     case kEpiLse: return run_bn<T, kEpiLse>(bn, ma, mb, a, sms, s);
     default: return run_bn<T, kEpiGrad>(bn, ma, mb, a, sms, s);
@@ -701,8 +865,8 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
   if (!encode(&ma, A, planes, half, kBM) || !encode(&mb, B, planes, half, p.bn))
     return set_error(VI_ERR_CUDA, "heads: a tensor map could not be encoded");
   Args a{};
-  a.M = A.rows;
-  a.N = B.rows;
+  a.M = (int)A.rows;
+  a.N = (int)B.rows;
   a.m_tiles = (int)((A.rows + kBM - 1) / kBM);
   a.n_tiles = (int)((B.rows + p.bn - 1) / p.bn);
   a.kblocks = (int)((A.k + kBK - 1) / kBK);
@@ -721,7 +885,13 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
   const uint32_t type = half ? 0 : 1;
   a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((A.k_major ? 0u : 1u) << 15) | ((B.k_major ? 0u : 1u) << 16) |
             ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-  a.items = epi == kEpiLse ? (int64_t)a.m_tiles * p.spans : (int64_t)a.m_tiles * a.n_tiles * p.splits;
+  const int64_t cols = epi == kEpiLse ? p.spans : a.n_tiles, items = (int64_t)a.m_tiles * cols * p.splits;
+  if (items > INT32_MAX - 65536 || 16 * cols > INT32_MAX)
+    return set_error(VI_ERR_UNSUPPORTED, "heads: more than 2^31 tiles");
+  a.items = (int)items;
+  a.per_split = FastDiv::of((uint32_t)(a.m_tiles * cols));
+  a.per_group = FastDiv::of((uint32_t)(16 * cols));
+  a.last_rows = FastDiv::of((uint32_t)(a.m_tiles % 16 ? a.m_tiles % 16 : 16));
   const char* test = getenv("VI_HEADS_TEST_TIMEOUT");
   a.withhold = test && test[0] == '1';
   a.spin_limit = a.withhold ? 1u << 12 : kSpinLimit;

@@ -38,21 +38,27 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
 __device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// act(z) and act'(z) of two values in float32.  A NaN stays a NaN.  EXACT: to a few
-// float32 steps, beside float32 outputs; else to 1e-6 of the value, beside 16-bit ones.
+// act(z) and, where SLOPE, act'(z) of two values in float32.  A NaN stays a NaN.  EXACT: to a
+// few float32 steps, beside float32 outputs; else to 6e-6 of the value, beside 16-bit ones.
 //
 // sigmoid: with e = exp(-z), s = 1 / (1 + e) and 1 - s = e s, without cancellation
-// for large z; e is kept finite, so e s tends to 1 and not to inf * 0.
-// gelu: with x = |z| and Q = Phi(-x), z Phi(z) = max(z, 0) - x Q.  Q = exp(-x^2 / 2) r(t),
-// t = 1 / (1 + 0.265 x), r a polynomial of degree 7 without constant term fitted
-// here to Mills' ratio / sqrt(2 pi) by iteratively reweighted least squares: 6.3e-7 of
-// the value over [0, 14], where float32 ends.  One exponential serves Q and the density.
+// for large z; for the slope e is kept finite, so e s tends to 1 and not to inf * 0.
+// gelu: with x = -|z| and Q = Phi(x), z Phi(z) = max(z, 0) + x Q, and act' is h = Q + x phi(x) for
+// z < 0, 1 - h else.  log2 Phi is smooth on [-6, 0]; Q is exp2 of a polynomial of degree 7
+// fitted to it here by iteratively reweighted least squares (6e-6 of the value in float32).
+// Below -6, where Q < 1e-9, x stays there.  13 instructions a pair instead of 22 with the
+// reciprocal form: they, not memory, bounded 64-channel frames.
 // Sums and products of pairs are one instruction each.
-template <int ACT, bool EXACT>
+template <int ACT, bool EXACT, bool SLOPE>
 __device__ __forceinline__ void activate(float2 z, float2& y, float2& d) {
   if constexpr (ACT == VI_ACT_RELU) {
     y = make_float2(z.x <= 0.0f ? 0.0f : z.x, z.y <= 0.0f ? 0.0f : z.y);
@@ -64,7 +70,8 @@ __device__ __forceinline__ void activate(float2 z, float2& y, float2& d) {
       s = make_float2(1.0f / (1.0f + e.x), 1.0f / (1.0f + e.y));
     } else {
       const float2 t = __fmul2_rn(z, pair(-kLog2e));
-      e = make_float2(exp2_fast(min_nan(t.x, 126.0f)), exp2_fast(min_nan(t.y, 126.0f)));
+      e = SLOPE ? make_float2(exp2_fast(min_nan(t.x, 126.0f)), exp2_fast(min_nan(t.y, 126.0f)))
+                : make_float2(exp2_fast(t.x), exp2_fast(t.y));
       const float2 q = __fadd2_rn(e, pair(1.0f));
       s = make_float2(rcp_fast(q.x), rcp_fast(q.y));
     }
@@ -83,22 +90,23 @@ __device__ __forceinline__ void activate(float2 z, float2& y, float2& d) {
       const float2 g = make_float2(expf(-0.5f * z.x * z.x), expf(-0.5f * z.y * z.y));
       d = __ffma2_rn(__fmul2_rn(z, pair(0.3989422804f)), g, cdf);
     } else {
-      const float2 x = make_float2(fminf(fabsf(z.x), 40.0f), fminf(fabsf(z.y), 40.0f));  // Q(40) is 0: no inf * 0
-      const float2 u = __ffma2_rn(x, pair(0.265f), pair(1.0f));
-      const float2 t = make_float2(rcp_fast(u.x), rcp_fast(u.y));
-      float2 r = __ffma2_rn(t, pair(-0.0677848929f), pair(0.195265483f));
-      r = __ffma2_rn(r, t, pair(-0.0663519581f));
-      r = __ffma2_rn(r, t, pair(0.142485184f));
-      r = __ffma2_rn(r, t, pair(0.0829498892f));
-      r = __ffma2_rn(r, t, pair(0.107836094f));
-      r = __ffma2_rn(r, t, pair(0.105599892f));
-      r = __fmul2_rn(r, t);
-      const float2 a = __fmul2_rn(__fmul2_rn(z, pair(-0.5f * kLog2e)), z);
-      const float2 g = make_float2(exp2_fast(a.x), exp2_fast(a.y)), q = __fmul2_rn(g, r);
-      const float2 top = make_float2(fmaxf(z.x, 0.0f), fmaxf(z.y, 0.0f));
-      y = __ffma2_rn(make_float2(-x.x, -x.y), q, top);
-      const float2 cdf = make_float2(z.x < 0.0f ? q.x : 1.0f - q.x, z.y < 0.0f ? q.y : 1.0f - q.y);
-      d = __ffma2_rn(__fmul2_rn(z, pair(0.3989422804f)), g, cdf);
+      const float2 x = make_float2(fmaxf(-fabsf(z.x), -6.0f), fmaxf(-fabsf(z.y), -6.0f));
+      float2 r = __ffma2_rn(x, pair(1.83482305e-06f), pair(6.1598517e-05f));
+      r = __ffma2_rn(r, x, pair(0.000930526497f));
+      r = __ffma2_rn(r, x, pair(0.00850789675f));
+      r = __ffma2_rn(r, x, pair(0.0539600791f));
+      r = __ffma2_rn(r, x, pair(-0.458464386f));
+      r = __ffma2_rn(r, x, pair(1.15125105f));
+      r = __ffma2_rn(r, x, pair(-0.999995295f));
+      const float2 q = make_float2(exp2_fast(r.x), exp2_fast(r.y));
+      y = __ffma2_rn(x, q, make_float2(max_nan(z.x, 0.0f), max_nan(z.y, 0.0f)));
+      if constexpr (SLOPE) {
+        const float2 a = __fmul2_rn(__fmul2_rn(x, pair(-0.5f * kLog2e)), x);
+        const float2 g = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+        const float2 h = __ffma2_rn(__fmul2_rn(x, pair(0.3989422804f)), g, q);
+        const float2 k = __ffma2_rn(h, pair(-1.0f), pair(1.0f));
+        d = make_float2(z.x > 0.0f ? k.x : h.x, z.y > 0.0f ? k.y : h.y);
+      }
     }
   } else {
     y = z;
