@@ -112,6 +112,7 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 // Waits for the phase of `parity` to end.  False when the block has given up (*dead) or
 // the limit ran out, which sets *dead.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead, uint32_t limit) {
+#pragma unroll 1
   for (uint32_t i = 0; i < limit; i++) {
     if (mbar_try(bar, parity)) return true;
     if ((i & 63) == 63 && *dead) return false;
@@ -281,6 +282,10 @@ struct Stage {
   static __device__ __forceinline__ uint32_t own(uint32_t st, int lane, int i) {
     return st + lane * kLine + ((uint32_t)(i << 4) ^ key(lane));
   }
+  // element j of a line
+  static __device__ __forceinline__ uint32_t cell(uint32_t st, int line, int j) {
+    return st + line * kLine + ((uint32_t)(j / kPer << 4) ^ key(line)) + j % kPer * (int)sizeof(Z);
+  }
   // the lane's piece of its line of step i
   static __device__ __forceinline__ uint32_t along(uint32_t st, int lane, int i) {
     const int line = lane / kLanes + i * kStep;
@@ -316,10 +321,10 @@ struct Place {
   int rows, cols;
 };
 
-// Loads a tile of v, 16 bytes a lane: along rows (kVector), along columns (kImage), to be
-// handed to their rows' lanes by own_row; or else each lane its row.  Returns the way.
+// Loads a tile of v, 16 bytes a lane: along rows (kVector), along columns (kImage), or else
+// element by element into the staging; own_row hands them to their rows' lanes.  Returns the way.
 template <typename Z>
-__device__ __forceinline__ int load_tile(Row<Z>& r, const View& v, int access, int lane, const Place& t) {
+__device__ __forceinline__ int load_tile(Row<Z>& r, const View& v, int access, uint32_t st, int lane, const Place& t) {
   using G = Stage<Z>;
   const Z* p = (const Z*)v.p;
   const int line = lane / G::kLanes, piece = lane % G::kLanes;
@@ -340,11 +345,12 @@ __device__ __forceinline__ int load_tile(Row<Z>& r, const View& v, int access, i
     }
     return kImage;
   }
+  // any strides, ragged ends: each lane its row, into the staging (rolled: the kernel's code has to stay small)
+  __syncwarp();
   if (lane < t.rows) {
-    const Z* q = p + (int64_t)(t.m0 + lane) * v.rs + (int64_t)t.n0 * v.cs;
-#pragma unroll
-    for (int j = 0; j < 32; j++, q += v.cs)
-      if (j < t.cols) r.z[j] = *q;
+    const typename Row<Z>::Bits* q = (const typename Row<Z>::Bits*)p + (int64_t)(t.m0 + lane) * v.rs + (int64_t)t.n0 * v.cs;
+#pragma unroll 1
+    for (int j = 0; j < t.cols; j++, q += v.cs) sts_cell(G::cell(st, lane, j), *q);
   }
   return kScalar;
 }
@@ -352,12 +358,13 @@ __device__ __forceinline__ int load_tile(Row<Z>& r, const View& v, int access, i
 template <typename Z>
 __device__ __forceinline__ void own_row(Row<Z>& r, int way, uint32_t st, int lane) {
   using G = Stage<Z>;
-  if (way == kScalar) return;
   __syncwarp();
-  if (way == kVector) {
+  if (way != kImage) {
+    if (way == kVector) {
 #pragma unroll
-    for (int i = 0; i < G::kLanes; i++) sts128(G::along(st, lane, i), r.q[i]);
-    __syncwarp();
+      for (int i = 0; i < G::kLanes; i++) sts128(G::along(st, lane, i), r.q[i]);
+      __syncwarp();
+    }
 #pragma unroll
     for (int i = 0; i < G::kLanes; i++) r.q[i] = lds128(G::own(st, lane, i));
   } else if constexpr (sizeof(Z) == 4) {  // staged as columns of 32 rows; neighbouring lanes read neighbouring elements
@@ -420,30 +427,28 @@ __device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int a
     }
     return;
   }
-  if (v.rs == 1 && v.cs != 1) {  // an image off 16 bytes, or its ragged end: lanes along the rows
-    if (lane < t.rows) {
-      Z* q = p + t.m0 + lane + (int64_t)t.n0 * v.cs;
-#pragma unroll
-      for (int j = 0; j < 32; j++, q += v.cs)
-        if (j < t.cols) *q = r.z[j];
-    }
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < G::kLanes; i++) sts128(G::own(st, lane, i), r.q[i]);
   __syncwarp();
+  typename Row<Z>::Bits* q = (typename Row<Z>::Bits*)p + (int64_t)t.m0 * v.rs + (int64_t)t.n0 * v.cs;
   if (access == kVector && t.cols >= 32) {
-    Z* q = p + (int64_t)(t.m0 + line) * v.rs + t.n0 + piece * G::kPer;
+    q += line * v.rs + piece * G::kPer;
     const int64_t step = G::kStep * v.rs;
 #pragma unroll
     for (int i = 0; i < G::kLanes; i++, q += step)
       if (line + i * G::kStep < t.rows) *(uint4*)q = lds128(G::along(st, lane, i));
+  } else if (v.rs == 1 && v.cs != 1) {  // an image off 16 bytes, or its ragged end: lanes along the rows
+    q += lane;
+    if (lane < t.rows) {
+#pragma unroll 1
+      for (int j = 0; j < t.cols; j++, q += v.cs) *q = lds_cell(G::cell(st, lane, j), typename Row<Z>::Bits());
+    }
   } else {  // a row at a time, each lane a column
-    typename Row<Z>::Bits* q = (typename Row<Z>::Bits*)p + (int64_t)t.m0 * v.rs + (int64_t)(t.n0 + lane) * v.cs;
-    for (int row = 0; row < min(32, t.rows); row++, q += v.rs)
-      if (lane < t.cols)
-        *q = lds_cell(st + row * G::kLine + ((uint32_t)(lane / G::kPer << 4) ^ G::key(row)) + lane % G::kPer * (int)sizeof(Z),
-                      typename Row<Z>::Bits());
+    q += lane * v.cs;
+    if (lane < t.cols) {
+#pragma unroll 1
+      for (int row = 0; row < t.rows; row++, q += v.rs) *q = lds_cell(G::cell(st, row, lane), typename Row<Z>::Bits());
+    }
   }
 }
 
@@ -503,13 +508,17 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
       uint32_t phase = 0;
       int64_t issued = 0;
       bool on = true;
+#pragma unroll 1
       for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
         const Item t = item_of<EPI>(a, i);
+#pragma unroll 1
         for (int nt = t.nt; nt < t.nt_end && on; nt++) {
+#pragma unroll 1
           for (int p = 0; p < a.pairs && on; p++) {
             // planes of the pair, smallest products first: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
             const int pa = a.pairs == 1 ? 0 : p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
             const int pb = a.pairs == 1 ? 0 : p == 2 ? 2 : p == 1 || p == 4 ? 1 : 0;
+#pragma unroll 1
             for (int kb = t.kb0; kb < t.kb1; kb++) {
               if (!mbar_wait(empty + 8 * stage, phase ^ 1, dead, a.spin_limit)) {
                 on = false;
@@ -556,9 +565,11 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool on = true;
+#pragma unroll 1
       for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
         const Item t = item_of<EPI>(a, i);
         const int steps = a.pairs * (t.kb1 - t.kb0);
+#pragma unroll 1
         for (int nt = t.nt; nt < t.nt_end && on; nt++) {
           if (!mbar_wait(tempty + 8 * acc, acc_phase ^ 1, dead, a.spin_limit)) {
             on = false;
@@ -566,6 +577,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
           }
           fence_after();
           const uint32_t d = tmem + acc * BN;
+#pragma unroll 1
           for (int s = 0; s < steps; s++) {
             if (!mbar_wait(full + 8 * stage, phase, dead, a.spin_limit)) {
               on = false;
@@ -602,6 +614,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
     int acc = 0;
     uint32_t acc_phase = 0;
     bool on = true;
+#pragma unroll 1
     for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
       const Item t = item_of<EPI>(a, i);
       const int m0 = t.mt * kBM + quad * 32, m = m0 + lane;
@@ -617,6 +630,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
       if (EPI == kEpiStore && e.alpha) alpha = *e.alpha;
       float row_bias = 0.0f;
       if (EPI == kEpiAct && e.bias_rows && m < a.M) row_bias = to_f(((const T*)e.bias)[m]);
+#pragma unroll 1
       for (int nt = t.nt; nt < t.nt_end; nt++) {
         // what the epilogue adds is asked for before the product is waited for
         constexpr bool kAdds = EPI == kEpiAct || EPI == kEpiPartial;
@@ -625,20 +639,22 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
         View add{nullptr, 0, 0};
         if (EPI == kEpiAct) add = e.res;
         if (EPI == kEpiPartial && e.add) add = View{e.part + (int64_t)t.split * a.M * a.N, a.N, 1};
-        Row<T> extra;
-        int way = kNone;
-        if (kAdds && add.p && col + first < a.N && m0 < a.M)
-          way = load_tile<T>(extra, add, EPI == kEpiAct ? res_access : access_of<T>(add), lane, place(col + first));
-        if (!mbar_wait(tfull + 8 * acc, acc_phase, dead, a.spin_limit)) on = false;
-        on = __all_sync(0xffffffffu, on);
-        if (!on) break;
-        fence_after();
+        bool waited = false;
+        auto wait_product = [&] {
+          if (!mbar_wait(tfull + 8 * acc, acc_phase, dead, a.spin_limit)) on = false;
+          on = __all_sync(0xffffffffu, on);
+          fence_after();
+          waited = true;
+        };
 #pragma unroll 1
         for (int c = first; c < BN && col + c < a.N && m0 < a.M; c += 32 * S::kParts) {
           const int n0 = col + c;
           const Place here = place(n0);
-          if (kAdds && add.p && c != first)
-            way = load_tile<T>(extra, add, EPI == kEpiAct ? res_access : access_of<T>(add), lane, here);
+          Row<T> extra;
+          int way = kNone;
+          if (kAdds && add.p) way = load_tile<T>(extra, add, EPI == kEpiAct ? res_access : access_of<T>(add), st, lane, here);
+          if (!waited) wait_product();
+          if (!on) break;
           const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + c;
           if (EPI != kEpiPartial && EPI != kEpiStore) {
             if (e.bias && !e.bias_rows && bias_at != n0) {  // a lane a column, then every lane all of them
@@ -773,6 +789,8 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
             }
           }
         }
+        if (!waited) wait_product();
+        if (!on) break;
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(tempty + 8 * acc);
