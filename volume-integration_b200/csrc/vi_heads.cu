@@ -22,10 +22,9 @@ namespace heads {
 namespace {
 
 // One operand laid out for the tensor cores: 16-bit planes, rows of `inner`
-// elements `ld` apart, a multiple of 8.  value = src (* slope) (0 in rows whose coef is 0).
+// elements `ld` apart, a multiple of 8; 0 in rows whose coef is 0.
 struct PackJob {
   View src;
-  View slope;         // act' beside it (float32, or the 16-bit code), p null = none
   const float* coef;  // [rows] or null
   int64_t rows, k;
   void* dst;
@@ -36,10 +35,62 @@ struct PackJobs {
   PackJob j[2];
 };
 
+// The 16-bit element type the tensor cores read for T.
 template <typename T>
-__device__ __forceinline__ float slope_at(const void* p, int64_t i) {
-  if constexpr (sizeof(T) == 4) return ((const float*)p)[i];
-  else return Slope<T>::unpack(((const uint16_t*)p)[i]);
+using Cell16 = typename std::conditional<std::is_same<T, __half>::value, __half, __nv_bfloat16>::type;
+
+// Eight elements `step` apart, n of them existing; 16 bytes at a time where they lie so.
+template <typename T>
+__device__ __forceinline__ void load8(const T* s, int64_t step, int n, float v[8]) {
+  if (step == 1 && n >= 8 && ((uintptr_t)s & 15) == 0) {
+    uint4 w[sizeof(T) / 2];
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; j++) w[j] = ((const uint4*)s)[j];
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = to_f(((const T*)w)[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = j < n ? to_f(s[j * step]) : 0.0f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load8_slope(const void* p, int64_t at, int64_t step, int n, float v[8]) {
+  if constexpr (sizeof(T) == 4) {
+    load8((const float*)p + at, step, n, v);
+  } else {
+    const uint16_t* s = (const uint16_t*)p + at;
+    uint4 w;
+    uint16_t* q = (uint16_t*)&w;
+    if (step == 1 && n >= 8 && ((uintptr_t)s & 15) == 0) {
+      w = *(const uint4*)s;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) q[j] = j < n ? s[j * step] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = Slope<T>::unpack(q[j]);
+  }
+}
+// Eight values as the tensor cores' elements, in one plane or three.
+template <typename T>
+__device__ __forceinline__ void store8(const float v[8], Cell16<T>* d, int64_t plane) {
+  if constexpr (sizeof(T) == 4) {
+    uint4 w[3];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      __nv_bfloat16 p[3];
+      split3(v[j], p);
+#pragma unroll
+      for (int pl = 0; pl < 3; pl++) ((__nv_bfloat16*)&w[pl])[j] = p[pl];
+    }
+#pragma unroll
+    for (int pl = 0; pl < 3; pl++) *(uint4*)(d + pl * plane) = w[pl];
+  } else {
+    uint4 w;
+#pragma unroll
+    for (int j = 0; j < 8; j++) ((Cell16<T>*)&w)[j] = from_f<Cell16<T>>(v[j]);
+    *(uint4*)d = w;
+  }
 }
 
 template <typename T>
@@ -49,99 +100,184 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJ
   const uint32_t chunks = (uint32_t)((inner + 7) / 8);
   const int64_t total = outer * chunks;
   const int64_t si = q.k_major ? q.src.cs : q.src.rs, so = q.k_major ? q.src.rs : q.src.cs;
-  const int64_t di = q.k_major ? q.slope.cs : q.slope.rs, dn = q.k_major ? q.slope.rs : q.slope.cs;
-  const T* src = (const T*)q.src.p;
-  using B16 = typename std::conditional<std::is_same<T, __half>::value, __half, __nv_bfloat16>::type;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t o = i / chunks, c = (i - o * chunks) * 8;
+    const int64_t o = i < INT32_MAX ? (uint32_t)i / chunks : i / chunks, c = (i - o * chunks) * 8;
+    const int n = (int)min((int64_t)8, inner - c);
     float v[8];
-    const T* s = src + o * so + c * si;
-    if (si == 1 && c + 8 <= inner && ((uintptr_t)s & 15) == 0) {
-      uint4 w[sizeof(T) / 2];
-#pragma unroll
-      for (int j = 0; j < (int)sizeof(T) / 2; j++) w[j] = ((const uint4*)s)[j];
-#pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = to_f(((const T*)w)[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = c + j < inner ? to_f(s[j * si]) : 0.0f;
-    }
-    if (q.slope.p) {
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (c + j < inner) v[j] *= slope_at<T>(q.slope.p, o * dn + (c + j) * di);
-    }
+    load8((const T*)q.src.p + o * so + c * si, si, n, v);
     if (q.coef) {
 #pragma unroll
       for (int j = 0; j < 8; j++)
-        if (c + j < inner && q.coef[q.k_major ? o : c + j] == 0.0f) v[j] = 0.0f;
+        if (j < n && q.coef[q.k_major ? o : c + j] == 0.0f) v[j] = 0.0f;
     }
-    B16* d = (B16*)q.dst + o * q.ld + c;
-    if constexpr (sizeof(T) == 4) {
-      uint4 w[3];
+    store8<T>(v, (Cell16<T>*)q.dst + o * q.ld + c, q.plane);
+  }
+}
+
+// s = src * slope (slope absent: src), laid out
+// for the tensor cores (dst null: not wanted) and its columns' sums over a piece of the
+// rows, part[piece][N] (null: not wanted): one pass over both.  Memory bounds it.
+struct Strip {
+  View src;
+  View slope;
+  int64_t M, N, rows;  // rows of a piece
+  void* dst;
+  int64_t ld, plane;
+  float* part;
+  bool padded;  // rows of src may be read up to their stride
+};
+
+template <typename T>
+__device__ __forceinline__ void strip8(const Strip& q, int64_t m, int64_t n, int64_t step_src, int64_t step_slope, int count,
+                                       float v[8]) {
+  load8((const T*)q.src.p + m * q.src.rs + n * q.src.cs, step_src, count, v);
+  if (q.slope.p) {
+    float w[8];
+    load8_slope<T>(q.slope.p, m * q.slope.rs + n * q.slope.cs, step_slope, count, w);
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        __nv_bfloat16 p[3];
-        split3(v[j], p);
+    for (int j = 0; j < 8; j++) v[j] *= w[j];
+  }
+}
+
+// Columns contiguous (or any strides): a thread takes 8 columns of every (256 / per)-th row.
+template <typename T>
+__global__ void __launch_bounds__(256) strip_rows_kernel(const __grid_constant__ Strip q, int per) {
+  __shared__ float sh[256 * 8];
+  const int tx = threadIdx.x % per, ty = threadIdx.x / per, step = 256 / per;
+  const int64_t n = ((int64_t)blockIdx.x * per + tx) * 8, m0 = (int64_t)blockIdx.y * q.rows, m1 = min(q.M, m0 + q.rows);
+  const int count = (int)min((int64_t)8, q.N - n);
+  float sum[8] = {};
+  const T* src = (const T*)q.src.p + n;
+  const typename std::conditional<sizeof(T) == 4, float, uint16_t>::type* slope = nullptr;
+  if (q.slope.p) slope = (decltype(slope))q.slope.p + n;
+  constexpr int kPer = 16 / (int)sizeof(T), kVec = (int)sizeof(T) / 2;  // elements a load, loads of 8 elements
+  const bool vec = (count == 8 || (count > 0 && q.padded)) && q.src.cs == 1 && q.src.rs % kPer == 0 && ((uintptr_t)src & 15) == 0 &&
+                   (!slope || (q.slope.cs == 1 && q.slope.rs % kPer == 0 && ((uintptr_t)slope & 15) == 0));
+  if (vec) {  // several rows' loads in flight before the first is used
+    constexpr int kRows = 4;
+    for (int64_t m = m0 + ty; m < m1; m += kRows * step) {
+      uint4 a[kRows][kVec], b[kRows][kVec];
 #pragma unroll
-        for (int pl = 0; pl < 3; pl++) ((__nv_bfloat16*)&w[pl])[j] = p[pl];
+      for (int i = 0; i < kRows; i++) {
+        const int64_t row = m + i * step;
+        if (row < m1) {
+#pragma unroll
+          for (int j = 0; j < kVec; j++) {
+            a[i][j] = __ldg((const uint4*)(src + row * q.src.rs) + j);
+            if (slope) b[i][j] = __ldg((const uint4*)(slope + row * q.slope.rs) + j);
+          }
+        }
       }
 #pragma unroll
-      for (int pl = 0; pl < 3; pl++) *(uint4*)(d + pl * q.plane) = w[pl];
-    } else {
-      uint4 w;
+      for (int i = 0; i < kRows; i++) {
+        const int64_t row = m + i * step;
+        if (row < m1) {
+          float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; j++) ((B16*)&w)[j] = from_f<B16>(v[j]);
-      *(uint4*)d = w;
+          for (int j = 0; j < 8; j++) {
+            v[j] = to_f(((const T*)a[i])[j]);
+            if (slope) {
+              if constexpr (sizeof(T) == 4) v[j] *= ((const float*)b[i])[j];
+              else v[j] *= Slope<T>::unpack(((const uint16_t*)b[i])[j]);
+            }
+          }
+          if (q.dst) store8<T>(v, (Cell16<T>*)q.dst + row * q.ld + n, q.plane);
+#pragma unroll
+          for (int j = 0; j < 8; j++) sum[j] += v[j];
+        }
+      }
+    }
+  } else if (count > 0) {
+    for (int64_t m = m0 + ty; m < m1; m += step) {
+      float v[8];
+      strip8<T>(q, m, n, q.src.cs, q.slope.cs, count, v);
+      if (q.dst) store8<T>(v, (Cell16<T>*)q.dst + m * q.ld + n, q.plane);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum[j] += v[j];
     }
   }
-}
-
-// part[piece][n] = sum of column n of src * slope over the piece's rows.
-template <typename T>
-__global__ void __launch_bounds__(256) column_sums_kernel(View src, View slope, int64_t M, int64_t N, int64_t rows,
-                                                          float* part) {
-  __shared__ float sh[8][33];
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
-  const int64_t m0 = blockIdx.y * rows, m_end = min(M, m0 + rows);
-  auto value = [&](int64_t m, int64_t n) {
-    const float v = to_f(((const T*)src.p)[m * src.rs + n * src.cs]);
-    return slope.p ? v * slope_at<T>(slope.p, m * slope.rs + n * slope.cs) : v;
-  };
-  if (src.rs == 1 && src.cs != 1) {  // rows contiguous: a warp runs along a column
-    for (int c = w; c < 32; c += 8) {
-      const int64_t n = (int64_t)blockIdx.x * 32 + c;
-      float sum = 0.0f;
-      if (n < N)
-        for (int64_t m = m0 + lane; m < m_end; m += 32) sum += value(m, n);
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0 && n < N) part[(int64_t)blockIdx.y * N + n] = sum;
-    }
-    return;
-  }
-  const int64_t n = (int64_t)blockIdx.x * 32 + lane;
-  float sum = 0.0f;
-  if (n < N)
-    for (int64_t m = m0 + w; m < m_end; m += 8) sum += value(m, n);
-  sh[w][lane] = sum;
+  if (!q.part) return;
+#pragma unroll
+  for (int j = 0; j < 8; j++) sh[(ty * per + tx) * 8 + j] = sum[j];
   __syncthreads();
-  if (w == 0 && n < N) {
-    for (int i = 1; i < 8; i++) sum += sh[i][lane];
-    part[(int64_t)blockIdx.y * N + n] = sum;
+  for (int i = threadIdx.x; i < per * 8; i += 256) {
+    float a = 0.0f;
+    for (int y = 0; y < step; y++) a += sh[y * per * 8 + i];
+    const int64_t col = (int64_t)blockIdx.x * per * 8 + i;
+    if (col < q.N) q.part[(int64_t)blockIdx.y * q.N + col] = a;
   }
 }
 
-// out(i / cols, i % cols) = alpha * sum of the pieces, added in order.
+// Rows contiguous (an image): a block takes a piece of one column after another.
 template <typename T>
-__global__ void sum_pieces_kernel(const float* part, int pieces, int64_t rows, int64_t cols, const float* alpha,
-                                  View out) {
-  const int64_t total = rows * cols;
-  const bool by_col = out.cs == 1;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = by_col ? i / cols : i % rows, c = by_col ? i % cols : i / rows;
+__global__ void __launch_bounds__(256) strip_image_kernel(const __grid_constant__ Strip q) {
+  __shared__ float sh[8];
+  const int64_t m0 = (int64_t)blockIdx.x * q.rows, m1 = min(q.M, m0 + q.rows);
+  for (int64_t n = blockIdx.y; n < q.N; n += gridDim.y) {
     float sum = 0.0f;
-    for (int p = 0; p < pieces; p++) sum += part[(int64_t)p * total + r * cols + c];
-    ((T*)out.p)[r * out.rs + c * out.cs] = from_f<T>(sum * (alpha ? *alpha : 1.0f));
+#pragma unroll 2
+    for (int64_t m = m0 + threadIdx.x * 8; m < m1; m += 2048) {
+      const int count = (int)min((int64_t)8, m1 - m);
+      float v[8];
+      strip8<T>(q, m, n, q.src.rs, q.slope.rs, count, v);
+      if (q.dst) store8<T>(v, (Cell16<T>*)q.dst + n * q.ld + m, q.plane);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum += v[j];
+    }
+    if (!q.part) continue;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 8; i++) sum += sh[i];
+      q.part[(int64_t)blockIdx.x * q.N + n] = sum;
+    }
+  }
+}
+
+// out(r, c) = alpha * sum of the pieces' elements (r, c), added in a fixed order.  Up to two jobs a launch.
+struct SumJob {
+  const float* part;
+  int pieces;
+  int64_t piece;     // elements from one piece to the next
+  int64_t prs, pcs;  // strides of an element in its piece
+  int64_t rows, cols;
+  const float* alpha;
+  View out;
+};
+struct SumJobs {
+  SumJob j[2];
+};
+
+// SPLIT threads share an element's pieces: 1 for few pieces, 8 (a block is 32 elements x 8) for many.
+template <typename T, int SPLIT>
+__global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumJobs jobs) {
+  __shared__ float sh[8][33];
+  const SumJob& q = jobs.j[blockIdx.y];
+  const int64_t total = q.rows * q.cols;
+  const bool by_col = q.out.cs == 1;
+  const uint32_t run = (uint32_t)(by_col ? q.cols : q.rows);
+  const float alpha = q.alpha ? *q.alpha : 1.0f;
+  const int lane = threadIdx.x % (256 / SPLIT), w = threadIdx.x / (256 / SPLIT);
+  for (int64_t base = (int64_t)blockIdx.x * (256 / SPLIT); base < total; base += (int64_t)gridDim.x * (256 / SPLIT)) {
+    const int64_t i = base + lane;
+    const int64_t hi = i < INT32_MAX ? (uint32_t)i / run : i / run, lo = i - hi * run;
+    const int64_t r = by_col ? hi : lo, c = by_col ? lo : hi;
+    float sum = 0.0f;
+    if (i < total) {
+      const float* p = q.part + r * q.prs + c * q.pcs;
+#pragma unroll 4
+      for (int k = w; k < q.pieces; k += SPLIT) sum += p[k * q.piece];
+    }
+    if (SPLIT > 1) {
+      sh[w][lane] = sum;
+      __syncthreads();
+      if (w == 0)
+        for (int k = 1; k < SPLIT; k++) sum += sh[k][lane];
+      __syncthreads();
+    }
+    if (w == 0 && i < total) ((T*)q.out.p)[r * q.out.rs + c * q.out.cs] = from_f<T>(sum * alpha);
   }
 }
 
@@ -293,7 +429,6 @@ struct Run {
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int grid_for(int64_t n) { return (int)std::min<int64_t>(ceil_div(n, 256), 148 * 16); }
 size_t elem(int dtype) { return dtype == VI_F32 ? 4 : 2; }
 View view(const vi_matrix* m) { return m ? View{m->data, m->row_stride, m->col_stride} : View{nullptr, 0, 0}; }
 View transposed(View v) { return View{v.p, v.cs, v.rs}; }
@@ -332,13 +467,13 @@ struct Packer {
   PackJobs jobs{};
   int n = 0;
   int64_t chunks = 0;
-  Operand add(const View& v, int64_t rows, int64_t k, const View& slope = {}, const float* coef = nullptr) {
+  Operand add(const View& v, int64_t rows, int64_t k, const float* coef = nullptr) {
     const bool k_major = v.cs == 1 || v.rs != 1;
-    if (!slope.p && !coef && direct(dtype, v, rows, k)) return Operand{v.p, rows, k, k_major ? v.rs : v.cs, 0, k_major};
+    if (!coef && direct(dtype, v, rows, k)) return Operand{v.p, rows, k, k_major ? v.rs : v.cs, 0, k_major};
     const int64_t inner = k_major ? k : rows, outer = k_major ? rows : k;
     const int64_t ld = ceil_div(inner, 8) * 8, plane = ld * outer;
     void* dst = r.take((size_t)plane * 2 * (dtype == VI_F32 ? 3 : 1));
-    jobs.j[n++] = PackJob{v, slope, coef, rows, k, dst, ld, plane, k_major};
+    jobs.j[n++] = PackJob{v, coef, rows, k, dst, ld, plane, k_major};
     chunks = std::max(chunks, outer * (ld / 8));
     if (n == 2) run();
     return Operand{dst, rows, k, ld, plane, k_major};
@@ -403,55 +538,82 @@ Plan split_plan(const Operand& A, const Operand& B, int sms) {
   return p;
 }
 
-// out = alpha * A B^T; a long sum with few tiles in pieces, in float32, added in order.
-int gemm_out(Run& r, int dtype, const Operand& A, const Operand& B, const float* alpha, const View& out) {
+// Sums of pieces that wait for their launch; their part buffers stay taken until then.
+struct Summer {
+  Run& r;
+  int dtype;
+  SumJobs jobs{};
+  int n = 0, pieces = 0;
+  int64_t total = 0;
+  void add(const SumJob& j) {
+    if (n == 2) run();
+    jobs.j[n++] = j;
+    pieces = std::max(pieces, j.pieces);
+    total = std::max(total, j.rows * j.cols);
+  }
+  void run() {
+    if (n && !r.dry) {
+      if (pieces > 8) {
+        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(total, 32), 148 * 16), n);
+        VI_DISPATCH(dtype, (sum_kernel<T, 8><<<grid, 256, 0, r.s>>>(jobs)));
+      } else {
+        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(total, 256), 148 * 16), n);
+        VI_DISPATCH(dtype, (sum_kernel<T, 1><<<grid, 256, 0, r.s>>>(jobs)));
+      }
+      r.launches++;
+    }
+    n = pieces = 0;
+    total = 0;
+  }
+};
+
+// out = alpha * A B^T; a long sum with few tiles in pieces, in float32, added in order (by `sums`).
+int gemm_out(Run& r, Summer& sums, const Operand& A, const Operand& B, const float* alpha, const View& out) {
   const Plan p = split_plan(A, B, r.sms);
   Epilogue e{};
   if (p.splits == 1) {
     e.out = out;
     e.alpha = alpha;
-    return gemm(r, dtype, kEpiStore, A, B, e);
+    return gemm(r, sums.dtype, kEpiStore, A, B, e);
   }
-  const size_t mark = r.cur;
   e.part = (float*)r.take((size_t)p.splits * A.rows * B.rows * 4);
-  r.release(mark);
-  if (r.dry) return VI_OK;
-  if (int rc = launch_gemm(dtype, kEpiPartial, A, B, p, e, r.sms, r.s)) return rc;
-  VI_DISPATCH(dtype, (sum_pieces_kernel<T><<<grid_for(A.rows * B.rows), 256, 0, r.s>>>(e.part, p.splits, A.rows, B.rows, alpha, out)));
-  r.launches++;
-  return VI_OK;
+  sums.add(SumJob{e.part, p.splits, A.rows * B.rows, B.rows, 1, A.rows, B.rows, alpha, out});
+  return r.dry ? VI_OK : launch_gemm(sums.dtype, kEpiPartial, A, B, p, e, r.sms, r.s);
 }
 
-// out[n] = alpha * sum over rows of src * slope.  planes: src is that many 16-bit matrices to add.
-void column_sums(Run& r, int dtype, const View& src, const View& slope, int planes, int64_t plane, int64_t M,
-                 int64_t N, const float* alpha, int out_dtype, void* out) {
-  const int64_t blocks = ceil_div(N, 32);
-  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(ceil_div(148 * 8, blocks), ceil_div(M, 64)));
-  const int64_t rows = ceil_div(M, pieces);
-  const size_t mark = r.cur;
-  float* part = (float*)r.take((size_t)planes * pieces * N * 4);
-  r.release(mark);
-  if (r.dry) return;
-  const dim3 grid((unsigned)blocks, (unsigned)pieces);
-  for (int pl = 0; pl < planes; pl++) {
-    const View v{(char*)src.p + pl * plane * 2, src.rs, src.cs};
-    VI_DISPATCH(dtype, (column_sums_kernel<T><<<grid, 256, 0, r.s>>>(planes > 1 ? v : src, slope, M, N, rows, part + pl * pieces * N)));
+// One pass over src * slope: laid out in dst (null: no), its columns' sums in `sums` (db null: no).
+void strip(Run& r, Summer& sums, int dtype, Strip q, const float* alpha, void* db) {
+  const bool image = q.src.rs == 1 && q.src.cs != 1;
+  int per = 256;  // threads along a row: long runs of it, so that DRAM pages are read whole
+  while (per > 1 && (per / 2) * 8 >= q.N) per /= 2;
+  const int64_t blocks = image ? std::min<int64_t>(q.N, 1024) : ceil_div(q.N, per * 8);
+  // enough pieces of the rows to fill the SMs, each long enough to be worth its sum
+  const int64_t least = image ? 8192 : 256 / per * 8;
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(ceil_div(r.sms * 8, blocks), q.M / least));
+  q.rows = ceil_div(ceil_div(q.M, pieces), 8) * 8;
+  const int64_t count = ceil_div(q.M, q.rows);
+  q.part = nullptr;
+  if (db) {
+    q.part = (float*)r.take((size_t)count * q.N * 4);
+    sums.add(SumJob{q.part, (int)count, q.N, 0, 1, 1, q.N, alpha, View{db, 0, 1}});
   }
-  VI_DISPATCH(out_dtype, (sum_pieces_kernel<T><<<grid_for(N), 256, 0, r.s>>>(part, (int)(pieces * planes), 1, N, alpha, View{out, 0, 1})));
-  r.launches += planes + 1;
+  if (r.dry) return;
+  if (image) {
+    const dim3 grid((unsigned)count, (unsigned)blocks);
+    VI_DISPATCH(dtype, (strip_image_kernel<T><<<grid, 256, 0, r.s>>>(q)));
+  } else {
+    const dim3 grid((unsigned)blocks, (unsigned)count);
+    VI_DISPATCH(dtype, (strip_rows_kernel<T><<<grid, 256, 0, r.s>>>(q, per)));
+  }
+  r.launches++;
 }
 
 // Gradients of the weights over no rows at all.
 void zero_gradients(Run& r, int dtype, int64_t N, int64_t K, const vi_matrix* dw, void* db) {
-  if (r.dry) return;
-  if (dw && dw->data) {
-    VI_DISPATCH(dtype, (sum_pieces_kernel<T><<<grid_for(N * K), 256, 0, r.s>>>(nullptr, 0, N, K, nullptr, view(dw))));
-    r.launches++;
-  }
-  if (db) {
-    VI_DISPATCH(dtype, (sum_pieces_kernel<T><<<grid_for(N), 256, 0, r.s>>>(nullptr, 0, 1, N, nullptr, View{db, 0, 1})));
-    r.launches++;
-  }
+  Summer sums{r, dtype};
+  if (dw && dw->data) sums.add(SumJob{nullptr, 0, 0, 0, 0, N, K, nullptr, view(dw)});
+  if (db) sums.add(SumJob{nullptr, 0, 0, 0, 0, 1, N, nullptr, View{db, 0, 1}});
+  sums.run();
 }
 
 // ---- argument checks ----
@@ -554,19 +716,33 @@ int act_backward(Run& r, int dtype, const vi_matrix* dy, const vi_matrix* dact, 
   }
   const View slope = view(dact);
   const bool need_dx = dx && dx->data, need_dw = dw && dw->data;
+  Summer sums{r, dtype};
   Packer pk{r, dtype};
+  Operand S{}, W{}, X{};
+  if (need_dx) W = pk.add(view(w), N, K);
+  if (need_dw) X = pk.add(view(x), M, K);
+  pk.run();
+  // s = dy * act', where dy itself does not serve; the bias's gradient in the same pass
+  const View d = view(dy);
+  const bool in_place = !slope.p && direct(dtype, d, M, N);
+  Strip q{d, slope, M, N};
   if (need_dx || need_dw) {
-    const Operand S = pk.add(view(dy), M, N, slope);
-    Operand W{}, X{};
-    if (need_dx) W = pk.add(view(w), N, K);
-    if (need_dw) X = pk.add(view(x), M, K);
-    pk.run();
-    if (need_dx)
-      if (int rc = gemm_out(r, dtype, S, transposed(W), nullptr, view(dx))) return rc;
-    if (need_dw)
-      if (int rc = gemm_out(r, dtype, transposed(S), transposed(X), nullptr, view(dw))) return rc;
+    const bool k_major = d.cs == 1 || d.rs != 1;
+    if (in_place) {
+      S = Operand{d.p, M, N, k_major ? d.rs : d.cs, 0, k_major};
+    } else {
+      q.ld = ceil_div(k_major ? N : M, 8) * 8;
+      q.plane = q.ld * (k_major ? M : N);
+      q.dst = r.take((size_t)q.plane * 2 * (dtype == VI_F32 ? 3 : 1));
+      S = Operand{q.dst, M, N, q.ld, q.plane, k_major};
+    }
   }
-  if (db) column_sums(r, dtype, view(dy), slope, 1, 0, M, N, nullptr, dtype, db);
+  if (q.dst || db) strip(r, sums, dtype, q, nullptr, db);
+  if (need_dx)
+    if (int rc = gemm_out(r, sums, S, transposed(W), nullptr, view(dx))) return rc;
+  if (need_dw)
+    if (int rc = gemm_out(r, sums, transposed(S), transposed(X), nullptr, view(dw))) return rc;
+  sums.run();
   return VI_OK;
 }
 
@@ -651,7 +827,7 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
   // x without the rows of ignored targets: their zero gradient times a NaN or an
   // infinity would else reach the weights' gradient
   Packer pk{r, dtype};
-  const Operand X = pk.add(view(x), M, K, {}, need_dw ? coef : nullptr), W = pk.add(view(w), V, K);
+  const Operand X = pk.add(view(x), M, K, need_dw ? coef : nullptr), W = pk.add(view(w), V, K);
   pk.run();
 
   // G in pieces of the vocabulary
@@ -669,6 +845,7 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
   for (int64_t c = 0; c < V; c += piece) {
     const int64_t n = std::min(piece, V - c);
     r.release(mark);
+    Summer sums{r, dtype};
     Operand Wc = W;
     Wc.rows = n;
     Wc.p = (const char*)W.p + c * (W.k_major ? W.ld : 1) * 2;
@@ -693,25 +870,29 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
         p.splits = (int)ceil_div(ceil_div(n, 64), p.kps);
         if (!r.dry)
           if (int rc = launch_gemm(dtype, kEpiPartial, G, transposed(Wc), p, d, r.sms, r.s)) return rc;
-      } else if (int rc = gemm_out(r, dtype, G, transposed(Wc), alpha, view(dx))) {
+      } else if (int rc = gemm_out(r, sums, G, transposed(Wc), alpha, view(dx))) {
         return rc;
       }
     }
     if (need_dw) {
       View out = view(dw);
       out.p = (char*)out.p + c * out.rs * elem(dtype);
-      if (int rc = gemm_out(r, dtype, transposed(G), transposed(X), alpha, out)) return rc;
+      if (int rc = gemm_out(r, sums, transposed(G), transposed(X), alpha, out)) return rc;
     }
-    if (db)
-      column_sums(r, dtype == VI_F16 ? VI_F16 : VI_BF16, View{grad, ld, 1}, View{}, planes, M * ld, M, n, alpha, dtype,
-                  (char*)db + c * elem(dtype));
+    if (db) {
+      Strip q{View{grad, ld, 1}, View{nullptr, 0, 0}, M * planes, n};  // the planes' rows one after another
+      q.padded = true;
+      strip(r, sums, dtype == VI_F16 ? VI_F16 : VI_BF16, q, alpha, (char*)db + c * elem(dtype));
+    }
+    sums.run();
     if (r.dry && c + piece < V) {  // the last piece alone may be smaller: one more round counts it
       c = (V - 1) / piece * piece - piece;
     }
   }
-  if (need_dx && several && !r.dry) {
-    VI_DISPATCH(dtype, (sum_pieces_kernel<T><<<grid_for(M * K), 256, 0, r.s>>>(acc, px.splits, M, K, alpha, view(dx))));
-    r.launches++;
+  if (need_dx && several) {
+    Summer sums{r, dtype};
+    sums.add(SumJob{acc, px.splits, M * K, K, 1, M, K, alpha, view(dx)});
+    sums.run();
   }
   return VI_OK;
 }
