@@ -336,7 +336,7 @@ typedef struct vi_matrix {
  * NULL), residual [M,N] (or NULL), y [M,N] with one of its strides 1 and rows
  * or columns that do not overlap.  dact (or NULL; same shape and strides as y)
  * receives act'(x weight^T + bias) in a form of its own for the backward
- * (float32, else a 16-bit code), which needs it unless the activation is VI_ACT_NONE.  K and N are at least 1, M may be 0.
+ * (float32, else a 16-bit code); see vi_linear_act_keeps_dact.  K and N are at least 1, M may be 0.
  */
 uint64_t vi_linear_act_forward_scratch_bytes(int dtype, int activation, const vi_matrix* x, const vi_matrix* weight,
                                              const void* bias, const vi_matrix* residual, const vi_matrix* y,
@@ -345,18 +345,23 @@ int vi_linear_act_forward(int dtype, int activation, const vi_matrix* x, const v
                           const vi_matrix* residual, const vi_matrix* y, const vi_matrix* dact, void* scratch,
                           uint64_t scratch_bytes, void* stream);
 
+/* Whether a forward should be asked for dact when a backward will follow: 0 where the backward finds act'
+ * again from x (images of few channels; no activation) more cheaply than it reads it. */
+int vi_linear_act_keeps_dact(int dtype, int activation, const vi_matrix* x, const vi_matrix* weight);
+
 /*
  * Gradients of vi_linear_act_forward for an incoming dy [M,N] (any strides):
- * with s = dy * dact (dact NULL: s = dy), dx = s weight, dweight = s^T x, dbias
- * = the column sums of s.  Each of dx, dweight, dbias may be NULL; dx and
- * dweight have one of their strides 1.  The residual's gradient is dy itself.
+ * with s = dy * act', dx = s weight, dweight = s^T x, dbias = the column sums of
+ * s.  dact is the forward's; NULL: act' is computed again from x, weight and
+ * bias (which is read for nothing else).  Each of dx, dweight, dbias may be NULL; dx
+ * and dweight have one of their strides 1.  The residual's gradient is dy itself.
  */
-uint64_t vi_linear_act_backward_scratch_bytes(int dtype, const vi_matrix* dy, const vi_matrix* dact,
-                                              const vi_matrix* x, const vi_matrix* weight, const vi_matrix* dx,
-                                              const vi_matrix* dweight, const void* dbias);
-int vi_linear_act_backward(int dtype, const vi_matrix* dy, const vi_matrix* dact, const vi_matrix* x,
-                           const vi_matrix* weight, const vi_matrix* dx, const vi_matrix* dweight, void* dbias,
-                           void* scratch, uint64_t scratch_bytes, void* stream);
+uint64_t vi_linear_act_backward_scratch_bytes(int dtype, int activation, const vi_matrix* dy, const vi_matrix* dact,
+                                              const vi_matrix* x, const vi_matrix* weight, const void* bias,
+                                              const vi_matrix* dx, const vi_matrix* dweight, const void* dbias);
+int vi_linear_act_backward(int dtype, int activation, const vi_matrix* dy, const vi_matrix* dact, const vi_matrix* x,
+                           const vi_matrix* weight, const void* bias, const vi_matrix* dx, const vi_matrix* dweight,
+                           void* dbias, void* scratch, uint64_t scratch_bytes, void* stream);
 
 /*
  * Softmax cross entropy of the logits z = x weight^T + bias, which are never

@@ -25,8 +25,9 @@ def load():
     fwd = [i, i, m, m, vp, m, m, m]
     lib.vi_linear_act_forward_scratch_bytes.argtypes = fwd
     lib.vi_linear_act_forward.argtypes = fwd + [vp, u64, vp]
-    bwd = [i, m, m, m, m, m, m, vp]
+    bwd = [i, i, m, m, m, m, vp, m, m, vp]
     lib.vi_linear_act_backward_scratch_bytes.argtypes = bwd
+    lib.vi_linear_act_keeps_dact.argtypes = [i, i, m, m]
     lib.vi_linear_act_backward.argtypes = bwd + [vp, u64, vp]
     lib.vi_linear_ce_forward_scratch_bytes.argtypes = [i, m, m, vp]
     lib.vi_linear_ce_forward.argtypes = [i, m, m, vp, vp, i64, i, vp, vp, vp, u64, vp]

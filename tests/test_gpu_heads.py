@@ -81,6 +81,45 @@ def test_linear_act_every_activation(act, dt):
     _act_check(*_act_inputs(200, 48, 72, dt, "rows", True, True, 3), act)
 
 
+@pytest.mark.parametrize("dt", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M,K,N,act,order,residual,dy_order", [
+    (1031, 3, 300, "gelu", "image", True, "image"),      # more channels than one backward pass keeps
+    (2052, 7, 256, "silu", "image", False, "image"),
+    (517, 5, 20, "sigmoid", "image-odd", True, "image-odd"),
+    (4096, 4, 64, "relu", "image", False, "rows"),       # the gradient comes in the other order
+    (3, 2, 9, "gelu", "image", True, "image"),
+    (700, 8, 130, "none", "image", True, "image"),
+    (900, 9, 40, "silu", "image", False, "image"),       # one channel too many for the narrow path
+    (20001, 4, 16, "gelu", "image", False, "image"),
+])
+def test_linear_act_images_of_few_channels(M, K, N, act, order, residual, dy_order, dt):
+    x, w, b, r, _ = _act_inputs(M, K, N, dt, order, True, residual, M + N)
+    dy = hl.matrix(M, N, dt, _gen(M), dy_order)
+    y = _act_check(x, w, b, r, dy, act)
+    assert y.t().is_contiguous() or order != "image"
+
+
+def test_backward_without_the_kept_derivative():
+    # a C ABI caller that kept no act': it is computed again from x, weight and bias
+    import ctypes
+    import heads_abi as ha
+    lib = ha.load()
+    p = ctypes.c_void_p
+    for dt, order in ((BF16, "rows"), (F32, "odd"), (F16, "image")):
+        x, w, b, _, dy = _act_inputs(300, 40, 70, dt, order, True, False, 41)
+        dx, dw, db = torch.empty(300, 40, device="cuda", dtype=dt), torch.empty_like(w), torch.empty_like(b)
+        args = (ha.DTYPE[dt], 2, ha.matrix(dy), None, ha.matrix(x), ha.matrix(w), p(b.data_ptr()), ha.matrix(dx),
+                ha.matrix(dw), p(db.data_ptr()))
+        n = lib.vi_linear_act_backward_scratch_bytes(*args)
+        assert n > 0, lib.vi_last_error()
+        scratch = torch.empty(n, device="cuda", dtype=torch.uint8)
+        rc = lib.vi_linear_act_backward(*args, p(scratch.data_ptr()), n, p(torch.cuda.current_stream().cuda_stream))
+        assert rc == 0, lib.vi_last_error()
+        want = hl.linear_act(x, w, b, None, "silu", dy)
+        for name, got, ref in (("dx", dx, want[1]), ("dweight", dw, want[2]), ("dbias", db, want[3])):
+            hl.assert_within(name, got, ref)
+
+
 @pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
 def test_linear_act_memory_order_of_the_result(dt):
     import volume_integration.heads as heads

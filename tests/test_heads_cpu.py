@@ -74,8 +74,13 @@ def test_c_abi_refusals():
     assert lib.vi_linear_ce_backward(*args, None, n, None) == 1 and b"scratch" in lib.vi_last_error()
     assert lib.vi_linear_ce_forward(2, x, w, None, p(256), -100, 5, p(256), p(256), p(256), 1 << 20, None) == 1
     assert b"reduction" in lib.vi_last_error()
-    assert lib.vi_linear_act_backward_scratch_bytes(2, _m(6, 4, 4, 1), None, x, w, None, None, None) == 0
-    assert lib.vi_linear_act_backward_scratch_bytes(2, y, None, x, w, _m(6, 5, 5, 1), None, None) == 0
+    assert lib.vi_linear_act_backward_scratch_bytes(2, 1, _m(6, 4, 4, 1), None, x, w, None, None, None, None) == 0
+    assert lib.vi_linear_act_backward_scratch_bytes(2, 1, y, None, x, w, None, _m(6, 5, 5, 1), None, None) == 0
+    assert lib.vi_linear_act_backward_scratch_bytes(2, 7, y, None, x, w, None, None, None, None) == 0
+    # act' is kept, but for no activation and for images of few channels
+    image, wide = _m(600, 4, 1, 600), _m(600, 9, 1, 600)
+    assert [lib.vi_linear_act_keeps_dact(2, a, v, u) for a, v, u in (
+        (1, x, w), (0, x, w), (1, image, w), (1, wide, _m(5, 9, 9, 1)), (1, image, _m(300, 4, 4, 1)))] == [1, 0, 0, 1, 1]
     assert lib.vi_linear_ce_backward_scratch_bytes(2, x, w, None, None, _m(5, 4, 2, 1), None) == 0
 
 
@@ -97,7 +102,7 @@ def test_scratch_covers_every_layout_step():
         assert f(dt, 0, odd, w, None, None, y, None) >= M * K * es
         assert f(dt, 0, _m(M, K, K, 1, 264), w, None, None, y, None) >= M * K * es
         b = lib.vi_linear_act_backward_scratch_bytes
-        assert b(dt, y, y, x, w, dx, dw, None) >= M * V * es
+        assert b(dt, 1, y, y, x, w, None, dx, dw, None) >= M * V * es
 
 
 @pytest.mark.parametrize("act", hl.ACTS)

@@ -416,7 +416,7 @@ Tensor head_scratch(uint64_t bytes, const Tensor& x) {
 std::tuple<Tensor, c10::optional<Tensor>> linear_act_forward(const Tensor& x, const Tensor& weight,
                                                              const c10::optional<Tensor>& bias,
                                                              const c10::optional<Tensor>& residual, int64_t activation,
-                                                             bool want_dact) {
+                                                             bool backward_follows) {
   head_check(x, weight);
   const at::cuda::OptionalCUDAGuard guard(x.device());
   const int dt = head_dtype(x, "x");
@@ -426,6 +426,7 @@ std::tuple<Tensor, c10::optional<Tensor>> linear_act_forward(const Tensor& x, co
   Tensor y = head_result(x, x.size(0), weight.size(0));
   c10::optional<Tensor> dact;
   vi_matrix my = head_matrix(y), md{};
+  const bool want_dact = backward_follows && vi_linear_act_keeps_dact(dt, (int)activation, &mx, &mw);
   if (want_dact) {
     dact = torch::empty_like(y);
     md = head_matrix(*dact);
@@ -456,19 +457,21 @@ struct GradTensors {
 
 // (dx, dweight, dbias), None where not wanted
 Grads linear_act_backward(const Tensor& dy, const c10::optional<Tensor>& dact, const Tensor& x, const Tensor& weight,
-                          bool need_x, bool need_w, bool need_b) {
+                          const c10::optional<Tensor>& bias, int64_t activation, bool need_x, bool need_w, bool need_b) {
   head_check(x, weight);
   head_like(dy, x, "dy");
   TORCH_CHECK(dy.dim() == 2, "dy must be 2D");
   const at::cuda::OptionalCUDAGuard guard(x.device());
   const int dt = head_dtype(x, "x");
+  const Tensor b = head_bias(bias, x, weight);
   const OptMatrix d(dact, x, "dact");
   const vi_matrix mdy = head_matrix(dy), mx = head_matrix(x), mw = head_matrix(weight);
   GradTensors g(x, weight, need_x, need_w, need_b);
-  const uint64_t n = vi_linear_act_backward_scratch_bytes(dt, &mdy, d.get(), &mx, &mw, g.x(), g.w(), g.b());
+  const uint64_t n = vi_linear_act_backward_scratch_bytes(dt, (int)activation, &mdy, d.get(), &mx, &mw, head_ptr(b),
+                                                          g.x(), g.w(), g.b());
   Tensor scratch = head_scratch(n, x);
-  ok(vi_linear_act_backward(dt, &mdy, d.get(), &mx, &mw, g.x(), g.w(), g.b(), scratch.data_ptr(), n,
-                            at::cuda::getCurrentCUDAStream().stream()));
+  ok(vi_linear_act_backward(dt, (int)activation, &mdy, d.get(), &mx, &mw, head_ptr(b), g.x(), g.w(), g.b(),
+                            scratch.data_ptr(), n, at::cuda::getCurrentCUDAStream().stream()));
   return {g.dx, g.dw, g.db};
 }
 

@@ -408,7 +408,7 @@ int sm_count() {
 }
 
 // Bytes of the logits' gradient that exist at a time, if 256 columns fit.
-constexpr int64_t kPieceBytes = 256ll << 20;
+constexpr int64_t kPieceBytes = 512ll << 20;
 
 struct Run {
   char* base;
@@ -431,6 +431,10 @@ struct Run {
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t elem(int dtype) { return dtype == VI_F32 ? 4 : 2; }
 View view(const vi_matrix* m) { return m ? View{m->data, m->row_stride, m->col_stride} : View{nullptr, 0, 0}; }
+// A [rows, cols] scratch matrix in the memory order of `like`.
+View scratch_like(void* p, const View& like, int64_t rows, int64_t cols) {
+  return like.rs == 1 && like.cs != 1 ? View{p, 1, rows} : View{p, cols, 1};
+}
 View transposed(View v) { return View{v.p, v.cs, v.rs}; }
 Operand transposed(Operand o) {
   std::swap(o.rows, o.k);
@@ -546,7 +550,7 @@ struct Summer {
   int n = 0, pieces = 0;
   int64_t total = 0;
   void add(const SumJob& j) {
-    if (n == 2) run();
+    if (n == 2 || (n && (pieces > 8) != (j.pieces > 8))) run();
     jobs.j[n++] = j;
     pieces = std::max(pieces, j.pieces);
     total = std::max(total, j.rows * j.cols);
@@ -694,15 +698,23 @@ int act_forward(Run& r, int dtype, int act, const vi_matrix* x, const vi_matrix*
   e.res = view(res);
   e.out = view(y);
   e.dact = dact ? dact->data : nullptr;
+  if (!e.dact && narrow_forward(N, K, view(x), e.out, e.res)) {
+    if (r.dry) return VI_OK;
+    const cudaError_t rc = launch_narrow(dtype, NarrowArgs{M, (int)N, (int)K, act, view(x), view(w), bias, e.out, e.res},
+                                         false, 0, r.sms, r.s);
+    r.launches++;
+    return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+  }
   Packer pk{r, dtype};
   const Operand A = pk.add(view(x), M, K), B = pk.add(view(w), N, K);
   pk.run();
   return gemm(r, dtype, kEpiAct, A, B, e);
 }
 
-int act_backward(Run& r, int dtype, const vi_matrix* dy, const vi_matrix* dact, const vi_matrix* x,
-                 const vi_matrix* w, const vi_matrix* dx, const vi_matrix* dw, void* db) {
+int act_backward(Run& r, int dtype, int act, const vi_matrix* dy, const vi_matrix* dact, const vi_matrix* x,
+                 const vi_matrix* w, const void* bias, const vi_matrix* dx, const vi_matrix* dw, void* db) {
   if (int rc = check_operands(dtype, x, w)) return rc;
+  if (act < VI_ACT_NONE || act > VI_ACT_SIGMOID) return bad("linear_act backward: unknown activation");
   const int64_t M = x->rows, K = x->cols, N = w->rows;
   if (!given(dy) || dy->rows != M) return bad("linear_act backward: dy is required, [M, N]");
   if (int rc = check_shape(dy, M, N, false, "linear_act backward: dy must be [M, N]")) return rc;
@@ -714,14 +726,38 @@ int act_backward(Run& r, int dtype, const vi_matrix* dy, const vi_matrix* dact, 
     zero_gradients(r, dtype, N, K, dw, db);
     return VI_OK;
   }
-  const View slope = view(dact);
+  View slope = view(dact);
   const bool need_dx = dx && dx->data, need_dw = dw && dw->data;
   Summer sums{r, dtype};
+  if (!slope.p && narrow_backward(N, K, view(x), view(dy), view(dx))) {
+    const int blocks = narrow_blocks(M, r.sms), per = narrow_sums(K);
+    NarrowArgs a{M, (int)N, (int)K, act, view(x), view(w), bias, view(dy), View{nullptr, 0, 0}, view(dx)};
+    if (need_dw || db) a.part = (float*)r.take((size_t)blocks * N * per * 4);
+    if (!r.dry) {
+      const cudaError_t rc = launch_narrow(dtype, a, true, blocks, r.sms, r.s);
+      r.launches++;
+      if (rc != cudaSuccess) return set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+    }
+    if (need_dw) sums.add(SumJob{a.part, blocks, N * per, per, 1, N, K, nullptr, view(dw)});
+    if (db) sums.add(SumJob{a.part + per - 1, blocks, N * per, 0, per, 1, N, nullptr, View{db, 0, 1}});
+    sums.run();
+    return VI_OK;
+  }
   Packer pk{r, dtype};
   Operand S{}, W{}, X{};
-  if (need_dx) W = pk.add(view(w), N, K);
-  if (need_dw) X = pk.add(view(x), M, K);
+  const bool again = !slope.p && act != VI_ACT_NONE;  // act' was not kept
+  if (need_dx || again) W = pk.add(view(w), N, K);
+  if (need_dw || again) X = pk.add(view(x), M, K);
   pk.run();
+  if (again) {
+    Epilogue e{};
+    e.act = act;
+    e.bias = bias;
+    e.out = scratch_like(r.take((size_t)M * N * es), view(dy), M, N);
+    slope = scratch_like(r.take((size_t)M * N * es), view(dy), M, N);
+    e.dact = slope.p;
+    if (int rc = gemm(r, dtype, kEpiAct, X, W, e)) return rc;
+  }
   // s = dy * act', where dy itself does not serve; the bias's gradient in the same pass
   const View d = view(dy);
   const bool in_place = !slope.p && direct(dtype, d, M, N);
@@ -917,19 +953,29 @@ extern "C" int vi_linear_act_forward(int dtype, int activation, const vi_matrix*
                  scratch_bytes, stream, "linear_act");
 }
 
-extern "C" uint64_t vi_linear_act_backward_scratch_bytes(int dtype, const vi_matrix* dy, const vi_matrix* dact,
-                                                         const vi_matrix* x, const vi_matrix* weight,
-                                                         const vi_matrix* dx, const vi_matrix* dweight,
-                                                         const void* dbias) {
-  return count_bytes(
-      [&](Run& r) { return act_backward(r, dtype, dy, dact, x, weight, dx, dweight, const_cast<void*>(dbias)); });
+extern "C" int vi_linear_act_keeps_dact(int dtype, int activation, const vi_matrix* x, const vi_matrix* weight) {
+  if (check_operands(dtype, x, weight) || activation == VI_ACT_NONE) return 0;
+  const View v = view(x);
+  return !narrow_backward(weight->rows, x->cols, v, View{v.p, 1, 2}, View{v.p, 1, 2});
 }
 
-extern "C" int vi_linear_act_backward(int dtype, const vi_matrix* dy, const vi_matrix* dact, const vi_matrix* x,
-                                      const vi_matrix* weight, const vi_matrix* dx, const vi_matrix* dweight,
-                                      void* dbias, void* scratch, uint64_t scratch_bytes, void* stream) {
-  return execute([&](Run& r) { return act_backward(r, dtype, dy, dact, x, weight, dx, dweight, dbias); }, scratch,
-                 scratch_bytes, stream, "linear_act backward");
+extern "C" uint64_t vi_linear_act_backward_scratch_bytes(int dtype, int activation, const vi_matrix* dy,
+                                                         const vi_matrix* dact, const vi_matrix* x,
+                                                         const vi_matrix* weight, const void* bias,
+                                                         const vi_matrix* dx, const vi_matrix* dweight,
+                                                         const void* dbias) {
+  return count_bytes([&](Run& r) {
+    return act_backward(r, dtype, activation, dy, dact, x, weight, bias, dx, dweight, const_cast<void*>(dbias));
+  });
+}
+
+extern "C" int vi_linear_act_backward(int dtype, int activation, const vi_matrix* dy, const vi_matrix* dact,
+                                      const vi_matrix* x, const vi_matrix* weight, const void* bias,
+                                      const vi_matrix* dx, const vi_matrix* dweight, void* dbias, void* scratch,
+                                      uint64_t scratch_bytes, void* stream) {
+  return execute(
+      [&](Run& r) { return act_backward(r, dtype, activation, dy, dact, x, weight, bias, dx, dweight, dbias); }, scratch,
+      scratch_bytes, stream, "linear_act backward");
 }
 
 extern "C" uint64_t vi_linear_ce_forward_scratch_bytes(int dtype, const vi_matrix* x, const vi_matrix* weight,

@@ -77,5 +77,24 @@ int lse_parts(int bn);
 int launch_gemm(int dtype, int epi, const Operand& a, const Operand& b, const Plan& p, const Epilogue& e, int sms,
                 cudaStream_t s);
 
+// linear_act on images (rows contiguous) of at most kNarrowK channels, on the FP32 cores.
+constexpr int kNarrowK = 8, kNarrowN = 256;
+struct NarrowArgs {
+  int64_t M;
+  int N, K, act;
+  View x, w;
+  const void* bias;
+  View y;        // the result; in the backward the incoming gradient
+  View res, dx;  // p null = none
+  float* part;   // backward: [blocks][N][narrow_sums(K)], the sums of s x[k], then zeros up to the last, of s
+  bool vec;      // set by the launcher
+  int span;      // set by the launcher: channels a block takes
+};
+bool narrow_forward(int64_t N, int64_t K, const View& x, const View& y, const View& res);
+bool narrow_backward(int64_t N, int64_t K, const View& x, const View& dy, const View& dx);
+int narrow_sums(int64_t K);
+int narrow_blocks(int64_t M, int sms);  // of the backward
+cudaError_t launch_narrow(int dtype, const NarrowArgs& a, bool backward, int blocks, int sms, cudaStream_t s);
+
 }  // namespace heads
 }  // namespace vi

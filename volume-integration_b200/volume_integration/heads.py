@@ -63,19 +63,20 @@ class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
         # act' is kept rather than z: it is exact for relu, and the backward needs no transcendental
-        want = activation != 0 and any(ctx.needs_input_grad[:3])
-        y, dact = _C.linear_act_forward(x, weight, bias, residual, activation, want)
-        ctx.save_for_backward(x, weight, dact)
+        # (images of few channels keep neither: dact is None)
+        y, dact = _C.linear_act_forward(x, weight, bias, residual, activation, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, bias, dact)
+        ctx.activation = activation
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, dact = ctx.saved_tensors
+        x, weight, bias, dact = ctx.saved_tensors
         nx, nw, nb, nr = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if nx or nw or nb:
-            dx, dw, db = _C.linear_act_backward(dy, dact, x, weight, nx, nw, nb)
+            dx, dw, db = _C.linear_act_backward(dy, dact, x, weight, bias, ctx.activation, nx, nw, nb)
         return dx, dw, db, dy if nr else None, None
 
 
