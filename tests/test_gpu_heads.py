@@ -460,6 +460,51 @@ def test_decoder_and_loss_together(dt, rel):
         _close(a, b, rel)
 
 
+@pytest.mark.parametrize("want", [("x",), ("w",), ("b",), ("r",), ("w", "b"), ("x", "r")])
+@pytest.mark.parametrize("order", ["rows", "image"])
+def test_linear_act_some_gradients(want, order):
+    import volume_integration.heads as heads
+    for K in (4, 40):
+        t = dict(zip("xwbr", _act_inputs(300, K, 24, BF16, order, True, True, 50)[:4]))
+        dy = hl.matrix(300, 24, BF16, _gen(51), order)
+        leaves = {k: (v.detach().requires_grad_(True) if k in want else v) for k, v in t.items()}
+        y = heads.linear_act(leaves["x"], leaves["w"], leaves["b"], leaves["r"], "gelu")
+        got = dict(zip(want, torch.autograd.grad(y, [leaves[k] for k in want], dy)))
+        ref = dict(zip("xwb", hl.linear_act(t["x"], t["w"], t["b"], t["r"], "gelu", dy)[1:]))
+        for k, g in got.items():
+            if k == "r":
+                assert torch.equal(g, dy)
+            else:
+                hl.assert_within(k, g, ref[k])
+        # of a graph that could give all of them
+        full = [v.detach().requires_grad_(True) for v in t.values()]
+        y = heads.linear_act(*full, activation="gelu")
+        for k, g in zip(want, torch.autograd.grad(y, [full["xwbr".index(k)] for k in want], dy)):
+            assert torch.equal(g, got[k])
+
+
+@pytest.mark.parametrize("want", [("x",), ("w",), ("b",), ("w", "b")])
+def test_linear_cross_entropy_some_gradients(want):
+    import volume_integration.heads as heads
+    x, w, b, t = _ce_inputs(300, 40, 130, BF16, "rows", True, 0.2, 52)
+    v = dict(zip("xwb", (x, w, b)))
+    leaves = {k: (u.detach().requires_grad_(True) if k in want else u) for k, u in v.items()}
+    loss = heads.linear_cross_entropy(leaves["x"], leaves["w"], t, leaves["b"])
+    ref = dict(zip("xwb", hl.linear_ce(x, w, b, t, -100, "mean", torch.ones((), device="cuda"))[1:]))
+    for k, g in zip(want, torch.autograd.grad(loss, [leaves[k] for k in want])):
+        hl.assert_within(k, g, ref[k])
+
+
+def test_no_second_derivative():
+    import volume_integration.heads as heads
+    x, w, b, t = _ce_inputs(30, 8, 9, F32, "rows", True, 0.0, 53)
+    x.requires_grad_(True)
+    for out in (heads.linear_act(x, w, b, activation="silu").sum(), heads.linear_cross_entropy(x, w, t, b)):
+        (g,) = torch.autograd.grad(out, (x,), create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            g.sum().backward()
+
+
 def test_another_stream_and_two_at_once():
     # two streams run the chain at the same time on inputs made on a third
     x, ws, t = _decoder(BF16, _gen(21), M=3000)

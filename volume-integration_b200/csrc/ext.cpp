@@ -6,6 +6,7 @@
 // (integrate_primitives.cu:54-68).  Errors raise RuntimeError.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <tuple>
@@ -515,6 +516,104 @@ Grads linear_ce_backward(const Tensor& x, const Tensor& weight, const c10::optio
   return {g.dx, g.dw, g.db};
 }
 
+// The heads as differentiable functions.  In C++, so that a step on a few rows does not spend its
+// time in the interpreter; a second derivative raises, as torch's once_differentiable does.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void differentiate_once(variable_list& grads) {
+  if (!torch::GradMode::is_enabled()) return;
+  variable_list fake;
+  std::vector<size_t> at;
+  for (size_t i = 0; i < grads.size(); i++) {
+    if (!grads[i].defined()) continue;
+    Tensor t = grads[i].detach();
+    t.set_requires_grad(true);
+    fake.push_back(t);
+    at.push_back(i);
+  }
+  if (fake.empty()) return;
+  auto fn = std::make_shared<torch::autograd::DelayedError>(
+      "trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)fake.size());
+  variable_list out = (*fn)(std::move(fake));
+  for (size_t i = 0; i < at.size(); i++) grads[at[i]] = out[i];
+}
+c10::optional<Tensor> optional_of(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+bool wants_grad(const c10::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
+
+struct LinearAct : torch::autograd::Function<LinearAct> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias,
+                        const c10::optional<Tensor>& residual, int64_t activation) {
+    // act' is kept rather than z: it is exact for relu, and the backward needs no transcendental
+    auto [y, dact] = linear_act_forward(x, weight, bias, residual, activation,
+                                        wants_grad(x) || wants_grad(weight) || wants_grad(bias));
+    ctx->save_for_backward({x, weight, bias.value_or(Tensor()), dact.value_or(Tensor())});
+    ctx->saved_data["activation"] = activation;
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = residual.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dys) {
+    const variable_list saved = ctx->get_saved_variables();
+    const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = has_b && ctx->needs_input_grad(2);
+    variable_list out(5);
+    if (nx || nw || nb) {
+      auto [dx, dw, db] = linear_act_backward(dys[0], optional_of(saved[3]), saved[0], saved[1], optional_of(saved[2]),
+                                              ctx->saved_data["activation"].toInt(), nx, nw, nb);
+      if (nx) out[0] = *dx;
+      if (nw) out[1] = *dw;
+      if (nb) out[2] = *db;
+    }
+    differentiate_once(out);
+    if (has_r && ctx->needs_input_grad(has_b ? 3 : 2)) out[3] = dys[0];
+    return out;
+  }
+};
+
+Tensor linear_act(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias,
+                  const c10::optional<Tensor>& residual, int64_t activation) {
+  if (torch::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual)))
+    return LinearAct::apply(x, weight, bias, residual, activation);
+  return std::get<0>(linear_act_forward(x, weight, bias, residual, activation, false));
+}
+
+struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias,
+                        const Tensor& target, int64_t ignore_index, int64_t reduction) {
+    auto [loss, lse] = linear_ce_forward(x, weight, bias, target, ignore_index, reduction);
+    ctx->save_for_backward({x, weight, bias.value_or(Tensor()), target, lse});
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["ignore"] = ignore_index;
+    ctx->saved_data["reduction"] = reduction;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dloss) {
+    const variable_list saved = ctx->get_saved_variables();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
+    const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+    variable_list out(6);
+    if (nx || nw || nb) {
+      auto [dx, dw, db] =
+          linear_ce_backward(saved[0], saved[1], optional_of(saved[2]), saved[3], ctx->saved_data["ignore"].toInt(),
+                             ctx->saved_data["reduction"].toInt(), saved[4], dloss[0], nx, nw, nb);
+      if (nx) out[0] = *dx;
+      if (nw) out[1] = *dw;
+      if (nb) out[2] = *db;
+    }
+    differentiate_once(out);
+    return out;
+  }
+};
+
+Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias,
+                            const Tensor& target, int64_t ignore_index, int64_t reduction) {
+  if (torch::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
+    return LinearCrossEntropy::apply(x, weight, bias, target, ignore_index, reduction);
+  return std::get<0>(linear_ce_forward(x, weight, bias, target, ignore_index, reduction));
+}
+
 // The heads' status word of a device (0 = no wait gave up).
 int64_t heads_status(int64_t device, bool reset) {
   const at::cuda::CUDAGuard guard((c10::DeviceIndex)device);
@@ -539,6 +638,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("preprocess_gaussians_backward", &preprocess_gaussians_backward,
         "Exact derivative of the Gaussian-attribute preprocess (extension)");
   m.def("bin_gaussians", &bin_gaussians, "Tile binning of projected Gaussians (extension)");
+  m.def("linear_act", &linear_act, "act(x W^T + b) + residual, differentiable (extension)");
+  m.def("linear_cross_entropy", &linear_cross_entropy, "Cross entropy of a linear classifier, differentiable (extension)");
   m.def("linear_act_forward", &linear_act_forward, "act(x W^T + b) + residual (extension)");
   m.def("linear_act_backward", &linear_act_backward, "Gradients of linear_act_forward (extension)");
   m.def("linear_ce_forward", &linear_ce_forward, "Cross entropy of a linear classifier (extension)");

@@ -9,6 +9,7 @@
 // rows are split into pieces that are added in a fixed order, so results do not
 // depend on scheduling.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 #include <utility>
 #include <cstdio>
@@ -281,15 +282,14 @@ __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumJob
   }
 }
 
-// Rows' losses from the parts' maxima and sums; per block the sum of its rows' losses and their count.
+// Rows' losses from the parts' maxima and sums; per block the sum of its rows' losses and their count (total not null: the one block's sum or mean itself).
 __global__ void __launch_bounds__(256) loss_kernel(const float* pmax, const float* psum, const float* ztarget,
                                                    int parts, int64_t M, int64_t V, const int64_t* target,
                                                    int64_t ignore, float* rows, float* lse, float* bsum,
-                                                   float* bcount) {
+                                                   float* bcount, float* total, int mean) {
   __shared__ float sh[2][8];
-  const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
   float loss = 0.0f, live = 0.0f;
-  if (m < M) {
+  for (int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x; m < M; m += (int64_t)gridDim.x * 256) {
     float top = -INFINITY, sum = 0.0f;
     for (int i = 0; i < parts; i++) top = fmaxf(top, pmax[(int64_t)i * M + m]);
     for (int i = 0; i < parts; i++) {
@@ -301,9 +301,10 @@ __global__ void __launch_bounds__(256) loss_kernel(const float* pmax, const floa
     const bool ignored = t == ignore, bad = !ignored && (t < 0 || t >= V);
     lse[m] = top;
     lse[M + m] = bad ? NAN : l;
-    loss = ignored ? 0.0f : bad ? NAN : fmaf(l, 0.6931471806f, top - ztarget[m]);
-    live = ignored ? 0.0f : 1.0f;
-    if (rows) rows[m] = loss;
+    const float row = ignored ? 0.0f : bad ? NAN : fmaf(l, 0.6931471806f, top - ztarget[m]);
+    loss += row;
+    live += ignored ? 0.0f : 1.0f;
+    if (rows) rows[m] = row;
   }
   for (int o = 16; o; o >>= 1) {
     loss += __shfl_xor_sync(0xffffffffu, loss, o);
@@ -311,10 +312,14 @@ __global__ void __launch_bounds__(256) loss_kernel(const float* pmax, const floa
   }
   if (threadIdx.x % 32 == 0) sh[0][threadIdx.x / 32] = loss, sh[1][threadIdx.x / 32] = live;
   __syncthreads();
-  if (threadIdx.x == 0 && bsum) {
+  if (threadIdx.x == 0 && (bsum || total)) {
     for (int i = 1; i < 8; i++) loss += sh[0][i], live += sh[1][i];
-    bsum[blockIdx.x] = loss;
-    bcount[blockIdx.x] = live;
+    if (total) {  // the only block
+      total[0] = mean ? loss / live : loss;
+    } else {
+      bsum[blockIdx.x] = loss;
+      bcount[blockIdx.x] = live;
+    }
   }
 }
 
@@ -365,14 +370,23 @@ __global__ void __launch_bounds__(256) coef_parts_kernel(const int64_t* target, 
   }
 }
 
-// Then the factors themselves; every block adds the (at most 256) parts up again.
+// Then the factors themselves; every block adds the (at most 256) parts up again (bmax null: there is one block).
 __global__ void __launch_bounds__(256) coef_kernel(const int64_t* target, int64_t ignore, int64_t M, int reduction,
                                                    const float* dloss, const float* bmax, const uint32_t* bcount,
                                                    int parts, float lift, float* coef, float* alpha) {
   __shared__ float shm[8];
   __shared__ uint32_t shc[8];
-  float top = threadIdx.x < parts ? bmax[threadIdx.x] : 0.0f;
-  uint32_t live = threadIdx.x < parts ? bcount[threadIdx.x] : 0;
+  float top = 0.0f;
+  uint32_t live = 0;
+  if (bmax) {
+    if (threadIdx.x < parts) top = bmax[threadIdx.x], live = bcount[threadIdx.x];
+  } else {  // one block: it finds them itself
+    for (int64_t m = threadIdx.x; m < M; m += 256) {
+      const bool on = target[m] != ignore;
+      live += on;
+      if (reduction == VI_REDUCE_NONE && on && isfinite(dloss[m])) top = fmaxf(top, fabsf(dloss[m]));
+    }
+  }
   for (int o = 16; o; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     live += __shfl_xor_sync(0xffffffffu, live, o);
@@ -401,9 +415,13 @@ __global__ void __launch_bounds__(256) coef_kernel(const int64_t* target, int64_
 // `dry` it only carves, which is how the _scratch_bytes queries count.
 // ---------------------------------------------------------------------------
 int sm_count() {
+  static std::atomic<int> known[64];
   int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64) {
+    if ((n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    known[dev].store(n, std::memory_order_relaxed);
+  }
   return n > 0 ? n : 148;
 }
 
@@ -789,7 +807,7 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
   if (reduction < VI_REDUCE_NONE || reduction > VI_REDUCE_SUM) return bad("linear_ce: unknown reduction");
   const int64_t M = x->rows, K = x->cols, V = w->rows;
   if (!r.dry && M && (!target || !loss || !lse)) return bad("linear_ce: target, loss and lse are required");
-  const int64_t blocks = ceil_div(M, 256);
+  const int64_t blocks = M <= 1024 ? std::min<int64_t>(M, 1) : ceil_div(M, 256);  // few rows: one block ends the sum too
   Plan p{};
   p.splits = 1;
   p.kps = (int)ceil_div(K, 64);
@@ -822,10 +840,11 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
     if (int rc = launch_gemm(dtype, kEpiLse, A, B, p, e, r.sms, r.s)) return rc;
     const bool none = reduction == VI_REDUCE_NONE;
     loss_kernel<<<(unsigned)blocks, 256, 0, r.s>>>(pmax, psum, zt, parts, M, V, target, ignore,
-                                                   none ? loss : nullptr, lse, none ? nullptr : bsum, bcount);
+                                                   none ? loss : nullptr, lse, none || blocks == 1 ? nullptr : bsum, bcount,
+                                                   !none && blocks == 1 ? loss : nullptr, reduction == VI_REDUCE_MEAN);
     r.launches++;
   }
-  if (reduction != VI_REDUCE_NONE) {
+  if (reduction != VI_REDUCE_NONE && blocks != 1) {
     if (!loss) return bad("linear_ce: loss is required");
     reduce_loss_kernel<<<1, 256, 0, r.s>>>(bsum, bcount, blocks, reduction == VI_REDUCE_MEAN, loss);
     r.launches++;
@@ -851,14 +870,17 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
   const int planes = dtype == VI_F32 ? 3 : 1;
   float* coef = (float*)r.take((size_t)M * 4);
   float* alpha = (float*)r.take(4);
-  const int parts = (int)std::min<int64_t>(ceil_div(M, 1024), 256);
+  const int parts = M <= 4096 ? 1 : (int)std::min<int64_t>(ceil_div(M, 1024), 256);
   float* bmax = (float*)r.take((size_t)parts * 4);
   uint32_t* bcount = (uint32_t*)r.take((size_t)parts * 4);
   if (!r.dry) {
-    coef_parts_kernel<<<parts, 256, 0, r.s>>>(target, ignore, M, reduction == VI_REDUCE_NONE ? dloss : nullptr, bmax, bcount);
-    coef_kernel<<<parts, 256, 0, r.s>>>(target, ignore, M, reduction, dloss, bmax, bcount, parts,
+    if (parts > 1) {
+      coef_parts_kernel<<<parts, 256, 0, r.s>>>(target, ignore, M, reduction == VI_REDUCE_NONE ? dloss : nullptr, bmax, bcount);
+      r.launches++;
+    }
+    coef_kernel<<<parts, 256, 0, r.s>>>(target, ignore, M, reduction, dloss, parts > 1 ? bmax : nullptr, bcount, parts,
                                         dtype == VI_F16 ? 16384.0f : 1.0f, coef, alpha);
-    r.launches += 2;
+    r.launches++;
   }
   // x without the rows of ignored targets: their zero gradient times a NaN or an
   // infinity would else reach the weights' gradient

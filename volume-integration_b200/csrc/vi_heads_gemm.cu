@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 #include <type_traits>
@@ -345,12 +346,25 @@ __device__ __forceinline__ int load_tile(Row<Z>& r, const View& v, int access, u
     }
     return kImage;
   }
-  // any strides, ragged ends: each lane its row, into the staging (rolled: the kernel's code has to stay small)
+  // ragged ends and any strides, into the staging: a row at a time where columns are contiguous, else a
+  // column at a time; eight loads in flight (more would unroll more code than they are worth)
   __syncwarp();
-  if (lane < t.rows) {
-    const typename Row<Z>::Bits* q = (const typename Row<Z>::Bits*)p + (int64_t)(t.m0 + lane) * v.rs + (int64_t)t.n0 * v.cs;
+  using Bits = typename Row<Z>::Bits;
+  const bool by_rows = v.cs == 1;
+  const int lines = by_rows ? t.rows : t.cols, along = by_rows ? t.cols : t.rows;
+  const int64_t step = by_rows ? v.rs : v.cs;
+  const Bits* q = (const Bits*)p + (int64_t)t.m0 * v.rs + (int64_t)t.n0 * v.cs + lane * (by_rows ? v.cs : v.rs);
+  if (lane < along) {
 #pragma unroll 1
-    for (int j = 0; j < t.cols; j++, q += v.cs) sts_cell(G::cell(st, lane, j), *q);
+    for (int l = 0; l < lines; l += 8) {
+      Bits b[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (l + i < lines) b[i] = q[(l + i) * step];
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (l + i < lines) sts_cell(by_rows ? G::cell(st, l + i, lane) : G::cell(st, lane, l + i), b[i]);
+    }
   }
   return kScalar;
 }
@@ -842,8 +856,16 @@ bool encode(CUtensorMap* map, const Operand& o, int planes, bool half, int box_r
 template <typename T, int BN, int EPI, int ACT>
 cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
   auto* k = gemm_tc_kernel<T, BN, EPI, ACT>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, BN, EPI>::kSmem);
-  if (e != cudaSuccess) return e;
+  // once per device: the call costs as much as a launch
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(done.load(std::memory_order_relaxed) & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, BN, EPI>::kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  }
   k<<<(unsigned)std::min<int64_t>(a.items, (int64_t)sms * Shape<T, BN, EPI>::kBlocks), Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>::kSmem, s>>>(ma, mb, a);
   return cudaPeekAtLastError();
 }

@@ -241,10 +241,7 @@ cudaError_t run(const NarrowArgs& args, bool backward, int blocks, int sms, cuda
   NarrowArgs a = args;
   if (backward) {
     const size_t smem = ((size_t)a.N * (KT + 1) + (size_t)kThreads / 32 * a.N * (KT + 1)) * 4;
-    auto* k = narrow_backward_kernel<T, KT, ACT>;
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    k<<<blocks, kThreads, smem, s>>>(a);
+    narrow_backward_kernel<T, KT, ACT><<<blocks, kThreads, smem, s>>>(a);
   } else {
     // few pixels: channels are spread over blocks too
     const int64_t tiles = (a.M + kTile - 1) / kTile;

@@ -23,7 +23,6 @@ bfloat16 parts, which keeps float32's precision (an infinite feature or weight
 gives NaN where float32 arithmetic might give an infinity).
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _C
 
@@ -59,27 +58,6 @@ def _check_like(x, t, what, name):
         raise ValueError(f"{what}: {name} is on {t.device} but x is on {x.device}")
 
 
-class _LinearAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation):
-        # act' is kept rather than z: it is exact for relu, and the backward needs no transcendental
-        # (images of few channels keep neither: dact is None)
-        y, dact = _C.linear_act_forward(x, weight, bias, residual, activation, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, weight, bias, dact)
-        ctx.activation = activation
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, dact = ctx.saved_tensors
-        nx, nw, nb, nr = ctx.needs_input_grad[:4]
-        dx = dw = db = None
-        if nx or nw or nb:
-            dx, dw, db = _C.linear_act_backward(dy, dact, x, weight, bias, ctx.activation, nx, nw, nb)
-        return dx, dw, db, dy if nr else None, None
-
-
 def linear_act(x, weight, bias=None, residual=None, activation="none"):
     """``act(x @ weight.T + bias) + residual`` in one pass over the output.
 
@@ -104,32 +82,8 @@ def linear_act(x, weight, bias=None, residual=None, activation="none"):
     two_d = x.dim() == 2
     x2 = x if two_d else x.reshape(-1, x.shape[-1])
     r2 = residual if two_d or residual is None else residual.reshape(-1, n)
-    act = ACTIVATIONS.index(activation)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias, r2)):
-        y = _LinearAct.apply(x2, weight, bias, r2, act)
-    else:
-        y = _C.linear_act_forward(x2, weight, bias, r2, act, False)[0]
+    y = _C.linear_act(x2, weight, bias, r2, ACTIVATIONS.index(activation))
     return y if two_d else y.reshape(lead + (n,))
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, target, ignore_index, reduction):
-        loss, lse = _C.linear_ce_forward(x, weight, bias, target, ignore_index, reduction)
-        ctx.save_for_backward(x, weight, bias, target, lse)
-        ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dloss):
-        x, weight, bias, target, lse = ctx.saved_tensors
-        nx, nw, nb = ctx.needs_input_grad[:3]
-        dx = dw = db = None
-        if nx or nw or nb:
-            dx, dw, db = _C.linear_ce_backward(x, weight, bias, target, ctx.ignore_index, ctx.reduction, lse,
-                                               dloss, nx, nw, nb)
-        return dx, dw, db, None, None, None
 
 
 def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean"):
@@ -156,11 +110,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
         raise ValueError(f"linear_cross_entropy: target is on {target.device} but x is on {x.device}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     t1 = target.reshape(-1).contiguous()
-    red = REDUCTIONS.index(reduction)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias)):
-        loss = _LinearCrossEntropy.apply(x2, weight, bias, t1, int(ignore_index), red)
-    else:
-        loss = _C.linear_ce_forward(x2, weight, bias, t1, int(ignore_index), red)[0]
+    loss = _C.linear_cross_entropy(x2, weight, bias, t1, int(ignore_index), REDUCTIONS.index(reduction))
     return loss.reshape(target.shape) if reduction == "none" else loss
 
 
