@@ -410,6 +410,7 @@ Tensor head_result(const Tensor& x, int64_t rows, int64_t cols) {
 }
 Tensor head_scratch(uint64_t bytes, const Tensor& x) {
   TORCH_CHECK(bytes > 0, "volume_integration: ", vi_last_error());
+  if (bytes <= 256) return {};  // nothing but the query's constant: the call takes none
   return torch::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8));
 }
 
@@ -436,7 +437,7 @@ std::tuple<Tensor, c10::optional<Tensor>> linear_act_forward(const Tensor& x, co
                                                          want_dact ? &md : nullptr);
   Tensor scratch = head_scratch(n, x);
   ok(vi_linear_act_forward(dt, (int)activation, &mx, &mw, head_ptr(b), r.get(), &my, want_dact ? &md : nullptr,
-                           scratch.data_ptr(), n, at::cuda::getCurrentCUDAStream().stream()));
+                           head_ptr(scratch), n, at::cuda::getCurrentCUDAStream().stream()));
   return {y, dact};
 }
 
@@ -472,7 +473,7 @@ Grads linear_act_backward(const Tensor& dy, const c10::optional<Tensor>& dact, c
                                                           g.x(), g.w(), g.b());
   Tensor scratch = head_scratch(n, x);
   ok(vi_linear_act_backward(dt, (int)activation, &mdy, d.get(), &mx, &mw, head_ptr(b), g.x(), g.w(), g.b(),
-                            scratch.data_ptr(), n, at::cuda::getCurrentCUDAStream().stream()));
+                            head_ptr(scratch), n, at::cuda::getCurrentCUDAStream().stream()));
   return {g.dx, g.dw, g.db};
 }
 
@@ -490,7 +491,7 @@ std::tuple<Tensor, Tensor> linear_ce_forward(const Tensor& x, const Tensor& weig
   const uint64_t n = vi_linear_ce_forward_scratch_bytes(dt, &mx, &mw, head_ptr(b));
   Tensor scratch = head_scratch(n, x);
   ok(vi_linear_ce_forward(dt, &mx, &mw, head_ptr(b), t.data_ptr<int64_t>(), ignore_index, (int)reduction,
-                          loss.data_ptr<float>(), lse.data_ptr<float>(), scratch.data_ptr(), n,
+                          loss.data_ptr<float>(), lse.data_ptr<float>(), head_ptr(scratch), n,
                           at::cuda::getCurrentCUDAStream().stream()));
   return {loss, lse};
 }
@@ -511,7 +512,7 @@ Grads linear_ce_backward(const Tensor& x, const Tensor& weight, const c10::optio
   const uint64_t n = vi_linear_ce_backward_scratch_bytes(dt, &mx, &mw, head_ptr(b), g.x(), g.w(), g.b());
   Tensor scratch = head_scratch(n, x);
   ok(vi_linear_ce_backward(dt, &mx, &mw, head_ptr(b), t.data_ptr<int64_t>(), ignore_index, (int)reduction,
-                           l.data_ptr<float>(), dl.data_ptr<float>(), g.x(), g.w(), g.b(), scratch.data_ptr(), n,
+                           l.data_ptr<float>(), dl.data_ptr<float>(), g.x(), g.w(), g.b(), head_ptr(scratch), n,
                            at::cuda::getCurrentCUDAStream().stream()));
   return {g.dx, g.dw, g.db};
 }

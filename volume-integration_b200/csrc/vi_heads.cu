@@ -513,11 +513,12 @@ struct Packer {
 
 // Tile width: the one whose waves of tiles take the least tensor-core time; narrow tiles
 // read their operands more often.
-int tile_width(int64_t M, int64_t N, int sms) {
+int tile_width(int dtype, int64_t M, int64_t N, int sms) {
   const int64_t mt = ceil_div(M, 128);
   int best = 64;
   double cost = 1e300;
   for (int bn : {256, 128, 64}) {
+    if (bn == 256 && dtype == VI_F32) continue;
     const double c = (double)ceil_div(mt * ceil_div(N, bn), sms) * (bn == 256 ? 256 : bn == 128 ? 150 : 90);
     if (c < cost) cost = c, best = bn;
   }
@@ -536,22 +537,22 @@ int gemm(Run& r, int dtype, int epi, const Operand& A, const Operand& B, const E
     f.res = transposed(e.res);
     f.bias_rows = e.bias != nullptr;
     Plan p{};
-    p.bn = tile_width(B.rows, A.rows, r.sms);
+    p.bn = tile_width(dtype, B.rows, A.rows, r.sms);
     p.splits = 1;
     p.kps = (int)ceil_div(A.k, 64);
     return launch_gemm(dtype, epi, B, A, p, f, r.sms, r.s);
   }
   Plan p{};
-  p.bn = tile_width(A.rows, B.rows, r.sms);
+  p.bn = tile_width(dtype, A.rows, B.rows, r.sms);
   p.splits = 1;
   p.kps = (int)ceil_div(A.k, 64);
   return launch_gemm(dtype, epi, A, B, p, e, r.sms, r.s);
 }
 
 // Pieces of a long sum over k when there are few tiles.
-Plan split_plan(const Operand& A, const Operand& B, int sms) {
+Plan split_plan(int dtype, const Operand& A, const Operand& B, int sms) {
   Plan p{};
-  p.bn = B.rows <= 64 ? 64 : B.rows <= 128 ? 128 : 256;
+  p.bn = B.rows <= 64 ? 64 : B.rows <= 128 || dtype == VI_F32 ? 128 : 256;
   const int64_t tiles = ceil_div(A.rows, 128) * ceil_div(B.rows, p.bn), kb = ceil_div(A.k, 64);
   // at least four blocks of k each, at most one piece per SM and tile
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(sms / std::min<int64_t>(tiles, sms), kb / 4));
@@ -565,17 +566,20 @@ struct Summer {
   Run& r;
   int dtype;
   SumJobs jobs{};
-  int n = 0, pieces = 0;
+  int n = 0;
+  bool shared = false;
   int64_t total = 0;
   void add(const SumJob& j) {
-    if (n == 2 || (n && (pieces > 8) != (j.pieces > 8))) run();
+    // many pieces of few elements: threads share an element
+    const bool s8 = j.pieces > 8 && j.rows * j.cols < 65536;
+    if (n == 2 || (n && shared != s8)) run();
+    shared = s8;
     jobs.j[n++] = j;
-    pieces = std::max(pieces, j.pieces);
     total = std::max(total, j.rows * j.cols);
   }
   void run() {
     if (n && !r.dry) {
-      if (pieces > 8) {
+      if (shared) {
         const dim3 grid((unsigned)std::min<int64_t>(ceil_div(total, 32), 148 * 16), n);
         VI_DISPATCH(dtype, (sum_kernel<T, 8><<<grid, 256, 0, r.s>>>(jobs)));
       } else {
@@ -584,14 +588,14 @@ struct Summer {
       }
       r.launches++;
     }
-    n = pieces = 0;
+    n = 0;
     total = 0;
   }
 };
 
 // out = alpha * A B^T; a long sum with few tiles in pieces, in float32, added in order (by `sums`).
 int gemm_out(Run& r, Summer& sums, const Operand& A, const Operand& B, const float* alpha, const View& out) {
-  const Plan p = split_plan(A, B, r.sms);
+  const Plan p = split_plan(sums.dtype, A, B, r.sms);
   Epilogue e{};
   if (p.splits == 1) {
     e.out = out;
@@ -811,7 +815,7 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
   Plan p{};
   p.splits = 1;
   p.kps = (int)ceil_div(K, 64);
-  p.bn = tile_width(M, V, r.sms);
+  p.bn = tile_width(dtype, M, V, r.sms);
   // column tiles in runs, so that a block keeps a row's maximum and sum in registers over several of them
   const int64_t nt = ceil_div(V, p.bn), mt = std::max<int64_t>(1, ceil_div(M, 128));
   p.span = (int)ceil_div(nt, std::min(nt, ceil_div(4 * r.sms, mt)));
@@ -896,7 +900,7 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
   float* acc = nullptr;  // dx over the pieces so far
   Plan px{};
   if (need_dx && several) {
-    px = split_plan(Operand{nullptr, M, piece}, Operand{nullptr, K, piece}, r.sms);
+    px = split_plan(dtype, Operand{nullptr, M, piece}, Operand{nullptr, K, piece}, r.sms);
     acc = (float*)r.take((size_t)px.splits * M * K * 4);
   }
   const size_t mark = r.cur;

@@ -62,7 +62,7 @@ struct Epilogue {
 
 // Tile shape and division of one product's work.
 struct Plan {
-  int bn;          // columns of a tile
+  int bn;          // columns of a tile: 64, 128, or 256 (16-bit types only)
   int splits;      // pieces of the sum over k (kEpiPartial)
   int kps;         // 64-wide blocks of k per piece
   int span;        // column tiles one work item takes in turn (kEpiLse)

@@ -10,8 +10,8 @@
 // transposes nothing.
 //
 // float32 operands come as three bfloat16 planes, x = x0 + x1 + x2.  Of the nine
-// products of planes the six with i + j <= 2 are summed, smallest first; the others
-// are below 2^-24 of |x||w|.
+// products of planes the six with i + j <= 2 are summed, smallest first within every
+// block of k; the others are below 2^-24 of |x||w|.
 //
 // Every wait is bounded; one that runs out ends the block's work, drains what it
 // has in flight, and is latched in a status word (VI_DEVICE_HEAD_TIMEOUT).
@@ -40,21 +40,28 @@ __device__ uint32_t g_status;  // VI_DEVICE_HEAD_TIMEOUT when a wait ran out
 // Narrow tiles belong to products that memory bounds (few columns, short sums): two
 // blocks per SM, so that one's epilogue runs while the other waits for memory.  A
 // 256-wide tile takes all tensor memory (two accumulators) and the SM for itself.
-template <typename T, int BN, int EPI>
+// PL planes of both operands share a stage, so that the six products of float32's are made of
+// each copied block once.
+template <typename T, int BN, int EPI, int PL>
 struct Shape {
-  // float32's epilogue with act' needs more registers than half an SM has
-  static constexpr int kBlocks = BN == 256 || (EPI == kEpiAct && sizeof(T) == 4) ? 1 : 2;
+  static_assert(PL == 1 || BN <= 128, "three planes of a 256-wide tile leave no second stage");
+  static constexpr int kBlocks = BN == 256 || PL == 3 ? 1 : 2;
   // Epilogue warps.  The softmax on a 256-wide tile has 16: with 8 its latency, not its
   // instructions, bound it (K = 256: gradient 289 us with 8, 230 with 16; statistics 207, 159).
   static constexpr int kWarps = BN == 256 && (EPI == kEpiLse || EPI == kEpiGrad) ? 16 : 8;
   static constexpr int kParts = kWarps / 4;  // warps that share a tile's columns, 32 at a time
   static constexpr int kThreads = (kWarps + 2) * 32;
-  static constexpr int kStages = BN == 256 ? (sizeof(T) == 4 && EPI == kEpiGrad ? 3 : 4) : BN == 128 ? (kBlocks == 2 ? 2 : 5) : (kBlocks == 2 ? 3 : 7);
-  static constexpr int kStage = (kBM + BN) * kBK * 2;  // bytes
+  static constexpr int kTileA = kBM * kBK * 2, kTileB = BN * kBK * 2;  // bytes of a plane
+  static constexpr int kStage = PL * (kTileA + kTileB);
+  static constexpr int kStages = PL == 3   ? 2
+                                 : BN == 256 ? 4
+                                 : BN == 128 ? (kBlocks == 2 ? 2 : 5)
+                                             : (kBlocks == 2 ? 3 : 7);
   static constexpr int kStageWarp = EPI == kEpiLse ? 0 : 32 * 32 * (int)sizeof(T);  // an epilogue warp's staging
   // beside the stages each epilogue warp has its staging and 32 float32 of bias
   static constexpr int kBars = kStages * kStage + kWarps * (kStageWarp + 128);
   static constexpr int kSmem = kBars + (2 * kStages + 5) * 8 + 8;
+  static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
 // n / d for 0 <= n < 2^31 by a multiplication: mul = ceil(2^(31 + s) / d), s = ceil(log2 d).
@@ -75,7 +82,6 @@ struct Args {
   int kblocks;           // 64-wide blocks of the whole sum
   int kps, splits;
   int span, spans;
-  int pairs;             // products of planes: 1 or 6
   uint32_t idesc;        // instruction descriptor
   uint32_t a_lbo, b_lbo; // bytes >> 4
   uint32_t a_step, b_step;  // bytes >> 4 from one 16-wide slice of k to the next
@@ -346,11 +352,11 @@ __device__ __forceinline__ int load_tile(Row<Z>& r, const View& v, int access, u
     }
     return kImage;
   }
-  // ragged ends and any strides, into the staging: a row at a time where columns are contiguous, else a
-  // column at a time; eight loads in flight (more would unroll more code than they are worth)
+  // ragged ends and any strides, into the staging: a row at a time where columns are contiguous and
+  // many, else a column at a time; eight loads in flight (more would unroll more code than they are worth)
   __syncwarp();
   using Bits = typename Row<Z>::Bits;
-  const bool by_rows = v.cs == 1;
+  const bool by_rows = v.cs == 1 && t.cols > 16;
   const int lines = by_rows ? t.rows : t.cols, along = by_rows ? t.cols : t.rows;
   const int64_t step = by_rows ? v.rs : v.cs;
   const Bits* q = (const Bits*)p + (int64_t)t.m0 * v.rs + (int64_t)t.n0 * v.cs + lane * (by_rows ? v.cs : v.rs);
@@ -451,8 +457,8 @@ __device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int a
 #pragma unroll
     for (int i = 0; i < G::kLanes; i++, q += step)
       if (line + i * G::kStep < t.rows) *(uint4*)q = lds128(G::along(st, lane, i));
-  } else if (v.rs == 1 && v.cs != 1) {  // an image off 16 bytes, or its ragged end: lanes along the rows
-    q += lane;
+  } else if (v.cs != 1 || t.cols <= 16) {  // an image off 16 bytes or its ragged end, or few columns: a column at a time
+    q += lane * v.rs;
     if (lane < t.rows) {
 #pragma unroll 1
       for (int j = 0; j < t.cols; j++, q += v.cs) *q = lds_cell(G::cell(st, lane, j), typename Row<Z>::Bits());
@@ -477,11 +483,11 @@ __device__ __forceinline__ void add_bias(uint32_t slot, float2* v) {
   }
 }
 
-template <typename T, int BN, int EPI, int ACT>
-__global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>::kBlocks)
+template <typename T, int BN, int EPI, int PL, int ACT>
+__global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, EPI, PL>::kBlocks)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ Args a) {
-  using S = Shape<T, BN, EPI>;
+  using S = Shape<T, BN, EPI, PL>;
   constexpr int kStages = S::kStages, kStage = S::kStage, kEpiWarps = S::kWarps;
   constexpr uint32_t kCols = BN < 128 ? 2 * 64 : 2 * BN;  // tensor memory columns: two accumulators
   extern __shared__ __align__(1024) char smem[];
@@ -528,39 +534,42 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
 #pragma unroll 1
         for (int nt = t.nt; nt < t.nt_end && on; nt++) {
 #pragma unroll 1
-          for (int p = 0; p < a.pairs && on; p++) {
-            // planes of the pair, smallest products first: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
-            const int pa = a.pairs == 1 ? 0 : p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
-            const int pb = a.pairs == 1 ? 0 : p == 2 ? 2 : p == 1 || p == 4 ? 1 : 0;
-#pragma unroll 1
-            for (int kb = t.kb0; kb < t.kb1; kb++) {
-              if (!mbar_wait(empty + 8 * stage, phase ^ 1, dead, a.spin_limit)) {
-                on = false;
-                break;
-              }
-              const uint32_t bar = full + 8 * stage, sa = smem_u32(smem + stage * kStage), sb = sa + kBM * kBK * 2;
-              if (a.withhold && issued == 0) {  // this stage is never filled: its consumer's wait runs out
-                issued++;
-              } else {
-                mbar_expect(bar, kStage);
+          for (int kb = t.kb0; kb < t.kb1; kb++) {
+            if (!mbar_wait(empty + 8 * stage, phase ^ 1, dead, a.spin_limit)) {
+              on = false;
+              break;
+            }
+            const uint32_t bar = full + 8 * stage;
+            uint32_t at = smem_u32(smem + stage * kStage);
+            if (a.withhold && issued == 0) {  // this stage is never filled: its consumer's wait runs out
+              issued++;
+            } else {
+              mbar_expect(bar, kStage);
+#pragma unroll
+              for (int pl = 0; pl < PL; pl++) {
                 if (a.a_k_major) {
-                  tma_load(sa, &map_a, bar, kb * kBK, t.mt * kBM, pa);
+                  tma_load(at, &map_a, bar, kb * kBK, t.mt * kBM, pl);
                 } else {
 #pragma unroll
                   for (int j = 0; j < kBM / 64; j++)
-                    tma_load(sa + j * 8192, &map_a, bar, t.mt * kBM + j * 64, kb * kBK, pa);
+                    tma_load(at + j * 8192, &map_a, bar, t.mt * kBM + j * 64, kb * kBK, pl);
                 }
+                at += S::kTileA;
+              }
+#pragma unroll
+              for (int pl = 0; pl < PL; pl++) {
                 if (a.b_k_major) {
-                  tma_load(sb, &map_b, bar, kb * kBK, nt * BN, pb);
+                  tma_load(at, &map_b, bar, kb * kBK, nt * BN, pl);
                 } else {
 #pragma unroll
                   for (int j = 0; j < BN / 64; j++)
-                    tma_load(sb + j * 8192, &map_b, bar, nt * BN + j * 64, kb * kBK, pb);
+                    tma_load(at + j * 8192, &map_b, bar, nt * BN + j * 64, kb * kBK, pl);
                 }
-                issued++;
+                at += S::kTileB;
               }
-              if (++stage == kStages) stage = 0, phase ^= 1;
+              issued++;
             }
+            if (++stage == kStages) stage = 0, phase ^= 1;
           }
         }
       }
@@ -582,7 +591,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
 #pragma unroll 1
       for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
         const Item t = item_of<EPI>(a, i);
-        const int steps = a.pairs * (t.kb1 - t.kb0);
+        const int steps = t.kb1 - t.kb0;
 #pragma unroll 1
         for (int nt = t.nt; nt < t.nt_end && on; nt++) {
           if (!mbar_wait(tempty + 8 * acc, acc_phase ^ 1, dead, a.spin_limit)) {
@@ -598,11 +607,18 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>
               break;
             }
             fence_after();
-            const uint32_t sa = smem_u32(smem + stage * kStage);
-            const uint64_t da = smem_desc(sa, a.a_lbo), db = smem_desc(sa + kBM * kBK * 2, a.b_lbo);
+            const uint32_t sa = smem_u32(smem + stage * kStage), sb = sa + PL * S::kTileA;
+            // planes of the six products, smallest first: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+            constexpr int kPairs = PL == 3 ? 6 : 1;
 #pragma unroll
-            for (int k = 0; k < kBK / 16; k++)
-              mma_f16(d, da + k * a.a_step, db + k * a.b_step, a.idesc, s > 0 || k > 0);
+            for (int p = 0; p < kPairs; p++) {
+              const int pa = PL == 1 ? 0 : p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
+              const int pb = PL == 1 ? 0 : p == 2 ? 2 : p == 1 || p == 4 ? 1 : 0;
+              const uint64_t da = smem_desc(sa + pa * S::kTileA, a.a_lbo), db = smem_desc(sb + pb * S::kTileB, a.b_lbo);
+#pragma unroll
+              for (int k = 0; k < kBK / 16; k++)
+                mma_f16(d, da + k * a.a_step, db + k * a.b_step, a.idesc, s > 0 || p > 0 || k > 0);
+            }
             mma_commit(empty + 8 * stage);
             if (++stage == kStages) stage = 0, phase ^= 1;
           }
@@ -853,49 +869,54 @@ bool encode(CUtensorMap* map, const Operand& o, int planes, bool half, int box_r
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int BN, int EPI, int ACT>
+template <typename T, int BN, int EPI, int PL, int ACT>
 cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
-  auto* k = gemm_tc_kernel<T, BN, EPI, ACT>;
+  using S = Shape<T, BN, EPI, PL>;
+  auto* k = gemm_tc_kernel<T, BN, EPI, PL, ACT>;
   // once per device: the call costs as much as a launch
   static std::atomic<uint64_t> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (!(done.load(std::memory_order_relaxed) & bit)) {
-    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T, BN, EPI>::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return e;
     if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
   }
-  k<<<(unsigned)std::min<int64_t>(a.items, (int64_t)sms * Shape<T, BN, EPI>::kBlocks), Shape<T, BN, EPI>::kThreads, Shape<T, BN, EPI>::kSmem, s>>>(ma, mb, a);
+  k<<<(unsigned)std::min<int64_t>(a.items, (int64_t)sms * S::kBlocks), S::kThreads, S::kSmem, s>>>(ma, mb, a);
   return cudaPeekAtLastError();
 }
-template <typename T, int EPI, int ACT = VI_ACT_NONE>
+template <typename T, int EPI, int PL, int ACT = VI_ACT_NONE>
 cudaError_t run_bn(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
-  return bn == 256   ? run<T, 256, EPI, ACT>(ma, mb, a, sms, s)
-         : bn == 128 ? run<T, 128, EPI, ACT>(ma, mb, a, sms, s)
-                     : run<T, 64, EPI, ACT>(ma, mb, a, sms, s);
+  if constexpr (PL == 1)
+    if (bn == 256) return run<T, 256, EPI, PL, ACT>(ma, mb, a, sms, s);
+  return bn == 64 ? run<T, 64, EPI, PL, ACT>(ma, mb, a, sms, s) : run<T, 128, EPI, PL, ACT>(ma, mb, a, sms, s);
 }
 template <typename T>
 cudaError_t run_epi(int epi, int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms,
                     cudaStream_t s) {
+  constexpr int PL = sizeof(T) == 4 ? 3 : 1;
   switch (epi) {
     case kEpiAct:
       switch (a.e.act) {
-        case VI_ACT_RELU: return run_bn<T, kEpiAct, VI_ACT_RELU>(bn, ma, mb, a, sms, s);
-        case VI_ACT_SILU: return run_bn<T, kEpiAct, VI_ACT_SILU>(bn, ma, mb, a, sms, s);
-        case VI_ACT_GELU: return run_bn<T, kEpiAct, VI_ACT_GELU>(bn, ma, mb, a, sms, s);
-        case VI_ACT_SIGMOID: return run_bn<T, kEpiAct, VI_ACT_SIGMOID>(bn, ma, mb, a, sms, s);
-        default: return run_bn<T, kEpiAct>(bn, ma, mb, a, sms, s);
+        case VI_ACT_RELU: return run_bn<T, kEpiAct, PL, VI_ACT_RELU>(bn, ma, mb, a, sms, s);
+        case VI_ACT_SILU: return run_bn<T, kEpiAct, PL, VI_ACT_SILU>(bn, ma, mb, a, sms, s);
+        case VI_ACT_GELU: return run_bn<T, kEpiAct, PL, VI_ACT_GELU>(bn, ma, mb, a, sms, s);
+        case VI_ACT_SIGMOID: return run_bn<T, kEpiAct, PL, VI_ACT_SIGMOID>(bn, ma, mb, a, sms, s);
+        default: return run_bn<T, kEpiAct, PL>(bn, ma, mb, a, sms, s);
       }
-    case kEpiStore: return run_bn<T, kEpiStore>(bn, ma, mb, a, sms, s);
-    case kEpiLse: return run_bn<T, kEpiLse>(bn, ma, mb, a, sms, s);
-    default: return run_bn<T, kEpiGrad>(bn, ma, mb, a, sms, s);
+    case kEpiStore: return run_bn<T, kEpiStore, PL>(bn, ma, mb, a, sms, s);
+    case kEpiPartial: return run_bn<float, kEpiPartial, PL>(bn, ma, mb, a, sms, s);
+    case kEpiLse: return run_bn<T, kEpiLse, PL>(bn, ma, mb, a, sms, s);
+    default: return run_bn<T, kEpiGrad, PL>(bn, ma, mb, a, sms, s);
   }
 }
 
 }  // namespace
 
-int lse_parts(int bn) { return Shape<float, 256, kEpiLse>::kParts * (bn == 256) + Shape<float, 64, kEpiLse>::kParts * (bn != 256); }
+int lse_parts(int bn) { return Shape<__half, 64, kEpiLse, 1>::kParts * (bn == 256 ? 2 : 1); }
+static_assert(Shape<__half, 256, kEpiLse, 1>::kParts == 2 * Shape<__half, 64, kEpiLse, 1>::kParts &&
+              Shape<float, 128, kEpiLse, 3>::kParts == Shape<__half, 64, kEpiLse, 1>::kParts, "lse_parts");
 
 int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Plan& p, const Epilogue& e, int sms,
                 cudaStream_t s) {
@@ -914,7 +935,6 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
   a.splits = p.splits;
   a.span = p.span;
   a.spans = p.spans;
-  a.pairs = planes == 3 ? 6 : 1;
   a.a_k_major = A.k_major;
   a.b_k_major = B.k_major;
   // k contiguous: 16 k are 32 bytes of a swizzled row.  Rows contiguous: 16 k are two groups of 1024 bytes.
@@ -937,9 +957,7 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
   a.spin_limit = a.withhold ? 1u << 12 : kSpinLimit;
   a.e = e;
   cudaError_t rc;
-  if (epi == kEpiPartial)
-    rc = run_bn<float, kEpiPartial>(p.bn, ma, mb, a, sms, s);
-  else if (dtype == VI_F32)
+  if (dtype == VI_F32)
     rc = run_epi<float>(epi, p.bn, ma, mb, a, sms, s);
   else if (dtype == VI_F16)
     rc = run_epi<__half>(epi, p.bn, ma, mb, a, sms, s);
