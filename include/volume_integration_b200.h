@@ -371,8 +371,8 @@ int vi_linear_act_backward(int dtype, int activation, const vi_matrix* dy, const
  * hold.  Any other target outside [0, V) makes its row's loss NaN.  loss
  * (float32): [M] for VI_REDUCE_NONE, else one value, the sum over the rows or
  * their mean over the rows not ignored (NaN when there are none).  lse
- * (float32, [2][M]) is what the backward needs: each row's largest logit and the
- * base-2 logarithm of the sum of exp(z - largest).
+ * (float32, [3][M]) is what the backward needs: each row's largest logit, the
+ * base-2 logarithm of the sum of exp(z - largest), and the target's logit.
  */
 uint64_t vi_linear_ce_forward_scratch_bytes(int dtype, const vi_matrix* x, const vi_matrix* weight, const void* bias);
 int vi_linear_ce_forward(int dtype, const vi_matrix* x, const vi_matrix* weight, const void* bias,

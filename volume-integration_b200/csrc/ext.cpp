@@ -487,7 +487,7 @@ std::tuple<Tensor, Tensor> linear_ce_forward(const Tensor& x, const Tensor& weig
   const vi_matrix mx = head_matrix(x), mw = head_matrix(weight);
   const auto f32 = x.options().dtype(torch::kFloat32);
   Tensor loss = reduction == VI_REDUCE_NONE ? torch::empty({x.size(0)}, f32) : torch::empty({}, f32);
-  Tensor lse = torch::empty({2, x.size(0)}, f32);
+  Tensor lse = torch::empty({3, x.size(0)}, f32);
   const uint64_t n = vi_linear_ce_forward_scratch_bytes(dt, &mx, &mw, head_ptr(b));
   Tensor scratch = head_scratch(n, x);
   ok(vi_linear_ce_forward(dt, &mx, &mw, head_ptr(b), t.data_ptr<int64_t>(), ignore_index, (int)reduction,
@@ -505,7 +505,7 @@ Grads linear_ce_backward(const Tensor& x, const Tensor& weight, const c10::optio
   const int dt = head_dtype(x, "x");
   const Tensor b = head_bias(bias, x, weight), t = head_target(target, x);
   Tensor l = cuda_f32(lse, "lse"), dl = cuda_f32(dloss, "dloss");
-  TORCH_CHECK(l.numel() == 2 * x.size(0), "lse must be [2, ", x.size(0), "]");
+  TORCH_CHECK(l.numel() == 3 * x.size(0), "lse must be [3, ", x.size(0), "]");
   TORCH_CHECK(dl.numel() == (reduction == VI_REDUCE_NONE ? x.size(0) : 1), "dloss does not fit the reduction");
   const vi_matrix mx = head_matrix(x), mw = head_matrix(weight);
   GradTensors g(x, weight, need_x, need_w, need_b);

@@ -251,10 +251,11 @@ struct SumJobs {
   SumJob j[2];
 };
 
-// SPLIT threads share an element's pieces: 1 for few pieces, 8 (a block is 32 elements x 8) for many.
+// SPLIT threads share an element's pieces: 1 for few pieces, 32 (a block is 8 elements, a sector of
+// every piece) for many.
 template <typename T, int SPLIT>
 __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumJobs jobs) {
-  __shared__ float sh[8][33];
+  __shared__ float sh[SPLIT][256 / SPLIT + 1];
   const SumJob& q = jobs.j[blockIdx.y];
   const int64_t total = q.rows * q.cols;
   const bool by_col = q.out.cs == 1;
@@ -283,8 +284,8 @@ __global__ void __launch_bounds__(256) sum_kernel(const __grid_constant__ SumJob
 }
 
 // Rows' losses from the parts' maxima and sums; per block the sum of its rows' losses and their count (total not null: the one block's sum or mean itself).
-__global__ void __launch_bounds__(256) loss_kernel(const float* pmax, const float* psum, const float* ztarget,
-                                                   int parts, int64_t M, int64_t V, const int64_t* target,
+__global__ void __launch_bounds__(256) loss_kernel(const float* pmax, const float* psum, int parts,
+                                                   int64_t M, int64_t V, const int64_t* target,
                                                    int64_t ignore, float* rows, float* lse, float* bsum,
                                                    float* bcount, float* total, int mean) {
   __shared__ float sh[2][8];
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(256) loss_kernel(const float* pmax, const floa
     const bool ignored = t == ignore, bad = !ignored && (t < 0 || t >= V);
     lse[m] = top;
     lse[M + m] = bad ? NAN : l;
-    const float row = ignored ? 0.0f : bad ? NAN : fmaf(l, 0.6931471806f, top - ztarget[m]);
+    const float row = ignored ? 0.0f : bad ? NAN : fmaf(l, 0.6931471806f, top - lse[2 * M + m]);
     loss += row;
     live += ignored ? 0.0f : 1.0f;
     if (rows) rows[m] = row;
@@ -580,8 +581,8 @@ struct Summer {
   void run() {
     if (n && !r.dry) {
       if (shared) {
-        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(total, 32), 148 * 16), n);
-        VI_DISPATCH(dtype, (sum_kernel<T, 8><<<grid, 256, 0, r.s>>>(jobs)));
+        const dim3 grid((unsigned)std::min<int64_t>(ceil_div(total, 8), 148 * 16), n);
+        VI_DISPATCH(dtype, (sum_kernel<T, 32><<<grid, 256, 0, r.s>>>(jobs)));
       } else {
         const dim3 grid((unsigned)std::min<int64_t>(ceil_div(total, 256), 148 * 16), n);
         VI_DISPATCH(dtype, (sum_kernel<T, 1><<<grid, 256, 0, r.s>>>(jobs)));
@@ -815,7 +816,8 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
   Plan p{};
   p.splits = 1;
   p.kps = (int)ceil_div(K, 64);
-  p.bn = tile_width(dtype, M, V, r.sms);
+  // a small vocabulary in narrow tiles, two blocks per SM (640000 x 64 x 150: 88 us in one 256-wide tile, 81)
+  p.bn = V <= 64 ? 64 : V <= 256 ? 128 : tile_width(dtype, M, V, r.sms);
   // column tiles in runs, so that a block keeps a row's maximum and sum in registers over several of them
   const int64_t nt = ceil_div(V, p.bn), mt = std::max<int64_t>(1, ceil_div(M, 128));
   p.span = (int)ceil_div(nt, std::min(nt, ceil_div(4 * r.sms, mt)));
@@ -823,7 +825,6 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
   const int parts = lse_parts(p.bn) * p.spans;
   float* pmax = (float*)r.take((size_t)parts * M * 4);
   float* psum = (float*)r.take((size_t)parts * M * 4);
-  float* zt = (float*)r.take((size_t)M * 4);
   float* bsum = (float*)r.take((size_t)blocks * 4);
   float* bcount = (float*)r.take((size_t)blocks * 4);
   Operand A{}, B{};
@@ -839,11 +840,11 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
     e.bias = bias;
     e.pmax = pmax;
     e.psum = psum;
-    e.ztarget = zt;
+    e.ztarget = lse + 2 * M;
     e.target = target;
     if (int rc = launch_gemm(dtype, kEpiLse, A, B, p, e, r.sms, r.s)) return rc;
     const bool none = reduction == VI_REDUCE_NONE;
-    loss_kernel<<<(unsigned)blocks, 256, 0, r.s>>>(pmax, psum, zt, parts, M, V, target, ignore,
+    loss_kernel<<<(unsigned)blocks, 256, 0, r.s>>>(pmax, psum, parts, M, V, target, ignore,
                                                    none ? loss : nullptr, lse, none || blocks == 1 ? nullptr : bsum, bcount,
                                                    !none && blocks == 1 ? loss : nullptr, reduction == VI_REDUCE_MEAN);
     r.launches++;

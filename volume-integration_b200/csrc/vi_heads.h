@@ -53,7 +53,7 @@ struct Epilogue {
   float* ztarget;
   const int64_t* target;
   // kEpiGrad: columns [col0, col0 + N) of the vocabulary
-  const float* lse;     // [2][M]: the largest logit, and log2 of the sum of exp(z - largest)
+  const float* lse;     // [3][M]: the largest logit, log2 of the sum of exp(z - largest), the target's logit
   const float* coef;    // per row
   int64_t col0;
   void* grad;           // [planes][M][grad_ld], 16-bit

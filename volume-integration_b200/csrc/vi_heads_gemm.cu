@@ -409,10 +409,11 @@ __device__ __forceinline__ void own_row(Row<Z>& r, int way, uint32_t st, int lan
   }
 }
 
-// Writes each lane's row to a tile of v, one of whose strides is 1.
+// Writes each lane's row to a tile of v, one of whose strides is 1.  The cell `fix` of the
+// lane's row (none if negative; matrices with contiguous columns only) gets the value `with`.
 template <typename Z>
 __device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int access, uint32_t st, int lane,
-                                           const Place& t) {
+                                           const Place& t, int fix = -1, typename Row<Z>::Bits with = 0) {
   using G = Stage<Z>;
   Z* p = (Z*)v.p;
   const int line = lane / G::kLanes, piece = lane % G::kLanes;
@@ -449,6 +450,7 @@ __device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int a
   }
 #pragma unroll
   for (int i = 0; i < G::kLanes; i++) sts128(G::own(st, lane, i), r.q[i]);
+  if (fix >= 0) sts_cell(G::cell(st, lane, fix), with);
   __syncwarp();
   typename Row<Z>::Bits* q = (typename Row<Z>::Bits*)p + (int64_t)t.m0 * v.rs + (int64_t)t.n0 * v.cs;
   if (access == kVector && t.cols >= 32) {
@@ -471,6 +473,9 @@ __device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int a
     }
   }
 }
+
+__device__ __forceinline__ uint16_t bits_of(__half v) { return __half_as_ushort(v); }
+__device__ __forceinline__ uint16_t bits_of(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 
 // v += COLS values of a bias slot.
 template <int COLS>
@@ -651,12 +656,17 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
       const int rows = min(32, a.M - m0);
       auto place = [&](int n0) { return Place{m0, n0, rows, min(32, a.N - n0)}; };
       float top = -INFINITY, sum = 0.0f;
-      int64_t target = -1;
-      float lsum = 0.0f, coef = 0.0f, alpha = 1.0f;
-      if (EPI == kEpiLse || EPI == kEpiGrad) {
-        if (m < a.M) target = e.target[m] - (EPI == kEpiGrad ? e.col0 : 0);
+      int target = -1;  // its column, if it is one of these
+      float lsum = 0.0f, coef = 0.0f, alpha = 1.0f, gtarget = 0.0f;
+      if ((EPI == kEpiLse || EPI == kEpiGrad) && m < a.M) {
+        const int64_t c = e.target[m] - (EPI == kEpiGrad ? e.col0 : 0);
+        if (c >= 0 && c < a.N) target = (int)c;
       }
-      if (EPI == kEpiGrad && m < a.M) top = e.lse[m], lsum = e.lse[a.M + m], coef = e.coef[m];
+      if (EPI == kEpiGrad && m < a.M) {
+        top = e.lse[m], lsum = e.lse[a.M + m], coef = e.coef[m];
+        // the target's gradient from the forward's logit, once a row
+        gtarget = coef == 0.0f ? 0.0f : coef * (exp2_fast(fmaf(e.lse[2 * (int64_t)a.M + m] - top, kLog2e, -lsum)) - 1.0f);
+      }
       if (EPI == kEpiStore && e.alpha) alpha = *e.alpha;
       float row_bias = 0.0f;
       if (EPI == kEpiAct && e.bias_rows && m < a.M) row_bias = to_f(((const T*)e.bias)[m]);
@@ -752,29 +762,38 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
             tmem_wait_load();
             if (e.bias) add_bias<32>(bias_slot, v);
             float* z = (float*)v;
-            if (__any_sync(0xffffffffu, target >= n0 && target < n0 + 32)) {
+            const int tc = target - n0;
+            if (__any_sync(0xffffffffu, tc >= 0 && tc < 32)) {  // the target's logit, by halves
+              float u[16];
 #pragma unroll
-              for (int j = 0; j < 32; j++)
-                if (target == n0 + j && n0 + j < a.N) e.ztarget[m] = z[j];
+              for (int j = 0; j < 16; j++) u[j] = tc & 16 ? z[j + 16] : z[j];
+#pragma unroll
+              for (int h = 8; h; h /= 2)
+#pragma unroll
+                for (int j = 0; j < h; j++) u[j] = tc & h ? u[j + h] : u[j];
+              if (tc >= 0 && tc < 32) e.ztarget[m] = u[0];
             }
             if (n0 + 32 > a.N) {
 #pragma unroll
               for (int j = 0; j < 32; j++)
                 if (n0 + j >= a.N) z[j] = -INFINITY;
             }
-            float best = top;
+            float u[8];  // several chains: one of 32 dependent steps would be waited for
 #pragma unroll
-            for (int j = 0; j < 32; j++) best = fmaxf(best, z[j]);
+            for (int j = 0; j < 8; j++) u[j] = fmaxf(fmaxf(z[j], z[j + 8]), fmaxf(z[j + 16], z[j + 24]));
+            const float best = fmaxf(fmaxf(fmaxf(fmaxf(u[0], u[1]), fmaxf(u[2], u[3])), top),
+                                     fmaxf(fmaxf(u[4], u[5]), fmaxf(u[6], u[7])));
             // a row of -inf so far: leave the sum at zero, without -inf - -inf
             const float ref = best == -INFINITY ? 0.0f : best;
-            float2 s2 = pair(0.0f);
+            float2 s2[4] = {pair(0.0f), pair(0.0f), pair(0.0f), pair(0.0f)};
 #pragma unroll
             for (int j = 0; j < 16; j++) {
               // the difference first: a logit of the type's lowest value times log2(e) would overflow
               const float2 x = __fmul2_rn(__fadd2_rn(v[j], pair(-ref)), pair(kLog2e));
-              s2 = __fadd2_rn(s2, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+              s2[j % 4] = __fadd2_rn(s2[j % 4], make_float2(exp2_fast(x.x), exp2_fast(x.y)));
             }
-            sum = sum * exp2_fast((top - ref) * kLog2e) + (s2.x + s2.y);
+            const float2 all = __fadd2_rn(__fadd2_rn(s2[0], s2[1]), __fadd2_rn(s2[2], s2[3]));
+            sum = sum * exp2_fast((top - ref) * kLog2e) + (all.x + all.y);
             top = best;
           } else if constexpr (EPI == kEpiGrad) {
             float2 v[16];
@@ -787,11 +806,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
               const float2 x = __ffma2_rn(__fadd2_rn(v[j], pair(-top)), pair(kLog2e), pair(-lsum));
               v[j] = make_float2(exp2_fast(x.x), exp2_fast(x.y));
             }
-            if (__any_sync(0xffffffffu, target >= n0 && target < n0 + 32)) {
-#pragma unroll
-              for (int j = 0; j < 32; j++)
-                if (target == n0 + j) z[j] -= 1.0f;
-            }
+            const int fix = target >= n0 && target < n0 + 32 ? target - n0 : -1;
 #pragma unroll
             for (int j = 0; j < 16; j++) v[j] = __fmul2_rn(v[j], pair(coef));
             if (__any_sync(0xffffffffu, coef == 0.0f)) {  // an ignored row's logits may be anything
@@ -809,13 +824,15 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
                   g.z[j] = s3[pl];
                 }
                 const View out{(__nv_bfloat16*)e.grad + pl * e.grad_plane, e.grad_ld, 1};
-                store_tile(g, out, kVector, st, lane, here);
+                __nv_bfloat16 t3[3];
+                split3(gtarget, t3);
+                store_tile(g, out, kVector, st, lane, here, fix, __bfloat16_as_ushort(t3[pl]));
               }
             } else {
               Row<T> g;
 #pragma unroll
               for (int j = 0; j < 16; j++) set_pair(g, j, v[j]);
-              store_tile(g, View{e.grad, e.grad_ld, 1}, kVector, st, lane, here);
+              store_tile(g, View{e.grad, e.grad_ld, 1}, kVector, st, lane, here, fix, bits_of(from_f<T>(gtarget)));
             }
           }
         }
