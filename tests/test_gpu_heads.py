@@ -156,6 +156,18 @@ def test_linear_act_strided_weight_and_shared_inputs(dt):
     hl.assert_within("shared bias", g1[0], (v, bound + hl.last(dt, v.abs() + bound) + 64 * hl.E * want[3][0].abs().sum()))
 
 
+@pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("M,K,N,act,order,bias,residual", [
+    (4100, 72, 1100, "silu", "rows", True, True),
+    (4099, 136, 1030, "gelu", "image", True, True),   # few more rows than tiles, an odd image
+    (9000, 1100, 700, "relu", "padded", True, False),
+    (5000, 2100, 1000, "none", "rows", False, False),
+])
+def test_linear_act_tiles_of_two_blocks(M, K, N, act, order, bias, residual, dt):
+    # enough tiles that every product takes 256 x 256 ones, made by pairs of blocks
+    _act_check(*_act_inputs(M, K, N, dt, order, bias, residual, M + K + N), act)
+
+
 def test_linear_act_gradient_against_differences():
     # float32: (f(p + h) - f(p - h)) / 2h of the kernel's own output, h = 2^-6, with a
     # smooth activation.  Truncation: h^2/6 times the third derivative along the direction;
@@ -297,10 +309,17 @@ def test_linear_cross_entropy(M, K, V, order, bias, ignored, reduction, dt):
     _ce_check(*_ce_inputs(M, K, V, dt, order, bias, ignored, M + V), reduction)
 
 
-@pytest.mark.parametrize("dt,V", [(F32, 4001), (F16, 9001), (BF16, 9001)], ids=["f32", "f16", "bf16"])
-def test_linear_cross_entropy_in_several_pieces(dt, V):
+@pytest.mark.parametrize("dt,M,V", [(F32, 30000, 4001), (F16, 40000, 9001), (BF16, 40000, 9001)],
+                         ids=["f32", "f16", "bf16"])
+def test_linear_cross_entropy_in_several_pieces(dt, M, V):
     # the gradient of the logits of this many rows does not exist at once
-    _ce_check(*_ce_inputs(30000, 24, V, dt, "rows", True, 0.1, 31), "mean")
+    _ce_check(*_ce_inputs(M, 24, V, dt, "rows", True, 0.1, 31), "mean")
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("M,K,V,order,reduction", [(4100, 300, 4100, "rows", "mean"), (3001, 130, 9999, "image", "none")])
+def test_linear_cross_entropy_tiles_of_two_blocks(M, K, V, order, reduction, dt):
+    _ce_check(*_ce_inputs(M, K, V, dt, order, True, 0.1, 32), reduction)
 
 
 @pytest.mark.parametrize("dt", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
@@ -588,15 +607,16 @@ def test_offsets_beyond_32_bits():
 def test_a_wait_that_runs_out_is_reported(monkeypatch):
     # the first load is withheld and the waits are short: the kernel gives up and says so
     import volume_integration.heads as heads
-    x, w, _, _, _ = _act_inputs(300, 200, 100, BF16, "rows", False, False, 28)
-    want = heads.linear_act(x, w)
-    assert heads.device_status(reset=True) == 0
-    monkeypatch.setenv("VI_HEADS_TEST_TIMEOUT", "1")
-    heads.linear_act(x, w)
-    assert heads.device_status(reset=True) == 8
-    monkeypatch.delenv("VI_HEADS_TEST_TIMEOUT")
-    assert torch.equal(heads.linear_act(x, w), want)  # and nothing is left behind
-    assert heads.device_status() == 0
+    for M, K, N in ((300, 200, 100), (4100, 200, 1100)):  # tiles of one block, and of two
+        x, w, _, _, _ = _act_inputs(M, K, N, BF16, "rows", False, False, 28)
+        want = heads.linear_act(x, w)
+        assert heads.device_status(reset=True) == 0
+        monkeypatch.setenv("VI_HEADS_TEST_TIMEOUT", "1")
+        heads.linear_act(x, w)
+        assert heads.device_status(reset=True) == 8
+        monkeypatch.delenv("VI_HEADS_TEST_TIMEOUT")
+        assert torch.equal(heads.linear_act(x, w), want)  # and nothing is left behind
+        assert heads.device_status() == 0
 
 
 def test_gradients_reach_the_renderer():

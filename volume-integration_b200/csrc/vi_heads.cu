@@ -427,7 +427,7 @@ int sm_count() {
 }
 
 // Bytes of the logits' gradient that exist at a time, if 256 columns fit.
-constexpr int64_t kPieceBytes = 512ll << 20;
+constexpr int64_t kPieceBytes = 640ll << 20;
 
 struct Run {
   char* base;
@@ -512,15 +512,18 @@ struct Packer {
   }
 };
 
+// Tiles of a width, and how many of them run at a time.
+int64_t tiles_of(int epi, int64_t M, int64_t N, int bn) { return ceil_div(M, pair_tile(epi, bn) ? 256 : 128) * ceil_div(N, bn); }
+int64_t tile_slots(int epi, int bn, int sms) { return std::max(1, pair_tile(epi, bn) ? sms / 2 : sms); }
+
 // Tile width: the one whose waves of tiles take the least tensor-core time; narrow tiles
 // read their operands more often.
-int tile_width(int dtype, int64_t M, int64_t N, int sms) {
-  const int64_t mt = ceil_div(M, 128);
+int tile_width(int dtype, int epi, int64_t M, int64_t N, int sms) {
   int best = 64;
   double cost = 1e300;
   for (int bn : {256, 128, 64}) {
-    if (bn == 256 && dtype == VI_F32) continue;
-    const double c = (double)ceil_div(mt * ceil_div(N, bn), sms) * (bn == 256 ? 256 : bn == 128 ? 150 : 90);
+    if (bn == 256 && (dtype == VI_F32 || (pair_tile(epi, bn) && M <= 128))) continue;
+    const double c = (double)ceil_div(tiles_of(epi, M, N, bn), tile_slots(epi, bn, sms)) * (bn == 256 ? 240 : bn == 128 ? 150 : 90);
     if (c < cost) cost = c, best = bn;
   }
   return best;
@@ -538,25 +541,37 @@ int gemm(Run& r, int dtype, int epi, const Operand& A, const Operand& B, const E
     f.res = transposed(e.res);
     f.bias_rows = e.bias != nullptr;
     Plan p{};
-    p.bn = tile_width(dtype, B.rows, A.rows, r.sms);
+    p.bn = tile_width(dtype, epi, B.rows, A.rows, r.sms);
     p.splits = 1;
     p.kps = (int)ceil_div(A.k, 64);
     return launch_gemm(dtype, epi, B, A, p, f, r.sms, r.s);
   }
   Plan p{};
-  p.bn = tile_width(dtype, A.rows, B.rows, r.sms);
+  p.bn = tile_width(dtype, epi, A.rows, B.rows, r.sms);
   p.splits = 1;
   p.kps = (int)ceil_div(A.k, 64);
   return launch_gemm(dtype, epi, A, B, p, e, r.sms, r.s);
 }
 
-// Pieces of a long sum over k when there are few tiles.
+// Pieces of a long sum over k: enough that the tiles fill the SMs, or fill their last wave where
+// that gains more than the pieces' float32 results cost to write and read (16384 x 512 over
+// 18944: 1.73 waves of tiles in one piece, 3.46 in two; 240 us -> 217).
 Plan split_plan(int dtype, const Operand& A, const Operand& B, int sms) {
   Plan p{};
-  p.bn = B.rows <= 64 ? 64 : B.rows <= 128 || dtype == VI_F32 ? 128 : 256;
-  const int64_t tiles = ceil_div(A.rows, 128) * ceil_div(B.rows, p.bn), kb = ceil_div(A.k, 64);
-  // at least four blocks of k each, at most one piece per SM and tile
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(sms / std::min<int64_t>(tiles, sms), kb / 4));
+  p.bn = B.rows <= 64 ? 64 : B.rows <= 128 || A.rows <= 128 || dtype == VI_F32 ? 128 : 256;
+  const int64_t tiles = tiles_of(kEpiPartial, A.rows, B.rows, p.bn), slots = tile_slots(kEpiPartial, p.bn, sms), kb = ceil_div(A.k, 64);
+  int64_t want = 1;
+  if (tiles < slots) {
+    want = std::max<int64_t>(1, std::min<int64_t>(slots / tiles, kb / 4));  // at least four blocks of k each
+  } else {
+    const double product = 2.0 * A.rows * B.rows * A.k * (dtype == VI_F32 ? 6 : 1) / 1.3e15, copy = 8.0 * A.rows * B.rows / 5e12;
+    double best = 1e300;
+    for (int64_t s = 1; s <= 4 && kb / s >= 32; s++) {
+      const double waves = (double)(ceil_div(tiles * s, slots) * slots) / (double)(tiles * s);
+      const double t = product * waves + (s > 1 ? copy * s : 0.0);
+      if (t < best) best = t, want = s;
+    }
+  }
   p.kps = (int)ceil_div(kb, want);
   p.splits = (int)ceil_div(kb, p.kps);
   return p;
@@ -817,7 +832,7 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
   p.splits = 1;
   p.kps = (int)ceil_div(K, 64);
   // a small vocabulary in narrow tiles, two blocks per SM (640000 x 64 x 150: 88 us in one 256-wide tile, 81)
-  p.bn = V <= 64 ? 64 : V <= 256 ? 128 : tile_width(dtype, M, V, r.sms);
+  p.bn = V <= 64 ? 64 : V <= 256 ? 128 : tile_width(dtype, kEpiLse, M, V, r.sms);
   // column tiles in runs, so that a block keeps a row's maximum and sum in registers over several of them
   const int64_t nt = ceil_div(V, p.bn), mt = std::max<int64_t>(1, ceil_div(M, 128));
   p.span = (int)ceil_div(nt, std::min(nt, ceil_div(4 * r.sms, mt)));
@@ -894,7 +909,12 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
   pk.run();
 
   // G in pieces of the vocabulary
-  const int64_t piece = std::min(V, std::max<int64_t>(256, kPieceBytes / (M * 2 * planes) / 256 * 256));
+  int64_t piece = std::max<int64_t>(256, kPieceBytes / (M * 2 * planes) / 256 * 256);
+  if (piece < V && dtype != VI_F32 && K > 128) {  // whole waves of dweight's 256 x 256 tiles
+    const int64_t nt = ceil_div(K, 256), slots = tile_slots(kEpiStore, 256, r.sms), waves = piece / 256 * nt / slots;
+    if (waves) piece = waves * slots / nt * 256;
+  }
+  piece = std::min(piece, V);
   const int64_t ld = ceil_div(piece, 8) * 8;
   void* grad = r.take((size_t)planes * M * ld * 2);
   const bool several = piece < V;

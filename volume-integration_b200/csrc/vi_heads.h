@@ -36,6 +36,14 @@ enum Epi {
   kEpiCount
 };
 
+// Whether a tile is 256 rows high and made by a pair of blocks.  The softmax's are not: its epilogue
+// is the longer part, and two blocks that wait for each other's lose (K = 512: statistics 904 us
+// apart, 974 in pairs; gradient 1027, 1095; the plain products 974, 921).
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+constexpr bool pair_tile(int epi, int bn) { return bn == 256 && epi != kEpiLse && epi != kEpiGrad; }
+
 // What happens to the product acc(m, n) = sum_k A(m, k) B(n, k).
 struct Epilogue {
   int act;              // kEpiAct: vi_activation

@@ -3,7 +3,7 @@
 //
 // Persistent blocks.  One warp copies 64-wide blocks of k of both operands into a ring
 // of shared-memory stages (cp.async.bulk.tensor, 128-byte swizzle), one issues
-// tcgen05.mma on them (128 x BN x 16, float32 accumulators in tensor memory), 8 or 16
+// tcgen05.mma on them (128 x BN x 16, or 256 x 256 x 16 by a pair of blocks, float32 accumulators in tensor memory), 8 or 16
 // take finished accumulators out of tensor memory and run the epilogue.  Two accumulators alternate, so the epilogue of one tile
 // overlaps the product of the next.  Either operand may have k or its rows
 // contiguous: both are layouts the tensor core reads, so a backward product
@@ -33,28 +33,31 @@ namespace heads {
 namespace {
 
 constexpr int kBM = 128, kBK = 64;
-constexpr uint32_t kSpinLimit = 1u << 24;
+constexpr int64_t kWaitLimit = 8ll << 30;  // cycles, about 4 s
 
 __device__ uint32_t g_status;  // VI_DEVICE_HEAD_TIMEOUT when a wait ran out
 
 // Narrow tiles belong to products that memory bounds (few columns, short sums): two
 // blocks per SM, so that one's epilogue runs while the other waits for memory.  A
-// 256-wide tile takes all tensor memory (two accumulators) and the SM for itself.
+// 256-wide tile takes all tensor memory (two accumulators) and its SMs for itself.
 // PL planes of both operands share a stage, so that the six products of float32's are made of
 // each copied block once.
 template <typename T, int BN, int EPI, int PL>
 struct Shape {
   static_assert(PL == 1 || BN <= 128, "three planes of a 256-wide tile leave no second stage");
+  // 256-wide tiles are 256 rows high and made by two blocks on neighbouring SMs (cta_group::2): each copies
+  // its 128 rows of A and half of B, which the other's tensor core reads too
+  static constexpr bool kPair = pair_tile(EPI, BN);
   static constexpr int kBlocks = BN == 256 || PL == 3 ? 1 : 2;
   // Epilogue warps.  The softmax on a 256-wide tile has 16: with 8 its latency, not its
   // instructions, bound it (K = 256: gradient 289 us with 8, 230 with 16; statistics 207, 159).
   static constexpr int kWarps = BN == 256 && (EPI == kEpiLse || EPI == kEpiGrad) ? 16 : 8;
   static constexpr int kParts = kWarps / 4;  // warps that share a tile's columns, 32 at a time
   static constexpr int kThreads = (kWarps + 2) * 32;
-  static constexpr int kTileA = kBM * kBK * 2, kTileB = BN * kBK * 2;  // bytes of a plane
+  static constexpr int kTileA = kBM * kBK * 2, kTileB = BN / (kPair ? 2 : 1) * kBK * 2;  // bytes of a plane
   static constexpr int kStage = PL * (kTileA + kTileB);
   static constexpr int kStages = PL == 3   ? 2
-                                 : BN == 256 ? 4
+                                 : BN == 256 ? (kPair ? 6 : 4)
                                  : BN == 128 ? (kBlocks == 2 ? 2 : 5)
                                              : (kBlocks == 2 ? 3 : 7);
   static constexpr int kStageWarp = EPI == kEpiLse ? 0 : 32 * 32 * (int)sizeof(T);  // an epilogue warp's staging
@@ -89,7 +92,7 @@ struct Args {
   int items;
   FastDiv per_split, per_group;  // items of one piece of the sum; of 16 row tiles
   FastDiv last_rows;             // row tiles of the last group
-  uint32_t spin_limit;
+  int64_t wait_limit;    // cycles
   int withhold;          // testing hook: the first load is never issued
   Epilogue e;
 };
@@ -109,26 +112,57 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 0x989680;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
       : "memory");
   return ok;
 }
-// Waits for the phase of `parity` to end.  False when the block has given up (*dead) or
-// the limit ran out, which sets *dead.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead, uint32_t limit) {
+// Waits for the phase of `parity` to end (each try is suspended for up to 20 us).  False when the
+// block has given up (*dead) or `limit` cycles have gone, which sets *dead.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead, int64_t limit) {
+  if (mbar_try(bar, parity)) return true;
+  const int64_t start = clock64();
 #pragma unroll 1
-  for (uint32_t i = 0; i < limit; i++) {
+  while (!*dead) {
     if (mbar_try(bar, parity)) return true;
-    if ((i & 63) == 63 && *dead) return false;
+    if (clock64() - start > limit) *dead = 1;
   }
-  *dead = 1;
   return false;
 }
+// The same when the block has given up already: only the limit counts.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, int64_t limit) {
+  const int64_t start = clock64();
+#pragma unroll 1
+  while (!mbar_try(bar, parity) && clock64() - start <= limit) {
+  }
+}
 
+// Address of the same shared-memory location in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t at_rank(uint32_t a, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// PAIR: the barrier may be the other block's.
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  if constexpr (PAIR) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+        "[%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+    return;
+  }
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
           dst),
@@ -170,7 +204,17 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo) {
   return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)lbo << 16) | ((uint64_t)(1024 >> 4) << 32) |
          (1ull << 46) | (2ull << 61);
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (PAIR) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+    return;
+  }
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
@@ -178,7 +222,16 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// Arrives at the barrier (of both blocks of a pair) when the products issued so far have ended.
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
+  if constexpr (PAIR) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+    return;
+  }
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // 32 columns of this warp's 32 lanes of tensor memory.
@@ -510,19 +563,31 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(tfull + 8 * i, 1);
-      mbar_init(tempty + 8 * i, kEpiWarps);
+      mbar_init(tempty + 8 * i, S::kPair ? 2 * kEpiWarps : kEpiWarps);
     }
     mbar_init(drain, 1);
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kEpiWarps + 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (S::kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(kCols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
+  // a pair's blocks: rank 0 issues the products of both; its barriers count both blocks' copies and epilogues
+  uint32_t rank = 0;
+  if constexpr (S::kPair) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int first_item = S::kPair ? blockIdx.x / 2 : blockIdx.x, item_step = S::kPair ? gridDim.x / 2 : gridDim.x;
   fence_before();
-  __syncthreads();
+  __syncwarp();
+  if constexpr (S::kPair) cluster_sync();
+  else __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
 
@@ -534,41 +599,44 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
       int64_t issued = 0;
       bool on = true;
 #pragma unroll 1
-      for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
+      for (int i = first_item; i < a.items && on; i += item_step) {
         const Item t = item_of<EPI>(a, i);
 #pragma unroll 1
         for (int nt = t.nt; nt < t.nt_end && on; nt++) {
+          const int row = S::kPair ? (2 * t.mt + (int)rank) * kBM : t.mt * kBM;
+          const int column = S::kPair ? nt * BN + (int)rank * (BN / 2) : nt * BN;
 #pragma unroll 1
           for (int kb = t.kb0; kb < t.kb1; kb++) {
-            if (!mbar_wait(empty + 8 * stage, phase ^ 1, dead, a.spin_limit)) {
+            if (!mbar_wait(empty + 8 * stage, phase ^ 1, dead, a.wait_limit)) {
               on = false;
               break;
             }
-            const uint32_t bar = full + 8 * stage;
+            uint32_t bar = full + 8 * stage;
+            if constexpr (S::kPair) bar = at_rank(bar, 0);
             uint32_t at = smem_u32(smem + stage * kStage);
             if (a.withhold && issued == 0) {  // this stage is never filled: its consumer's wait runs out
               issued++;
             } else {
-              mbar_expect(bar, kStage);
+              if (rank == 0) mbar_expect(full + 8 * stage, S::kPair ? 2 * kStage : kStage);
 #pragma unroll
               for (int pl = 0; pl < PL; pl++) {
                 if (a.a_k_major) {
-                  tma_load(at, &map_a, bar, kb * kBK, t.mt * kBM, pl);
+                  tma_load<S::kPair>(at, &map_a, bar, kb * kBK, row, pl);
                 } else {
 #pragma unroll
                   for (int j = 0; j < kBM / 64; j++)
-                    tma_load(at + j * 8192, &map_a, bar, t.mt * kBM + j * 64, kb * kBK, pl);
+                    tma_load<S::kPair>(at + j * 8192, &map_a, bar, row + j * 64, kb * kBK, pl);
                 }
                 at += S::kTileA;
               }
 #pragma unroll
               for (int pl = 0; pl < PL; pl++) {
                 if (a.b_k_major) {
-                  tma_load(at, &map_b, bar, kb * kBK, nt * BN, pl);
+                  tma_load<S::kPair>(at, &map_b, bar, kb * kBK, column, pl);
                 } else {
 #pragma unroll
-                  for (int j = 0; j < BN / 64; j++)
-                    tma_load(at + j * 8192, &map_b, bar, nt * BN + j * 64, kb * kBK, pl);
+                  for (int j = 0; j < BN / 64 / (S::kPair ? 2 : 1); j++)
+                    tma_load<S::kPair>(at + j * 8192, &map_b, bar, column + j * 64, kb * kBK, pl);
                 }
                 at += S::kTileB;
               }
@@ -578,28 +646,27 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
           }
         }
       }
-      if (*dead) {  // wait for the copies in flight: the last fill of every stage
+      if (*dead && rank == 0) {  // wait for the copies in flight (a pair's: both blocks'): the last fill of every stage
         for (int j = 0; j < kStages && j < issued; j++) {
           const int64_t f = issued - 1 - j;  // fill number: stage f % kStages, phase (f / kStages) & 1
           if (a.withhold && f == 0) continue;
-          for (uint32_t n = 0; n < a.spin_limit && !mbar_try(full + 8 * (uint32_t)(f % kStages), (uint32_t)(f / kStages) & 1); n++) {
-          }
+          mbar_drain(full + 8 * (uint32_t)(f % kStages), (uint32_t)(f / kStages) & 1, a.wait_limit);
         }
       }
     }
   } else if (warp == kEpiWarps + 1) {
     // ---- products ----
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool on = true;
 #pragma unroll 1
-      for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
+      for (int i = first_item; i < a.items && on; i += item_step) {
         const Item t = item_of<EPI>(a, i);
         const int steps = t.kb1 - t.kb0;
 #pragma unroll 1
         for (int nt = t.nt; nt < t.nt_end && on; nt++) {
-          if (!mbar_wait(tempty + 8 * acc, acc_phase ^ 1, dead, a.spin_limit)) {
+          if (!mbar_wait(tempty + 8 * acc, acc_phase ^ 1, dead, a.wait_limit)) {
             on = false;
             break;
           }
@@ -607,7 +674,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
           const uint32_t d = tmem + acc * BN;
 #pragma unroll 1
           for (int s = 0; s < steps; s++) {
-            if (!mbar_wait(full + 8 * stage, phase, dead, a.spin_limit)) {
+            if (!mbar_wait(full + 8 * stage, phase, dead, a.wait_limit)) {
               on = false;
               break;
             }
@@ -622,20 +689,19 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
               const uint64_t da = smem_desc(sa + pa * S::kTileA, a.a_lbo), db = smem_desc(sb + pb * S::kTileB, a.b_lbo);
 #pragma unroll
               for (int k = 0; k < kBK / 16; k++)
-                mma_f16(d, da + k * a.a_step, db + k * a.b_step, a.idesc, s > 0 || p > 0 || k > 0);
+                mma_f16<S::kPair>(d, da + k * a.a_step, db + k * a.b_step, a.idesc, s > 0 || p > 0 || k > 0);
             }
-            mma_commit(empty + 8 * stage);
+            mma_commit<S::kPair>(empty + 8 * stage);
             if (++stage == kStages) stage = 0, phase ^= 1;
           }
           if (!on) break;
-          mma_commit(tfull + 8 * acc);
+          mma_commit<S::kPair>(tfull + 8 * acc);
           if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
       }
       if (*dead) {
-        mma_commit(drain);
-        for (uint32_t n = 0; n < a.spin_limit && !mbar_try(drain, 0); n++) {
-        }
+        mma_commit<S::kPair>(drain);
+        mbar_drain(drain, 0, a.wait_limit);
       }
     }
   } else {
@@ -650,9 +716,9 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
     uint32_t acc_phase = 0;
     bool on = true;
 #pragma unroll 1
-    for (int i = blockIdx.x; i < a.items && on; i += gridDim.x) {
+    for (int i = first_item; i < a.items && on; i += item_step) {
       const Item t = item_of<EPI>(a, i);
-      const int m0 = t.mt * kBM + quad * 32, m = m0 + lane;
+      const int m0 = (S::kPair ? 2 * t.mt + (int)rank : t.mt) * kBM + quad * 32, m = m0 + lane;
       const int rows = min(32, a.M - m0);
       auto place = [&](int n0) { return Place{m0, n0, rows, min(32, a.N - n0)}; };
       float top = -INFINITY, sum = 0.0f;
@@ -681,7 +747,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
         if (EPI == kEpiPartial && e.add) add = View{e.part + (int64_t)t.split * a.M * a.N, a.N, 1};
         bool waited = false;
         auto wait_product = [&] {
-          if (!mbar_wait(tfull + 8 * acc, acc_phase, dead, a.spin_limit)) on = false;
+          if (!mbar_wait(tfull + 8 * acc, acc_phase, dead, a.wait_limit)) on = false;
           on = __all_sync(0xffffffffu, on);
           fence_after();
           waited = true;
@@ -840,7 +906,10 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
         if (!on) break;
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(tempty + 8 * acc);
+        if (lane == 0) {
+          if constexpr (S::kPair) mbar_arrive_cluster(at_rank(tempty + 8 * acc, 0));
+          else mbar_arrive(tempty + 8 * acc);
+        }
         if (++acc == 2) acc = 0, acc_phase ^= 1;
       }
       if (EPI == kEpiLse && on && m < a.M) {
@@ -850,9 +919,15 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
     }
   }
   __syncwarp();
-  __syncthreads();
-  if (warp == kEpiWarps + 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+  // a pair ends together: its blocks arrive at each other's barriers
+  if constexpr (S::kPair) cluster_sync();
+  else __syncthreads();
+  if (warp == kEpiWarps + 1) {
+    if constexpr (S::kPair)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+  }
   if (threadIdx.x == 0 && *dead) atomicOr(&g_status, VI_DEVICE_HEAD_TIMEOUT);
 }
 
@@ -900,8 +975,23 @@ cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int
     if (e != cudaSuccess) return e;
     if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
   }
-  k<<<(unsigned)std::min<int64_t>(a.items, (int64_t)sms * S::kBlocks), S::kThreads, S::kSmem, s>>>(ma, mb, a);
-  return cudaPeekAtLastError();
+  if constexpr (S::kPair) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(2 * (unsigned)std::min<int64_t>(a.items, std::max(1, sms / 2)));
+    c.blockDim = dim3(S::kThreads);
+    c.dynamicSmemBytes = S::kSmem;
+    c.stream = s;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    c.attrs = &attr;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, k, ma, mb, a);
+  } else {
+    k<<<(unsigned)std::min<int64_t>(a.items, (int64_t)sms * S::kBlocks), S::kThreads, S::kSmem, s>>>(ma, mb, a);
+    return cudaPeekAtLastError();
+  }
 }
 template <typename T, int EPI, int PL, int ACT = VI_ACT_NONE>
 cudaError_t run_bn(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
@@ -939,13 +1029,15 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
                 cudaStream_t s) {
   const int planes = dtype == VI_F32 ? 3 : 1;
   const bool half = dtype == VI_F16;
+  const bool pair = pair_tile(epi, p.bn);
   CUtensorMap ma, mb;
-  if (!encode(&ma, A, planes, half, kBM) || !encode(&mb, B, planes, half, p.bn))
+  if (!encode(&ma, A, planes, half, kBM) || !encode(&mb, B, planes, half, pair ? 128 : p.bn))
     return set_error(VI_ERR_CUDA, "heads: a tensor map could not be encoded");
   Args a{};
   a.M = (int)A.rows;
   a.N = (int)B.rows;
-  a.m_tiles = (int)((A.rows + kBM - 1) / kBM);
+  const int64_t rows = pair ? 2 * kBM : kBM;  // of a tile
+  a.m_tiles = (int)((A.rows + rows - 1) / rows);
   a.n_tiles = (int)((B.rows + p.bn - 1) / p.bn);
   a.kblocks = (int)((A.k + kBK - 1) / kBK);
   a.kps = p.kps;
@@ -961,7 +1053,7 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
   a.b_step = B.k_major ? 32 >> 4 : 2048 >> 4;
   const uint32_t type = half ? 0 : 1;
   a.idesc = (1u << 4) | (type << 7) | (type << 10) | ((A.k_major ? 0u : 1u) << 15) | ((B.k_major ? 0u : 1u) << 16) |
-            ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+            ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(rows >> 4) << 24);
   const int64_t cols = epi == kEpiLse ? p.spans : a.n_tiles, items = (int64_t)a.m_tiles * cols * p.splits;
   if (items > INT32_MAX - 65536 || 16 * cols > INT32_MAX)
     return set_error(VI_ERR_UNSUPPORTED, "heads: more than 2^31 tiles");
@@ -971,7 +1063,7 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
   a.last_rows = FastDiv::of((uint32_t)(a.m_tiles % 16 ? a.m_tiles % 16 : 16));
   const char* test = getenv("VI_HEADS_TEST_TIMEOUT");
   a.withhold = test && test[0] == '1';
-  a.spin_limit = a.withhold ? 1u << 12 : kSpinLimit;
+  a.wait_limit = a.withhold ? 1 << 20 : kWaitLimit;
   a.e = e;
   cudaError_t rc;
   if (dtype == VI_F32)
