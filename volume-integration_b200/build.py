@@ -24,7 +24,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libvi_b200.so")
 SOURCES = ["vi_sort.cu", "vi_binning.cu", "vi_features.cu", "vi_render.cu", "vi_backward.cu", "vi_api.cu",
            "vi_sort_noalloc.cu", "vi_gaussians.cu", "vi_table.cu", "vi_heads.cu",
-           "vi_heads_gemm.cu", "vi_heads_narrow.cu"]
+           "vi_heads_gemm.cu", "vi_heads_narrow.cu", "vi_heads_small.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

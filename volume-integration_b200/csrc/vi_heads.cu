@@ -650,6 +650,13 @@ void strip(Run& r, Summer& sums, int dtype, Strip q, const float* alpha, void* d
   r.launches++;
 }
 
+int small(Run& r, int dtype, const SmallJob& a, const SmallJob* b) {
+  if (r.dry) return VI_OK;
+  const cudaError_t rc = launch_small(dtype, a, b, r.s);
+  r.launches++;
+  return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+}
+
 // Gradients of the weights over no rows at all.
 void zero_gradients(Run& r, int dtype, int64_t N, int64_t K, const vi_matrix* dw, void* db) {
   Summer sums{r, dtype};
@@ -743,6 +750,15 @@ int act_forward(Run& r, int dtype, int act, const vi_matrix* x, const vi_matrix*
     r.launches++;
     return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
   }
+  // a small product whose operands would have to be laid out first
+  if (small_product(M, N, K, K) && !(direct(dtype, view(x), M, K) && direct(dtype, view(w), N, K))) {
+    SmallJob q{view(x), {}, view(w), nullptr, (int)M, (int)N, (int)K, e.out};
+    q.bias = bias;
+    q.act = act;
+    q.res = e.res;
+    q.dact = e.dact;
+    return small(r, dtype, q, nullptr);
+  }
   Packer pk{r, dtype};
   const Operand A = pk.add(view(x), M, K), B = pk.add(view(w), N, K);
   pk.run();
@@ -780,6 +796,13 @@ int act_backward(Run& r, int dtype, int act, const vi_matrix* dy, const vi_matri
     if (db) sums.add(SumJob{a.part + per - 1, blocks, N * per, 0, per, 1, N, nullptr, View{db, 0, 1}});
     sums.run();
     return VI_OK;
+  }
+  if ((slope.p || act == VI_ACT_NONE) && small_product(M, N, K, std::max(M, N))) {
+    const SmallJob jx{view(dy), slope, transposed(view(w)), nullptr, (int)M, (int)K, (int)N, view(dx)};
+    SmallJob jw{transposed(view(dy)), transposed(slope), transposed(view(x)), nullptr, (int)N, need_dw ? (int)K : 1, (int)M, view(dw)};
+    jw.sums = db;
+    const bool second = need_dw || db;
+    return need_dx ? small(r, dtype, jx, second ? &jw : nullptr) : second ? small(r, dtype, jw, nullptr) : VI_OK;
   }
   Packer pk{r, dtype};
   Operand S{}, W{}, X{};
@@ -901,6 +924,19 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
     coef_kernel<<<parts, 256, 0, r.s>>>(target, ignore, M, reduction, dloss, parts > 1 ? bmax : nullptr, bcount, parts,
                                         dtype == VI_F16 ? 16384.0f : 1.0f, coef, alpha);
     r.launches++;
+  }
+  if (small_product(M, V, K, std::max({M, V, K}))) {
+    const View G{r.take((size_t)M * V * es), V, 1};
+    SmallJob g{view(x), {}, view(w), nullptr, (int)M, (int)V, (int)K, G};
+    g.bias = bias;
+    g.coef = coef;
+    g.lse = lse;
+    g.target = target;
+    if (int rc = small(r, dtype, g, nullptr)) return rc;
+    SmallJob jx{G, {}, transposed(view(w)), nullptr, (int)M, (int)K, (int)V, view(dx), alpha};
+    SmallJob jw{transposed(G), {}, transposed(view(x)), coef, (int)V, need_dw ? (int)K : 1, (int)M, view(dw), alpha, db};
+    const bool second = need_dw || db;
+    return need_dx ? small(r, dtype, jx, second ? &jw : nullptr) : second ? small(r, dtype, jw, nullptr) : VI_OK;
   }
   // x without the rows of ignored targets: their zero gradient times a NaN or an
   // infinity would else reach the weights' gradient

@@ -104,5 +104,34 @@ int narrow_sums(int64_t K);
 int narrow_blocks(int64_t M, int sms);  // of the backward
 cudaError_t launch_narrow(int dtype, const NarrowArgs& a, bool backward, int blocks, int sms, cudaStream_t s);
 
+// out(m, n) = f(sum_k A(m, k) B(n, k)) on the FP32 cores, for small products.
+struct SmallJob {
+  View a, slope;       // A = a * slope (p null: a)
+  View b;
+  const float* skip;   // B(n, k) counts as 0 where skip[k] is 0; null = nowhere
+  int M, N, K;
+  View out;            // p null: only the sums are wanted
+  const float* alpha;  // device factor, null = 1
+  void* sums;          // [M] alpha * sum_k A(m, k), null = not wanted
+  // forward: act(. + bias) + res, act' to dact (in out's strides)
+  const void* bias;
+  int act;
+  View res;
+  void* dact;
+  // the logits' gradient instead of act: as kEpiGrad
+  const float* coef;
+  const float* lse;
+  const int64_t* target;
+};
+struct SmallJobs {
+  SmallJob j[2];
+  int tiles0;
+};
+// Whether the launches of the tensor-core path would cost more than the product does here; `longest`
+// is the longest of its sums, which one block makes alone.
+constexpr int64_t kSmallWork = 1 << 24, kSmallSum = 1024;
+bool small_product(int64_t M, int64_t N, int64_t K, int64_t longest);
+cudaError_t launch_small(int dtype, const SmallJob& a, const SmallJob* b, cudaStream_t s);
+
 }  // namespace heads
 }  // namespace vi

@@ -515,13 +515,13 @@ __device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int a
   } else if (v.cs != 1 || t.cols <= 16) {  // an image off 16 bytes or its ragged end, or few columns: a column at a time
     q += lane * v.rs;
     if (lane < t.rows) {
-#pragma unroll 1
+#pragma unroll 4
       for (int j = 0; j < t.cols; j++, q += v.cs) *q = lds_cell(G::cell(st, lane, j), typename Row<Z>::Bits());
     }
   } else {  // a row at a time, each lane a column
     q += lane * v.cs;
     if (lane < t.cols) {
-#pragma unroll 1
+#pragma unroll 4
       for (int row = 0; row < t.rows; row++, q += v.rs) *q = lds_cell(G::cell(st, row, lane), typename Row<Z>::Bits());
     }
   }
