@@ -61,7 +61,12 @@ def test_c_abi_refusals():
         ((2, 0, x, w, None, None, y, _m(6, 5, 6, 1)), b"strides"),
         ((2, 0, _m(6, 4, -4, 1), w, None, None, y, None), b"negative"),
         ((2, 0, _m(6, 4, 4, 1, 0), w, None, None, y, None), b"data"),
-        ((2, 0, _m(2 ** 31, 4, 4, 1), w, None, None, y, None), b"2^31"),
+        ((2, 0, _m(2 ** 30 + 1, 4, 4, 1), w, None, None, y, None), b"2^30"),
+        ((2, 0, _m(6, 4, 4, 1, 257), w, None, None, y, None), b"whole elements"),
+        ((0, 0, x, _m(5, 4, 4, 1, 258), None, None, y, None), b"whole elements"),
+        ((2, 0, x, w, ctypes.c_void_p(257), None, y, None), b"whole elements"),
+        ((2, 0, x, w, None, _m(6, 5, 5, 1, 257), y, None), b"whole elements"),
+        ((2, 0, x, w, None, None, _m(6, 5, 5, 1, 257), None), b"whole elements"),
     ]:
         assert q(*args) == 0 and text in lib.vi_last_error(), (args, lib.vi_last_error())
     # a call refuses what its query refuses, and scratch that is short or not aligned

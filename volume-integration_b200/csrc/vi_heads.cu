@@ -572,6 +572,12 @@ Plan split_plan(int dtype, const Operand& A, const Operand& B, int sms) {
       if (t < best) best = t, want = s;
     }
   }
+  if (dtype == VI_F32) {
+    // the tensor core cuts what it adds, always towards zero, so a float32 sum drifts with its length: 768
+    // terms a piece (9e-7 of the result; 1536 gave 1.8e-6, 14000 5e-6), while the pieces fit in 512 MB
+    const int64_t room = std::max<int64_t>(1, (512ll << 20) / (A.rows * B.rows * 4));
+    want = std::max(want, std::min(ceil_div(kb, 12), room));
+  }
   p.kps = (int)ceil_div(kb, want);
   p.splits = (int)ceil_div(kb, p.kps);
   return p;
@@ -668,6 +674,8 @@ void zero_gradients(Run& r, int dtype, int64_t N, int64_t K, const vi_matrix* dw
 // ---- argument checks ----
 int bad(const char* msg) { return set_error(VI_ERR_INVALID_ARGUMENT, msg); }
 
+constexpr int64_t kMaxSize = 1ll << 30;  // tile coordinates are 32-bit
+
 bool dense(const vi_matrix* m) {  // one stride 1, the other at least the extent
   if (m->rows <= 0 || m->cols <= 0) return true;
   return (m->col_stride == 1 && (m->row_stride >= m->cols || m->rows == 1)) ||
@@ -680,15 +688,20 @@ int check_operands(int dtype, const vi_matrix* x, const vi_matrix* w) {
   if (!x || !w) return bad("heads: x and weight are required");
   if (x->rows < 0 || x->cols < 1 || w->rows < 1) return bad("heads: x needs at least one column and weight one row");
   if (w->cols != x->cols) return bad("heads: weight and x differ in their number of columns");
-  if (x->rows > INT32_MAX || w->rows > INT32_MAX || x->cols > INT32_MAX) return bad("heads: sizes are limited to 2^31 - 1");
+  if (x->rows > kMaxSize || w->rows > kMaxSize || x->cols > kMaxSize) return bad("heads: sizes are limited to 2^30");
   if ((!x->data && x->rows) || !w->data) return bad("heads: x and weight need data");
   if (x->row_stride < 0 || x->col_stride < 0 || w->row_stride < 0 || w->col_stride < 0)
     return bad("heads: strides must not be negative");
+  if ((uintptr_t)x->data % elem(dtype) || (uintptr_t)w->data % elem(dtype)) return bad("heads: data must lie on whole elements");
   return VI_OK;
 }
-int check_shape(const vi_matrix* m, int64_t rows, int64_t cols, bool need_dense, const char* msg) {
+int check_vector(int dtype, const void* p) {
+  return (uintptr_t)p % elem(dtype) ? bad("heads: data must lie on whole elements") : VI_OK;
+}
+int check_shape(int dtype, const vi_matrix* m, int64_t rows, int64_t cols, bool need_dense, const char* msg) {
   if (!m || !m->data) return VI_OK;
   if (m->rows != rows || m->cols != cols || m->row_stride < 0 || m->col_stride < 0) return bad(msg);
+  if (int rc = check_vector(dtype, m->data)) return rc;
   if (need_dense && !dense(m)) return bad(msg);
   return VI_OK;
 }
@@ -729,11 +742,12 @@ int act_forward(Run& r, int dtype, int act, const vi_matrix* x, const vi_matrix*
                 const vi_matrix* res, const vi_matrix* y, const vi_matrix* dact) {
   if (int rc = check_operands(dtype, x, w)) return rc;
   if (act < VI_ACT_NONE || act > VI_ACT_SIGMOID) return bad("linear_act: unknown activation");
+  if (int rc = check_vector(dtype, bias)) return rc;
   const int64_t M = x->rows, K = x->cols, N = w->rows;
   if (!given(y) || y->rows != M) return bad("linear_act: y is required, [M, N]");
-  if (int rc = check_shape(res, M, N, false, "linear_act: residual must be [M, N]")) return rc;
-  if (int rc = check_shape(y, M, N, true, "linear_act: y must be a dense [M, N]")) return rc;
-  if (int rc = check_shape(dact, M, N, true, "linear_act: dact must be a dense [M, N]")) return rc;
+  if (int rc = check_shape(dtype, res, M, N, false, "linear_act: residual must be [M, N]")) return rc;
+  if (int rc = check_shape(dtype, y, M, N, true, "linear_act: y must be a dense [M, N]")) return rc;
+  if (int rc = check_shape(dtype, dact, M, N, true, "linear_act: dact must be a dense [M, N]")) return rc;
   if (dact && dact->data && (dact->row_stride != y->row_stride || dact->col_stride != y->col_stride))
     return bad("linear_act: dact must have y's strides");
   if (M == 0) return VI_OK;
@@ -750,8 +764,9 @@ int act_forward(Run& r, int dtype, int act, const vi_matrix* x, const vi_matrix*
     r.launches++;
     return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
   }
-  // a small product whose operands would have to be laid out first
-  if (small_product(M, N, K, K) && !(direct(dtype, view(x), M, K) && direct(dtype, view(w), N, K))) {
+  // a small product whose operands would have to be laid out first (with longer sums that launch is worth it:
+  // 37 x 203 -> 131: 16 us, 20 here)
+  if (K <= 128 && small_product(M, N, K, K) && !(direct(dtype, view(x), M, K) && direct(dtype, view(w), N, K))) {
     SmallJob q{view(x), {}, view(w), nullptr, (int)M, (int)N, (int)K, e.out};
     q.bias = bias;
     q.act = act;
@@ -769,12 +784,14 @@ int act_backward(Run& r, int dtype, int act, const vi_matrix* dy, const vi_matri
                  const vi_matrix* w, const void* bias, const vi_matrix* dx, const vi_matrix* dw, void* db) {
   if (int rc = check_operands(dtype, x, w)) return rc;
   if (act < VI_ACT_NONE || act > VI_ACT_SIGMOID) return bad("linear_act backward: unknown activation");
+  if (int rc = check_vector(dtype, bias)) return rc;
+  if (int rc = check_vector(dtype, db)) return rc;
   const int64_t M = x->rows, K = x->cols, N = w->rows;
   if (!given(dy) || dy->rows != M) return bad("linear_act backward: dy is required, [M, N]");
-  if (int rc = check_shape(dy, M, N, false, "linear_act backward: dy must be [M, N]")) return rc;
-  if (int rc = check_shape(dact, M, N, true, "linear_act backward: dact must be a dense [M, N]")) return rc;
-  if (int rc = check_shape(dx, M, K, true, "linear_act backward: dx must be a dense [M, K]")) return rc;
-  if (int rc = check_shape(dw, N, K, true, "linear_act backward: dweight must be a dense [N, K]")) return rc;
+  if (int rc = check_shape(dtype, dy, M, N, false, "linear_act backward: dy must be [M, N]")) return rc;
+  if (int rc = check_shape(dtype, dact, M, N, true, "linear_act backward: dact must be a dense [M, N]")) return rc;
+  if (int rc = check_shape(dtype, dx, M, K, true, "linear_act backward: dx must be a dense [M, K]")) return rc;
+  if (int rc = check_shape(dtype, dw, N, K, true, "linear_act backward: dweight must be a dense [N, K]")) return rc;
   const size_t es = elem(dtype);
   if (M == 0) {
     zero_gradients(r, dtype, N, K, dw, db);
@@ -848,6 +865,7 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
                int64_t ignore, int reduction, float* loss, float* lse) {
   if (int rc = check_operands(dtype, x, w)) return rc;
   if (reduction < VI_REDUCE_NONE || reduction > VI_REDUCE_SUM) return bad("linear_ce: unknown reduction");
+  if (int rc = check_vector(dtype, bias)) return rc;
   const int64_t M = x->rows, K = x->cols, V = w->rows;
   if (!r.dry && M && (!target || !loss || !lse)) return bad("linear_ce: target, loss and lse are required");
   const int64_t blocks = M <= 1024 ? std::min<int64_t>(M, 1) : ceil_div(M, 256);  // few rows: one block ends the sum too
@@ -900,9 +918,11 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
                 const vi_matrix* dw, void* db) {
   if (int rc = check_operands(dtype, x, w)) return rc;
   if (reduction < VI_REDUCE_NONE || reduction > VI_REDUCE_SUM) return bad("linear_ce backward: unknown reduction");
+  if (int rc = check_vector(dtype, bias)) return rc;
+  if (int rc = check_vector(dtype, db)) return rc;
   const int64_t M = x->rows, K = x->cols, V = w->rows;
-  if (int rc = check_shape(dx, M, K, true, "linear_ce backward: dx must be a dense [M, K]")) return rc;
-  if (int rc = check_shape(dw, V, K, true, "linear_ce backward: dweight must be a dense [V, K]")) return rc;
+  if (int rc = check_shape(dtype, dx, M, K, true, "linear_ce backward: dx must be a dense [M, K]")) return rc;
+  if (int rc = check_shape(dtype, dw, V, K, true, "linear_ce backward: dweight must be a dense [V, K]")) return rc;
   if (!r.dry && M && (!target || !lse || !dloss)) return bad("linear_ce backward: target, lse and dloss are required");
   const size_t es = elem(dtype);
   if (M == 0) {

@@ -129,7 +129,7 @@ struct SmallJobs {
 };
 // Whether the launches of the tensor-core path would cost more than the product does here; `longest`
 // is the longest of its sums, which one block makes alone.
-constexpr int64_t kSmallWork = 1 << 24, kSmallSum = 1024;
+constexpr int64_t kSmallWork = 1 << 24, kSmallSum = 512;
 bool small_product(int64_t M, int64_t N, int64_t K, int64_t longest);
 cudaError_t launch_small(int dtype, const SmallJob& a, const SmallJob* b, cudaStream_t s);
 

@@ -10,8 +10,11 @@
 // transposes nothing.
 //
 // float32 operands come as three bfloat16 planes, x = x0 + x1 + x2.  Of the nine
-// products of planes the six with i + j <= 2 are summed, smallest first within every
-// block of k; the others are below 2^-24 of |x||w|.
+// products of planes the six with i + j <= 2 are summed; the others are below 2^-24
+// of |x||w|.  x0 w0 has an accumulator of its own and the five small products share
+// another, added to it in the epilogue: the tensor core cuts an addend's bits below the
+// accumulator's, and small ones cut 5 times as often cost ten times the error (5001 x 515 ->
+// 257: 3.3e-6 in one accumulator, 3e-7 in two).
 //
 // Every wait is bounded; one that runs out ends the block's work, drains what it
 // has in flight, and is latched in a status word (VI_DEVICE_HEAD_TIMEOUT).
@@ -547,7 +550,8 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
                    const __grid_constant__ Args a) {
   using S = Shape<T, BN, EPI, PL>;
   constexpr int kStages = S::kStages, kStage = S::kStage, kEpiWarps = S::kWarps;
-  constexpr uint32_t kCols = BN < 128 ? 2 * 64 : 2 * BN;  // tensor memory columns: two accumulators
+  constexpr int kAcc = PL == 3 ? 2 * BN : BN;   // tensor memory columns of an accumulator
+  constexpr uint32_t kCols = 2 * kAcc;          // two of them alternate
   extern __shared__ __align__(1024) char smem[];
   uint64_t* bars = (uint64_t*)(smem + S::kBars);
   uint32_t* tmem_slot = (uint32_t*)(bars + 2 * kStages + 5);
@@ -671,7 +675,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
             break;
           }
           fence_after();
-          const uint32_t d = tmem + acc * BN;
+          const uint32_t d = tmem + acc * kAcc;
 #pragma unroll 1
           for (int s = 0; s < steps; s++) {
             if (!mbar_wait(full + 8 * stage, phase, dead, a.wait_limit)) {
@@ -689,7 +693,8 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
               const uint64_t da = smem_desc(sa + pa * S::kTileA, a.a_lbo), db = smem_desc(sb + pb * S::kTileB, a.b_lbo);
 #pragma unroll
               for (int k = 0; k < kBK / 16; k++)
-                mma_f16<S::kPair>(d, da + k * a.a_step, db + k * a.b_step, a.idesc, s > 0 || p > 0 || k > 0);
+                mma_f16<S::kPair>(PL == 3 && p < 5 ? d + BN : d, da + k * a.a_step, db + k * a.b_step, a.idesc,
+                                  s > 0 || (p > 0 && p < 5) || k > 0);
             }
             mma_commit<S::kPair>(empty + 8 * stage);
             if (++stage == kStages) stage = 0, phase ^= 1;
@@ -761,7 +766,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
           if (kAdds && add.p) way = load_tile<T>(extra, add, EPI == kEpiAct ? res_access : access_of<T>(add), st, lane, here);
           if (!waited) wait_product();
           if (!on) break;
-          const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + c;
+          const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + acc * kAcc + c;
           if (EPI != kEpiPartial && EPI != kEpiStore) {
             if (e.bias && !e.bias_rows && bias_at != n0) {  // a lane a column, then every lane all of them
               __syncwarp();
@@ -779,7 +784,15 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
               for (int h = 0; h < 2; h++) {  // 16 columns at a time: with 32 the activations spill
                 float2 v[8];
                 tmem_load16(src + h * 16, (float*)v);
-                tmem_wait_load();
+                if constexpr (PL == 3) {
+                  float2 u[8];
+                  tmem_load16(src + BN + h * 16, (float*)u);
+                  tmem_wait_load();
+#pragma unroll
+                  for (int j = 0; j < 8; j++) v[j] = __fadd2_rn(v[j], u[j]);
+                } else {
+                  tmem_wait_load();
+                }
                 if constexpr (EPI == kEpiAct) {
                   if (e.bias_rows) {
 #pragma unroll
@@ -825,7 +838,15 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
           } else if constexpr (EPI == kEpiLse) {
             float2 v[16];
             tmem_load32(src, (float*)v);
-            tmem_wait_load();
+            if constexpr (PL == 3) {
+              float2 u[16];
+              tmem_load32(src + BN, (float*)u);
+              tmem_wait_load();
+#pragma unroll
+              for (int j = 0; j < 16; j++) v[j] = __fadd2_rn(v[j], u[j]);
+            } else {
+              tmem_wait_load();
+            }
             if (e.bias) add_bias<32>(bias_slot, v);
             float* z = (float*)v;
             const int tc = target - n0;
@@ -864,7 +885,15 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
           } else if constexpr (EPI == kEpiGrad) {
             float2 v[16];
             tmem_load32(src, (float*)v);
-            tmem_wait_load();
+            if constexpr (PL == 3) {
+              float2 u[16];
+              tmem_load32(src + BN, (float*)u);
+              tmem_wait_load();
+#pragma unroll
+              for (int j = 0; j < 16; j++) v[j] = __fadd2_rn(v[j], u[j]);
+            } else {
+              tmem_wait_load();
+            }
             if (e.bias) add_bias<32>(bias_slot, v);
             float* z = (float*)v;
 #pragma unroll

@@ -4,7 +4,7 @@
 // A step on a few rows is bound by its launches (3 us each on the host, as much again before a kernel does
 // work), not by arithmetic: the tensor-core path takes five to seven of them for a backward
 // (lay out, two products, their pieces' sums), this one takes one.  A block makes a 32 x 32 tile
-// of a product, 2 x 2 outputs a thread, with the next 32 of k on their way in registers.
+// of a product, 2 x 2 outputs a thread, with the next 64 of k on their way in registers.
 // Elements are float32 once loaded, so dy * act' is not rounded here.
 #include <algorithm>
 
@@ -16,8 +16,10 @@ namespace vi {
 namespace heads {
 namespace {
 
-constexpr int kT = 32;  // tile, and depth of k
+constexpr int kT = 32;      // tile
+constexpr int kDepth = 64;  // of k in shared memory: a block waits for memory once per this many
 constexpr int kThreads = 256;
+constexpr int kEach = kT * kDepth / kThreads;  // elements a thread loads of either operand
 
 template <typename T>
 __device__ __forceinline__ float slope_at(const void* p, int64_t i) {
@@ -25,17 +27,17 @@ __device__ __forceinline__ float slope_at(const void* p, int64_t i) {
   else return Slope<T>::unpack(((const uint16_t*)p)[i]);
 }
 
-// Element `i` of a thread's four of a 32 x 32 tile: neighbouring threads along the contiguous axis.
+// Element `i` of a thread's share of 32 rows x 64 k: neighbouring threads along the contiguous axis.
 __device__ __forceinline__ void place(bool k_fast, int i, int& row, int& k) {
   const int e = threadIdx.x + i * kThreads;
-  row = k_fast ? e / kT : e % kT;
-  k = k_fast ? e % kT : e / kT;
+  row = k_fast ? e / kDepth : e % kT;
+  k = k_fast ? e % kDepth : e / kT;
 }
 
 template <typename T>
-__device__ __forceinline__ void fetch_a(const SmallJob& q, bool k_fast, int m0, int k0, float v[4]) {
+__device__ __forceinline__ void fetch_a(const SmallJob& q, bool k_fast, int m0, int k0, float (&v)[kEach]) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int i = 0; i < kEach; i++) {
     int r, k;
     place(k_fast, i, r, k);
     r += m0, k += k0;
@@ -47,9 +49,9 @@ __device__ __forceinline__ void fetch_a(const SmallJob& q, bool k_fast, int m0, 
   }
 }
 template <typename T>
-__device__ __forceinline__ void fetch_b(const SmallJob& q, bool k_fast, int n0, int k0, float v[4]) {
+__device__ __forceinline__ void fetch_b(const SmallJob& q, bool k_fast, int n0, int k0, float (&v)[kEach]) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
+  for (int i = 0; i < kEach; i++) {
     int r, k;
     place(k_fast, i, r, k);
     r += n0, k += k0;
@@ -76,7 +78,7 @@ __device__ __forceinline__ void activate1(int act, bool exact, float z, float& y
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) small_kernel(const __grid_constant__ SmallJobs jobs) {
-  __shared__ float sa[kT][kT + 2], sb[kT][kT + 2];  // [k][row]
+  __shared__ float sa[kDepth][kT + 2], sb[kDepth][kT + 2];  // [k][row]
   const bool second = (int)blockIdx.x >= jobs.tiles0;
   const SmallJob& q = jobs.j[second];
   const int tile = blockIdx.x - (second ? jobs.tiles0 : 0), nt = (q.N + kT - 1) / kT;
@@ -84,13 +86,13 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const __grid_constant__
   const bool fa = q.a.cs == 1, fb = q.b.cs == 1;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   float acc[2][2] = {}, rows[2] = {};
-  float va[4], vb[4];
+  float va[kEach], vb[kEach];
   fetch_a<T>(q, fa, m0, 0, va);
   fetch_b<T>(q, fb, n0, 0, vb);
-  for (int k0 = 0; k0 < q.K; k0 += kT) {
+  for (int k0 = 0; k0 < q.K; k0 += kDepth) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < kEach; i++) {
       int r, k;
       place(fa, i, r, k);
       sa[k][r] = va[i];
@@ -98,12 +100,12 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const __grid_constant__
       sb[k][r] = vb[i];
     }
     __syncthreads();
-    if (k0 + kT < q.K) {
-      fetch_a<T>(q, fa, m0, k0 + kT, va);
-      fetch_b<T>(q, fb, n0, k0 + kT, vb);
+    if (k0 + kDepth < q.K) {
+      fetch_a<T>(q, fa, m0, k0 + kDepth, va);
+      fetch_b<T>(q, fb, n0, k0 + kDepth, vb);
     }
 #pragma unroll 8
-    for (int k = 0; k < kT; k++) {
+    for (int k = 0; k < kDepth; k++) {
       const float2 a = *(const float2*)&sa[k][2 * ty], b = *(const float2*)&sb[k][2 * tx];
       acc[0][0] = fmaf(a.x, b.x, acc[0][0]);
       acc[0][1] = fmaf(a.x, b.y, acc[0][1]);
