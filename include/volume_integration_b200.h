@@ -352,8 +352,9 @@ int vi_linear_act_keeps_dact(int dtype, int activation, const vi_matrix* x, cons
 /*
  * Gradients of vi_linear_act_forward for an incoming dy [M,N] (any strides):
  * with s = dy * act', dx = s weight, dweight = s^T x, dbias = the column sums of
- * s.  dact is the forward's; NULL: act' is computed again from x, weight and
- * bias (which is read for nothing else).  Each of dx, dweight, dbias may be NULL; dx
+ * s.  dact is the forward's; for VI_ACT_RELU its result y serves as well, if there
+ * was no residual (positive means 1); NULL: act' is computed again from x, weight
+ * and bias (which is read for nothing else).  Each of dx, dweight, dbias may be NULL; dx
  * and dweight have one of their strides 1.  The residual's gradient is dy itself.
  */
 uint64_t vi_linear_act_backward_scratch_bytes(int dtype, int activation, const vi_matrix* dy, const vi_matrix* dact,

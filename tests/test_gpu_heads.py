@@ -99,6 +99,24 @@ def test_linear_act_images_of_few_channels(M, K, N, act, order, residual, dy_ord
     assert y.t().is_contiguous() or order != "image"
 
 
+@pytest.mark.parametrize("dt", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_relu_keeps_its_result_and_nothing_else(dt):
+    # the backward reads relu's derivative off the result, which an in-place change would spoil: torch says so
+    import volume_integration.heads as heads
+    x, w, b, _, dy = _act_inputs(1200, 40, 200, dt, "rows", True, False, 42)
+    x.requires_grad_(True)
+    y = heads.linear_act(x, w, b, activation="relu")
+    used = torch.cuda.memory_allocated()
+    z = heads.linear_act(x, w, b, activation="relu")
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - used <= z.numel() * z.element_size() + 4096
+    (dx,) = torch.autograd.grad(y, (x,), dy)
+    hl.assert_within("dx", dx, hl.linear_act(x.detach(), w, b, None, "relu", dy)[1])
+    z.mul_(2)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(z, (x,), dy)
+
+
 def test_backward_without_the_kept_derivative():
     # a C ABI caller that kept no act': it is computed again from x, weight and bias
     import ctypes

@@ -546,9 +546,14 @@ bool wants_grad(const c10::optional<Tensor>& t) { return t.has_value() && t->req
 struct LinearAct : torch::autograd::Function<LinearAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias,
                         const c10::optional<Tensor>& residual, int64_t activation) {
-    // act' is kept rather than z: it is exact for relu, and the backward needs no transcendental
+    // act' is kept rather than z, so the backward needs no transcendental; relu's is read off the result
+    head_check(x, weight);
+    const vi_matrix mx = head_matrix(x), mw = head_matrix(weight);
+    const bool from_y = activation == VI_ACT_RELU && !residual.has_value() &&
+                        vi_linear_act_keeps_dact(head_dtype(x, "x"), VI_ACT_RELU, &mx, &mw);
     auto [y, dact] = linear_act_forward(x, weight, bias, residual, activation,
-                                        wants_grad(x) || wants_grad(weight) || wants_grad(bias));
+                                        !from_y && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)));
+    if (from_y) dact = y;
     ctx->save_for_backward({x, weight, bias.value_or(Tensor()), dact.value_or(Tensor())});
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["bias"] = bias.has_value();

@@ -55,9 +55,11 @@ __device__ __forceinline__ void load8(const T* s, int64_t step, int n, float v[8
   }
 }
 template <typename T>
-__device__ __forceinline__ void load8_slope(const void* p, int64_t at, int64_t step, int n, float v[8]) {
+__device__ __forceinline__ void load8_slope(const void* p, int64_t at, int64_t step, int n, bool relu, float v[8]) {
   if constexpr (sizeof(T) == 4) {
     load8((const float*)p + at, step, n, v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = kept_slope(v[j], relu);
   } else {
     const uint16_t* s = (const uint16_t*)p + at;
     uint4 w;
@@ -69,7 +71,7 @@ __device__ __forceinline__ void load8_slope(const void* p, int64_t at, int64_t s
       for (int j = 0; j < 8; j++) q[j] = j < n ? s[j * step] : 0;
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = Slope<T>::unpack(q[j]);
+    for (int j = 0; j < 8; j++) v[j] = kept_slope<T>(q[j], relu);
   }
 }
 // Eight values as the tensor cores' elements, in one plane or three.
@@ -126,6 +128,7 @@ struct Strip {
   int64_t ld, plane;
   float* part;
   bool padded;  // rows of src may be read up to their stride
+  bool relu;    // slope is positive where act' is 1
 };
 
 template <typename T>
@@ -134,7 +137,7 @@ __device__ __forceinline__ void strip8(const Strip& q, int64_t m, int64_t n, int
   load8((const T*)q.src.p + m * q.src.rs + n * q.src.cs, step_src, count, v);
   if (q.slope.p) {
     float w[8];
-    load8_slope<T>(q.slope.p, m * q.slope.rs + n * q.slope.cs, step_slope, count, w);
+    load8_slope<T>(q.slope.p, m * q.slope.rs + n * q.slope.cs, step_slope, count, q.relu, w);
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] *= w[j];
   }
@@ -178,8 +181,8 @@ __global__ void __launch_bounds__(256) strip_rows_kernel(const __grid_constant__
           for (int j = 0; j < 8; j++) {
             v[j] = to_f(((const T*)a[i])[j]);
             if (slope) {
-              if constexpr (sizeof(T) == 4) v[j] *= ((const float*)b[i])[j];
-              else v[j] *= Slope<T>::unpack(((const uint16_t*)b[i])[j]);
+              if constexpr (sizeof(T) == 4) v[j] *= kept_slope(((const float*)b[i])[j], q.relu);
+              else v[j] *= kept_slope<T>(((const uint16_t*)b[i])[j], q.relu);
             }
           }
           if (q.dst) store8<T>(v, (Cell16<T>*)q.dst + row * q.ld + n, q.plane);
@@ -815,9 +818,10 @@ int act_backward(Run& r, int dtype, int act, const vi_matrix* dy, const vi_matri
     return VI_OK;
   }
   if ((slope.p || act == VI_ACT_NONE) && small_product(M, N, K, std::max(M, N))) {
-    const SmallJob jx{view(dy), slope, transposed(view(w)), nullptr, (int)M, (int)K, (int)N, view(dx)};
+    SmallJob jx{view(dy), slope, transposed(view(w)), nullptr, (int)M, (int)K, (int)N, view(dx)};
     SmallJob jw{transposed(view(dy)), transposed(slope), transposed(view(x)), nullptr, (int)N, need_dw ? (int)K : 1, (int)M, view(dw)};
     jw.sums = db;
+    jx.relu = jw.relu = act == VI_ACT_RELU;
     const bool second = need_dw || db;
     return need_dx ? small(r, dtype, jx, second ? &jw : nullptr) : second ? small(r, dtype, jw, nullptr) : VI_OK;
   }
@@ -840,6 +844,7 @@ int act_backward(Run& r, int dtype, int act, const vi_matrix* dy, const vi_matri
   const View d = view(dy);
   const bool in_place = !slope.p && direct(dtype, d, M, N);
   Strip q{d, slope, M, N};
+  q.relu = act == VI_ACT_RELU;
   if (need_dx || need_dw) {
     const bool k_major = d.cs == 1 || d.rs != 1;
     if (in_place) {

@@ -122,6 +122,7 @@ struct SmallJob {
   const float* coef;
   const float* lse;
   const int64_t* target;
+  bool relu;           // slope is positive where act' is 1
 };
 struct SmallJobs {
   SmallJob j[2];

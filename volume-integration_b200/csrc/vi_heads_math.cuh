@@ -144,6 +144,14 @@ struct Slope<__half> {
   }
 };
 
+// act' as kept: the code above (float32 beside float32), or for relu anything that is positive where it
+// is 1, so that the result itself serves.
+template <typename T>
+__device__ __forceinline__ float kept_slope(uint16_t v, bool relu) {
+  return relu ? ((int16_t)v > 0 ? 1.0f : 0.0f) : Slope<T>::unpack(v);
+}
+__device__ __forceinline__ float kept_slope(float v, bool relu) { return relu ? (v > 0.0f ? 1.0f : 0.0f) : v; }
+
 // Two float32 values rounded to T, packed.
 __device__ __forceinline__ uint32_t pack2(float2 v, __half) {
   const __half2 h = __float22half2_rn(v);

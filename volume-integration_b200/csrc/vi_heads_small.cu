@@ -22,9 +22,9 @@ constexpr int kThreads = 256;
 constexpr int kEach = kT * kDepth / kThreads;  // elements a thread loads of either operand
 
 template <typename T>
-__device__ __forceinline__ float slope_at(const void* p, int64_t i) {
-  if constexpr (sizeof(T) == 4) return ((const float*)p)[i];
-  else return Slope<T>::unpack(((const uint16_t*)p)[i]);
+__device__ __forceinline__ float slope_at(const void* p, int64_t i, bool relu) {
+  if constexpr (sizeof(T) == 4) return kept_slope(((const float*)p)[i], relu);
+  else return kept_slope<T>(((const uint16_t*)p)[i], relu);
 }
 
 // Element `i` of a thread's share of 32 rows x 64 k: neighbouring threads along the contiguous axis.
@@ -44,7 +44,7 @@ __device__ __forceinline__ void fetch_a(const SmallJob& q, bool k_fast, int m0, 
     v[i] = 0.0f;
     if (r < q.M && k < q.K) {
       v[i] = to_f(((const T*)q.a.p)[r * q.a.rs + k * q.a.cs]);
-      if (q.slope.p) v[i] *= slope_at<T>(q.slope.p, r * q.slope.rs + k * q.slope.cs);
+      if (q.slope.p) v[i] *= slope_at<T>(q.slope.p, r * q.slope.rs + k * q.slope.cs, q.relu);
     }
   }
 }
