@@ -386,6 +386,43 @@ struct Place {
   int rows, cols;
 };
 
+// Ragged ends and any strides: into the staging, and out of it.  A row at a time where columns are
+// contiguous and many, else a column at a time, eight loads in flight.  Calls, not inlined: in the
+// epilogue's code they cost the common case its registers (frame 203 us, 220).
+template <typename Z>
+__device__ __noinline__ void load_ragged(const typename Row<Z>::Bits* q, int64_t rs, int64_t cs, uint32_t st, int lane, int rows,
+                                         int cols) {
+  using Bits = typename Row<Z>::Bits;
+  using G = Stage<Z>;
+  const bool by_rows = cs == 1 && cols > 16;
+  const int lines = by_rows ? rows : cols, along = by_rows ? cols : rows;
+  const int64_t step = by_rows ? rs : cs;
+  if (lane >= along) return;
+  q += lane * (by_rows ? cs : rs);
+#pragma unroll 1
+  for (int l = 0; l < lines; l += 8) {
+    Bits b[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (l + i < lines) b[i] = q[(l + i) * step];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (l + i < lines) sts_cell(by_rows ? G::cell(st, l + i, lane) : G::cell(st, lane, l + i), b[i]);
+  }
+}
+template <typename Z>
+__device__ __noinline__ void store_ragged(typename Row<Z>::Bits* q, int64_t rs, int64_t cs, uint32_t st, int lane, int rows, int cols) {
+  using Bits = typename Row<Z>::Bits;
+  using G = Stage<Z>;
+  const bool by_rows = cs == 1 && cols > 16;
+  const int lines = by_rows ? rows : cols, along = by_rows ? cols : rows;
+  const int64_t step = by_rows ? rs : cs;
+  if (lane >= along) return;
+  q += lane * (by_rows ? cs : rs);
+#pragma unroll 4
+  for (int l = 0; l < lines; l++, q += step) *q = lds_cell(by_rows ? G::cell(st, l, lane) : G::cell(st, lane, l), Bits());
+}
+
 // Loads a tile of v, 16 bytes a lane: along rows (kVector), along columns (kImage), or else
 // element by element into the staging; own_row hands them to their rows' lanes.  Returns the way.
 template <typename Z>
@@ -410,26 +447,8 @@ __device__ __forceinline__ int load_tile(Row<Z>& r, const View& v, int access, u
     }
     return kImage;
   }
-  // ragged ends and any strides, into the staging: a row at a time where columns are contiguous and
-  // many, else a column at a time; eight loads in flight (more would unroll more code than they are worth)
   __syncwarp();
-  using Bits = typename Row<Z>::Bits;
-  const bool by_rows = v.cs == 1 && t.cols > 16;
-  const int lines = by_rows ? t.rows : t.cols, along = by_rows ? t.cols : t.rows;
-  const int64_t step = by_rows ? v.rs : v.cs;
-  const Bits* q = (const Bits*)p + (int64_t)t.m0 * v.rs + (int64_t)t.n0 * v.cs + lane * (by_rows ? v.cs : v.rs);
-  if (lane < along) {
-#pragma unroll 1
-    for (int l = 0; l < lines; l += 8) {
-      Bits b[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (l + i < lines) b[i] = q[(l + i) * step];
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (l + i < lines) sts_cell(by_rows ? G::cell(st, l + i, lane) : G::cell(st, lane, l + i), b[i]);
-    }
-  }
+  load_ragged<Z>((const typename Row<Z>::Bits*)p + (int64_t)t.m0 * v.rs + (int64_t)t.n0 * v.cs, v.rs, v.cs, st, lane, t.rows, t.cols);
   return kScalar;
 }
 // What load_tile left along lines, to a row each, through the staging.
@@ -517,18 +536,8 @@ __device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int a
 #pragma unroll
     for (int i = 0; i < G::kLanes; i++, q += step)
       if (line + i * G::kStep < t.rows) *(uint4*)q = lds128(G::along(st, lane, i));
-  } else if (v.cs != 1 || t.cols <= 16) {  // an image off 16 bytes or its ragged end, or few columns: a column at a time
-    q += lane * v.rs;
-    if (lane < t.rows) {
-#pragma unroll 4
-      for (int j = 0; j < t.cols; j++, q += v.cs) *q = lds_cell(G::cell(st, lane, j), typename Row<Z>::Bits());
-    }
-  } else {  // a row at a time, each lane a column
-    q += lane * v.cs;
-    if (lane < t.cols) {
-#pragma unroll 4
-      for (int row = 0; row < t.rows; row++, q += v.rs) *q = lds_cell(G::cell(st, row, lane), typename Row<Z>::Bits());
-    }
+  } else {
+    store_ragged<Z>(q, v.rs, v.cs, st, lane, t.rows, t.cols);
   }
 }
 
