@@ -1002,6 +1002,11 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
     e.grad = grad;
     e.grad_ld = ld;
     e.grad_plane = M * ld;
+    if (db && dtype != VI_F32) {  // the columns' sums on the way
+      const int64_t blocks = ceil_div(M, 32);
+      e.column_part = (float*)r.take((size_t)blocks * n * 4);
+      sums.add(SumJob{e.column_part, (int)blocks, n, 0, 1, 1, n, alpha, View{(char*)db + c * elem(dtype), 0, 1}});
+    }
     if (int rc = gemm(r, dtype, kEpiGrad, X, Wc, e)) return rc;
     const Operand G{grad, M, n, ld, M * ld, true};
     if (need_dx) {
@@ -1023,10 +1028,10 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
       out.p = (char*)out.p + c * out.rs * elem(dtype);
       if (int rc = gemm_out(r, sums, transposed(G), transposed(X), alpha, out)) return rc;
     }
-    if (db) {
+    if (db && dtype == VI_F32) {
       Strip q{View{grad, ld, 1}, View{nullptr, 0, 0}, M * planes, n};  // the planes' rows one after another
       q.padded = true;
-      strip(r, sums, dtype == VI_F16 ? VI_F16 : VI_BF16, q, alpha, (char*)db + c * elem(dtype));
+      strip(r, sums, VI_BF16, q, alpha, (char*)db + c * elem(dtype));
     }
     sums.run();
     if (r.dry && c + piece < V) {  // the last piece alone may be smaller: one more round counts it

@@ -544,6 +544,38 @@ __device__ __forceinline__ void store_tile(const Row<Z>& r, const View& v, int a
 __device__ __forceinline__ uint16_t bits_of(__half v) { return __half_as_ushort(v); }
 __device__ __forceinline__ uint16_t bits_of(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*(const __half2*)&w); }
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) { return __bfloat1622float2(*(const __nv_bfloat162*)&w); }
+
+// Sum over the 32 rows of one column of the tile that store_tile has left in the staging: a lane adds 4 rows of
+// 8 columns, then lanes hand halves of their columns to each other.  Which column: `column`.
+template <typename T>
+__device__ __forceinline__ float staged_column_sum(uint32_t st, int lane, int& column) {
+  using G = Stage<T>;
+  float2 s[4] = {pair(0.0f), pair(0.0f), pair(0.0f), pair(0.0f)};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint4 q = lds128(G::along(st, lane, i));
+    s[0] = __fadd2_rn(s[0], unpack2(q.x, T()));
+    s[1] = __fadd2_rn(s[1], unpack2(q.y, T()));
+    s[2] = __fadd2_rn(s[2], unpack2(q.z, T()));
+    s[3] = __fadd2_rn(s[3], unpack2(q.w, T()));
+  }
+  float t[8] = {s[0].x, s[0].y, s[1].x, s[1].y, s[2].x, s[2].y, s[3].x, s[3].y};
+  column = (lane % 4) * 8;
+#pragma unroll
+  for (int h = 4; h; h /= 2) {
+    const bool up = lane & (4 * h);
+    if (up) column += h;
+#pragma unroll
+    for (int j = 0; j < h; j++) {
+      const float give = up ? t[j] : t[j + h], keep = up ? t[j + h] : t[j];
+      t[j] = keep + __shfl_xor_sync(0xffffffffu, give, 4 * h);
+    }
+  }
+  return t[0];
+}
+
 // v += COLS values of a bias slot.
 template <int COLS>
 __device__ __forceinline__ void add_bias(uint32_t slot, float2* v) {
@@ -939,6 +971,12 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
 #pragma unroll
               for (int j = 0; j < 16; j++) set_pair(g, j, v[j]);
               store_tile(g, View{e.grad, e.grad_ld, 1}, kVector, st, lane, here, fix, bits_of(from_f<T>(gtarget)));
+              if (e.column_part) {
+                __syncwarp();
+                int column;
+                const float sum = staged_column_sum<T>(st, lane, column);
+                if (column < here.cols) e.column_part[(int64_t)(m0 / 32) * a.N + n0 + column] = sum;
+              }
             }
           }
         }
