@@ -10,9 +10,9 @@
 // depend on scheduling.
 #include <algorithm>
 #include <atomic>
+#include <cstdio>
 #include <type_traits>
 #include <utility>
-#include <cstdio>
 
 #include "vi_heads.h"
 #include "vi_heads_math.cuh"
@@ -586,7 +586,8 @@ Plan split_plan(int dtype, const Operand& A, const Operand& B, int sms) {
   return p;
 }
 
-// Sums of pieces that wait for their launch; their part buffers stay taken until then.
+// Sums of pieces that wait for their launch; their part buffers stay taken until then.  A job is added just
+// before the kernel that writes its pieces is launched: adding the next one may launch the sums so far.
 struct Summer {
   Run& r;
   int dtype;
@@ -596,9 +597,9 @@ struct Summer {
   int64_t total = 0;
   void add(const SumJob& j) {
     // many pieces of few elements: threads share an element
-    const bool s8 = j.pieces > 8 && j.rows * j.cols < 65536;
-    if (n == 2 || (n && shared != s8)) run();
-    shared = s8;
+    const bool share = j.pieces > 8 && j.rows * j.cols < 65536;
+    if (n == 2 || (n && shared != share)) run();
+    shared = share;
     jobs.j[n++] = j;
     total = std::max(total, j.rows * j.cols);
   }
