@@ -637,6 +637,25 @@ def test_a_wait_that_runs_out_is_reported(monkeypatch):
         assert heads.device_status() == 0
 
 
+@pytest.mark.parametrize("M,K,N,dt,order", [
+    (36_000_001, 16, 64, BF16, "image"),   # results beyond element 2^31, odd columns
+    (9_000_000, 4, 256, F32, "image"),     # the narrow path's
+    (2_200_000, 24, 1000, F16, "rows"),
+])
+def test_results_beyond_32_bits(M, K, N, dt, order):
+    import volume_integration.heads as heads
+    g = _gen(29)
+    x, w, b = hl.matrix(M, K, dt, g, order), hl.matrix(N, K, dt, g, scale=0.2), hl.matrix(1, N, dt, g)[0]
+    y = heads.linear_act(x, w, b, activation="silu")
+    for rows in (slice(0, 300), slice(M // 2, M // 2 + 300), slice(M - 300, M)):
+        hl.assert_within("y", y[rows], hl.linear_act(x[rows], w, b, None, "silu")[0])
+    if dt == F16:
+        t = torch.randint(0, N, (M,), generator=g, device="cuda")
+        loss = heads.linear_cross_entropy(x, w, t, b, reduction="none")
+        for rows in (slice(0, 300), slice(M - 300, M)):
+            hl.assert_within("loss", loss[rows], hl.linear_ce(x[rows], w, b, t[rows], -100, "none")[0])
+
+
 def test_gradients_reach_the_renderer():
     # features of a rendered view -> decoder -> label loss -> the scene's parameters
     import vi_testlib as tl
