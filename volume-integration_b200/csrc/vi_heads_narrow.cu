@@ -277,7 +277,7 @@ bool narrow_backward(int64_t N, int64_t K, const View& x, const View& dy, const 
 }
 int narrow_sums(int64_t K) { return K <= 4 ? 5 : 9; }
 int narrow_blocks(int64_t M, int sms) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>((M + kTile - 1) / kTile, (int64_t)sms * 4));
+  return (int)std::max<int64_t>(1, std::min<int64_t>((M + kTile - 1) / kTile, (int64_t)sms * 3));
 }
 
 cudaError_t launch_narrow(int dtype, const NarrowArgs& args, bool backward, int blocks, int sms, cudaStream_t s) {
