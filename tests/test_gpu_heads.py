@@ -595,6 +595,38 @@ def test_captured_and_replayed():
     del graphs
 
 
+def test_tiles_of_two_blocks_captured_and_on_two_streams():
+    import volume_integration.heads as heads
+    x, w, b, r, dy = _act_inputs(5000, 300, 1100, BF16, "rows", True, True, 54)
+    static = [v.detach().clone().requires_grad_(True) for v in (x, w, b, r)]
+
+    def step(leaves):
+        y = heads.linear_act(*leaves, activation="silu")
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+    want = step(static)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(3):  # a replay beside two eager streams
+        graph.replay()
+        for s in (side, torch.cuda.Stream()):
+            s.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(s):
+                results.append(step([v.detach().requires_grad_(True) for v in (x, w, b, r)]))
+    torch.cuda.synchronize()
+    for res in results + [out]:
+        for a, c in zip(res, want):
+            assert torch.equal(a, c)
+    del graph
+
+
 def test_same_call_same_bits():
     x, w, b, t = _ce_inputs(3000, 64, 3001, BF16, "rows", True, 0.1, 25)
     import volume_integration.heads as heads
