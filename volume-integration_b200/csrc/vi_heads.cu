@@ -974,7 +974,8 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
   int64_t piece = std::max<int64_t>(256, kPieceBytes / (M * 2 * planes) / 256 * 256);
   if (piece < V && dtype != VI_F32 && K > 128) {  // whole waves of dweight's 256 x 256 tiles
     const int64_t nt = ceil_div(K, 256), slots = tile_slots(kEpiStore, 256, r.sms), waves = piece / 256 * nt / slots;
-    if (waves) piece = waves * slots / nt * 256;
+    // more features than the slots take side by side: a wave is less than one piece of 256 columns
+    if (waves) piece = std::max<int64_t>(256, waves * slots / nt * 256);
   }
   piece = std::min(piece, V);
   const int64_t ld = ceil_div(piece, 8) * 8;
