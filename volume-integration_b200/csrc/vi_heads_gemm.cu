@@ -693,6 +693,13 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
           }
         }
       }
+      // every arrival that the products still owe this block's barriers (a pair's second block gets them from
+      // the first) comes before the block leaves: the last release of every stage
+#pragma unroll 1
+      for (int j = 0; j < kStages && j < issued && on; j++) {
+        const int64_t f = issued - 1 - j;
+        on = mbar_wait(empty + 8 * (uint32_t)(f % kStages), (uint32_t)(f / kStages) & 1, dead, a.wait_limit);
+      }
       if (*dead && rank == 0) {  // wait for the copies in flight (a pair's: both blocks'): the last fill of every stage
         for (int j = 0; j < kStages && j < issued; j++) {
           const int64_t f = issued - 1 - j;  // fill number: stage f % kStages, phase (f / kStages) & 1
@@ -997,9 +1004,16 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
     }
   }
   __syncwarp();
-  // a pair ends together: its blocks arrive at each other's barriers
-  if constexpr (S::kPair) cluster_sync();
-  else __syncthreads();
+  // a pair ends together: its blocks arrive at each other's barriers.  Where both gave up, the first one's
+  // last arrival at the second is that of its drain
+  if constexpr (S::kPair) {
+    __syncthreads();
+    if (threadIdx.x == 0 && rank == 1 && *dead) mbar_drain(drain, 0, a.wait_limit);
+    __syncwarp();
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
   if (warp == kEpiWarps + 1) {
     if constexpr (S::kPair)
       asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
