@@ -3,7 +3,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/volume_integration_b200.h"
 
@@ -49,6 +51,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // act(z) and, where SLOPE, act'(z) of two values in float32.  A NaN stays a NaN.  EXACT: to a
 // few float32 steps, beside float32 outputs; else to 6e-6 of the value, beside 16-bit ones.
+// act' of a NaN is a NaN too, but relu's, which is 0 there (z > 0 is false).
 //
 // sigmoid: with e = exp(-z), s = 1 / (1 + e) and 1 - s = e s, without cancellation
 // for large z; for the slope e is kept finite, so e s tends to 1 and not to inf * 0.
@@ -90,7 +93,7 @@ __device__ __forceinline__ void activate(float2 z, float2& y, float2& d) {
       const float2 g = make_float2(expf(-0.5f * z.x * z.x), expf(-0.5f * z.y * z.y));
       d = __ffma2_rn(__fmul2_rn(z, pair(0.3989422804f)), g, cdf);
     } else {
-      const float2 x = make_float2(fmaxf(-fabsf(z.x), -6.0f), fmaxf(-fabsf(z.y), -6.0f));
+      const float2 x = make_float2(max_nan(-fabsf(z.x), -6.0f), max_nan(-fabsf(z.y), -6.0f));
       float2 r = __ffma2_rn(x, pair(1.83482305e-06f), pair(6.1598517e-05f));
       r = __ffma2_rn(r, x, pair(0.000930526497f));
       r = __ffma2_rn(r, x, pair(0.00850789675f));
@@ -119,7 +122,8 @@ __device__ __forceinline__ void activate(float2 z, float2& y, float2& d) {
 // and little else: beside bfloat16 as float16 (half a step 2^-11 of the value, a quarter
 // of bfloat16's), beside float16 with a sign, 4 bits of exponent and 11 of mantissa (2^-12,
 // half of float16's, down to 2^-14; 2^-26 absolute below).  For the latter the float
-// scaled by 2^-112 has its exponent in the low 4 bits of the field.
+// scaled by 2^-112 has its exponent in the low 4 bits of the field; a NaN, like all above the
+// range, becomes the largest code, which no act' has.
 template <typename T>
 struct Slope;
 template <>
@@ -134,21 +138,24 @@ template <>
 struct Slope<__half> {
   static __device__ __forceinline__ uint32_t pack(float2 d) {
     const float2 s = __fmul2_rn(d, pair(0x1p-112f));
-    const uint32_t a = __float_as_uint(s.x) + 0x800u, b = __float_as_uint(s.y) + 0x800u;
-    const uint32_t m = ((a >> 12) & 0x7fffu) | ((b << 4) & 0x7fff0000u);
-    return m | ((a >> 16) & 0x8000u) | (b & 0x80000000u);
+    const uint32_t a = __float_as_uint(s.x), b = __float_as_uint(s.y);
+    const uint32_t m = min(((a & 0x7fffffffu) + 0x800u) >> 12, kNan), n = min(((b & 0x7fffffffu) + 0x800u) >> 12, kNan);
+    return m | (n << 16) | ((a >> 16) & 0x8000u) | (b & 0x80000000u);
   }
   static __device__ __forceinline__ float unpack(uint16_t v) {
-    const float m = __uint_as_float((uint32_t)(v & 0x7fffu) << 12) * 0x1p112f;
+    const uint32_t a = v & 0x7fffu;
+    const float m = a == kNan ? NAN : __uint_as_float(a << 12) * 0x1p112f;
     return v & 0x8000u ? -m : m;
   }
+  static constexpr uint32_t kNan = 0x7fff;
 };
 
 // act' as kept: the code above (float32 beside float32), or for relu anything that is positive where it
-// is 1, so that the result itself serves.
+// is 1, so that the result itself serves (a NaN is not).
 template <typename T>
 __device__ __forceinline__ float kept_slope(uint16_t v, bool relu) {
-  return relu ? ((int16_t)v > 0 ? 1.0f : 0.0f) : Slope<T>::unpack(v);
+  constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return relu ? ((uint32_t)v - 1u < kInf ? 1.0f : 0.0f) : Slope<T>::unpack(v);
 }
 __device__ __forceinline__ float kept_slope(float v, bool relu) { return relu ? (v > 0.0f ? 1.0f : 0.0f) : v; }
 
