@@ -80,3 +80,74 @@ def test_a_nan_reaches_the_gradients(M, K, N, order, act, dt):
         d5 = (dy[5].double() * hl.act64(act, hl.product(x[5:6], w, b)[0])[1][0]) - s.double()
         value, bound = want[3]
         hl.assert_within("dbias", db, (value - d5, bound + hl.last(dt, d5.abs())))
+
+
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("M,K,N,order", PATHS)
+def test_infinite_preactivations(M, K, N, order, dt):
+    # through the bias, which float32's planes do not pass: sigmoid and relu have limits, silu's derivative is NaN
+    x, w, b, _, dy = _inputs(M, K, N, dt, order, True, False, 61)
+    b[1], b[2] = INF, -INF
+    for act, high, low, dhigh, dlow in (("relu", INF, 0.0, 1.0, 0.0), ("sigmoid", 1.0, 0.0, 0.0, 0.0),
+                                        ("silu", INF, NAN, NAN, NAN)):
+        y, (_, _, db) = _step(x, w, b, None, act, dy)
+        for j, v, d in ((1, high, dhigh), (2, low, dlow)):
+            want = torch.full_like(y[:, j], v)
+            assert torch.equal(y[:, j].nan_to_num(nan=7.0), want.nan_to_num(nan=7.0)), (act, j, y[:3, j])
+            if math.isnan(d):
+                assert bool(torch.isnan(db[j]))
+            else:
+                total = dy[:, j].double().sum() * d
+                assert abs(float(db[j]) - float(total)) <= float((M + 16) * hl.E * dy[:, j].double().abs().sum() * d
+                                                                 + hl.last(dt, total.abs()))
+
+
+# ---- the far tails ----
+def _tail_values(dt):
+    v = [0.0, 2.0 ** -9, 0.5, 3.0, 5.0, 5.5, 6.0, 6.5, 7.0, 8.0, 9.0, 10.0, 11.0, 12.0, 12.5, 13.0, 13.5, 14.0, 15.0,
+         16.0, 17.0, 18.0, 19.0, 20.0, 24.0, 30.0, 40.0, 43.0, 60.0, 80.0, 86.5, 87.5, 88.0, 89.0, 100.0, 127.0, 200.0,
+         1000.0, 60000.0]
+    if dt != F16:
+        v += [1e6, 1e20, 1e30, 1e37, 2e38, torch.finfo(dt).max]
+    t = torch.tensor(v, dtype=torch.float64).to(dt)
+    return torch.cat([t, -t]).cuda()
+
+
+@pytest.mark.parametrize("dt", [F32, F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "sigmoid"])
+@pytest.mark.parametrize("M,K,N,image", [(90, 16, 8, False), (700, 16, 64, False), (700, 4, 8, True), (700, 16, 130, True),
+                                         (700, 136, 64, False)])
+def test_activations_far_out(M, K, N, image, act, dt):
+    # z is one element of x, so it is exact; y and act' at every magnitude the type holds, with and without gradients
+    import volume_integration.heads as heads
+    values = _tail_values(dt)
+    z = values.repeat(M // values.numel() + 1)[:M]
+    x = torch.zeros(K, M, device="cuda", dtype=dt).t() if image else torch.zeros(M, K, device="cuda", dtype=dt)
+    w = torch.zeros(N, K, device="cuda", dtype=dt)
+    x[:, 1], w[:, 1] = z, 1.0
+    dy = torch.zeros(N, M, device="cuda", dtype=dt).t() if image else torch.zeros(M, N, device="cuda", dtype=dt)
+    dy[:, 3] = 1.0
+    y, (dx, _) = _step(x, w, None, None, act, dy)
+    with torch.no_grad():
+        assert torch.equal(heads.linear_act(x, w, None, None, act), y)
+    y64, d64 = hl.act64(act, z.double())
+    u = hl.half_step(dt)
+    # silu and sigmoid to 64 e of the value; where 1 / (1 + exp(-z)) is below 2^-126 the 16-bit forms may take it for 0,
+    # 87.4 * 2^-126 of a product with z there.
+    # gelu's polynomial beside 16-bit types: 64 e of the value down to 1e-3, then 1e-7 absolute of it to -5,
+    # and 2% of what is left (below 1e-6) beyond, where Phi < 3e-7.
+    by = (u + 64 * hl.E) * y64.abs() + hl.tiny(dt) + 2.0 ** -119
+    bd = (3 * u + 64 * hl.E) * d64.abs() + 2.0 ** -119
+    if act == "gelu":
+        zd = z.double()
+        far = zd < -5
+        floor = torch.full_like(zd, 1e-7)
+        by = by + torch.where(far, 0.02 * y64.abs(), torch.where(zd < 0, floor, 0 * floor))
+        # act' = Q + x phi: its terms are up to 1/2, and cancel near their zero
+        bd = bd + torch.where(far, 0.02 * d64.abs(), 64 * hl.E * torch.full_like(zd, 0.5) + floor)
+    if dt == BF16:
+        bd = bd + 2.0 ** -70  # the kept form's smallest steps
+    if dt == F16:
+        bd = bd + 2.0 ** -26 + 2.0 ** -24  # the kept form's, and s's and dx's own
+    hl.assert_within("y", y[:, 5], (y64, by))
+    hl.assert_within("act'", dx[:, 1], (d64, bd))

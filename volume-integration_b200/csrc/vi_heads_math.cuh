@@ -54,7 +54,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // act' of a NaN is a NaN too, but relu's, which is 0 there (z > 0 is false).
 //
 // sigmoid: with e = exp(-z), s = 1 / (1 + e) and 1 - s = e s, without cancellation
-// for large z; for the slope e is kept finite, so e s tends to 1 and not to inf * 0.
+// for large z.  The slope's e is kept finite, so that e s is 0 and not inf * 0 where s is 0; the
+// value does not depend on whether the slope is wanted.
 // gelu: with x = -|z| and Q = Phi(x), z Phi(z) = max(z, 0) + x Q, and act' is h = Q + x phi(x) for
 // z < 0, 1 - h else.  log2 Phi is smooth on [-6, 0]; Q is exp2 of a polynomial of degree 7
 // fitted to it here by iteratively reweighted least squares (6e-6 of the value in float32).
@@ -69,16 +70,15 @@ __device__ __forceinline__ void activate(float2 z, float2& y, float2& d) {
   } else if constexpr (ACT == VI_ACT_SILU || ACT == VI_ACT_SIGMOID) {
     float2 e, s;
     if constexpr (EXACT) {
-      e = make_float2(expf(min_nan(-z.x, 87.0f)), expf(min_nan(-z.y, 87.0f)));
+      e = make_float2(expf(-z.x), expf(-z.y));
       s = make_float2(1.0f / (1.0f + e.x), 1.0f / (1.0f + e.y));
     } else {
       const float2 t = __fmul2_rn(z, pair(-kLog2e));
-      e = SLOPE ? make_float2(exp2_fast(min_nan(t.x, 126.0f)), exp2_fast(min_nan(t.y, 126.0f)))
-                : make_float2(exp2_fast(t.x), exp2_fast(t.y));
+      e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
       const float2 q = __fadd2_rn(e, pair(1.0f));
       s = make_float2(rcp_fast(q.x), rcp_fast(q.y));
     }
-    const float2 c = __fmul2_rn(e, s);
+    const float2 c = __fmul2_rn(make_float2(min_nan(e.x, 0x1p126f), min_nan(e.y, 0x1p126f)), s);
     if constexpr (ACT == VI_ACT_SILU) {
       y = __fmul2_rn(z, s);
       d = __fmul2_rn(s, __ffma2_rn(z, c, pair(1.0f)));
