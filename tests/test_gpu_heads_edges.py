@@ -113,7 +113,7 @@ def _tail_values(dt):
     return torch.cat([t, -t]).cuda()
 
 
-@pytest.mark.parametrize("dt", [F32, F16], ids=["f32", "f16"])
+@pytest.mark.parametrize("dt", **TYPES)
 @pytest.mark.parametrize("act", hl.ACTS)
 @pytest.mark.parametrize("M,K,N,image", [(90, 16, 8, False), (700, 16, 64, False), (700, 4, 8, True), (700, 16, 130, True),
                                          (700, 136, 64, False)])

@@ -121,36 +121,34 @@ __device__ __forceinline__ void activate(float2 z, float2& y, float2& d) {
 
 // act' lies in (-0.2, 1.2) and is kept in 16 bits beside 16-bit types, more precisely
 // than they hold values, so that the product dy * act' is off by its own rounding
-// and little else: beside bfloat16 as float16 (half a step 2^-11 of the value, a quarter
-// of bfloat16's), beside float16 with a sign, 4 bits of exponent and 11 of mantissa (2^-12,
-// half of float16's, down to 2^-14; 2^-26 absolute below).  For the latter the float
-// scaled by 2^-112 has its exponent in the low 4 bits of the field; a NaN, like all above the
-// range, becomes the largest code, which no act' has.
-template <typename T>
-struct Slope;
-template <>
-struct Slope<__nv_bfloat16> {
+// and little else: a sign, EXP bits of exponent and the rest of mantissa, scaled so that the largest exponent is
+// that of 1.  Beside float16 4 and 11 (half a step 2^-12 of the value, half of float16's, down to 2^-14;
+// 2^-26 absolute below).  Beside bfloat16, whose range a saturated unit's gradient may use, 6 and 9 (2^-10, a quarter of
+// bfloat16's, down to 2^-62; as float16 it was 0 from sigmoid(18) on).  The float scaled by 2^(2^EXP - 128) has its
+// exponent in the low EXP bits of the field; a NaN, like all above the range, becomes the largest code, which no
+// act' has.
+template <int EXP>
+struct SlopeCode {
+  static constexpr uint32_t kShift = 8 + EXP, kHalf = 1u << (kShift - 1), kNan = 0x7fff;
+  static constexpr float kScale = EXP == 4 ? 0x1p-112f : 0x1p-64f;
   static __device__ __forceinline__ uint32_t pack(float2 d) {
-    const __half2 h = __float22half2_rn(d);
-    return *(const uint32_t*)&h;
-  }
-  static __device__ __forceinline__ float unpack(uint16_t v) { return __half2float(__ushort_as_half(v)); }
-};
-template <>
-struct Slope<__half> {
-  static __device__ __forceinline__ uint32_t pack(float2 d) {
-    const float2 s = __fmul2_rn(d, pair(0x1p-112f));
+    const float2 s = __fmul2_rn(d, pair(kScale));
     const uint32_t a = __float_as_uint(s.x), b = __float_as_uint(s.y);
-    const uint32_t m = min(((a & 0x7fffffffu) + 0x800u) >> 12, kNan), n = min(((b & 0x7fffffffu) + 0x800u) >> 12, kNan);
+    const uint32_t m = min(((a & 0x7fffffffu) + kHalf) >> kShift, kNan), n = min(((b & 0x7fffffffu) + kHalf) >> kShift, kNan);
     return m | (n << 16) | ((a >> 16) & 0x8000u) | (b & 0x80000000u);
   }
   static __device__ __forceinline__ float unpack(uint16_t v) {
     const uint32_t a = v & 0x7fffu;
-    const float m = a == kNan ? NAN : __uint_as_float(a << 12) * 0x1p112f;
+    const float m = a == kNan ? NAN : __uint_as_float(a << kShift) * (1.0f / kScale);
     return v & 0x8000u ? -m : m;
   }
-  static constexpr uint32_t kNan = 0x7fff;
 };
+template <typename T>
+struct Slope;
+template <>
+struct Slope<__nv_bfloat16> : SlopeCode<6> {};
+template <>
+struct Slope<__half> : SlopeCode<4> {};
 
 // act' as kept: the code above (float32 beside float32), or for relu anything that is positive where it
 // is 1, so that the result itself serves (a NaN is not).
