@@ -353,7 +353,8 @@ int vi_linear_act_keeps_dact(int dtype, int activation, const vi_matrix* x, cons
  * Gradients of vi_linear_act_forward for an incoming dy [M,N] (any strides):
  * with s = dy * act', dx = s weight, dweight = s^T x, dbias = the column sums of
  * s.  dact is the forward's; for VI_ACT_RELU its result y serves as well, if there
- * was no residual (positive means 1); NULL: act' is computed again from x, weight
+ * was no residual (positive means 1, and so does float16's -0, which the forward writes
+ * for a positive value that rounds to 0); NULL: act' is computed again from x, weight
  * and bias (which is read for nothing else).  Each of dx, dweight, dbias may be NULL; dx
  * and dweight have one of their strides 1.  The residual's gradient is dy itself.
  */

@@ -151,3 +151,23 @@ def test_activations_far_out(M, K, N, image, act, dt):
         bd = bd + 2.0 ** -26 + 2.0 ** -24  # the kept form's, and s's and dx's own
     hl.assert_within("y", y[:, 5], (y64, by))
     hl.assert_within("act'", dx[:, 1], (d64, bd))
+
+
+@pytest.mark.parametrize("M,K,N,order", [(60, 25, 40, "rows"), (60, 24, 40, "rows"), (900, 24, 40, "rows"),
+                                         (900, 4, 40, "image"), (900, 24, 130, "image")])
+@pytest.mark.parametrize("residual", [False, True])
+def test_relu_of_a_value_under_the_type(M, K, N, order, residual):
+    # float16: z = 2^-26 rounds to a result of 0, but it is positive, and its gradient passes
+    x, _, _, r, dy = _inputs(M, K, N, F16, order, False, residual, 62)
+    x.zero_()
+    w = torch.zeros(N, K, device="cuda", dtype=F16)
+    x[:, 2] = 2.0 ** -13
+    x[::3, 2] = -2.0 ** -13
+    w[:, 2] = 2.0 ** -13
+    y, grads = _step(x, w, None, r, "relu", dy)
+    assert torch.equal(y, r if residual else torch.zeros_like(y))
+    s = dy.double() * (x[:, 2:3] > 0)
+    value, bound = hl.weighted_sum(s, torch.zeros_like(s), w, F16)
+    hl.assert_within("dx", grads[0], (value, bound + hl.last(F16, value.abs() + bound)))
+    value, bound = hl.weighted_sum(s.t(), torch.zeros_like(s.t()), x, F16)
+    hl.assert_within("dweight", grads[1], (value, bound + hl.last(F16, value.abs() + bound)))

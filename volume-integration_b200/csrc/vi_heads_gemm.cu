@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
                   for (int j = 0; j < 8; j++) {
                     float2 w, s;
                     activate<ACT, sizeof(T) == 4, kSlope>(v[j], w, s);
-                    v[j] = w;
+                    v[j] = ACT == VI_ACT_RELU ? relu_signed_zero<T>(w) : w;
                     if constexpr (kSlope) {
                       if constexpr (sizeof(T) == 4) set_pair(d, h * 8 + j, s);
                       else d.w[h * 8 + j] = Slope<T>::pack(s);

@@ -150,12 +150,22 @@ struct Slope<__nv_bfloat16> : SlopeCode<6> {};
 template <>
 struct Slope<__half> : SlopeCode<4> {};
 
+// A relu result that may serve as its act': a positive value that float16 rounds to 0 becomes -0 (equal to it, but told
+// from the 0 of z <= 0), so that its gradient passes.  bfloat16's smallest step is below float32's normal range.
+template <typename T>
+__device__ __forceinline__ float2 relu_signed_zero(float2 y) {
+  if constexpr (std::is_same<T, __half>::value)
+    return make_float2(y.x > 0.0f && y.x <= 0x1p-25f ? -0.0f : y.x, y.y > 0.0f && y.y <= 0x1p-25f ? -0.0f : y.y);
+  return y;
+}
+
 // act' as kept: the code above (float32 beside float32), or for relu anything that is positive where it
-// is 1, so that the result itself serves (a NaN is not).
+// is 1, so that the result itself serves (float16's -0 is, a NaN is not).
 template <typename T>
 __device__ __forceinline__ float kept_slope(uint16_t v, bool relu) {
-  constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return relu ? ((uint32_t)v - 1u < kInf ? 1.0f : 0.0f) : Slope<T>::unpack(v);
+  constexpr bool kIsHalf = std::is_same<T, __half>::value;
+  constexpr uint32_t kInf = kIsHalf ? 0x7c00u : 0x7f80u;
+  return relu ? ((uint32_t)v - 1u < kInf || (kIsHalf && v == 0x8000u) ? 1.0f : 0.0f) : Slope<T>::unpack(v);
 }
 __device__ __forceinline__ float kept_slope(float v, bool relu) { return relu ? (v > 0.0f ? 1.0f : 0.0f) : v; }
 

@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(kThreads) small_kernel(const __grid_constant__
       } else {
         float d;
         activate1(q.act, sizeof(T) == 4, z * alpha, z, d);
+        if (q.act == VI_ACT_RELU) z = relu_signed_zero<T>(pair(z)).x;
         if (q.dact) {
           const int64_t at = m * q.out.rs + n * q.out.cs;
           if constexpr (sizeof(T) == 4) ((float*)q.dact)[at] = d;
