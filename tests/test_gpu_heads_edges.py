@@ -171,3 +171,31 @@ def test_relu_of_a_value_under_the_type(M, K, N, order, residual):
     hl.assert_within("dx", grads[0], (value, bound + hl.last(F16, value.abs() + bound)))
     value, bound = hl.weighted_sum(s.t(), torch.zeros_like(s.t()), x, F16)
     hl.assert_within("dweight", grads[1], (value, bound + hl.last(F16, value.abs() + bound)))
+
+
+# ---- tangents ----
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwad
+    import volume_integration.heads as heads
+    x, w, b, r, _ = _inputs(20, 8, 9, F32, "rows", True, True, 68)
+    t = torch.zeros(20, dtype=torch.int64, device="cuda")
+    with fwad.dual_level():
+        for i in range(4):
+            v = [x, w, b, r]
+            v[i] = fwad.make_dual(v[i], torch.ones_like(v[i]))
+            for grad in (False, True):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    heads.linear_act(*v, activation="silu")
+                if i < 3:
+                    with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                        heads.linear_cross_entropy(v[0], v[1], t, v[2])
+    heads.linear_act(x, w, b, r)  # and nothing is left behind
+    # nor does a backward drop the tangent of what comes in
+    y = heads.linear_act(x.requires_grad_(True), w, b, r)
+    loss = heads.linear_cross_entropy(x, w, t, b)
+    with fwad.dual_level():
+        for out in (y, loss):
+            dual = fwad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, (x,), dual, retain_graph=True)
+    torch.autograd.grad(y, (x,), torch.ones_like(y))

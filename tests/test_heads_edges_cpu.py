@@ -3,6 +3,9 @@
 import subprocess
 import sys
 
+import pytest
+import torch
+
 # The queries in a process of their own: a division by zero there would end this one.
 QUERIES = """
 import ctypes, sys
@@ -28,3 +31,22 @@ def test_many_rows_of_many_features():
     assert len(lines) == 2 * len(cases)
     for dt, M, K, V, got in lines:  # the masked copy of x, and one piece of G
         assert got >= (M * K + M * min(V, 256)) * 2 * (3 if dt == 0 else 1)
+
+
+def test_tangents_are_refused():
+    # before anything else is looked at, so that no device is needed to see it
+    import torch.autograd.forward_ad as fwad
+    from volume_integration import _C
+    x, w, b, r = torch.randn(6, 4), torch.randn(5, 4), torch.randn(5), torch.randn(6, 5)
+    t = torch.zeros(6, dtype=torch.int64)
+    with fwad.dual_level():
+        for i in range(4):
+            v = [x, w, b, r]
+            v[i] = fwad.make_dual(v[i], torch.ones_like(v[i]))
+            with pytest.raises(RuntimeError, match="linear_act: forward-mode"):
+                _C.linear_act(v[0], v[1], v[2], v[3], 0)
+            if i < 3:
+                with pytest.raises(RuntimeError, match="linear_cross_entropy: forward-mode"):
+                    _C.linear_cross_entropy(v[0], v[1], v[2], t, -100, 1)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        _C.linear_act(x, w, None, None, 0)

@@ -540,6 +540,12 @@ void differentiate_once(variable_list& grads) {
   for (size_t i = 0; i < at.size(); i++) grads[at[i]] = out[i];
 }
 c10::optional<Tensor> optional_of(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
+// The kernels carry no tangents, and an input with one need not require a gradient: it would be dropped without a word.
+template <class... T>
+void no_tangents(const char* what, const T&... ts) {
+  const auto has = [](const c10::optional<Tensor>& t) { return t.has_value() && t->defined() && t->_fw_grad(0).defined(); };
+  TORCH_CHECK(!(has(ts) || ...), what, ": forward-mode differentiation is not supported");
+}
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const c10::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
 
@@ -561,6 +567,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dys) {
+    no_tangents("linear_act backward", dys[0]);
     const variable_list saved = ctx->get_saved_variables();
     const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = has_b && ctx->needs_input_grad(2);
@@ -580,6 +587,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
 
 Tensor linear_act(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias,
                   const c10::optional<Tensor>& residual, int64_t activation) {
+  no_tangents("linear_act", x, weight, bias, residual);
   if (torch::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias) || wants_grad(residual)))
     return LinearAct::apply(x, weight, bias, residual, activation);
   return std::get<0>(linear_act_forward(x, weight, bias, residual, activation, false));
@@ -596,6 +604,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dloss) {
+    no_tangents("linear_cross_entropy backward", dloss[0]);
     const variable_list saved = ctx->get_saved_variables();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
     const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
@@ -615,6 +624,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
 
 Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const c10::optional<Tensor>& bias,
                             const Tensor& target, int64_t ignore_index, int64_t reduction) {
+  no_tangents("linear_cross_entropy", x, weight, bias);
   if (torch::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
     return LinearCrossEntropy::apply(x, weight, bias, target, ignore_index, reduction);
   return std::get<0>(linear_ce_forward(x, weight, bias, target, ignore_index, reduction));
