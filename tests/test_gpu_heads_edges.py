@@ -173,6 +173,26 @@ def test_relu_of_a_value_under_the_type(M, K, N, order, residual):
     hl.assert_within("dweight", grads[1], (value, bound + hl.last(F16, value.abs() + bound)))
 
 
+# ---- incoming gradients ----
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("M,V", [(60, 40), (900, 700)])
+def test_ignored_rows_under_an_infinite_gradient(M, V, reduction, dt):
+    # a scaled loss that overflows: ignored rows have no part in it
+    import volume_integration.heads as heads
+    g = _gen(66)
+    x, w = hl.matrix(M, 24, dt, g), hl.matrix(V, 24, dt, g)
+    t = torch.randint(0, V, (M,), generator=g, device="cuda")
+    t[::4] = -100
+    for v in (INF, NAN):
+        xl = x.clone().requires_grad_(True)
+        loss = heads.linear_cross_entropy(xl, w, t, reduction=reduction)
+        (dx,) = torch.autograd.grad(loss, (xl,), torch.tensor(v, device="cuda"))
+        assert float(dx[::4].abs().max()) == 0.0
+        live = torch.arange(M, device="cuda") % 4 != 0
+        assert not bool(torch.isfinite(dx[live]).any())
+
+
 # ---- tangents ----
 def test_forward_mode_is_refused():
     import torch.autograd.forward_ad as fwad

@@ -403,13 +403,16 @@ __global__ void __launch_bounds__(256) coef_kernel(const int64_t* target, int64_
   int ex = 0;
   frexpf(top, &ex);
   ex = min(max(ex, -100), 100);  // a power of two at or above every finite |g|: the division is exact
-  if (blockIdx.x == 0 && threadIdx.x == 0)
-    *alpha = (reduction == VI_REDUCE_NONE  ? ldexpf(1.0f, ex)
-              : reduction == VI_REDUCE_SUM ? *dloss
-              : live                       ? *dloss / (float)live
-                                           : 0.0f) / lift;
+  // a common size that is not finite stays in the rows that it belongs to: at the products' end it would
+  // meet the zeros of the ignored ones
+  const float common = reduction == VI_REDUCE_NONE  ? ldexpf(1.0f, ex)
+                       : reduction == VI_REDUCE_SUM ? *dloss
+                       : live                       ? *dloss / (float)live
+                                                    : 0.0f;
+  const bool finite = isfinite(common);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *alpha = (finite ? common : 1.0f) / lift;
   for (int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x; m < M; m += (int64_t)gridDim.x * 256) {
-    const float g = reduction == VI_REDUCE_NONE ? ldexpf(dloss[m], -ex) : 1.0f;
+    const float g = reduction == VI_REDUCE_NONE ? ldexpf(dloss[m], -ex) : finite ? 1.0f : common;
     coef[m] = target[m] != ignore ? g * lift : 0.0f;
   }
 }
