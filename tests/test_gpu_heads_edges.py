@@ -193,6 +193,32 @@ def test_ignored_rows_under_an_infinite_gradient(M, V, reduction, dt):
         assert not bool(torch.isfinite(dx[live]).any())
 
 
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("M,K,N", [(40, 24, 30), (700, 72, 136)])
+def test_c_callers_derivative_of_no_activation(M, K, N, dt):
+    # dact is written for every activation, and a backward that is given it agrees with one that is not
+    lib = ha.load()
+    p = ctypes.c_void_p
+    x, w, _, _, dy = _inputs(M, K, N, dt, "rows", False, False, 67)
+    y, d = torch.empty_like(dy), torch.full_like(dy, NAN)
+    stream = p(torch.cuda.current_stream().cuda_stream)
+    args = (ha.DTYPE[dt], 0, ha.matrix(x), ha.matrix(w), None, None, ha.matrix(y), ha.matrix(d))
+    n = lib.vi_linear_act_forward_scratch_bytes(*args)
+    scratch = torch.empty(max(n, 1 << 22), device="cuda", dtype=torch.uint8)
+    assert lib.vi_linear_act_forward(*args, p(scratch.data_ptr()), n, stream) == 0, lib.vi_last_error()
+    hl.assert_within("y", y, hl.linear_act(x, w, None, None, "none")[0])
+    grads = []
+    for da in (None, ha.matrix(d)):
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        args = (ha.DTYPE[dt], 0, ha.matrix(dy), da, ha.matrix(x), ha.matrix(w), None, ha.matrix(dx), ha.matrix(dw), None)
+        n = lib.vi_linear_act_backward_scratch_bytes(*args)
+        scratch = torch.empty(n, device="cuda", dtype=torch.uint8)
+        assert lib.vi_linear_act_backward(*args, p(scratch.data_ptr()), n, stream) == 0, lib.vi_last_error()
+        grads.append((dx, dw))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+
+
 # ---- tangents ----
 def test_forward_mode_is_refused():
     import torch.autograd.forward_ad as fwad

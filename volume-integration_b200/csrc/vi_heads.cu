@@ -240,6 +240,18 @@ __global__ void __launch_bounds__(256) strip_image_kernel(const __grid_constant_
   }
 }
 
+// act' of no activation, 1, as kept: for a caller that asks for it (the backward does not read it).
+template <typename T>
+__global__ void __launch_bounds__(256) ones_kernel(View d, int64_t M, int64_t N) {
+  const bool by_col = d.cs == 1;
+  const int64_t run = by_col ? N : M, total = M * N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t hi = i / run, at = hi * (by_col ? d.rs : d.cs) + (i - hi * run);
+    if constexpr (sizeof(T) == 4) ((float*)d.p)[at] = 1.0f;
+    else ((uint16_t*)d.p)[at] = (uint16_t)Slope<T>::pack(pair(1.0f));
+  }
+}
+
 // out(r, c) = alpha * sum of the pieces' elements (r, c), added in a fixed order.  Up to two jobs a launch.
 struct SumJob {
   const float* part;
@@ -763,7 +775,12 @@ int act_forward(Run& r, int dtype, int act, const vi_matrix* x, const vi_matrix*
   e.bias = bias;
   e.res = view(res);
   e.out = view(y);
-  e.dact = dact ? dact->data : nullptr;
+  e.dact = dact && act != VI_ACT_NONE ? dact->data : nullptr;
+  if (act == VI_ACT_NONE && dact && dact->data && !r.dry) {
+    const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div(M * N, 256), 148 * 16);
+    VI_DISPATCH(dtype, (ones_kernel<T><<<blocks, 256, 0, r.s>>>(view(dact), M, N)));
+    r.launches++;
+  }
   if (!e.dact && narrow_forward(N, K, view(x), e.out, e.res)) {
     if (r.dry) return VI_OK;
     const cudaError_t rc = launch_narrow(dtype, NarrowArgs{M, (int)N, (int)K, act, view(x), view(w), bias, e.out, e.res},
@@ -804,7 +821,7 @@ int act_backward(Run& r, int dtype, int act, const vi_matrix* dy, const vi_matri
     zero_gradients(r, dtype, N, K, dw, db);
     return VI_OK;
   }
-  View slope = view(dact);
+  View slope = act == VI_ACT_NONE ? View{nullptr, 0, 0} : view(dact);
   const bool need_dx = dx && dx->data, need_dw = dw && dw->data;
   Summer sums{r, dtype};
   if (!slope.p && narrow_backward(N, K, view(x), view(dy), view(dx))) {
