@@ -404,6 +404,10 @@ int vi_linear_ce_backward(int dtype, const vi_matrix* x, const vi_matrix* weight
  */
 int vi_heads_status(uint32_t* status, int reset, void* stream);
 
+/* How many of the heads' products this process has launched with 256 x 256 tiles, which pairs of blocks make (for
+ * tests and measurements: which sizes take them is a rule on sizes and the number of SMs). */
+uint64_t vi_heads_pair_launches(void);
+
 /* Reads the status word a forward latched in its geometry buffer (blocks). */
 int vi_read_device_status(const char* geom_buffer, uint32_t* status, void* stream);
 

@@ -173,6 +173,103 @@ def test_relu_of_a_value_under_the_type(M, K, N, order, residual):
     hl.assert_within("dweight", grads[1], (value, bound + hl.last(F16, value.abs() + bound)))
 
 
+# ---- tiles made by pairs of blocks ----
+def _pairs():
+    lib = ha.load()
+    lib.vi_heads_pair_launches.restype = ctypes.c_uint64
+    return lib.vi_heads_pair_launches()
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("M,K,N,act,order,bias,residual,pairs", [
+    # 64 tiles of 256 x 256 (one wave of 74 pairs, where narrower tiles take two and more): the forward's,
+    # dx's where K is as wide, and dweight's in pieces
+    (4096, 1024, 1024, "silu", "rows", True, True, 3),
+    (4090, 1020, 1020, "gelu", "rows", True, True, 3),
+    (4093, 1016, 1021, "gelu", "image", True, True, 3),
+    (4090, 1020, 1020, "relu", "image", True, False, 3),
+    (4088, 1024, 1016, "sigmoid", "image", True, True, 3),
+    (4096, 520, 1024, "sigmoid", "padded", True, False, 1),
+    (4090, 136, 1020, "none", "odd", False, True, 1),
+])
+def test_linear_act_on_tiles_of_pairs(M, K, N, act, order, bias, residual, pairs, dt):
+    import volume_integration.heads as heads
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("the sizes fill 148 SMs")
+    x, w, b, r, dy = _inputs(M, K, N, dt, order, bias, residual, M + N)
+    before = _pairs()
+    with torch.no_grad():
+        y = heads.linear_act(x, w, b, r, act)
+    assert _pairs() == before + 1
+    _check(x, w, b, r, act, dy)
+    assert _pairs() >= before + 1 + pairs
+    assert torch.equal(_step(x, w, b, r, act, dy)[0], y)
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("M,K,V,order", [(4096, 1024, 4096, "rows"), (4090, 1020, 4090, "image")])
+def test_label_gradients_on_tiles_of_pairs(M, K, V, order, dt):
+    import volume_integration.heads as heads
+    g = _gen(M)
+    x, w = hl.matrix(M, K, dt, g, order), hl.matrix(V, K, dt, g, scale=3.0 / K ** 0.5)
+    t = torch.randint(0, V, (M,), generator=g, device="cuda")
+    t[::9] = -100
+    leaves = [v.detach().requires_grad_(True) for v in (x, w)]
+    before = _pairs()
+    loss = heads.linear_cross_entropy(leaves[0], leaves[1], t)
+    grads = torch.autograd.grad(loss, leaves)
+    assert torch.cuda.get_device_properties(0).multi_processor_count != 148 or _pairs() == before + 2
+    want = hl.linear_ce(x, w, None, t, -100, "mean", torch.ones((), device="cuda"))
+    for name, got, ref in zip(("loss", "dx", "dweight"), (loss.detach(),) + grads, want):
+        hl.assert_within(name, got, ref)
+
+
+def test_tiles_of_pairs_captured_and_on_two_streams():
+    x, w, b, r, dy = _inputs(4090, 1020, 1020, BF16, "rows", True, True, 69)
+    before = _pairs()
+    want = _step(x, w, b, r, "silu", dy)
+    assert _pairs() >= before + 3 or torch.cuda.get_device_properties(0).multi_processor_count != 148
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _step(x, w, b, r, "silu", dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _step(x, w, b, r, "silu", dy)
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(3):  # a replay beside two eager streams
+        graph.replay()
+        for s in (side, torch.cuda.Stream()):
+            s.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(s):
+                results.append(_step(x, w, b, r, "silu", dy))
+    torch.cuda.synchronize()
+    for y, grads in results + [out]:
+        assert torch.equal(y, want[0])
+        for a, c in zip(grads, want[1]):
+            assert torch.equal(a, c)
+    del graph
+
+
+@pytest.mark.parametrize("K", [200, 1000])  # fewer blocks of k than stages, and more
+def test_a_wait_that_runs_out_in_a_pair_is_reported(K, monkeypatch):
+    # the first load is withheld and the waits are short: both blocks of a pair give up and say so
+    import volume_integration.heads as heads
+    x, w, _, _, _ = _inputs(4090, K, 1020, BF16, "rows", False, False, 70)
+    before = _pairs()
+    want = heads.linear_act(x, w)
+    assert _pairs() == before + 1 or torch.cuda.get_device_properties(0).multi_processor_count != 148
+    assert heads.device_status(reset=True) == 0
+    monkeypatch.setenv("VI_HEADS_TEST_TIMEOUT", "1")
+    heads.linear_act(x, w)
+    assert heads.device_status(reset=True) == 8
+    monkeypatch.delenv("VI_HEADS_TEST_TIMEOUT")
+    assert torch.equal(heads.linear_act(x, w), want)  # and nothing is left behind
+    assert heads.device_status() == 0
+
+
 # ---- incoming gradients ----
 @pytest.mark.parametrize("dt", **TYPES)
 @pytest.mark.parametrize("reduction", ["mean", "sum"])

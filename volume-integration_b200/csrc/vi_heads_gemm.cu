@@ -1024,6 +1024,8 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
 }
 
 // ---- host ----
+std::atomic<uint64_t> g_pair_launches{0};
+
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1170,11 +1172,14 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
     return set_error(VI_ERR_CUDA, msg);
   }
   note_launches(1);
+  if (pair) g_pair_launches.fetch_add(1, std::memory_order_relaxed);
   return VI_OK;
 }
 
 }  // namespace heads
 }  // namespace vi
+
+extern "C" uint64_t vi_heads_pair_launches(void) { return vi::heads::g_pair_launches.load(); }
 
 extern "C" int vi_heads_status(uint32_t* status, int reset, void* stream) {
   using namespace vi;
