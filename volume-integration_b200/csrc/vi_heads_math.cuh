@@ -121,34 +121,39 @@ __device__ __forceinline__ void activate(float2 z, float2& y, float2& d) {
 
 // act' lies in (-0.2, 1.2) and is kept in 16 bits beside 16-bit types, more precisely
 // than they hold values, so that the product dy * act' is off by its own rounding
-// and little else: a sign, EXP bits of exponent and the rest of mantissa, scaled so that the largest exponent is
-// that of 1.  Beside float16 4 and 11 (half a step 2^-12 of the value, half of float16's, down to 2^-14;
-// 2^-26 absolute below).  Beside bfloat16, whose range a saturated unit's gradient may use, 6 and 9 (2^-10, a quarter of
-// bfloat16's, down to 2^-62; as float16 it was 0 from sigmoid(18) on).  The float scaled by 2^(2^EXP - 128) has its
-// exponent in the low EXP bits of the field; a NaN, like all above the range, becomes the largest code, which no
-// act' has.
-template <int EXP>
-struct SlopeCode {
-  static constexpr uint32_t kShift = 8 + EXP, kHalf = 1u << (kShift - 1), kNan = 0x7fff;
-  static constexpr float kScale = EXP == 4 ? 0x1p-112f : 0x1p-64f;
+// and little else.
+// Beside bfloat16 as float16 of act' * 2^15 (half a step 2^-11 of the value, an eighth of bfloat16's, down to 2^-29;
+// 2^-40 absolute below: a saturated unit keeps its gradient to sigmoid(27), where float16 alone gave 0 from 18 on).  A code
+// with 6 bits of exponent and 9 of mantissa reached 2^-62, but packing it cost the forward of 65536 x 512 -> 512 with
+// silu 10 us of 97.
+// Beside float16 with a sign, 4 bits of exponent and 11 of mantissa (2^-12, half of float16's, down to 2^-14; 2^-26
+// absolute below).  The float scaled by 2^-112 has its exponent in the low 4 bits of the field; a
+// NaN, like all above the range, becomes the largest code, which no act' has.
+template <typename T>
+struct Slope;
+template <>
+struct Slope<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t pack(float2 d) {
-    const float2 s = __fmul2_rn(d, pair(kScale));
+    const __half2 h = __float22half2_rn(__fmul2_rn(d, pair(0x1p15f)));
+    return *(const uint32_t*)&h;
+  }
+  static __device__ __forceinline__ float unpack(uint16_t v) { return __half2float(__ushort_as_half(v)) * 0x1p-15f; }
+};
+template <>
+struct Slope<__half> {
+  static constexpr uint32_t kNan = 0x7fff;
+  static __device__ __forceinline__ uint32_t pack(float2 d) {
+    const float2 s = __fmul2_rn(d, pair(0x1p-112f));
     const uint32_t a = __float_as_uint(s.x), b = __float_as_uint(s.y);
-    const uint32_t m = min(((a & 0x7fffffffu) + kHalf) >> kShift, kNan), n = min(((b & 0x7fffffffu) + kHalf) >> kShift, kNan);
+    const uint32_t m = min(((a & 0x7fffffffu) + 0x800u) >> 12, kNan), n = min(((b & 0x7fffffffu) + 0x800u) >> 12, kNan);
     return m | (n << 16) | ((a >> 16) & 0x8000u) | (b & 0x80000000u);
   }
   static __device__ __forceinline__ float unpack(uint16_t v) {
     const uint32_t a = v & 0x7fffu;
-    const float m = a == kNan ? NAN : __uint_as_float(a << kShift) * (1.0f / kScale);
+    const float m = a == kNan ? NAN : __uint_as_float(a << 12) * 0x1p112f;
     return v & 0x8000u ? -m : m;
   }
 };
-template <typename T>
-struct Slope;
-template <>
-struct Slope<__nv_bfloat16> : SlopeCode<6> {};
-template <>
-struct Slope<__half> : SlopeCode<4> {};
 
 // A relu result that may serve as its act': a positive value that float16 rounds to 0 becomes -0 (equal to it, but told
 // from the 0 of z <= 0), so that its gradient passes.  bfloat16's smallest step is below float32's normal range.

@@ -68,7 +68,7 @@ def linear_act(x, weight, bias=None, residual=None, activation="none"):
 
     float16 and bfloat16 results are rounded once, from float32.  The backward
     keeps act' in 16 bits (float16: to 2^-12 of its value down to 2^-14, to 2^-26 absolute below;
-    bfloat16: to 2^-10 of its value down to 2^-62) and, but for small products, rounds the product of dy
+    bfloat16: to 2^-11 of its value down to 2^-29, to 2^-40 absolute below) and, but for small products, rounds the product of dy
     and act' to the operands' type before the two matrix products.
     """
     _check_operands(x, weight, bias, "linear_act", "N")
