@@ -173,6 +173,115 @@ def test_relu_of_a_value_under_the_type(M, K, N, order, residual):
     hl.assert_within("dweight", grads[1], (value, bound + hl.last(F16, value.abs() + bound)))
 
 
+# ---- long sums ----
+# The tensor core cuts what it adds towards zero, so a sum of positive terms drifts down: measured, 1.5e-3 over 262144
+# terms, as if each of four additions per 16 terms lost half a step of a running sum that is on average half its end: a step e
+# per 16 terms.  The chain without a rounded addition in between is 768 terms in float32 (48 e) and 16384 beside
+# float16 (1024 e), whatever the length.
+F32_CHAIN = 48 + 16
+
+
+@pytest.mark.parametrize("K,act,order", [(32768, "none", "rows"), (20011, "silu", "image")])
+def test_long_float32_products(K, act, order):
+    # every term positive: the whole drift adds up
+    import volume_integration.heads as heads
+    g = _gen(63)
+    x = torch.rand(K, 300, generator=g, device="cuda").t() if order == "image" else torch.rand(300, K, generator=g, device="cuda")
+    w = torch.rand(140, K, generator=g, device="cuda") / K
+    y = heads.linear_act(x, w, activation=act)
+    z = x.double() @ w.double().t()
+    y64, d = hl.act64(act, z)
+    # rounded additions of the pieces: half a step each
+    bound = (F32_CHAIN + K / 768 / 2) * hl.E * z * d.abs().clamp(min=1) + 32 * hl.E * y64.abs() + 1e-7
+    hl.assert_within("y", y, (y64, bound))
+
+
+@pytest.mark.parametrize("V", [2, 300])
+def test_long_float32_logits(V):
+    # class 0 has logit 0, the others about 20 from positive terms, so that a drift does not cancel
+    K, M = 32768, 260
+    g = _gen(64)
+    x = torch.rand(M, K, generator=g, device="cuda")
+    w = torch.rand(V, K, generator=g, device="cuda") * (80.0 / K)
+    w[0] = 0.0
+    t = torch.zeros(M, dtype=torch.int64, device="cuda")
+    import volume_integration.heads as heads
+    wl = w.clone().requires_grad_(True)
+    loss = heads.linear_cross_entropy(x, wl, t, reduction="none")
+    (dw,) = torch.autograd.grad(loss.sum(), (wl,))
+    z = x.double() @ w.double().t()
+    lse = torch.logsumexp(z, 1)
+    dz = (F32_CHAIN + K / 768 / 2) * hl.E * z
+    bound = dz.max(1).values + (V + 16) * hl.E + 8 * hl.E * lse
+    hl.assert_within("loss", loss.detach(), (lse, bound))
+    # G = p - onehot: p off by p (dz + dlse + 16 e (1 + |z - lse|))
+    p = torch.exp(z - lse[:, None])
+    G = p.clone()
+    G[:, 0] -= 1
+    bG = p * (dz + bound[:, None] + 16 * hl.E * (1 + (z - lse[:, None]).abs())) + 4 * hl.E * G.abs() + 1e-38
+    value, vb = hl.weighted_sum(G.t(), bG.t(), x, F32)
+    hl.assert_within("dweight", dw, (value, vb + 4 * hl.E * value.abs() + hl.last(F32, value.abs() + vb)))
+
+
+def test_long_float16_weight_gradients():
+    # 262144 rows into 2048 x 2048: as many tiles as run at a time, so each is one long sum.  The mean over many
+    # elements leaves the drift: roundings of the result (u each, either way) average out.
+    M, N = 262144, 2048
+    g = _gen(65)
+    x = torch.empty(M, N, device="cuda", dtype=F16).uniform_(0.5, 1.5, generator=g)
+    dy = torch.empty(M, N, device="cuda", dtype=F16).uniform_(2.0 ** -12, 3 * 2.0 ** -12, generator=g)
+    w = torch.zeros(N, N, device="cuda", dtype=F16).requires_grad_(True)
+    import volume_integration.heads as heads
+    (dw,) = torch.autograd.grad(heads.linear_act(x, w), (w,), dy)
+    some = slice(0, N, 64)
+    want = dy[:, some].double().t() @ x.double()
+    drift = float(((dw[some].double() - want) / want).mean())
+    # the chain's 1024 e; 2^18 / 2^14 rounded additions; 65536 roundings of at most u
+    assert abs(drift) <= 1024 * hl.E + 16 * hl.E + 4 * 2.0 ** -11 / 256, drift
+
+
+@pytest.mark.parametrize("M,K,N,act,order,dt", [
+    (300, 20011, 140, "silu", "rows", F16), (300, 16448, 140, "gelu", "image", F16), (40, 20000, 1000, "relu", "rows", F16),
+    (130, 140003, 70, "sigmoid", "rows", BF16), (130, 5000, 70, "gelu", "image", F32), (700, 1003, 300, "relu", "odd", F32),
+])
+def test_long_products_with_everything(M, K, N, act, order, dt):
+    # more than a chain of k in the forward, with act', bias and residual; dx and dweight in their own tiles
+    x, w, b, r, dy = _inputs(M, K, N, dt, order, True, True, 71)
+    _check(x, w, b, r, act, dy)
+    _check(x, w, b, None, act, dy)
+
+
+@pytest.mark.parametrize("M,K,V,dt", [(260, 20000, 50, F16), (260, 16500, 300, F16), (130, 140000, 70, BF16),
+                                      (700, 1000, 5003, F32), (20000, 24, 21, F32)])
+def test_long_logits_and_long_gradients(M, K, V, dt):
+    import volume_integration.heads as heads
+    g = _gen(72)
+    x, w = hl.matrix(M, K, dt, g), hl.matrix(V, K, dt, g, scale=3.0 / K ** 0.5)
+    b = hl.matrix(1, V, dt, g, scale=0.5)[0]
+    t = torch.randint(0, V, (M,), generator=g, device="cuda")
+    t[::7] = -100
+    leaves = [v.detach().requires_grad_(True) for v in (x, w, b)]
+    loss = heads.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+    grads = torch.autograd.grad(loss, leaves)
+    want = hl.linear_ce(x, w, b, t, -100, "mean", torch.ones((), device="cuda"))
+    for name, got, ref in zip(("loss", "dx", "dweight", "dbias"), (loss.detach(),) + grads, want):
+        hl.assert_within(name, got, ref)
+
+
+def test_long_float32_gradients():
+    # positive terms again: dweight over 300000 rows, dx over 20000 columns
+    import volume_integration.heads as heads
+    g = _gen(73)
+    for M, K, N in ((300000, 70, 130), (260, 140, 20000)):
+        x = torch.rand(M, K, generator=g, device="cuda").requires_grad_(True)
+        w = torch.rand(N, K, generator=g, device="cuda").requires_grad_(True)
+        dy = torch.rand(M, N, generator=g, device="cuda") / max(M, N)
+        dx, dw = torch.autograd.grad(heads.linear_act(x, w), (x, w), dy)
+        for name, got, a, b, terms in (("dx", dx, dy, w, N), ("dweight", dw, dy.t(), x.t().contiguous().t(), M)):
+            want = a.double() @ b.detach().double()
+            hl.assert_within(name, got, (want, (F32_CHAIN + terms / 768 / 2) * hl.E * want))
+
+
 # ---- tiles made by pairs of blocks ----
 def _pairs():
     lib = ha.load()

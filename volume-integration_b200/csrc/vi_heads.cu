@@ -536,7 +536,8 @@ int64_t tile_slots(int epi, int bn, int sms) { return std::max(1, pair_tile(epi,
 
 // Tile width: the one whose waves of tiles take the least tensor-core time; narrow tiles
 // read their operands more often.
-int tile_width(int dtype, int epi, int64_t M, int64_t N, int sms) {
+int tile_width(int dtype, int epi, int64_t M, int64_t N, int64_t kblocks, int sms) {
+  if (long_chain_kernel(dtype, epi, kblocks)) return 128;
   int best = 64;
   double cost = 1e300;
   for (int bn : {256, 128, 64}) {
@@ -559,21 +560,22 @@ int gemm(Run& r, int dtype, int epi, const Operand& A, const Operand& B, const E
     f.res = transposed(e.res);
     f.bias_rows = e.bias != nullptr;
     Plan p{};
-    p.bn = tile_width(dtype, epi, B.rows, A.rows, r.sms);
     p.splits = 1;
     p.kps = (int)ceil_div(A.k, 64);
+    p.bn = tile_width(dtype, epi, B.rows, A.rows, p.kps, r.sms);
     return launch_gemm(dtype, epi, B, A, p, f, r.sms, r.s);
   }
   Plan p{};
-  p.bn = tile_width(dtype, epi, A.rows, B.rows, r.sms);
   p.splits = 1;
   p.kps = (int)ceil_div(A.k, 64);
+  p.bn = tile_width(dtype, epi, A.rows, B.rows, p.kps, r.sms);
   return launch_gemm(dtype, epi, A, B, p, e, r.sms, r.s);
 }
 
 // Pieces of a long sum over k: enough that the tiles fill the SMs, or fill their last wave where
 // that gains more than the pieces' float32 results cost to write and read (16384 x 512 over
-// 18944: 1.73 waves of tiles in one piece, 3.46 in two; 240 us -> 217).
+// 18944: 1.73 waves of tiles in one piece, 3.46 in two; 240 us -> 217).  Precision asks for no pieces: the product makes
+// a long one of chains (float32 dx of 16384 x 4096 <- 1024 in pieces of 768 terms: 1077 us, in chains 636).
 Plan split_plan(int dtype, const Operand& A, const Operand& B, int sms) {
   Plan p{};
   p.bn = B.rows <= 64 ? 64 : B.rows <= 128 || A.rows <= 128 || dtype == VI_F32 ? 128 : 256;
@@ -589,12 +591,6 @@ Plan split_plan(int dtype, const Operand& A, const Operand& B, int sms) {
       const double t = product * waves + (s > 1 ? copy * s : 0.0);
       if (t < best) best = t, want = s;
     }
-  }
-  if (dtype == VI_F32) {
-    // the tensor core cuts what it adds, always towards zero, so a float32 sum drifts with its length: 768
-    // terms a piece (9e-7 of the result; 1536 gave 1.8e-6, 14000 5e-6), while the pieces fit in 512 MB
-    const int64_t room = std::max<int64_t>(1, (512ll << 20) / (A.rows * B.rows * 4));
-    want = std::max(want, std::min(ceil_div(kb, 12), room));
   }
   p.kps = (int)ceil_div(kb, want);
   p.splits = (int)ceil_div(kb, p.kps);
@@ -899,7 +895,7 @@ int ce_forward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const 
   p.splits = 1;
   p.kps = (int)ceil_div(K, 64);
   // a small vocabulary in narrow tiles, two blocks per SM (640000 x 64 x 150: 88 us in one 256-wide tile, 81)
-  p.bn = V <= 64 ? 64 : V <= 256 ? 128 : tile_width(dtype, kEpiLse, M, V, r.sms);
+  p.bn = V <= 64 && !long_chain_kernel(dtype, kEpiLse, p.kps) ? 64 : V <= 256 ? 128 : tile_width(dtype, kEpiLse, M, V, p.kps, r.sms);
   // column tiles in runs, so that a block keeps a row's maximum and sum in registers over several of them
   const int64_t nt = ceil_div(V, p.bn), mt = std::max<int64_t>(1, ceil_div(M, 128));
   p.span = (int)ceil_div(nt, std::min(nt, ceil_div(4 * r.sms, mt)));

@@ -16,6 +16,11 @@
 // accumulator's, and small ones cut 5 times as often cost ten times the error (5001 x 515 ->
 // 257: 3.3e-6 in one accumulator, 3e-7 in two).
 //
+// A sum longer than a chain (chain_blocks) is made of several accumulations, added up in tensor memory by the
+// epilogue's warps.  A float32 product's error is then 7.5e-7 of it at any K (in one accumulation 1.6e-6 at 1536 terms, 3.9e-5 at
+// 32768; terms of one sign 1.4e-6, 1.6e-4); 16384 x 4096 -> 1024 takes 730 us (707), the statistics of 4096 x 1024,
+// V = 8192, 380 (360).
+//
 // Every wait is bounded; one that runs out ends the block's work, drains what it
 // has in flight, and is latched in a status word (VI_DEVICE_HEAD_TIMEOUT).
 #include <cuda.h>
@@ -87,6 +92,7 @@ struct Args {
   int m_tiles, n_tiles;  // n_tiles: column tiles
   int kblocks;           // 64-wide blocks of the whole sum
   int kps, splits;
+  int chain;             // blocks of k that one accumulation takes (chain_blocks); 0: all of a piece's
   int span, spans;
   uint32_t idesc;        // instruction descriptor
   uint32_t a_lbo, b_lbo; // bytes >> 4
@@ -261,6 +267,28 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float* v) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
 }
+__device__ __forceinline__ void tmem_load8(uint32_t addr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const float* v) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const float* v) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -576,6 +604,34 @@ __device__ __forceinline__ float staged_column_sum(uint32_t st, int lane, int& c
   return t[0];
 }
 
+// A long sum's accumulations are added up here, rounded: 32 columns of this warp's lanes from `acc` to `total` (the
+// first, to them), COLS at a time.
+template <int COLS>
+__device__ __forceinline__ void fold_chain(uint32_t total, uint32_t acc, bool first) {
+  static_assert(COLS == 8 || COLS == 16, "columns");
+#pragma unroll
+  for (int c = 0; c < 32; c += COLS) {
+    float2 v[COLS / 2], u[COLS / 2];
+    if constexpr (COLS == 16) {
+      tmem_load16(acc + c, (float*)v);
+      if (!first) tmem_load16(total + c, (float*)u);
+    } else {
+      tmem_load8(acc + c, (float*)v);
+      if (!first) tmem_load8(total + c, (float*)u);
+    }
+    tmem_wait_load();
+    if (!first) {
+#pragma unroll
+      for (int j = 0; j < COLS / 2; j++) v[j] = __fadd2_rn(v[j], u[j]);
+    }
+    if constexpr (COLS == 16) tmem_store16(total + c, (float*)v);
+    else tmem_store8(total + c, (float*)v);
+  }
+  tmem_wait_store();
+}
+// Where two blocks share an SM, a call of few registers.
+__device__ __noinline__ void fold_chain_call(uint32_t total, uint32_t acc, bool first) { fold_chain<8>(total, acc, first); }
+
 // v += COLS values of a bias slot.
 template <int COLS>
 __device__ __forceinline__ void add_bias(uint32_t slot, float2* v) {
@@ -587,7 +643,8 @@ __device__ __forceinline__ void add_bias(uint32_t slot, float2* v) {
   }
 }
 
-template <typename T, int BN, int EPI, int PL, int ACT>
+// CHAIN: sums may be longer than a chain.
+template <typename T, int BN, int EPI, int PL, int ACT, bool CHAIN>
 __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, EPI, PL>::kBlocks)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ Args a) {
@@ -720,38 +777,43 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
         const int steps = t.kb1 - t.kb0;
 #pragma unroll 1
         for (int nt = t.nt; nt < t.nt_end && on; nt++) {
-          if (!mbar_wait(tempty + 8 * acc, acc_phase ^ 1, dead, a.wait_limit)) {
-            on = false;
-            break;
-          }
-          fence_after();
-          const uint32_t d = tmem + acc * kAcc;
+          const int chain = CHAIN && a.chain ? a.chain : steps;
 #pragma unroll 1
-          for (int s = 0; s < steps; s++) {
-            if (!mbar_wait(full + 8 * stage, phase, dead, a.wait_limit)) {
+          for (int s0 = 0; s0 < steps; s0 += chain) {
+            if (!mbar_wait(tempty + 8 * acc, acc_phase ^ 1, dead, a.wait_limit)) {
               on = false;
               break;
             }
             fence_after();
-            const uint32_t sa = smem_u32(smem + stage * kStage), sb = sa + PL * S::kTileA;
-            // planes of the six products, smallest first: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
-            constexpr int kPairs = PL == 3 ? 6 : 1;
+            const uint32_t d = tmem + acc * kAcc;
+            const int s1 = min(steps, s0 + chain);
+#pragma unroll 1
+            for (int s = s0; s < s1; s++) {
+              if (!mbar_wait(full + 8 * stage, phase, dead, a.wait_limit)) {
+                on = false;
+                break;
+              }
+              fence_after();
+              const uint32_t sa = smem_u32(smem + stage * kStage), sb = sa + PL * S::kTileA;
+              // planes of the six products, smallest first: (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+              constexpr int kPairs = PL == 3 ? 6 : 1;
 #pragma unroll
-            for (int p = 0; p < kPairs; p++) {
-              const int pa = PL == 1 ? 0 : p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
-              const int pb = PL == 1 ? 0 : p == 2 ? 2 : p == 1 || p == 4 ? 1 : 0;
-              const uint64_t da = smem_desc(sa + pa * S::kTileA, a.a_lbo), db = smem_desc(sb + pb * S::kTileB, a.b_lbo);
+              for (int p = 0; p < kPairs; p++) {
+                const int pa = PL == 1 ? 0 : p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
+                const int pb = PL == 1 ? 0 : p == 2 ? 2 : p == 1 || p == 4 ? 1 : 0;
+                const uint64_t da = smem_desc(sa + pa * S::kTileA, a.a_lbo), db = smem_desc(sb + pb * S::kTileB, a.b_lbo);
 #pragma unroll
-              for (int k = 0; k < kBK / 16; k++)
-                mma_f16<S::kPair>(PL == 3 && p < 5 ? d + BN : d, da + k * a.a_step, db + k * a.b_step, a.idesc,
-                                  s > 0 || (p > 0 && p < 5) || k > 0);
+                for (int k = 0; k < kBK / 16; k++)
+                  mma_f16<S::kPair>(PL == 3 && p < 5 ? d + BN : d, da + k * a.a_step, db + k * a.b_step, a.idesc,
+                                    s > s0 || (p > 0 && p < 5) || k > 0);
+              }
+              mma_commit<S::kPair>(empty + 8 * stage);
+              if (++stage == kStages) stage = 0, phase ^= 1;
             }
-            mma_commit<S::kPair>(empty + 8 * stage);
-            if (++stage == kStages) stage = 0, phase ^= 1;
+            if (!on) break;
+            mma_commit<S::kPair>(tfull + 8 * acc);
+            if ((CHAIN && a.chain) || ++acc == 2) acc = 0, acc_phase ^= 1;
           }
-          if (!on) break;
-          mma_commit<S::kPair>(tfull + 8 * acc);
-          if (++acc == 2) acc = 0, acc_phase ^= 1;
         }
       }
       if (*dead) {
@@ -807,6 +869,30 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
           fence_after();
           waited = true;
         };
+        if (CHAIN && a.chain) {
+          // a sum longer than a chain: each accumulation, in the first accumulator, is added to the second, which no
+          // product writes; the product waits for that once a chain
+#pragma unroll 1
+          for (int s0 = t.kb0; s0 < t.kb1; s0 += a.chain) {
+            wait_product();
+            if (!on) break;
+#pragma unroll 1
+            for (int c = first; c < kAcc && m0 < a.M; c += 32 * S::kParts) {
+              if (col + c % BN >= a.N) continue;
+              const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + c;
+              if constexpr (S::kBlocks == 2) fold_chain_call(from + kAcc, from, s0 == t.kb0);
+              else fold_chain<16>(from + kAcc, from, s0 == t.kb0);
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (S::kPair) mbar_arrive_cluster(at_rank(tempty, 0));
+              else mbar_arrive(tempty);
+            }
+            acc_phase ^= 1;
+          }
+          if (!on) break;
+        }
 #pragma unroll 1
         for (int c = first; c < BN && col + c < a.N && m0 < a.M; c += 32 * S::kParts) {
           const int n0 = col + c;
@@ -816,7 +902,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
           if (kAdds && add.p) way = load_tile<T>(extra, add, EPI == kEpiAct ? res_access : access_of<T>(add), st, lane, here);
           if (!waited) wait_product();
           if (!on) break;
-          const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + acc * kAcc + c;
+          const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + (CHAIN && a.chain ? kAcc : acc * kAcc) + c;
           if (EPI != kEpiPartial && EPI != kEpiStore) {
             if (e.bias && !e.bias_rows && bias_at != n0) {  // a lane a column, then every lane all of them
               __syncwarp();
@@ -989,6 +1075,7 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
         }
         if (!waited) wait_product();
         if (!on) break;
+        if (CHAIN && a.chain) continue;  // the accumulators were handed back as they were added
         fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -1055,10 +1142,10 @@ bool encode(CUtensorMap* map, const Operand& o, int planes, bool half, int box_r
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int BN, int EPI, int PL, int ACT>
+template <typename T, int BN, int EPI, int PL, int ACT, bool CHAIN>
 cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
   using S = Shape<T, BN, EPI, PL>;
-  auto* k = gemm_tc_kernel<T, BN, EPI, PL, ACT>;
+  auto* k = gemm_tc_kernel<T, BN, EPI, PL, ACT, CHAIN>;
   // once per device: the call costs as much as a launch
   static std::atomic<uint64_t> done{0};
   int dev = 0;
@@ -1089,9 +1176,12 @@ cudaError_t run(const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int
 }
 template <typename T, int EPI, int PL, int ACT = VI_ACT_NONE>
 cudaError_t run_bn(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms, cudaStream_t s) {
+  constexpr bool kOwn = own_chain_kernel(EPI);
+  if constexpr (kOwn)
+    if (a.chain) return run<T, 128, EPI, PL, ACT, true>(ma, mb, a, sms, s);
   if constexpr (PL == 1)
-    if (bn == 256) return run<T, 256, EPI, PL, ACT>(ma, mb, a, sms, s);
-  return bn == 64 ? run<T, 64, EPI, PL, ACT>(ma, mb, a, sms, s) : run<T, 128, EPI, PL, ACT>(ma, mb, a, sms, s);
+    if (bn == 256) return run<T, 256, EPI, PL, ACT, !kOwn>(ma, mb, a, sms, s);
+  return bn == 64 ? run<T, 64, EPI, PL, ACT, !kOwn>(ma, mb, a, sms, s) : run<T, 128, EPI, PL, ACT, !kOwn>(ma, mb, a, sms, s);
 }
 template <typename T>
 cudaError_t run_epi(int epi, int bn, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int sms,
@@ -1124,6 +1214,7 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
   const int planes = dtype == VI_F32 ? 3 : 1;
   const bool half = dtype == VI_F16;
   const bool pair = pair_tile(epi, p.bn);
+  if (long_chain_kernel(dtype, epi, p.kps) && p.bn != 128) return set_error(VI_ERR_UNSUPPORTED, "heads: a long sum's tiles are 128 wide");
   CUtensorMap ma, mb;
   if (!encode(&ma, A, planes, half, kBM) || !encode(&mb, B, planes, half, pair ? 128 : p.bn))
     return set_error(VI_ERR_CUDA, "heads: a tensor map could not be encoded");
@@ -1136,6 +1227,10 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
   a.kblocks = (int)((A.k + kBK - 1) / kBK);
   a.kps = p.kps;
   a.splits = p.splits;
+  if (p.kps > chain_blocks(dtype)) {
+    const int chains = (p.kps + chain_blocks(dtype) - 1) / chain_blocks(dtype);
+    a.chain = (p.kps + chains - 1) / chains;
+  }
   a.span = p.span;
   a.spans = p.spans;
   a.a_k_major = A.k_major;
