@@ -360,7 +360,9 @@ __global__ void __launch_bounds__(256) reduce_loss_kernel(const float* bsum, con
 // Per-row factors of the logits' gradient.  Their common size goes to the
 // products' end instead (alpha): G is kept in 16 bits, and float16 would lose
 // probabilities divided by a pixel count.  lift (a power of two) moves float16's G
-// up further, so that a probability keeps float16's full precision down to 4e-9.
+// up further, so that a probability keeps float16's full precision down to 4e-9.  Rows with gradients of their
+// own share one scale, the largest's, because dweight sums over them: beside float16 a row of 2^-20 of the largest
+// |dloss| keeps G to 2^-19 of its own scale (its dx is rounded to 2^-12), and one below 2^-26 loses its small probabilities.
 // First per block: the largest finite |dloss| and the number of rows not ignored.
 __global__ void __launch_bounds__(256) coef_parts_kernel(const int64_t* target, int64_t ignore, int64_t M,
                                                          const float* dloss, float* bmax, uint32_t* bcount) {

@@ -81,7 +81,8 @@ struct Epilogue {
   int64_t col0;
   void* grad;           // [planes][M][grad_ld], 16-bit
   int64_t grad_ld, grad_plane;
-  float* column_part;   // 16-bit types: [4 per tile of 128 rows][N] sums of G's columns over 32 rows, null = not wanted
+  float* column_part;   // 16-bit types: [4 per tile of 128 rows][N] sums of G's columns over 32 rows, of the cells as
+                        // rounded, which dx and dweight use too; null = not wanted
 };
 
 // Tile shape and division of one product's work.
