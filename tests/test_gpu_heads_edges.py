@@ -451,3 +451,59 @@ def test_forward_mode_is_refused():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, (x,), dual, retain_graph=True)
     torch.autograd.grad(y, (x,), torch.ones_like(y))
+
+
+# ---- captures ----
+def test_a_captured_backward_beside_a_living_eager_graph_is_refused():
+    # autograd would make the default stream wait for the captured one, which ends the process
+    import volume_integration.heads as heads
+    x, w, b, r, dy = _inputs(200, 24, 40, F32, "rows", True, True, 74)
+    t = torch.randint(0, 40, (200,), device="cuda")
+    leaves = [v.detach().requires_grad_(True) for v in (x, w, b, r)]
+
+    def act():
+        y = heads.linear_act(*leaves, activation="silu")
+        return torch.autograd.grad(y, leaves, dy)
+
+    def loss():
+        return torch.autograd.grad(heads.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2]), leaves[:3])
+    for step, eager in ((act, lambda: heads.linear_act(*leaves, activation="silu")),
+                        (loss, lambda: heads.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2]))):
+        want = step()
+        alive = eager()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="default stream"):
+                step()
+        for a, c in zip(step(), want):  # eagerly it may go on beside it
+            assert torch.equal(a, c)
+        del alive, graph
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(out, want):
+            assert torch.equal(a, c)
+        del graph, out
+
+
+def test_a_captured_backward_beside_a_graph_of_another_stream():
+    # as when the steps before the capture ran on a side stream and their result is kept
+    import volume_integration.heads as heads
+    x, w, b, _, dy = _inputs(200, 24, 40, F32, "rows", True, False, 75)
+    leaves = [v.detach().requires_grad_(True) for v in (x, w, b)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = heads.linear_act(*leaves, activation="silu")
+        want = torch.autograd.grad(alive, leaves, dy, retain_graph=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch.autograd.grad(heads.linear_act(*leaves, activation="silu"), leaves, dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, c in zip(out, want):
+        assert torch.equal(a, c)
+    del graph, alive

@@ -5,6 +5,7 @@
 // resize callback, as the reference's resizeFunctional does
 // (integrate_primitives.cu:54-68).  Errors raise RuntimeError.
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -546,6 +547,26 @@ void no_tangents(const char* what, const T&... ts) {
   const auto has = [](const c10::optional<Tensor>& t) { return t.has_value() && t->defined() && t->_fw_grad(0).defined(); };
   TORCH_CHECK(!(has(ts) || ...), what, ": forward-mode differentiation is not supported");
 }
+bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
+// Whether a leaf's gradient would be handed to the default stream, because an eager graph on it still lives.  Under a
+// capture autograd would then make that stream wait for the captured one, which CUDA forbids, and
+// the error ends the process: the backward refuses before.
+bool bound_to_default_stream(const c10::optional<Tensor>& t) {
+  if (!t.has_value() || !t->defined() || !t->requires_grad() || !t->is_leaf()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+  const auto s = node ? node->stream() : std::nullopt;
+  return s.has_value() && s->device_type() == c10::DeviceType::CUDA &&
+         c10::cuda::CUDAStream(c10::cuda::CUDAStream::UNCHECKED, *s).stream() == nullptr;
+}
+template <class... T>
+void note_capture(AutogradContext* ctx, const T&... ts) {
+  ctx->saved_data["default_stream"] = capturing() && (bound_to_default_stream(ts) || ...);
+}
+void check_capture(AutogradContext* ctx, const char* what) {
+  TORCH_CHECK(!(ctx->saved_data["default_stream"].toBool() && capturing()), what,
+              ": captured, while an earlier result of the same leaves, computed on the default stream, is still alive; let go of "
+              "it (del) before the capture, or compute it on another stream");
+}
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const c10::optional<Tensor>& t) { return t.has_value() && t->requires_grad(); }
 
@@ -564,10 +585,12 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["residual"] = residual.has_value();
+    note_capture(ctx, x, weight, bias, residual);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dys) {
     no_tangents("linear_act backward", dys[0]);
+    check_capture(ctx, "linear_act backward");
     const variable_list saved = ctx->get_saved_variables();
     const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = has_b && ctx->needs_input_grad(2);
@@ -601,10 +624,12 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["reduction"] = reduction;
+    note_capture(ctx, x, weight, bias);
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dloss) {
     no_tangents("linear_cross_entropy backward", dloss[0]);
+    check_capture(ctx, "linear_cross_entropy backward");
     const variable_list saved = ctx->get_saved_variables();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
     const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
