@@ -50,6 +50,13 @@ def _check(x, w, b, r, act, dy):
         hl.assert_within("dbias", grads[2], want[3])
 
 
+def _pairs():
+    # launches so far with tiles of two blocks
+    lib = ha.load()
+    lib.vi_heads_pair_launches.restype = ctypes.c_uint64
+    return lib.vi_heads_pair_launches()
+
+
 # ---- values that are not finite ----
 # M, K, N and order: the small products, the tensor cores, an image of few channels, an image
 PATHS = [(90, 40, 70, "rows"), (900, 40, 70, "rows"), (900, 4, 70, "image"), (900, 40, 130, "image")]
@@ -223,6 +230,23 @@ def test_long_float32_logits(V):
     hl.assert_within("dweight", dw, (value, vb + 4 * hl.E * value.abs() + hl.last(F32, value.abs() + vb)))
 
 
+@pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+def test_long_logits_of_16_bit_features(dt):
+    # the loss is float32 whatever the features are: a chain of logits is 4096 terms (256 e)
+    import volume_integration.heads as heads
+    K, M, V = 32768, 260, 300
+    g = _gen(78)
+    x = torch.rand(M, K, generator=g, device="cuda").to(dt)
+    w = (torch.rand(V, K, generator=g, device="cuda") * (80.0 / K)).to(dt)
+    w[0] = 0.0
+    t = torch.zeros(M, dtype=torch.int64, device="cuda")
+    loss = heads.linear_cross_entropy(x, w, t, reduction="none")
+    z = x.double() @ w.double().t()
+    lse = torch.logsumexp(z, 1)
+    bound = (256 + 16 + K / 4096 / 2) * hl.E * z.max(1).values + (V + 16) * hl.E + 8 * hl.E * lse
+    hl.assert_within("loss", loss, (lse, bound))
+
+
 def test_long_float16_weight_gradients():
     # 262144 rows into 2048 x 2048: as many tiles as run at a time, so each is one long sum.  The mean over many
     # elements leaves the drift: roundings of the result (u each, either way) average out.
@@ -252,7 +276,8 @@ def test_long_products_with_everything(M, K, N, act, order, dt):
 
 
 @pytest.mark.parametrize("M,K,V,dt", [(260, 20000, 50, F16), (260, 16500, 300, F16), (130, 140000, 70, BF16),
-                                      (700, 1000, 5003, F32), (20000, 24, 21, F32)])
+                                      (700, 1000, 5003, F32), (20000, 24, 21, F32),
+                                      (17000, 800, 1500, F32)])  # the last: several tiles a block, in runs
 def test_long_logits_and_long_gradients(M, K, V, dt):
     import volume_integration.heads as heads
     g = _gen(72)
@@ -266,6 +291,21 @@ def test_long_logits_and_long_gradients(M, K, V, dt):
     want = hl.linear_ce(x, w, b, t, -100, "mean", torch.ones((), device="cuda"))
     for name, got, ref in zip(("loss", "dx", "dweight", "dbias"), (loss.detach(),) + grads, want):
         hl.assert_within(name, got, ref)
+
+
+def test_long_sums_on_tiles_of_pairs():
+    # dx over 16500 columns: 192 tiles for 74 pairs, each of two chains
+    import volume_integration.heads as heads
+    g = _gen(76)
+    M, K, N = 12288, 1024, 16500
+    w = hl.matrix(N, K, F16, g, scale=N ** -0.5)
+    x = torch.zeros(M, K, device="cuda", dtype=F16, requires_grad=True)
+    dy = hl.matrix(M, N, F16, g)
+    before = _pairs()
+    (dx,) = torch.autograd.grad(heads.linear_act(x, w), (x,), dy)
+    assert _pairs() > before
+    value, bound = hl.weighted_sum(dy.double(), torch.zeros(1, 1, device="cuda", dtype=torch.float64).expand(M, N), w, F16)
+    hl.assert_within("dx", dx, (value, bound + hl.last(F16, value.abs() + bound)))
 
 
 def test_long_float32_gradients():
@@ -283,12 +323,6 @@ def test_long_float32_gradients():
 
 
 # ---- tiles made by pairs of blocks ----
-def _pairs():
-    lib = ha.load()
-    lib.vi_heads_pair_launches.restype = ctypes.c_uint64
-    return lib.vi_heads_pair_launches()
-
-
 @pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
 @pytest.mark.parametrize("M,K,N,act,order,bias,residual,pairs", [
     # 64 tiles of 256 x 256 (one wave of 74 pairs, where narrower tiles take two and more): the forward's,
@@ -360,6 +394,19 @@ def test_tiles_of_pairs_captured_and_on_two_streams():
         for a, c in zip(grads, want[1]):
             assert torch.equal(a, c)
     del graph
+
+
+def test_a_wait_that_runs_out_in_a_long_sum_is_reported(monkeypatch):
+    import volume_integration.heads as heads
+    x, w, _, _, _ = _inputs(300, 3000, 200, F32, "rows", False, False, 77)
+    want = heads.linear_act(x, w)
+    assert heads.device_status(reset=True) == 0
+    monkeypatch.setenv("VI_HEADS_TEST_TIMEOUT", "1")
+    heads.linear_act(x, w)
+    assert heads.device_status(reset=True) == 8
+    monkeypatch.delenv("VI_HEADS_TEST_TIMEOUT")
+    assert torch.equal(heads.linear_act(x, w), want)
+    assert heads.device_status() == 0
 
 
 @pytest.mark.parametrize("K", [200, 1000])  # fewer blocks of k than stages, and more

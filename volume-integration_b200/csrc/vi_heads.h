@@ -47,16 +47,19 @@ constexpr bool pair_tile(int epi, int bn) { return bn == 256 && epi != kEpiLse &
 // Blocks of k (64 terms each) that one accumulation may take.  The tensor core cuts what it adds, always towards
 // zero, so a sum of terms of one sign drifts with its length: by about 0.8 * 2^-23 of it for every 16 terms (a float16 weight
 // gradient over 262144 rows: 1.5e-3, three half steps).  Longer sums are made in accumulations that the epilogue
-// adds up, rounded: 768 terms in float32, else as many as stay within a fifth of the type's
-// half step.
-constexpr int chain_blocks(int dtype) { return dtype == VI_F32 ? 12 : dtype == VI_F16 ? 256 : 2048; }
+// adds up, rounded: 768 terms in float32; 4096 in logits of 16-bit features, whose loss is float32 (5e-6 of a
+// logit); else as many as stay within a fifth of the type's half step.
+constexpr int chain_blocks(int dtype, int epi) {
+  if (dtype == VI_F32) return 12;
+  return epi == kEpiLse || epi == kEpiGrad ? 64 : dtype == VI_F16 ? 256 : 2048;
+}
 
 // Whether a product's accumulations are added up by a kernel of its own, with 128-wide tiles: the epilogues that have no
 // registers to spare for that code (with it in the common one: 2M x 64 -> 64 with gelu 222 us, 240; float32 logits of
 // 4096 x 256, V = 8192: 113, 127).
 constexpr bool own_chain_kernel(int epi) { return epi != kEpiStore && epi != kEpiPartial; }
 constexpr bool long_chain_kernel(int dtype, int epi, int64_t kblocks) {
-  return own_chain_kernel(epi) && kblocks > chain_blocks(dtype);
+  return own_chain_kernel(epi) && kblocks > chain_blocks(dtype, epi);
 }
 
 // What happens to the product acc(m, n) = sum_k A(m, k) B(n, k).

@@ -1227,8 +1227,8 @@ int launch_gemm(int dtype, int epi, const Operand& A, const Operand& B, const Pl
   a.kblocks = (int)((A.k + kBK - 1) / kBK);
   a.kps = p.kps;
   a.splits = p.splits;
-  if (p.kps > chain_blocks(dtype)) {
-    const int chains = (p.kps + chain_blocks(dtype) - 1) / chain_blocks(dtype);
+  if (const int most = chain_blocks(dtype, epi); p.kps > most) {
+    const int chains = (p.kps + most - 1) / most;
     a.chain = (p.kps + chains - 1) / chains;
   }
   a.span = p.span;
