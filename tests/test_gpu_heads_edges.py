@@ -554,3 +554,22 @@ def test_a_captured_backward_beside_a_graph_of_another_stream():
     for a, c in zip(out, want):
         assert torch.equal(a, c)
     del graph, alive
+
+
+def test_a_captured_backward_to_other_leaves_than_the_living_ones():
+    # the living graph is of x alone, and the capture asks for the other gradients
+    import volume_integration.heads as heads
+    x, w, b, r, dy = _inputs(200, 24, 40, F32, "rows", True, True, 79)
+    leaves = [v.detach().requires_grad_(True) for v in (x, w, b, r)]
+    want = torch.autograd.grad(heads.linear_act(*leaves, activation="silu"), leaves, dy)
+    alive = heads.linear_act(leaves[0], w, b, activation="silu")
+    for part in ((1, 2, 3), (3,), (2,)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = torch.autograd.grad(heads.linear_act(*leaves, activation="silu"), [leaves[i] for i in part], dy)
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, a in zip(part, out):
+            assert torch.equal(a, want[i])
+        del graph, out
+    del alive

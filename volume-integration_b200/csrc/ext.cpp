@@ -558,12 +558,18 @@ bool bound_to_default_stream(const c10::optional<Tensor>& t) {
   return s.has_value() && s->device_type() == c10::DeviceType::CUDA &&
          c10::cuda::CUDAStream(c10::cuda::CUDAStream::UNCHECKED, *s).stream() == nullptr;
 }
+// The inputs of which that holds, bit i for the i-th; 0 outside a capture.
 template <class... T>
-void note_capture(AutogradContext* ctx, const T&... ts) {
-  ctx->saved_data["default_stream"] = capturing() && (bound_to_default_stream(ts) || ...);
+int64_t bound_to_default_stream(const T&... ts) {
+  if (!capturing()) return 0;
+  int64_t mask = 0, bit = 1;
+  ((mask |= bound_to_default_stream(c10::optional<Tensor>(ts)) ? bit : 0, bit *= 2), ...);
+  return mask;
 }
-void check_capture(AutogradContext* ctx, const char* what) {
-  TORCH_CHECK(!(ctx->saved_data["default_stream"].toBool() && capturing()), what,
+void check_capture(AutogradContext* ctx, std::initializer_list<bool> needed, const char* what) {
+  int64_t mask = 0, bit = 1;
+  for (const bool n : needed) mask |= n ? bit : 0, bit *= 2;
+  TORCH_CHECK(!(ctx->saved_data["default_stream"].toInt() & mask) || !capturing(), what,
               ": captured, while an earlier result of the same leaves, computed on the default stream, is still alive; let go of "
               "it (del) before the capture, or compute it on another stream");
 }
@@ -585,15 +591,16 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
     ctx->saved_data["activation"] = activation;
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["residual"] = residual.has_value();
-    note_capture(ctx, x, weight, bias, residual);
+    ctx->saved_data["default_stream"] = bound_to_default_stream(x, weight, bias, residual);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dys) {
     no_tangents("linear_act backward", dys[0]);
-    check_capture(ctx, "linear_act backward");
     const variable_list saved = ctx->get_saved_variables();
     const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = has_b && ctx->needs_input_grad(2);
+    const bool nr = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
+    check_capture(ctx, {nx, nw, nb, nr}, "linear_act backward");
     variable_list out(5);
     if (nx || nw || nb) {
       auto [dx, dw, db] = linear_act_backward(dys[0], optional_of(saved[3]), saved[0], saved[1], optional_of(saved[2]),
@@ -603,7 +610,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
       if (nb) out[2] = *db;
     }
     differentiate_once(out);
-    if (has_r && ctx->needs_input_grad(has_b ? 3 : 2)) out[3] = dys[0];
+    if (nr) out[3] = dys[0];
     return out;
   }
 };
@@ -624,15 +631,15 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     ctx->saved_data["bias"] = bias.has_value();
     ctx->saved_data["ignore"] = ignore_index;
     ctx->saved_data["reduction"] = reduction;
-    note_capture(ctx, x, weight, bias);
+    ctx->saved_data["default_stream"] = bound_to_default_stream(x, weight, bias);
     return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list dloss) {
     no_tangents("linear_cross_entropy backward", dloss[0]);
-    check_capture(ctx, "linear_cross_entropy backward");
     const variable_list saved = ctx->get_saved_variables();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
     const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+    check_capture(ctx, {nx, nw, nb}, "linear_cross_entropy backward");
     variable_list out(6);
     if (nx || nw || nb) {
       auto [dx, dw, db] =
