@@ -397,6 +397,68 @@ int vi_linear_ce_backward(int dtype, const vi_matrix* x, const vi_matrix* weight
                           void* scratch, uint64_t scratch_bytes, void* stream);
 
 /*
+ * Layer norm of rows: y = (x - mean) / sqrt(var + eps) * weight + bias, mean and
+ * var (of x - mean, over K) each row's own.  x [M,K] in any strides, weight and
+ * bias [K] (either NULL: 1, 0), y [M,K] with one of its strides 1.  stats (float32
+ * [3][M], or NULL) is what the backward needs: each row's mean as rounded, what
+ * that lacks, and 1 / sqrt(var + eps).  No scratch.  Rows share nothing: a NaN stays in its row.
+ */
+int vi_layer_norm_forward(int dtype, const vi_matrix* x, const void* weight, const void* bias, float eps,
+                          const vi_matrix* y, float* stats, void* stream);
+
+/*
+ * Gradients for an incoming dy [M,K] (any strides): with h = (x - mean) / sqrt(var + eps) and g = dy weight,
+ * dx = (g - mean(g) - h mean(g h)) / sqrt(var + eps), dweight = the column sums of dy h, dbias those of dy.
+ * Each of dx (one of its strides 1), dweight, dbias may be NULL.
+ */
+uint64_t vi_layer_norm_backward_scratch_bytes(int dtype, const vi_matrix* dy, const vi_matrix* x, const void* weight,
+                                              const vi_matrix* dx, const void* dweight, const void* dbias);
+int vi_layer_norm_backward(int dtype, const vi_matrix* dy, const vi_matrix* x, const void* weight, const float* stats,
+                           const vi_matrix* dx, void* dweight, void* dbias, void* scratch, uint64_t scratch_bytes,
+                           void* stream);
+
+/*
+ * Rows in 8-bit integers with a scale each: scale_m = max_k |x_mk| / 127 in float32, q_mk = x_mk / scale_m rounded
+ * to the nearest whole number (ties to even, of the exact quotient).  x [M,K] of `dtype` in any strides; q int8 [M,K]
+ * with contiguous rows (a row stride and address that are multiples of 16 spare vi_linear_act_int8 a copy); scale
+ * float32 [M].  A row of zeros has scale 0; one with an infinity or a NaN has scale NaN, and q 0.
+ */
+int vi_quantize_rows(int dtype, const vi_matrix* x, const vi_matrix* q, float* scale, void* stream);
+
+/*
+ * vi_linear_act_forward with 8-bit integer products: y = act(x_scale_m weight_scale_n sum_k x_mk weight_nk + bias_n) + residual.
+ * weight int8 [N,K] (any strides) and weight_scale float32 [N] as vi_quantize_rows gives them.  x [M,K]: int8 with
+ * x_scale float32 [M]; or, x_scale NULL, of `dtype`: its rows are quantised in the call.  bias, residual and y are of `dtype`.
+ * Sums are exact; K is at most 2^17.
+ */
+uint64_t vi_linear_act_int8_scratch_bytes(int dtype, int activation, const vi_matrix* x, const float* x_scale,
+                                          const vi_matrix* weight, const float* weight_scale, const void* bias,
+                                          const vi_matrix* residual, const vi_matrix* y);
+int vi_linear_act_int8(int dtype, int activation, const vi_matrix* x, const float* x_scale, const vi_matrix* weight,
+                       const float* weight_scale, const void* bias, const vi_matrix* residual, const vi_matrix* y,
+                       void* scratch, uint64_t scratch_bytes, void* stream);
+
+/*
+ * Labels drawn from rows of logits.  With w_v = exp((z_v - max z) / temperature) and the candidates in the order of falling
+ * z (ties: lowest index first): top_k (0: off) keeps the first top_k; top_p (1 or more: off) those of them in front
+ * of which lies less than top_p of their mass (the first always); min_p (0: off) those with w >= min_p.  label_m is the first
+ * index at which the sum of the kept w, in index order, exceeds u_m times their sum (u_m in [0, 1), float32; from 1 on the last
+ * one kept).  temperature 0: the first of the largest.  A row whose logits are all -inf, or hold a NaN, has label -1; a +inf takes all
+ * mass (several share it).  Each setting is one value, or an array of one per row where its array is not NULL (there a
+ * temperature of 0 or less is 0, one that is NaN gives -1, a top_k under 1 is off, a top_p of 0 or less keeps the first).
+ * Weights and sums are 64 bits wide.
+ */
+typedef struct vi_sampling {
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const float* temperatures;
+  const int64_t* top_ks;
+  const float *top_ps, *min_ps;
+} vi_sampling;
+int vi_sample_labels(int dtype, const vi_matrix* logits, const float* u, const vi_sampling* settings, int64_t* label,
+                     void* stream);
+
+/*
  * The current device's status word of the heads' matrix products: 0, or
  * VI_DEVICE_HEAD_TIMEOUT when a bounded wait gave up in one of them since the last
  * reset (the results of that call are then unspecified).  Waits for `stream`; reset

@@ -662,6 +662,164 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& weight, const c10::op
   return std::get<0>(linear_ce_forward(x, weight, bias, target, ignore_index, reduction));
 }
 
+// A vector of K elements that belongs to x's columns, contiguous.
+Tensor norm_vector(const c10::optional<Tensor>& v, const Tensor& x, const char* name) {
+  if (!v.has_value()) return {};
+  head_like(*v, x, name);
+  TORCH_CHECK(v->dim() == 1 && v->size(0) == x.size(1), name, " must be [", x.size(1), "]");
+  return v->contiguous();
+}
+
+// (y, stats or None)
+std::tuple<Tensor, c10::optional<Tensor>> layer_norm_forward(const Tensor& x, const c10::optional<Tensor>& weight,
+                                                             const c10::optional<Tensor>& bias, double eps, bool backward_follows) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a 2D CUDA tensor");
+  const at::cuda::OptionalCUDAGuard guard(x.device());
+  const int dt = head_dtype(x, "x");
+  const Tensor w = norm_vector(weight, x, "weight"), b = norm_vector(bias, x, "bias");
+  Tensor y = head_result(x, x.size(0), x.size(1));
+  c10::optional<Tensor> stats;
+  if (backward_follows) stats = torch::empty({3, x.size(0)}, x.options().dtype(torch::kFloat32));
+  const vi_matrix mx = head_matrix(x), my = head_matrix(y);
+  ok(vi_layer_norm_forward(dt, &mx, head_ptr(w), head_ptr(b), (float)eps, &my, stats ? stats->data_ptr<float>() : nullptr,
+                           at::cuda::getCurrentCUDAStream().stream()));
+  return {y, stats};
+}
+
+// (dx, dweight, dbias), None where not wanted
+Grads layer_norm_backward(const Tensor& dy, const Tensor& x, const c10::optional<Tensor>& weight, const Tensor& stats, bool need_x,
+                          bool need_w, bool need_b) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a 2D CUDA tensor");
+  head_like(dy, x, "dy");
+  TORCH_CHECK(dy.dim() == 2 && dy.size(0) == x.size(0) && dy.size(1) == x.size(1), "dy must have x's shape");
+  const at::cuda::OptionalCUDAGuard guard(x.device());
+  const int dt = head_dtype(x, "x");
+  const Tensor w = norm_vector(weight, x, "weight"), st = cuda_f32(stats, "stats");
+  TORCH_CHECK(st.numel() == 3 * x.size(0) && st.device() == x.device(), "stats must be [3, ", x.size(0), "] on ", x.device());
+  const vi_matrix mdy = head_matrix(dy), mx = head_matrix(x);
+  c10::optional<Tensor> dx, dw, db;
+  vi_matrix mdx{};
+  if (need_x) dx = head_result(x, x.size(0), x.size(1)), mdx = head_matrix(*dx);
+  if (need_w) dw = torch::empty({x.size(1)}, x.options());
+  if (need_b) db = torch::empty({x.size(1)}, x.options());
+  const vi_matrix* pdx = need_x ? &mdx : nullptr;
+  void *pdw = need_w ? dw->data_ptr() : nullptr, *pdb = need_b ? db->data_ptr() : nullptr;
+  const uint64_t n = vi_layer_norm_backward_scratch_bytes(dt, &mdy, &mx, head_ptr(w), pdx, pdw, pdb);
+  Tensor scratch = head_scratch(n, x);
+  ok(vi_layer_norm_backward(dt, &mdy, &mx, head_ptr(w), st.data_ptr<float>(), pdx, pdw, pdb, head_ptr(scratch), n,
+                            at::cuda::getCurrentCUDAStream().stream()));
+  return {dx, dw, db};
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& weight,
+                        const c10::optional<Tensor>& bias, double eps) {
+    auto [y, stats] = layer_norm_forward(x, weight, bias, eps, true);
+    ctx->save_for_backward({x, weight.value_or(Tensor()), *stats});
+    ctx->saved_data["weight"] = weight.has_value();
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["default_stream"] = bound_to_default_stream(x, weight, bias);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list dys) {
+    no_tangents("layer_norm backward", dys[0]);
+    const variable_list saved = ctx->get_saved_variables();
+    const bool has_w = ctx->saved_data["weight"].toBool(), has_b = ctx->saved_data["bias"].toBool();
+    const bool nx = ctx->needs_input_grad(0), nw = has_w && ctx->needs_input_grad(1);
+    const bool nb = has_b && ctx->needs_input_grad(has_w ? 2 : 1);
+    check_capture(ctx, {nx, nw, nb}, "layer_norm backward");
+    variable_list out(4);
+    if (nx || nw || nb) {
+      auto [dx, dw, db] = layer_norm_backward(dys[0], saved[0], optional_of(saved[1]), saved[2], nx, nw, nb);
+      if (nx) out[0] = *dx;
+      if (nw) out[1] = *dw;
+      if (nb) out[2] = *db;
+    }
+    differentiate_once(out);
+    return out;
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias, double eps) {
+  no_tangents("layer_norm", x, weight, bias);
+  if (torch::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
+    return LayerNorm::apply(x, weight, bias, eps);
+  return std::get<0>(layer_norm_forward(x, weight, bias, eps, false));
+}
+
+// (q [M, K] int8 with rows a multiple of 16 bytes apart, scale [M])
+std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
+  no_tangents("quantize_rows", x);
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "x must be a 2D CUDA tensor");
+  const at::cuda::OptionalCUDAGuard guard(x.device());
+  const int dt = head_dtype(x, "x");
+  const int64_t K = x.size(1);
+  Tensor q = torch::empty({x.size(0), (K + 15) / 16 * 16}, x.options().dtype(torch::kInt8)).slice(1, 0, K);
+  Tensor scale = torch::empty({x.size(0)}, x.options().dtype(torch::kFloat32));
+  const vi_matrix mx = head_matrix(x), mq = head_matrix(q);
+  ok(vi_quantize_rows(dt, &mx, &mq, scale.data_ptr<float>(), at::cuda::getCurrentCUDAStream().stream()));
+  return {q, scale};
+}
+
+// x of `dtype`, or int8 with x_scale
+Tensor linear_act_int8(const Tensor& x, const c10::optional<Tensor>& x_scale, const Tensor& weight, const Tensor& weight_scale,
+                       const c10::optional<Tensor>& bias, const c10::optional<Tensor>& residual, int64_t activation,
+                       c10::ScalarType dtype) {
+  no_tangents("linear_act_int8", x, x_scale, weight_scale, bias, residual);
+  TORCH_CHECK(!torch::GradMode::is_enabled() || !(wants_grad(x) || wants_grad(x_scale) || wants_grad(weight_scale) ||
+                                                  wants_grad(bias) || wants_grad(residual)),
+              "linear_act_int8 has no backward: call it under torch.no_grad(), or with detached tensors");
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && weight.dim() == 2, "x and weight must be 2D CUDA tensors");
+  const at::cuda::OptionalCUDAGuard guard(x.device());
+  const auto scale_of = [&](const Tensor& s, int64_t n, const char* name) {
+    TORCH_CHECK(s.device() == x.device() && s.scalar_type() == torch::kFloat32 && s.dim() == 1 && s.size(0) == n, name,
+                " must be float32 [", n, "] on ", x.device());
+    return s.contiguous();
+  };
+  TORCH_CHECK(weight.device() == x.device() && weight.scalar_type() == torch::kInt8, "weight must be int8 on ", x.device());
+  TORCH_CHECK(x.scalar_type() == (x_scale.has_value() ? torch::kInt8 : dtype), "x must be ", x_scale.has_value() ? torch::kInt8 : dtype);
+  const Tensor ws = scale_of(weight_scale, weight.size(0), "weight's scale");
+  const Tensor xs = x_scale.has_value() ? scale_of(*x_scale, x.size(0), "x's scale") : Tensor();
+  const Tensor like = torch::empty({0}, x.options().dtype(dtype));
+  const int dt = head_dtype(like, "the result");
+  const Tensor b = head_bias(bias, like, weight);
+  const OptMatrix r(residual, like, "residual");
+  Tensor y = x.stride(0) == 1 && x.stride(1) != 1 ? torch::empty({weight.size(0), x.size(0)}, like.options()).t()
+                                                  : torch::empty({x.size(0), weight.size(0)}, like.options());
+  const vi_matrix mx = head_matrix(x), mw = head_matrix(weight), my = head_matrix(y);
+  const float *pxs = xs.defined() ? xs.data_ptr<float>() : nullptr, *pws = ws.data_ptr<float>();
+  const uint64_t n = vi_linear_act_int8_scratch_bytes(dt, (int)activation, &mx, pxs, &mw, pws, head_ptr(b), r.get(), &my);
+  Tensor scratch = head_scratch(n, x);
+  ok(vi_linear_act_int8(dt, (int)activation, &mx, pxs, &mw, pws, head_ptr(b), r.get(), &my, head_ptr(scratch), n,
+                        at::cuda::getCurrentCUDAStream().stream()));
+  return y;
+}
+
+// A setting is its tensor, where that is given, else its number.
+Tensor sample_labels(const Tensor& logits, const Tensor& u, double temperature, const c10::optional<Tensor>& temperatures,
+                     int64_t top_k, const c10::optional<Tensor>& top_ks, double top_p, const c10::optional<Tensor>& top_ps,
+                     double min_p, const c10::optional<Tensor>& min_ps) {
+  no_tangents("sample_labels", logits, u, temperatures, top_ps, min_ps);
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "logits must be a 2D CUDA tensor");
+  const at::cuda::OptionalCUDAGuard guard(logits.device());
+  const int dt = head_dtype(logits, "logits");
+  const auto rows_of = [&](const c10::optional<Tensor>& t, c10::ScalarType type, const char* name) {
+    if (!t.has_value()) return Tensor();
+    TORCH_CHECK(t->device() == logits.device() && t->scalar_type() == type && t->dim() == 1 && t->size(0) == logits.size(0), name,
+                " must be ", type, " [", logits.size(0), "] on ", logits.device());
+    return t->contiguous();
+  };
+  const Tensor v = rows_of(u, torch::kFloat32, "u"), t = rows_of(temperatures, torch::kFloat32, "temperature"),
+               k = rows_of(top_ks, torch::kInt64, "top_k"), p = rows_of(top_ps, torch::kFloat32, "top_p"),
+               m = rows_of(min_ps, torch::kFloat32, "min_p");
+  const auto f32 = [](const Tensor& x) { return x.defined() ? x.data_ptr<float>() : nullptr; };
+  const vi_sampling s{temperature, top_p, min_p, top_k, f32(t), k.defined() ? k.data_ptr<int64_t>() : nullptr, f32(p), f32(m)};
+  Tensor label = torch::empty({logits.size(0)}, logits.options().dtype(torch::kInt64));
+  const vi_matrix mz = head_matrix(logits);
+  ok(vi_sample_labels(dt, &mz, v.data_ptr<float>(), &s, label.data_ptr<int64_t>(), at::cuda::getCurrentCUDAStream().stream()));
+  return label;
+}
+
 // The heads' status word of a device (0 = no wait gave up).
 int64_t heads_status(int64_t device, bool reset) {
   const at::cuda::CUDAGuard guard((c10::DeviceIndex)device);
@@ -692,6 +850,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_act_backward", &linear_act_backward, "Gradients of linear_act_forward (extension)");
   m.def("linear_ce_forward", &linear_ce_forward, "Cross entropy of a linear classifier (extension)");
   m.def("linear_ce_backward", &linear_ce_backward, "Gradients of linear_ce_forward (extension)");
+  m.def("layer_norm", &layer_norm, "Layer norm of rows, differentiable (extension)");
+  m.def("layer_norm_forward", &layer_norm_forward, "Layer norm of rows (extension)");
+  m.def("layer_norm_backward", &layer_norm_backward, "Gradients of layer_norm_forward (extension)");
+  m.def("quantize_rows", &quantize_rows, "Rows in 8-bit integers with a scale each (extension)");
+  m.def("linear_act_int8", &linear_act_int8, "act(x W^T + b) + residual with 8-bit integer products (extension)");
+  m.def("sample_labels", &sample_labels, "Labels drawn from rows of logits (extension)");
   m.def("heads_status", &heads_status, "Status word of the heads' kernels on a device (extension)");
   m.def("state_views", &state_views, "Integer state of a forward call in the reference's formats");
   m.def("sort_pairs", &sort_pairs, "Stable radix sort of (uint64 key, uint32 value) pairs");

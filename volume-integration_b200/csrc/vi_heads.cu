@@ -1,10 +1,12 @@
 // Per-pixel heads: dense layers and the label loss on rendered feature images.
 //
-// Mathematics.  Both operators are one product z = x W^T + b with an epilogue:
+// Mathematics.  The products are one z = x W^T + b with an epilogue:
 //   linear_act            y = act(z) + r
 //                         s = dy * act'(z); dx = s W; dW = s^T x; db = sum_m s
 //   linear_cross_entropy  l_m = log sum_v exp z_mv - z_m,t
 //                         G = g_m (softmax(z) - onehot(t)); dx = G W; dW = G^T x; db = sum_m G
+// Beside them, with kernels of their own: layer_norm (vi_norm.cu), linear_act in 8-bit integers (vi_quant.cu,
+// vi_heads_int8.cu) and sample_labels (vi_sample.cu).
 // Sums, the softmax's maximum and sum, and biases' gradients are float32; sums over
 // rows are split into pieces that are added in a fixed order, so results do not
 // depend on scheduling.
@@ -1066,11 +1068,221 @@ int ce_backward(Run& r, int dtype, const vi_matrix* x, const vi_matrix* w, const
   return VI_OK;
 }
 
+// ---- layer_norm ----
+int check_norm(int dtype, const vi_matrix* x, const void* w, const void* b, double eps) {
+  if (dtype < VI_F32 || dtype > VI_BF16) return bad("layer_norm: unknown element type");
+  if (!x || x->rows < 0 || x->cols < 1) return bad("layer_norm: x needs at least one column");
+  if (x->rows > kMaxSize || x->cols > kMaxSize) return bad("layer_norm: sizes are limited to 2^30");
+  if (!x->data && x->rows) return bad("layer_norm: x needs data");
+  if (x->row_stride < 0 || x->col_stride < 0) return bad("layer_norm: strides must not be negative");
+  if (!(eps >= 0.0) || eps > 3e38) return bad("layer_norm: eps must be a number of at least 0");
+  if (int rc = check_vector(dtype, x->data)) return rc;
+  if (int rc = check_vector(dtype, w)) return rc;
+  return check_vector(dtype, b);
+}
+
+int norm_forward(Run& r, int dtype, const vi_matrix* x, const void* w, const void* b, float eps, const vi_matrix* y, float* stats) {
+  if (int rc = check_norm(dtype, x, w, b, eps)) return rc;
+  if (!given(y) || y->rows != x->rows) return bad("layer_norm: y is required, [M, K]");
+  if (int rc = check_shape(dtype, y, x->rows, x->cols, true, "layer_norm: y must be a dense [M, K]")) return rc;
+  if (x->rows == 0 || r.dry) return VI_OK;
+  NormArgs a{x->rows, (int)x->cols, view(x), {}, view(y), w, b, eps, stats, nullptr};
+  const cudaError_t rc = launch_norm(dtype, a, false, r.sms, r.s, &r.launches);
+  return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+}
+
+int norm_backward(Run& r, int dtype, const vi_matrix* dy, const vi_matrix* x, const void* w, const float* stats, const vi_matrix* dx,
+                  void* dw, void* db) {
+  if (int rc = check_norm(dtype, x, w, nullptr, 0.0)) return rc;
+  if (int rc = check_vector(dtype, dw)) return rc;
+  if (int rc = check_vector(dtype, db)) return rc;
+  const int64_t M = x->rows, K = x->cols;
+  if (!given(dy) || dy->rows != M) return bad("layer_norm backward: dy is required, [M, K]");
+  if (int rc = check_shape(dtype, dy, M, K, false, "layer_norm backward: dy must be [M, K]")) return rc;
+  if (int rc = check_shape(dtype, dx, M, K, true, "layer_norm backward: dx must be a dense [M, K]")) return rc;
+  if (!r.dry && M && !stats) return bad("layer_norm backward: stats is required");
+  Summer sums{r, dtype};
+  if (M == 0) {
+    if (dw) sums.add(SumJob{nullptr, 0, 0, 0, 0, 1, K, nullptr, View{dw, 0, 1}});
+    if (db) sums.add(SumJob{nullptr, 0, 0, 0, 0, 1, K, nullptr, View{db, 0, 1}});
+    sums.run();
+    return VI_OK;
+  }
+  NormArgs a{M, (int)K, view(x), view(dy), view(dx), w, nullptr, 0.0f, const_cast<float*>(stats), nullptr};
+  const int pieces = norm_pieces(dtype, a, r.sms);
+  if (dw || db) a.part = (float*)r.take((size_t)pieces * 2 * K * 4);
+  if (!r.dry) {
+    const cudaError_t rc = launch_norm(dtype, a, true, r.sms, r.s, &r.launches);
+    if (rc != cudaSuccess) return set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+  }
+  if (dw) sums.add(SumJob{a.part, pieces, 2 * K, 0, 1, 1, K, nullptr, View{dw, 0, 1}});
+  if (db) sums.add(SumJob{a.part + K, pieces, 2 * K, 0, 1, 1, K, nullptr, View{db, 0, 1}});
+  sums.run();
+  return VI_OK;
+}
+
+// ---- 8-bit integers ----
+int quantize_rows(Run& r, int dtype, const vi_matrix* x, const vi_matrix* q, float* scale) {
+  if (dtype < VI_F32 || dtype > VI_BF16) return bad("quantize_rows: unknown element type");
+  if (!x || x->rows < 0 || x->cols < 1) return bad("quantize_rows: x needs at least one column");
+  if (x->rows > kMaxSize || x->cols > kMaxSize) return bad("quantize_rows: sizes are limited to 2^30");
+  if (!x->data && x->rows) return bad("quantize_rows: x needs data");
+  if (x->row_stride < 0 || x->col_stride < 0) return bad("quantize_rows: strides must not be negative");
+  if (int rc = check_vector(dtype, x->data)) return rc;
+  if (!q || q->rows != x->rows || q->cols != x->cols || q->col_stride != 1 || (q->rows > 1 && q->row_stride < q->cols))
+    return bad("quantize_rows: q must be [M, K] with contiguous rows");
+  if (x->rows == 0 || r.dry) return VI_OK;
+  if (!q->data || !scale || (uintptr_t)scale % 4) return bad("quantize_rows: q and scale are required");
+  const cudaError_t rc =
+      launch_quantize(dtype, QuantArgs{x->rows, (int)x->cols, view(x), (int8_t*)q->data, q->row_stride, scale}, r.sms, r.s);
+  r.launches++;
+  return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+}
+
+// Rows of 8-bit integers as the tensor cores' copies read them: in place, or copied.
+int operand8(Run& r, const vi_matrix* m, Operand& o) {
+  o = Operand{m->data, m->rows, m->cols, m->row_stride, 0, true};
+  if (m->col_stride == 1 && (m->row_stride >= m->cols || m->rows == 1) && (uintptr_t)m->data % 16 == 0 &&
+      (m->row_stride % 16 == 0 || m->rows == 1) && m->row_stride < (1ll << 38)) {
+    if (m->rows == 1) o.ld = ceil_div(m->cols, 16) * 16;
+    return VI_OK;
+  }
+  o.ld = ceil_div(m->cols, 16) * 16;
+  int8_t* dst = (int8_t*)r.take((size_t)m->rows * o.ld);
+  o.p = dst;
+  if (r.dry) return VI_OK;
+  const cudaError_t rc = launch_pack8(view(m), m->rows, m->cols, dst, o.ld, r.s);
+  r.launches++;
+  return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+}
+
+int int8_forward(Run& r, int dtype, int act, const vi_matrix* x, const float* x_scale, const vi_matrix* w, const float* w_scale,
+                 const void* bias, const vi_matrix* res, const vi_matrix* y) {
+  if (dtype < VI_F32 || dtype > VI_BF16) return bad("linear_act_int8: unknown element type");
+  if (act < VI_ACT_NONE || act > VI_ACT_SIGMOID) return bad("linear_act_int8: unknown activation");
+  if (!x || !w) return bad("linear_act_int8: x and weight are required");
+  if (x->rows < 0 || x->cols < 1 || w->rows < 1) return bad("linear_act_int8: x needs at least one column and weight one row");
+  if (w->cols != x->cols) return bad("linear_act_int8: weight and x differ in their number of columns");
+  if (x->cols > kInt8Terms) return bad("linear_act_int8: more than 2^17 columns do not fit a 32-bit sum");
+  if (x->rows > kMaxSize || w->rows > kMaxSize) return bad("linear_act_int8: sizes are limited to 2^30");
+  if ((!x->data && x->rows) || !w->data || !w_scale) return bad("linear_act_int8: x, weight and its scale need data");
+  if (x->row_stride < 0 || x->col_stride < 0 || w->row_stride < 0 || w->col_stride < 0)
+    return bad("linear_act_int8: strides must not be negative");
+  if ((!x_scale && (uintptr_t)x->data % elem(dtype)) || (uintptr_t)x_scale % 4 || (uintptr_t)w_scale % 4)
+    return bad("linear_act_int8: data must lie on whole elements");
+  if (int rc = check_vector(dtype, bias)) return rc;
+  const int64_t M = x->rows, K = x->cols, N = w->rows;
+  if (!given(y) || y->rows != M) return bad("linear_act_int8: y is required, [M, N]");
+  if (int rc = check_shape(dtype, res, M, N, false, "linear_act_int8: residual must be [M, N]")) return rc;
+  if (int rc = check_shape(dtype, y, M, N, true, "linear_act_int8: y must be a dense [M, N]")) return rc;
+  if (M == 0) return VI_OK;
+  Operand A{}, B{};
+  Epilogue e{};
+  e.act = act;
+  e.bias = bias;
+  e.res = view(res);
+  e.out = view(y);
+  e.col_scale = w_scale;
+  e.row_scale = x_scale;
+  if (x_scale) {
+    if (int rc = operand8(r, x, A)) return rc;
+  } else {
+    A = Operand{nullptr, M, K, ceil_div(K, 16) * 16, 0, true};
+    int8_t* q = (int8_t*)r.take((size_t)M * A.ld);
+    float* s = (float*)r.take((size_t)M * 4);
+    A.p = q;
+    e.row_scale = s;
+    if (!r.dry) {
+      const cudaError_t rc = launch_quantize(dtype, QuantArgs{M, (int)K, view(x), q, A.ld, s}, r.sms, r.s);
+      r.launches++;
+      if (rc != cudaSuccess) return set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+    }
+  }
+  if (int rc = operand8(r, w, B)) return rc;
+  if (r.dry) return VI_OK;
+  Plan p{};
+  p.splits = 1;
+  p.kps = (int)ceil_div(K, 128);
+  if (e.out.rs == 1 && e.out.cs != 1 && 4 * N >= 3 * 128 * ceil_div(N, 128)) {  // as gemm()
+    e.out = transposed(e.out);
+    e.res = transposed(e.res);
+    e.bias_rows = bias != nullptr;
+    std::swap(e.row_scale, e.col_scale);
+    std::swap(A, B);
+  }
+  p.bn = tile_width(dtype == VI_F32 ? VI_BF16 : dtype, kEpiInt8, A.rows, B.rows, 1, r.sms);
+  return launch_int8_gemm(dtype, A, B, p, e, r.sms, r.s);
+}
+
+// ---- sample_labels ----
+int sample_labels(Run& r, int dtype, const vi_matrix* z, const float* u, const vi_sampling* s, int64_t* label) {
+  if (dtype < VI_F32 || dtype > VI_BF16) return bad("sample_labels: unknown element type");
+  if (!z || !s) return bad("sample_labels: logits and settings are required");
+  if (z->rows < 0 || z->cols < 1) return bad("sample_labels: logits need at least one column");
+  if (z->rows > kMaxSize || z->cols > kMaxSize) return bad("sample_labels: sizes are limited to 2^30");
+  if (z->row_stride < 0 || z->col_stride < 0) return bad("sample_labels: strides must not be negative");
+  if (int rc = check_vector(dtype, z->data)) return rc;
+  if (!s->temperatures && !(s->temperature >= 0.0)) return bad("sample_labels: temperature must be at least 0");
+  if (!s->top_ks && s->top_k < 0) return bad("sample_labels: top_k must be at least 0");
+  if (!s->top_ps && !(s->top_p > 0.0)) return bad("sample_labels: top_p must be above 0");
+  if (!s->min_ps && !(s->min_p >= 0.0 && s->min_p <= 1.0)) return bad("sample_labels: min_p must lie in [0, 1]");
+  if (z->rows == 0 || r.dry) return VI_OK;
+  if (!z->data || !u || !label) return bad("sample_labels: logits, u and label need data");
+  SampleArgs a{z->rows,       (int)z->cols, view(z),     u,          s->temperatures, s->top_ks, s->top_ps,
+               s->min_ps,     s->temperature, s->top_p,  s->min_p,   s->top_k,        label};
+  const cudaError_t rc = launch_sample(dtype, a, r.sms, r.s);
+  r.launches++;
+  return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+}
+
 }  // namespace
 }  // namespace heads
 }  // namespace vi
 
 using namespace vi::heads;
+
+extern "C" int vi_layer_norm_forward(int dtype, const vi_matrix* x, const void* weight, const void* bias, float eps,
+                                     const vi_matrix* y, float* stats, void* stream) {
+  return execute([&](Run& r) { return norm_forward(r, dtype, x, weight, bias, eps, y, stats); }, nullptr, 0, stream, "layer_norm");
+}
+
+extern "C" uint64_t vi_layer_norm_backward_scratch_bytes(int dtype, const vi_matrix* dy, const vi_matrix* x, const void* weight,
+                                                         const vi_matrix* dx, const void* dweight, const void* dbias) {
+  return count_bytes([&](Run& r) {
+    return norm_backward(r, dtype, dy, x, weight, nullptr, dx, const_cast<void*>(dweight), const_cast<void*>(dbias));
+  });
+}
+
+extern "C" int vi_layer_norm_backward(int dtype, const vi_matrix* dy, const vi_matrix* x, const void* weight, const float* stats,
+                                      const vi_matrix* dx, void* dweight, void* dbias, void* scratch, uint64_t scratch_bytes,
+                                      void* stream) {
+  return execute([&](Run& r) { return norm_backward(r, dtype, dy, x, weight, stats, dx, dweight, dbias); }, scratch, scratch_bytes,
+                 stream, "layer_norm backward");
+}
+
+extern "C" int vi_quantize_rows(int dtype, const vi_matrix* x, const vi_matrix* q, float* scale, void* stream) {
+  return execute([&](Run& r) { return quantize_rows(r, dtype, x, q, scale); }, nullptr, 0, stream, "quantize_rows");
+}
+
+extern "C" uint64_t vi_linear_act_int8_scratch_bytes(int dtype, int activation, const vi_matrix* x, const float* x_scale,
+                                                     const vi_matrix* weight, const float* weight_scale, const void* bias,
+                                                     const vi_matrix* residual, const vi_matrix* y) {
+  return count_bytes(
+      [&](Run& r) { return int8_forward(r, dtype, activation, x, x_scale, weight, weight_scale, bias, residual, y); });
+}
+
+extern "C" int vi_linear_act_int8(int dtype, int activation, const vi_matrix* x, const float* x_scale, const vi_matrix* weight,
+                                  const float* weight_scale, const void* bias, const vi_matrix* residual, const vi_matrix* y,
+                                  void* scratch, uint64_t scratch_bytes, void* stream) {
+  return execute(
+      [&](Run& r) { return int8_forward(r, dtype, activation, x, x_scale, weight, weight_scale, bias, residual, y); }, scratch,
+      scratch_bytes, stream, "linear_act_int8");
+}
+
+extern "C" int vi_sample_labels(int dtype, const vi_matrix* logits, const float* u, const vi_sampling* settings, int64_t* label,
+                                void* stream) {
+  return execute([&](Run& r) { return sample_labels(r, dtype, logits, u, settings, label); }, nullptr, 0, stream, "sample_labels");
+}
 
 extern "C" uint64_t vi_linear_act_forward_scratch_bytes(int dtype, int activation, const vi_matrix* x,
                                                         const vi_matrix* weight, const void* bias,

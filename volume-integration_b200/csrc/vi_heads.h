@@ -33,6 +33,7 @@ enum Epi {
   kEpiPartial,  // part[split] = acc, or += acc (float32)
   kEpiLse,      // per row the maximum and the sum of exponentials of the logits, the target's logit
   kEpiGrad,     // G = coef * (softmax - onehot)
+  kEpiInt8,     // out = act(acc * row_scale * col_scale + bias) + res, acc of 8-bit integers
   kEpiCount
 };
 
@@ -84,6 +85,9 @@ struct Epilogue {
   int64_t col0;
   void* grad;           // [planes][M][grad_ld], 16-bit
   int64_t grad_ld, grad_plane;
+  // kEpiInt8: [M], [N]
+  const float* row_scale;
+  const float* col_scale;
   float* column_part;   // 16-bit types: [4 per tile of 128 rows][N] sums of G's columns over 32 rows, of the cells as
                         // rounded, which dx and dweight use too; null = not wanted
 };
@@ -99,6 +103,10 @@ struct Plan {
 
 // Partial results of kEpiLse per span.
 int lse_parts(int bn);
+
+// The current device's word of the products' timeouts (null: no device), and the count of launches in pairs.
+uint32_t* status_word();
+void note_pair_launch();
 
 // dtype: of outputs, bias and residual.  Planes: 1, or 3 for float32.
 // Returns a vi_status.
@@ -153,6 +161,53 @@ struct SmallJobs {
 constexpr int64_t kSmallWork = 1 << 24, kSmallSum = 512;
 bool small_product(int64_t M, int64_t N, int64_t K, int64_t longest);
 cudaError_t launch_small(int dtype, const SmallJob& a, const SmallJob* b, cudaStream_t s);
+
+// kEpiInt8's product (vi_heads_int8.cu): operands of 8-bit integers, k contiguous, ld a multiple of 16.
+constexpr int64_t kInt8Terms = 1 << 17;  // 127^2 of each fit the 32-bit sum
+int launch_int8_gemm(int dtype, const Operand& a, const Operand& b, const Plan& p, const Epilogue& e, int sms, cudaStream_t s);
+
+// Rows of 8-bit integers with a scale each: q = x / scale rounded to even, scale = largest |x| / 127.
+struct QuantArgs {
+  int64_t M;
+  int K;
+  View x;
+  int8_t* q;
+  int64_t ld;    // q's row stride
+  float* scale;  // [M]
+};
+cudaError_t launch_quantize(int dtype, const QuantArgs& a, int sms, cudaStream_t s);
+// Copies [rows, k] 8-bit integers of any strides to rows `ld` apart.
+cudaError_t launch_pack8(const View& src, int64_t rows, int64_t k, int8_t* dst, int64_t ld, cudaStream_t s);
+
+// Labels drawn from rows of logits (vi_sample.cu).
+struct SampleArgs {
+  int64_t M;
+  int V;
+  View z;
+  const float* u;            // [M]
+  const float* temperature;  // [M], null: the same for all; so the others
+  const int64_t* top_k;
+  const float *top_p, *min_p;
+  double temperature_all, top_p_all, min_p_all;
+  int64_t top_k_all;
+  int64_t* label;            // [M]
+  double unit;               // set by the launcher: of weights that are added as whole numbers
+};
+cudaError_t launch_sample(int dtype, const SampleArgs& a, int sms, cudaStream_t s);
+
+// Layer norm of rows (vi_norm.cu).
+struct NormArgs {
+  int64_t M;
+  int K;
+  View x, dy;          // dy: backward, else p null
+  View y;              // the result; in the backward dx, p null = not wanted
+  const void *w, *b;   // null = 1, 0
+  float eps;
+  float* stats;        // [3][M] the mean, what it still lacked, 1 / sqrt(v + eps); forward: null = not wanted
+  float* part;         // backward: [norm_pieces][2][K] sums of dy h and of dy; null = not wanted
+};
+int norm_pieces(int dtype, const NormArgs& a, int sms);
+cudaError_t launch_norm(int dtype, const NormArgs& a, bool backward, int sms, cudaStream_t s, int* launches);
 
 }  // namespace heads
 }  // namespace vi

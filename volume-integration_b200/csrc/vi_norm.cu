@@ -1,0 +1,714 @@
+// Layer norm of rows, forward and backward.
+//
+// Mathematics.  For a row x of K features: mu = mean x, v = mean (x - mu)^2, r = 1 / sqrt(v + eps),
+//   h = (x - mu) r,  y = h w + b.
+// Backward, g = dy w:  dx = r (g - mean g - h mean(g h));  dw = sum_m dy h;  db = sum_m dy.
+// All sums are float32.  The mean's own rounding is taken out again: with d = x - mu the mean of d is subtracted
+// from d, so rows far from zero lose nothing (mean 1000, spread 1: 6e-5 of h otherwise).
+//
+// Memory bounds it: a row is read once, kept in registers, and its statistics are made of what the registers
+// hold.  Rows of contiguous features belong to 1 to 32 lanes or to a block (vectors of 16 bytes, or single elements
+// where strides or sizes do not allow them); images, where pixels are contiguous, to blocks whose lanes hold
+// neighbouring pixels and whose warps share the channels.  Rows that no block can hold are read again for each step.
+// The weights' gradients are summed in registers over a persistent block's rows, then over blocks in order.
+#include <algorithm>
+#include <atomic>
+
+#include "vi_heads.h"
+#include "vi_heads_math.cuh"
+#include "vi_internal.h"
+
+namespace vi {
+namespace heads {
+namespace {
+
+template <typename T, int N>
+struct __align__(N * sizeof(T) >= 16 ? 16 : N * sizeof(T)) Chunk {
+  T v[N];
+};
+template <typename T, int N>
+__device__ __forceinline__ Chunk<T, N> chunk_zero() {
+  Chunk<T, N> c;
+#pragma unroll
+  for (int i = 0; i < N; i++) c.v[i] = from_f<T>(0.0f);
+  return c;
+}
+
+// Sum of S values over the lanes of a row: G lanes of a warp, or a block.  Every lane gets it, always added in the same
+// order.
+template <int S, bool BLOCK>
+__device__ __forceinline__ void row_sum(float (&s)[S], int lanes, float (*sh)[16][S], int& turn) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    if (!BLOCK && o >= lanes) continue;
+#pragma unroll
+    for (int i = 0; i < S; i++) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+  }
+  if constexpr (BLOCK) {  // two buffers in turn: a barrier each sum
+    const int warps = blockDim.x / 32;
+    if (threadIdx.x % 32 == 0) {
+#pragma unroll
+      for (int i = 0; i < S; i++) sh[turn][threadIdx.x / 32][i] = s[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S; i++) s[i] = 0.0f;
+    for (int w = 0; w < warps; w++) {
+#pragma unroll
+      for (int i = 0; i < S; i++) s[i] += sh[turn][w][i];
+    }
+    turn ^= 1;
+  }
+}
+
+// The lane's NV chunks of a row: columns (v * lanes + lane) * VEC on.
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void load_row(Chunk<T, VEC> (&c)[NV], const View& m, int64_t row, int K, int lanes, int lane) {
+  const T* p = (const T*)m.p + row * m.rs;
+#pragma unroll
+  for (int v = 0; v < NV; v++) {
+    const int at = (v * lanes + lane) * VEC;
+    if constexpr (VEC > 1) c[v] = at < K ? *(const Chunk<T, VEC>*)(p + at) : chunk_zero<T, VEC>();
+    else c[v].v[0] = at < K ? p[at * m.cs] : from_f<T>(0.0f);
+  }
+}
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void load_weights(Chunk<T, VEC> (&c)[NV], const void* w, float none, int K, int lanes, int lane) {
+#pragma unroll
+  for (int v = 0; v < NV; v++) {
+    const int at = (v * lanes + lane) * VEC;
+    if (w && at < K) c[v] = *(const Chunk<T, VEC>*)((const T*)w + at);
+    else {
+#pragma unroll
+      for (int i = 0; i < VEC; i++) c[v].v[i] = from_f<T>(none);
+    }
+  }
+}
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void store_row(const Chunk<T, VEC> (&c)[NV], const View& m, int64_t row, int K, int lanes, int lane) {
+  T* p = (T*)m.p + row * m.rs;
+#pragma unroll
+  for (int v = 0; v < NV; v++) {
+    const int at = (v * lanes + lane) * VEC;
+    if (at < K) {
+      if constexpr (VEC > 1) *(Chunk<T, VEC>*)(p + at) = c[v];
+      else p[at * m.cs] = c[v].v[0];
+    }
+  }
+}
+
+constexpr int kRowThreads = 256;  // of a block whose rows belong to lanes
+constexpr int kBlockMost = 512;   // of a block that a row belongs to
+
+// R rows at a time for each group of lanes, so that short rows have loads in flight too.
+template <typename T, int VEC, int NV, int R, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
+    norm_rows_forward(const __grid_constant__ NormArgs a, int lanes) {
+  __shared__ float sh1[2][16][R], sh2[2][16][2 * R];
+  int turn1 = 0, turn2 = 0;
+  const int lane = BLOCK ? threadIdx.x : threadIdx.x % lanes, group = BLOCK ? 0 : threadIdx.x / lanes;
+  const int groups = BLOCK ? 1 : kRowThreads / lanes;
+  const float inv = 1.0f / (float)a.K;
+  Chunk<T, VEC> w[NV], b[NV];
+  load_weights(w, a.w, 1.0f, a.K, lanes, lane);
+  load_weights(b, a.b, 0.0f, a.K, lanes, lane);
+  for (int64_t m0 = (int64_t)blockIdx.x * groups * R; m0 < a.M; m0 += (int64_t)gridDim.x * groups * R) {
+    Chunk<T, VEC> x[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; r++) load_row(x[r], a.x, min(m0 + r * groups + group, a.M - 1), a.K, lanes, lane);
+    float mean[R], q[2 * R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      mean[r] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < NV; v++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) mean[r] += to_f(x[r][v].v[i]);
+    }
+    row_sum<R, BLOCK>(mean, lanes, sh1, turn1);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      mean[r] *= inv;
+      q[2 * r] = q[2 * r + 1] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < NV; v++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          const float d = (v * lanes + lane) * VEC < a.K ? to_f(x[r][v].v[i]) - mean[r] : 0.0f;
+          q[2 * r] += d;
+          q[2 * r + 1] = fmaf(d, d, q[2 * r + 1]);
+        }
+    }
+    row_sum<2 * R, BLOCK>(q, lanes, sh2, turn2);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int64_t m = m0 + r * groups + group;
+      const float shift = q[2 * r] * inv;
+      const float rstd = 1.0f / sqrtf(fmaxf(fmaf(-shift, shift, q[2 * r + 1] * inv), 0.0f) + a.eps);
+      if (m < a.M) {
+        Chunk<T, VEC> y[NV];
+#pragma unroll
+        for (int v = 0; v < NV; v++)
+#pragma unroll
+          for (int i = 0; i < VEC; i++)
+            y[v].v[i] = from_f<T>(fmaf((to_f(x[r][v].v[i]) - mean[r] - shift) * rstd, to_f(w[v].v[i]), to_f(b[v].v[i])));
+        store_row(y, a.y, m, a.K, lanes, lane);
+        if (a.stats && lane == 0) a.stats[m] = mean[r], a.stats[a.M + m] = shift, a.stats[2 * a.M + m] = rstd;
+      }
+    }
+  }
+}
+
+template <typename T, int VEC, int NV, int R, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
+    norm_rows_backward(const __grid_constant__ NormArgs a, int lanes) {
+  __shared__ float sh[2][16][2 * R];
+  __shared__ float cols[BLOCK ? 1 : kRowThreads / 32][BLOCK ? 1 : 32 * VEC * NV];
+  int turn = 0;
+  const int lane = BLOCK ? threadIdx.x : threadIdx.x % lanes, group = BLOCK ? 0 : threadIdx.x / lanes;
+  const int groups = BLOCK ? 1 : kRowThreads / lanes;
+  const float inv = 1.0f / (float)a.K;
+  Chunk<T, VEC> w[NV];
+  load_weights(w, a.w, 1.0f, a.K, lanes, lane);
+  float dw[NV][VEC] = {}, db[NV][VEC] = {};
+  for (int64_t m0 = (int64_t)blockIdx.x * groups * R; m0 < a.M; m0 += (int64_t)gridDim.x * groups * R) {
+    Chunk<T, VEC> x[R][NV], dy[R][NV];
+    float mean[R], shift[R], rstd[R], q[2 * R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int64_t m = min(m0 + r * groups + group, a.M - 1);
+      load_row(x[r], a.x, m, a.K, lanes, lane);
+      load_row(dy[r], a.dy, m, a.K, lanes, lane);
+      mean[r] = a.stats[m], shift[r] = a.stats[a.M + m], rstd[r] = a.stats[2 * a.M + m];
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const bool on = m0 + r * groups + group < a.M;
+      q[2 * r] = q[2 * r + 1] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < NV; v++)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+          // beyond K and beyond M nothing is added: h of a zero is not one
+          const bool in = on && (v * lanes + lane) * VEC < a.K;
+          const float h = in ? (to_f(x[r][v].v[i]) - mean[r] - shift[r]) * rstd[r] : 0.0f, d = in ? to_f(dy[r][v].v[i]) : 0.0f;
+          const float g = d * to_f(w[v].v[i]);
+          q[2 * r] += g;
+          q[2 * r + 1] = fmaf(g, h, q[2 * r + 1]);
+          dw[v][i] = fmaf(d, h, dw[v][i]);
+          db[v][i] += d;
+        }
+    }
+    if (!a.y.p) continue;
+    row_sum<2 * R, BLOCK>(q, lanes, sh, turn);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int64_t m = m0 + r * groups + group;
+      if (m < a.M) {
+        const float mg = q[2 * r] * inv, mgh = q[2 * r + 1] * inv;
+        Chunk<T, VEC> y[NV];
+#pragma unroll
+        for (int v = 0; v < NV; v++)
+#pragma unroll
+          for (int i = 0; i < VEC; i++) {
+            const float h = (to_f(x[r][v].v[i]) - mean[r] - shift[r]) * rstd[r];
+            y[v].v[i] = from_f<T>(rstd[r] * (fmaf(to_f(dy[r][v].v[i]), to_f(w[v].v[i]), -mg) - h * mgh));
+          }
+        store_row(y, a.y, m, a.K, lanes, lane);
+      }
+    }
+  }
+  if (!a.part) return;
+  float* out = a.part + (int64_t)blockIdx.x * 2 * a.K;
+#pragma unroll
+  for (int which = 0; which < 2; which++) {
+#pragma unroll
+    for (int v = 0; v < NV; v++)
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        float s = which ? db[v][i] : dw[v][i];
+        const int at = (v * lanes + lane) * VEC + i;
+        if constexpr (BLOCK) {
+          if (at < a.K) out[which * a.K + at] = s;
+        } else {
+          for (int o = lanes; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if (threadIdx.x % 32 < lanes) cols[threadIdx.x / 32][at] = s;
+        }
+      }
+    if constexpr (!BLOCK) {
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.K; c += kRowThreads) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRowThreads / 32; i++) s += cols[i][c];
+        out[which * a.K + c] = s;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Rows of any length: a block a row, which it reads again for each step.
+template <typename T, bool BACKWARD>
+__global__ void __launch_bounds__(512) norm_long_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float sh1[2][16][1], sh2[2][16][2];
+  int turn1 = 0, turn2 = 0;
+  const float inv = 1.0f / (float)a.K;
+  const T *w = (const T*)a.w, *b = (const T*)a.b;
+  for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
+    const T* x = (const T*)a.x.p + m * a.x.rs;
+    const T* dy = (const T*)a.dy.p + m * a.dy.rs;
+    T* y = (T*)a.y.p + m * a.y.rs;
+    float q[2] = {0.0f, 0.0f};
+    if constexpr (BACKWARD) {
+      const float mean = a.stats[m], shift = a.stats[a.M + m], rstd = a.stats[2 * a.M + m];
+      for (int k = threadIdx.x; k < a.K; k += 512) {
+        const float h = (to_f(x[k * a.x.cs]) - mean - shift) * rstd, g = to_f(dy[k * a.dy.cs]) * (w ? to_f(w[k]) : 1.0f);
+        q[0] += g;
+        q[1] = fmaf(g, h, q[1]);
+      }
+      row_sum<2, true>(q, 512, sh2, turn2);
+      for (int k = threadIdx.x; k < a.K; k += 512) {
+        const float h = (to_f(x[k * a.x.cs]) - mean - shift) * rstd;
+        y[k * a.y.cs] = from_f<T>(rstd * (fmaf(to_f(dy[k * a.dy.cs]), w ? to_f(w[k]) : 1.0f, -q[0] * inv) - h * (q[1] * inv)));
+      }
+    } else {
+      float s[1] = {0.0f};
+      for (int k = threadIdx.x; k < a.K; k += 512) s[0] += to_f(x[k * a.x.cs]);
+      row_sum<1, true>(s, 512, sh1, turn1);
+      const float mean = s[0] * inv;
+      for (int k = threadIdx.x; k < a.K; k += 512) {
+        const float d = to_f(x[k * a.x.cs]) - mean;
+        q[0] += d;
+        q[1] = fmaf(d, d, q[1]);
+      }
+      row_sum<2, true>(q, 512, sh2, turn2);
+      const float shift = q[0] * inv, rstd = 1.0f / sqrtf(fmaxf(fmaf(-shift, shift, q[1] * inv), 0.0f) + a.eps);
+      for (int k = threadIdx.x; k < a.K; k += 512)
+        y[k * a.y.cs] = from_f<T>(fmaf((to_f(x[k * a.x.cs]) - mean - shift) * rstd, w ? to_f(w[k]) : 1.0f, b ? to_f(b[k]) : 0.0f));
+      if (a.stats && threadIdx.x == 0) a.stats[m] = mean, a.stats[a.M + m] = shift, a.stats[2 * a.M + m] = rstd;
+    }
+  }
+}
+
+// The weights' gradients alone, of rows that no block holds: lanes along columns (or along rows, for images), a block
+// 32 columns of a piece of the rows.
+template <typename T>
+__global__ void __launch_bounds__(256) norm_columns_kernel(const __grid_constant__ NormArgs a, int64_t rows, bool image) {
+  __shared__ float sh[2][8][32];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int64_t m0 = (int64_t)blockIdx.y * rows, m1 = min(a.M, m0 + rows);
+  float* out = a.part + (int64_t)blockIdx.y * 2 * a.K;
+  const T *x = (const T*)a.x.p, *dy = (const T*)a.dy.p;
+  const auto add = [&](int64_t m, int64_t k, float& dw, float& db) {
+    const float d = to_f(dy[m * a.dy.rs + k * a.dy.cs]);
+    dw = fmaf(d, (to_f(x[m * a.x.rs + k * a.x.cs]) - a.stats[m] - a.stats[a.M + m]) * a.stats[2 * a.M + m], dw);
+    db += d;
+  };
+  if (image) {  // a warp a column
+    for (int c = ty; c < 32; c += 8) {
+      const int64_t k = (int64_t)blockIdx.x * 32 + c;
+      if (k >= a.K) break;
+      float dw = 0.0f, db = 0.0f;
+      for (int64_t m = m0 + tx; m < m1; m += 32) add(m, k, dw, db);
+      for (int o = 16; o; o >>= 1) {
+        dw += __shfl_xor_sync(0xffffffffu, dw, o);
+        db += __shfl_xor_sync(0xffffffffu, db, o);
+      }
+      if (tx == 0) out[k] = dw, out[a.K + k] = db;
+    }
+    return;
+  }
+  const int64_t k = (int64_t)blockIdx.x * 32 + tx;
+  float dw = 0.0f, db = 0.0f;
+  if (k < a.K)
+    for (int64_t m = m0 + ty; m < m1; m += 8) add(m, k, dw, db);
+  sh[0][ty][tx] = dw, sh[1][ty][tx] = db;
+  __syncthreads();
+  if (ty < 2 && k < a.K) {
+    float s = 0.0f;
+    for (int i = 0; i < 8; i++) s += sh[ty][i][tx];
+    out[ty * a.K + k] = s;
+  }
+}
+
+// ---- images: pixels contiguous ----
+// A lane holds VP neighbouring pixels, a warp every `warps`-th channel of them, up to R; `warps` warps make a tile of
+// 32 VP pixels.  VP = 1: any strides.
+template <typename T, int VP>
+__device__ __forceinline__ Chunk<T, VP> load_pixels(const View& m, int64_t row, int64_t c, int64_t M) {
+  const T* p = (const T*)m.p + row * m.rs + c * m.cs;
+  Chunk<T, VP> r = chunk_zero<T, VP>();
+  if (row + VP <= M) {
+    r = *(const Chunk<T, VP>*)p;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VP; j++)
+      if (row + j < M) r.v[j] = p[j * m.rs];
+  }
+  return r;
+}
+template <typename T, int VP>
+__device__ __forceinline__ void store_pixels(const Chunk<T, VP>& r, const View& m, int64_t row, int64_t c, int64_t M) {
+  T* p = (T*)m.p + row * m.rs + c * m.cs;
+  if (row + VP <= M) {
+    *(Chunk<T, VP>*)p = r;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VP; j++)
+      if (row + j < M) p[j * m.rs] = r.v[j];
+  }
+}
+// Sum of a lane's VP values over the warps of its tile, in order; sh holds a block's lanes' values.
+template <int VP>
+__device__ __forceinline__ void tile_sum(float (&s)[VP], float* sh, int first, int warps, int lane) {
+#pragma unroll
+  for (int j = 0; j < VP; j++) s[j] = 0.0f;
+  for (int i = 0; i < warps; i++) {
+#pragma unroll
+    for (int j = 0; j < VP; j++) s[j] += sh[((first + i) * VP + j) * 32 + lane];
+  }
+}
+template <int VP>
+__device__ __forceinline__ void tile_put(const float (&s)[VP], float* sh, int warp, int lane) {
+#pragma unroll
+  for (int j = 0; j < VP; j++) sh[(warp * VP + j) * 32 + lane] = s[j];
+}
+
+// LONG: more channels than the warps hold, so each step reads them again.
+template <typename T, int VP, int R, bool LONG>
+__global__ void __launch_bounds__(512) norm_image_forward(const __grid_constant__ NormArgs a, int warps) {
+  extern __shared__ float sh[];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, first = warp - tw, per = blockDim.x / 32 / warps;
+  const int size = blockDim.x * VP;  // floats of one exchange
+  const float inv = 1.0f / (float)a.K;
+  const T *w = (const T*)a.w, *b = (const T*)a.b;
+  const int64_t tiles = (a.M + 32 * VP - 1) / (32 * VP);
+  for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < tiles; t0 += (int64_t)gridDim.x * per) {
+    const int64_t m = ((t0 + warp / warps) * 32 + lane) * VP;
+    Chunk<T, VP> x[R];
+    const auto load = [&](int k0) {
+#pragma unroll
+      for (int i = 0; i < R; i++)
+        if (k0 + tw + i * warps < a.K) x[i] = load_pixels<T, VP>(a.x, m, k0 + tw + i * warps, a.M);
+    };
+    const auto channels = [&](auto f) {
+      if (m >= a.M) return;
+      for (int k0 = 0; k0 < (LONG ? a.K : 1); k0 += R * warps) {
+        if (LONG) load(k0);
+#pragma unroll
+        for (int i = 0; i < R; i++)
+          if (k0 + tw + i * warps < a.K) f(x[i], k0 + tw + i * warps);
+      }
+    };
+    float mean[VP] = {}, d1[VP] = {}, d2[VP] = {}, rstd[VP];
+    if (!LONG && m < a.M) load(0);
+    channels([&](const Chunk<T, VP>& v, int) {
+#pragma unroll
+      for (int j = 0; j < VP; j++) mean[j] += to_f(v.v[j]);
+    });
+    if (warps > 1) {
+      tile_put(mean, sh, warp, lane);
+      __syncthreads();
+      tile_sum(mean, sh, first, warps, lane);
+    }
+#pragma unroll
+    for (int j = 0; j < VP; j++) mean[j] *= inv;
+    channels([&](const Chunk<T, VP>& v, int) {
+#pragma unroll
+      for (int j = 0; j < VP; j++) {
+        const float d = to_f(v.v[j]) - mean[j];
+        d1[j] += d;
+        d2[j] = fmaf(d, d, d2[j]);
+      }
+    });
+    if (warps > 1) {
+      tile_put(d1, sh + size, warp, lane);
+      tile_put(d2, sh + 2 * size, warp, lane);
+      __syncthreads();
+      tile_sum(d1, sh + size, first, warps, lane);
+      tile_sum(d2, sh + 2 * size, first, warps, lane);
+    }
+#pragma unroll
+    for (int j = 0; j < VP; j++) {
+      d1[j] *= inv;
+      rstd[j] = 1.0f / sqrtf(fmaxf(fmaf(-d1[j], d1[j], d2[j] * inv), 0.0f) + a.eps);
+      if (a.stats && tw == 0 && m + j < a.M)
+        a.stats[m + j] = mean[j], a.stats[a.M + m + j] = d1[j], a.stats[2 * a.M + m + j] = rstd[j];
+    }
+    channels([&](const Chunk<T, VP>& v, int c) {
+      const float wc = w ? to_f(w[c]) : 1.0f, bc = b ? to_f(b[c]) : 0.0f;
+      Chunk<T, VP> y;
+#pragma unroll
+      for (int j = 0; j < VP; j++) y.v[j] = from_f<T>(fmaf((to_f(v.v[j]) - mean[j] - d1[j]) * rstd[j], wc, bc));
+      store_pixels<T, VP>(y, a.y, m, c, a.M);
+    });
+  }
+}
+
+template <typename T, int VP, int R, bool LONG>
+__global__ void __launch_bounds__(512) norm_image_backward(const __grid_constant__ NormArgs a, int warps) {
+  extern __shared__ float sh[];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, first = warp - tw, per = blockDim.x / 32 / warps;
+  const int size = blockDim.x * VP;
+  const float inv = 1.0f / (float)a.K;
+  const T* w = (const T*)a.w;
+  float dw[R] = {}, db[R] = {};  // not LONG
+  const int64_t tiles = (a.M + 32 * VP - 1) / (32 * VP);
+  int turn = 0;
+  for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < tiles; t0 += (int64_t)gridDim.x * per) {
+    const int64_t m = ((t0 + warp / warps) * 32 + lane) * VP;
+    Chunk<T, VP> x[R], dy[R];
+    const auto load = [&](int k0) {
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const int c = k0 + tw + i * warps;
+        if (c < a.K) x[i] = load_pixels<T, VP>(a.x, m, c, a.M), dy[i] = load_pixels<T, VP>(a.dy, m, c, a.M);
+      }
+    };
+    const auto channels = [&](auto f) {
+      if (m >= a.M) return;
+      for (int k0 = 0; k0 < (LONG ? a.K : 1); k0 += R * warps) {
+        if (LONG) load(k0);
+#pragma unroll
+        for (int i = 0; i < R; i++)
+          if (k0 + tw + i * warps < a.K) f(i, k0 + tw + i * warps);
+      }
+    };
+    float mean[VP], shift[VP], rstd[VP], q1[VP] = {}, q2[VP] = {};
+    if (!LONG && m < a.M) load(0);
+#pragma unroll
+    for (int j = 0; j < VP; j++) {  // h of a pixel that is not there: 0
+      const bool in = m + j < a.M;
+      mean[j] = in ? a.stats[m + j] : 0.0f;
+      shift[j] = in ? a.stats[a.M + m + j] : 0.0f;
+      rstd[j] = in ? a.stats[2 * a.M + m + j] : 0.0f;
+    }
+    channels([&](int i, int c) {
+      const float wc = w ? to_f(w[c]) : 1.0f;
+#pragma unroll
+      for (int j = 0; j < VP; j++) {
+        const float h = (to_f(x[i].v[j]) - mean[j] - shift[j]) * rstd[j], d = to_f(dy[i].v[j]), g = d * wc;
+        q1[j] += g;
+        q2[j] = fmaf(g, h, q2[j]);
+        if (!LONG) {
+          dw[i] = fmaf(d, h, dw[i]);
+          db[i] += d;
+        }
+      }
+    });
+    if (!a.y.p) continue;
+    if (warps > 1) {  // two exchanges in turn: one barrier a tile
+      float* s = sh + turn * 2 * size;
+      tile_put(q1, s, warp, lane);
+      tile_put(q2, s + size, warp, lane);
+      __syncthreads();
+      tile_sum(q1, s, first, warps, lane);
+      tile_sum(q2, s + size, first, warps, lane);
+      turn ^= 1;
+    }
+    channels([&](int i, int c) {
+      const float wc = w ? to_f(w[c]) : 1.0f;
+      Chunk<T, VP> y;
+#pragma unroll
+      for (int j = 0; j < VP; j++) {
+        const float h = (to_f(x[i].v[j]) - mean[j] - shift[j]) * rstd[j];
+        y.v[j] = from_f<T>(rstd[j] * (fmaf(to_f(dy[i].v[j]), wc, -q1[j] * inv) - h * (q2[j] * inv)));
+      }
+      store_pixels<T, VP>(y, a.y, m, c, a.M);
+    });
+  }
+  if (LONG || !a.part) return;
+  float* out = a.part + ((int64_t)blockIdx.x * per + warp / warps) * 2 * a.K;
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int c = tw + i * warps;
+    float s = dw[i], t = db[i];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if (lane == 0 && c < a.K) out[c] = s, out[a.K + c] = t;
+  }
+}
+
+// ---- host ----
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// One call: what is launched, in how many blocks; `pieces` partial sums of the weights' gradients.
+struct Call {
+  const NormArgs& a;
+  int sms;
+  cudaStream_t s;
+  bool dry;
+  int pieces = 0, launches = 0;
+  cudaError_t rc = cudaSuccess;
+
+  // `units` pieces of work, one a block at a time; `per` partial sums a block.
+  template <auto kernel>
+  void run(int threads, size_t smem, int64_t units, int lanes, int per) {
+    static std::atomic<int> known[33];  // blocks per SM by warps a block (one size of smem each)
+    static std::atomic<uint64_t> large;  // devices on which the kernel may have more than 48 KB
+    if (smem > 48 * 1024) {
+      int dev = 0;
+      cudaGetDevice(&dev);
+      const uint64_t bit = 1ull << (dev & 63);
+      if (dev >= 64 || !(large.load(std::memory_order_relaxed) & bit)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) cudaGetLastError();
+        else if (dev < 64) large.fetch_or(bit, std::memory_order_relaxed);
+      }
+    }
+    int n = known[threads / 32].load(std::memory_order_relaxed);
+    if (n <= 0) {
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess && n > 0)
+        known[threads / 32].store(n, std::memory_order_relaxed);
+      else
+        cudaGetLastError(), n = 1;
+    }
+    const int64_t blocks = std::min<int64_t>(units, (int64_t)sms * n);
+    pieces = (int)blocks * per;
+    if (dry || (!a.y.p && !a.part)) return;
+    kernel<<<(unsigned)blocks, threads, smem, s>>>(a, lanes);
+    rc = cudaPeekAtLastError();
+    launches++;
+  }
+  template <typename T>
+  void run_long(bool backward, bool image) {
+    const unsigned blocks = (unsigned)std::min<int64_t>(a.M, (int64_t)sms * 4);
+    if (!dry && a.y.p) {
+      if (backward) norm_long_kernel<T, true><<<blocks, 512, 0, s>>>(a);
+      else norm_long_kernel<T, false><<<blocks, 512, 0, s>>>(a);
+      rc = cudaPeekAtLastError();
+      launches++;
+    }
+    if (backward) columns<T>(image);
+  }
+  template <typename T>
+  void columns(bool image) {
+    const int64_t strips = ceil_div(a.K, 32);
+    const int64_t rows = std::max<int64_t>(64, ceil_div(a.M, std::max<int64_t>(1, sms * 8 / strips)));
+    pieces = (int)ceil_div(a.M, rows);
+    if (dry || !a.part || rc != cudaSuccess) return;
+    norm_columns_kernel<T><<<dim3((unsigned)strips, (unsigned)pieces), 256, 0, s>>>(a, rows, image);
+    rc = cudaPeekAtLastError();
+    launches++;
+  }
+};
+
+int pow2_at_least(int64_t n) {
+  int p = 1;
+  while (p < n) p *= 2;
+  return p;
+}
+
+// Rows of `units` vectors or elements by lanes, or by a block: false where this shape does not hold them.
+template <typename T, int VEC, int NV, int R, bool BACKWARD>
+bool rows_lanes(Call& c, int64_t units) {
+  if (units > 32 * NV) return false;
+  const int lanes = NV > 1 ? 32 : pow2_at_least(units);
+  const int64_t work = ceil_div(c.a.M, (int64_t)kRowThreads / lanes * R);
+  if constexpr (BACKWARD) c.run<norm_rows_backward<T, VEC, NV, R, false>>(kRowThreads, 0, work, lanes, 1);
+  else c.run<norm_rows_forward<T, VEC, NV, R, false>>(kRowThreads, 0, work, lanes, 1);
+  return true;
+}
+template <typename T, int VEC, int NV, bool BACKWARD>
+bool rows_block(Call& c, int64_t units) {
+  if (units > (int64_t)kBlockMost * NV) return false;
+  const int threads = (int)ceil_div(ceil_div(units, NV), 32) * 32;
+  if constexpr (BACKWARD) c.run<norm_rows_backward<T, VEC, NV, 1, true>>(threads, 0, c.a.M, threads, 1);
+  else c.run<norm_rows_forward<T, VEC, NV, 1, true>>(threads, 0, c.a.M, threads, 1);
+  return true;
+}
+template <typename T, int VP, int R, bool LONG, bool BACKWARD>
+void image_tiles(Call& c) {
+  const int need = (int)std::min<int64_t>(16, ceil_div(c.a.K, R));
+  const int warps = pow2_at_least(need), block = std::max(8, warps);
+  const int64_t work = ceil_div(ceil_div(c.a.M, 32 * VP), block / warps);
+  const size_t smem = (size_t)block * 32 * VP * 4 * (BACKWARD ? 4 : 3);
+  if constexpr (BACKWARD) c.run<norm_image_backward<T, VP, R, LONG>>(block * 32, smem, work, warps, block / warps);
+  else c.run<norm_image_forward<T, VP, R, LONG>>(block * 32, smem, work, warps, block / warps);
+}
+
+template <typename T>
+void norm_call(Call& c, bool backward) {
+  const NormArgs& a = c.a;
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const bool image = a.x.rs == 1 && a.x.cs != 1 && a.M > 1;
+  // whether n neighbouring elements along the contiguous axis may be moved at once, everywhere
+  const auto wide = [&](int n, bool along_rows) {
+    for (const View* v : {&a.x, &a.dy, &a.y}) {
+      if (!v->p) continue;
+      if ((along_rows ? v->rs : v->cs) != 1 || (along_rows ? v->cs : v->rs) % n || (uintptr_t)v->p % (n * sizeof(T))) return false;
+    }
+    return along_rows || (a.K % n == 0 && (uintptr_t)a.w % (n * sizeof(T)) == 0 && (uintptr_t)a.b % (n * sizeof(T)) == 0);
+  };
+  if (image) {
+    constexpr int VP = 4 / (int)sizeof(T);
+    if (!backward) {
+      if (a.K <= 128 && wide(VEC, true)) image_tiles<T, VEC, 8, false, false>(c);
+      else if (a.K <= 512 && wide(VP, true)) image_tiles<T, VP, 32, false, false>(c);
+      else if (a.K <= 512) image_tiles<T, 1, 32, false, false>(c);
+      else if (wide(VP, true)) image_tiles<T, VP, 32, true, false>(c);
+      else image_tiles<T, 1, 32, true, false>(c);
+      return;
+    }
+    if (a.K <= 64 && wide(VEC, true)) image_tiles<T, VEC, 4, false, true>(c);
+    else if (a.K <= 256 && wide(VP, true)) image_tiles<T, VP, 16, false, true>(c);
+    else if (a.K <= 256) image_tiles<T, 1, 16, false, true>(c);
+    else {
+      if (a.y.p) {
+        if (wide(VP, true)) image_tiles<T, VP, 16, true, true>(c);
+        else image_tiles<T, 1, 16, true, true>(c);
+      }
+      c.columns<T>(true);
+    }
+    return;
+  }
+  const int64_t n = a.K / VEC;
+  if (wide(VEC, false)) {
+    if (!backward) {
+      if (rows_lanes<T, VEC, 1, 4, false>(c, n) || rows_lanes<T, VEC, 2, 2, false>(c, n) || rows_lanes<T, VEC, 4, 1, false>(c, n) ||
+          rows_block<T, VEC, 2, false>(c, n) || rows_block<T, VEC, 4, false>(c, n))
+        return;
+    } else {  // sums of 16 columns a lane at most, in registers
+      if (rows_lanes<T, VEC, 1, 2, true>(c, n) || rows_lanes<T, VEC, 2, 1, true>(c, n)) return;
+      if constexpr (sizeof(T) == 4) {
+        if (rows_lanes<T, VEC, 4, 1, true>(c, n) || rows_block<T, VEC, 4, true>(c, n)) return;
+      } else {
+        if (rows_block<T, VEC, 2, true>(c, n)) return;
+      }
+    }
+  } else if (!backward) {
+    if (rows_lanes<T, 1, 1, 4, false>(c, a.K) || rows_lanes<T, 1, 4, 1, false>(c, a.K) || rows_lanes<T, 1, 16, 1, false>(c, a.K) ||
+        rows_block<T, 1, 8, false>(c, a.K) || rows_block<T, 1, 16, false>(c, a.K))
+      return;
+  } else {
+    if (rows_lanes<T, 1, 1, 2, true>(c, a.K) || rows_lanes<T, 1, 4, 1, true>(c, a.K) || rows_lanes<T, 1, 16, 1, true>(c, a.K) ||
+        rows_block<T, 1, 8, true>(c, a.K) || rows_block<T, 1, 16, true>(c, a.K))
+      return;
+  }
+  c.run_long<T>(backward, image);
+}
+
+}  // namespace
+
+int norm_pieces(int dtype, const NormArgs& a, int sms) {
+  Call c{a, sms, nullptr, true};
+  if (dtype == VI_F32) norm_call<float>(c, true);
+  else if (dtype == VI_F16) norm_call<__half>(c, true);
+  else norm_call<__nv_bfloat16>(c, true);
+  return c.pieces;
+}
+
+cudaError_t launch_norm(int dtype, const NormArgs& a, bool backward, int sms, cudaStream_t s, int* launches) {
+  Call c{a, sms, s, false};
+  if (dtype == VI_F32) norm_call<float>(c, backward);
+  else if (dtype == VI_F16) norm_call<__half>(c, backward);
+  else norm_call<__nv_bfloat16>(c, backward);
+  *launches += c.launches;
+  return c.rc;
+}
+
+}  // namespace heads
+}  // namespace vi
