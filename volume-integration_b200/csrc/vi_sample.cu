@@ -6,13 +6,18 @@
 // threshold, or equal to it and among the first few that are".  The answer is the first index, in index order, at
 // which the running sum of the kept w exceeds u times their sum.
 //
-// The answer is a whole number that a border decides, so weights and sums are 64 bits wide: of 65536 candidates in
-// float32 (1e-7 a weight) one draw in a hundred would fall on the wrong side.  Sums of weights are added in a fixed order, or as whole
-// numbers of a unit (2^-46 of the largest up to V = 65536), so the same call gives the same label.
+// The answer is a whole number that a border decides.  Weights and sums in 64 bits decide it; where no top-k or
+// top-p is asked for, float32 does, with a bound on its error, and a row whose draw falls within that bound of
+// a border is done again in 64 bits (150 labels: one row in a thousand).  Sums are added in a fixed order: the same
+// call gives the same labels.
 //
-// The threshold is found without sorting: the logits' bits, made to order as unsigned integers, are narrowed by 8 bits
-// at a time through histograms of counts (top-k) or masses (top-p).
+// The threshold is found without sorting, by bisection over the logits' bits, made to order as unsigned integers:
+// of rows that the registers hold (up to 8192 labels), or of a longer row's candidates.  Those are the labels above a
+// guess, made from a sample of the row: one pass over the row keeps them, and shows (by their number, or their share
+// of the mass) that no other label can be kept.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "vi_heads.h"
 #include "vi_heads_math.cuh"
@@ -22,16 +27,50 @@ namespace vi {
 namespace heads {
 namespace {
 
-// Bits that order as the value does; -0 as 0.
-__device__ __forceinline__ uint32_t order_of(float z) {
-  const uint32_t b = __float_as_uint(z + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+constexpr uint32_t kAll = 0xffffffffu;
+constexpr uint32_t kManyTies = 0x7fffffffu;
+
+// Bits that order as the value does; -0 as 0.  A 16-bit type's values, as floats, have low bits that are all alike: they
+// are left out, which saves as many steps of a bisection.
+template <typename T>
+struct Order {
+  static constexpr int kShift = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16, kBits = 32 - kShift;
+  static __device__ __forceinline__ uint32_t of(float z) {
+    const uint32_t b = __float_as_uint(z + 0.0f);
+    return (b & 0x80000000u ? ~b : b | 0x80000000u) >> kShift;
+  }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    return __uint_as_float(k >> (kBits - 1) ? k << kShift & 0x7fffffffu : ~(k << kShift | ((1u << kShift) - 1)));
+  }
+};
+
+// 2^x for x <= 0, to 1e-14 of it (0 below 2^-1000): 2^x = 2^k e^(f ln 2) with k whole and |f| <= 1/2, by the
+// exponential's series to the 12th power.
+__device__ __forceinline__ double pow2_64(double x) {
+  constexpr double l = 0.693147180559945309417232121458;
+  constexpr double c[13] = {1.0,
+                            l,
+                            l * l / 2,
+                            l * l * l / 6,
+                            l * l * l * l / 24,
+                            l * l * l * l * l / 120,
+                            l * l * l * l * l * l / 720,
+                            l * l * l * l * l * l * l / 5040,
+                            l * l * l * l * l * l * l * l / 40320,
+                            l * l * l * l * l * l * l * l * l / 362880,
+                            l * l * l * l * l * l * l * l * l * l / 3628800,
+                            l * l * l * l * l * l * l * l * l * l * l / 39916800,
+                            l * l * l * l * l * l * l * l * l * l * l * l / 479001600};
+  const double y = fmax(x, -1000.0), m = y + 0x1.8p52, f = y - (m - 0x1.8p52);
+  double p = c[12];
+#pragma unroll
+  for (int i = 11; i >= 0; i--) p = fma(p, f, c[i]);
+  return x < -1000.0 ? 0.0 : __hiloint2double(__double2hiint(p) + (__double2loint(m) << 20), __double2loint(p));
 }
-__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 // A row's settings.
 struct Setting {
-  double t, p, m;
+  double t, p, m, u;
   int64_t k;
 };
 __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int64_t row) {
@@ -40,222 +79,1148 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int64_t row) 
   s.p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
   s.m = a.min_p ? (double)a.min_p[row] : a.min_p_all;
   s.k = a.top_k ? a.top_k[row] : a.top_k_all;
+  s.u = a.u[row];
   return s;
 }
+constexpr double kLog2e64 = 1.44269504088896340735992468100;
+struct Weight {
+  float best;
+  double scale;  // log2(e) / T
+  __device__ __forceinline__ Weight(float best, double t) : best(best), scale(kLog2e64 / t) {}
+  __device__ __forceinline__ double of(float z) const {
+    return z == best ? 1.0 : z == -INFINITY ? 0.0 : pow2_64(((double)z - (double)best) * scale);
+  }
+};
 
-constexpr int kThreads = 512;
+// ---- a team of warps that holds a row, or a row's candidates ----
+struct TeamShared {
+  double d[2][16];
+  uint32_t u[2][16];
+};
+template <int WARPS>
+struct Team {
+  TeamShared& sh;
+  int warp, lane, turn = 0;  // two buffers in turn: a barrier each exchange
+  __device__ __forceinline__ void sync() const {
+    if constexpr (WARPS > 1) __syncthreads();
+  }
+  __device__ __forceinline__ uint32_t sum(uint32_t v) {
+    v = __reduce_add_sync(kAll, v);
+    if constexpr (WARPS > 1) {
+      if (lane == 0) sh.u[turn][warp] = v;
+      __syncthreads();
+      v = lane < WARPS ? sh.u[turn][lane] : 0;
+      v = __reduce_add_sync(kAll, v);
+      turn ^= 1;
+    }
+    return v;
+  }
+  __device__ __forceinline__ uint32_t most(uint32_t v) {
+    v = __reduce_max_sync(kAll, v);
+    if constexpr (WARPS > 1) {
+      if (lane == 0) sh.u[turn][warp] = v;
+      __syncthreads();
+      v = lane < WARPS ? sh.u[turn][lane] : 0;
+      v = __reduce_max_sync(kAll, v);
+      turn ^= 1;
+    }
+    return v;
+  }
+  __device__ __forceinline__ double sum(double v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    if constexpr (WARPS > 1) {
+      if (lane == 0) sh.d[turn][warp] = v;
+      __syncthreads();
+      v = lane < WARPS ? sh.d[turn][lane] : 0.0;
+#pragma unroll
+      for (int o = WARPS / 2; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+      v = __shfl_sync(kAll, v, 0);
+      turn ^= 1;
+    }
+    return v;
+  }
+  // what the warps in front of this one hold, and all
+  __device__ __forceinline__ void ahead(uint32_t v, uint32_t& before) {
+    before = 0;
+    if constexpr (WARPS > 1) {
+      if (lane == 0) sh.u[turn][warp] = v;
+      __syncthreads();
+      for (int i = 0; i < warp; i++) before += sh.u[turn][i];
+      turn ^= 1;
+    }
+  }
+  __device__ __forceinline__ void ahead(double v, double& before, double& all) {
+    before = 0.0;
+    all = v;
+    if constexpr (WARPS > 1) {
+      if (lane == 0) sh.d[turn][warp] = v;
+      __syncthreads();
+      all = 0.0;
+      for (int i = 0; i < WARPS; i++) {
+        if (i == warp) before = all;
+        all += sh.d[turn][i];
+      }
+      turn ^= 1;
+    }
+  }
+};
 
-struct Shared {
-  double d[kThreads / 32];
-  uint32_t u[kThreads / 32];
-  unsigned long long mass[256];
-  uint32_t count[256];
-  uint32_t key, ties;
-  unsigned long long above;
+constexpr int kUnsure = -2;
+
+// The draw among held values, by the definition, in 64 bits.  A lane's value e stands for place (warp * E + e) * 32 + lane,
+// which is index order.  `best` is the largest and finite or +inf; empty places hold -inf.  all: the mass that top-p's share is
+// of, if it is known to `slack` (mass that is not held counts), else negative.  Returns the place; kUnsure where
+// another mass within the slack would move the threshold, or where more than is held is asked for.
+template <typename T, int E, int WARPS>
+__device__ __forceinline__ int draw(Team<WARPS>& team, const float (&z)[E], float best, const Setting& s, int64_t labels,
+                                    double all = -1.0, double slack = 0.0) {
+  using O = Order<T>;
+  const Weight weight(best, s.t);
+  const bool greedy = !(s.t > 0.0);
+  const int lane = team.lane;
+  // kept: order above `low`, and the first `ties` of those equal to it
+  uint32_t low = greedy ? O::of(best) : 0, ties = greedy ? 1 : kManyTies;
+  // bisections begin at the first bit in which what is held differs
+  uint32_t least = kAll;
+  if (!greedy && (s.p < 1.0 || (s.k > 0 && s.k < labels))) {
+#pragma unroll
+    for (int e = 0; e < E; e++) least = z[e] > -INFINITY ? min(least, O::of(z[e])) : least;
+    least = ~team.most(~least);
+  }
+  const uint32_t differ = least ^ O::of(best);
+  const int start = differ ? 31 - __clz(differ) : -1;
+  const uint32_t common = start < 0 ? least : least >> start >> 1 << start << 1;
+  if (!greedy && s.k > 0 && s.k < labels) {
+    low = common;
+#pragma unroll 1
+    for (int bit = start; bit >= 0; bit--) {
+      const uint32_t c = low | 1u << bit;
+      uint32_t n = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) n += O::of(z[e]) >= c;
+      if (team.sum(n) >= s.k) low = c;
+    }
+    uint32_t n = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) n += O::of(z[e]) > low;
+    ties = (uint32_t)(s.k - team.sum(n));
+  }
+  double w[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) w[e] = greedy ? (z[e] == best ? 1.0 : 0.0) : weight.of(z[e]);
+  if (!greedy && s.p < 1.0) {
+    const auto mass = [&](uint32_t from) {  // of what is above low, from `from` on
+      double v = 0.0;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const uint32_t o = O::of(z[e]);
+        v += o >= from && o > low ? w[e] : 0.0;
+      }
+      return team.sum(v);
+    };
+    uint32_t n = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) n += O::of(z[e]) == low;
+    n = min(team.sum(n), ties);
+    const double at_low = n ? n * (low ? weight.of(O::value(low)) : 0.0) : 0.0;
+    const bool all_known = all >= 0.0;
+    if (!all_known) all = mass(0) + at_low;
+    const double want = fmax(s.p * all, 1e-300);
+    slack *= s.p;
+    if (all_known && !(mass(0) + at_low - want > slack)) return kUnsure;
+    uint32_t cut = common;
+#pragma unroll 1
+    for (int bit = start; bit >= 0; bit--) {
+      const uint32_t c = cut | 1u << bit;
+      if (c <= low || mass(c) >= want) cut = c;
+    }
+    cut = max(cut, low);
+    const double above = mass(cut + 1), one = cut ? weight.of(O::value(cut)) : 0.0;
+    uint32_t have = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) have += O::of(z[e]) == cut;
+    have = team.sum(have);
+    if (cut == low) have = min(have, ties);
+    const double need = one > 0.0 ? ceil((want - above) / one) : (double)have;
+    ties = (uint32_t)fmin(fmax(need, 1.0), (double)have);
+    low = cut;
+    if (slack > 0.0 && !(want - above - (ties - 1.0) * one > slack && above + ties * one - want > slack)) return kUnsure;
+  }
+  // kept weights; those equal to low by their number in index order
+  uint32_t equal = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) equal += __popc(__ballot_sync(kAll, O::of(z[e]) == low));
+  uint32_t seen;
+  team.ahead(equal, seen);
+  double mine = 0.0, run[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const uint32_t o = O::of(z[e]), b = __ballot_sync(kAll, o == low);
+    const bool in = o > low || (o == low && seen + __popc(b & ((1u << lane) - 1)) < ties);
+    seen += __popc(b);
+    w[e] = in && (!(w[e] < s.m) || z[e] == best) ? w[e] : 0.0;
+    double v = w[e];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double t = __shfl_up_sync(kAll, v, d);
+      if (lane >= d) v += t;
+    }
+    run[e] = mine + v;
+    mine += __shfl_sync(kAll, v, 31);
+  }
+  double before, total;
+  team.ahead(mine, before, total);
+  const double want = s.u * total;
+  uint32_t hit = 0, last = 0;  // 0: none; the first hit as its complement
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const uint32_t at = (team.warp * E + e) * 32 + lane;
+    if (w[e] > 0.0) last = max(last, at + 1);
+    if (w[e] > 0.0 && before + run[e] > want) hit = max(hit, ~at);
+  }
+  hit = team.most(hit);
+  if (hit) return (int)~hit;
+  return (int)team.most(last) - 1;  // u of 1 and more
+}
+
+// The same where neither top-k nor top-p is asked for, in float32; -1 where the draw, or a label at min_p, is within the error of
+// a border.  Sums of chains of E + 5 additions and of the warps.
+template <int E, int WARPS>
+__device__ __forceinline__ int draw_fast(Team<WARPS>& team, const float (&z)[E], float best, const Setting& s, float margin) {
+  const float scale = (float)(kLog2e64 / s.t), least = (float)s.m;
+  const int lane = team.lane;
+  float run[E], w[E], mine = 0.0f;
+  uint32_t doubt = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const float x = z[e] == best ? 1.0f : exp2_fast((z[e] - best) * scale);
+    doubt |= fabsf(x - least) <= 3e-5f * least && s.m > 0.0 && z[e] != best;
+    w[e] = !(x < least) || z[e] == best ? x : 0.0f;
+    float v = w[e];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const float t = __shfl_up_sync(kAll, v, d);
+      if (lane >= d) v += t;
+    }
+    run[e] = mine + v;
+    mine += __shfl_sync(kAll, v, 31);
+  }
+  double before, total;
+  team.ahead((double)mine, before, total);
+  const double want = s.u * total, slack = total * margin;
+  uint32_t hit = 0;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const double r = before + (double)run[e];
+    const uint32_t at = (team.warp * E + e) * 32 + lane;
+    // a sum that ends near the border from either side: the label before it, or behind it, may be the answer
+    doubt |= w[e] > 0.0f && fabs(r - want) <= slack;
+    if (w[e] > 0.0f && r > want) hit = max(hit, ~at);
+  }
+  doubt |= !(want > slack) || !(total - want > slack);
+  if constexpr (WARPS > 1) doubt = __syncthreads_or(doubt);
+  else doubt = __any_sync(kAll, doubt);
+  hit = team.most(hit);
+  return doubt || !hit ? -1 : (int)~hit;
+}
+
+// Whether float32's weights serve: its reach, and no inf - inf.
+__device__ __forceinline__ bool plain_scale(const Setting& s, float best) {
+  return s.t > 1e-30 && s.t < 1e30 && fabsf(best) < 1e37f;
+}
+
+// Loads a row into registers and draws.
+template <typename T, int E, int WARPS>
+__device__ __forceinline__ int64_t row_label(Team<WARPS>& team, const SampleArgs& a, int64_t row, float margin) {
+  using O = Order<T>;
+  const T* p = (const T*)a.z.p + row * a.z.rs;
+  float z[E];
+  uint32_t top = 0;
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int v = (team.warp * E + e) * 32 + team.lane;
+    z[e] = v < a.V ? to_f(p[v * a.z.cs]) : -INFINITY;
+  }
+  const Setting s = setting_of(a, row);
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    nan |= z[e] != z[e];
+    top = max(top, O::of(z[e]));
+  }
+  top = team.most(nan || s.t != s.t ? kAll : top);  // no value's order is kAll
+  if (top == kAll) return -1;
+  const float best = O::value(top);
+  if (best == -INFINITY) return -1;
+  if (margin > 0.0f && !(s.k > 0 && s.k < a.V) && !(s.p < 1.0) && plain_scale(s, best)) {
+    const int v = draw_fast<E, WARPS>(team, z, best, s, margin);
+    if (v >= 0) return v;
+  }
+  return draw<T, E, WARPS>(team, z, best, s, a.V);
+}
+
+// Rows of up to 32 E WARPS labels: WARPS warps a row.
+template <typename T, int E, int WARPS>
+__global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS) sample_rows_kernel(const __grid_constant__ SampleArgs a) {
+  __shared__ TeamShared sh;
+  Team<WARPS> team{sh, WARPS == 1 ? 0 : (int)threadIdx.x / 32, (int)threadIdx.x % 32};
+  const int teams = WARPS == 1 ? 8 : 1;
+  for (int64_t row = (int64_t)blockIdx.x * teams + (WARPS == 1 ? threadIdx.x / 32 : 0); row < a.M; row += (int64_t)gridDim.x * teams) {
+    const int64_t v = row_label<T, E, WARPS>(team, a, row, a.margin);
+    if (team.lane == 0 && team.warp == 0) a.label[row] = v;
+    team.sync();
+  }
+}
+
+// ---- images: neighbouring rows lie next to each other ----
+// A thread a pixel, or two of 16-bit logits, where neither top-k nor top-p is asked for: no exchange between lanes.  The first pass
+// finds the largest, the second the sums of 16 pieces of the row, the third walks through the piece that holds the draw.
+// The first reads memory, the others mostly the caches.
+constexpr int kPieces = 16, kImageThreads = 128;
+// A row by a warp in 64 bits, without top-k, top-p and temperature 0: 32 labels at a time, once for the sum and once for the draw.
+template <typename T>
+__device__ __noinline__ int64_t image_row_again(const SampleArgs& a, int64_t row) {
+  const T* p = (const T*)a.z.p + row * a.z.rs;
+  const int lane = threadIdx.x % 32;
+  const Setting s = setting_of(a, row);
+  float best = -INFINITY;
+  for (int v = lane; v < a.V; v += 32) best = fmaxf(best, to_f(p[v * a.z.cs]));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(kAll, best, o));
+  const Weight weight(best, s.t);
+  double run = 0.0, want = 0.0;
+  int last = -1;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; pass++) {
+    if (pass) want = s.u * run;
+    run = 0.0;
+    for (int first = 0; first < a.V; first += 32) {
+      const float z = first + lane < a.V ? to_f(p[(first + lane) * a.z.cs]) : -INFINITY;
+      double w = weight.of(z);
+      if (w < s.m && z != best) w = 0.0;
+      double scan = w;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double t = __shfl_up_sync(kAll, scan, d);
+        if (lane >= d) scan += t;
+      }
+      const uint32_t kept = __ballot_sync(kAll, w > 0.0), hit = __ballot_sync(kAll, pass && w > 0.0 && run + scan > want);
+      if (hit) return first + __ffs(hit) - 1;
+      if (kept) last = first + 31 - __clz(kept);
+      run += __shfl_sync(kAll, scan, 31);
+    }
+  }
+  return last;  // u of 1 and more
+}
+template <typename T, int PX>
+struct Pixels {
+  float v[PX];
+  __device__ __forceinline__ explicit Pixels(const T* p) {
+    if constexpr (PX == 1) {
+      v[0] = to_f(*p);
+    } else {
+      const uint32_t w = *(const uint32_t*)p;
+      const float2 f = std::is_same<T, __half>::value ? __half22float2(*(const __half2*)&w) : __bfloat1622float2(*(const __nv_bfloat162*)&w);
+      v[0] = f.x, v[1] = f.y;
+    }
+  }
+};
+template <typename T, int PX>
+__global__ void __launch_bounds__(kImageThreads) sample_image_kernel(const __grid_constant__ SampleArgs a) {
+  __shared__ float pieces[kPieces][PX][kImageThreads];
+  const int len = (a.V + kPieces - 1) / kPieces;
+  const int64_t step = (int64_t)gridDim.x * kImageThreads * PX;
+  for (int64_t base = (int64_t)blockIdx.x * kImageThreads * PX; base < a.M; base += step) {
+    const int64_t row = base + threadIdx.x * PX;
+    const bool here = row < a.M;
+    uint32_t again = 0;  // pixels that float32 does not decide
+    if (here) {
+      const T* p = (const T*)a.z.p + row * a.z.rs;
+      float best[PX], scale[PX], least[PX];
+      bool first[PX];  // temperature 0
+#pragma unroll
+      for (int j = 0; j < PX; j++) best[j] = -INFINITY;
+#pragma unroll 8
+      for (int v = 0; v < a.V; v++) {
+        const Pixels<T, PX> z(p + v * a.z.cs);
+#pragma unroll
+        for (int j = 0; j < PX; j++) best[j] = max_nan(best[j], z.v[j]);
+      }
+      Setting s[PX];
+      bool draws = false, firsts = false;
+#pragma unroll
+      for (int j = 0; j < PX; j++) {
+        s[j] = setting_of(a, row + j);
+        first[j] = !(s[j].t > 0.0) && s[j].t == s[j].t;
+        if (best[j] != best[j] || s[j].t != s[j].t || best[j] == -INFINITY) {
+          a.label[row + j] = -1;
+          s[j].u = -1.0;  // done
+        } else if (first[j]) {
+          firsts = true;
+        } else if (!plain_scale(s[j], best[j])) {
+          again |= 1u << j;
+          s[j].u = -1.0;
+        } else {
+          draws = true;
+        }
+        scale[j] = (float)(kLog2e64 / s[j].t);
+        least[j] = (float)s[j].m;
+      }
+      if (firsts) {
+        int at[PX];
+#pragma unroll
+        for (int j = 0; j < PX; j++) at[j] = a.V;
+#pragma unroll 8
+        for (int v = a.V - 1; v >= 0; v--) {
+          const Pixels<T, PX> z(p + v * a.z.cs);
+#pragma unroll
+          for (int j = 0; j < PX; j++) at[j] = z.v[j] == best[j] ? v : at[j];
+        }
+#pragma unroll
+        for (int j = 0; j < PX; j++)
+          if (first[j] && s[j].u >= 0.0) a.label[row + j] = at[j];
+      }
+      if (draws) {
+        float run[PX] = {};
+        bool doubt[PX] = {};
+        const auto weight = [&](float z, int j) {
+          const float x = exp2_fast((z - best[j]) * scale[j]);
+          doubt[j] |= fabsf(x - least[j]) < 3e-5f * least[j];
+          return x < least[j] ? 0.0f : x;
+        };
+        for (int c = 0; c < kPieces; c++) {
+          const int v1 = min(a.V, (c + 1) * len);
+          float sum[PX] = {};
+#pragma unroll 8
+          for (int v = c * len; v < v1; v++) {
+            const Pixels<T, PX> z(p + v * a.z.cs);
+#pragma unroll
+            for (int j = 0; j < PX; j++) sum[j] += weight(z.v[j], j);
+          }
+#pragma unroll
+          for (int j = 0; j < PX; j++) {
+            run[j] += sum[j];
+            pieces[c][j][threadIdx.x] = run[j];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < PX; j++) {
+          if (first[j] || s[j].u < 0.0) continue;
+          const float total = run[j], want = (float)s[j].u * total, slack = total * a.margin;
+          int c = 0;
+          while (c < kPieces - 1 && pieces[c][j][threadIdx.x] <= want) c++;
+          float r = c ? pieces[c - 1][j][threadIdx.x] : 0.0f, sum = 0.0f;
+          const float start = r;
+          int at = -1;
+          bool near = fabsf(r - want) <= slack;
+          for (int v = c * len; v < min(a.V, (c + 1) * len); v++) {
+            sum += weight(to_f(p[v * a.z.cs + j]), j);
+            r = start + sum;
+            near |= fabsf(r - want) <= slack;
+            if (at < 0 && r > want) at = v;
+          }
+          if (near || doubt[j] || at < 0 || !(s[j].u < 1.0)) again |= 1u << j;
+          else a.label[row + j] = at;
+        }
+      }
+    }
+    // what is left, a warp a row
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < PX; j++) {
+      uint32_t todo = __ballot_sync(kAll, again >> j & 1);
+      while (todo) {
+        const int l = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const int64_t r = __shfl_sync(kAll, row, l) + j, v = image_row_again<T>(a, r);
+        if (threadIdx.x % 32 == 0) a.label[r] = v;
+      }
+    }
+  }
+}
+
+// The same with the pixel's logits in registers (up to NV labels): memory is read once, with all of a thread's loads in flight.
+// The piece that holds the draw is picked out of them by comparisons.
+template <typename T, int PX, int NV>
+__global__ void __launch_bounds__(kImageThreads) sample_pixels_kernel(const __grid_constant__ SampleArgs a) {
+  constexpr int kLen = 16, kCount = NV / kLen;
+  using Word = typename std::conditional<PX == 2, uint32_t, float>::type;
+  const auto value = [](Word w, int j) -> float {
+    if constexpr (PX == 1) {
+      return w;
+    } else if constexpr (std::is_same<T, __half>::value) {
+      return __half2float(__ushort_as_half((unsigned short)(j ? w >> 16 : w & 0xffffu)));
+    } else {
+      return __uint_as_float(j ? w & 0xffff0000u : w << 16);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * kImageThreads * PX;
+  for (int64_t base = (int64_t)blockIdx.x * kImageThreads * PX; base < a.M; base += step) {
+    const int64_t row = base + threadIdx.x * PX;
+    uint32_t again = 0;  // pixels that float32 does not decide
+    if (row < a.M) {
+      const T* p = (const T*)a.z.p + row * a.z.rs;
+      Word z[NV];
+#pragma unroll
+      for (int v = 0; v < NV; v++) {
+        if constexpr (PX == 1) z[v] = v < a.V ? to_f(p[v * a.z.cs]) : -INFINITY;
+        else z[v] = v < a.V ? *(const uint32_t*)(p + v * a.z.cs) : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+      }
+      float best[PX];
+      if constexpr (PX == 1) {
+        best[0] = z[0];
+#pragma unroll
+        for (int v = 1; v < NV; v++) best[0] = max_nan(best[0], z[v]);
+      } else {
+        Word m = z[0];
+#pragma unroll
+        for (int v = 1; v < NV; v++) {
+          if constexpr (std::is_same<T, __half>::value) {
+            const __half2 r = __hmax2_nan(*(const __half2*)&m, *(const __half2*)&z[v]);
+            m = *(const Word*)&r;
+          } else {
+            const __nv_bfloat162 r = __hmax2_nan(*(const __nv_bfloat162*)&m, *(const __nv_bfloat162*)&z[v]);
+            m = *(const Word*)&r;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < PX; j++) best[j] = value(m, j);
+      }
+#pragma unroll
+      for (int j = 0; j < PX; j++) {
+        const Setting s = setting_of(a, row + j);
+        if (best[j] != best[j] || s.t != s.t || best[j] == -INFINITY) {
+          a.label[row + j] = -1;
+        } else if (!(s.t > 0.0)) {
+          int at = 0;
+#pragma unroll
+          for (int v = NV - 1; v >= 0; v--) at = value(z[v], j) == best[j] ? v : at;
+          a.label[row + j] = at;
+        } else if (!plain_scale(s, best[j])) {
+          again |= 1u << j;
+        } else {
+          const double scale64 = kLog2e64 / s.t;
+          const float scale = (float)scale64;
+          bool near = !(s.u < 1.0);
+          // min-p keeps the logits from a value on: the type's first value there
+          float least = -INFINITY;
+          if (s.m >= 1.0) {
+            least = best[j];
+          } else if (s.m > 0.0) {
+            const double at = (double)best[j] + log2(s.m) / scale64;
+            T up;
+            double round;
+            if constexpr (sizeof(T) == 4) up = __double2float_ru(at), round = (double)(float)at;
+            else if constexpr (std::is_same<T, __half>::value) up = __float2half_ru(__double2float_ru(at)), round = (double)__half2float(__double2half(at));
+            else up = __float2bfloat16_ru(__double2float_ru(at)), round = (double)__bfloat162float(__double2bfloat16(at));
+            least = to_f(up);
+            near |= fabs(round - at) <= 1e-12 * (fabs(at) + fabs((double)best[j]));
+          }
+          const auto weight = [&](Word w) {
+            const float x = value(w, j);
+            return x >= least ? exp2_fast((x - best[j]) * scale) : 0.0f;
+          };
+          float run[kCount], sum = 0.0f;
+#pragma unroll
+          for (int c = 0; c < kCount; c++) {
+            float q[2] = {0.0f, 0.0f};
+            if (c * kLen < a.V) {
+#pragma unroll
+              for (int i = 0; i < kLen; i++) q[i & 1] += weight(z[c * kLen + i]);
+            }
+            run[c] = sum += q[0] + q[1];
+          }
+          const float want = (float)s.u * sum, slack = sum * a.margin;
+          int c = 0;
+          float start = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kCount - 1; i++) {
+            const bool behind = run[i] <= want;
+            c += behind;
+            start = behind ? run[i] : start;
+          }
+          Word cell[kLen];
+#pragma unroll
+          for (int i = 0; i < kLen; i++) cell[i] = z[i];
+#pragma unroll
+          for (int k = 1; k < kCount; k++) {
+#pragma unroll
+            for (int i = 0; i < kLen; i++) cell[i] = c == k ? z[k * kLen + i] : cell[i];
+          }
+          near |= fabsf(start - want) <= slack;
+          int at = -1;
+          float r = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kLen; i++) {
+            r += weight(cell[i]);
+            near |= fabsf(start + r - want) <= slack;
+            at = at < 0 && start + r > want ? c * kLen + i : at;
+          }
+          if (near || at < 0) again |= 1u << j;
+          else a.label[row + j] = at;
+        }
+      }
+    }
+    // what is left, a warp a row
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < PX; j++) {
+      uint32_t todo = __ballot_sync(kAll, again >> j & 1);
+      while (todo) {
+        const int l = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const int64_t r = __shfl_sync(kAll, row, l) + j, v = image_row_again<T>(a, r);
+        if (threadIdx.x % 32 == 0) a.label[r] = v;
+      }
+    }
+  }
+}
+
+// ---- long rows: a block a row ----
+constexpr int kLongWarps = 8, kLongThreads = 256, kHeld = 16;
+constexpr int kListWarp = 32 * kHeld;          // candidates a warp keeps
+constexpr int kSample = 16;                    // labels a lane looks at for the guess
+constexpr int kSums = 64;                      // sums of steps a warp keeps
+constexpr int kBins = 256;
+constexpr int kFew = 256;                      // candidates that one warp draws from
+struct LongShared {
+  TeamShared team;
+  float z[kLongWarps][kListWarp];
+  int at[kLongWarps][kListWarp];
+  float sums[kLongWarps][kSums];
+  uint32_t bins[kBins];
+  float few_z[kFew];
+  int few_at[kFew];
+  float guess;
   int answer;
 };
 
-// A block a row, which it reads again for each step.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
-  __shared__ Shared sh;
-  const int tid = threadIdx.x;
-  for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-    const T* z = (const T*)a.z.p + row * a.z.rs;
-    const auto key_at = [&](int v) { return order_of(to_f(z[v * a.z.cs])); };
-    const Setting s = setting_of(a, row);
-    // the largest key; whether there is a NaN
-    uint32_t top = 0;
-    bool nan = false;
-    for (int v = tid; v < a.V; v += kThreads) {
-      const float x = to_f(z[v * a.z.cs]);
-      nan |= x != x;
-      top = max(top, order_of(x));
-    }
-    nan = __syncthreads_or(nan || s.t != s.t);
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (tid % 32 == 0) sh.u[tid / 32] = top;
-    __syncthreads();
-    for (int i = 0; i < kThreads / 32; i++) top = max(top, sh.u[i]);
-    const float best = value_of(top);
-    if (nan || best == -INFINITY) {
-      if (tid == 0) a.label[row] = -1;
-      __syncthreads();
-      continue;
-    }
-    const bool greedy = !(s.t > 0.0);
-    const auto weight = [&](uint32_t key) {
-      const double x = (double)value_of(key);
-      return key == top ? 1.0 : x == -INFINITY ? 0.0 : exp((x - (double)best) / s.t);
-    };
-
-    // kept: keys above `low`, and the first `ties` of those equal to it
-    uint32_t low = greedy ? top : 0;
-    uint32_t ties = greedy ? 1 : 0x7fffffff;
-    // narrowed from the front of the order: count (by_mass false) or mass in front of the last one kept
-    const auto narrow = [&](bool by_mass, uint64_t want) {
-      uint32_t prefix = 0;
-      uint64_t before = 0;  // in front of the keys that share the prefix
-      const uint32_t old_low = low, old_ties = ties;
-      uint32_t cut = 0;
-      for (int shift = 24; shift >= 0; shift -= 8) {
-        __syncthreads();
-        if (tid < 256) sh.mass[tid] = 0, sh.count[tid] = 0;
-        __syncthreads();
-        for (int v = tid; v < a.V; v += kThreads) {
-          const uint32_t k = key_at(v);
-          if (k < old_low || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
-          atomicAdd(&sh.count[k >> shift & 255], 1u);
-          if (by_mass && k != old_low) atomicAdd(&sh.mass[k >> shift & 255], (unsigned long long)rint(weight(k) * a.unit));
+// What a lane holds of 256 labels from `first` on: 8 in a row (VEC: loaded as vectors), or every 32nd.
+template <typename T, bool VEC>
+struct Step {
+  float z[8];
+  static __device__ __forceinline__ int place(int first, int lane, int e) { return VEC ? first + lane * 8 + e : first + e * 32 + lane; }
+  // ends at `end`; with VEC whole vectors lie on one side of it
+  __device__ __forceinline__ void load(const T* p, int64_t cs, int first, int lane, int end) {
+    if constexpr (VEC) {
+      constexpr int per = 16 / (int)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < 8; i += per) {
+        const int v = first + lane * 8 + i;
+        if (v < end) {
+          const uint4 q = *(const uint4*)(p + v);
+#pragma unroll
+          for (int j = 0; j < per; j++) z[i + j] = to_f(((const T*)&q)[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < per; j++) z[i + j] = -INFINITY;
         }
-        __syncthreads();
-        if (tid == 0) {
-          uint64_t sum = before;
-          int bin = 255;
-          for (;; bin--) {
-            uint64_t here = sh.count[bin];
-            if (by_mass) {
-              here = sh.mass[bin];
-              // the last step's keys are told apart; of those at the old threshold only some are left
-              if (old_low && old_low >> shift == ((shift < 24 ? prefix << 8 : 0) | (uint32_t)bin) && sh.count[bin])
-                here += min(old_ties, sh.count[bin]) * (uint64_t)rint(weight(old_low) * a.unit);
-            }
-            if (bin == 0 || sum + here >= want) break;
-            sum += here;
-          }
-          sh.key = bin;
-          sh.ties = sh.count[bin];
-          sh.above = sum;
-        }
-        __syncthreads();
-        prefix = (shift < 24 ? prefix << 8 : 0) | sh.key;
-        before = sh.above;
-        cut = sh.ties;
       }
-      low = prefix;
-      uint64_t n = want - before;  // how many, or how much, of the keys equal to it
-      if (by_mass) {
-        const uint64_t one = (uint64_t)rint(weight(low) * a.unit);
-        n = one ? (n + one - 1) / one : cut;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int v = first + e * 32 + lane;
+        z[e] = v < end ? to_f(p[v * cs]) : -INFINITY;
       }
-      ties = (uint32_t)min(n, (uint64_t)cut);
-      if (low == old_low) ties = min(ties, old_ties);
-    };
-    if (!greedy && s.k > 0 && s.k < a.V) narrow(false, s.k);
-    if (!greedy && s.p < 1.0) {
-      unsigned long long part = 0;
-      uint32_t equal = 0;
-      for (int v = tid; v < a.V; v += kThreads) {
-        const uint32_t k = key_at(v);
-        if (k > low) part += (unsigned long long)rint(weight(k) * a.unit);
-        equal += k == low;
-      }
-      __syncthreads();
-      if (tid == 0) sh.mass[0] = 0, sh.count[0] = 0;
-      __syncthreads();
-      atomicAdd(&sh.mass[0], part);
-      atomicAdd(&sh.count[0], equal);
-      __syncthreads();
-      const uint64_t all = sh.mass[0] + min(ties, sh.count[0]) * (uint64_t)rint(weight(low) * a.unit);
-      narrow(true, max((uint64_t)1, (uint64_t)ceil(fmax(s.p, 0.0) * (double)all)));
     }
-    if (!greedy && s.m > 0.0 && low < top) {
-      // the threshold rises to the lowest key whose weight is enough, if that is above it
-      uint32_t least = 0xffffffffu;
-      for (int v = tid; v < a.V; v += kThreads) {
-        const uint32_t k = key_at(v);
-        if (k >= low && (k == top || weight(k) >= s.m)) least = min(least, k);
-      }
-      least = __reduce_min_sync(0xffffffffu, least);
-      __syncthreads();
-      if (tid % 32 == 0) sh.u[tid / 32] = least;
-      __syncthreads();
-      for (int i = 0; i < kThreads / 32; i++) least = min(least, sh.u[i]);
-      if (least > low) low = least, ties = 0x7fffffff;
-    }
+  }
+};
 
-    // kept mass in index order: a piece of the row a thread, then the piece that holds the draw
-    const int per = (a.V + kThreads - 1) / kThreads, v0 = min(a.V, tid * per), v1 = min(a.V, v0 + per);
-    const double w_low = weight(low);
-    uint32_t equal = 0;
-    for (int v = v0; v < v1; v++) equal += key_at(v) == low;
-    // equal ones in front of this thread's piece
-    uint32_t scan = equal;
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t n = __shfl_up_sync(0xffffffffu, scan, o);
-      if (tid % 32 >= o) scan += n;
+// f of every label of a row, in any order: several loads in flight.
+template <typename T, bool VEC, typename F>
+__device__ __forceinline__ void each_of_row(const T* p, int64_t cs, int V, int warp, int lane, F f) {
+  constexpr int kDeep = 4;
+  for (int first = warp * 256; first < V; first += kDeep * kLongThreads * 8) {
+    Step<T, VEC> x[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; i++) x[i].load(p, cs, first + i * kLongThreads * 8, lane, V);
+#pragma unroll
+    for (int i = 0; i < kDeep; i++) {
+      if (first + i * kLongThreads * 8 >= V) continue;
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (Step<T, VEC>::place(first + i * kLongThreads * 8, lane, e) < V) f(x[i].z[e]);
     }
-    __syncthreads();
-    if (tid % 32 == 31) sh.u[tid / 32] = scan;
-    __syncthreads();
-    uint32_t ahead = scan - equal;
-    for (int i = 0; i < tid / 32; i++) ahead += sh.u[i];
-    double mine = 0.0;
-    uint32_t seen = ahead;
-    for (int v = v0; v < v1; v++) {
-      const uint32_t k = key_at(v);
-      if (k > low) mine += weight(k);
-      else if (k == low && seen++ < ties) mine += w_low;
+  }
+}
+
+// The whole row by the definition in 64 bits, read again for every step of the bisections: where the guess was
+// wrong, or candidates are too many to be held.
+template <typename T, bool VEC>
+__device__ __noinline__ int whole_row(Team<kLongWarps>& team, LongShared& sh, const SampleArgs& a, const T* p, float best, const Setting& s) {
+  using O = Order<T>;
+  const Weight weight(best, s.t);
+  const int tid = threadIdx.x, V = a.V;
+  const int64_t cs = a.z.cs;
+  const bool greedy = !(s.t > 0.0);
+  uint32_t low = greedy ? O::of(best) : 0, ties = greedy ? 1 : kManyTies;
+  const auto each = [&](auto f) {
+    each_of_row<T, VEC>(p, cs, V, tid / 32, tid % 32, f);
+  };
+  const auto count = [&](auto f) {
+    uint32_t n = 0;
+    each([&](float z) { n += f(O::of(z)); });
+    return team.sum(n);
+  };
+  const auto mass = [&](uint32_t from, uint32_t to) {  // orders in [from, to)
+    double m = 0.0;
+    each([&](float z) {
+      const uint32_t o = O::of(z);
+      if (o >= from && o < to) m += weight.of(z);
+    });
+    return team.sum(m);
+  };
+  const uint32_t end = O::of(best) + 1;
+  if (!greedy && s.k > 0 && s.k < V) {
+    for (int bit = O::kBits - 1; bit >= 0; bit--) {
+      const uint32_t c = low | 1u << bit;
+      if (count([&](uint32_t o) { return o >= c; }) >= s.k) low = c;
     }
-    double sum = mine;
-    for (int o = 1; o < 32; o <<= 1) {
-      const double n = __shfl_up_sync(0xffffffffu, sum, o);
-      if (tid % 32 >= o) sum += n;
+    ties = (uint32_t)(s.k - count([&](uint32_t o) { return o > low; }));
+  }
+  if (!greedy && s.p < 1.0) {
+    const uint32_t n = min(count([&](uint32_t o) { return o == low; }), ties);
+    const double at_low = n ? n * weight.of(O::value(low)) : 0.0;
+    const double want = fmax(s.p * (mass(low + 1, end) + at_low), 1e-300);
+    uint32_t cut = 0, top = end;
+    double above = 0.0;  // mass from `top` on; the threshold lies under it
+    for (int bit = O::kBits - 1; bit >= 0; bit--) {
+      const uint32_t c = cut | 1u << bit;
+      if (c >= top) continue;
+      if (c <= low) {
+        cut = c;
+        continue;
+      }
+      const double m = above + mass(c, top);
+      if (m >= want) cut = c;
+      else above = m, top = c;
     }
-    __syncthreads();
-    if (tid % 32 == 31) sh.d[tid / 32] = sum;
-    if (tid == 0) sh.answer = 0x7fffffff;
-    __syncthreads();
-    double front = 0.0, total = 0.0;
-    for (int i = 0; i < kThreads / 32; i++) {
-      if (i == tid / 32) front = total;
-      total += sh.d[i];
+    cut = max(cut, low);
+    above += mass(cut + 1, top);
+    uint32_t have = count([&](uint32_t o) { return o == cut; });
+    if (cut == low) have = min(have, ties);
+    const double one = cut ? weight.of(O::value(cut)) : 0.0, need = one > 0.0 ? ceil((want - above) / one) : (double)have;
+    ties = (uint32_t)fmin(fmax(need, 1.0), (double)have);
+    low = cut;
+  }
+  // in index order: a warp a part of the row, step by step, once for the sum and once for the draw
+  const int part = (V + kLongWarps * 256 - 1) / (kLongWarps * 256) * 256, v0 = min(V, team.warp * part), v1 = min(V, v0 + part);
+  uint32_t equal = 0;
+  Step<T, VEC> x;
+  for (int first = v0; first < v1; first += 256) {
+    x.load(p, cs, first, team.lane, v1);
+#pragma unroll
+    for (int e = 0; e < 8; e++) equal += O::of(x.z[e]) == low;
+  }
+  uint32_t ahead;
+  team.ahead(__reduce_add_sync(kAll, equal), ahead);
+  // the lanes' running sums of a step's kept weights (r, from `run` on; the step's end in run), with each label's weight
+  const auto walk = [&](int first, uint32_t& seen, double& run, double (&r)[8], double (&w)[8]) {
+    x.load(p, cs, first, team.lane, v1);
+    const auto kept = [&](float z, uint32_t rank) {
+      const uint32_t o = O::of(z);
+      if (!(o > low || (o == low && rank < ties))) return 0.0;
+      const double q = weight.of(z);
+      return greedy || !(q < s.m) || z == best ? q : 0.0;
+    };
+    if constexpr (VEC) {
+      uint32_t n = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) n += O::of(x.z[e]) == low;
+      uint32_t rank = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t t = __shfl_up_sync(kAll, rank, d);
+        if (team.lane >= d) rank += t;
+      }
+      const uint32_t all = __shfl_sync(kAll, rank, 31);
+      rank += seen - n;
+      seen += all;
+      double sum = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        w[e] = kept(x.z[e], rank);
+        rank += O::of(x.z[e]) == low;
+        r[e] = sum += w[e];
+      }
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double t = __shfl_up_sync(kAll, sum, d);
+        if (team.lane >= d) sum += t;
+      }
+      const double front = __shfl_up_sync(kAll, sum, 1);
+#pragma unroll
+      for (int e = 0; e < 8; e++) r[e] += run + (team.lane ? front : 0.0);
+      run += __shfl_sync(kAll, sum, 31);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const uint32_t b = __ballot_sync(kAll, O::of(x.z[e]) == low);
+        w[e] = kept(x.z[e], seen + __popc(b & ((1u << team.lane) - 1)));
+        seen += __popc(b);
+        double sum = w[e];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const double t = __shfl_up_sync(kAll, sum, d);
+          if (team.lane >= d) sum += t;
+        }
+        r[e] = run + sum;
+        run += __shfl_sync(kAll, sum, 31);
+      }
     }
-    front += sum - mine;
-    const double want = (double)a.u[row] * total;
-    // the first index at which the running sum exceeds `want`; else (u >= 1) the last one kept
-    int last = -1, hit = 0x7fffffff;
-    double run = front;
+  };
+  double run = 0.0, r[8], w[8], before, total;
+  uint32_t seen = ahead;
+  for (int first = v0; first < v1; first += 256) walk(first, seen, run, r, w);
+  const double mine = run;
+  team.ahead(mine, before, total);
+  const double want = s.u * total;
+  uint32_t hit = 0, last = 0;
+  if (before + mine > want || !(total > want)) {
+    run = before;
     seen = ahead;
-    for (int v = v0; v < v1; v++) {
-      const uint32_t k = key_at(v);
-      const bool in = k > low || (k == low && seen++ < ties);
-      if (!in) continue;
-      const double w = k == low ? w_low : weight(k);
-      if (w > 0.0) last = v;
-      run += w;
-      if (run > want && w > 0.0) {
-        hit = v;
-        break;
+    for (int first = v0; first < v1 && !hit; first += 256) {
+      walk(first, seen, run, r, w);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const uint32_t v = Step<T, VEC>::place(first, team.lane, e);
+        if (w[e] > 0.0) last = max(last, v + 1);
+        if (w[e] > 0.0 && r[e] > want) hit = max(hit, ~v);
+      }
+      hit = __reduce_max_sync(kAll, hit);
+    }
+  }
+  hit = team.most(hit);
+  if (hit) return (int)~hit;
+  return (int)team.most(last) - 1;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __grid_constant__ SampleArgs a) {
+  using O = Order<T>;
+  __shared__ LongShared sh;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, V = a.V;
+  Team<kLongWarps> team{sh.team, warp, lane};
+  // a warp's part of the row: whole steps of 256
+  const int part = (V + kLongWarps * 256 - 1) / (kLongWarps * 256) * 256, v0 = min(V, warp * part), v1 = min(V, v0 + part);
+  const int steps = part / 256, group = (steps + kSums - 1) / kSums;
+  for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+    const T* p = (const T*)a.z.p + row * a.z.rs;
+    const Setting s = setting_of(a, row);
+    const bool greedy = !(s.t > 0.0), top_k = !greedy && s.k > 0 && s.k < V, top_p = !greedy && !top_k && s.p < 1.0;
+    const bool list = greedy || top_k || top_p || s.m > 0.0;
+    const float scale = (float)(kLog2e64 / s.t);
+
+    // the sample: two steps of each warp
+    float ref = -INFINITY, low = INFINITY, sample[kSample];
+    {
+      Step<T, VEC> x[kSample / 8];
+#pragma unroll
+      for (int i = 0; i < kSample / 8; i++) x[i].load(p, a.z.cs, v0 + i * (steps / 2) * 256, lane, v1);
+#pragma unroll
+      for (int i = 0; i < kSample; i++) {
+        sample[i] = x[i / 8].z[i % 8];
+        ref = fmaxf(ref, sample[i]);
+        if (sample[i] > -INFINITY) low = fminf(low, sample[i]);
       }
     }
-    if (hit != 0x7fffffff) atomicMin(&sh.answer, hit);
-    __syncthreads();
-    const bool none = sh.answer == 0x7fffffff;
-    __syncthreads();
-    if (none) {
-      if (tid == 0) sh.answer = -1;
-      __syncthreads();
-      atomicMax(&sh.answer, last);
-      __syncthreads();
+    ref = O::value(max(team.most(O::of(ref)), O::of(-INFINITY)));
+    const bool workable = plain_scale(s, ref) || (greedy && fabsf(ref) < INFINITY);
+
+    // one pass over the row, for sums of the weights beside 2^(ref scale), or for the labels from `guess` on
+    float best = -INFINITY;
+    bool nan = s.t != s.t;
+    int n = 0;
+    double sum = 0.0;
+    const auto pass = [&](auto wants_list, float guess) {
+      constexpr bool kList = decltype(wants_list)::value;
+      float group_sum = 0.0f;
+      Step<T, VEC> next;
+      next.load(p, a.z.cs, v0, lane, v1);
+      for (int i = 0; i < steps && v0 + i * 256 < v1; i++) {
+        const Step<T, VEC> x = next;
+        next.load(p, a.z.cs, v0 + (i + 1) * 256, lane, v1);
+        uint32_t in = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          nan |= x.z[e] != x.z[e];
+          best = fmaxf(best, x.z[e]);
+          in |= (uint32_t)(x.z[e] >= guess) << e;
+        }
+        if constexpr (!kList) {
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) w[e] = exp2_fast((x.z[e] - ref) * scale);
+          group_sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+          if (i % group == group - 1 || v0 + (i + 1) * 256 >= v1) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) group_sum += __shfl_xor_sync(kAll, group_sum, o);
+            if (lane == 0) sh.sums[warp][i / group] = group_sum;
+            sum += group_sum;
+            group_sum = 0.0f;
+          }
+        } else if (__any_sync(kAll, in)) {
+          if constexpr (VEC) {
+            const int mine = __popc(in);
+            int scan = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+              const int t = __shfl_up_sync(kAll, scan, d);
+              if (lane >= d) scan += t;
+            }
+            int to = n + scan - mine;
+            n += __shfl_sync(kAll, scan, 31);
+            if (n <= kListWarp) {
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (in >> e & 1) sh.z[warp][to] = x.z[e], sh.at[warp][to++] = Step<T, VEC>::place(v0 + i * 256, lane, e);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const uint32_t b = __ballot_sync(kAll, in >> e & 1);
+              const int to = n + __popc(b & ((1u << lane) - 1));
+              n += __popc(b);
+              if (n <= kListWarp && (in >> e & 1)) sh.z[warp][to] = x.z[e], sh.at[warp][to] = Step<T, VEC>::place(v0 + i * 256, lane, e);
+            }
+          }
+        }
+      }
+    };
+    double all = -1.0, slack = 0.0, before = 0.0;  // all: the row's mass, known to the slack
+    if (!workable) {                               // infinite, or nothing seen yet
+      each_of_row<T, VEC>(p, a.z.cs, V, warp, lane, [&](float z) {
+        nan |= z != z;
+        best = fmaxf(best, z);
+      });
+    } else if (!list || top_p) {
+      pass(std::false_type(), INFINITY);
+      team.ahead(sum, before, all);
+      slack = all * a.margin;
     }
-    if (tid == 0) a.label[row] = sh.answer;
+    if (workable && list) {
+      // the guess: from where on candidates are kept
+      float guess = ref;
+      if (top_k || top_p) {
+        low = -O::value(max(team.most(O::of(-low)), O::of(-INFINITY)));
+        const float range = top_k ? ref - low : fminf(ref - low, 40.0f / scale), width = range * (1.0f / kBins);
+        for (int i = threadIdx.x; i < kBins; i += kLongThreads) sh.bins[i] = 0;
+        __syncthreads();
+        const float to_bin = width > 0.0f ? 1.0f / width : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSample; i++)
+          if (sample[i] > -INFINITY) atomicAdd(&sh.bins[(int)fminf((ref - sample[i]) * to_bin, (float)(kBins - 1))], 1u);
+        __syncthreads();
+        if (warp == 0) {
+          const float share = (float)(kLongThreads * kSample) / (float)V;
+          // top-k: the rank in the sample that the row's k-th is hardly ever behind.  top-p: as much of the tail as leaves a
+          // quarter of what is not kept, beside the whole mass; the tail's small weights are sampled well
+          const float mean = (float)s.k * share, want = top_k ? mean + 4.0f * sqrtf(mean) + 2.0f : 0.75f * (1.0f - (float)fmax(s.p, 0.0)) * (float)all * share;
+          float c[8], mine = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int b = lane * 8 + i;
+            mine += c[i] = (float)sh.bins[b] * (top_k ? 1.0f : exp2_fast(-(b + 0.5f) * width * scale));
+          }
+          float run = mine;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const float t = __shfl_up_sync(kAll, run, d);
+            if (lane >= d) run += t;
+          }
+          const float total = __shfl_sync(kAll, run, 31);
+          run -= mine;
+          int bin = kBins;  // the first bin that, with those in front of it, is enough
+#pragma unroll
+          for (int i = 7; i >= 0; i--) {
+            float r = run;
+#pragma unroll
+            for (int j = 0; j <= i; j++) r += c[j];
+            if (top_k ? r >= want : total - r <= want) bin = lane * 8 + i;
+          }
+          bin = __reduce_min_sync(kAll, bin);
+          if (lane == 0) sh.guess = bin >= kBins - 1 ? -INFINITY : ref - (bin + 1) * width;
+        }
+        __syncthreads();
+        guess = sh.guess;
+      } else if (!greedy) {
+        guess = ref + (float)(log2(s.m) * (s.t / kLog2e64)) * (1.0f + 1e-5f) - 1e-6f * fabsf(ref);
+      }
+      pass(std::true_type(), guess);
+    }
+    const uint32_t top = team.most(nan ? kAll : O::of(best));
+    int label = -1;
+    if (top != kAll && O::value(top) > -INFINITY) {
+      best = O::value(top);
+      label = kUnsure;
+      const uint32_t longest = team.most((uint32_t)n), held = team.sum((uint32_t)(lane == 0 ? n : 0));
+      if (workable && list && longest <= kListWarp && fabsf(best) < INFINITY && (!top_k || held >= s.k)) {
+        if (top_p) {
+          const double up = exp2((double)(ref - best) * (double)scale);
+          all *= up;
+          slack *= up;
+          if (!((best - ref) * scale < 8.0f)) all = INFINITY;  // the bound counts on a sample that comes near the largest
+        }
+        const bool few = held <= kFew;
+        if (few) {  // to one warp, which exchanges without barriers
+          uint32_t to;
+          team.ahead((uint32_t)n, to);
+          for (int i = lane; i < n; i += 32) sh.few_z[to + i] = sh.z[warp][i], sh.few_at[to + i] = sh.at[warp][i];
+        }
+        __syncthreads();
+        const auto from_list = [&](auto places) {
+          constexpr int E = decltype(places)::value;
+          float z[E];
+#pragma unroll
+          for (int e = 0; e < E; e++) z[e] = e * 32 + lane < n ? sh.z[warp][e * 32 + lane] : -INFINITY;
+          const int at = draw<T, E, kLongWarps>(team, z, best, s, V, all, slack);
+          return at < 0 ? at : sh.at[at / (32 * E)][at % (32 * E)];
+        };
+        for (int again = 0; again < 2; again++) {
+          if (few) {
+            if (warp == 0) {
+              constexpr int E = kFew / 32;
+              float z[E];
+#pragma unroll
+              for (int e = 0; e < E; e++) z[e] = e * 32 + lane < (int)held ? sh.few_z[e * 32 + lane] : -INFINITY;
+              Team<1> one{sh.team, 0, lane};
+              const int at = draw<T, E, 1>(one, z, best, s, V, all, slack);
+              if (lane == 0) sh.answer = at < 0 ? at : sh.few_at[at];
+            }
+            __syncthreads();
+            label = sh.answer;
+          } else {
+            label = longest <= 128 ? from_list(std::integral_constant<int, 4>()) : from_list(std::integral_constant<int, kHeld>());
+          }
+          if (label != kUnsure || !(slack > 0.0)) break;
+          const Weight weight(best, s.t);  // the mass again, in 64 bits
+          double m = 0.0;
+          each_of_row<T, VEC>(p, a.z.cs, V, warp, lane, [&](float z) { m += weight.of(z); });
+          all = team.sum(m);
+          slack = 0.0;
+        }
+      } else if (workable && !list && (best - ref) * scale < 8.0f) {
+        const double want = s.u * all;
+        if (threadIdx.x == 0) sh.answer = kUnsure;
+        __syncthreads();
+        if (want > slack && all - want > slack && before <= want && before + sum > want) {
+          // this warp's part holds the draw: its group, then its label
+          const int groups = (steps + group - 1) / group;
+          int g = 0;
+          double run = before;
+          while (g < groups - 1 && run + sh.sums[warp][g] <= want) run += sh.sums[warp][g++];
+          int found = -1;
+          bool near = fabs(run - want) <= slack;
+          for (int i = g * group; i < min(steps, (g + 1) * group) && found < 0; i++) {
+            Step<T, VEC> x;
+            const int first = v0 + i * 256;
+            x.load(p, a.z.cs, first, lane, v1);
+            // running sums in index order
+            uint32_t hit = 0;
+            if constexpr (VEC) {
+              float w[8], mine = 0.0f;
+#pragma unroll
+              for (int e = 0; e < 8; e++) mine += w[e] = exp2_fast((x.z[e] - ref) * scale);
+              float scan = mine;
+#pragma unroll
+              for (int d = 1; d < 32; d <<= 1) {
+                const float t = __shfl_up_sync(kAll, scan, d);
+                if (lane >= d) scan += t;
+              }
+              double r = run + (double)(scan - mine);
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                r += w[e];
+                near |= fabs(r - want) <= slack && w[e] > 0.0f;
+                if (!hit && r > want) hit = ~(uint32_t)(lane * 8 + e);
+              }
+              run += (double)__shfl_sync(kAll, scan, 31);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const float w = exp2_fast((x.z[e] - ref) * scale);
+                float scan = w;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                  const float t = __shfl_up_sync(kAll, scan, d);
+                  if (lane >= d) scan += t;
+                }
+                const double r = run + (double)scan;
+                near |= fabs(r - want) <= slack && w > 0.0f;
+                if (!hit && r > want) hit = ~(uint32_t)(e * 32 + lane);
+                run += (double)__shfl_sync(kAll, scan, 31);
+              }
+            }
+            hit = __reduce_max_sync(kAll, hit);
+            if (hit) found = first + (int)~hit;
+          }
+          near = __any_sync(kAll, near);
+          if (lane == 0 && found >= 0 && !near) sh.answer = found;
+        }
+        __syncthreads();
+        label = sh.answer;
+      }
+      if (label == kUnsure) label = whole_row<T, VEC>(team, sh, a, p, best, s);
+    }
+    if (threadIdx.x == 0) a.label[row] = label;
     __syncthreads();
   }
+}
+
+template <typename T>
+cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
+  SampleArgs b = a;
+  int bits = 1;
+  while ((1ll << bits) < a.V) bits++;
+  // twice the error, relative to the whole sum, of a running sum in float32 and of u times the sum.  exp2 is off by 2^-22 of a weight; its
+  // argument by 2.1 * 2^-24 of it (times ln 2), which counts with the weights: at most by log2 V (the entropy), and 16 where
+  // the largest was not known; additions by 2^-24 each.
+  const auto margin = [&](double chain, double extra) {
+    return (float)(2.0 * (0x1p-22 + 2.1 * 0.7 * 0x1p-24 * (bits + extra) + (chain + 4) * 0x1p-24));
+  };
+  const auto run = [&](auto* kernel, int64_t units, int threads, int per_sm) {
+    kernel<<<(unsigned)std::min<int64_t>(units, (int64_t)sms * per_sm), threads, 0, s>>>(b);
+    return cudaPeekAtLastError();
+  };
+  const bool image = a.z.rs == 1 && a.z.cs != 1 && a.M > 1;
+  if (image && a.V <= 1024 && !a.top_k && !a.top_p && (a.top_k_all <= 0 || a.top_k_all >= a.V) && a.top_p_all >= 1.0) {
+    b.margin = margin((a.V + kPieces - 1) / kPieces + kPieces, 0);
+    const auto pixels = [&](auto px) {
+      constexpr int PX = decltype(px)::value;
+      const int64_t units = (a.M + PX * kImageThreads - 1) / (PX * kImageThreads);
+      if (a.V > 160) return run(sample_image_kernel<T, PX>, units, kImageThreads, 64);
+      b.margin = margin(8 + 2 + 16 + 10, 0);
+      return a.V <= 32    ? run(sample_pixels_kernel<T, PX, 32>, units, kImageThreads, 64)
+             : a.V <= 64  ? run(sample_pixels_kernel<T, PX, 64>, units, kImageThreads, 64)
+             : a.V <= 96  ? run(sample_pixels_kernel<T, PX, 96>, units, kImageThreads, 64)
+             : a.V <= 128 ? run(sample_pixels_kernel<T, PX, 128>, units, kImageThreads, 64)
+                          : run(sample_pixels_kernel<T, PX, 160>, units, kImageThreads, 64);
+    };
+    if constexpr (sizeof(T) == 2)
+      if (a.M % 2 == 0 && a.z.cs % 2 == 0 && (uintptr_t)a.z.p % 4 == 0) return pixels(std::integral_constant<int, 2>());
+    return pixels(std::integral_constant<int, 1>());
+  }
+  if (a.V <= 256) {
+    b.margin = margin(8 + 5, 0);
+    return run(sample_rows_kernel<T, 8, 1>, (a.M + 7) / 8, 256, 64);
+  }
+  b.margin = margin(16 + 5 + 8, 0);
+  if (a.V <= 1024) return run(sample_rows_kernel<T, 16, 2>, a.M, 64, 64);
+  if (a.V <= 4096) return run(sample_rows_kernel<T, 16, 8>, a.M, 256, 16);
+  if (a.V <= 8192) return run(sample_rows_kernel<T, 16, 16>, a.M, 512, 8);
+  const int64_t part = (a.V + kLongWarps * 256ll - 1) / (kLongWarps * 256), group = (part + kSums - 1) / kSums;
+  b.margin = margin((double)group + 3 + 5 + 3 + 5, 16);
+  constexpr int per = 16 / (int)sizeof(T);
+  if (a.z.cs == 1 && a.z.rs % per == 0 && a.V % per == 0 && (uintptr_t)a.z.p % 16 == 0)
+    return run(sample_long_kernel<T, true>, a.M, kLongThreads, 8);
+  return run(sample_long_kernel<T, false>, a.M, kLongThreads, 8);
 }
 
 }  // namespace
 
 cudaError_t launch_sample(int dtype, const SampleArgs& a, int sms, cudaStream_t s) {
-  SampleArgs b = a;
-  int bits = 0;
-  while ((1ll << bits) < a.V) bits++;
-  b.unit = ldexp(1.0, 62 - std::max(bits, 16));
-  const unsigned blocks = (unsigned)std::min<int64_t>(a.M, (int64_t)sms * 4);
-  if (dtype == VI_F32) sample_kernel<float><<<blocks, kThreads, 0, s>>>(b);
-  else if (dtype == VI_F16) sample_kernel<__half><<<blocks, kThreads, 0, s>>>(b);
-  else sample_kernel<__nv_bfloat16><<<blocks, kThreads, 0, s>>>(b);
-  return cudaPeekAtLastError();
+  return dtype == VI_F32 ? launch<float>(a, sms, s) : dtype == VI_F16 ? launch<__half>(a, sms, s) : launch<__nv_bfloat16>(a, sms, s);
 }
 
 }  // namespace heads
