@@ -68,10 +68,12 @@ __device__ __forceinline__ double pow2_64(double x) {
   return x < -1000.0 ? 0.0 : __hiloint2double(__double2hiint(p) + (__double2loint(m) << 20), __double2loint(p));
 }
 
+constexpr double kLog2e64 = 1.44269504088896340735992468100;
 // A row's settings.
 struct Setting {
   double t, p, m, u;
   int64_t k;
+  double scale;  // log2(e) / t
 };
 __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int64_t row) {
   Setting s;
@@ -80,17 +82,20 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int64_t row) 
   s.m = a.min_p ? (double)a.min_p[row] : a.min_p_all;
   s.k = a.top_k ? a.top_k[row] : a.top_k_all;
   s.u = a.u[row];
+  s.scale = a.temperature ? kLog2e64 / s.t : a.scale_all;
   return s;
 }
-constexpr double kLog2e64 = 1.44269504088896340735992468100;
+__device__ __forceinline__ double log2_min_p(const SampleArgs& a, const Setting& s) { return a.min_p ? log2(s.m) : a.log2_min_p_all; }
 struct Weight {
   float best;
   double scale;  // log2(e) / T
-  __device__ __forceinline__ Weight(float best, double t) : best(best), scale(kLog2e64 / t) {}
+  __device__ __forceinline__ Weight(float best, double scale) : best(best), scale(scale) {}
   __device__ __forceinline__ double of(float z) const {
     return z == best ? 1.0 : z == -INFINITY ? 0.0 : pow2_64(((double)z - (double)best) * scale);
   }
 };
+
+constexpr int kUnsure = -2;
 
 // ---- a team of warps that holds a row, or a row's candidates ----
 struct TeamShared {
@@ -140,6 +145,49 @@ struct Team {
     }
     return v;
   }
+  // The place at which the running sum of the held w, in index order, exceeds u times their sum.  mine: the sum of the lane's; last:
+  // its last place with weight, and one, in case u is 1 or more.  margin: kUnsure where a running sum is as near to
+  // u times the sum as that share of it, or where `doubt`.
+  template <int E, typename F>
+  __device__ __forceinline__ int place(const F (&w)[E], double mine, double u, uint32_t last, float margin = 0.0f, bool doubt = false) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(kAll, mine, o);
+    double before, total;
+    ahead(mine, before, total);
+    const double want = u * total, slack = total * margin;
+    uint32_t hit = 0;
+    // one warp's values hold it; its neighbours at the borders are looked at for the margin's sake
+    if (before - slack <= want && before + mine + slack >= want && mine > 0.0) {
+      double run = before;
+      if (margin > 0.0f) doubt |= fabs(run - want) <= slack;
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        F v = w[e];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const F t = __shfl_up_sync(kAll, v, d);
+          if (lane >= d) v += t;
+        }
+        const double r = run + (double)v;
+        if (w[e] > (F)0) {
+          if (margin > 0.0f) doubt |= fabs(r - want) <= slack;
+          if (r > want) hit = max(hit, ~(uint32_t)((warp * E + e) * 32 + lane));
+          last = max(last, (uint32_t)((warp * E + e) * 32 + lane) + 1);
+        }
+        run += (double)__shfl_sync(kAll, v, 31);
+      }
+      // by its sum the warp holds the draw, though its running sums, added in another order, stay under it
+      if (before <= want && before + mine > want && !__any_sync(kAll, hit)) hit = __reduce_max_sync(kAll, last) ? ~(__reduce_max_sync(kAll, last) - 1) : 0;
+    }
+    if (margin > 0.0f) {
+      if constexpr (WARPS > 1) doubt = __syncthreads_or(doubt);
+      else doubt = __any_sync(kAll, doubt);
+      if (doubt) return kUnsure;
+    }
+    hit = most(hit);
+    if (hit) return (int)~hit;
+    return margin > 0.0f ? kUnsure : (int)most(last) - 1;
+  }
   // what the warps in front of this one hold, and all
   __device__ __forceinline__ void ahead(uint32_t v, uint32_t& before) {
     before = 0;
@@ -166,8 +214,6 @@ struct Team {
   }
 };
 
-constexpr int kUnsure = -2;
-
 // The draw among held values, by the definition, in 64 bits.  A lane's value e stands for place (warp * E + e) * 32 + lane,
 // which is index order.  `best` is the largest and finite or +inf; empty places hold -inf.  all: the mass that top-p's share is
 // of, if it is known to `slack` (mass that is not held counts), else negative.  Returns the place; kUnsure where
@@ -176,16 +222,19 @@ template <typename T, int E, int WARPS>
 __device__ __forceinline__ int draw(Team<WARPS>& team, const float (&z)[E], float best, const Setting& s, int64_t labels,
                                     double all = -1.0, double slack = 0.0) {
   using O = Order<T>;
-  const Weight weight(best, s.t);
+  const Weight weight(best, s.scale);
   const bool greedy = !(s.t > 0.0);
   const int lane = team.lane;
+  uint32_t o[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) o[e] = O::of(z[e]);
   // kept: order above `low`, and the first `ties` of those equal to it
   uint32_t low = greedy ? O::of(best) : 0, ties = greedy ? 1 : kManyTies;
   // bisections begin at the first bit in which what is held differs
   uint32_t least = kAll;
   if (!greedy && (s.p < 1.0 || (s.k > 0 && s.k < labels))) {
 #pragma unroll
-    for (int e = 0; e < E; e++) least = z[e] > -INFINITY ? min(least, O::of(z[e])) : least;
+    for (int e = 0; e < E; e++) least = z[e] > -INFINITY ? min(least, o[e]) : least;
     least = ~team.most(~least);
   }
   const uint32_t differ = least ^ O::of(best);
@@ -198,30 +247,27 @@ __device__ __forceinline__ int draw(Team<WARPS>& team, const float (&z)[E], floa
       const uint32_t c = low | 1u << bit;
       uint32_t n = 0;
 #pragma unroll
-      for (int e = 0; e < E; e++) n += O::of(z[e]) >= c;
+      for (int e = 0; e < E; e++) n += o[e] >= c;
       if (team.sum(n) >= s.k) low = c;
     }
     uint32_t n = 0;
 #pragma unroll
-    for (int e = 0; e < E; e++) n += O::of(z[e]) > low;
+    for (int e = 0; e < E; e++) n += o[e] > low;
     ties = (uint32_t)(s.k - team.sum(n));
   }
   double w[E];
 #pragma unroll
-  for (int e = 0; e < E; e++) w[e] = greedy ? (z[e] == best ? 1.0 : 0.0) : weight.of(z[e]);
+  for (int e = 0; e < E; e++) w[e] = greedy ? (o[e] == low ? 1.0 : 0.0) : weight.of(z[e]);
   if (!greedy && s.p < 1.0) {
     const auto mass = [&](uint32_t from) {  // of what is above low, from `from` on
       double v = 0.0;
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const uint32_t o = O::of(z[e]);
-        v += o >= from && o > low ? w[e] : 0.0;
-      }
+      for (int e = 0; e < E; e++) v += o[e] >= from && o[e] > low ? w[e] : 0.0;
       return team.sum(v);
     };
     uint32_t n = 0;
 #pragma unroll
-    for (int e = 0; e < E; e++) n += O::of(z[e]) == low;
+    for (int e = 0; e < E; e++) n += o[e] == low;
     n = min(team.sum(n), ties);
     const double at_low = n ? n * (low ? weight.of(O::value(low)) : 0.0) : 0.0;
     const bool all_known = all >= 0.0;
@@ -239,7 +285,7 @@ __device__ __forceinline__ int draw(Team<WARPS>& team, const float (&z)[E], floa
     const double above = mass(cut + 1), one = cut ? weight.of(O::value(cut)) : 0.0;
     uint32_t have = 0;
 #pragma unroll
-    for (int e = 0; e < E; e++) have += O::of(z[e]) == cut;
+    for (int e = 0; e < E; e++) have += o[e] == cut;
     have = team.sum(have);
     if (cut == low) have = min(have, ties);
     const double need = one > 0.0 ? ceil((want - above) / one) : (double)have;
@@ -250,84 +296,47 @@ __device__ __forceinline__ int draw(Team<WARPS>& team, const float (&z)[E], floa
   // kept weights; those equal to low by their number in index order
   uint32_t equal = 0;
 #pragma unroll
-  for (int e = 0; e < E; e++) equal += __popc(__ballot_sync(kAll, O::of(z[e]) == low));
+  for (int e = 0; e < E; e++) equal += __popc(__ballot_sync(kAll, o[e] == low));
   uint32_t seen;
   team.ahead(equal, seen);
-  double mine = 0.0, run[E];
+  const uint32_t first = O::of(best);
+  double mine = 0.0;
+  uint32_t last = 0;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    const uint32_t o = O::of(z[e]), b = __ballot_sync(kAll, o == low);
-    const bool in = o > low || (o == low && seen + __popc(b & ((1u << lane) - 1)) < ties);
+    const uint32_t b = __ballot_sync(kAll, o[e] == low);
+    const bool in = o[e] > low || (o[e] == low && seen + __popc(b & ((1u << lane) - 1)) < ties);
     seen += __popc(b);
-    w[e] = in && (!(w[e] < s.m) || z[e] == best) ? w[e] : 0.0;
-    double v = w[e];
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const double t = __shfl_up_sync(kAll, v, d);
-      if (lane >= d) v += t;
-    }
-    run[e] = mine + v;
-    mine += __shfl_sync(kAll, v, 31);
+    w[e] = in && (!(w[e] < s.m) || o[e] == first) ? w[e] : 0.0;
+    mine += w[e];
+    if (w[e] > 0.0) last = (team.warp * E + e) * 32 + lane + 1;
   }
-  double before, total;
-  team.ahead(mine, before, total);
-  const double want = s.u * total;
-  uint32_t hit = 0, last = 0;  // 0: none; the first hit as its complement
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const uint32_t at = (team.warp * E + e) * 32 + lane;
-    if (w[e] > 0.0) last = max(last, at + 1);
-    if (w[e] > 0.0 && before + run[e] > want) hit = max(hit, ~at);
-  }
-  hit = team.most(hit);
-  if (hit) return (int)~hit;
-  return (int)team.most(last) - 1;  // u of 1 and more
+  return team.template place<E, double>(w, mine, s.u, last);
 }
 
-// The same where neither top-k nor top-p is asked for, in float32; -1 where the draw, or a label at min_p, is within the error of
-// a border.  Sums of chains of E + 5 additions and of the warps.
+// The same where neither top-k nor top-p is asked for, in float32; kUnsure where the draw, or a label at min_p, is within
+// the error of a border.  Sums of chains of E + 5 additions; the warps' in 64 bits.
 template <int E, int WARPS>
 __device__ __forceinline__ int draw_fast(Team<WARPS>& team, const float (&z)[E], float best, const Setting& s, float margin) {
-  const float scale = (float)(kLog2e64 / s.t), least = (float)s.m;
-  const int lane = team.lane;
-  float run[E], w[E], mine = 0.0f;
-  uint32_t doubt = 0;
+  const float scale = (float)s.scale, least = (float)s.m;
+  float w[E];
+  double mine = 0.0;
+  bool doubt = !(s.u < 1.0);
+  float part = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    const float x = z[e] == best ? 1.0f : exp2_fast((z[e] - best) * scale);
+    const float x = exp2_fast((z[e] - best) * scale);
     doubt |= fabsf(x - least) <= 3e-5f * least && s.m > 0.0 && z[e] != best;
     w[e] = !(x < least) || z[e] == best ? x : 0.0f;
-    float v = w[e];
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const float t = __shfl_up_sync(kAll, v, d);
-      if (lane >= d) v += t;
-    }
-    run[e] = mine + v;
-    mine += __shfl_sync(kAll, v, 31);
+    part += w[e];
   }
-  double before, total;
-  team.ahead((double)mine, before, total);
-  const double want = s.u * total, slack = total * margin;
-  uint32_t hit = 0;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const double r = before + (double)run[e];
-    const uint32_t at = (team.warp * E + e) * 32 + lane;
-    // a sum that ends near the border from either side: the label before it, or behind it, may be the answer
-    doubt |= w[e] > 0.0f && fabs(r - want) <= slack;
-    if (w[e] > 0.0f && r > want) hit = max(hit, ~at);
-  }
-  doubt |= !(want > slack) || !(total - want > slack);
-  if constexpr (WARPS > 1) doubt = __syncthreads_or(doubt);
-  else doubt = __any_sync(kAll, doubt);
-  hit = team.most(hit);
-  return doubt || !hit ? -1 : (int)~hit;
+  mine = part;
+  return team.template place<E, float>(w, mine, s.u, 0, margin, doubt);
 }
 
-// Whether float32's weights serve: its reach, and no inf - inf.
+// Whether float32's weights serve: exponents within its reach (2^17 / 2^24 of one: the rounding that all weights share).
 __device__ __forceinline__ bool plain_scale(const Setting& s, float best) {
-  return s.t > 1e-30 && s.t < 1e30 && fabsf(best) < 1e37f;
+  return s.t > 1e-30 && s.t < 1e30 && fabs((double)best) * s.scale < 0x1p17;
 }
 
 // Loads a row into registers and draws.
@@ -388,7 +397,7 @@ __device__ __noinline__ int64_t image_row_again(const SampleArgs& a, int64_t row
   for (int v = lane; v < a.V; v += 32) best = fmaxf(best, to_f(p[v * a.z.cs]));
 #pragma unroll
   for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(kAll, best, o));
-  const Weight weight(best, s.t);
+  const Weight weight(best, s.scale);
   double run = 0.0, want = 0.0;
   int last = -1;
 #pragma unroll 1
@@ -464,7 +473,7 @@ __global__ void __launch_bounds__(kImageThreads) sample_image_kernel(const __gri
         } else {
           draws = true;
         }
-        scale[j] = (float)(kLog2e64 / s[j].t);
+        scale[j] = (float)s[j].scale;
         least[j] = (float)s[j].m;
       }
       if (firsts) {
@@ -540,8 +549,28 @@ __global__ void __launch_bounds__(kImageThreads) sample_image_kernel(const __gri
   }
 }
 
+__device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b, __half) {
+  const __half2 r = __hmax2_nan(*(const __half2*)&a, *(const __half2*)&b);
+  return *(const uint32_t*)&r;
+}
+__device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 r = __hmax2_nan(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+  return *(const uint32_t*)&r;
+}
+// All bits of each half of `a` that is at least b's.
+__device__ __forceinline__ uint32_t at_least2(uint32_t a, uint32_t b, __half) { return __hge2_mask(*(const __half2*)&a, *(const __half2*)&b); }
+__device__ __forceinline__ uint32_t at_least2(uint32_t a, uint32_t b, __nv_bfloat16) {
+  return __hge2_mask(*(const __nv_bfloat162*)&a, *(const __nv_bfloat162*)&b);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pair_bits(T a, T b) {
+  return (uint32_t) * (const unsigned short*)&a | (uint32_t) * (const unsigned short*)&b << 16;
+}
+
 // The same with the pixel's logits in registers (up to NV labels): memory is read once, with all of a thread's loads in flight.
 // The piece that holds the draw is picked out of them by comparisons.
+// Weights beside the largest's: exp2(z scale - best scale), whose constant's rounding is a factor of all alike.
+// The matrix is under 4 GB, so that 32-bit offsets reach all of it.
 template <typename T, int PX, int NV>
 __global__ void __launch_bounds__(kImageThreads) sample_pixels_kernel(const __grid_constant__ SampleArgs a) {
   constexpr int kLen = 16, kCount = NV / kLen;
@@ -560,12 +589,16 @@ __global__ void __launch_bounds__(kImageThreads) sample_pixels_kernel(const __gr
     const int64_t row = base + threadIdx.x * PX;
     uint32_t again = 0;  // pixels that float32 does not decide
     if (row < a.M) {
-      const T* p = (const T*)a.z.p + row * a.z.rs;
       Word z[NV];
+      {
+        const char* p = (const char*)a.z.p;
+        const uint32_t by = (uint32_t)(a.z.cs * sizeof(T));
+        uint32_t at = (uint32_t)(row * sizeof(T));
 #pragma unroll
-      for (int v = 0; v < NV; v++) {
-        if constexpr (PX == 1) z[v] = v < a.V ? to_f(p[v * a.z.cs]) : -INFINITY;
-        else z[v] = v < a.V ? *(const uint32_t*)(p + v * a.z.cs) : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        for (int v = 0; v < NV; v++, at += by) {
+          if constexpr (PX == 1) z[v] = v < a.V ? to_f(*(const T*)(p + at)) : -INFINITY;
+          else z[v] = v < a.V ? *(const uint32_t*)(p + at) : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        }
       }
       float best[PX];
       if constexpr (PX == 1) {
@@ -573,93 +606,104 @@ __global__ void __launch_bounds__(kImageThreads) sample_pixels_kernel(const __gr
 #pragma unroll
         for (int v = 1; v < NV; v++) best[0] = max_nan(best[0], z[v]);
       } else {
-        Word m = z[0];
+        Word m[2] = {z[0], z[1]};
 #pragma unroll
-        for (int v = 1; v < NV; v++) {
-          if constexpr (std::is_same<T, __half>::value) {
-            const __half2 r = __hmax2_nan(*(const __half2*)&m, *(const __half2*)&z[v]);
-            m = *(const Word*)&r;
-          } else {
-            const __nv_bfloat162 r = __hmax2_nan(*(const __nv_bfloat162*)&m, *(const __nv_bfloat162*)&z[v]);
-            m = *(const Word*)&r;
-          }
-        }
+        for (int v = 2; v < NV; v++) m[v & 1] = max_nan2(m[v & 1], z[v], T());
+        m[0] = max_nan2(m[0], m[1], T());
 #pragma unroll
-        for (int j = 0; j < PX; j++) best[j] = value(m, j);
+        for (int j = 0; j < PX; j++) best[j] = value(m[0], j);
       }
+      Setting s[PX];
+      bool draws[PX], near[PX], cut = false;
+      T least[PX];  // min-p keeps the logits from a value on: the type's first value there
 #pragma unroll
       for (int j = 0; j < PX; j++) {
-        const Setting s = setting_of(a, row + j);
-        if (best[j] != best[j] || s.t != s.t || best[j] == -INFINITY) {
+        s[j] = setting_of(a, row + j);
+        draws[j] = false;
+        near[j] = !(s[j].u < 1.0);
+        least[j] = from_f<T>(-INFINITY);
+        if (best[j] != best[j] || s[j].t != s[j].t || best[j] == -INFINITY) {
           a.label[row + j] = -1;
-        } else if (!(s.t > 0.0)) {
+        } else if (!(s[j].t > 0.0)) {
           int at = 0;
 #pragma unroll
           for (int v = NV - 1; v >= 0; v--) at = value(z[v], j) == best[j] ? v : at;
           a.label[row + j] = at;
-        } else if (!plain_scale(s, best[j])) {
+        } else if (!plain_scale(s[j], best[j])) {
           again |= 1u << j;
         } else {
-          const double scale64 = kLog2e64 / s.t;
-          const float scale = (float)scale64;
-          bool near = !(s.u < 1.0);
-          // min-p keeps the logits from a value on: the type's first value there
-          float least = -INFINITY;
-          if (s.m >= 1.0) {
-            least = best[j];
-          } else if (s.m > 0.0) {
-            const double at = (double)best[j] + log2(s.m) / scale64;
-            T up;
+          draws[j] = true;
+          if (s[j].m >= 1.0) {
+            least[j] = from_f<T>(best[j]);
+            cut = true;
+          } else if (s[j].m > 0.0) {
+            const double at = (double)best[j] + log2_min_p(a, s[j]) / s[j].scale;
             double round;
-            if constexpr (sizeof(T) == 4) up = __double2float_ru(at), round = (double)(float)at;
-            else if constexpr (std::is_same<T, __half>::value) up = __float2half_ru(__double2float_ru(at)), round = (double)__half2float(__double2half(at));
-            else up = __float2bfloat16_ru(__double2float_ru(at)), round = (double)__bfloat162float(__double2bfloat16(at));
-            least = to_f(up);
-            near |= fabs(round - at) <= 1e-12 * (fabs(at) + fabs((double)best[j]));
+            if constexpr (sizeof(T) == 4) least[j] = __double2float_ru(at), round = (double)(float)at;
+            else if constexpr (std::is_same<T, __half>::value) least[j] = __float2half_ru(__double2float_ru(at)), round = (double)__half2float(__double2half(at));
+            else least[j] = __float2bfloat16_ru(__double2float_ru(at)), round = (double)__bfloat162float(__double2bfloat16(at));
+            near[j] |= fabs(round - at) <= 1e-12 * (fabs(at) + fabs((double)best[j]));
+            cut = true;
           }
-          const auto weight = [&](Word w) {
-            const float x = value(w, j);
-            return x >= least ? exp2_fast((x - best[j]) * scale) : 0.0f;
-          };
-          float run[kCount], sum = 0.0f;
-#pragma unroll
-          for (int c = 0; c < kCount; c++) {
-            float q[2] = {0.0f, 0.0f};
-            if (c * kLen < a.V) {
-#pragma unroll
-              for (int i = 0; i < kLen; i++) q[i & 1] += weight(z[c * kLen + i]);
-            }
-            run[c] = sum += q[0] + q[1];
-          }
-          const float want = (float)s.u * sum, slack = sum * a.margin;
-          int c = 0;
-          float start = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kCount - 1; i++) {
-            const bool behind = run[i] <= want;
-            c += behind;
-            start = behind ? run[i] : start;
-          }
-          Word cell[kLen];
-#pragma unroll
-          for (int i = 0; i < kLen; i++) cell[i] = z[i];
-#pragma unroll
-          for (int k = 1; k < kCount; k++) {
-#pragma unroll
-            for (int i = 0; i < kLen; i++) cell[i] = c == k ? z[k * kLen + i] : cell[i];
-          }
-          near |= fabsf(start - want) <= slack;
-          int at = -1;
-          float r = 0.0f;
-#pragma unroll
-          for (int i = 0; i < kLen; i++) {
-            r += weight(cell[i]);
-            near |= fabsf(start + r - want) <= slack;
-            at = at < 0 && start + r > want ? c * kLen + i : at;
-          }
-          if (near || at < 0) again |= 1u << j;
-          else a.label[row + j] = at;
         }
+      }
+      if (cut) {  // what min-p drops counts as -inf
+        if constexpr (PX == 1) {
+#pragma unroll
+          for (int v = 0; v < NV; v++) z[v] = z[v] >= to_f(least[0]) ? z[v] : -INFINITY;
+        } else {
+          const uint32_t from = pair_bits(least[0], least[1]), none = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+          for (int v = 0; v < NV; v++) {
+            const uint32_t in = at_least2(z[v], from, T());
+            z[v] = (z[v] & in) | (none & ~in);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < PX; j++) {
+        if (!draws[j]) continue;
+        const float scale = (float)s[j].scale, shift = -best[j] * scale;
+        const auto weight = [&](Word w) { return exp2_fast(fmaf(value(w, j), scale, shift)); };
+        float run[kCount], sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kCount; c++) {
+          float q[2] = {0.0f, 0.0f};
+          if (c * kLen < a.V) {
+#pragma unroll
+            for (int i = 0; i < kLen; i++) q[i & 1] += weight(z[c * kLen + i]);
+          }
+          run[c] = sum += q[0] + q[1];
+        }
+        const float want = (float)s[j].u * sum, slack = sum * a.margin;
+        int c = 0;
+        float start = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kCount - 1; i++) {
+          const bool behind = run[i] <= want;
+          c += behind;
+          start = behind ? run[i] : start;
+        }
+        Word cell[kLen];
+#pragma unroll
+        for (int i = 0; i < kLen; i++) cell[i] = z[i];
+#pragma unroll
+        for (int k = 1; k < kCount; k++) {
+          const bool here = c == k;
+#pragma unroll
+          for (int i = 0; i < kLen; i++) cell[i] = here ? z[k * kLen + i] : cell[i];
+        }
+        bool close = near[j] | (fabsf(start - want) <= slack);
+        int at = -1;
+        float r = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kLen; i++) {
+          r += weight(cell[i]);
+          close |= fabsf(start + r - want) <= slack;
+          at = at < 0 && start + r > want ? c * kLen + i : at;
+        }
+        if (close || at < 0) again |= 1u << j;
+        else a.label[row + j] = at;
       }
     }
     // what is left, a warp a row
@@ -683,15 +727,14 @@ constexpr int kListWarp = 32 * kHeld;          // candidates a warp keeps
 constexpr int kSample = 16;                    // labels a lane looks at for the guess
 constexpr int kSums = 64;                      // sums of steps a warp keeps
 constexpr int kBins = 256;
+constexpr int kBatch = 4;                      // steps whose loads are in flight together
 constexpr int kFew = 256;                      // candidates that one warp draws from
 struct LongShared {
   TeamShared team;
-  float z[kLongWarps][kListWarp];
   int at[kLongWarps][kListWarp];
   float sums[kLongWarps][kSums];
   uint32_t bins[kBins];
-  float few_z[kFew];
-  int few_at[kFew];
+  int few[kFew];
   float guess;
   int answer;
 };
@@ -699,35 +742,60 @@ struct LongShared {
 // What a lane holds of 256 labels from `first` on: 8 in a row (VEC: loaded as vectors), or every 32nd.
 template <typename T, bool VEC>
 struct Step {
-  float z[8];
+  static constexpr int kPer = 16 / (int)sizeof(T);
+  union {
+    uint4 q[8 / kPer];
+    T t[8];
+  };
+  __device__ __forceinline__ Step() {}
+  __device__ __forceinline__ float z(int e) const { return to_f(t[e]); }
   static __device__ __forceinline__ int place(int first, int lane, int e) { return VEC ? first + lane * 8 + e : first + e * 32 + lane; }
   // ends at `end`; with VEC whole vectors lie on one side of it
   __device__ __forceinline__ void load(const T* p, int64_t cs, int first, int lane, int end) {
     if constexpr (VEC) {
-      constexpr int per = 16 / (int)sizeof(T);
+      constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
 #pragma unroll
-      for (int i = 0; i < 8; i += per) {
-        const int v = first + lane * 8 + i;
-        if (v < end) {
-          const uint4 q = *(const uint4*)(p + v);
-#pragma unroll
-          for (int j = 0; j < per; j++) z[i + j] = to_f(((const T*)&q)[j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < per; j++) z[i + j] = -INFINITY;
-        }
+      for (int i = 0; i < 8 / kPer; i++) {
+        const int v = first + lane * 8 + i * kPer;
+        q[i] = v < end ? *(const uint4*)(p + v) : make_uint4(none, none, none, none);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const int v = first + e * 32 + lane;
-        z[e] = v < end ? to_f(p[v * cs]) : -INFINITY;
+        t[e] = v < end ? p[v * cs] : from_f<T>(-INFINITY);
       }
     }
   }
+  // The largest, or a NaN if there is one.
+  __device__ __forceinline__ float most(float m) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) m = max_nan(m, z(e));
+      return m;
+    } else {
+      uint32_t w = max_nan2(max_nan2(q[0].x, q[0].y, T()), max_nan2(q[0].z, q[0].w, T()), T());
+      const T a = ((const T*)&w)[0], b = ((const T*)&w)[1];
+      return max_nan(m, max_nan(to_f(a), to_f(b)));
+    }
+  }
+  // Bit e: whether value e is at least `from`.
+  __device__ __forceinline__ uint32_t at_least(float from, uint32_t from2) const {
+    uint32_t in = 0;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) in |= z(e) >= from ? 1u << e : 0u;
+    } else {
+      const uint32_t a = at_least2(q[0].x, from2, T()), b = at_least2(q[0].y, from2, T()), c = at_least2(q[0].z, from2, T()),
+                     d = at_least2(q[0].w, from2, T());
+      if (a | b | c | d)
+        in = (a & 1) | (a >> 30 & 2) | (b & 4) | (b >> 28 & 8) | (c & 16) | (c >> 26 & 32) | (d & 64) | (d >> 24 & 128);
+    }
+    return in;
+  }
 };
 
-// f of every label of a row, in any order: several loads in flight.
+// f of every label of a row and of some -inf, in any order: several loads in flight.
 template <typename T, bool VEC, typename F>
 __device__ __forceinline__ void each_of_row(const T* p, int64_t cs, int V, int warp, int lane, F f) {
   constexpr int kDeep = 4;
@@ -737,10 +805,8 @@ __device__ __forceinline__ void each_of_row(const T* p, int64_t cs, int V, int w
     for (int i = 0; i < kDeep; i++) x[i].load(p, cs, first + i * kLongThreads * 8, lane, V);
 #pragma unroll
     for (int i = 0; i < kDeep; i++) {
-      if (first + i * kLongThreads * 8 >= V) continue;
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (Step<T, VEC>::place(first + i * kLongThreads * 8, lane, e) < V) f(x[i].z[e]);
+      for (int e = 0; e < 8; e++) f(x[i].z(e));
     }
   }
 }
@@ -750,7 +816,7 @@ __device__ __forceinline__ void each_of_row(const T* p, int64_t cs, int V, int w
 template <typename T, bool VEC>
 __device__ __noinline__ int whole_row(Team<kLongWarps>& team, LongShared& sh, const SampleArgs& a, const T* p, float best, const Setting& s) {
   using O = Order<T>;
-  const Weight weight(best, s.t);
+  const Weight weight(best, s.scale);
   const int tid = threadIdx.x, V = a.V;
   const int64_t cs = a.z.cs;
   const bool greedy = !(s.t > 0.0);
@@ -811,7 +877,7 @@ __device__ __noinline__ int whole_row(Team<kLongWarps>& team, LongShared& sh, co
   for (int first = v0; first < v1; first += 256) {
     x.load(p, cs, first, team.lane, v1);
 #pragma unroll
-    for (int e = 0; e < 8; e++) equal += O::of(x.z[e]) == low;
+    for (int e = 0; e < 8; e++) equal += O::of(x.z(e)) == low;
   }
   uint32_t ahead;
   team.ahead(__reduce_add_sync(kAll, equal), ahead);
@@ -827,7 +893,7 @@ __device__ __noinline__ int whole_row(Team<kLongWarps>& team, LongShared& sh, co
     if constexpr (VEC) {
       uint32_t n = 0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) n += O::of(x.z[e]) == low;
+      for (int e = 0; e < 8; e++) n += O::of(x.z(e)) == low;
       uint32_t rank = n;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -840,8 +906,8 @@ __device__ __noinline__ int whole_row(Team<kLongWarps>& team, LongShared& sh, co
       double sum = 0.0;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        w[e] = kept(x.z[e], rank);
-        rank += O::of(x.z[e]) == low;
+        w[e] = kept(x.z(e), rank);
+        rank += O::of(x.z(e)) == low;
         r[e] = sum += w[e];
       }
 #pragma unroll
@@ -856,8 +922,8 @@ __device__ __noinline__ int whole_row(Team<kLongWarps>& team, LongShared& sh, co
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const uint32_t b = __ballot_sync(kAll, O::of(x.z[e]) == low);
-        w[e] = kept(x.z[e], seen + __popc(b & ((1u << team.lane) - 1)));
+        const uint32_t b = __ballot_sync(kAll, O::of(x.z(e)) == low);
+        w[e] = kept(x.z(e), seen + __popc(b & ((1u << team.lane) - 1)));
         seen += __popc(b);
         double sum = w[e];
 #pragma unroll
@@ -897,7 +963,7 @@ __device__ __noinline__ int whole_row(Team<kLongWarps>& team, LongShared& sh, co
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __grid_constant__ SampleArgs a) {
   using O = Order<T>;
   __shared__ LongShared sh;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, V = a.V;
@@ -910,7 +976,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
     const Setting s = setting_of(a, row);
     const bool greedy = !(s.t > 0.0), top_k = !greedy && s.k > 0 && s.k < V, top_p = !greedy && !top_k && s.p < 1.0;
     const bool list = greedy || top_k || top_p || s.m > 0.0;
-    const float scale = (float)(kLog2e64 / s.t);
+    const float scale = (float)s.scale;
 
     // the sample: two steps of each warp
     float ref = -INFINITY, low = INFINITY, sample[kSample];
@@ -920,7 +986,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
       for (int i = 0; i < kSample / 8; i++) x[i].load(p, a.z.cs, v0 + i * (steps / 2) * 256, lane, v1);
 #pragma unroll
       for (int i = 0; i < kSample; i++) {
-        sample[i] = x[i / 8].z[i % 8];
+        sample[i] = x[i / 8].z(i % 8);
         ref = fmaxf(ref, sample[i]);
         if (sample[i] > -INFINITY) low = fminf(low, sample[i]);
       }
@@ -928,61 +994,68 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
     ref = O::value(max(team.most(O::of(ref)), O::of(-INFINITY)));
     const bool workable = plain_scale(s, ref) || (greedy && fabsf(ref) < INFINITY);
 
+    const float ref_scaled = ref * scale;  // its rounding is a factor of all weights alike
+
     // one pass over the row, for sums of the weights beside 2^(ref scale), or for the labels from `guess` on
     float best = -INFINITY;
-    bool nan = s.t != s.t;
     int n = 0;
     double sum = 0.0;
-    const auto pass = [&](auto wants_list, float guess) {
-      constexpr bool kList = decltype(wants_list)::value;
+    const auto pass = [&](auto wants_list, auto wants_best, float guess) {
+      constexpr bool kList = decltype(wants_list)::value, kBest = decltype(wants_best)::value;
+      // the type's last value that is not above the guess
+      T under = from_f<T>(guess);
+      if constexpr (std::is_same<T, __half>::value) under = __float2half_rd(guess);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) under = __float2bfloat16_rd(guess);
+      const uint32_t guess2 = sizeof(T) == 4 ? 0 : pair_bits(under, under);
       float group_sum = 0.0f;
-      Step<T, VEC> next;
-      next.load(p, a.z.cs, v0, lane, v1);
-      for (int i = 0; i < steps && v0 + i * 256 < v1; i++) {
-        const Step<T, VEC> x = next;
-        next.load(p, a.z.cs, v0 + (i + 1) * 256, lane, v1);
-        uint32_t in = 0;
+      for (int i0 = 0; i0 < steps && v0 + i0 * 256 < v1; i0 += kBatch) {
+        Step<T, VEC> batch[kBatch];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          nan |= x.z[e] != x.z[e];
-          best = fmaxf(best, x.z[e]);
-          in |= (uint32_t)(x.z[e] >= guess) << e;
-        }
-        if constexpr (!kList) {
-          float w[8];
+        for (int j = 0; j < kBatch; j++) batch[j].load(p, a.z.cs, v0 + (i0 + j) * 256, lane, v1);
 #pragma unroll
-          for (int e = 0; e < 8; e++) w[e] = exp2_fast((x.z[e] - ref) * scale);
-          group_sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-          if (i % group == group - 1 || v0 + (i + 1) * 256 >= v1) {
+        for (int j = 0; j < kBatch; j++) {
+          const int i = i0 + j, first = v0 + i * 256;
+          const Step<T, VEC>& x = batch[j];
+          if (first >= v1) break;
+          if (kBest) best = x.most(best);
+          uint32_t in = kList ? x.at_least(guess, guess2) : 0;
+          if constexpr (!kList) {
+            float w[8];
 #pragma unroll
-            for (int o = 16; o; o >>= 1) group_sum += __shfl_xor_sync(kAll, group_sum, o);
-            if (lane == 0) sh.sums[warp][i / group] = group_sum;
-            sum += group_sum;
-            group_sum = 0.0f;
-          }
-        } else if (__any_sync(kAll, in)) {
-          if constexpr (VEC) {
+            for (int e = 0; e < 8; e++) w[e] = exp2_fast(fmaf(x.z(e), scale, -ref_scaled));
+            group_sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            if (group == 1 || i % group == group - 1 || first + 256 >= v1) {
+#pragma unroll
+              for (int o = 16; o; o >>= 1) group_sum += __shfl_xor_sync(kAll, group_sum, o);
+              if (lane == 0) sh.sums[warp][i / group] = group_sum;
+              sum += group_sum;
+              group_sum = 0.0f;
+            }
+          } else if (__any_sync(kAll, in)) {
             const int mine = __popc(in);
-            int scan = mine;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-              const int t = __shfl_up_sync(kAll, scan, d);
-              if (lane >= d) scan += t;
-            }
-            int to = n + scan - mine;
-            n += __shfl_sync(kAll, scan, 31);
-            if (n <= kListWarp) {
-#pragma unroll
-              for (int e = 0; e < 8; e++)
-                if (in >> e & 1) sh.z[warp][to] = x.z[e], sh.at[warp][to++] = Step<T, VEC>::place(v0 + i * 256, lane, e);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const uint32_t b = __ballot_sync(kAll, in >> e & 1);
+            if (VEC && !__any_sync(kAll, mine > 1)) {
+              const uint32_t b = __ballot_sync(kAll, in);
               const int to = n + __popc(b & ((1u << lane) - 1));
               n += __popc(b);
-              if (n <= kListWarp && (in >> e & 1)) sh.z[warp][to] = x.z[e], sh.at[warp][to] = Step<T, VEC>::place(v0 + i * 256, lane, e);
+              if (in && to < kListWarp) sh.at[warp][to] = first + lane * 8 + __ffs(in) - 1;
+            } else if constexpr (VEC) {
+              int scan = mine;
+#pragma unroll
+              for (int d = 1; d < 32; d <<= 1) {
+                const int t = __shfl_up_sync(kAll, scan, d);
+                if (lane >= d) scan += t;
+              }
+              int to = n + scan - mine;
+              n += __shfl_sync(kAll, scan, 31);
+              for (; in && to < kListWarp; in &= in - 1) sh.at[warp][to++] = first + lane * 8 + __ffs(in) - 1;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const uint32_t b = __ballot_sync(kAll, in >> e & 1);
+                const int to = n + __popc(b & ((1u << lane) - 1));
+                n += __popc(b);
+                if (to < kListWarp && (in >> e & 1)) sh.at[warp][to] = first + e * 32 + lane;
+              }
             }
           }
         }
@@ -991,15 +1064,16 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
     double all = -1.0, slack = 0.0, before = 0.0;  // all: the row's mass, known to the slack
     if (!workable) {                               // infinite, or nothing seen yet
       each_of_row<T, VEC>(p, a.z.cs, V, warp, lane, [&](float z) {
-        nan |= z != z;
-        best = fmaxf(best, z);
+        best = max_nan(best, z);
       });
     } else if (!list || top_p) {
-      pass(std::false_type(), INFINITY);
+      pass(std::false_type(), std::true_type(), INFINITY);
       team.ahead(sum, before, all);
       slack = all * a.margin;
     }
-    if (workable && list) {
+    float tail = 0.75f;  // top-p: of the share that is not kept, what may lie under the guess
+    int tries = 2;
+    while (workable && list) {
       // the guess: from where on candidates are kept
       float guess = ref;
       if (top_k || top_p) {
@@ -1014,9 +1088,9 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
         __syncthreads();
         if (warp == 0) {
           const float share = (float)(kLongThreads * kSample) / (float)V;
-          // top-k: the rank in the sample that the row's k-th is hardly ever behind.  top-p: as much of the tail as leaves a
-          // quarter of what is not kept, beside the whole mass; the tail's small weights are sampled well
-          const float mean = (float)s.k * share, want = top_k ? mean + 4.0f * sqrtf(mean) + 2.0f : 0.75f * (1.0f - (float)fmax(s.p, 0.0)) * (float)all * share;
+          // top-k: the rank in the sample that the row's k-th is hardly ever behind.  top-p: as much of the tail as leaves some
+          // of what is not kept, beside the whole mass; the tail's small weights are sampled well
+          const float mean = (float)s.k * share, want = top_k ? mean + 4.0f * sqrtf(mean) + 2.0f : tail * (1.0f - (float)fmax(s.p, 0.0)) * (float)all * share;
           float c[8], mine = 0.0f;
 #pragma unroll
           for (int i = 0; i < 8; i++) {
@@ -1045,11 +1119,20 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
         __syncthreads();
         guess = sh.guess;
       } else if (!greedy) {
-        guess = ref + (float)(log2(s.m) * (s.t / kLog2e64)) * (1.0f + 1e-5f) - 1e-6f * fabsf(ref);
+        guess = ref + (float)(log2_min_p(a, s) / s.scale) * (1.0f + 1e-5f) - 1e-6f * fabsf(ref);
       }
-      pass(std::true_type(), guess);
+      n = 0;
+      if (top_p) pass(std::true_type(), std::false_type(), guess);
+      else pass(std::true_type(), std::true_type(), guess);
+      if (!top_p || --tries == 0) break;
+      // more of the tail, if what is held is not enough
+      __syncwarp();
+      double m = 0.0;
+      for (int i = lane; i < min(n, kListWarp); i += 32) m += exp2_fast((to_f(p[(int64_t)sh.at[warp][i] * a.z.cs]) - ref) * scale);
+      if (team.sum(m) > s.p * all * (1.0 + 1e-5) || guess == -INFINITY) break;
+      tail = 0.3f;
     }
-    const uint32_t top = team.most(nan ? kAll : O::of(best));
+    const uint32_t top = team.most(best != best || s.t != s.t ? kAll : O::of(best));
     int label = -1;
     if (top != kAll && O::value(top) > -INFINITY) {
       best = O::value(top);
@@ -1059,21 +1142,21 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
         if (top_p) {
           const double up = exp2((double)(ref - best) * (double)scale);
           all *= up;
-          slack *= up;
+          slack *= 0.5 * up;  // of the sum alone
           if (!((best - ref) * scale < 8.0f)) all = INFINITY;  // the bound counts on a sample that comes near the largest
         }
         const bool few = held <= kFew;
         if (few) {  // to one warp, which exchanges without barriers
           uint32_t to;
           team.ahead((uint32_t)n, to);
-          for (int i = lane; i < n; i += 32) sh.few_z[to + i] = sh.z[warp][i], sh.few_at[to + i] = sh.at[warp][i];
+          for (int i = lane; i < n; i += 32) sh.few[to + i] = sh.at[warp][i];
         }
         __syncthreads();
         const auto from_list = [&](auto places) {
           constexpr int E = decltype(places)::value;
           float z[E];
 #pragma unroll
-          for (int e = 0; e < E; e++) z[e] = e * 32 + lane < n ? sh.z[warp][e * 32 + lane] : -INFINITY;
+          for (int e = 0; e < E; e++) z[e] = e * 32 + lane < n ? to_f(p[(int64_t)sh.at[warp][e * 32 + lane] * a.z.cs]) : -INFINITY;
           const int at = draw<T, E, kLongWarps>(team, z, best, s, V, all, slack);
           return at < 0 ? at : sh.at[at / (32 * E)][at % (32 * E)];
         };
@@ -1083,18 +1166,18 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
               constexpr int E = kFew / 32;
               float z[E];
 #pragma unroll
-              for (int e = 0; e < E; e++) z[e] = e * 32 + lane < (int)held ? sh.few_z[e * 32 + lane] : -INFINITY;
+              for (int e = 0; e < E; e++) z[e] = e * 32 + lane < (int)held ? to_f(p[(int64_t)sh.few[e * 32 + lane] * a.z.cs]) : -INFINITY;
               Team<1> one{sh.team, 0, lane};
               const int at = draw<T, E, 1>(one, z, best, s, V, all, slack);
-              if (lane == 0) sh.answer = at < 0 ? at : sh.few_at[at];
+              if (lane == 0) sh.answer = at < 0 ? at : sh.few[at];
             }
             __syncthreads();
             label = sh.answer;
           } else {
-            label = longest <= 128 ? from_list(std::integral_constant<int, 4>()) : from_list(std::integral_constant<int, kHeld>());
+            label = longest <= 32 * 8 ? from_list(std::integral_constant<int, 8>()) : from_list(std::integral_constant<int, kHeld>());
           }
           if (label != kUnsure || !(slack > 0.0)) break;
-          const Weight weight(best, s.t);  // the mass again, in 64 bits
+          const Weight weight(best, s.scale);  // the mass again, in 64 bits
           double m = 0.0;
           each_of_row<T, VEC>(p, a.z.cs, V, warp, lane, [&](float z) { m += weight.of(z); });
           all = team.sum(m);
@@ -1121,7 +1204,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
             if constexpr (VEC) {
               float w[8], mine = 0.0f;
 #pragma unroll
-              for (int e = 0; e < 8; e++) mine += w[e] = exp2_fast((x.z[e] - ref) * scale);
+              for (int e = 0; e < 8; e++) mine += w[e] = exp2_fast(fmaf(x.z(e), scale, -ref_scaled));
               float scan = mine;
 #pragma unroll
               for (int d = 1; d < 32; d <<= 1) {
@@ -1139,7 +1222,7 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
             } else {
 #pragma unroll
               for (int e = 0; e < 8; e++) {
-                const float w = exp2_fast((x.z[e] - ref) * scale);
+                const float w = exp2_fast(fmaf(x.z(e), scale, -ref_scaled));
                 float scan = w;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
@@ -1171,13 +1254,15 @@ __global__ void __launch_bounds__(kLongThreads, 2) sample_long_kernel(const __gr
 template <typename T>
 cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
   SampleArgs b = a;
+  b.scale_all = kLog2e64 / a.temperature_all;
+  b.log2_min_p_all = a.min_p_all > 0.0 ? log2(a.min_p_all) : 0.0;
   int bits = 1;
   while ((1ll << bits) < a.V) bits++;
   // twice the error, relative to the whole sum, of a running sum in float32 and of u times the sum.  exp2 is off by 2^-22 of a weight; its
-  // argument by 2.1 * 2^-24 of it (times ln 2), which counts with the weights: at most by log2 V (the entropy), and 16 where
-  // the largest was not known; additions by 2^-24 each.
+  // argument by three half steps, 3 ln 2 = 2.1 times 2^-24 |t| of the weight, where |t| counts with the weights: at most as
+  // log2 V (the entropy), and twice the distance to the largest, up to 8, where that was not known; additions by 2^-24 each.
   const auto margin = [&](double chain, double extra) {
-    return (float)(2.0 * (0x1p-22 + 2.1 * 0.7 * 0x1p-24 * (bits + extra) + (chain + 4) * 0x1p-24));
+    return (float)(2.0 * (0x1p-22 + 2.1 * 0x1p-24 * (bits + extra) + (chain + 4) * 0x1p-24));
   };
   const auto run = [&](auto* kernel, int64_t units, int threads, int per_sm) {
     kernel<<<(unsigned)std::min<int64_t>(units, (int64_t)sms * per_sm), threads, 0, s>>>(b);
@@ -1189,7 +1274,7 @@ cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
     const auto pixels = [&](auto px) {
       constexpr int PX = decltype(px)::value;
       const int64_t units = (a.M + PX * kImageThreads - 1) / (PX * kImageThreads);
-      if (a.V > 160) return run(sample_image_kernel<T, PX>, units, kImageThreads, 64);
+      if (a.V > 160 || (a.V * a.z.cs + a.M) * (int64_t)sizeof(T) >= (1ll << 32)) return run(sample_image_kernel<T, PX>, units, kImageThreads, 64);
       b.margin = margin(8 + 2 + 16 + 10, 0);
       return a.V <= 32    ? run(sample_pixels_kernel<T, PX, 32>, units, kImageThreads, 64)
              : a.V <= 64  ? run(sample_pixels_kernel<T, PX, 64>, units, kImageThreads, 64)
@@ -1210,7 +1295,7 @@ cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
   if (a.V <= 4096) return run(sample_rows_kernel<T, 16, 8>, a.M, 256, 16);
   if (a.V <= 8192) return run(sample_rows_kernel<T, 16, 16>, a.M, 512, 8);
   const int64_t part = (a.V + kLongWarps * 256ll - 1) / (kLongWarps * 256), group = (part + kSums - 1) / kSums;
-  b.margin = margin((double)group + 3 + 5 + 3 + 5, 16);
+  b.margin = margin((double)group + 3 + 5 + 3, 16);
   constexpr int per = 16 / (int)sizeof(T);
   if (a.z.cs == 1 && a.z.rs % per == 0 && a.V % per == 0 && (uintptr_t)a.z.p % 16 == 0)
     return run(sample_long_kernel<T, true>, a.M, kLongThreads, 8);
