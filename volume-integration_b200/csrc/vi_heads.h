@@ -191,7 +191,8 @@ struct SampleArgs {
   double temperature_all, top_p_all, min_p_all;
   int64_t top_k_all;
   int64_t* label;            // [M]
-  double scale_all, log2_min_p_all;  // set by the launcher: log2(e) / temperature_all
+  double scale_all, log2_min_p_all, cut_all;  // set by the launcher: log2(e) / temperature_all; their quotient
+  uint32_t* status;          // set by the launcher: the word of the heads' timeouts
   float margin;              // set by the launcher: how near to a border float32 does not decide, of the whole sum
 };
 cudaError_t launch_sample(int dtype, const SampleArgs& a, int sms, cudaStream_t s);

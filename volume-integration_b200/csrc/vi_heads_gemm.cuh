@@ -38,6 +38,7 @@
 
 #include "vi_heads.h"
 #include "vi_heads_math.cuh"
+#include "vi_heads_tma.cuh"
 #include "vi_internal.h"
 
 namespace vi {
@@ -47,7 +48,6 @@ namespace {
 constexpr int kBM = 128, kBK = 64;
 // Terms of a block of k: 128 bytes of a row.
 __host__ __device__ constexpr int block_terms(int epi) { return epi == kEpiInt8 ? 128 : kBK; }
-constexpr int64_t kWaitLimit = 8ll << 30;  // cycles, about 4 s
 
 // Narrow tiles belong to products that memory bounds (few columns, short sums): two
 // blocks per SM, so that one's epilogue runs while the other waits for memory.  A
@@ -112,48 +112,6 @@ struct Args {
   Epilogue e;
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok;
-}
-// Waits for the phase of `parity` to end (each try is suspended for up to 20 us).  False when the
-// block has given up (*dead) or `limit` cycles have gone, which sets *dead.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead, int64_t limit) {
-  if (mbar_try(bar, parity)) return true;
-  const int64_t start = clock64();
-#pragma unroll 1
-  while (!*dead) {
-    if (mbar_try(bar, parity)) return true;
-    if (clock64() - start > limit) *dead = 1;
-  }
-  return false;
-}
-// The same when the block has given up already: only the limit counts.
-__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, int64_t limit) {
-  const int64_t start = clock64();
-#pragma unroll 1
-  while (!mbar_try(bar, parity) && clock64() - start <= limit) {
-  }
-}
-
 // Address of the same shared-memory location in block `rank` of the cluster.
 __device__ __forceinline__ uint32_t at_rank(uint32_t a, uint32_t rank) {
   uint32_t r;
@@ -167,24 +125,6 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-
-// PAIR: the barrier may be the other block's.
-template <bool PAIR>
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
-  if constexpr (PAIR) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
-        "[%2];" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-        : "memory");
-    return;
-  }
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-          dst),
-      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-      : "memory");
 }
 
 // Shared memory by its 32-bit address: a generic pointer would cost 64-bit arithmetic per access.
@@ -1160,21 +1100,6 @@ __global__ void __launch_bounds__(Shape<T, BN, EPI, PL>::kThreads, Shape<T, BN, 
 }
 
 // ---- host ----
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode_fn() {
-  static const EncodeFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return (EncodeFn)p;
-  }();
-  return fn;
-}
-
 constexpr int kInt8 = -1;  // operands of 8-bit integers, k contiguous
 
 // The operand as [plane][outer][inner] with boxes of `box_rows` rows x 128 bytes of k.

@@ -16,11 +16,13 @@
 // guess, made from a sample of the row: one pass over the row keeps them, and shows (by their number, or their share
 // of the mass) that no other label can be kept.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
 #include "vi_heads.h"
 #include "vi_heads_math.cuh"
+#include "vi_heads_tma.cuh"
 #include "vi_internal.h"
 
 namespace vi {
@@ -387,16 +389,11 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : 32 * WARPS) sample_rows_ker
 // finds the largest, the second the sums of 16 pieces of the row, the third walks through the piece that holds the draw.
 // The first reads memory, the others mostly the caches.
 constexpr int kPieces = 16, kImageThreads = 128;
-// A row by a warp in 64 bits, without top-k, top-p and temperature 0: 32 labels at a time, once for the sum and once for the draw.
-template <typename T>
-__device__ __noinline__ int64_t image_row_again(const SampleArgs& a, int64_t row) {
-  const T* p = (const T*)a.z.p + row * a.z.rs;
+// A row by a warp in 64 bits, without top-k, top-p and temperature 0: 32 labels at a time, once for the sum and once for the
+// draw.  at(v): the logit of label v.
+template <typename F>
+__device__ __forceinline__ int row_again(int V, const Setting& s, float best, F at) {
   const int lane = threadIdx.x % 32;
-  const Setting s = setting_of(a, row);
-  float best = -INFINITY;
-  for (int v = lane; v < a.V; v += 32) best = fmaxf(best, to_f(p[v * a.z.cs]));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(kAll, best, o));
   const Weight weight(best, s.scale);
   double run = 0.0, want = 0.0;
   int last = -1;
@@ -404,8 +401,9 @@ __device__ __noinline__ int64_t image_row_again(const SampleArgs& a, int64_t row
   for (int pass = 0; pass < 2; pass++) {
     if (pass) want = s.u * run;
     run = 0.0;
-    for (int first = 0; first < a.V; first += 32) {
-      const float z = first + lane < a.V ? to_f(p[(first + lane) * a.z.cs]) : -INFINITY;
+#pragma unroll 1
+    for (int first = 0; first < V; first += 32) {
+      const float z = first + lane < V ? at(first + lane) : -INFINITY;
       double w = weight.of(z);
       if (w < s.m && z != best) w = 0.0;
       double scan = w;
@@ -421,6 +419,15 @@ __device__ __noinline__ int64_t image_row_again(const SampleArgs& a, int64_t row
     }
   }
   return last;  // u of 1 and more
+}
+template <typename T>
+__device__ __noinline__ int64_t image_row_again(const SampleArgs& a, int64_t row) {
+  const T* p = (const T*)a.z.p + row * a.z.rs;
+  float best = -INFINITY;
+  for (int v = threadIdx.x % 32; v < a.V; v += 32) best = fmaxf(best, to_f(p[v * a.z.cs]));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) best = fmaxf(best, __shfl_xor_sync(kAll, best, o));
+  return row_again(a.V, setting_of(a, row), best, [&](int v) { return to_f(p[v * a.z.cs]); });
 }
 template <typename T, int PX>
 struct Pixels {
@@ -567,144 +574,154 @@ __device__ __forceinline__ uint32_t pair_bits(T a, T b) {
   return (uint32_t) * (const unsigned short*)&a | (uint32_t) * (const unsigned short*)&b << 16;
 }
 
-// The same with the pixel's logits in registers (up to NV labels): memory is read once, with all of a thread's loads in flight.
-// The piece that holds the draw is picked out of them by comparisons.
+// The same from shared memory, where bulk copies reach the image (16-byte strides) and its labels are at most 256: a block
+// takes 256 bytes of each label's pixels, 64 threads with a pixel or a pair of 16-bit ones each.  The copy needs no
+// registers and no address arithmetic, and each pass reads shared memory at constant offsets.
 // Weights beside the largest's: exp2(z scale - best scale), whose constant's rounding is a factor of all alike.
-// The matrix is under 4 GB, so that 32-bit offsets reach all of it.
-template <typename T, int PX, int NV>
-__global__ void __launch_bounds__(kImageThreads) sample_pixels_kernel(const __grid_constant__ SampleArgs a) {
-  constexpr int kLen = 16, kCount = NV / kLen;
-  using Word = typename std::conditional<PX == 2, uint32_t, float>::type;
-  const auto value = [](Word w, int j) -> float {
-    if constexpr (PX == 1) {
-      return w;
-    } else if constexpr (std::is_same<T, __half>::value) {
-      return __half2float(__ushort_as_half((unsigned short)(j ? w >> 16 : w & 0xffffu)));
-    } else {
-      return __uint_as_float(j ? w & 0xffff0000u : w << 16);
-    }
+constexpr int kTileThreads = 64, kTileLabels = 256;
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads) sample_tiles_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ SampleArgs a) {
+  constexpr int PX = 4 / (int)sizeof(T), kLen = 16;
+  constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  extern __shared__ __align__(128) uint32_t words[];  // [labels, whole pieces][threads]
+  const int tid = threadIdx.x, pieces = (a.V + kLen - 1) / kLen;
+  uint32_t* const own = words + tid;
+  float* const runs = (float*)(words + pieces * kLen * kTileThreads) + tid;  // [pieces][PX][threads]
+  __shared__ uint64_t bar_word;
+  __shared__ int dead_word;
+  volatile int* dead = &dead_word;
+  const uint32_t bar = smem_u32(&bar_word);
+  const auto value = [](uint32_t w, int j) -> float {
+    if constexpr (PX == 1) return __uint_as_float(w);
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(j ? w >> 16 : w & 0xffffu)));
+    else return __uint_as_float(j ? w & 0xffff0000u : w << 16);
   };
-  const int64_t step = (int64_t)gridDim.x * kImageThreads * PX;
-  for (int64_t base = (int64_t)blockIdx.x * kImageThreads * PX; base < a.M; base += step) {
-    const int64_t row = base + threadIdx.x * PX;
+  for (int v = a.V; v < pieces * kLen; v++) own[v * kTileThreads] = none;
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    dead_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  uint32_t phase = 0;
+  const int64_t tiles = (a.M + kTileThreads * PX - 1) / (kTileThreads * PX);
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, phase ^= 1) {
+    if (tid == 0) {
+      mbar_expect(bar, a.V * kTileThreads * 4);
+      tma_load<false>(smem_u32(words), &map, bar, (int)(tile * kTileThreads * PX), 0, 0);
+    }
+    if (!mbar_wait(bar, phase, dead, kWaitLimit)) break;
+    const int64_t row = (tile * kTileThreads + tid) * PX;
     uint32_t again = 0;  // pixels that float32 does not decide
-    if (row < a.M) {
-      Word z[NV];
-      {
-        const char* p = (const char*)a.z.p;
-        const uint32_t by = (uint32_t)(a.z.cs * sizeof(T));
-        uint32_t at = (uint32_t)(row * sizeof(T));
+    float best[PX];
+    {
+      uint32_t m[2] = {none, none};
+      for (int c = 0; c < pieces; c++) {
 #pragma unroll
-        for (int v = 0; v < NV; v++, at += by) {
-          if constexpr (PX == 1) z[v] = v < a.V ? to_f(*(const T*)(p + at)) : -INFINITY;
-          else z[v] = v < a.V ? *(const uint32_t*)(p + at) : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        for (int i = 0; i < kLen; i++) {
+          const uint32_t w = own[(c * kLen + i) * kTileThreads];
+          if constexpr (PX == 1) m[i & 1] = __float_as_uint(max_nan(__uint_as_float(m[i & 1]), __uint_as_float(w)));
+          else m[i & 1] = max_nan2(m[i & 1], w, T());
         }
       }
-      float best[PX];
-      if constexpr (PX == 1) {
-        best[0] = z[0];
 #pragma unroll
-        for (int v = 1; v < NV; v++) best[0] = max_nan(best[0], z[v]);
+      for (int j = 0; j < PX; j++) best[j] = max_nan(value(m[0], j), value(m[1], j));
+    }
+    Setting s[PX];
+    bool draws[PX], near[PX], cut = false, any = false;
+    T least[PX];  // min-p keeps the logits from a value on: the type's first value there
+    float scale[PX], shift[PX];
+#pragma unroll
+    for (int j = 0; j < PX; j++) {
+      draws[j] = false;
+      least[j] = from_f<T>(-INFINITY);
+      scale[j] = shift[j] = 0.0f;
+      if (row + j >= a.M) continue;
+      s[j] = setting_of(a, row + j);
+      near[j] = !(s[j].u < 1.0);
+      if (best[j] != best[j] || s[j].t != s[j].t || best[j] == -INFINITY) {
+        a.label[row + j] = -1;
+      } else if (!(s[j].t > 0.0)) {
+        int at = 0;
+        for (int c = pieces - 1; c >= 0; c--) {
+#pragma unroll
+          for (int i = kLen - 1; i >= 0; i--) at = value(own[(c * kLen + i) * kTileThreads], j) == best[j] ? c * kLen + i : at;
+        }
+        a.label[row + j] = at;
+      } else if (!plain_scale(s[j], best[j])) {
+        again |= 1u << j;
       } else {
-        Word m[2] = {z[0], z[1]};
-#pragma unroll
-        for (int v = 2; v < NV; v++) m[v & 1] = max_nan2(m[v & 1], z[v], T());
-        m[0] = max_nan2(m[0], m[1], T());
-#pragma unroll
-        for (int j = 0; j < PX; j++) best[j] = value(m[0], j);
-      }
-      Setting s[PX];
-      bool draws[PX], near[PX], cut = false;
-      T least[PX];  // min-p keeps the logits from a value on: the type's first value there
-#pragma unroll
-      for (int j = 0; j < PX; j++) {
-        s[j] = setting_of(a, row + j);
-        draws[j] = false;
-        near[j] = !(s[j].u < 1.0);
-        least[j] = from_f<T>(-INFINITY);
-        if (best[j] != best[j] || s[j].t != s[j].t || best[j] == -INFINITY) {
-          a.label[row + j] = -1;
-        } else if (!(s[j].t > 0.0)) {
-          int at = 0;
-#pragma unroll
-          for (int v = NV - 1; v >= 0; v--) at = value(z[v], j) == best[j] ? v : at;
-          a.label[row + j] = at;
-        } else if (!plain_scale(s[j], best[j])) {
-          again |= 1u << j;
-        } else {
-          draws[j] = true;
-          if (s[j].m >= 1.0) {
-            least[j] = from_f<T>(best[j]);
-            cut = true;
-          } else if (s[j].m > 0.0) {
-            const double at = (double)best[j] + log2_min_p(a, s[j]) / s[j].scale;
-            double round;
-            if constexpr (sizeof(T) == 4) least[j] = __double2float_ru(at), round = (double)(float)at;
-            else if constexpr (std::is_same<T, __half>::value) least[j] = __float2half_ru(__double2float_ru(at)), round = (double)__half2float(__double2half(at));
-            else least[j] = __float2bfloat16_ru(__double2float_ru(at)), round = (double)__bfloat162float(__double2bfloat16(at));
-            near[j] |= fabs(round - at) <= 1e-12 * (fabs(at) + fabs((double)best[j]));
-            cut = true;
-          }
+        draws[j] = any = true;
+        scale[j] = (float)s[j].scale;
+        shift[j] = -best[j] * scale[j];
+        if (s[j].m >= 1.0) {
+          least[j] = from_f<T>(best[j]);
+          cut = true;
+        } else if (s[j].m > 0.0) {
+          const double at = (double)best[j] + (a.min_p || a.temperature ? log2_min_p(a, s[j]) / s[j].scale : a.cut_all);
+          double round;
+          if constexpr (sizeof(T) == 4) least[j] = __double2float_ru(at), round = (double)(float)at;
+          else if constexpr (std::is_same<T, __half>::value) least[j] = __float2half_ru(__double2float_ru(at)), round = (double)__half2float(__double2half(at));
+          else least[j] = __float2bfloat16_ru(__double2float_ru(at)), round = (double)__bfloat162float(__double2bfloat16(at));
+          near[j] |= fabs(round - at) <= 1e-12 * (fabs(at) + fabs((double)best[j]));
+          cut = true;
         }
       }
-      if (cut) {  // what min-p drops counts as -inf
-        if constexpr (PX == 1) {
+    }
+    uint32_t from;
+    if constexpr (PX == 1) from = __float_as_uint(least[0]);
+    else from = pair_bits(least[0], least[1]);
+    // the word of label v without what min-p drops
+    const auto kept = [&](auto cuts, uint32_t w) {
+      if constexpr (!decltype(cuts)::value) return w;
+      else if constexpr (PX == 1) return __uint_as_float(w) >= __uint_as_float(from) ? w : none;
+      else {
+        const uint32_t in = at_least2(w, from, T());
+        return (w & in) | (none & ~in);
+      }
+    };
+    const auto draw_pixels = [&](auto cuts) {
+      float run[PX] = {};
+      for (int c = 0; c < pieces; c++) {
+        float q[PX][2] = {};
 #pragma unroll
-          for (int v = 0; v < NV; v++) z[v] = z[v] >= to_f(least[0]) ? z[v] : -INFINITY;
-        } else {
-          const uint32_t from = pair_bits(least[0], least[1]), none = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+        for (int i = 0; i < kLen; i++) {
+          const uint32_t w = kept(cuts, own[(c * kLen + i) * kTileThreads]);
 #pragma unroll
-          for (int v = 0; v < NV; v++) {
-            const uint32_t in = at_least2(z[v], from, T());
-            z[v] = (z[v] & in) | (none & ~in);
-          }
+          for (int j = 0; j < PX; j++) q[j][i & 1] += exp2_fast(fmaf(value(w, j), scale[j], shift[j]));
         }
+#pragma unroll
+        for (int j = 0; j < PX; j++) runs[(c * PX + j) * kTileThreads] = run[j] += q[j][0] + q[j][1];
       }
 #pragma unroll
       for (int j = 0; j < PX; j++) {
         if (!draws[j]) continue;
-        const float scale = (float)s[j].scale, shift = -best[j] * scale;
-        const auto weight = [&](Word w) { return exp2_fast(fmaf(value(w, j), scale, shift)); };
-        float run[kCount], sum = 0.0f;
-#pragma unroll
-        for (int c = 0; c < kCount; c++) {
-          float q[2] = {0.0f, 0.0f};
-          if (c * kLen < a.V) {
-#pragma unroll
-            for (int i = 0; i < kLen; i++) q[i & 1] += weight(z[c * kLen + i]);
-          }
-          run[c] = sum += q[0] + q[1];
-        }
-        const float want = (float)s[j].u * sum, slack = sum * a.margin;
+        const float want = (float)s[j].u * run[j], slack = run[j] * a.margin;
         int c = 0;
         float start = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kCount - 1; i++) {
-          const bool behind = run[i] <= want;
+        for (int i = 0; i < pieces - 1; i++) {
+          const float r = runs[(i * PX + j) * kTileThreads];
+          const bool behind = r <= want;
           c += behind;
-          start = behind ? run[i] : start;
-        }
-        Word cell[kLen];
-#pragma unroll
-        for (int i = 0; i < kLen; i++) cell[i] = z[i];
-#pragma unroll
-        for (int k = 1; k < kCount; k++) {
-          const bool here = c == k;
-#pragma unroll
-          for (int i = 0; i < kLen; i++) cell[i] = here ? z[k * kLen + i] : cell[i];
+          start = behind ? r : start;
         }
         bool close = near[j] | (fabsf(start - want) <= slack);
         int at = -1;
         float r = 0.0f;
+        const uint32_t* piece = own + c * kLen * kTileThreads;
 #pragma unroll
         for (int i = 0; i < kLen; i++) {
-          r += weight(cell[i]);
+          r += exp2_fast(fmaf(value(kept(cuts, piece[i * kTileThreads]), j), scale[j], shift[j]));
           close |= fabsf(start + r - want) <= slack;
           at = at < 0 && start + r > want ? c * kLen + i : at;
         }
         if (close || at < 0) again |= 1u << j;
         else a.label[row + j] = at;
       }
+    };
+    if (any) {
+      if (cut) draw_pixels(std::true_type());
+      else draw_pixels(std::false_type());
     }
     // what is left, a warp a row
     __syncwarp();
@@ -714,10 +731,17 @@ __global__ void __launch_bounds__(kImageThreads) sample_pixels_kernel(const __gr
       while (todo) {
         const int l = __ffs(todo) - 1;
         todo &= todo - 1;
-        const int64_t r = __shfl_sync(kAll, row, l) + j, v = image_row_again<T>(a, r);
-        if (threadIdx.x % 32 == 0) a.label[r] = v;
+        const int64_t r = __shfl_sync(kAll, row, l) + j;
+        const uint32_t* column = words + (tid & 32) + l;
+        const int v = row_again(a.V, setting_of(a, r), __shfl_sync(kAll, best[j], l), [&](int v) { return value(column[v * kTileThreads], j); });
+        if (tid % 32 == 0) a.label[r] = v;
       }
     }
+    __syncthreads();
+  }
+  if (tid == 0 && *dead) {  // the copy in flight ends before the block does
+    mbar_drain(bar, phase, kWaitLimit);
+    atomicOr(a.status, VI_DEVICE_HEAD_TIMEOUT);
   }
 }
 
@@ -1251,10 +1275,24 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
   }
 }
 
+// More than 48 KB of shared memory for a kernel, once a device.
+template <auto kernel>
+cudaError_t allow_shared(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (rc == cudaSuccess && dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return rc;
+}
+
 template <typename T>
 cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
   SampleArgs b = a;
   b.scale_all = kLog2e64 / a.temperature_all;
+  b.cut_all = a.min_p_all > 0.0 ? log2(a.min_p_all) / b.scale_all : 0.0;
   b.log2_min_p_all = a.min_p_all > 0.0 ? log2(a.min_p_all) : 0.0;
   int bits = 1;
   while ((1ll << bits) < a.V) bits++;
@@ -1271,20 +1309,33 @@ cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
   const bool image = a.z.rs == 1 && a.z.cs != 1 && a.M > 1;
   if (image && a.V <= 1024 && !a.top_k && !a.top_p && (a.top_k_all <= 0 || a.top_k_all >= a.V) && a.top_p_all >= 1.0) {
     b.margin = margin((a.V + kPieces - 1) / kPieces + kPieces, 0);
-    const auto pixels = [&](auto px) {
-      constexpr int PX = decltype(px)::value;
-      const int64_t units = (a.M + PX * kImageThreads - 1) / (PX * kImageThreads);
-      if (a.V > 160 || (a.V * a.z.cs + a.M) * (int64_t)sizeof(T) >= (1ll << 32)) return run(sample_image_kernel<T, PX>, units, kImageThreads, 64);
-      b.margin = margin(8 + 2 + 16 + 10, 0);
-      return a.V <= 32    ? run(sample_pixels_kernel<T, PX, 32>, units, kImageThreads, 64)
-             : a.V <= 64  ? run(sample_pixels_kernel<T, PX, 64>, units, kImageThreads, 64)
-             : a.V <= 96  ? run(sample_pixels_kernel<T, PX, 96>, units, kImageThreads, 64)
-             : a.V <= 128 ? run(sample_pixels_kernel<T, PX, 128>, units, kImageThreads, 64)
-                          : run(sample_pixels_kernel<T, PX, 160>, units, kImageThreads, 64);
-    };
+    constexpr int PX = 4 / (int)sizeof(T);
+    if (a.V <= kTileLabels && a.z.cs * (int64_t)sizeof(T) % 16 == 0 && (uintptr_t)a.z.p % 16 == 0 && a.z.cs >= a.M) {
+      CUtensorMap map;
+      EncodeFn fn = encode_fn();
+      const cuuint64_t dims[3] = {(cuuint64_t)a.M, (cuuint64_t)a.V, 1}, strides[2] = {(cuuint64_t)a.z.cs * sizeof(T), (cuuint64_t)a.z.cs * sizeof(T)};
+      const cuuint32_t box[3] = {(cuuint32_t)(kTileThreads * PX), (cuuint32_t)a.V, 1}, unit[3] = {1, 1, 1};
+      b.status = status_word();
+      if (fn && b.status &&
+          fn(&map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(a.z.p), dims, strides, box,
+             unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS) {
+        const int pieces = (a.V + 15) / 16;
+        const int smem = pieces * (16 + PX) * kTileThreads * 4;
+        b.margin = margin(8 + 2 + 16 + 16, 0);
+        cudaError_t rc = cudaSuccess;
+        if (smem > 48 * 1024) rc = allow_shared<sample_tiles_kernel<T>>(kTileLabels / 16 * (16 + PX) * kTileThreads * 4);
+        if (rc != cudaSuccess) return rc;
+        const int64_t tiles = (a.M + kTileThreads * PX - 1) / (kTileThreads * PX);
+        const int per_sm = std::min(16, 220 * 1024 / (smem + 1100));
+        sample_tiles_kernel<T><<<(unsigned)std::min<int64_t>(tiles, (int64_t)sms * per_sm), kTileThreads, smem, s>>>(map, b);
+        return cudaPeekAtLastError();
+      }
+    }
     if constexpr (sizeof(T) == 2)
-      if (a.M % 2 == 0 && a.z.cs % 2 == 0 && (uintptr_t)a.z.p % 4 == 0) return pixels(std::integral_constant<int, 2>());
-    return pixels(std::integral_constant<int, 1>());
+      if (a.M % 2 == 0 && a.z.cs % 2 == 0 && (uintptr_t)a.z.p % 4 == 0)
+        return run(sample_image_kernel<T, 2>, (a.M + 2 * kImageThreads - 1) / (2 * kImageThreads), kImageThreads, 64);
+    return run(sample_image_kernel<T, 1>, (a.M + kImageThreads - 1) / kImageThreads, kImageThreads, 64);
   }
   if (a.V <= 256) {
     b.margin = margin(8 + 5, 0);
