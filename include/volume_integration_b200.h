@@ -455,8 +455,9 @@ typedef struct vi_sampling {
   const int64_t* top_ks;
   const float *top_ps, *min_ps;
 } vi_sampling;
+uint64_t vi_sample_labels_scratch_bytes(int dtype, const vi_matrix* logits, const vi_sampling* settings);
 int vi_sample_labels(int dtype, const vi_matrix* logits, const float* u, const vi_sampling* settings, int64_t* label,
-                     void* stream);
+                     void* scratch, uint64_t scratch_bytes, void* stream);
 
 /*
  * The current device's status word of the heads' matrix products: 0, or

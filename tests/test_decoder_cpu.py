@@ -31,7 +31,9 @@ def _lib():
     lib.vi_linear_act_int8_scratch_bytes.argtypes = [i, i, m, P, m, P, P, m, m]
     lib.vi_linear_act_int8_scratch_bytes.restype = u64
     lib.vi_linear_act_int8.argtypes = [i, i, m, P, m, P, P, m, m, P, u64, P]
-    lib.vi_sample_labels.argtypes = [i, m, P, ctypes.POINTER(Sampling), P, P]
+    lib.vi_sample_labels_scratch_bytes.argtypes = [i, m, ctypes.POINTER(Sampling)]
+    lib.vi_sample_labels_scratch_bytes.restype = u64
+    lib.vi_sample_labels.argtypes = [i, m, P, ctypes.POINTER(Sampling), P, P, u64, P]
     return lib
 
 
@@ -167,8 +169,17 @@ def test_c_abi_refusals():
         (2, x, dict(top_p=0.0), vec, b"top_p"), (2, x, dict(min_p=2.0), vec, b"min_p"), (2, x, {}, None, b"need data"),
     ]:
         s = Sampling(**{**ok, **change})
-        assert lib.vi_sample_labels(dt, z, u, ctypes.byref(s), vec, None) == 1
+        assert lib.vi_sample_labels(dt, z, u, ctypes.byref(s), vec, None, 0, None) == 1
         assert text in lib.vi_last_error(), (text, lib.vi_last_error())
+        if u:
+            assert lib.vi_sample_labels_scratch_bytes(dt, z, ctypes.byref(s)) == 0
+    s = Sampling(**ok)
+    assert lib.vi_sample_labels_scratch_bytes(2, x, ctypes.byref(s)) == 256
+    long = _m(6, 60000, 60000, 1)
+    n = lib.vi_sample_labels_scratch_bytes(2, long, ctypes.byref(s))
+    assert n > 6 * 4096
+    assert lib.vi_sample_labels(2, long, vec, ctypes.byref(s), vec, vec, n // 2, None) == 1
+    assert b"scratch" in lib.vi_last_error()
 
 
 @pytest.mark.parametrize("affine", [False, True])

@@ -816,7 +816,10 @@ Tensor sample_labels(const Tensor& logits, const Tensor& u, double temperature, 
   const vi_sampling s{temperature, top_p, min_p, top_k, f32(t), k.defined() ? k.data_ptr<int64_t>() : nullptr, f32(p), f32(m)};
   Tensor label = torch::empty({logits.size(0)}, logits.options().dtype(torch::kInt64));
   const vi_matrix mz = head_matrix(logits);
-  ok(vi_sample_labels(dt, &mz, v.data_ptr<float>(), &s, label.data_ptr<int64_t>(), at::cuda::getCurrentCUDAStream().stream()));
+  const uint64_t n = vi_sample_labels_scratch_bytes(dt, &mz, &s);
+  Tensor scratch = head_scratch(n, logits);
+  ok(vi_sample_labels(dt, &mz, v.data_ptr<float>(), &s, label.data_ptr<int64_t>(), head_ptr(scratch), n,
+                      at::cuda::getCurrentCUDAStream().stream()));
   return label;
 }
 

@@ -1226,13 +1226,38 @@ int sample_labels(Run& r, int dtype, const vi_matrix* z, const float* u, const v
   if (!s->top_ks && s->top_k < 0) return bad("sample_labels: top_k must be at least 0");
   if (!s->top_ps && !(s->top_p > 0.0)) return bad("sample_labels: top_p must be above 0");
   if (!s->min_ps && !(s->min_p >= 0.0 && s->min_p <= 1.0)) return bad("sample_labels: min_p must lie in [0, 1]");
-  if (z->rows == 0 || r.dry) return VI_OK;
-  if (!z->data || !u || !label) return bad("sample_labels: logits, u and label need data");
-  SampleArgs a{z->rows,       (int)z->cols, view(z),     u,          s->temperatures, s->top_ks, s->top_ps,
-               s->min_ps,     s->temperature, s->top_p,  s->min_p,   s->top_k,        label};
-  const cudaError_t rc = launch_sample(dtype, a, r.sms, r.s);
-  r.launches++;
-  return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+  if (z->rows == 0) return VI_OK;
+  if (!z->data || (!r.dry && (!u || !label))) return bad("sample_labels: logits, u and label need data");
+  // long rows keep candidates: as many rows at a time as fill the device many times over
+  constexpr int64_t kRows = 16384;
+  const uint64_t bytes = sample_scratch(std::min(z->rows, kRows), z->cols, r.sms);
+  void* scratch = bytes ? r.take(bytes) : nullptr;
+  if (r.dry) return VI_OK;
+  const int64_t step = bytes ? kRows : z->rows;
+  const size_t es = elem(dtype);
+  for (int64_t m = 0; m < z->rows; m += step) {
+    const auto from = [&](auto* p) { return p ? p + m : nullptr; };
+    SampleArgs a{};
+    a.M = std::min(step, z->rows - m);
+    a.V = (int)z->cols;
+    a.z = view(z);
+    a.z.p = (char*)a.z.p + m * a.z.rs * es;
+    a.u = u + m;
+    a.temperature = from(s->temperatures);
+    a.top_k = from(s->top_ks);
+    a.top_p = from(s->top_ps);
+    a.min_p = from(s->min_ps);
+    a.temperature_all = s->temperature;
+    a.top_p_all = s->top_p;
+    a.min_p_all = s->min_p;
+    a.top_k_all = s->top_k;
+    a.label = label + m;
+    a.scratch = scratch;
+    const cudaError_t rc = launch_sample(dtype, a, r.sms, r.s);
+    r.launches += bytes ? 2 : 1;
+    if (rc != cudaSuccess) return set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
+  }
+  return VI_OK;
 }
 
 }  // namespace
@@ -1279,9 +1304,14 @@ extern "C" int vi_linear_act_int8(int dtype, int activation, const vi_matrix* x,
       scratch_bytes, stream, "linear_act_int8");
 }
 
+extern "C" uint64_t vi_sample_labels_scratch_bytes(int dtype, const vi_matrix* logits, const vi_sampling* settings) {
+  return count_bytes([&](Run& r) { return sample_labels(r, dtype, logits, nullptr, settings, nullptr); });
+}
+
 extern "C" int vi_sample_labels(int dtype, const vi_matrix* logits, const float* u, const vi_sampling* settings, int64_t* label,
-                                void* stream) {
-  return execute([&](Run& r) { return sample_labels(r, dtype, logits, u, settings, label); }, nullptr, 0, stream, "sample_labels");
+                                void* scratch, uint64_t scratch_bytes, void* stream) {
+  return execute([&](Run& r) { return sample_labels(r, dtype, logits, u, settings, label); }, scratch, scratch_bytes, stream,
+                 "sample_labels");
 }
 
 extern "C" uint64_t vi_linear_act_forward_scratch_bytes(int dtype, int activation, const vi_matrix* x,

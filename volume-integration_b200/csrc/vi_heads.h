@@ -192,9 +192,13 @@ struct SampleArgs {
   int64_t top_k_all;
   int64_t* label;            // [M]
   double scale_all, log2_min_p_all, cut_all;  // set by the launcher: log2(e) / temperature_all; their quotient
+  void* scratch;             // sample_scratch() bytes
+  int64_t list_at, list_bytes;  // set by the launcher: where the rows' candidates lie in it
   uint32_t* status;          // set by the launcher: the word of the heads' timeouts
   float margin;              // set by the launcher: how near to a border float32 does not decide, of the whole sum
+  float margin_far;          // set by the launcher: more of it by octaves between the guessed and the true largest
 };
+uint64_t sample_scratch(int64_t M, int64_t V, int sms);
 cudaError_t launch_sample(int dtype, const SampleArgs& a, int sms, cudaStream_t s);
 
 // Layer norm of rows (vi_norm.cu).

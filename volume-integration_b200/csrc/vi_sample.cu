@@ -133,6 +133,20 @@ struct Team {
     }
     return v;
   }
+  __device__ __forceinline__ float sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    if constexpr (WARPS > 1) {
+      if (lane == 0) sh.u[turn][warp] = __float_as_uint(v);
+      __syncthreads();
+      v = lane < WARPS ? __uint_as_float(sh.u[turn][lane]) : 0.0f;
+#pragma unroll
+      for (int o = WARPS / 2; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+      v = __shfl_sync(kAll, v, 0);
+      turn ^= 1;
+    }
+    return v;
+  }
   __device__ __forceinline__ double sum(double v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
@@ -277,14 +291,35 @@ __device__ __forceinline__ int draw(Team<WARPS>& team, const float (&z)[E], floa
     const double want = fmax(s.p * all, 1e-300);
     slack *= s.p;
     if (all_known && !(mass(0) + at_low - want > slack)) return kUnsure;
+    // in float32, and again in 64 bits where that gives another threshold than 64 bits would
     uint32_t cut = common;
+    {
+      float f[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) f[e] = o[e] > low ? (float)w[e] : 0.0f;
+      const float about = (float)want;
 #pragma unroll 1
-    for (int bit = start; bit >= 0; bit--) {
-      const uint32_t c = cut | 1u << bit;
-      if (c <= low || mass(c) >= want) cut = c;
+      for (int bit = start; bit >= 0; bit--) {
+        const uint32_t c = cut | 1u << bit;
+        float v = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) v += o[e] >= c ? f[e] : 0.0f;
+        if (c <= low || team.sum(v) >= about) cut = c;
+      }
+      cut = max(cut, low);
     }
-    cut = max(cut, low);
-    const double above = mass(cut + 1), one = cut ? weight.of(O::value(cut)) : 0.0;
+    double above = mass(cut + 1);
+    if (!((cut == low || mass(cut) >= want) && above < want)) {
+      cut = common;
+#pragma unroll 1
+      for (int bit = start; bit >= 0; bit--) {
+        const uint32_t c = cut | 1u << bit;
+        if (c <= low || mass(c) >= want) cut = c;
+      }
+      cut = max(cut, low);
+      above = mass(cut + 1);
+    }
+    const double one = cut ? weight.of(O::value(cut)) : 0.0;
     uint32_t have = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) have += o[e] == cut;
@@ -746,25 +781,62 @@ __global__ void __launch_bounds__(kTileThreads) sample_tiles_kernel(const __grid
 }
 
 // ---- long rows: a block a row ----
-constexpr int kLongWarps = 8, kLongThreads = 256, kHeld = 16;
+constexpr int kRowLabels = 8192;               // that a block's registers hold
+constexpr int kHeld = 16;
 constexpr int kListWarp = 32 * kHeld;          // candidates a warp keeps
-constexpr int kSample = 16;                    // labels a lane looks at for the guess
+constexpr int kSample = 32;                    // labels a lane looks at for the guess
 constexpr int kSums = 64;                      // sums of steps a warp keeps
 constexpr int kBins = 256;
-constexpr int kBatch = 4;                      // steps whose loads are in flight together
 constexpr int kFew = 256;                      // candidates that one warp draws from
+template <int W>
 struct LongShared {
   TeamShared team;
-  int at[kLongWarps][kListWarp];
-  float sums[kLongWarps][kSums];
+  union {
+    float sums[W][kSums];
+    double mass[W][kSums];
+  };
+  uint32_t equal[W][kSums];
   uint32_t bins[kBins];
   int few[kFew];
   float guess;
   int answer;
 };
+// What the passes over a row leave for the draw.
+enum { kDone, kFromList, kWhole };
+struct RowNote {
+  double all;       // mass beside exp2(ref scale)
+  float best, ref;
+  int state;
+  int n[16];        // candidates of each warp
+  int pad[3];
+};
+__host__ __device__ constexpr int64_t list_bytes(int warps) { return (int64_t)warps * kListWarp * 4; }
+__device__ __forceinline__ int* list_of(const SampleArgs& a, int64_t row) { return (int*)((char*)a.scratch + a.list_at + row * a.list_bytes); }
 
-// What a lane holds of 256 labels from `first` on: 8 in a row (VEC: loaded as vectors), or every 32nd.
-template <typename T, bool VEC>
+// How a row is read: any stride, or contiguous, in 16-byte vectors.
+enum { kStrided, kVectors };
+
+// A row whose labels are counted from the 16-byte boundary at or before its first one (kVectors): label v has place v + shift.
+template <typename T, int MODE>
+struct Row {
+  const T* p;  // of place 0, which is not read where shift is not 0
+  int64_t cs;
+  int shift, end;
+  __device__ __forceinline__ Row(const SampleArgs& a, int64_t row) {
+    p = (const T*)a.z.p + row * a.z.rs;
+    cs = a.z.cs;
+    shift = MODE == kVectors ? (int)((uintptr_t)p % 16 / sizeof(T)) : 0;
+    p -= shift;
+    end = a.V + shift;
+  }
+  __device__ __forceinline__ float at(int place) const { return to_f(p[MODE == kVectors ? (int64_t)place : place * cs]); }
+};
+// Steps of 256 places of each of W warps.
+template <int W, typename T>
+__host__ __device__ constexpr int64_t part_of(int64_t V) { return (V + 16 / (int)sizeof(T) + W * 256 - 1) / (W * 256) * 256; }
+
+// What a lane holds of 256 places from `first` on: 8 in a row (kVectors), or every 32nd; -inf where there is no label.
+template <typename T, int MODE>
 struct Step {
   static constexpr int kPer = 16 / (int)sizeof(T);
   union {
@@ -773,27 +845,34 @@ struct Step {
   };
   __device__ __forceinline__ Step() {}
   __device__ __forceinline__ float z(int e) const { return to_f(t[e]); }
-  static __device__ __forceinline__ int place(int first, int lane, int e) { return VEC ? first + lane * 8 + e : first + e * 32 + lane; }
-  // ends at `end`; with VEC whole vectors lie on one side of it
-  __device__ __forceinline__ void load(const T* p, int64_t cs, int first, int lane, int end) {
-    if constexpr (VEC) {
-      constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  static __device__ __forceinline__ int place(int first, int lane, int e) { return MODE == kVectors ? first + lane * 8 + e : first + e * 32 + lane; }
+  __device__ __forceinline__ void load(const Row<T, MODE>& r, int first, int lane, int end) {
+    if constexpr (MODE == kVectors) {
+      if (first + 256 <= end && first >= kPer) {
+#pragma unroll
+        for (int i = 0; i < 8 / kPer; i++) q[i] = ((const uint4*)(r.p + first + lane * 8))[i];
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < 8 / kPer; i++) {
         const int v = first + lane * 8 + i * kPer;
-        q[i] = v < end ? *(const uint4*)(p + v) : make_uint4(none, none, none, none);
+        if (v >= r.shift && v + kPer <= end) {
+          q[i] = *(const uint4*)(r.p + v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kPer; e++) t[i * kPer + e] = v + e >= r.shift && v + e < end ? r.p[v + e] : from_f<T>(-INFINITY);
+        }
       }
     } else {
+      const T* at = r.p + (first + lane) * r.cs;
+      const int64_t step = 32 * r.cs;
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int v = first + e * 32 + lane;
-        t[e] = v < end ? p[v * cs] : from_f<T>(-INFINITY);
-      }
+      for (int e = 0; e < 8; e++) t[e] = first + e * 32 + lane < end ? at[e * step] : from_f<T>(-INFINITY);
     }
   }
   // The largest, or a NaN if there is one.
   __device__ __forceinline__ float most(float m) const {
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4 || MODE != kVectors) {
 #pragma unroll
       for (int e = 0; e < 8; e++) m = max_nan(m, z(e));
       return m;
@@ -806,7 +885,7 @@ struct Step {
   // Bit e: whether value e is at least `from`.
   __device__ __forceinline__ uint32_t at_least(float from, uint32_t from2) const {
     uint32_t in = 0;
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4 || MODE != kVectors) {
 #pragma unroll
       for (int e = 0; e < 8; e++) in |= z(e) >= from ? 1u << e : 0u;
     } else {
@@ -820,13 +899,13 @@ struct Step {
 };
 
 // f of every label of a row and of some -inf, in any order: several loads in flight.
-template <typename T, bool VEC, typename F>
-__device__ __forceinline__ void each_of_row(const T* p, int64_t cs, int V, int warp, int lane, F f) {
-  constexpr int kDeep = 4;
-  for (int first = warp * 256; first < V; first += kDeep * kLongThreads * 8) {
-    Step<T, VEC> x[kDeep];
+template <int W, typename T, int MODE, typename F>
+__device__ __forceinline__ void each_of_row(const Row<T, MODE>& row, int warp, int lane, F f) {
+  constexpr int kDeep = sizeof(T) == 4 ? 2 : 4;
+  for (int first = warp * 256; first < row.end; first += kDeep * W * 256) {
+    Step<T, MODE> x[kDeep];
 #pragma unroll
-    for (int i = 0; i < kDeep; i++) x[i].load(p, cs, first + i * kLongThreads * 8, lane, V);
+    for (int i = 0; i < kDeep; i++) x[i].load(row, first + i * W * 256, lane, row.end);
 #pragma unroll
     for (int i = 0; i < kDeep; i++) {
 #pragma unroll
@@ -836,32 +915,29 @@ __device__ __forceinline__ void each_of_row(const T* p, int64_t cs, int V, int w
 }
 
 // The whole row by the definition in 64 bits, read again for every step of the bisections: where the guess was
-// wrong, or candidates are too many to be held.
-template <typename T, bool VEC>
-__device__ __noinline__ int whole_row(Team<kLongWarps>& team, LongShared& sh, const SampleArgs& a, const T* p, float best, const Setting& s) {
+// wrong, or candidates are too many to be held; and where float32 leaves a plain draw in doubt.
+template <int W, typename T, int MODE>
+__device__ __noinline__ int whole_row(Team<W>& team, LongShared<W>& sh, const Row<T, MODE>& row, int V, float best, const Setting& s) {
   using O = Order<T>;
   const Weight weight(best, s.scale);
-  const int tid = threadIdx.x, V = a.V;
-  const int64_t cs = a.z.cs;
+  const int warp = team.warp, lane = team.lane;
   const bool greedy = !(s.t > 0.0);
   uint32_t low = greedy ? O::of(best) : 0, ties = greedy ? 1 : kManyTies;
-  const auto each = [&](auto f) {
-    each_of_row<T, VEC>(p, cs, V, tid / 32, tid % 32, f);
-  };
+  const auto each = [&](auto f) { each_of_row<W, T, MODE>(row, warp, lane, f); };
   const auto count = [&](auto f) {
     uint32_t n = 0;
     each([&](float z) { n += f(O::of(z)); });
     return team.sum(n);
   };
-  const auto mass = [&](uint32_t from, uint32_t to) {  // orders in [from, to)
+  const auto mass = [&](uint32_t from) {  // of what is above low, from `from` on
     double m = 0.0;
     each([&](float z) {
       const uint32_t o = O::of(z);
-      if (o >= from && o < to) m += weight.of(z);
+      const double w = weight.of(z);
+      m += o >= from && o > low ? w : 0.0;
     });
     return team.sum(m);
   };
-  const uint32_t end = O::of(best) + 1;
   if (!greedy && s.k > 0 && s.k < V) {
     for (int bit = O::kBits - 1; bit >= 0; bit--) {
       const uint32_t c = low | 1u << bit;
@@ -870,151 +946,244 @@ __device__ __noinline__ int whole_row(Team<kLongWarps>& team, LongShared& sh, co
     ties = (uint32_t)(s.k - count([&](uint32_t o) { return o > low; }));
   }
   if (!greedy && s.p < 1.0) {
-    const uint32_t n = min(count([&](uint32_t o) { return o == low; }), ties);
-    const double at_low = n ? n * weight.of(O::value(low)) : 0.0;
-    const double want = fmax(s.p * (mass(low + 1, end) + at_low), 1e-300);
-    uint32_t cut = 0, top = end;
-    double above = 0.0;  // mass from `top` on; the threshold lies under it
-    for (int bit = O::kBits - 1; bit >= 0; bit--) {
-      const uint32_t c = cut | 1u << bit;
-      if (c >= top) continue;
-      if (c <= low) {
-        cut = c;
-        continue;
+    const uint32_t end = O::of(best), n_low = low ? min(count([&](uint32_t o) { return o == low; }), ties) : 0;
+    const double at_low = n_low ? n_low * weight.of(O::value(low)) : 0.0;
+    uint32_t cut = 0, have = 0;
+    double want = 0.0, above = 0.0;
+    bool found = false;
+    // the threshold's own label count, the mass above it and the whole, in one pass of 64 bits: does the threshold stand?
+    const auto stands = [&] {
+      double whole = 0.0, front = 0.0;
+      uint32_t n = 0;
+      each([&](float z) {
+        const uint32_t o = O::of(z);
+        const double w = o > low ? weight.of(z) : 0.0;
+        whole += w;
+        front += o > cut ? w : 0.0;
+        n += o == cut;
+      });
+      want = fmax(s.p * (team.sum(whole) + at_low), 1e-300);
+      above = team.sum(front);
+      have = team.sum(n);
+      if (cut == low) have = min(have, ties);
+      return above < want && (cut == low || above + have * weight.of(O::value(cut)) >= want);
+    };
+    if (plain_scale(s, best)) {  // in float32 first
+      const float scale = (float)s.scale, shift = -best * scale;
+      const auto mass32 = [&](uint32_t from) {
+        float m = 0.0f;
+        each([&](float z) {
+          const uint32_t o = O::of(z);
+          m += o >= from && o > low ? exp2_fast(fmaf(z, scale, shift)) : 0.0f;
+        });
+        return team.sum(m);
+      };
+      const float about = (float)s.p * (mass32(0) + (float)at_low);
+      for (int bit = O::kBits - 1; bit >= 0; bit--) {
+        const uint32_t c = cut | 1u << bit;
+        if (c <= end && (c <= low || mass32(c) >= about)) cut = c;
       }
-      const double m = above + mass(c, top);
-      if (m >= want) cut = c;
-      else above = m, top = c;
+      cut = max(cut, low);
+      found = stands();
     }
-    cut = max(cut, low);
-    above += mass(cut + 1, top);
-    uint32_t have = count([&](uint32_t o) { return o == cut; });
-    if (cut == low) have = min(have, ties);
+    if (!found) {
+      cut = 0;
+      stands();  // for `want`
+      for (int bit = O::kBits - 1; bit >= 0; bit--) {
+        const uint32_t c = cut | 1u << bit;
+        if (c <= end && (c <= low || mass(c) >= want)) cut = c;
+      }
+      cut = max(cut, low);
+      stands();
+    }
     const double one = cut ? weight.of(O::value(cut)) : 0.0, need = one > 0.0 ? ceil((want - above) / one) : (double)have;
     ties = (uint32_t)fmin(fmax(need, 1.0), (double)have);
     low = cut;
   }
-  // in index order: a warp a part of the row, step by step, once for the sum and once for the draw
-  const int part = (V + kLongWarps * 256 - 1) / (kLongWarps * 256) * 256, v0 = min(V, team.warp * part), v1 = min(V, v0 + part);
-  uint32_t equal = 0;
-  Step<T, VEC> x;
-  for (int first = v0; first < v1; first += 256) {
-    x.load(p, cs, first, team.lane, v1);
+  // in index order: a warp a part of the row.  Of each group of its steps the mass above the threshold, and how many labels
+  // are equal to it
+  const int part = (int)part_of<W, T>(V), v0 = min(row.end, warp * part), v1 = min(row.end, v0 + part);
+  const int steps = part / 256, group = (steps + kSums - 1) / kSums;
+  const auto enough = [&](double w, float z) { return greedy || !(w < s.m) || z == best; };
+  const float z_low = low ? O::value(low) : -INFINITY;
+  double w_low = weight.of(z_low);
+  if (!enough(w_low, z_low)) w_low = 0.0;
+  const bool limited = low > 0;
+  for (int g = lane; g < kSums; g += 32) sh.mass[warp][g] = 0.0, sh.equal[warp][g] = 0;
+  __syncwarp();
+  Step<T, MODE> next;
+  next.load(row, v0, lane, v1);
+  for (int i0 = 0; i0 < steps && v0 + i0 * 256 < v1; i0 += group) {
+    double m = 0.0;
+    uint32_t n = 0;
+    for (int i = i0; i < min(steps, i0 + group) && v0 + i * 256 < v1; i++) {
+      const Step<T, MODE> x = next;
+      next.load(row, v0 + (i + 1) * 256, lane, v1);
 #pragma unroll
-    for (int e = 0; e < 8; e++) equal += O::of(x.z(e)) == low;
+      for (int e = 0; e < 8; e++) {
+        const float z = x.z(e);
+        const uint32_t o = O::of(z);
+        const double w = weight.of(z);
+        m += o > low && enough(w, z) ? w : 0.0;
+        n += o == low;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m += __shfl_xor_sync(kAll, m, o);
+    n = __reduce_add_sync(kAll, n);
+    if (lane == 0) sh.mass[warp][i0 / group] = m, sh.equal[warp][i0 / group] = limited ? n : 0;
+  }
+  __syncwarp();
+  // groups 2 lane and 2 lane + 1: equal ones in front of them, then running masses
+  static_assert(kSums == 64, "two groups a lane");
+  const uint32_t n0 = sh.equal[warp][2 * lane], n1 = sh.equal[warp][2 * lane + 1];
+  uint32_t scan = n0 + n1;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t t = __shfl_up_sync(kAll, scan, d);
+    if (lane >= d) scan += t;
   }
   uint32_t ahead;
-  team.ahead(__reduce_add_sync(kAll, equal), ahead);
-  // the lanes' running sums of a step's kept weights (r, from `run` on; the step's end in run), with each label's weight
-  const auto walk = [&](int first, uint32_t& seen, double& run, double (&r)[8], double (&w)[8]) {
-    x.load(p, cs, first, team.lane, v1);
-    const auto kept = [&](float z, uint32_t rank) {
-      const uint32_t o = O::of(z);
-      if (!(o > low || (o == low && rank < ties))) return 0.0;
-      const double q = weight.of(z);
-      return greedy || !(q < s.m) || z == best ? q : 0.0;
-    };
-    if constexpr (VEC) {
-      uint32_t n = 0;
+  team.ahead(__shfl_sync(kAll, scan, 31), ahead);
+  const uint32_t e0 = ahead + scan - n0 - n1, e1 = e0 + n0;
+  const auto some = [&](uint32_t from, uint32_t n) { return (double)(min(ties, from + n) - min(ties, from)) * w_low; };
+  const double m0 = sh.mass[warp][2 * lane] + some(e0, n0), m1 = sh.mass[warp][2 * lane + 1] + some(e1, n1);
+  double run = m0 + m1;
 #pragma unroll
-      for (int e = 0; e < 8; e++) n += O::of(x.z(e)) == low;
-      uint32_t rank = n;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t t = __shfl_up_sync(kAll, rank, d);
-        if (team.lane >= d) rank += t;
-      }
-      const uint32_t all = __shfl_sync(kAll, rank, 31);
-      rank += seen - n;
-      seen += all;
-      double sum = 0.0;
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        w[e] = kept(x.z(e), rank);
-        rank += O::of(x.z(e)) == low;
-        r[e] = sum += w[e];
-      }
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const double t = __shfl_up_sync(kAll, sum, d);
-        if (team.lane >= d) sum += t;
-      }
-      const double front = __shfl_up_sync(kAll, sum, 1);
-#pragma unroll
-      for (int e = 0; e < 8; e++) r[e] += run + (team.lane ? front : 0.0);
-      run += __shfl_sync(kAll, sum, 31);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const uint32_t b = __ballot_sync(kAll, O::of(x.z(e)) == low);
-        w[e] = kept(x.z(e), seen + __popc(b & ((1u << team.lane) - 1)));
-        seen += __popc(b);
-        double sum = w[e];
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const double t = __shfl_up_sync(kAll, sum, d);
-          if (team.lane >= d) sum += t;
-        }
-        r[e] = run + sum;
-        run += __shfl_sync(kAll, sum, 31);
-      }
-    }
-  };
-  double run = 0.0, r[8], w[8], before, total;
-  uint32_t seen = ahead;
-  for (int first = v0; first < v1; first += 256) walk(first, seen, run, r, w);
-  const double mine = run;
+  for (int d = 1; d < 32; d <<= 1) {
+    const double t = __shfl_up_sync(kAll, run, d);
+    if (lane >= d) run += t;
+  }
+  const double mine = __shfl_sync(kAll, run, 31);
+  double before, total;
   team.ahead(mine, before, total);
-  const double want = s.u * total;
+  const double want = s.u < 1.0 ? s.u * total : INFINITY;
+  // the warp whose part holds the draw (u of 1 and more: every warp, for its last label)
   uint32_t hit = 0, last = 0;
-  if (before + mine > want || !(total > want)) {
-    run = before;
-    seen = ahead;
-    for (int first = v0; first < v1 && !hit; first += 256) {
-      walk(first, seen, run, r, w);
+  if (mine > 0.0 && ((before <= want && before + mine > want) || !(s.u < 1.0))) {
+    const double f0 = before + run - m1 - m0, f1 = before + run - m1;  // in front of the lane's groups
+    const uint32_t holds = __ballot_sync(kAll, (f1 > want && m0 > 0.0) || (before + run > want && m1 > 0.0));
+    const uint32_t some_mass = __ballot_sync(kAll, m0 + m1 > 0.0);
+    const int l = holds ? __ffs(holds) - 1 : 31 - __clz(some_mass);
+    for (int half = 0; half < 2 && !hit; half++) {
+      const int g = 2 * l + half;
+      double r = __shfl_sync(kAll, half ? f1 : f0, l);
+      uint32_t seen = __shfl_sync(kAll, half ? e1 : e0, l);
+      for (int i = g * group; i < min(steps, (g + 1) * group) && v0 + i * 256 < v1 && !hit; i++) {
+        Step<T, MODE> x;
+        const int first = v0 + i * 256;
+        x.load(row, first, lane, v1);
+        double w[8], sum = 0.0, front = 0.0;
+        if constexpr (MODE == kVectors) {  // a lane's labels lie in a row
+          uint32_t n = 0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const uint32_t v = Step<T, VEC>::place(first, team.lane, e);
-        if (w[e] > 0.0) last = max(last, v + 1);
-        if (w[e] > 0.0 && r[e] > want) hit = max(hit, ~v);
+          for (int e = 0; e < 8; e++) n += limited && O::of(x.z(e)) == low;
+          uint32_t rank = n;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t t = __shfl_up_sync(kAll, rank, d);
+            if (lane >= d) rank += t;
+          }
+          const uint32_t all = __shfl_sync(kAll, rank, 31);
+          rank += seen - n;
+          seen += all;
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float z = x.z(e);
+            const uint32_t o = O::of(z);
+            const double q = weight.of(z);
+            w[e] = (o > low && enough(q, z)) ? q : limited && o == low && rank < ties ? w_low : 0.0;
+            rank += limited && o == low;
+            sum += w[e];
+          }
+          front = sum;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const double t = __shfl_up_sync(kAll, front, d);
+            if (lane >= d) front += t;
+          }
+          const double all_sum = __shfl_sync(kAll, front, 31);
+          front = __shfl_up_sync(kAll, front, 1);
+          double q = r + (lane ? front : 0.0);
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            q += w[e];
+            if (w[e] > 0.0) {
+              const uint32_t v = first + lane * 8 + e;
+              last = max(last, v + 1);
+              if (q > want) hit = max(hit, ~v);
+            }
+          }
+          r += all_sum;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float z = x.z(e);
+            const uint32_t o = O::of(z), b = __ballot_sync(kAll, limited && o == low);
+            const double q = weight.of(z);
+            w[e] = (o > low && enough(q, z)) ? q : (b >> lane & 1) && seen + __popc(b & ((1u << lane) - 1)) < ties ? w_low : 0.0;
+            seen += __popc(b);
+            sum = w[e];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+              const double t = __shfl_up_sync(kAll, sum, d);
+              if (lane >= d) sum += t;
+            }
+            if (w[e] > 0.0) {
+              const uint32_t v = first + e * 32 + lane;
+              last = max(last, v + 1);
+              if (r + sum > want) hit = max(hit, ~v);
+            }
+            r += __shfl_sync(kAll, sum, 31);
+          }
+        }
+        hit = __reduce_max_sync(kAll, hit);
       }
-      hit = __reduce_max_sync(kAll, hit);
     }
+    last = __reduce_max_sync(kAll, last);
+    // by their sums the groups hold the draw, though running sums added in another order stay under it
+    if (!hit && s.u < 1.0 && last) hit = ~(last - 1);
   }
   hit = team.most(hit);
-  if (hit) return (int)~hit;
-  return (int)team.most(last) - 1;
+  if (hit) return (int)~hit - row.shift;
+  return (int)team.most(last) - 1 - row.shift;
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __grid_constant__ SampleArgs a) {
+template <int W, typename T, int MODE>
+__global__ void __launch_bounds__(32 * W, W == 8 ? 5 : 2) sample_long_kernel(const __grid_constant__ SampleArgs a) {
   using O = Order<T>;
-  __shared__ LongShared sh;
+  __shared__ LongShared<W> sh;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, V = a.V;
-  Team<kLongWarps> team{sh.team, warp, lane};
+  Team<W> team{sh.team, warp, lane};
   // a warp's part of the row: whole steps of 256
-  const int part = (V + kLongWarps * 256 - 1) / (kLongWarps * 256) * 256, v0 = min(V, warp * part), v1 = min(V, v0 + part);
+  const int part = (int)part_of<W, T>(V);
   const int steps = part / 256, group = (steps + kSums - 1) / kSums;
   for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-    const T* p = (const T*)a.z.p + row * a.z.rs;
+    const Row<T, MODE> r(a, row);
     const Setting s = setting_of(a, row);
+    RowNote& note = ((RowNote*)a.scratch)[row];
+    const int v0 = min(r.end, warp * part), v1 = min(r.end, v0 + part);
+    int* const candidates = list_of(a, row) + warp * kListWarp;
     const bool greedy = !(s.t > 0.0), top_k = !greedy && s.k > 0 && s.k < V, top_p = !greedy && !top_k && s.p < 1.0;
     const bool list = greedy || top_k || top_p || s.m > 0.0;
     const float scale = (float)s.scale;
 
     // the sample: two steps of each warp
-    float ref = -INFINITY, low = INFINITY, sample[kSample];
-    {
-      Step<T, VEC> x[kSample / 8];
+    float ref = -INFINITY, low = INFINITY;
+    const auto each_sample = [&](auto f) {
+#pragma unroll 1
+      for (int h = 0; h < kSample / 16; h++) {
+        Step<T, MODE> x[2];
 #pragma unroll
-      for (int i = 0; i < kSample / 8; i++) x[i].load(p, a.z.cs, v0 + i * (steps / 2) * 256, lane, v1);
+        for (int i = 0; i < 2; i++) x[i].load(r, v0 + (2 * h + i) * max(1, steps / (kSample / 8)) * 256, lane, v1);
 #pragma unroll
-      for (int i = 0; i < kSample; i++) {
-        sample[i] = x[i / 8].z(i % 8);
-        ref = fmaxf(ref, sample[i]);
-        if (sample[i] > -INFINITY) low = fminf(low, sample[i]);
+        for (int i = 0; i < 16; i++) f(x[i / 8].z(i % 8));
       }
-    }
+    };
+    each_sample([&](float z) {
+      ref = fmaxf(ref, z);
+      if (z > -INFINITY) low = fminf(low, z);
+    });
     ref = O::value(max(team.most(O::of(ref)), O::of(-INFINITY)));
     const bool workable = plain_scale(s, ref) || (greedy && fabsf(ref) < INFINITY);
 
@@ -1030,19 +1199,19 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
       T under = from_f<T>(guess);
       if constexpr (std::is_same<T, __half>::value) under = __float2half_rd(guess);
       if constexpr (std::is_same<T, __nv_bfloat16>::value) under = __float2bfloat16_rd(guess);
-      const uint32_t guess2 = sizeof(T) == 4 ? 0 : pair_bits(under, under);
+      [[maybe_unused]] const uint32_t guess2 = sizeof(T) == 4 ? 0 : pair_bits(under, under);
+      constexpr int kBatch = sizeof(T) == 4 ? 2 : 4;  // steps whose loads are in flight together
       float group_sum = 0.0f;
       for (int i0 = 0; i0 < steps && v0 + i0 * 256 < v1; i0 += kBatch) {
-        Step<T, VEC> batch[kBatch];
+        Step<T, MODE> batch[kBatch];
 #pragma unroll
-        for (int j = 0; j < kBatch; j++) batch[j].load(p, a.z.cs, v0 + (i0 + j) * 256, lane, v1);
+        for (int j = 0; j < kBatch; j++) batch[j].load(r, v0 + (i0 + j) * 256, lane, v1);
 #pragma unroll
         for (int j = 0; j < kBatch; j++) {
           const int i = i0 + j, first = v0 + i * 256;
-          const Step<T, VEC>& x = batch[j];
+          const Step<T, MODE>& x = batch[j];
           if (first >= v1) break;
           if (kBest) best = x.most(best);
-          uint32_t in = kList ? x.at_least(guess, guess2) : 0;
           if constexpr (!kList) {
             float w[8];
 #pragma unroll
@@ -1055,31 +1224,35 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
               sum += group_sum;
               group_sum = 0.0f;
             }
-          } else if (__any_sync(kAll, in)) {
+          } else if constexpr (MODE == kVectors) {
+            uint32_t in = x.at_least(guess, guess2);
+            const uint32_t lanes = __ballot_sync(kAll, in);
+            if (!lanes) continue;
             const int mine = __popc(in);
-            if (VEC && !__any_sync(kAll, mine > 1)) {
+            if (!__any_sync(kAll, mine > 1)) {
+              const int to = n + __popc(lanes & ((1u << lane) - 1));
+              n += __popc(lanes);
+              if (in && to < kListWarp) candidates[to] = first + lane * 8 + __ffs(in) - 1;
+              continue;
+            }
+            int scan = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+              const int t = __shfl_up_sync(kAll, scan, d);
+              if (lane >= d) scan += t;
+            }
+            int to = n + scan - mine;
+            n += __shfl_sync(kAll, scan, 31);
+            for (; in && to < kListWarp; in &= in - 1) candidates[to++] = first + lane * 8 + __ffs(in) - 1;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const bool in = x.z(e) >= guess;
               const uint32_t b = __ballot_sync(kAll, in);
+              if (!b) continue;
               const int to = n + __popc(b & ((1u << lane) - 1));
               n += __popc(b);
-              if (in && to < kListWarp) sh.at[warp][to] = first + lane * 8 + __ffs(in) - 1;
-            } else if constexpr (VEC) {
-              int scan = mine;
-#pragma unroll
-              for (int d = 1; d < 32; d <<= 1) {
-                const int t = __shfl_up_sync(kAll, scan, d);
-                if (lane >= d) scan += t;
-              }
-              int to = n + scan - mine;
-              n += __shfl_sync(kAll, scan, 31);
-              for (; in && to < kListWarp; in &= in - 1) sh.at[warp][to++] = first + lane * 8 + __ffs(in) - 1;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; e++) {
-                const uint32_t b = __ballot_sync(kAll, in >> e & 1);
-                const int to = n + __popc(b & ((1u << lane) - 1));
-                n += __popc(b);
-                if (to < kListWarp && (in >> e & 1)) sh.at[warp][to] = first + e * 32 + lane;
-              }
+              if (to < kListWarp && in) candidates[to] = first + e * 32 + lane;
             }
           }
         }
@@ -1087,13 +1260,12 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
     };
     double all = -1.0, slack = 0.0, before = 0.0;  // all: the row's mass, known to the slack
     if (!workable) {                               // infinite, or nothing seen yet
-      each_of_row<T, VEC>(p, a.z.cs, V, warp, lane, [&](float z) {
+      each_of_row<W, T, MODE>(r, warp, lane, [&](float z) {
         best = max_nan(best, z);
       });
     } else if (!list || top_p) {
       pass(std::false_type(), std::true_type(), INFINITY);
       team.ahead(sum, before, all);
-      slack = all * a.margin;
     }
     float tail = 0.75f;  // top-p: of the share that is not kept, what may lie under the guess
     int tries = 2;
@@ -1103,15 +1275,15 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
       if (top_k || top_p) {
         low = -O::value(max(team.most(O::of(-low)), O::of(-INFINITY)));
         const float range = top_k ? ref - low : fminf(ref - low, 40.0f / scale), width = range * (1.0f / kBins);
-        for (int i = threadIdx.x; i < kBins; i += kLongThreads) sh.bins[i] = 0;
+        for (int i = threadIdx.x; i < kBins; i += (32 * W)) sh.bins[i] = 0;
         __syncthreads();
         const float to_bin = width > 0.0f ? 1.0f / width : 0.0f;
-#pragma unroll
-        for (int i = 0; i < kSample; i++)
-          if (sample[i] > -INFINITY) atomicAdd(&sh.bins[(int)fminf((ref - sample[i]) * to_bin, (float)(kBins - 1))], 1u);
+        each_sample([&](float z) {
+          if (z > -INFINITY) atomicAdd(&sh.bins[(int)fminf((ref - z) * to_bin, (float)(kBins - 1))], 1u);
+        });
         __syncthreads();
         if (warp == 0) {
-          const float share = (float)(kLongThreads * kSample) / (float)V;
+          const float share = fminf(1.0f, (float)(32 * W * kSample) / (float)V);
           // top-k: the rank in the sample that the row's k-th is hardly ever behind.  top-p: as much of the tail as leaves some
           // of what is not kept, beside the whole mass; the tail's small weights are sampled well
           const float mean = (float)s.k * share, want = top_k ? mean + 4.0f * sqrtf(mean) + 2.0f : tail * (1.0f - (float)fmax(s.p, 0.0)) * (float)all * share;
@@ -1132,10 +1304,10 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
           int bin = kBins;  // the first bin that, with those in front of it, is enough
 #pragma unroll
           for (int i = 7; i >= 0; i--) {
-            float r = run;
+            float front = run;
 #pragma unroll
-            for (int j = 0; j <= i; j++) r += c[j];
-            if (top_k ? r >= want : total - r <= want) bin = lane * 8 + i;
+            for (int j = 0; j <= i; j++) front += c[j];
+            if (top_k ? front >= want : total - front <= want) bin = lane * 8 + i;
           }
           bin = __reduce_min_sync(kAll, bin);
           if (lane == 0) sh.guess = bin >= kBins - 1 ? -INFINITY : ref - (bin + 1) * width;
@@ -1152,63 +1324,23 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
       // more of the tail, if what is held is not enough
       __syncwarp();
       double m = 0.0;
-      for (int i = lane; i < min(n, kListWarp); i += 32) m += exp2_fast((to_f(p[(int64_t)sh.at[warp][i] * a.z.cs]) - ref) * scale);
+      for (int i = lane; i < min(n, kListWarp); i += 32) m += exp2_fast((r.at(candidates[i]) - ref) * scale);
       if (team.sum(m) > s.p * all * (1.0 + 1e-5) || guess == -INFINITY) break;
       tail = 0.3f;
     }
     const uint32_t top = team.most(best != best || s.t != s.t ? kAll : O::of(best));
-    int label = -1;
+    const uint32_t longest = team.most((uint32_t)n);
+    int state = kDone, label = -1;
     if (top != kAll && O::value(top) > -INFINITY) {
       best = O::value(top);
-      label = kUnsure;
-      const uint32_t longest = team.most((uint32_t)n), held = team.sum((uint32_t)(lane == 0 ? n : 0));
-      if (workable && list && longest <= kListWarp && fabsf(best) < INFINITY && (!top_k || held >= s.k)) {
-        if (top_p) {
-          const double up = exp2((double)(ref - best) * (double)scale);
-          all *= up;
-          slack *= 0.5 * up;  // of the sum alone
-          if (!((best - ref) * scale < 8.0f)) all = INFINITY;  // the bound counts on a sample that comes near the largest
-        }
-        const bool few = held <= kFew;
-        if (few) {  // to one warp, which exchanges without barriers
-          uint32_t to;
-          team.ahead((uint32_t)n, to);
-          for (int i = lane; i < n; i += 32) sh.few[to + i] = sh.at[warp][i];
-        }
-        __syncthreads();
-        const auto from_list = [&](auto places) {
-          constexpr int E = decltype(places)::value;
-          float z[E];
-#pragma unroll
-          for (int e = 0; e < E; e++) z[e] = e * 32 + lane < n ? to_f(p[(int64_t)sh.at[warp][e * 32 + lane] * a.z.cs]) : -INFINITY;
-          const int at = draw<T, E, kLongWarps>(team, z, best, s, V, all, slack);
-          return at < 0 ? at : sh.at[at / (32 * E)][at % (32 * E)];
-        };
-        for (int again = 0; again < 2; again++) {
-          if (few) {
-            if (warp == 0) {
-              constexpr int E = kFew / 32;
-              float z[E];
-#pragma unroll
-              for (int e = 0; e < E; e++) z[e] = e * 32 + lane < (int)held ? to_f(p[(int64_t)sh.few[e * 32 + lane] * a.z.cs]) : -INFINITY;
-              Team<1> one{sh.team, 0, lane};
-              const int at = draw<T, E, 1>(one, z, best, s, V, all, slack);
-              if (lane == 0) sh.answer = at < 0 ? at : sh.few[at];
-            }
-            __syncthreads();
-            label = sh.answer;
-          } else {
-            label = longest <= 32 * 8 ? from_list(std::integral_constant<int, 8>()) : from_list(std::integral_constant<int, kHeld>());
-          }
-          if (label != kUnsure || !(slack > 0.0)) break;
-          const Weight weight(best, s.scale);  // the mass again, in 64 bits
-          double m = 0.0;
-          each_of_row<T, VEC>(p, a.z.cs, V, warp, lane, [&](float z) { m += weight.of(z); });
-          all = team.sum(m);
-          slack = 0.0;
-        }
+      state = kWhole;
+      if (workable && list) {
+        if (longest <= kListWarp && fabsf(best) < INFINITY) state = kFromList;
       } else if (workable && !list && (best - ref) * scale < 8.0f) {
+        // both sums, up to the draw and u times the whole, are u times the whole or so; that part's mean exponent is at most
+        // log2 V - log2 u
         const double want = s.u * all;
+        slack = (want + 1e-6 * all) * (a.margin + (fmax(0.0, (double)(best - ref) * s.scale) - 0.5 * log2f(fmaxf((float)s.u, 1e-6f))) * a.margin_far);
         if (threadIdx.x == 0) sh.answer = kUnsure;
         __syncthreads();
         if (want > slack && all - want > slack && before <= want && before + sum > want) {
@@ -1220,12 +1352,12 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
           int found = -1;
           bool near = fabs(run - want) <= slack;
           for (int i = g * group; i < min(steps, (g + 1) * group) && found < 0; i++) {
-            Step<T, VEC> x;
+            Step<T, MODE> x;
             const int first = v0 + i * 256;
-            x.load(p, a.z.cs, first, lane, v1);
+            x.load(r, first, lane, v1);
             // running sums in index order
             uint32_t hit = 0;
-            if constexpr (VEC) {
+            if constexpr (MODE == kVectors) {
               float w[8], mine = 0.0f;
 #pragma unroll
               for (int e = 0; e < 8; e++) mine += w[e] = exp2_fast(fmaf(x.z(e), scale, -ref_scaled));
@@ -1235,12 +1367,12 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
                 const float t = __shfl_up_sync(kAll, scan, d);
                 if (lane >= d) scan += t;
               }
-              double r = run + (double)(scan - mine);
+              double q = run + (double)(scan - mine);
 #pragma unroll
               for (int e = 0; e < 8; e++) {
-                r += w[e];
-                near |= fabs(r - want) <= slack && w[e] > 0.0f;
-                if (!hit && r > want) hit = ~(uint32_t)(lane * 8 + e);
+                q += w[e];
+                near |= fabs(q - want) <= slack && w[e] > 0.0f;
+                if (!hit && q > want) hit = ~(uint32_t)(lane * 8 + e);
               }
               run += (double)__shfl_sync(kAll, scan, 31);
             } else {
@@ -1253,9 +1385,9 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
                   const float t = __shfl_up_sync(kAll, scan, d);
                   if (lane >= d) scan += t;
                 }
-                const double r = run + (double)scan;
-                near |= fabs(r - want) <= slack && w > 0.0f;
-                if (!hit && r > want) hit = ~(uint32_t)(e * 32 + lane);
+                const double q = run + (double)scan;
+                near |= fabs(q - want) <= slack && w > 0.0f;
+                if (!hit && q > want) hit = ~(uint32_t)(e * 32 + lane);
                 run += (double)__shfl_sync(kAll, scan, 31);
               }
             }
@@ -1263,13 +1395,90 @@ __global__ void __launch_bounds__(kLongThreads, 3) sample_long_kernel(const __gr
             if (hit) found = first + (int)~hit;
           }
           near = __any_sync(kAll, near);
-          if (lane == 0 && found >= 0 && !near) sh.answer = found;
+          if (lane == 0 && found >= 0 && !near) sh.answer = found - r.shift;
         }
         __syncthreads();
         label = sh.answer;
+        if (label != kUnsure) state = kDone;
       }
-      if (label == kUnsure) label = whole_row<T, VEC>(team, sh, a, p, best, s);
     }
+    if (threadIdx.x == 0) {
+      a.label[row] = label;
+      note.state = state, note.best = best, note.ref = ref, note.all = all;
+    }
+    if (lane == 0) note.n[warp] = n;
+    __syncthreads();
+  }
+}
+
+// What the passes left open: the draw from a row's candidates, or from the whole row.  Apart from the passes, so that
+// the draws of many rows, whose steps wait for one another, run side by side.  W: warps of the passes.
+template <int W, typename T, int MODE>
+__global__ void __launch_bounds__(32 * W, W == 8 ? 4 : 1) sample_held_kernel(const __grid_constant__ SampleArgs a) {
+  __shared__ LongShared<W> sh;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  Team<W> team{sh.team, warp, lane};
+  for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+    const RowNote& note = ((const RowNote*)a.scratch)[row];
+    if (note.state == kDone) continue;
+    const Row<T, MODE> r(a, row);
+    const int* const candidates = list_of(a, row);
+    const Setting s = setting_of(a, row);
+    const bool greedy = !(s.t > 0.0), top_k = !greedy && s.k > 0 && s.k < a.V, top_p = !greedy && !top_k && s.p < 1.0;
+    const float best = note.best;
+    int label = kUnsure;
+    if (note.state == kFromList) {
+      int before = 0, held = 0, longest = 0;
+#pragma unroll
+      for (int i = 0; i < W; i++) {
+        if (i == warp) before = held;
+        held += note.n[i];
+        longest = max(longest, note.n[i]);
+      }
+      double all = -1.0, slack = 0.0;  // all: the row's mass, known to the slack
+      if (top_p) {
+        const double far = fmax(0.0, (double)(best - note.ref) * s.scale), up = exp2((double)(note.ref - best) * (double)(float)s.scale);
+        all = note.all * up;
+        slack = 0.5 * all * (a.margin + far * a.margin_far);
+        if (!(far < 8.0)) all = INFINITY;  // the sum in float32 counts on a sample that comes near the largest
+      }
+      for (int again = 0; again < 2 && (!top_k || held >= s.k); again++) {
+        if (held <= kFew) {  // one warp, which exchanges without barriers
+          for (int i = lane; i < note.n[warp]; i += 32) sh.few[before + i] = candidates[warp * kListWarp + i];
+          __syncthreads();
+          if (warp == 0) {
+            constexpr int E = kFew / 32;
+            float z[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) z[e] = e * 32 + lane < held ? r.at(sh.few[e * 32 + lane]) : -INFINITY;
+            Team<1> one{sh.team, 0, lane};
+            const int at = draw<T, E, 1>(one, z, best, s, a.V, all, slack);
+            if (lane == 0) sh.answer = at < 0 ? at : sh.few[at] - r.shift;
+          }
+          __syncthreads();
+          label = sh.answer;
+        } else {
+          const auto from_list = [&](auto places) {
+            constexpr int E = decltype(places)::value;
+            const int n = note.n[warp];
+            float z[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) z[e] = e * 32 + lane < n ? r.at(candidates[warp * kListWarp + e * 32 + lane]) : -INFINITY;
+            const int at = draw<T, E, W>(team, z, best, s, a.V, all, slack);
+            label = at < 0 ? at : candidates[at / (32 * E) * kListWarp + at % (32 * E)] - r.shift;
+          };
+          if (longest <= 32 * kHeld / 2) from_list(std::integral_constant<int, kHeld / 2>());
+          else from_list(std::integral_constant<int, kHeld>());
+        }
+        if (label != kUnsure || !(slack > 0.0)) break;
+        const Weight weight(best, s.scale);  // the mass again, in 64 bits
+        double m = 0.0;
+        each_of_row<W, T, MODE>(r, warp, lane, [&](float z) { m += weight.of(z); });
+        all = team.sum(m);
+        slack = 0.0;
+      }
+    }
+    if (label == kUnsure) label = whole_row<W, T, MODE>(team, sh, r, a.V, best, s);
     if (threadIdx.x == 0) a.label[row] = label;
     __syncthreads();
   }
@@ -1288,6 +1497,8 @@ cudaError_t allow_shared(int bytes) {
   return rc;
 }
 
+int long_warps(int64_t M, int sms) { return M <= sms ? 16 : 8; }
+
 template <typename T>
 cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
   SampleArgs b = a;
@@ -1298,7 +1509,7 @@ cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
   while ((1ll << bits) < a.V) bits++;
   // twice the error, relative to the whole sum, of a running sum in float32 and of u times the sum.  exp2 is off by 2^-22 of a weight; its
   // argument by three half steps, 3 ln 2 = 2.1 times 2^-24 |t| of the weight, where |t| counts with the weights: at most as
-  // log2 V (the entropy), and twice the distance to the largest, up to 8, where that was not known; additions by 2^-24 each.
+  // log2 V (the entropy), and twice the distance to the largest where that was not known; additions by 2^-24 each.
   const auto margin = [&](double chain, double extra) {
     return (float)(2.0 * (0x1p-22 + 2.1 * 0x1p-24 * (bits + extra) + (chain + 4) * 0x1p-24));
   };
@@ -1344,17 +1555,30 @@ cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
   b.margin = margin(16 + 5 + 8, 0);
   if (a.V <= 1024) return run(sample_rows_kernel<T, 16, 2>, a.M, 64, 64);
   if (a.V <= 4096) return run(sample_rows_kernel<T, 16, 8>, a.M, 256, 16);
-  if (a.V <= 8192) return run(sample_rows_kernel<T, 16, 16>, a.M, 512, 8);
-  const int64_t part = (a.V + kLongWarps * 256ll - 1) / (kLongWarps * 256), group = (part + kSums - 1) / kSums;
-  b.margin = margin((double)group + 3 + 5 + 3, 16);
-  constexpr int per = 16 / (int)sizeof(T);
-  if (a.z.cs == 1 && a.z.rs % per == 0 && a.V % per == 0 && (uintptr_t)a.z.p % 16 == 0)
-    return run(sample_long_kernel<T, true>, a.M, kLongThreads, 8);
-  return run(sample_long_kernel<T, false>, a.M, kLongThreads, 8);
+  if (a.V <= kRowLabels) return run(sample_rows_kernel<T, 16, 16>, a.M, 512, 8);
+  // few rows: more warps for each
+  const auto rows = [&](auto warps) {
+    constexpr int W = decltype(warps)::value;
+    const int64_t steps = part_of<W, T>(a.V) / 256, group = (steps + kSums - 1) / kSums;
+    b.margin = margin((double)group + 3 + 5 + 3, 0);
+    b.margin_far = (float)(2.0 * 2.0 * 2.1 * 0x1p-24);
+    b.list_at = a.M * (int64_t)sizeof(RowNote);
+    b.list_bytes = list_bytes(W);
+    const auto both = [&](auto mode) {
+      constexpr int MODE = decltype(mode)::value;
+      const cudaError_t rc = run(sample_long_kernel<W, T, MODE>, a.M, 32 * W, W == 8 ? 5 : 2);
+      return rc == cudaSuccess ? run(sample_held_kernel<W, T, MODE>, a.M, 32 * W, W == 8 ? 16 : 2) : rc;
+    };
+    return a.z.cs == 1 ? both(std::integral_constant<int, kVectors>()) : both(std::integral_constant<int, kStrided>());
+  };
+  return long_warps(a.M, sms) == 16 ? rows(std::integral_constant<int, 16>()) : rows(std::integral_constant<int, 8>());
 }
 
 }  // namespace
 
+uint64_t sample_scratch(int64_t M, int64_t V, int sms) {
+  return V <= kRowLabels ? 0 : (uint64_t)M * (sizeof(RowNote) + list_bytes(long_warps(M, sms)));
+}
 cudaError_t launch_sample(int dtype, const SampleArgs& a, int sms, cudaStream_t s) {
   return dtype == VI_F32 ? launch<float>(a, sms, s) : dtype == VI_F16 ? launch<__half>(a, sms, s) : launch<__nv_bfloat16>(a, sms, s);
 }
