@@ -848,11 +848,7 @@ struct Step {
   static __device__ __forceinline__ int place(int first, int lane, int e) { return MODE == kVectors ? first + lane * 8 + e : first + e * 32 + lane; }
   __device__ __forceinline__ void load(const Row<T, MODE>& r, int first, int lane, int end) {
     if constexpr (MODE == kVectors) {
-      if (first + 256 <= end && first >= kPer) {
-#pragma unroll
-        for (int i = 0; i < 8 / kPer; i++) q[i] = ((const uint4*)(r.p + first + lane * 8))[i];
-        return;
-      }
+      if (first + 256 <= end && first >= kPer) return load_whole(r, first, lane);
 #pragma unroll
       for (int i = 0; i < 8 / kPer; i++) {
         const int v = first + lane * 8 + i * kPer;
@@ -869,6 +865,11 @@ struct Step {
 #pragma unroll
       for (int e = 0; e < 8; e++) t[e] = first + e * 32 + lane < end ? at[e * step] : from_f<T>(-INFINITY);
     }
+  }
+  // The same where all 256 places hold labels.
+  __device__ __forceinline__ void load_whole(const Row<T, MODE>& r, int first, int lane) {
+#pragma unroll
+    for (int i = 0; i < 8 / kPer; i++) q[i] = ((const uint4*)(r.p + first + lane * 8))[i];
   }
   // The largest, or a NaN if there is one.
   __device__ __forceinline__ float most(float m) const {
@@ -1193,8 +1194,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 5 : 2) sample_long_kernel(con
     float best = -INFINITY;
     int n = 0;
     double sum = 0.0;
-    const auto pass = [&](auto wants_list, auto wants_best, float guess) {
-      constexpr bool kList = decltype(wants_list)::value, kBest = decltype(wants_best)::value;
+    const auto pass = [&](auto wants_list, auto wants_best, auto wants_groups, float guess) {
+      constexpr bool kList = decltype(wants_list)::value, kBest = decltype(wants_best)::value, kGroups = decltype(wants_groups)::value;
       // the type's last value that is not above the guess
       T under = from_f<T>(guess);
       if constexpr (std::is_same<T, __half>::value) under = __float2half_rd(guess);
@@ -1202,39 +1203,51 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 5 : 2) sample_long_kernel(con
       [[maybe_unused]] const uint32_t guess2 = sizeof(T) == 4 ? 0 : pair_bits(under, under);
       constexpr int kBatch = sizeof(T) == 4 ? 2 : 4;  // steps whose loads are in flight together
       float group_sum = 0.0f;
-      for (int i0 = 0; i0 < steps && v0 + i0 * 256 < v1; i0 += kBatch) {
+      int left = group, g = 0;
+      for (int first0 = v0; first0 < v1; first0 += kBatch * 256) {
         Step<T, MODE> batch[kBatch];
+        if (MODE == kVectors && first0 >= Step<T, MODE>::kPer && first0 + kBatch * 256 <= v1) {
 #pragma unroll
-        for (int j = 0; j < kBatch; j++) batch[j].load(r, v0 + (i0 + j) * 256, lane, v1);
+          for (int j = 0; j < kBatch; j++) batch[j].load_whole(r, first0 + j * 256, lane);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kBatch; j++) {
-          const int i = i0 + j, first = v0 + i * 256;
+          for (int j = 0; j < kBatch; j++) batch[j].load(r, first0 + j * 256, lane, v1);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; j++) {  // steps behind the end hold -inf
+          const int first = first0 + j * 256;
           const Step<T, MODE>& x = batch[j];
-          if (first >= v1) break;
           if (kBest) best = x.most(best);
           if constexpr (!kList) {
             float w[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) w[e] = exp2_fast(fmaf(x.z(e), scale, -ref_scaled));
-            group_sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-            if (group == 1 || i % group == group - 1 || first + 256 >= v1) {
+            const float v = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            if constexpr (kGroups) {
+              group_sum += v;
+              if (--left == 0 || first + 256 >= v1) {
 #pragma unroll
-              for (int o = 16; o; o >>= 1) group_sum += __shfl_xor_sync(kAll, group_sum, o);
-              if (lane == 0) sh.sums[warp][i / group] = group_sum;
-              sum += group_sum;
-              group_sum = 0.0f;
+                for (int o = 16; o; o >>= 1) group_sum += __shfl_xor_sync(kAll, group_sum, o);
+                if (lane == 0 && g < kSums) sh.sums[warp][g] = group_sum;
+                if (lane == 0) sum += group_sum;
+                g++;
+                group_sum = 0.0f;
+                left = group;
+              }
+            } else {
+              sum += v;
             }
           } else if constexpr (MODE == kVectors) {
             uint32_t in = x.at_least(guess, guess2);
             const uint32_t lanes = __ballot_sync(kAll, in);
             if (!lanes) continue;
-            const int mine = __popc(in);
-            if (!__any_sync(kAll, mine > 1)) {
+            if (!__any_sync(kAll, in & (in - 1))) {
               const int to = n + __popc(lanes & ((1u << lane) - 1));
               n += __popc(lanes);
               if (in && to < kListWarp) candidates[to] = first + lane * 8 + __ffs(in) - 1;
               continue;
             }
+            const int mine = __popc(in);
             int scan = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -1257,6 +1270,10 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 5 : 2) sample_long_kernel(con
           }
         }
       }
+      if (!kList) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+      }
     };
     double all = -1.0, slack = 0.0, before = 0.0;  // all: the row's mass, known to the slack
     if (!workable) {                               // infinite, or nothing seen yet
@@ -1264,7 +1281,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 5 : 2) sample_long_kernel(con
         best = max_nan(best, z);
       });
     } else if (!list || top_p) {
-      pass(std::false_type(), std::true_type(), INFINITY);
+      if (list) pass(std::false_type(), std::true_type(), std::false_type(), INFINITY);
+      else pass(std::false_type(), std::true_type(), std::true_type(), INFINITY);
       team.ahead(sum, before, all);
     }
     float tail = 0.75f;  // top-p: of the share that is not kept, what may lie under the guess
@@ -1318,8 +1336,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 5 : 2) sample_long_kernel(con
         guess = ref + (float)(log2_min_p(a, s) / s.scale) * (1.0f + 1e-5f) - 1e-6f * fabsf(ref);
       }
       n = 0;
-      if (top_p) pass(std::true_type(), std::false_type(), guess);
-      else pass(std::true_type(), std::true_type(), guess);
+      if (top_p) pass(std::true_type(), std::false_type(), std::false_type(), guess);
+      else pass(std::true_type(), std::true_type(), std::false_type(), guess);
       if (!top_p || --tries == 0) break;
       // more of the tail, if what is held is not enough
       __syncwarp();
