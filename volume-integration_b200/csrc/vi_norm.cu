@@ -17,22 +17,11 @@
 #include "vi_heads.h"
 #include "vi_heads_math.cuh"
 #include "vi_internal.h"
+#include "vi_rows.cuh"
 
 namespace vi {
 namespace heads {
 namespace {
-
-template <typename T, int N>
-struct __align__(N * sizeof(T) >= 16 ? 16 : N * sizeof(T)) Chunk {
-  T v[N];
-};
-template <typename T, int N>
-__device__ __forceinline__ Chunk<T, N> chunk_zero() {
-  Chunk<T, N> c;
-#pragma unroll
-  for (int i = 0; i < N; i++) c.v[i] = from_f<T>(0.0f);
-  return c;
-}
 
 // Sum of S values over the lanes of a row: G lanes of a warp, or a block.  Every lane gets it, always added in the same
 // order.
@@ -61,17 +50,6 @@ __device__ __forceinline__ void row_sum(float (&s)[S], int lanes, float (*sh)[16
   }
 }
 
-// The lane's NV chunks of a row: columns (v * lanes + lane) * VEC on.
-template <typename T, int VEC, int NV>
-__device__ __forceinline__ void load_row(Chunk<T, VEC> (&c)[NV], const View& m, int64_t row, int K, int lanes, int lane) {
-  const T* p = (const T*)m.p + row * m.rs;
-#pragma unroll
-  for (int v = 0; v < NV; v++) {
-    const int at = (v * lanes + lane) * VEC;
-    if constexpr (VEC > 1) c[v] = at < K ? *(const Chunk<T, VEC>*)(p + at) : chunk_zero<T, VEC>();
-    else c[v].v[0] = at < K ? p[at * m.cs] : from_f<T>(0.0f);
-  }
-}
 template <typename T, int VEC, int NV>
 __device__ __forceinline__ void load_weights(Chunk<T, VEC> (&c)[NV], const void* w, float none, int K, int lanes, int lane) {
 #pragma unroll
@@ -336,19 +314,6 @@ __global__ void __launch_bounds__(256) norm_columns_kernel(const __grid_constant
 // A lane holds VP neighbouring pixels, a warp every `warps`-th channel of them, up to R; `warps` warps make a tile of
 // 32 VP pixels.  VP = 1: any strides.
 template <typename T, int VP>
-__device__ __forceinline__ Chunk<T, VP> load_pixels(const View& m, int64_t row, int64_t c, int64_t M) {
-  const T* p = (const T*)m.p + row * m.rs + c * m.cs;
-  Chunk<T, VP> r = chunk_zero<T, VP>();
-  if (row + VP <= M) {
-    r = *(const Chunk<T, VP>*)p;
-  } else {
-#pragma unroll
-    for (int j = 0; j < VP; j++)
-      if (row + j < M) r.v[j] = p[j * m.rs];
-  }
-  return r;
-}
-template <typename T, int VP>
 __device__ __forceinline__ void store_pixels(const Chunk<T, VP>& r, const View& m, int64_t row, int64_t c, int64_t M) {
   T* p = (T*)m.p + row * m.rs + c * m.cs;
   if (row + VP <= M) {
@@ -534,8 +499,6 @@ __global__ void __launch_bounds__(512) norm_image_backward(const __grid_constant
 }
 
 // ---- host ----
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // One call: what is launched, in how many blocks; `pieces` partial sums of the weights' gradients.
 struct Call {
   const NormArgs& a;
@@ -596,12 +559,6 @@ struct Call {
   }
 };
 
-int pow2_at_least(int64_t n) {
-  int p = 1;
-  while (p < n) p *= 2;
-  return p;
-}
-
 // Rows of `units` vectors or elements by lanes, or by a block: false where this shape does not hold them.
 template <typename T, int VEC, int NV, int R, bool BACKWARD>
 bool rows_lanes(Call& c, int64_t units) {
@@ -635,12 +592,9 @@ void norm_call(Call& c, bool backward) {
   const NormArgs& a = c.a;
   constexpr int VEC = 16 / (int)sizeof(T);
   const bool image = a.x.rs == 1 && a.x.cs != 1 && a.M > 1;
-  // whether n neighbouring elements along the contiguous axis may be moved at once, everywhere
   const auto wide = [&](int n, bool along_rows) {
-    for (const View* v : {&a.x, &a.dy, &a.y}) {
-      if (!v->p) continue;
-      if ((along_rows ? v->rs : v->cs) != 1 || (along_rows ? v->cs : v->rs) % n || (uintptr_t)v->p % (n * sizeof(T))) return false;
-    }
+    for (const View* v : {&a.x, &a.dy, &a.y})
+      if (v->p && !moves<T>(*v, n, along_rows)) return false;
     return along_rows || (a.K % n == 0 && (uintptr_t)a.w % (n * sizeof(T)) == 0 && (uintptr_t)a.b % (n * sizeof(T)) == 0);
   };
   if (image) {

@@ -11,6 +11,7 @@
 #include "vi_heads.h"
 #include "vi_heads_math.cuh"
 #include "vi_internal.h"
+#include "vi_rows.cuh"
 
 namespace vi {
 namespace heads {
@@ -24,27 +25,113 @@ __device__ __noinline__ int quotient(float x, float s) {
   const double q = rint((double)x / (double)s);
   return (int)fmin(fmax(q, -127.0), 127.0);
 }
+
+// The bits of magnitudes, which order as they do, infinities and NaNs last.  Two 16-bit ones at a time.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t magnitude(const Chunk<T, N>& c, uint32_t top) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < N; i++) top = max(top, __float_as_uint(to_f(c.v[i])) & 0x7fffffffu);
+  } else if constexpr (N == 1) {
+    top = max(top, (uint32_t)(*(const uint16_t*)&c.v[0] & 0x7fff));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) top = __vmaxu2(top, ((const uint32_t*)c.v)[i] & 0x7fff7fffu);
+  }
+  return top;
+}
+// The magnitude as float32's bits: of one, or the larger of two.
+template <typename T>
+__device__ __forceinline__ uint32_t magnitude_bits(uint32_t top) {
+  if constexpr (sizeof(T) == 4) {
+    return top;
+  } else {
+    const uint16_t m = (uint16_t)max(top & 0xffffu, top >> 16);
+    return __float_as_uint(to_f(*(const T*)&m));
+  }
+}
+
 struct Scale {
   float s, inv;
-  bool slow;
+  bool slow, none;
+  __device__ __forceinline__ Scale() {}
   // of the largest magnitude's bits
   __device__ __forceinline__ explicit Scale(uint32_t top) {
     s = __fdiv_rn(__uint_as_float(top), 127.0f);
     if (top >= 0x7f800000u) s = NAN;
+    none = !(s > 0.0f);  // zeros, or not finite: q is 0
     slow = s > 0.0f && s < 0x1p-100f;
     inv = s >= 0x1p-100f ? __fdiv_rn(1.0f, s) : 0.0f;
   }
-  __device__ __forceinline__ int of(float x) const {
-    if (!(s > 0.0f)) return 0;  // zeros; not finite
-    const float t = x * inv, r = rintf(t);
-    if (slow || fabsf(t - r) > 0.4999f) return quotient(x, s);
-    return (int)r;
-  }
 };
+// x / s rounded.  x inv is within 2^-16 of the quotient (127 * 2 * 2^-24), so it decides but within that of a half.
+__device__ __forceinline__ int quantize(float x, const Scale& s) {
+  const float f = fmaf(x, s.inv, 12582912.0f);  // 1.5 * 2^23: the whole number is in the low bits
+  const float d = fmaf(x, s.inv, 12582912.0f - f);
+  int q = __float_as_int(f);
+  if (fabsf(d) > 0.49998f || s.slow) q = quotient(x, s.s);
+  return s.none ? 0 : q;
+}
+__device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 
-// A block a row at a time, any strides and lengths.
+// Rows of contiguous features: a row belongs to `lanes` lanes, or to a block; R rows at a time.
+template <typename T, int VEC, int NV, int R, bool BLOCK>
+__global__ void __launch_bounds__(BLOCK ? 512 : kThreads) quantize_rows_kernel(const __grid_constant__ QuantArgs a, int lanes) {
+  __shared__ uint32_t sh[2][16];
+  int turn = 0;
+  const int lane = BLOCK ? threadIdx.x : threadIdx.x % lanes, group = BLOCK ? 0 : threadIdx.x / lanes;
+  const int groups = BLOCK ? 1 : kThreads / lanes;
+  for (int64_t m0 = (int64_t)blockIdx.x * groups * R; m0 < a.M; m0 += (int64_t)gridDim.x * groups * R) {
+    Chunk<T, VEC> x[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; r++) load_row(x[r], a.x, min(m0 + r * groups + group, a.M - 1), a.K, lanes, lane);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int64_t m = m0 + r * groups + group;
+      uint32_t top = 0;
+#pragma unroll
+      for (int v = 0; v < NV; v++) top = magnitude(x[r][v], top);
+      top = magnitude_bits<T>(top);
+      if constexpr (BLOCK) {
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (threadIdx.x % 32 == 0) sh[turn][threadIdx.x / 32] = top;
+        __syncthreads();
+        for (int w = 0; w < blockDim.x / 32; w++) top = max(top, sh[turn][w]);
+        turn ^= 1;
+      } else if (lanes == 32) {
+        top = __reduce_max_sync(0xffffffffu, top);
+      } else {
+        for (int o = lanes / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      }
+      const Scale s(top);
+      if (m >= a.M) continue;
+      int8_t* q = a.q + m * a.ld;
+#pragma unroll
+      for (int v = 0; v < NV; v++) {
+        const int at = (v * lanes + lane) * VEC;
+        if (at >= a.K) continue;
+        if constexpr (VEC == 1) {
+          q[at] = (int8_t)quantize(to_f(x[r][v].v[0]), s);
+        } else {
+          uint32_t w[VEC / 4];
+#pragma unroll
+          for (int i = 0; i < VEC; i += 4)
+            w[i / 4] = bytes4(quantize(to_f(x[r][v].v[i]), s), quantize(to_f(x[r][v].v[i + 1]), s), quantize(to_f(x[r][v].v[i + 2]), s),
+                              quantize(to_f(x[r][v].v[i + 3]), s));
+          if constexpr (VEC == 8) *(uint2*)(q + at) = make_uint2(w[0], w[1]);
+          else *(uint32_t*)(q + at) = w[0];
+        }
+      }
+      if (lane == 0) a.scale[m] = s.s;
+    }
+  }
+}
+
+// Any strides and lengths: a block a row, which it reads twice.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(const __grid_constant__ QuantArgs a) {
+__global__ void __launch_bounds__(kThreads) quantize_long_kernel(const __grid_constant__ QuantArgs a) {
   __shared__ uint32_t sh[kThreads / 32];
   for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
     const T* x = (const T*)a.x.p + m * a.x.rs;
@@ -57,8 +144,74 @@ __global__ void __launch_bounds__(kThreads) quantize_kernel(const __grid_constan
 #pragma unroll
     for (int i = 0; i < kThreads / 32; i++) top = max(top, sh[i]);
     const Scale s(top);
-    for (int k = threadIdx.x; k < a.K; k += kThreads) a.q[m * a.ld + k] = (int8_t)s.of(to_f(x[k * a.x.cs]));
+    for (int k = threadIdx.x; k < a.K; k += kThreads) a.q[m * a.ld + k] = (int8_t)quantize(to_f(x[k * a.x.cs]), s);
     if (threadIdx.x == 0) a.scale[m] = s.s;
+  }
+}
+
+// Images: a lane holds VP neighbouring pixels, a warp every warps-th group of 4 channels, up to R channels; the bytes go to
+// their pixels' rows through shared memory, in words whose pitch is odd so that no two lanes meet in a bank.
+// LONG: more channels than the warps hold, so they are read twice.
+template <typename T, int VP, int R, bool LONG>
+__global__ void __launch_bounds__(512) quantize_image_kernel(const __grid_constant__ QuantArgs a) {
+  extern __shared__ uint32_t sh[];
+  constexpr int kPixels = 32 * VP;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  const int words = (a.K + 3) / 4, pitch = words | 1;
+  uint32_t* const tops = sh + kPixels * pitch;  // [2][warps][kPixels]
+  int turn = 0;
+  const int64_t tiles = (a.M + kPixels - 1) / kPixels;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+    const int64_t m = (tile * 32 + lane) * VP;
+    Chunk<T, VP> x[R];
+    const auto load = [&](int k0) {
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const int c = k0 + (i / 4 * warps + warp) * 4 + i % 4;
+        x[i] = c < a.K && m < a.M ? load_pixels<T, VP>(a.x, m, c, a.M) : chunk_zero<T, VP>();
+      }
+    };
+    uint32_t top[VP] = {};
+    load(0);
+    for (int k0 = 0; k0 < (LONG ? a.K : 1); k0 += R * warps) {
+      if (LONG && k0) load(k0);
+#pragma unroll
+      for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int j = 0; j < VP; j++) top[j] = max(top[j], __float_as_uint(to_f(x[i].v[j])) & 0x7fffffffu);
+    }
+    uint32_t* const own = tops + turn * warps * kPixels + lane;
+#pragma unroll
+    for (int j = 0; j < VP; j++) own[(warp * VP + j) * 32] = top[j];
+    __syncthreads();
+    Scale s[VP];
+#pragma unroll
+    for (int j = 0; j < VP; j++) {
+      for (int w = 0; w < warps; w++) top[j] = max(top[j], own[(w * VP + j) * 32]);
+      s[j] = Scale(top[j]);
+      if (warp == 0 && m + j < a.M) a.scale[m + j] = s[j].s;
+    }
+    if (LONG) load(0);
+    for (int k0 = 0; k0 < (LONG ? a.K : 1); k0 += R * warps) {
+      if (LONG && k0) load(k0);
+#pragma unroll
+      for (int i = 0; i < R; i += 4) {
+        const int w = k0 / 4 + i / 4 * warps + warp;
+        if (w < words) {
+#pragma unroll
+          for (int j = 0; j < VP; j++)
+            sh[(j * 32 + lane) * pitch + w] = bytes4(quantize(to_f(x[i].v[j]), s[j]), quantize(to_f(x[i + 1].v[j]), s[j]),
+                                                     quantize(to_f(x[i + 2].v[j]), s[j]), quantize(to_f(x[i + 3].v[j]), s[j]));
+        }
+      }
+    }
+    __syncthreads();
+    const int64_t first = tile * kPixels;
+    const int count = (int)min((int64_t)kPixels, a.M - first) * words;
+    for (int i = threadIdx.x; i < count; i += blockDim.x) {
+      const int p = i / words, w = i - p * words;
+      *(uint32_t*)(a.q + (first + p) * a.ld + 4 * w) = sh[(p % VP * 32 + p / VP) * pitch + w];
+    }
   }
 }
 
@@ -68,13 +221,65 @@ __global__ void __launch_bounds__(kThreads) pack8_kernel(View src, int64_t rows,
     dst[i / k * ld + i % k] = p[i / k * src.rs + i % k * src.cs];
 }
 
+// ---- host ----
+struct Call {
+  const QuantArgs& a;
+  int sms;
+  cudaStream_t s;
+
+  template <typename T, int VEC, int NV, int R, bool BLOCK>
+  bool rows(int64_t units) {
+    if (units > (BLOCK ? 512 : 32) * NV) return false;
+    const int threads = BLOCK ? (int)ceil_div(ceil_div(units, NV), 32) * 32 : kThreads;
+    const int lanes = BLOCK ? threads : NV > 1 ? 32 : pow2_at_least(units);
+    const int64_t work = BLOCK ? a.M : ceil_div(a.M, (int64_t)kThreads / lanes * R);
+    quantize_rows_kernel<T, VEC, NV, R, BLOCK><<<(unsigned)std::min<int64_t>(work, (int64_t)sms * 16), threads, 0, s>>>(a, lanes);
+    return true;
+  }
+  template <typename T, int VP, int R, bool LONG>
+  bool image() {
+    const int warps = (int)std::min<int64_t>(16, ceil_div(ceil_div(a.K, 4), R / 4));
+    const size_t smem = (size_t)32 * VP * ((ceil_div(a.K, 4) | 1) + 2 * warps) * 4;
+    if (smem > 200 * 1024) return false;
+    auto* kernel = quantize_image_kernel<T, VP, R, LONG>;
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+    const int per_sm = (int)std::max<int64_t>(1, std::min<int64_t>(16 / warps * 2, (int64_t)(220 * 1024 / (smem + 1024))));
+    kernel<<<(unsigned)std::min<int64_t>(ceil_div(a.M, 32 * VP), (int64_t)sms * per_sm), warps * 32, smem, s>>>(a);
+    return true;
+  }
+  template <typename T>
+  void run() {
+    constexpr int VEC = 16 / (int)sizeof(T), VP = 4 / (int)sizeof(T);
+    const int64_t K = a.K;
+    const bool words = a.ld % 8 == 0 && (uintptr_t)a.q % 8 == 0;  // as this library lays rows out
+    if (a.x.rs == 1 && a.x.cs != 1 && a.M > 1 && a.ld % 4 == 0 && a.ld >= (K + 3) / 4 * 4 && (uintptr_t)a.q % 4 == 0) {
+      if (K <= 128 && moves<T>(a.x, VEC, true)) {
+        if (image<T, VEC, 8, false>()) return;
+      } else if (K <= 512) {
+        if (moves<T>(a.x, VP, true) ? image<T, VP, 32, false>() : image<T, 1, 32, false>()) return;
+      } else if (moves<T>(a.x, VP, true) ? image<T, VP, 32, true>() : image<T, 1, 32, true>()) {
+        return;
+      }
+    } else if (words && K % VEC == 0 && moves<T>(a.x, VEC, false)) {
+      const int64_t n = K / VEC;
+      if (rows<T, VEC, 1, 4, false>(n) || rows<T, VEC, 2, 2, false>(n) || rows<T, VEC, 4, 1, false>(n) || rows<T, VEC, 4, 1, true>(n)) return;
+    } else if (a.x.cs == 1 || a.x.rs != 1) {
+      if (rows<T, 1, 1, 4, false>(K) || rows<T, 1, 4, 1, false>(K) || rows<T, 1, 16, 1, false>(K) || rows<T, 1, 16, 1, true>(K)) return;
+    }
+    quantize_long_kernel<T><<<(unsigned)std::min<int64_t>(a.M, (int64_t)sms * 8), kThreads, 0, s>>>(a);
+  }
+};
+
 }  // namespace
 
 cudaError_t launch_quantize(int dtype, const QuantArgs& a, int sms, cudaStream_t s) {
-  const unsigned blocks = (unsigned)std::min<int64_t>(a.M, (int64_t)sms * 8);
-  if (dtype == VI_F32) quantize_kernel<float><<<blocks, kThreads, 0, s>>>(a);
-  else if (dtype == VI_F16) quantize_kernel<__half><<<blocks, kThreads, 0, s>>>(a);
-  else quantize_kernel<__nv_bfloat16><<<blocks, kThreads, 0, s>>>(a);
+  Call c{a, sms, s};
+  if (dtype == VI_F32) c.run<float>();
+  else if (dtype == VI_F16) c.run<__half>();
+  else c.run<__nv_bfloat16>();
   return cudaPeekAtLastError();
 }
 cudaError_t launch_pack8(const View& src, int64_t rows, int64_t k, int8_t* dst, int64_t ld, cudaStream_t s) {
