@@ -19,8 +19,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Near a half, or for a scale whose reciprocal is no float: the quotient of two floats is never so near a half without being
-// one that 53 bits would not tell.
+// For a scale whose reciprocal is no float: the quotient of two floats is never so near a half without being one that 53
+// bits would not tell.
 __device__ __noinline__ int quotient(float x, float s) {
   const double q = rint((double)x / (double)s);
   return (int)fmin(fmax(q, -127.0), 127.0);
@@ -53,24 +53,47 @@ __device__ __forceinline__ uint32_t magnitude_bits(uint32_t top) {
 
 struct Scale {
   float s, inv;
-  bool slow, none;
+  bool exact;  // x inv does not decide: the row is not finite, of zeros, or its scale has no float reciprocal
   __device__ __forceinline__ Scale() {}
   // of the largest magnitude's bits
   __device__ __forceinline__ explicit Scale(uint32_t top) {
-    s = __fdiv_rn(__uint_as_float(top), 127.0f);
-    if (top >= 0x7f800000u) s = NAN;
-    none = !(s > 0.0f);  // zeros, or not finite: q is 0
-    slow = s > 0.0f && s < 0x1p-100f;
-    inv = s >= 0x1p-100f ? __fdiv_rn(1.0f, s) : 0.0f;
+    const float x = __uint_as_float(top);
+    if (top >= 0x10000000u && top < 0x7f000000u) {  // within normal numbers a rounded reciprocal and one correction divide exactly
+      constexpr float r = 1.0f / 127.0f;
+      const float q = x * r;
+      s = fmaf(fmaf(-127.0f, q, x), r, q);
+      inv = rcp_fast(s);
+      exact = false;
+    } else {
+      s = top >= 0x7f800000u ? NAN : __fdiv_rn(x, 127.0f);
+      inv = 0.0f;
+      exact = true;
+    }
   }
 };
-// x / s rounded.  x inv is within 2^-16 of the quotient (127 * 2 * 2^-24), so it decides but within that of a half.
-__device__ __forceinline__ int quantize(float x, const Scale& s) {
-  const float f = fmaf(x, s.inv, 12582912.0f);  // 1.5 * 2^23: the whole number is in the low bits
-  const float d = fmaf(x, s.inv, 12582912.0f - f);
-  int q = __float_as_int(f);
-  if (fabsf(d) > 0.49998f || s.slow) q = quotient(x, s.s);
-  return s.none ? 0 : q;
+// N values of a lane divided and rounded.  x inv is within 127 * 2^-22 of the quotient, so it decides but within that of a
+// half.  There the rest x - q s does, which is exact: it is a multiple of half a last place of s and at most s / 2 or so.  (A
+// bfloat16 row has its largest value's half in one of 400 places, whose quotient is 63.5: halves are not rare.)
+template <int N>
+__device__ __forceinline__ void quantize(const float (&x)[N], const Scale& s, int (&q)[N]) {
+  float far = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const float f = fmaf(x[i], s.inv, 12582912.0f);  // 1.5 * 2^23: the whole number is in the low bits
+    far = fmaxf(far, fabsf(fmaf(x[i], s.inv, 12582912.0f - f)));
+    q[i] = __float_as_int(f);
+  }
+  if (s.exact) {
+#pragma unroll
+    for (int i = 0; i < N; i++) q[i] = s.s > 0.0f ? quotient(x[i], s.s) : 0;
+  } else if (far > 0.49996f) {
+    const float half = 0.5f * s.s;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float e = fmaf(12582912.0f - __int_as_float(q[i]), s.s, x[i]);
+      if (fabsf(e) > half || (fabsf(e) == half && (q[i] & 1))) q[i] += e > 0.0f ? 1 : -1;
+    }
+  }
 }
 __device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
@@ -112,17 +135,14 @@ __global__ void __launch_bounds__(BLOCK ? 512 : kThreads) quantize_rows_kernel(c
       for (int v = 0; v < NV; v++) {
         const int at = (v * lanes + lane) * VEC;
         if (at >= a.K) continue;
-        if constexpr (VEC == 1) {
-          q[at] = (int8_t)quantize(to_f(x[r][v].v[0]), s);
-        } else {
-          uint32_t w[VEC / 4];
+        float f[VEC];
+        int b[VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; i += 4)
-            w[i / 4] = bytes4(quantize(to_f(x[r][v].v[i]), s), quantize(to_f(x[r][v].v[i + 1]), s), quantize(to_f(x[r][v].v[i + 2]), s),
-                              quantize(to_f(x[r][v].v[i + 3]), s));
-          if constexpr (VEC == 8) *(uint2*)(q + at) = make_uint2(w[0], w[1]);
-          else *(uint32_t*)(q + at) = w[0];
-        }
+        for (int i = 0; i < VEC; i++) f[i] = to_f(x[r][v].v[i]);
+        quantize(f, s, b);
+        if constexpr (VEC == 1) q[at] = (int8_t)b[0];
+        else if constexpr (VEC == 4) *(uint32_t*)(q + at) = bytes4(b[0], b[1], b[2], b[3]);
+        else *(uint2*)(q + at) = make_uint2(bytes4(b[0], b[1], b[2], b[3]), bytes4(b[4], b[5], b[6], b[7]));
       }
       if (lane == 0) a.scale[m] = s.s;
     }
@@ -144,7 +164,12 @@ __global__ void __launch_bounds__(kThreads) quantize_long_kernel(const __grid_co
 #pragma unroll
     for (int i = 0; i < kThreads / 32; i++) top = max(top, sh[i]);
     const Scale s(top);
-    for (int k = threadIdx.x; k < a.K; k += kThreads) a.q[m * a.ld + k] = (int8_t)quantize(to_f(x[k * a.x.cs]), s);
+    for (int k = threadIdx.x; k < a.K; k += kThreads) {
+      const float f[1] = {to_f(x[k * a.x.cs])};
+      int q[1];
+      quantize(f, s, q);
+      a.q[m * a.ld + k] = (int8_t)q[0];
+    }
     if (threadIdx.x == 0) a.scale[m] = s.s;
   }
 }
@@ -158,7 +183,7 @@ __global__ void __launch_bounds__(512) quantize_image_kernel(const __grid_consta
   constexpr int kPixels = 32 * VP;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
   const int words = (a.K + 3) / 4, pitch = words | 1;
-  uint32_t* const tops = sh + kPixels * pitch;  // [2][warps][kPixels]
+  uint32_t* const tops = sh + kPixels * pitch;  // [2][warps][up to kPixels]
   int turn = 0;
   const int64_t tiles = (a.M + kPixels - 1) / kPixels;
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
@@ -171,24 +196,38 @@ __global__ void __launch_bounds__(512) quantize_image_kernel(const __grid_consta
         x[i] = c < a.K && m < a.M ? load_pixels<T, VP>(a.x, m, c, a.M) : chunk_zero<T, VP>();
       }
     };
-    uint32_t top[VP] = {};
+    // magnitudes of 16-bit neighbours stay in pairs
+    constexpr int kTops = sizeof(T) == 2 && VP > 1 ? VP / 2 : VP;
+    const auto larger = [](uint32_t p, uint32_t q) { return kTops < VP ? __vmaxu2(p, q) : max(p, q); };
+    uint32_t top[kTops] = {};
     load(0);
     for (int k0 = 0; k0 < (LONG ? a.K : 1); k0 += R * warps) {
       if (LONG && k0) load(k0);
 #pragma unroll
       for (int i = 0; i < R; i++)
 #pragma unroll
-        for (int j = 0; j < VP; j++) top[j] = max(top[j], __float_as_uint(to_f(x[i].v[j])) & 0x7fffffffu);
+        for (int j = 0; j < kTops; j++) {
+          if constexpr (kTops < VP) top[j] = __vmaxu2(top[j], ((const uint32_t*)x[i].v)[j] & 0x7fff7fffu);
+          else top[j] = max(top[j], __float_as_uint(to_f(x[i].v[j])) & 0x7fffffffu);
+        }
     }
-    uint32_t* const own = tops + turn * warps * kPixels + lane;
+    uint32_t* const own = tops + turn * warps * 32 * kTops + lane;
 #pragma unroll
-    for (int j = 0; j < VP; j++) own[(warp * VP + j) * 32] = top[j];
+    for (int j = 0; j < kTops; j++) own[(warp * kTops + j) * 32] = top[j];
     __syncthreads();
     Scale s[VP];
 #pragma unroll
+    for (int j = 0; j < kTops; j++) {
+      for (int w = 0; w < warps; w++) top[j] = larger(top[j], own[(w * kTops + j) * 32]);
+    }
+#pragma unroll
     for (int j = 0; j < VP; j++) {
-      for (int w = 0; w < warps; w++) top[j] = max(top[j], own[(w * VP + j) * 32]);
-      s[j] = Scale(top[j]);
+      if constexpr (kTops < VP) {
+        const uint16_t h = (uint16_t)(j % 2 ? top[j / 2] >> 16 : top[j / 2] & 0xffffu);
+        s[j] = Scale(__float_as_uint(to_f(*(const T*)&h)));
+      } else {
+        s[j] = Scale(top[j]);
+      }
       if (warp == 0 && m + j < a.M) a.scale[m + j] = s[j].s;
     }
     if (LONG) load(0);
@@ -199,19 +238,24 @@ __global__ void __launch_bounds__(512) quantize_image_kernel(const __grid_consta
         const int w = k0 / 4 + i / 4 * warps + warp;
         if (w < words) {
 #pragma unroll
-          for (int j = 0; j < VP; j++)
-            sh[(j * 32 + lane) * pitch + w] = bytes4(quantize(to_f(x[i].v[j]), s[j]), quantize(to_f(x[i + 1].v[j]), s[j]),
-                                                     quantize(to_f(x[i + 2].v[j]), s[j]), quantize(to_f(x[i + 3].v[j]), s[j]));
+          for (int j = 0; j < VP; j++) {
+            const float f[4] = {to_f(x[i].v[j]), to_f(x[i + 1].v[j]), to_f(x[i + 2].v[j]), to_f(x[i + 3].v[j])};
+            int q[4];
+            quantize(f, s[j], q);
+            sh[(j * 32 + lane) * pitch + w] = bytes4(q[0], q[1], q[2], q[3]);
+          }
         }
       }
     }
     __syncthreads();
     const int64_t first = tile * kPixels;
-    const int count = (int)min((int64_t)kPixels, a.M - first) * words;
-    for (int i = threadIdx.x; i < count; i += blockDim.x) {
-      const int p = i / words, w = i - p * words;
-      *(uint32_t*)(a.q + (first + p) * a.ld + 4 * w) = sh[(p % VP * 32 + p / VP) * pitch + w];
-    }
+    // a pixel's words by as many lanes as a power of two holds
+    const int count = (int)min((int64_t)kPixels, a.M - first);
+    int span = 1;
+    while (span < words && span < 32) span *= 2;
+    for (int p = threadIdx.x / span; p < count; p += blockDim.x / span)
+      for (int w = threadIdx.x % span; w < words; w += span)
+        *(uint32_t*)(a.q + (first + p) * a.ld + 4 * w) = sh[(p % VP * 32 + p / VP) * pitch + w];
   }
 }
 
