@@ -586,3 +586,31 @@ def test_results_of_images_beyond_2_31_elements():
 
 def test_heads_status_stays_clear():
     assert _heads().device_status() == 0
+
+
+@pytest.mark.parametrize("dt", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("M,K,N,act,order,bias,residual", [
+    (32768, 64, 64, "none", "rows", True, False),
+    (32769, 64, 33, "relu", "rows", False, True),
+    (40001, 8, 64, "silu", "rows", True, True),
+    (33000, 40, 5, "gelu", "padded", True, False),
+    (32768, 64, 64, "gelu", "image", True, True),
+    (32770, 33, 64, "sigmoid", "image", True, True),
+    (100002, 5, 40, "silu", "image", False, False),
+    (38001, 64, 64, "none", "image-odd", True, True),  # not in whole pairs
+])
+def test_linear_act_int8_of_few_features(M, K, N, act, order, bias, residual, dt):
+    heads, g = _heads(), _gen(M + K + N)
+    x = hl.matrix(M, K, dt, g, order)
+    if K > 1:
+        x[M - 1, 1], x[7, 0], x[M // 2] = NAN, INF, 0
+    w = heads.quantize_rows(hl.matrix(N, K, F32, g, scale=1.5 / K ** 0.5))
+    b = hl.matrix(1, N, dt, g, scale=0.3)[0] if bias else None
+    r = hl.matrix(M, N, dt, g, "image" if order.startswith("image") else "rows") if residual else None
+    y = heads.linear_act_int8(x, w, b, residual=r, activation=act)
+    fine = torch.ones(M, dtype=torch.bool, device="cuda")
+    fine[[7, M - 1]] = False
+    assert bool(torch.isnan(y[~fine]).all())
+    q, s = dl.quantize(x)
+    value, bound = dl.linear_act_int8(q, s, *w, b, r, act, dt)
+    hl.assert_within("y", y[fine], (value[fine], bound[fine]))

@@ -1184,6 +1184,10 @@ int int8_forward(Run& r, int dtype, int act, const vi_matrix* x, const float* x_
   e.out = view(y);
   e.col_scale = w_scale;
   e.row_scale = x_scale;
+  if (!x_scale && int8_fused(dtype, M, N, K, view(x))) {
+    if (int rc = operand8(r, w, B)) return rc;
+    return r.dry ? VI_OK : launch_int8_fused(dtype, M, view(x), B, e, r.sms, r.s);
+  }
   if (x_scale) {
     if (int rc = operand8(r, x, A)) return rc;
   } else {

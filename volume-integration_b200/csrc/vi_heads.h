@@ -165,6 +165,9 @@ cudaError_t launch_small(int dtype, const SmallJob& a, const SmallJob* b, cudaSt
 // kEpiInt8's product (vi_heads_int8.cu): operands of 8-bit integers, k contiguous, ld a multiple of 16.
 constexpr int64_t kInt8Terms = 1 << 17;  // 127^2 of each fit the 32-bit sum
 int launch_int8_gemm(int dtype, const Operand& a, const Operand& b, const Plan& p, const Epilogue& e, int sms, cudaStream_t s);
+// The same with float rows of few features, quantised in the kernel (e.row_scale is not read).
+bool int8_fused(int dtype, int64_t M, int64_t N, int64_t K, const View& x);
+int launch_int8_fused(int dtype, int64_t M, const View& x, const Operand& b, const Epilogue& e, int sms, cudaStream_t s);
 
 // Rows of 8-bit integers with a scale each: q = x / scale rounded to even, scale = largest |x| / 127.
 struct QuantArgs {
