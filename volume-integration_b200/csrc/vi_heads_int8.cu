@@ -12,12 +12,12 @@ namespace {
 // ---- few features: quantised on the way into the product ----
 // Up to 64 features and 64 channels of 16-bit types are bound by memory and by the epilogue, and a pass that quantises would
 // write and read the features once more (2M x 64 -> 64 with gelu and a residual: 284 us + 235 apart).  Here one warp
-// copies 256 rows of x at a time into shared memory, four find their scales and write the tensor core's operand, two products
-// of 128 rows follow, and 16 warps run the epilogue.
+// copies 256 rows of x at a time into shared memory, eight find their scales and write the tensor core's operand, two products
+// of 128 rows follow, and 8 warps run the epilogue.
 constexpr int kFusedK = 64, kFusedN = 64;
 template <typename T>
 struct Fused {
-  static constexpr int kEpi = 16, kMake = 4, kThreads = (kEpi + kMake + 2) * 32, kRows = 256;
+  static constexpr int kEpi = 16, kMake = 8, kThreads = (kEpi + kMake + 2) * 32, kRows = 256;
   static constexpr int kStage = kRows * 128, kStages = 2, kScales = 4;
   static constexpr int kX = kStages * kStage, kXBytes = kRows * kFusedK * 2, kXStages = 3;
   static constexpr int kB = kX + kXStages * kXBytes, kStaging = kB + kFusedN * 128;
@@ -78,28 +78,30 @@ __global__ void __launch_bounds__(Fused<T>::kThreads, 1) int8_fused_kernel(const
   float* const scales = (float*)(smem + S::kScale);
 
   if (warp >= S::kEpi && warp < S::kEpi + S::kMake) {
-    // ---- quantise: 64 rows a warp ----
-    const int first = (warp - S::kEpi) * 64;
+    // ---- quantise: 32 rows a warp ----
+    const int first = (warp - S::kEpi) * (S::kRows / S::kMake);
     int i = 0, xs = 0;
     uint32_t xphase = 0;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, i++) {
       const uint32_t base = smem_u32(smem) + (i & 1) * S::kStage, x = smem_u32(smem + S::kX) + xs * S::kXBytes;
       // the last product that read this stage has ended, and with it the epilogue of four tiles ago
       if (!mbar_wait(xfull + 8 * xs, xphase, dead, kWaitLimit) || !mbar_wait(aempty + 8 * (i & 1), (i / 2 & 1) ^ 1, dead, kWaitLimit)) break;
-      if (a.image) {  // a lane: two neighbouring pixels, every channel
-        const uint32_t own = x + (first + 2 * lane) * 2;
+      if (a.image) {  // a lane: two neighbouring pixels, half of the channels
+        const int pair_row = first + lane % 16 * 2, k0 = lane / 16 * (kFusedK / 2);
+        const uint32_t own = x + pair_row * 2 + k0 * (S::kRows * 2);
         uint32_t top = 0;
-#pragma unroll 16
-        for (int k = 0; k < kFusedK; k++) top = __vmaxu2(top, lds_cell(own + k * (S::kRows * 2), 0u) & 0x7fff7fffu);
+#pragma unroll
+        for (int k = 0; k < kFusedK / 2; k++) top = __vmaxu2(top, lds_cell(own + k * (S::kRows * 2), 0u) & 0x7fff7fffu);
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 16));
         Scale s[2];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           const uint16_t h = (uint16_t)(j ? top >> 16 : top & 0xffffu);
           s[j] = Scale(__float_as_uint(to_f(*(const T*)&h)));
-          scales[(i & 3) * S::kRows + first + 2 * lane + j] = s[j].s;
+          if (lane < 16) scales[(i & 3) * S::kRows + pair_row + j] = s[j].s;
         }
-#pragma unroll 1
-        for (int c = 0; c < kFusedK / 16; c++) {
+#pragma unroll
+        for (int c = 0; c < kFusedK / 32; c++) {
           uint32_t w[2][4];
 #pragma unroll
           for (int g = 0; g < 4; g++) {
@@ -117,11 +119,11 @@ __global__ void __launch_bounds__(Fused<T>::kThreads, 1) int8_fused_kernel(const
             }
           }
 #pragma unroll
-          for (int j = 0; j < 2; j++) sts128(swizzled(base, first + 2 * lane + j, c), make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]));
+          for (int j = 0; j < 2; j++) sts128(swizzled(base, pair_row + j, k0 / 16 + c), make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]));
         }
       } else {  // 8 lanes a row, 8 features each
-#pragma unroll 4
-        for (int n = 0; n < 16; n++) {
+#pragma unroll
+        for (int n = 0; n < S::kRows / S::kMake / 4; n++) {
           const int r = first + n * 4 + lane / 8;
           const uint4 u = lds128(x + r * (kFusedK * 2) + lane % 8 * 16);
           uint32_t top = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
@@ -194,8 +196,8 @@ __global__ void __launch_bounds__(Fused<T>::kThreads, 1) int8_fused_kernel(const
       }
     }
   } else {
-    // ---- epilogue: a warp 32 rows x 32 columns ----
-    const int quad = warp % 4, half = warp / 4 % 2, c = warp / 8 * 32;
+    // ---- epilogue: a warp 32 columns of 32 rows of each product ----
+    const int quad = warp % 4, c = warp / 4 % 2 * 32;
     const uint32_t st = smem_u32(smem + S::kStaging) + warp * S::kWarpBytes, bias_slot = st + 32 * 32 * (int)sizeof(T);
     const Epilogue& e = a.e;
     const int out_access = access_of<T>(e.out), res_access = access_of<T>(e.res);
@@ -206,44 +208,53 @@ __global__ void __launch_bounds__(Fused<T>::kThreads, 1) int8_fused_kernel(const
     }
     __syncwarp();
     int i = 0;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, i++) {
-      const int row = half * 128 + quad * 32;
-      const int64_t m0 = t * S::kRows + row;
-      const bool some = m0 < a.M && c < a.N;
-      const Place here{(int)m0, c, (int)min((int64_t)32, a.M - m0), min(32, a.N - c)};
-      Row<T> extra, y;
-      int way = kNone;
-      if (some && e.res.p) way = load_tile<T>(extra, e.res, res_access, st, lane, here);  // asked for before the product is waited for
-      bool on = mbar_wait(sfull + 8 * (i & 3), i / 4 & 1, dead, kWaitLimit) && mbar_wait(tfull + 8 * (i & 1), i / 2 & 1, dead, kWaitLimit);
-      if (!__all_sync(0xffffffffu, on)) break;
-      fence_after();
-      if (some) {
-        const float row_scale = scales[(i & 3) * S::kRows + row + lane];
-        const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + (i & 1) * 128 + half * 64 + c;
-        if (e.res.p) own_row<T>(extra, way, st, lane);
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          float2 v[8];
-          tmem_load16(src + h * 16, (float*)v);
-          tmem_wait_load();
-          scale_sums(bias_slot + 128 + h * 64, row_scale, v);
-          if (e.bias) add_bias<16>(bias_slot + h * 64, v);
-#pragma unroll
-          for (int j = 0; j < 8; j++) {
-            float2 w, d;
-            activate<ACT, false, false>(v[j], w, d);
-            v[j] = ACT == VI_ACT_RELU ? relu_signed_zero<T>(w) : w;
-            if (e.res.p) v[j] = __fadd2_rn(v[j], get_pair(extra, h * 8 + j));
-            set_pair(y, h * 8 + j, v[j]);
-          }
-#pragma unroll
-          for (int j = 0; j < 8; j++) asm volatile("" : "+r"(y.w[h * 8 + j]));
+    bool on = true;
+    for (int64_t t = blockIdx.x; t < tiles && on; t += gridDim.x, i++) {
+      {
+        const int half = warp / 8;
+        const int row = half * 128 + quad * 32;
+        const int64_t m0 = t * S::kRows + row;
+        const bool some = m0 < a.M && c < a.N;
+        const Place here{(int)m0, c, (int)min((int64_t)32, a.M - m0), min(32, a.N - c)};
+        Row<T> extra, y;
+        int way = kNone;
+        if (some && e.res.p) way = load_tile<T>(extra, e.res, res_access, st, lane, here);  // asked for before the product is waited for
+        {
+          on = mbar_wait(sfull + 8 * (i & 3), i / 4 & 1, dead, kWaitLimit) && mbar_wait(tfull + 8 * (i & 1), i / 2 & 1, dead, kWaitLimit);
+          on = __all_sync(0xffffffffu, on);
+          if (!on) break;
+          fence_after();
         }
+        if (some) {
+          const float row_scale = scales[(i & 3) * S::kRows + row + lane];
+          const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + (i & 1) * 128 + half * 64 + c;
+          if (e.res.p) own_row<T>(extra, way, st, lane);
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            float2 v[8];
+            tmem_load16(src + h * 16, (float*)v);
+            tmem_wait_load();
+            scale_sums(bias_slot + 128 + h * 64, row_scale, v);
+            if (e.bias) add_bias<16>(bias_slot + h * 64, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+              float2 w, d;
+              activate<ACT, false, false>(v[j], w, d);
+              v[j] = ACT == VI_ACT_RELU ? relu_signed_zero<T>(w) : w;
+              if (e.res.p) v[j] = __fadd2_rn(v[j], get_pair(extra, h * 8 + j));
+              set_pair(y, h * 8 + j, v[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) asm volatile("" : "+r"(y.w[h * 8 + j]));
+          }
+        }
+        {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(tempty + 8 * (i & 1));
+        }
+        if (some) store_tile(y, e.out, out_access, st, lane, here);
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(tempty + 8 * (i & 1));
-      if (some) store_tile(y, e.out, out_access, st, lane, here);
     }
   }
   __syncwarp();
