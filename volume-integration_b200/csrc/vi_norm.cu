@@ -78,44 +78,84 @@ __device__ __forceinline__ void store_row(const Chunk<T, VEC> (&c)[NV], const Vi
 constexpr int kRowThreads = 256;  // of a block whose rows belong to lanes
 constexpr int kBlockMost = 512;   // of a block that a row belongs to
 
+// A lane's elements of a row as pairs, which one instruction adds or multiplies.
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void pairs_of(const Chunk<T, VEC> (&c)[NV], float2 (&p)[(VEC * NV + 1) / 2]) {
+#pragma unroll
+  for (int i = 0; i < VEC * NV; i += 2)
+    p[i / 2] = make_float2(to_f(c[i / VEC].v[i % VEC]), i + 1 < VEC * NV ? to_f(c[(i + 1) / VEC].v[(i + 1) % VEC]) : 0.0f);
+}
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void chunks_of(const float2 (&p)[(VEC * NV + 1) / 2], Chunk<T, VEC> (&c)[NV]) {
+#pragma unroll
+  for (int i = 0; i < VEC * NV; i += 2) {
+    if constexpr (sizeof(T) == 2 && VEC > 1) {
+      ((uint32_t*)c[i / VEC].v)[i % VEC / 2] = pack2(p[i / 2], T());
+    } else {
+      c[i / VEC].v[i % VEC] = from_f<T>(p[i / 2].x);
+      if (i + 1 < VEC * NV) c[(i + 1) / VEC].v[(i + 1) % VEC] = from_f<T>(p[i / 2].y);
+    }
+  }
+}
+// Whether element i of the lane lies in the row (whole vectors do or do not).
+template <int VEC>
+__device__ __forceinline__ bool in_row(int i, int lanes, int lane, int K) {
+  return (i / VEC * lanes + lane) * VEC < K;
+}
+template <int N>
+__device__ __forceinline__ float total(const float2 (&p)[N]) {
+  float2 s[2] = {pair(0.0f), pair(0.0f)};
+#pragma unroll
+  for (int i = 0; i < N; i++) s[i & 1] = __fadd2_rn(s[i & 1], p[i]);
+  s[0] = __fadd2_rn(s[0], s[1]);
+  return s[0].x + s[0].y;
+}
+
 // R rows at a time for each group of lanes, so that short rows have loads in flight too.
 template <typename T, int VEC, int NV, int R, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
     norm_rows_forward(const __grid_constant__ NormArgs a, int lanes) {
   __shared__ float sh1[2][16][R], sh2[2][16][2 * R];
+  constexpr int E = VEC * NV, P = (E + 1) / 2;
   int turn1 = 0, turn2 = 0;
   const int lane = BLOCK ? threadIdx.x : threadIdx.x % lanes, group = BLOCK ? 0 : threadIdx.x / lanes;
   const int groups = BLOCK ? 1 : kRowThreads / lanes;
   const float inv = 1.0f / (float)a.K;
-  Chunk<T, VEC> w[NV], b[NV];
-  load_weights(w, a.w, 1.0f, a.K, lanes, lane);
-  load_weights(b, a.b, 0.0f, a.K, lanes, lane);
+  float2 w[P], b[P];
+  {
+    Chunk<T, VEC> c[NV];
+    load_weights(c, a.w, 1.0f, a.K, lanes, lane);
+    pairs_of(c, w);
+    load_weights(c, a.b, 0.0f, a.K, lanes, lane);
+    pairs_of(c, b);
+  }
   for (int64_t m0 = (int64_t)blockIdx.x * groups * R; m0 < a.M; m0 += (int64_t)gridDim.x * groups * R) {
-    Chunk<T, VEC> x[R][NV];
+    float2 x[R][P];
+    {
+      Chunk<T, VEC> c[R][NV];
 #pragma unroll
-    for (int r = 0; r < R; r++) load_row(x[r], a.x, min(m0 + r * groups + group, a.M - 1), a.K, lanes, lane);
+      for (int r = 0; r < R; r++) load_row(c[r], a.x, min(m0 + r * groups + group, a.M - 1), a.K, lanes, lane);
+#pragma unroll
+      for (int r = 0; r < R; r++) pairs_of(c[r], x[r]);
+    }
     float mean[R], q[2 * R];
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-      mean[r] = 0.0f;
-#pragma unroll
-      for (int v = 0; v < NV; v++)
-#pragma unroll
-        for (int i = 0; i < VEC; i++) mean[r] += to_f(x[r][v].v[i]);
-    }
+    for (int r = 0; r < R; r++) mean[r] = total(x[r]);
     row_sum<R, BLOCK>(mean, lanes, sh1, turn1);
 #pragma unroll
     for (int r = 0; r < R; r++) {
       mean[r] *= inv;
-      q[2 * r] = q[2 * r + 1] = 0.0f;
+      float2 s1 = pair(0.0f), s2 = pair(0.0f);
 #pragma unroll
-      for (int v = 0; v < NV; v++)
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-          const float d = (v * lanes + lane) * VEC < a.K ? to_f(x[r][v].v[i]) - mean[r] : 0.0f;
-          q[2 * r] += d;
-          q[2 * r + 1] = fmaf(d, d, q[2 * r + 1]);
-        }
+      for (int i = 0; i < P; i++) {
+        x[r][i] = __fadd2_rn(x[r][i], pair(-mean[r]));
+        if (!in_row<VEC>(2 * i, lanes, lane, a.K)) x[r][i].x = 0.0f;
+        if (2 * i + 1 >= E || !in_row<VEC>(2 * i + 1, lanes, lane, a.K)) x[r][i].y = 0.0f;
+        s1 = __fadd2_rn(s1, x[r][i]);
+        s2 = __ffma2_rn(x[r][i], x[r][i], s2);
+      }
+      q[2 * r] = s1.x + s1.y;
+      q[2 * r + 1] = s2.x + s2.y;
     }
     row_sum<2 * R, BLOCK>(q, lanes, sh2, turn2);
 #pragma unroll
@@ -124,12 +164,10 @@ __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
       const float shift = q[2 * r] * inv;
       const float rstd = 1.0f / sqrtf(fmaxf(fmaf(-shift, shift, q[2 * r + 1] * inv), 0.0f) + a.eps);
       if (m < a.M) {
+#pragma unroll
+        for (int i = 0; i < P; i++) x[r][i] = __ffma2_rn(__fmul2_rn(__fadd2_rn(x[r][i], pair(-shift)), pair(rstd)), w[i], b[i]);
         Chunk<T, VEC> y[NV];
-#pragma unroll
-        for (int v = 0; v < NV; v++)
-#pragma unroll
-          for (int i = 0; i < VEC; i++)
-            y[v].v[i] = from_f<T>(fmaf((to_f(x[r][v].v[i]) - mean[r] - shift) * rstd, to_f(w[v].v[i]), to_f(b[v].v[i])));
+        chunks_of(x[r], y);
         store_row(y, a.y, m, a.K, lanes, lane);
         if (a.stats && lane == 0) a.stats[m] = mean[r], a.stats[a.M + m] = shift, a.stats[2 * a.M + m] = rstd;
       }
@@ -137,21 +175,29 @@ __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
   }
 }
 
+// The next rows are asked for before the present ones are worked on.
 template <typename T, int VEC, int NV, int R, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
     norm_rows_backward(const __grid_constant__ NormArgs a, int lanes) {
   __shared__ float sh[2][16][2 * R];
   __shared__ float cols[BLOCK ? 1 : kRowThreads / 32][BLOCK ? 1 : 32 * VEC * NV];
+  constexpr int E = VEC * NV, P = (E + 1) / 2;
   int turn = 0;
   const int lane = BLOCK ? threadIdx.x : threadIdx.x % lanes, group = BLOCK ? 0 : threadIdx.x / lanes;
   const int groups = BLOCK ? 1 : kRowThreads / lanes;
   const float inv = 1.0f / (float)a.K;
-  Chunk<T, VEC> w[NV];
-  load_weights(w, a.w, 1.0f, a.K, lanes, lane);
-  float dw[NV][VEC] = {}, db[NV][VEC] = {};
-  for (int64_t m0 = (int64_t)blockIdx.x * groups * R; m0 < a.M; m0 += (int64_t)gridDim.x * groups * R) {
-    Chunk<T, VEC> x[R][NV], dy[R][NV];
-    float mean[R], shift[R], rstd[R], q[2 * R];
+  float2 w[P];
+  {
+    Chunk<T, VEC> c[NV];
+    load_weights(c, a.w, 1.0f, a.K, lanes, lane);
+    pairs_of(c, w);
+  }
+  float2 dw[P], db[P];
+#pragma unroll
+  for (int i = 0; i < P; i++) dw[i] = db[i] = pair(0.0f);
+  Chunk<T, VEC> x[R][NV], dy[R][NV];
+  float mean[R], shift[R], rstd[R];
+  const auto load = [&](int64_t m0) {
 #pragma unroll
     for (int r = 0; r < R; r++) {
       const int64_t m = min(m0 + r * groups + group, a.M - 1);
@@ -159,24 +205,36 @@ __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
       load_row(dy[r], a.dy, m, a.K, lanes, lane);
       mean[r] = a.stats[m], shift[r] = a.stats[a.M + m], rstd[r] = a.stats[2 * a.M + m];
     }
+  };
+  int64_t m0 = (int64_t)blockIdx.x * groups * R;
+  const int64_t step = (int64_t)gridDim.x * groups * R;
+  if (m0 < a.M) load(m0);
+  for (; m0 < a.M; m0 += step) {
+    float2 h[R][P], g[R][P];
+    float q[2 * R], scale[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
+      pairs_of(x[r], h[r]);
+      pairs_of(dy[r], g[r]);
+      scale[r] = rstd[r];
       const bool on = m0 + r * groups + group < a.M;
-      q[2 * r] = q[2 * r + 1] = 0.0f;
+      float2 s1 = pair(0.0f), s2 = pair(0.0f);
 #pragma unroll
-      for (int v = 0; v < NV; v++)
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-          // beyond K and beyond M nothing is added: h of a zero is not one
-          const bool in = on && (v * lanes + lane) * VEC < a.K;
-          const float h = in ? (to_f(x[r][v].v[i]) - mean[r] - shift[r]) * rstd[r] : 0.0f, d = in ? to_f(dy[r][v].v[i]) : 0.0f;
-          const float g = d * to_f(w[v].v[i]);
-          q[2 * r] += g;
-          q[2 * r + 1] = fmaf(g, h, q[2 * r + 1]);
-          dw[v][i] = fmaf(d, h, dw[v][i]);
-          db[v][i] += d;
-        }
+      for (int i = 0; i < P; i++) {
+        // beyond K and beyond M nothing is added: h of a zero is not one
+        h[r][i] = __fmul2_rn(__fadd2_rn(__fadd2_rn(h[r][i], pair(-mean[r])), pair(-shift[r])), pair(rstd[r]));
+        if (!on || !in_row<VEC>(2 * i, lanes, lane, a.K)) h[r][i].x = 0.0f, g[r][i].x = 0.0f;
+        if (!on || 2 * i + 1 >= E || !in_row<VEC>(2 * i + 1, lanes, lane, a.K)) h[r][i].y = 0.0f, g[r][i].y = 0.0f;
+        dw[i] = __ffma2_rn(g[r][i], h[r][i], dw[i]);
+        db[i] = __fadd2_rn(db[i], g[r][i]);
+        g[r][i] = __fmul2_rn(g[r][i], w[i]);
+        s1 = __fadd2_rn(s1, g[r][i]);
+        s2 = __ffma2_rn(g[r][i], h[r][i], s2);
+      }
+      q[2 * r] = s1.x + s1.y;
+      q[2 * r + 1] = s2.x + s2.y;
     }
+    if (m0 + step < a.M) load(m0 + step);
     if (!a.y.p) continue;
     row_sum<2 * R, BLOCK>(q, lanes, sh, turn);
 #pragma unroll
@@ -184,14 +242,11 @@ __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
       const int64_t m = m0 + r * groups + group;
       if (m < a.M) {
         const float mg = q[2 * r] * inv, mgh = q[2 * r + 1] * inv;
+#pragma unroll
+        for (int i = 0; i < P; i++)
+          g[r][i] = __fmul2_rn(__ffma2_rn(h[r][i], pair(-mgh), __fadd2_rn(g[r][i], pair(-mg))), pair(scale[r]));
         Chunk<T, VEC> y[NV];
-#pragma unroll
-        for (int v = 0; v < NV; v++)
-#pragma unroll
-          for (int i = 0; i < VEC; i++) {
-            const float h = (to_f(x[r][v].v[i]) - mean[r] - shift[r]) * rstd[r];
-            y[v].v[i] = from_f<T>(rstd[r] * (fmaf(to_f(dy[r][v].v[i]), to_f(w[v].v[i]), -mg) - h * mgh));
-          }
+        chunks_of(g[r], y);
         store_row(y, a.y, m, a.K, lanes, lane);
       }
     }
@@ -201,18 +256,17 @@ __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
 #pragma unroll
   for (int which = 0; which < 2; which++) {
 #pragma unroll
-    for (int v = 0; v < NV; v++)
-#pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        float s = which ? db[v][i] : dw[v][i];
-        const int at = (v * lanes + lane) * VEC + i;
-        if constexpr (BLOCK) {
-          if (at < a.K) out[which * a.K + at] = s;
-        } else {
-          for (int o = lanes; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          if (threadIdx.x % 32 < lanes) cols[threadIdx.x / 32][at] = s;
-        }
+    for (int i = 0; i < E; i++) {
+      const float2 v = which ? db[i / 2] : dw[i / 2];
+      float s = i % 2 ? v.y : v.x;
+      const int at = (i / VEC * lanes + lane) * VEC + i % VEC;
+      if constexpr (BLOCK) {
+        if (at < a.K) out[which * a.K + at] = s;
+      } else {
+        for (int o = lanes; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (threadIdx.x % 32 < lanes) cols[threadIdx.x / 32][at] = s;
       }
+    }
     if constexpr (!BLOCK) {
       __syncthreads();
       for (int c = threadIdx.x; c < a.K; c += kRowThreads) {
@@ -340,9 +394,210 @@ __device__ __forceinline__ void tile_put(const float (&s)[VP], float* sh, int wa
   for (int j = 0; j < VP; j++) sh[(warp * VP + j) * 32 + lane] = s[j];
 }
 
-// LONG: more channels than the warps hold, so each step reads them again.
-template <typename T, int VP, int R, bool LONG>
-__global__ void __launch_bounds__(512) norm_image_forward(const __grid_constant__ NormArgs a, int warps) {
+// One pixel or two as a value that one instruction adds or multiplies.
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float fma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float2 fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+// VP pixels of one channel as they lie in memory: a pair of 16-bit ones in a word.
+template <typename T, int VP>
+struct Pixels;
+template <typename T>
+struct Pixels<T, 1> {
+  using V = float;
+  T t;
+  __device__ __forceinline__ void load(const View& m, int64_t row, int64_t c, int64_t M) { t = ((const T*)m.p)[row * m.rs + c * m.cs]; }
+  __device__ __forceinline__ V get() const { return to_f(t); }
+  static __device__ __forceinline__ void store(V v, const View& m, int64_t row, int64_t c, int64_t M) {
+    ((T*)m.p)[row * m.rs + c * m.cs] = from_f<T>(v);
+  }
+  static __device__ __forceinline__ V all(float f) { return f; }
+  static __device__ __forceinline__ float sum(V v) { return v; }
+};
+template <typename T>
+struct Pixels<T, 2> {
+  using V = float2;
+  uint32_t w;
+  __device__ __forceinline__ void load(const View& m, int64_t row, int64_t c, int64_t M) {
+    const T* p = (const T*)m.p + row + c * m.cs;
+    w = row + 1 < M ? *(const uint32_t*)p : *(const uint16_t*)p;
+  }
+  __device__ __forceinline__ V get() const {
+    const T* t = (const T*)&w;
+    return make_float2(to_f(t[0]), to_f(t[1]));
+  }
+  static __device__ __forceinline__ void store(V v, const View& m, int64_t row, int64_t c, int64_t M) {
+    T* p = (T*)m.p + row + c * m.cs;
+    if (row + 1 < M) *(uint32_t*)p = pack2(v, T());
+    else *p = from_f<T>(v.x);
+  }
+  static __device__ __forceinline__ V all(float f) { return pair(f); }
+  static __device__ __forceinline__ float sum(V v) { return v.x + v.y; }
+};
+// Sum of a lane's value over the warps of its tile, in order, through sh (one value a thread of the block).
+template <typename V>
+__device__ __forceinline__ V tile_total(V v, V* sh, int warps) {
+  if (warps == 1) return v;
+  sh[threadIdx.x] = v;
+  __syncthreads();
+  const int first = threadIdx.x / 32 / warps * warps * 32 + threadIdx.x % 32;
+  v = sh[first];
+  for (int i = 1; i < warps; i++) v = add(v, sh[first + i * 32]);
+  return v;
+}
+
+// The channels' weights, doubled, in shared memory: (w, w, b, b).
+template <typename T>
+__device__ __forceinline__ void stage_weights(float4* to, const NormArgs& a) {
+  for (int c = threadIdx.x; c < a.K; c += blockDim.x) {
+    const float w = a.w ? to_f(((const T*)a.w)[c]) : 1.0f, b = a.b ? to_f(((const T*)a.b)[c]) : 0.0f;
+    to[c] = make_float4(w, w, b, b);
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ float low(float4 q, float) { return q.x; }
+__device__ __forceinline__ float2 low(float4 q, float2) { return make_float2(q.x, q.y); }
+__device__ __forceinline__ float high(float4 q, float) { return q.z; }
+__device__ __forceinline__ float2 high(float4 q, float2) { return make_float2(q.z, q.w); }
+
+// A lane holds every warps-th channel of its pixels, up to R, as they lie in memory.  With one warp a tile (up to 64 channels)
+// nothing is exchanged, and a warp has 8 KB on the way at a time.
+constexpr int kImageThreads = 256;
+template <typename T, int VP, int R>
+__global__ void __launch_bounds__(kImageThreads) norm_image_forward(const __grid_constant__ NormArgs a, int warps) {
+  using X = Pixels<T, VP>;
+  using V = typename X::V;
+  extern __shared__ float4 weights[];
+  V* const sh = (V*)(weights + a.K);  // three exchanges
+  stage_weights<T>(weights, a);
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, per = kImageThreads / 32 / warps;
+  const V inv = X::all(1.0f / (float)a.K);
+  const int64_t tiles = (a.M + 32 * VP - 1) / (32 * VP);
+  for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < tiles; t0 += (int64_t)gridDim.x * per) {
+    const int64_t m = ((t0 + warp / warps) * 32 + lane) * VP;
+    const bool on = m < a.M;
+    X x[R];
+    V s = X::all(0.0f);
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < R; i++)
+        if (tw + i * warps < a.K) x[i].load(a.x, m, tw + i * warps, a.M);
+#pragma unroll
+      for (int i = 0; i < R; i++)
+        if (tw + i * warps < a.K) s = add(s, x[i].get());
+    }
+    const V mean = mul(tile_total(s, sh, warps), inv), less = mul(mean, X::all(-1.0f));
+    V s1 = X::all(0.0f), s2 = s1;
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < R; i++)
+        if (tw + i * warps < a.K) {
+          const V d = add(x[i].get(), less);
+          s1 = add(s1, d);
+          s2 = fma(d, d, s2);
+        }
+    }
+    const V shift = mul(tile_total(s1, sh + kImageThreads, warps), inv), sq = mul(tile_total(s2, sh + 2 * kImageThreads, warps), inv);
+    if (!on) continue;
+    V var = fma(mul(shift, X::all(-1.0f)), shift, sq), rstd;
+#pragma unroll
+    for (int j = 0; j < VP; j++) {
+      ((float*)&rstd)[j] = 1.0f / sqrtf(fmaxf(((float*)&var)[j], 0.0f) + a.eps);
+      if (a.stats && tw == 0 && m + j < a.M) {
+        a.stats[m + j] = ((const float*)&mean)[j];
+        a.stats[a.M + m + j] = ((const float*)&shift)[j];
+        a.stats[2 * a.M + m + j] = ((const float*)&rstd)[j];
+      }
+    }
+    const V under = mul(shift, X::all(-1.0f));
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int c = tw + i * warps;
+      if (c < a.K) {
+        const float4 q = weights[c];
+        X::store(fma(mul(add(add(x[i].get(), less), under), rstd), low(q, V()), high(q, V())), a.y, m, c, a.M);
+      }
+    }
+  }
+}
+
+template <typename T, int VP, int R>
+__global__ void __launch_bounds__(kImageThreads, 2) norm_image_backward(const __grid_constant__ NormArgs a, int warps) {
+  using X = Pixels<T, VP>;
+  using V = typename X::V;
+  extern __shared__ float4 weights[];
+  V* const sh = (V*)(weights + a.K);  // two exchanges, twice
+  stage_weights<T>(weights, a);
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, per = kImageThreads / 32 / warps;
+  const V inv = X::all(-1.0f / (float)a.K);
+  V dw[R], db[R];
+#pragma unroll
+  for (int i = 0; i < R; i++) dw[i] = db[i] = X::all(0.0f);
+  const int64_t tiles = (a.M + 32 * VP - 1) / (32 * VP);
+  int turn = 0;
+  for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < tiles; t0 += (int64_t)gridDim.x * per) {
+    const int64_t m = ((t0 + warp / warps) * 32 + lane) * VP;
+    const bool on = m < a.M;
+    X x[R], dy[R];
+    V less = X::all(0.0f), under = less, rstd = less, q1 = less, q2 = less;
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < R; i++)
+        if (tw + i * warps < a.K) x[i].load(a.x, m, tw + i * warps, a.M), dy[i].load(a.dy, m, tw + i * warps, a.M);
+#pragma unroll
+      for (int j = 0; j < VP; j++)
+        if (m + j < a.M) {  // a pixel that is not there keeps an h and a dy of 0
+          ((float*)&less)[j] = -a.stats[m + j];
+          ((float*)&under)[j] = -a.stats[a.M + m + j];
+          ((float*)&rstd)[j] = a.stats[2 * a.M + m + j];
+        }
+#pragma unroll
+      for (int i = 0; i < R; i++) {
+        const int c = tw + i * warps;
+        if (c < a.K) {
+          const V h = mul(add(add(x[i].get(), less), under), rstd), d = dy[i].get(), g = mul(d, low(weights[c], V()));
+          q1 = add(q1, g);
+          q2 = fma(g, h, q2);
+          dw[i] = fma(d, h, dw[i]);
+          db[i] = add(db[i], d);
+        }
+      }
+    }
+    if (!a.y.p) continue;
+    V* const s = sh + turn * 2 * kImageThreads;
+    turn ^= 1;
+    q1 = mul(tile_total(q1, s, warps), inv);
+    q2 = mul(tile_total(q2, s + kImageThreads, warps), inv);
+    if (!on) continue;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const int c = tw + i * warps;
+      if (c < a.K) {
+        const V h = mul(add(add(x[i].get(), less), under), rstd), g = mul(dy[i].get(), low(weights[c], V()));
+        X::store(mul(fma(h, q2, add(g, q1)), rstd), a.y, m, c, a.M);
+      }
+    }
+  }
+  if (!a.part) return;
+  float* out = a.part + ((int64_t)blockIdx.x * per + warp / warps) * 2 * a.K;
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const int c = tw + i * warps;
+    float s = X::sum(dw[i]), t = X::sum(db[i]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if (lane == 0 && c < a.K) out[c] = s, out[a.K + c] = t;
+  }
+}
+
+// More channels than the warps hold: each step reads them again.
+template <typename T, int VP, int R>
+__global__ void __launch_bounds__(512) norm_image_long_forward(const __grid_constant__ NormArgs a, int warps) {
   extern __shared__ float sh[];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, first = warp - tw, per = blockDim.x / 32 / warps;
   const int size = blockDim.x * VP;  // floats of one exchange
@@ -359,15 +614,14 @@ __global__ void __launch_bounds__(512) norm_image_forward(const __grid_constant_
     };
     const auto channels = [&](auto f) {
       if (m >= a.M) return;
-      for (int k0 = 0; k0 < (LONG ? a.K : 1); k0 += R * warps) {
-        if (LONG) load(k0);
+      for (int k0 = 0; k0 < a.K; k0 += R * warps) {
+        load(k0);
 #pragma unroll
         for (int i = 0; i < R; i++)
           if (k0 + tw + i * warps < a.K) f(x[i], k0 + tw + i * warps);
       }
     };
     float mean[VP] = {}, d1[VP] = {}, d2[VP] = {}, rstd[VP];
-    if (!LONG && m < a.M) load(0);
     channels([&](const Chunk<T, VP>& v, int) {
 #pragma unroll
       for (int j = 0; j < VP; j++) mean[j] += to_f(v.v[j]);
@@ -411,14 +665,13 @@ __global__ void __launch_bounds__(512) norm_image_forward(const __grid_constant_
   }
 }
 
-template <typename T, int VP, int R, bool LONG>
-__global__ void __launch_bounds__(512) norm_image_backward(const __grid_constant__ NormArgs a, int warps) {
+template <typename T, int VP, int R>
+__global__ void __launch_bounds__(512) norm_image_long_backward(const __grid_constant__ NormArgs a, int warps) {
   extern __shared__ float sh[];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, first = warp - tw, per = blockDim.x / 32 / warps;
   const int size = blockDim.x * VP;
   const float inv = 1.0f / (float)a.K;
   const T* w = (const T*)a.w;
-  float dw[R] = {}, db[R] = {};  // not LONG
   const int64_t tiles = (a.M + 32 * VP - 1) / (32 * VP);
   int turn = 0;
   for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < tiles; t0 += (int64_t)gridDim.x * per) {
@@ -433,15 +686,14 @@ __global__ void __launch_bounds__(512) norm_image_backward(const __grid_constant
     };
     const auto channels = [&](auto f) {
       if (m >= a.M) return;
-      for (int k0 = 0; k0 < (LONG ? a.K : 1); k0 += R * warps) {
-        if (LONG) load(k0);
+      for (int k0 = 0; k0 < a.K; k0 += R * warps) {
+        load(k0);
 #pragma unroll
         for (int i = 0; i < R; i++)
           if (k0 + tw + i * warps < a.K) f(i, k0 + tw + i * warps);
       }
     };
     float mean[VP], shift[VP], rstd[VP], q1[VP] = {}, q2[VP] = {};
-    if (!LONG && m < a.M) load(0);
 #pragma unroll
     for (int j = 0; j < VP; j++) {  // h of a pixel that is not there: 0
       const bool in = m + j < a.M;
@@ -456,10 +708,6 @@ __global__ void __launch_bounds__(512) norm_image_backward(const __grid_constant
         const float h = (to_f(x[i].v[j]) - mean[j] - shift[j]) * rstd[j], d = to_f(dy[i].v[j]), g = d * wc;
         q1[j] += g;
         q2[j] = fmaf(g, h, q2[j]);
-        if (!LONG) {
-          dw[i] = fmaf(d, h, dw[i]);
-          db[i] += d;
-        }
       }
     });
     if (!a.y.p) continue;
@@ -483,19 +731,6 @@ __global__ void __launch_bounds__(512) norm_image_backward(const __grid_constant
       store_pixels<T, VP>(y, a.y, m, c, a.M);
     });
   }
-  if (LONG || !a.part) return;
-  float* out = a.part + ((int64_t)blockIdx.x * per + warp / warps) * 2 * a.K;
-#pragma unroll
-  for (int i = 0; i < R; i++) {
-    const int c = tw + i * warps;
-    float s = dw[i], t = db[i];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      s += __shfl_xor_sync(0xffffffffu, s, o);
-      t += __shfl_xor_sync(0xffffffffu, t, o);
-    }
-    if (lane == 0 && c < a.K) out[c] = s, out[a.K + c] = t;
-  }
 }
 
 // ---- host ----
@@ -511,7 +746,7 @@ struct Call {
   // `units` pieces of work, one a block at a time; `per` partial sums a block.
   template <auto kernel>
   void run(int threads, size_t smem, int64_t units, int lanes, int per) {
-    static std::atomic<int> known[33];  // blocks per SM by warps a block (one size of smem each)
+    static std::atomic<int> known[33];  // blocks per SM by warps a block (shared memory differs little)
     static std::atomic<uint64_t> large;  // devices on which the kernel may have more than 48 KB
     if (smem > 48 * 1024) {
       int dev = 0;
@@ -577,14 +812,20 @@ bool rows_block(Call& c, int64_t units) {
   else c.run<norm_rows_forward<T, VEC, NV, 1, true>>(threads, 0, c.a.M, threads, 1);
   return true;
 }
-template <typename T, int VP, int R, bool LONG, bool BACKWARD>
+template <typename T, int VP, int R, bool BACKWARD>
 void image_tiles(Call& c) {
-  const int need = (int)std::min<int64_t>(16, ceil_div(c.a.K, R));
-  const int warps = pow2_at_least(need), block = std::max(8, warps);
-  const int64_t work = ceil_div(ceil_div(c.a.M, 32 * VP), block / warps);
-  const size_t smem = (size_t)block * 32 * VP * 4 * (BACKWARD ? 4 : 3);
-  if constexpr (BACKWARD) c.run<norm_image_backward<T, VP, R, LONG>>(block * 32, smem, work, warps, block / warps);
-  else c.run<norm_image_forward<T, VP, R, LONG>>(block * 32, smem, work, warps, block / warps);
+  const int warps = pow2_at_least(ceil_div(c.a.K, R)), per = kImageThreads / 32 / warps;
+  const int64_t work = ceil_div(ceil_div(c.a.M, 32 * VP), per);
+  const size_t smem = (size_t)c.a.K * 16 + (size_t)kImageThreads * VP * 4 * (BACKWARD ? 4 : 3);
+  if constexpr (BACKWARD) c.run<norm_image_backward<T, VP, R>>(kImageThreads, smem, work, warps, per);
+  else c.run<norm_image_forward<T, VP, R>>(kImageThreads, smem, work, warps, per);
+}
+template <typename T, int VP, int R, bool BACKWARD>
+void image_long(Call& c) {
+  const int64_t work = ceil_div(c.a.M, 32 * VP);
+  const size_t smem = (size_t)512 * VP * 4 * (BACKWARD ? 4 : 3);
+  if constexpr (BACKWARD) c.run<norm_image_long_backward<T, VP, R>>(512, smem, work, 16, 1);
+  else c.run<norm_image_long_forward<T, VP, R>>(512, smem, work, 16, 1);
 }
 
 template <typename T>
@@ -599,22 +840,19 @@ void norm_call(Call& c, bool backward) {
   };
   if (image) {
     constexpr int VP = 4 / (int)sizeof(T);
+    const bool pairs = wide(VP, true);  // else any strides
     if (!backward) {
-      if (a.K <= 128 && wide(VEC, true)) image_tiles<T, VEC, 8, false, false>(c);
-      else if (a.K <= 512 && wide(VP, true)) image_tiles<T, VP, 32, false, false>(c);
-      else if (a.K <= 512) image_tiles<T, 1, 32, false, false>(c);
-      else if (wide(VP, true)) image_tiles<T, VP, 32, true, false>(c);
-      else image_tiles<T, 1, 32, true, false>(c);
-      return;
-    }
-    if (a.K <= 64 && wide(VEC, true)) image_tiles<T, VEC, 4, false, true>(c);
-    else if (a.K <= 256 && wide(VP, true)) image_tiles<T, VP, 16, false, true>(c);
-    else if (a.K <= 256) image_tiles<T, 1, 16, false, true>(c);
-    else {
-      if (a.y.p) {
-        if (wide(VP, true)) image_tiles<T, VP, 16, true, true>(c);
-        else image_tiles<T, 1, 16, true, true>(c);
+      if (a.K <= 512) {
+        if (a.K <= 16) pairs ? image_tiles<T, VP, 16, false>(c) : image_tiles<T, 1, 16, false>(c);
+        else if (a.K <= 32) pairs ? image_tiles<T, VP, 32, false>(c) : image_tiles<T, 1, 32, false>(c);
+        else pairs ? image_tiles<T, VP, 64, false>(c) : image_tiles<T, 1, 64, false>(c);
+      } else {
+        pairs ? image_long<T, VP, 32, false>(c) : image_long<T, 1, 32, false>(c);
       }
+    } else if (a.K <= 128) {
+      pairs ? image_tiles<T, VP, 16, true>(c) : image_tiles<T, 1, 16, true>(c);
+    } else {
+      if (a.y.p) pairs ? image_long<T, VP, 16, true>(c) : image_long<T, 1, 16, true>(c);
       c.columns<T>(true);
     }
     return;
