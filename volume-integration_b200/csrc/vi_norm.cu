@@ -13,6 +13,7 @@
 // The weights' gradients are summed in registers over a persistent block's rows, then over blocks in order.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "vi_heads.h"
 #include "vi_heads_math.cuh"
@@ -401,18 +402,16 @@ __device__ __forceinline__ float mul(float a, float b) { return a * b; }
 __device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float fma(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ float2 fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-// VP pixels of one channel as they lie in memory: a pair of 16-bit ones in a word.
+// VP pixels of one channel as they lie in memory: a pair of 16-bit ones in a word (M is even then).
 template <typename T, int VP>
 struct Pixels;
 template <typename T>
 struct Pixels<T, 1> {
   using V = float;
   T t;
-  __device__ __forceinline__ void load(const View& m, int64_t row, int64_t c, int64_t M) { t = ((const T*)m.p)[row * m.rs + c * m.cs]; }
+  __device__ __forceinline__ void load(const char* p) { t = *(const T*)p; }
   __device__ __forceinline__ V get() const { return to_f(t); }
-  static __device__ __forceinline__ void store(V v, const View& m, int64_t row, int64_t c, int64_t M) {
-    ((T*)m.p)[row * m.rs + c * m.cs] = from_f<T>(v);
-  }
+  static __device__ __forceinline__ void store(V v, char* p) { *(T*)p = from_f<T>(v); }
   static __device__ __forceinline__ V all(float f) { return f; }
   static __device__ __forceinline__ float sum(V v) { return v; }
 };
@@ -420,22 +419,24 @@ template <typename T>
 struct Pixels<T, 2> {
   using V = float2;
   uint32_t w;
-  __device__ __forceinline__ void load(const View& m, int64_t row, int64_t c, int64_t M) {
-    const T* p = (const T*)m.p + row + c * m.cs;
-    w = row + 1 < M ? *(const uint32_t*)p : *(const uint16_t*)p;
-  }
+  __device__ __forceinline__ void load(const char* p) { w = *(const uint32_t*)p; }
   __device__ __forceinline__ V get() const {
     const T* t = (const T*)&w;
     return make_float2(to_f(t[0]), to_f(t[1]));
   }
-  static __device__ __forceinline__ void store(V v, const View& m, int64_t row, int64_t c, int64_t M) {
-    T* p = (T*)m.p + row + c * m.cs;
-    if (row + 1 < M) *(uint32_t*)p = pack2(v, T());
-    else *p = from_f<T>(v.x);
-  }
+  static __device__ __forceinline__ void store(V v, char* p) { *(uint32_t*)p = pack2(v, T()); }
   static __device__ __forceinline__ V all(float f) { return pair(f); }
   static __device__ __forceinline__ float sum(V v) { return v.x + v.y; }
 };
+// f(i, p) for each of the lane's channels, p the bytes of its pixels there; WHOLE: it has R of them.
+template <typename T, int R, bool WHOLE, typename F>
+__device__ __forceinline__ void each_channel(const View& m, int64_t row, int tw, int warps, int K, F f) {
+  char* p = (char*)m.p + (row * m.rs + tw * m.cs) * (int64_t)sizeof(T);
+  const int64_t step = warps * m.cs * (int64_t)sizeof(T);
+#pragma unroll
+  for (int i = 0; i < R; i++, p += step)
+    if (WHOLE || tw + i * warps < K) f(i, p);
+}
 // Sum of a lane's value over the warps of its tile, in order, through sh (one value a thread of the block).
 template <typename V>
 __device__ __forceinline__ V tile_total(V v, V* sh, int warps) {
@@ -465,8 +466,8 @@ __device__ __forceinline__ float2 high(float4 q, float2) { return make_float2(q.
 // A lane holds every warps-th channel of its pixels, up to R, as they lie in memory.  With one warp a tile (up to 64 channels)
 // nothing is exchanged, and a warp has 8 KB on the way at a time.
 constexpr int kImageThreads = 256;
-template <typename T, int VP, int R>
-__global__ void __launch_bounds__(kImageThreads) norm_image_forward(const __grid_constant__ NormArgs a, int warps) {
+template <typename T, int VP, int R, bool WHOLE>
+__global__ void __launch_bounds__(kImageThreads, R > 32 ? 2 : 3) norm_image_forward(const __grid_constant__ NormArgs a, int warps) {
   using X = Pixels<T, VP>;
   using V = typename X::V;
   extern __shared__ float4 weights[];
@@ -481,19 +482,17 @@ __global__ void __launch_bounds__(kImageThreads) norm_image_forward(const __grid
     X x[R];
     V s = X::all(0.0f);
     if (on) {
+      each_channel<T, R, WHOLE>(a.x, m, tw, warps, a.K, [&](int i, const char* p) { x[i].load(p); });
 #pragma unroll
       for (int i = 0; i < R; i++)
-        if (tw + i * warps < a.K) x[i].load(a.x, m, tw + i * warps, a.M);
-#pragma unroll
-      for (int i = 0; i < R; i++)
-        if (tw + i * warps < a.K) s = add(s, x[i].get());
+        if (WHOLE || tw + i * warps < a.K) s = add(s, x[i].get());
     }
     const V mean = mul(tile_total(s, sh, warps), inv), less = mul(mean, X::all(-1.0f));
     V s1 = X::all(0.0f), s2 = s1;
     if (on) {
 #pragma unroll
       for (int i = 0; i < R; i++)
-        if (tw + i * warps < a.K) {
+        if (WHOLE || tw + i * warps < a.K) {
           const V d = add(x[i].get(), less);
           s1 = add(s1, d);
           s2 = fma(d, d, s2);
@@ -505,25 +504,21 @@ __global__ void __launch_bounds__(kImageThreads) norm_image_forward(const __grid
 #pragma unroll
     for (int j = 0; j < VP; j++) {
       ((float*)&rstd)[j] = 1.0f / sqrtf(fmaxf(((float*)&var)[j], 0.0f) + a.eps);
-      if (a.stats && tw == 0 && m + j < a.M) {
+      if (a.stats && tw == 0) {
         a.stats[m + j] = ((const float*)&mean)[j];
         a.stats[a.M + m + j] = ((const float*)&shift)[j];
         a.stats[2 * a.M + m + j] = ((const float*)&rstd)[j];
       }
     }
     const V under = mul(shift, X::all(-1.0f));
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-      const int c = tw + i * warps;
-      if (c < a.K) {
-        const float4 q = weights[c];
-        X::store(fma(mul(add(add(x[i].get(), less), under), rstd), low(q, V()), high(q, V())), a.y, m, c, a.M);
-      }
-    }
+    each_channel<T, R, WHOLE>(a.y, m, tw, warps, a.K, [&](int i, char* p) {
+      const float4 q = weights[tw + i * warps];
+      X::store(fma(mul(add(add(x[i].get(), less), under), rstd), low(q, V()), high(q, V())), p);
+    });
   }
 }
 
-template <typename T, int VP, int R>
+template <typename T, int VP, int R, bool WHOLE>
 __global__ void __launch_bounds__(kImageThreads, 2) norm_image_backward(const __grid_constant__ NormArgs a, int warps) {
   using X = Pixels<T, VP>;
   using V = typename X::V;
@@ -543,20 +538,18 @@ __global__ void __launch_bounds__(kImageThreads, 2) norm_image_backward(const __
     X x[R], dy[R];
     V less = X::all(0.0f), under = less, rstd = less, q1 = less, q2 = less;
     if (on) {
+      each_channel<T, R, WHOLE>(a.x, m, tw, warps, a.K, [&](int i, const char* p) { x[i].load(p); });
+      each_channel<T, R, WHOLE>(a.dy, m, tw, warps, a.K, [&](int i, const char* p) { dy[i].load(p); });
 #pragma unroll
-      for (int i = 0; i < R; i++)
-        if (tw + i * warps < a.K) x[i].load(a.x, m, tw + i * warps, a.M), dy[i].load(a.dy, m, tw + i * warps, a.M);
-#pragma unroll
-      for (int j = 0; j < VP; j++)
-        if (m + j < a.M) {  // a pixel that is not there keeps an h and a dy of 0
-          ((float*)&less)[j] = -a.stats[m + j];
-          ((float*)&under)[j] = -a.stats[a.M + m + j];
-          ((float*)&rstd)[j] = a.stats[2 * a.M + m + j];
-        }
+      for (int j = 0; j < VP; j++) {
+        ((float*)&less)[j] = -a.stats[m + j];
+        ((float*)&under)[j] = -a.stats[a.M + m + j];
+        ((float*)&rstd)[j] = a.stats[2 * a.M + m + j];
+      }
 #pragma unroll
       for (int i = 0; i < R; i++) {
         const int c = tw + i * warps;
-        if (c < a.K) {
+        if (WHOLE || c < a.K) {
           const V h = mul(add(add(x[i].get(), less), under), rstd), d = dy[i].get(), g = mul(d, low(weights[c], V()));
           q1 = add(q1, g);
           q2 = fma(g, h, q2);
@@ -571,14 +564,10 @@ __global__ void __launch_bounds__(kImageThreads, 2) norm_image_backward(const __
     q1 = mul(tile_total(q1, s, warps), inv);
     q2 = mul(tile_total(q2, s + kImageThreads, warps), inv);
     if (!on) continue;
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-      const int c = tw + i * warps;
-      if (c < a.K) {
-        const V h = mul(add(add(x[i].get(), less), under), rstd), g = mul(dy[i].get(), low(weights[c], V()));
-        X::store(mul(fma(h, q2, add(g, q1)), rstd), a.y, m, c, a.M);
-      }
-    }
+    each_channel<T, R, WHOLE>(a.y, m, tw, warps, a.K, [&](int i, char* p) {
+      const V h = mul(add(add(x[i].get(), less), under), rstd), g = mul(dy[i].get(), low(weights[tw + i * warps], V()));
+      X::store(mul(fma(h, q2, add(g, q1)), rstd), p);
+    });
   }
   if (!a.part) return;
   float* out = a.part + ((int64_t)blockIdx.x * per + warp / warps) * 2 * a.K;
@@ -817,8 +806,13 @@ void image_tiles(Call& c) {
   const int warps = pow2_at_least(ceil_div(c.a.K, R)), per = kImageThreads / 32 / warps;
   const int64_t work = ceil_div(ceil_div(c.a.M, 32 * VP), per);
   const size_t smem = (size_t)c.a.K * 16 + (size_t)kImageThreads * VP * 4 * (BACKWARD ? 4 : 3);
-  if constexpr (BACKWARD) c.run<norm_image_backward<T, VP, R>>(kImageThreads, smem, work, warps, per);
-  else c.run<norm_image_forward<T, VP, R>>(kImageThreads, smem, work, warps, per);
+  const auto run = [&](auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    if constexpr (BACKWARD) c.run<norm_image_backward<T, VP, R, WHOLE>>(kImageThreads, smem, work, warps, per);
+    else c.run<norm_image_forward<T, VP, R, WHOLE>>(kImageThreads, smem, work, warps, per);
+  };
+  if (c.a.K == R * warps) run(std::true_type());
+  else run(std::false_type());
 }
 template <typename T, int VP, int R, bool BACKWARD>
 void image_long(Call& c) {
@@ -840,7 +834,7 @@ void norm_call(Call& c, bool backward) {
   };
   if (image) {
     constexpr int VP = 4 / (int)sizeof(T);
-    const bool pairs = wide(VP, true);  // else any strides
+    const bool pairs = a.M % VP == 0 && wide(VP, true);  // else any strides
     if (!backward) {
       if (a.K <= 512) {
         if (a.K <= 16) pairs ? image_tiles<T, VP, 16, false>(c) : image_tiles<T, 1, 16, false>(c);
