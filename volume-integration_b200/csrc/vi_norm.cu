@@ -176,9 +176,10 @@ __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
   }
 }
 
-// The next rows are asked for before the present ones are worked on.
-template <typename T, int VEC, int NV, int R, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
+// h and g are made twice of what memory gave, so that the registers leave room for three blocks of 256 threads on an SM: with
+// them held, or the next rows on their way, two or one (65536 x 512: 53 us, 97; here 47).
+template <typename T, int VEC, int NV, int R, bool BLOCK, int MOST>
+__global__ void __launch_bounds__(BLOCK ? MOST : kRowThreads, BLOCK ? 512 / MOST : VEC * NV > 8 ? 2 : 3)
     norm_rows_backward(const __grid_constant__ NormArgs a, int lanes) {
   __shared__ float sh[2][16][2 * R];
   __shared__ float cols[BLOCK ? 1 : kRowThreads / 32][BLOCK ? 1 : 32 * VEC * NV];
@@ -187,67 +188,68 @@ __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
   const int lane = BLOCK ? threadIdx.x : threadIdx.x % lanes, group = BLOCK ? 0 : threadIdx.x / lanes;
   const int groups = BLOCK ? 1 : kRowThreads / lanes;
   const float inv = 1.0f / (float)a.K;
-  float2 w[P];
-  {
-    Chunk<T, VEC> c[NV];
-    load_weights(c, a.w, 1.0f, a.K, lanes, lane);
-    pairs_of(c, w);
-  }
+  Chunk<T, VEC> w[NV];
+  load_weights(w, a.w, 1.0f, a.K, lanes, lane);
   float2 dw[P], db[P];
 #pragma unroll
   for (int i = 0; i < P; i++) dw[i] = db[i] = pair(0.0f);
-  Chunk<T, VEC> x[R][NV], dy[R][NV];
-  float mean[R], shift[R], rstd[R];
-  const auto load = [&](int64_t m0) {
+  for (int64_t m0 = (int64_t)blockIdx.x * groups * R; m0 < a.M; m0 += (int64_t)gridDim.x * groups * R) {
+    // of a row that is not there, and behind a row's end, all is 0 and adds nothing
+    Chunk<T, VEC> x[R][NV], dy[R][NV];
+    float mean[R], shift[R], rstd[R], q[2 * R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-      const int64_t m = min(m0 + r * groups + group, a.M - 1);
-      load_row(x[r], a.x, m, a.K, lanes, lane);
-      load_row(dy[r], a.dy, m, a.K, lanes, lane);
-      mean[r] = a.stats[m], shift[r] = a.stats[a.M + m], rstd[r] = a.stats[2 * a.M + m];
+      const int64_t m = m0 + r * groups + group;
+      const int K = m < a.M ? a.K : 0;
+      load_row(x[r], a.x, m, K, lanes, lane);
+      load_row(dy[r], a.dy, m, K, lanes, lane);
+      mean[r] = shift[r] = rstd[r] = 0.0f;
+      if (K) mean[r] = -a.stats[m], shift[r] = -a.stats[a.M + m], rstd[r] = a.stats[2 * a.M + m];
     }
-  };
-  int64_t m0 = (int64_t)blockIdx.x * groups * R;
-  const int64_t step = (int64_t)gridDim.x * groups * R;
-  if (m0 < a.M) load(m0);
-  for (; m0 < a.M; m0 += step) {
-    float2 h[R][P], g[R][P];
-    float q[2 * R], scale[R];
+    float2 wp[P];
+    pairs_of(w, wp);
 #pragma unroll
     for (int r = 0; r < R; r++) {
-      pairs_of(x[r], h[r]);
-      pairs_of(dy[r], g[r]);
-      scale[r] = rstd[r];
-      const bool on = m0 + r * groups + group < a.M;
-      float2 s1 = pair(0.0f), s2 = pair(0.0f);
+      float2 h[P], g[P], s1 = pair(0.0f), s2 = pair(0.0f);
+      pairs_of(x[r], h);
+      pairs_of(dy[r], g);
 #pragma unroll
       for (int i = 0; i < P; i++) {
-        // beyond K and beyond M nothing is added: h of a zero is not one
-        h[r][i] = __fmul2_rn(__fadd2_rn(__fadd2_rn(h[r][i], pair(-mean[r])), pair(-shift[r])), pair(rstd[r]));
-        if (!on || !in_row<VEC>(2 * i, lanes, lane, a.K)) h[r][i].x = 0.0f, g[r][i].x = 0.0f;
-        if (!on || 2 * i + 1 >= E || !in_row<VEC>(2 * i + 1, lanes, lane, a.K)) h[r][i].y = 0.0f, g[r][i].y = 0.0f;
-        dw[i] = __ffma2_rn(g[r][i], h[r][i], dw[i]);
-        db[i] = __fadd2_rn(db[i], g[r][i]);
-        g[r][i] = __fmul2_rn(g[r][i], w[i]);
-        s1 = __fadd2_rn(s1, g[r][i]);
-        s2 = __ffma2_rn(g[r][i], h[r][i], s2);
+        h[i] = __fmul2_rn(__fadd2_rn(__fadd2_rn(h[i], pair(mean[r])), pair(shift[r])), pair(rstd[r]));
+        dw[i] = __ffma2_rn(g[i], h[i], dw[i]);
+        db[i] = __fadd2_rn(db[i], g[i]);
+        g[i] = __fmul2_rn(g[i], wp[i]);
+        s1 = __fadd2_rn(s1, g[i]);
+        s2 = __ffma2_rn(g[i], h[i], s2);
       }
       q[2 * r] = s1.x + s1.y;
       q[2 * r + 1] = s2.x + s2.y;
     }
-    if (m0 + step < a.M) load(m0 + step);
     if (!a.y.p) continue;
     row_sum<2 * R, BLOCK>(q, lanes, sh, turn);
 #pragma unroll
     for (int r = 0; r < R; r++) {
       const int64_t m = m0 + r * groups + group;
       if (m < a.M) {
-        const float mg = q[2 * r] * inv, mgh = q[2 * r + 1] * inv;
+        const float mg = -q[2 * r] * inv, mgh = -q[2 * r + 1] * inv;
+        float2 h[P], g[P];
 #pragma unroll
-        for (int i = 0; i < P; i++)
-          g[r][i] = __fmul2_rn(__ffma2_rn(h[r][i], pair(-mgh), __fadd2_rn(g[r][i], pair(-mg))), pair(scale[r]));
+        for (int v = 0; v < NV; v++) {  // not to be kept from above
+          uint32_t* t = (uint32_t*)x[r][v].v;
+          if constexpr (sizeof(x[r][v]) >= 4) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(x[r][v]) / 4; i++) asm volatile("" : "+r"(t[i]));
+          }
+        }
+        pairs_of(x[r], h);
+        pairs_of(dy[r], g);
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+          h[i] = __fmul2_rn(__fadd2_rn(__fadd2_rn(h[i], pair(mean[r])), pair(shift[r])), pair(rstd[r]));
+          g[i] = __fmul2_rn(__ffma2_rn(h[i], pair(mgh), __ffma2_rn(g[i], wp[i], pair(mg))), pair(rstd[r]));
+        }
         Chunk<T, VEC> y[NV];
-        chunks_of(g[r], y);
+        chunks_of(g, y);
         store_row(y, a.y, m, a.K, lanes, lane);
       }
     }
@@ -789,7 +791,7 @@ bool rows_lanes(Call& c, int64_t units) {
   if (units > 32 * NV) return false;
   const int lanes = NV > 1 ? 32 : pow2_at_least(units);
   const int64_t work = ceil_div(c.a.M, (int64_t)kRowThreads / lanes * R);
-  if constexpr (BACKWARD) c.run<norm_rows_backward<T, VEC, NV, R, false>>(kRowThreads, 0, work, lanes, 1);
+  if constexpr (BACKWARD) c.run<norm_rows_backward<T, VEC, NV, R, false, 1>>(kRowThreads, 0, work, lanes, 1);
   else c.run<norm_rows_forward<T, VEC, NV, R, false>>(kRowThreads, 0, work, lanes, 1);
   return true;
 }
@@ -797,8 +799,10 @@ template <typename T, int VEC, int NV, bool BACKWARD>
 bool rows_block(Call& c, int64_t units) {
   if (units > (int64_t)kBlockMost * NV) return false;
   const int threads = (int)ceil_div(ceil_div(units, NV), 32) * 32;
-  if constexpr (BACKWARD) c.run<norm_rows_backward<T, VEC, NV, 1, true>>(threads, 0, c.a.M, threads, 1);
-  else c.run<norm_rows_forward<T, VEC, NV, 1, true>>(threads, 0, c.a.M, threads, 1);
+  if constexpr (BACKWARD) {
+    if (threads <= 256) c.run<norm_rows_backward<T, VEC, NV, 1, true, 256>>(threads, 0, c.a.M, threads, 1);
+    else c.run<norm_rows_backward<T, VEC, NV, 1, true, kBlockMost>>(threads, 0, c.a.M, threads, 1);
+  } else c.run<norm_rows_forward<T, VEC, NV, 1, true>>(threads, 0, c.a.M, threads, 1);
   return true;
 }
 template <typename T, int VP, int R, bool BACKWARD>
