@@ -780,12 +780,12 @@ Tensor linear_act_int8(const Tensor& x, const c10::optional<Tensor>& x_scale, co
   TORCH_CHECK(x.scalar_type() == (x_scale.has_value() ? torch::kInt8 : dtype), "x must be ", x_scale.has_value() ? torch::kInt8 : dtype);
   const Tensor ws = scale_of(weight_scale, weight.size(0), "weight's scale");
   const Tensor xs = x_scale.has_value() ? scale_of(*x_scale, x.size(0), "x's scale") : Tensor();
-  const Tensor like = torch::empty({0}, x.options().dtype(dtype));
-  const int dt = head_dtype(like, "the result");
-  const Tensor b = head_bias(bias, like, weight);
-  const OptMatrix r(residual, like, "residual");
-  Tensor y = x.stride(0) == 1 && x.stride(1) != 1 ? torch::empty({weight.size(0), x.size(0)}, like.options()).t()
-                                                  : torch::empty({x.size(0), weight.size(0)}, like.options());
+  const auto options = x.options().dtype(dtype);
+  Tensor y = x.stride(0) == 1 && x.stride(1) != 1 ? torch::empty({weight.size(0), x.size(0)}, options).t()
+                                                  : torch::empty({x.size(0), weight.size(0)}, options);
+  const int dt = head_dtype(y, "the result");
+  const Tensor b = head_bias(bias, y, weight);
+  const OptMatrix r(residual, y, "residual");
   const vi_matrix mx = head_matrix(x), mw = head_matrix(weight), my = head_matrix(y);
   const float *pxs = xs.defined() ? xs.data_ptr<float>() : nullptr, *pws = ws.data_ptr<float>();
   const uint64_t n = vi_linear_act_int8_scratch_bytes(dt, (int)activation, &mx, pxs, &mw, pws, head_ptr(b), r.get(), &my);

@@ -7,6 +7,7 @@
 //
 // Memory bounds it: one pass over x, held in registers between the maximum and the rounding.
 #include <algorithm>
+#include <type_traits>
 
 #include "vi_heads.h"
 #include "vi_heads_math.cuh"
@@ -211,6 +212,110 @@ __global__ void __launch_bounds__(kThreads) pack8_kernel(View src, int64_t rows,
     dst[i / k * ld + i % k] = p[i / k * src.rs + i % k * src.cs];
 }
 
+// ---- a few rows: quantised and multiplied by one launch ----
+// At up to 8 rows the launches cost more than the product does.  Every block quantises all rows into its shared memory, and each
+// of its warps makes 4 channels: lanes along the sum, 16 products an instruction quartet, one reduction a result.
+constexpr int kFewRows = 8, kFewTerms = 4096, kFewColumns = 4;
+struct FewArgs {
+  int M, N, K, act;
+  View x, res, y;
+  const int8_t* w;
+  int64_t ld;
+  const float* w_scale;
+  const void* bias;
+};
+template <typename T>
+__device__ __forceinline__ float act_of(int act, float z) {
+  constexpr bool kExact = sizeof(T) == 4;
+  float2 y, d;
+  switch (act) {
+    case VI_ACT_RELU:
+      activate<VI_ACT_RELU, kExact, false>(pair(z), y, d);
+      return relu_signed_zero<T>(y).x;
+    case VI_ACT_SILU: activate<VI_ACT_SILU, kExact, false>(pair(z), y, d); return y.x;
+    case VI_ACT_GELU: activate<VI_ACT_GELU, kExact, false>(pair(z), y, d); return y.x;
+    case VI_ACT_SIGMOID: activate<VI_ACT_SIGMOID, kExact, false>(pair(z), y, d); return y.x;
+    default: return z;
+  }
+}
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(kThreads) few_rows_kernel(const __grid_constant__ FewArgs a) {
+  extern __shared__ __align__(16) int8_t terms_of[];  // [ROWS][terms]
+  __shared__ uint32_t tops[kThreads / 32];
+  __shared__ float scales[ROWS];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, terms = (a.K + 15) / 16 * 16;
+  // the weights are asked for before the rows are known
+  const int n0 = (blockIdx.x * (kThreads / 32) + warp) * kFewColumns;
+  int4 first[kFewColumns];
+  const bool ahead = lane * 16 + 16 <= a.K;
+#pragma unroll
+  for (int c = 0; c < kFewColumns; c++)
+    if (ahead && n0 + c < a.N) first[c] = *(const int4*)(a.w + (n0 + c) * a.ld + lane * 16);
+  {
+    constexpr int kTeam = kThreads / ROWS;
+    const int r = threadIdx.x / kTeam, t = threadIdx.x % kTeam;
+    const T* x = (const T*)a.x.p + r * a.x.rs;
+    uint32_t top = 0;
+    if (r < a.M)
+      for (int k = t; k < a.K; k += kTeam) top = max(top, __float_as_uint(to_f(x[k * a.x.cs])) & 0x7fffffffu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kTeam / 32; w++) top = max(top, tops[r * (kTeam / 32) + w]);
+    const Scale s(top);
+    if (t == 0) scales[r] = s.s;
+    for (int k = t; k < terms; k += kTeam) {
+      int q[1] = {0};
+      if (r < a.M && k < a.K) {
+        const float f[1] = {to_f(x[k * a.x.cs])};
+        quantize(f, s, q);
+      }
+      terms_of[r * terms + k] = (int8_t)q[0];
+    }
+  }
+  __syncthreads();
+  if (n0 >= a.N) return;
+  int acc[kFewColumns][ROWS] = {};
+  for (int k = lane * 16; k < a.K; k += 512) {
+    int4 w[kFewColumns];
+#pragma unroll
+    for (int c = 0; c < kFewColumns; c++) {
+      w[c] = make_int4(0, 0, 0, 0);
+      if (n0 + c < a.N) {
+        const int8_t* p = a.w + (n0 + c) * a.ld + k;
+        if (k == lane * 16 && ahead) w[c] = first[c];
+        else if (k + 16 <= a.K) w[c] = *(const int4*)p;
+        else
+          for (int i = 0; i < a.K - k; i++) ((int8_t*)&w[c])[i] = p[i];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+      const int4 x = *(const int4*)(terms_of + r * terms + k);
+#pragma unroll
+      for (int c = 0; c < kFewColumns; c++)
+        acc[c][r] = __dp4a(w[c].x, x.x, __dp4a(w[c].y, x.y, __dp4a(w[c].z, x.z, __dp4a(w[c].w, x.w, acc[c][r]))));
+    }
+  }
+  int mine = 0;  // lane c * ROWS + r keeps that result
+#pragma unroll
+  for (int c = 0; c < kFewColumns; c++)
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+      const int sum = __reduce_add_sync(0xffffffffu, acc[c][r]);
+      if (lane == c * ROWS + r) mine = sum;
+    }
+  const int r = lane % ROWS, n = n0 + lane / ROWS;
+  if (lane >= kFewColumns * ROWS || r >= a.M || n >= a.N) return;
+  float z = (float)mine * (scales[r] * a.w_scale[n]);
+  if (a.bias) z += to_f(((const T*)a.bias)[n]);
+  z = act_of<T>(a.act, z);
+  if (a.res.p) z += to_f(((const T*)a.res.p)[r * a.res.rs + n * a.res.cs]);
+  ((T*)a.y.p)[r * a.y.rs + n * a.y.cs] = from_f<T>(z);
+}
+static_assert(kFewColumns * kFewRows <= 32, "a result a lane");
+
 // ---- host ----
 struct Call {
   const QuantArgs& a;
@@ -270,6 +375,25 @@ cudaError_t launch_quantize(int dtype, const QuantArgs& a, int sms, cudaStream_t
   if (dtype == VI_F32) c.run<float>();
   else if (dtype == VI_F16) c.run<__half>();
   else c.run<__nv_bfloat16>();
+  return cudaPeekAtLastError();
+}
+bool int8_few(int64_t M, int64_t K, const Operand& w) {
+  return M <= kFewRows && K <= kFewTerms && (uintptr_t)w.p % 16 == 0 && w.ld % 16 == 0;
+}
+cudaError_t launch_int8_few(int dtype, int64_t M, const View& x, const Operand& w, const Epilogue& e, cudaStream_t s) {
+  FewArgs a{(int)M, (int)w.rows, (int)w.k, e.act, x, e.res, e.out, (const int8_t*)w.p, w.ld, e.col_scale, e.bias};
+  const unsigned blocks = (unsigned)ceil_div(w.rows, kThreads / 32 * kFewColumns);
+  const auto run = [&](auto rows) {
+    constexpr int ROWS = decltype(rows)::value;
+    const size_t smem = (size_t)ROWS * ceil_div(w.k, 16) * 16;
+    if (dtype == VI_F32) few_rows_kernel<float, ROWS><<<blocks, kThreads, smem, s>>>(a);
+    else if (dtype == VI_F16) few_rows_kernel<__half, ROWS><<<blocks, kThreads, smem, s>>>(a);
+    else few_rows_kernel<__nv_bfloat16, ROWS><<<blocks, kThreads, smem, s>>>(a);
+  };
+  if (M == 1) run(std::integral_constant<int, 1>());
+  else if (M == 2) run(std::integral_constant<int, 2>());
+  else if (M <= 4) run(std::integral_constant<int, 4>());
+  else run(std::integral_constant<int, 8>());
   return cudaPeekAtLastError();
 }
 cudaError_t launch_pack8(const View& src, int64_t rows, int64_t k, int8_t* dst, int64_t ld, cudaStream_t s) {
