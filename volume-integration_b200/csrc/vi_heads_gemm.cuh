@@ -63,13 +63,14 @@ struct Shape {
   static constexpr int kBlocks = BN == 256 || PL == 3 ? 1 : 2;
   // Epilogue warps.  The softmax on a 256-wide tile has 16: with 8 its latency, not its
   // instructions, bound it (K = 256: gradient 289 us with 8, 230 with 16; statistics 207, 159).
-  static constexpr int kWarps = BN == 256 && (EPI == kEpiLse || EPI == kEpiGrad) ? 16 : 8;
+  // So do the 8-bit products, whose sums are made twice as fast (32768 x 1024 -> 4096: 185 us with 8).
+  static constexpr int kWarps = BN == 256 && (EPI == kEpiLse || EPI == kEpiGrad || EPI == kEpiInt8) ? 16 : 8;
   static constexpr int kParts = kWarps / 4;  // warps that share a tile's columns, 32 at a time
   static constexpr int kThreads = (kWarps + 2) * 32;
   static constexpr int kTileA = kBM * kBK * 2, kTileB = BN / (kPair ? 2 : 1) * kBK * 2;  // bytes of a plane
   static constexpr int kStage = PL * (kTileA + kTileB);
   static constexpr int kStages = PL == 3   ? 2
-                                 : BN == 256 ? (kPair ? 6 : 4)
+                                 : BN == 256 ? (EPI == kEpiInt8 ? (sizeof(T) == 4 ? 4 : 5) : kPair ? 6 : 4)
                                  : BN == 128 ? (kBlocks == 2 ? 2 : 5)
                                              : (kBlocks == 2 ? 3 : 7);
   static constexpr int kStageWarp = EPI == kEpiLse ? 0 : 32 * 32 * (int)sizeof(T);  // an epilogue warp's staging
