@@ -25,9 +25,9 @@ namespace heads {
 namespace {
 
 // Sum of S values over the lanes of a row: G lanes of a warp, or a block.  Every lane gets it, always added in the same
-// order.
+// order.  Of a block's up to 16 warps those that are not there left zeros (clear_sums).
 template <int S, bool BLOCK>
-__device__ __forceinline__ void row_sum(float (&s)[S], int lanes, float (*sh)[16][S], int& turn) {
+__device__ __forceinline__ void row_sum(float (&s)[S], int lanes, float (*sh)[S][16], int& turn) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     if (!BLOCK && o >= lanes) continue;
@@ -35,20 +35,28 @@ __device__ __forceinline__ void row_sum(float (&s)[S], int lanes, float (*sh)[16
     for (int i = 0; i < S; i++) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
   }
   if constexpr (BLOCK) {  // two buffers in turn: a barrier each sum
-    const int warps = blockDim.x / 32;
     if (threadIdx.x % 32 == 0) {
 #pragma unroll
-      for (int i = 0; i < S; i++) sh[turn][threadIdx.x / 32][i] = s[i];
+      for (int i = 0; i < S; i++) sh[turn][i][threadIdx.x / 32] = s[i];
     }
     __syncthreads();
+    const bool few = blockDim.x <= 256;
 #pragma unroll
-    for (int i = 0; i < S; i++) s[i] = 0.0f;
-    for (int w = 0; w < warps; w++) {
-#pragma unroll
-      for (int i = 0; i < S; i++) s[i] += sh[turn][w][i];
+    for (int i = 0; i < S; i++) {
+      const float4 p = *(const float4*)&sh[turn][i][0], q = *(const float4*)&sh[turn][i][4];
+      s[i] = ((p.x + p.y) + (p.z + p.w)) + ((q.x + q.y) + (q.z + q.w));
+      if (!few) {
+        const float4 u = *(const float4*)&sh[turn][i][8], v = *(const float4*)&sh[turn][i][12];
+        s[i] += ((u.x + u.y) + (u.z + u.w)) + ((v.x + v.y) + (v.z + v.w));
+      }
     }
     turn ^= 1;
   }
+}
+template <int N>
+__device__ __forceinline__ void clear_sums(float* sh) {
+  for (int i = threadIdx.x; i < N; i += blockDim.x) sh[i] = 0.0f;
+  __syncthreads();
 }
 
 template <typename T, int VEC, int NV>
@@ -116,8 +124,10 @@ __device__ __forceinline__ float total(const float2 (&p)[N]) {
 template <typename T, int VEC, int NV, int R, bool BLOCK>
 __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
     norm_rows_forward(const __grid_constant__ NormArgs a, int lanes) {
-  __shared__ float sh1[2][16][R], sh2[2][16][2 * R];
+  __shared__ __align__(16) float sh1[2][R][16], sh2[2][2 * R][16];
   constexpr int E = VEC * NV, P = (E + 1) / 2;
+  if constexpr (BLOCK) clear_sums<32 * R>(&sh1[0][0][0]), clear_sums<64 * R>(&sh2[0][0][0]);
+  const bool whole = a.K == lanes * E;  // of the lanes' elements none lies behind the row
   int turn1 = 0, turn2 = 0;
   const int lane = BLOCK ? threadIdx.x : threadIdx.x % lanes, group = BLOCK ? 0 : threadIdx.x / lanes;
   const int groups = BLOCK ? 1 : kRowThreads / lanes;
@@ -150,8 +160,11 @@ __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
 #pragma unroll
       for (int i = 0; i < P; i++) {
         x[r][i] = __fadd2_rn(x[r][i], pair(-mean[r]));
-        if (!in_row<VEC>(2 * i, lanes, lane, a.K)) x[r][i].x = 0.0f;
-        if (2 * i + 1 >= E || !in_row<VEC>(2 * i + 1, lanes, lane, a.K)) x[r][i].y = 0.0f;
+        if (E % 2 && 2 * i + 1 >= E) x[r][i].y = 0.0f;
+        if (!whole) {
+          if (!in_row<VEC>(2 * i, lanes, lane, a.K)) x[r][i].x = 0.0f;
+          if (2 * i + 1 < E && !in_row<VEC>(2 * i + 1, lanes, lane, a.K)) x[r][i].y = 0.0f;
+        }
         s1 = __fadd2_rn(s1, x[r][i]);
         s2 = __ffma2_rn(x[r][i], x[r][i], s2);
       }
@@ -181,9 +194,10 @@ __global__ void __launch_bounds__(BLOCK ? kBlockMost : kRowThreads)
 template <typename T, int VEC, int NV, int R, bool BLOCK, int MOST>
 __global__ void __launch_bounds__(BLOCK ? MOST : kRowThreads, BLOCK ? 512 / MOST : VEC * NV > 8 ? 2 : 3)
     norm_rows_backward(const __grid_constant__ NormArgs a, int lanes) {
-  __shared__ float sh[2][16][2 * R];
+  __shared__ __align__(16) float sh[2][2 * R][16];
   __shared__ float cols[BLOCK ? 1 : kRowThreads / 32][BLOCK ? 1 : 32 * VEC * NV];
   constexpr int E = VEC * NV, P = (E + 1) / 2;
+  if constexpr (BLOCK) clear_sums<64 * R>(&sh[0][0][0]);
   int turn = 0;
   const int lane = BLOCK ? threadIdx.x : threadIdx.x % lanes, group = BLOCK ? 0 : threadIdx.x / lanes;
   const int groups = BLOCK ? 1 : kRowThreads / lanes;
@@ -286,7 +300,9 @@ __global__ void __launch_bounds__(BLOCK ? MOST : kRowThreads, BLOCK ? 512 / MOST
 // Rows of any length: a block a row, which it reads again for each step.
 template <typename T, bool BACKWARD>
 __global__ void __launch_bounds__(512) norm_long_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float sh1[2][16][1], sh2[2][16][2];
+  __shared__ __align__(16) float sh1[2][1][16], sh2[2][2][16];
+  clear_sums<32>(&sh1[0][0][0]);
+  clear_sums<64>(&sh2[0][0][0]);
   int turn1 = 0, turn2 = 0;
   const float inv = 1.0f / (float)a.K;
   const T *w = (const T*)a.w, *b = (const T*)a.b;
