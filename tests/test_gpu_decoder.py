@@ -92,6 +92,10 @@ NORM_CASES = [
     (264, 600, "image", "image", "both"),
     (77, 1100, "image", "same", "both"),
     (40000, 24, "image", "image", "both"),
+    (36, 7216, "image", "image", "none"),       # few pixels of many channels
+    (8194, 600, "image", "image", "both"),
+    (9001, 300, "image", "image", "weight"),
+    (4000, 256, "image", "image", "both"),
 ]
 
 

@@ -483,15 +483,14 @@ __device__ __forceinline__ float2 high(float4 q, float2) { return make_float2(q.
 
 // A lane holds every warps-th channel of its pixels, up to R, as they lie in memory.  With one warp a tile (up to 64 channels)
 // nothing is exchanged, and a warp has 8 KB on the way at a time.
-constexpr int kImageThreads = 256;
-template <typename T, int VP, int R, bool WHOLE>
-__global__ void __launch_bounds__(kImageThreads, R > 32 ? 2 : 3) norm_image_forward(const __grid_constant__ NormArgs a, int warps) {
+template <typename T, int VP, int R, bool WHOLE, int THREADS>
+__global__ void __launch_bounds__(THREADS, R > 32 ? 2 : 3) norm_image_forward(const __grid_constant__ NormArgs a, int warps) {
   using X = Pixels<T, VP>;
   using V = typename X::V;
   extern __shared__ float4 weights[];
   V* const sh = (V*)(weights + a.K);  // three exchanges
   stage_weights<T>(weights, a);
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, per = kImageThreads / 32 / warps;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, per = THREADS / 32 / warps;
   const V inv = X::all(1.0f / (float)a.K);
   const int64_t tiles = (a.M + 32 * VP - 1) / (32 * VP);
   for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < tiles; t0 += (int64_t)gridDim.x * per) {
@@ -516,7 +515,7 @@ __global__ void __launch_bounds__(kImageThreads, R > 32 ? 2 : 3) norm_image_forw
           s2 = fma(d, d, s2);
         }
     }
-    const V shift = mul(tile_total(s1, sh + kImageThreads, warps), inv), sq = mul(tile_total(s2, sh + 2 * kImageThreads, warps), inv);
+    const V shift = mul(tile_total(s1, sh + THREADS, warps), inv), sq = mul(tile_total(s2, sh + 2 * THREADS, warps), inv);
     if (!on) continue;
     V var = fma(mul(shift, X::all(-1.0f)), shift, sq), rstd;
 #pragma unroll
@@ -536,14 +535,14 @@ __global__ void __launch_bounds__(kImageThreads, R > 32 ? 2 : 3) norm_image_forw
   }
 }
 
-template <typename T, int VP, int R, bool WHOLE>
-__global__ void __launch_bounds__(kImageThreads, 2) norm_image_backward(const __grid_constant__ NormArgs a, int warps) {
+template <typename T, int VP, int R, bool WHOLE, int THREADS>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) norm_image_backward(const __grid_constant__ NormArgs a, int warps) {
   using X = Pixels<T, VP>;
   using V = typename X::V;
   extern __shared__ float4 weights[];
   V* const sh = (V*)(weights + a.K);  // two exchanges, twice
   stage_weights<T>(weights, a);
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, per = kImageThreads / 32 / warps;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, tw = warp % warps, per = THREADS / 32 / warps;
   const V inv = X::all(-1.0f / (float)a.K);
   V dw[R], db[R];
 #pragma unroll
@@ -577,10 +576,10 @@ __global__ void __launch_bounds__(kImageThreads, 2) norm_image_backward(const __
       }
     }
     if (!a.y.p) continue;
-    V* const s = sh + turn * 2 * kImageThreads;
+    V* const s = sh + turn * 2 * THREADS;
     turn ^= 1;
     q1 = mul(tile_total(q1, s, warps), inv);
-    q2 = mul(tile_total(q2, s + kImageThreads, warps), inv);
+    q2 = mul(tile_total(q2, s + THREADS, warps), inv);
     if (!on) continue;
     each_channel<T, R, WHOLE>(a.y, m, tw, warps, a.K, [&](int i, char* p) {
       const V h = mul(add(add(x[i].get(), less), under), rstd), g = mul(dy[i].get(), low(weights[tw + i * warps], V()));
@@ -821,15 +820,15 @@ bool rows_block(Call& c, int64_t units) {
   } else c.run<norm_rows_forward<T, VEC, NV, 1, true>>(threads, 0, c.a.M, threads, 1);
   return true;
 }
-template <typename T, int VP, int R, bool BACKWARD>
+template <typename T, int VP, int R, bool BACKWARD, int THREADS = 256>
 void image_tiles(Call& c) {
-  const int warps = pow2_at_least(ceil_div(c.a.K, R)), per = kImageThreads / 32 / warps;
+  const int warps = pow2_at_least(ceil_div(c.a.K, R)), per = THREADS / 32 / warps;
   const int64_t work = ceil_div(ceil_div(c.a.M, 32 * VP), per);
-  const size_t smem = (size_t)c.a.K * 16 + (size_t)kImageThreads * VP * 4 * (BACKWARD ? 4 : 3);
+  const size_t smem = (size_t)c.a.K * 16 + (size_t)THREADS * VP * 4 * (BACKWARD ? 4 : 3);
   const auto run = [&](auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
-    if constexpr (BACKWARD) c.run<norm_image_backward<T, VP, R, WHOLE>>(kImageThreads, smem, work, warps, per);
-    else c.run<norm_image_forward<T, VP, R, WHOLE>>(kImageThreads, smem, work, warps, per);
+    if constexpr (BACKWARD) c.run<norm_image_backward<T, VP, R, WHOLE, THREADS>>(THREADS, smem, work, warps, per);
+    else c.run<norm_image_forward<T, VP, R, WHOLE, THREADS>>(THREADS, smem, work, warps, per);
   };
   if (c.a.K == R * warps) run(std::true_type());
   else run(std::false_type());
@@ -846,7 +845,9 @@ template <typename T>
 void norm_call(Call& c, bool backward) {
   const NormArgs& a = c.a;
   constexpr int VEC = 16 / (int)sizeof(T);
-  const bool image = a.x.rs == 1 && a.x.cs != 1 && a.M > 1;
+  // An image of many channels and so few pixels that its tiles leave most SMs idle goes by rows, a block each, element by
+  // element (36 pixels x 7216 channels: 890 us by tiles).
+  const bool image = a.x.rs == 1 && a.x.cs != 1 && a.M > 1 && (a.K <= (backward ? 256 : 512) || a.M > 8192);
   const auto wide = [&](int n, bool along_rows) {
     for (const View* v : {&a.x, &a.dy, &a.y})
       if (v->p && !moves<T>(*v, n, along_rows)) return false;
@@ -865,6 +866,8 @@ void norm_call(Call& c, bool backward) {
       }
     } else if (a.K <= 128) {
       pairs ? image_tiles<T, VP, 16, true>(c) : image_tiles<T, 1, 16, true>(c);
+    } else if (a.K <= 256) {
+      pairs ? image_tiles<T, VP, 16, true, 512>(c) : image_tiles<T, 1, 16, true, 512>(c);
     } else {
       if (a.y.p) pairs ? image_long<T, VP, 16, true>(c) : image_long<T, 1, 16, true>(c);
       c.columns<T>(true);
