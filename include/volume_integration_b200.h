@@ -429,7 +429,8 @@ int vi_quantize_rows(int dtype, const vi_matrix* x, const vi_matrix* q, float* s
  * vi_linear_act_forward with 8-bit integer products: y = act(x_scale_m weight_scale_n sum_k x_mk weight_nk + bias_n) + residual.
  * weight int8 [N,K] (any strides) and weight_scale float32 [N] as vi_quantize_rows gives them.  x [M,K]: int8 with
  * x_scale float32 [M]; or, x_scale NULL, of `dtype`: its rows are quantised in the call.  bias, residual and y are of `dtype`.
- * Sums are exact; K is at most 2^17.
+ * Sums are exact; K is less than 2^17.  Up to 8 float rows are one launch, and so are rows and images of at most 64 16-bit
+ * features and 64 channels.
  */
 uint64_t vi_linear_act_int8_scratch_bytes(int dtype, int activation, const vi_matrix* x, const float* x_scale,
                                           const vi_matrix* weight, const float* weight_scale, const void* bias,

@@ -303,8 +303,8 @@ def test_linear_act_int8(M, K, N, act, order, bias, residual, dt):
 
 
 def test_linear_act_int8_longest_sums():
-    # all products 127^2 of one sign: the sum of 2^17 is just within 32 bits
-    heads, K = _heads(), 1 << 17
+    # all products of one sign: the sum of 2^17 - 1 is just within 32 bits, with a caller's -128 too
+    heads, K = _heads(), (1 << 17) - 1
     for M in (1, 3, 140):
         x = torch.ones(M, K, device="cuda")
         x[1::2] = -1
@@ -312,6 +312,8 @@ def test_linear_act_int8_longest_sums():
         y = heads.linear_act_int8(x, w)
         want = dl.linear_act_int8(*dl.quantize(x), *w, None, None, "none", F32)
         hl.assert_within("y", y, want)
+    low, one = torch.full((150, K), -128, device="cuda", dtype=torch.int8), torch.ones(150, device="cuda")
+    assert bool((heads.linear_act_int8((low, one), (low[:4], one[:4]), dtype=F32) == float(128 * 128 * K)).all())
     with pytest.raises(RuntimeError, match="2\\^17"):
         heads.linear_act_int8(torch.ones(2, K + 1, device="cuda"), heads.quantize_rows(torch.ones(2, K + 1, device="cuda")))
 
@@ -350,6 +352,23 @@ def test_linear_act_int8_shapes_gradients_and_empty_batches():
     with torch.no_grad():
         assert heads.linear_act_int8(x, w).shape == (2, 3, 5)
     assert heads.quantize_rows(x)[1].requires_grad is False
+
+
+def test_quantize_rows_into_a_part_of_a_matrix():
+    # a C caller's q may be columns of a wider matrix: what lies beside them stays
+    import ctypes
+    import heads_abi as ha
+    lib, p = ha.load(), ctypes.c_void_p
+    lib.vi_quantize_rows.argtypes = [ctypes.c_int, ctypes.POINTER(ha.Matrix), ctypes.POINTER(ha.Matrix), p, p]
+    for dt, order, K in ((BF16, "image", 5), (F32, "image", 130), (F16, "rows", 24), (BF16, "odd", 7), (F16, "image", 601)):
+        x = hl.matrix(300, K, dt, _gen(K), order)
+        wide = torch.full((300, (K + 31) // 16 * 16), 77, device="cuda", dtype=torch.int8)
+        scale = torch.empty(300, device="cuda")
+        q = wide[:, :K]
+        assert lib.vi_quantize_rows(ha.DTYPE[dt], ha.matrix(x), ha.matrix(q), p(scale.data_ptr()),
+                                    p(torch.cuda.current_stream().cuda_stream)) == 0, lib.vi_last_error()
+        wq, ws = dl.quantize(x)
+        assert torch.equal(q, wq) and torch.equal(scale, ws) and bool((wide[:, K:] == 77).all())
 
 
 # ---- labels ----
@@ -426,6 +445,35 @@ def test_sample_labels_rows_are_drawn_by_their_share():
     got = _heads().sample_labels(z.expand(100000, 5), u)
     share = torch.bincount(got, minlength=5).double() / 100000
     assert float((share - torch.softmax(z.double(), 0)).abs().max()) <= 2e-5
+
+
+def test_sample_labels_of_more_long_rows_than_are_drawn_at_a_time():
+    g = _gen(8)
+    z = hl.matrix(16390, 8200, BF16, g, scale=3.0)
+    u = torch.rand(16390, generator=g, device="cuda")
+    got = _heads().sample_labels(z, u, top_k=9)
+    at = torch.tensor([0, 1, 16382, 16383, 16384, 16385, 16389], device="cuda")
+    assert torch.equal(got[at].cpu(), dl.sample(z[at], u[at], top_k=9))
+
+
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("M,V", [(3, 9000), (200, 20011), (2, 100003)])
+def test_sample_labels_of_long_rows_of_every_kind(M, V, dt):
+    # flat and peaked, sorted both ways, constant, with all mass in front or behind: guesses from a sample go wrong here
+    g = _gen(V)
+    kinds = [hl.matrix(M, V, dt, g, scale=0.01), hl.matrix(M, V, dt, g, scale=30.0),
+             hl.matrix(M, V, dt, g, scale=3.0).sort(1).values, hl.matrix(M, V, dt, g, scale=3.0).sort(1, descending=True).values,
+             torch.full((M, V), -2.5, device="cuda", dtype=dt)]
+    spike = hl.matrix(M, V, dt, g, scale=1.0)
+    spike[:, V - 1] = 40.0
+    kinds.append(spike)
+    rows = slice(0, 3)
+    for z in kinds:
+        u = torch.rand(M, generator=g, device="cuda")
+        for settings in (dict(), dict(top_p=0.9), dict(top_p=0.999, temperature=1.9), dict(top_k=V // 2), dict(top_k=3, top_p=0.4),
+                         dict(min_p=0.001), dict(min_p=0.9, temperature=0.4), dict(temperature=0.0)):
+            got = _heads().sample_labels(z, u, **settings)
+            assert torch.equal(got[rows].cpu(), dl.sample(z[rows], u[rows], **settings)), settings
 
 
 def test_sample_labels_shapes():

@@ -1085,6 +1085,7 @@ int norm_forward(Run& r, int dtype, const vi_matrix* x, const void* w, const voi
   if (int rc = check_norm(dtype, x, w, b, eps)) return rc;
   if (!given(y) || y->rows != x->rows) return bad("layer_norm: y is required, [M, K]");
   if (int rc = check_shape(dtype, y, x->rows, x->cols, true, "layer_norm: y must be a dense [M, K]")) return rc;
+  if ((uintptr_t)stats % 4) return bad("layer_norm: data must lie on whole elements");
   if (x->rows == 0 || r.dry) return VI_OK;
   NormArgs a{x->rows, (int)x->cols, view(x), {}, view(y), w, b, eps, stats, nullptr};
   const cudaError_t rc = launch_norm(dtype, a, false, r.sms, r.s, &r.launches);
@@ -1163,7 +1164,7 @@ int int8_forward(Run& r, int dtype, int act, const vi_matrix* x, const float* x_
   if (!x || !w) return bad("linear_act_int8: x and weight are required");
   if (x->rows < 0 || x->cols < 1 || w->rows < 1) return bad("linear_act_int8: x needs at least one column and weight one row");
   if (w->cols != x->cols) return bad("linear_act_int8: weight and x differ in their number of columns");
-  if (x->cols > kInt8Terms) return bad("linear_act_int8: more than 2^17 columns do not fit a 32-bit sum");
+  if (x->cols > kInt8Terms) return bad("linear_act_int8: sums of 2^17 columns and more do not fit 32 bits");
   if (x->rows > kMaxSize || w->rows > kMaxSize) return bad("linear_act_int8: sizes are limited to 2^30");
   if ((!x->data && x->rows) || !w->data || !w_scale) return bad("linear_act_int8: x, weight and its scale need data");
   if (x->row_stride < 0 || x->col_stride < 0 || w->row_stride < 0 || w->col_stride < 0)
@@ -1243,6 +1244,9 @@ int sample_labels(Run& r, int dtype, const vi_matrix* z, const float* u, const v
   if (!s->min_ps && !(s->min_p >= 0.0 && s->min_p <= 1.0)) return bad("sample_labels: min_p must lie in [0, 1]");
   if (z->rows == 0) return VI_OK;
   if (!z->data || (!r.dry && (!u || !label))) return bad("sample_labels: logits, u and label need data");
+  if ((uintptr_t)u % 4 || (uintptr_t)s->temperatures % 4 || (uintptr_t)s->top_ps % 4 || (uintptr_t)s->min_ps % 4 ||
+      (uintptr_t)s->top_ks % 8 || (uintptr_t)label % 8)
+    return bad("sample_labels: data must lie on whole elements");
   // long rows keep candidates: as many rows at a time as fill the device many times over
   constexpr int64_t kRows = 16384;
   const uint64_t bytes = sample_scratch(std::min(z->rows, kRows), z->cols, r.sms);

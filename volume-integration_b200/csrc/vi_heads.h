@@ -163,7 +163,7 @@ bool small_product(int64_t M, int64_t N, int64_t K, int64_t longest);
 cudaError_t launch_small(int dtype, const SmallJob& a, const SmallJob* b, cudaStream_t s);
 
 // kEpiInt8's product (vi_heads_int8.cu): operands of 8-bit integers, k contiguous, ld a multiple of 16.
-constexpr int64_t kInt8Terms = 1 << 17;  // 127^2 of each fit the 32-bit sum
+constexpr int64_t kInt8Terms = (1 << 17) - 1;  // of at most 128^2 each: their sum fits 32 bits
 int launch_int8_gemm(int dtype, const Operand& a, const Operand& b, const Plan& p, const Epilogue& e, int sms, cudaStream_t s);
 // The same with float rows of few features, quantised in the kernel (e.row_scale is not read).
 bool int8_fused(int dtype, int64_t M, int64_t N, int64_t K, const View& x);

@@ -1,7 +1,7 @@
 // The dense layer in 8-bit integers: vi_heads_gemm.cuh's product with kEpiInt8.
 //
 // Mathematics.  x_mk is about s_m q_mk and w_nk about t_n p_nk with whole q and p in [-127, 127]; the sum over k of
-// q p is exact in 32 bits (up to 2^17 terms), and y = act(s_m t_n sum + b_n) + res is rounded once to the type.
+// q p is exact in 32 bits (under 2^17 terms), and y = act(s_m t_n sum + b_n) + res is rounded once to the type.
 #include "vi_heads_gemm.cuh"
 #include "vi_quant.cuh"
 

@@ -201,8 +201,13 @@ __global__ void __launch_bounds__(512) quantize_image_kernel(const __grid_consta
     int span = 1;
     while (span < words && span < 32) span *= 2;
     for (int p = threadIdx.x / span; p < count; p += blockDim.x / span)
-      for (int w = threadIdx.x % span; w < words; w += span)
-        *(uint32_t*)(a.q + (first + p) * a.ld + 4 * w) = sh[(p % VP * 32 + p / VP) * pitch + w];
+      for (int w = threadIdx.x % span; w < words; w += span) {
+        const uint32_t v = sh[(p % VP * 32 + p / VP) * pitch + w];
+        int8_t* to = a.q + (first + p) * a.ld + 4 * w;
+        if (4 * w + 4 <= a.K) *(uint32_t*)to = v;
+        else
+          for (int i = 0; i < a.K - 4 * w; i++) to[i] = (int8_t)(v >> (8 * i));  // what lies behind the row stays
+      }
   }
 }
 
@@ -350,7 +355,7 @@ struct Call {
     constexpr int VEC = 16 / (int)sizeof(T), VP = 4 / (int)sizeof(T);
     const int64_t K = a.K;
     const bool words = a.ld % 8 == 0 && (uintptr_t)a.q % 8 == 0;  // as this library lays rows out
-    if (a.x.rs == 1 && a.x.cs != 1 && a.M > 1 && a.ld % 4 == 0 && a.ld >= (K + 3) / 4 * 4 && (uintptr_t)a.q % 4 == 0) {
+    if (a.x.rs == 1 && a.x.cs != 1 && a.M > 1 && a.ld % 4 == 0 && (uintptr_t)a.q % 4 == 0) {
       if (K <= 128 && moves<T>(a.x, VEC, true)) {
         if (image<T, VEC, 8, false>()) return;
       } else if (K <= 512) {

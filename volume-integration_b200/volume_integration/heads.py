@@ -185,7 +185,7 @@ def linear_act_int8(x, weight, bias=None, residual=None, activation="none", dtyp
     weight: the pair ``quantize_rows`` makes of [N, K], one scale an output channel.  x: [..., K] of float32, float16
     or bfloat16, whose rows are quantised in the call, one scale a row; or such a pair, for several layers
     that read the same features: then ``dtype`` says the result's type.  bias: [N] and residual: [..., N] of the result's type
-    (x's).  K is at most 2^17: sums are exact, then scaled in float32, and results are rounded once.  Rows or channels whose scale is
+    (x's).  K is less than 2^17: sums are exact, then scaled in float32, and results are rounded once.  Rows or channels whose scale is
     NaN come out as NaN.  For display: there is no backward, and inputs that require gradients are refused
     where they are recorded.
     """
