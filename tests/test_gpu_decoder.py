@@ -636,6 +636,27 @@ def test_results_of_images_beyond_2_31_elements():
     assert torch.equal(got[at].cpu(), dl.sample(x[at], u[at], min_p=0.02))
 
 
+def test_waits_that_run_out_are_reported(monkeypatch):
+    # the first copy is never issued: a limit on every wait, then the status word; no fault
+    heads, g = _heads(), _gen(41)
+    w = heads.quantize_rows(hl.matrix(200, 64, F32, g))
+    w64 = (w[0][:64], w[1][:64])
+    x, z = hl.matrix(33000, 64, BF16, g, "image"), hl.matrix(1024, 20, F16, g, "image")
+    u = torch.rand(1024, generator=g, device="cuda")
+    calls = (lambda: heads.linear_act_int8(x, w), lambda: heads.linear_act_int8(x, w64, activation="gelu"),
+             lambda: heads.linear_act_int8(x.contiguous(), w64), lambda: heads.sample_labels(z, u))
+    before = [call() for call in calls]
+    assert heads.device_status() == 0
+    monkeypatch.setenv("VI_HEADS_TEST_TIMEOUT", "1")
+    for call in calls:
+        call()
+        assert heads.device_status(reset=True) == 8
+    monkeypatch.delenv("VI_HEADS_TEST_TIMEOUT")
+    for call, want in zip(calls, before):
+        assert torch.equal(call(), want)
+    assert heads.device_status() == 0
+
+
 def test_heads_status_stays_clear():
     assert _heads().device_status() == 0
 
