@@ -2,6 +2,7 @@
 //
 // Mathematics.  x_mk is about s_m q_mk and w_nk about t_n p_nk with whole q and p in [-127, 127]; the sum over k of
 // q p is exact in 32 bits (under 2^17 terms), and y = act(s_m t_n sum + b_n) + res is rounded once to the type.
+// 32768 x 1024 -> 4096 with relu: 153 us, 1.8 * 10^15 operations a second; the float16 product 237.
 #include "vi_heads_gemm.cuh"
 #include "vi_quant.cuh"
 
@@ -12,7 +13,7 @@ namespace {
 // ---- few features: quantised on the way into the product ----
 // Up to 64 features and 64 channels of 16-bit types are bound by memory and by the epilogue, and a pass that quantises would
 // write and read the features once more (2M x 64 -> 64 with gelu and a residual: 284 us + 235 apart).  Here one warp
-// copies 256 rows of x at a time into shared memory, eight find their scales and write the tensor core's operand, two products
+// copies 256 rows of x at a time into shared memory (316 us in all: the latency of 26 warps at 72 registers), eight find their scales and write the tensor core's operand, two products
 // of 128 rows follow, and 8 warps run the epilogue.
 constexpr int kFusedK = 64, kFusedN = 64;
 template <typename T>

@@ -15,6 +15,10 @@
 // of rows that the registers hold (up to 8192 labels), or of a longer row's candidates.  Those are the labels above a
 // guess, made from a sample of the row: one pass over the row keeps them, and shows (by their number, or their share
 // of the mass) that no other label can be kept.
+//
+// 640000 x 150 (float16 image, min-p) takes 71 us (31 at the copy rate; instructions bound it); 1024 x 30011 (float32, top-k, top-p,
+// min-p) 74 (19; the chains of bisections and the passes' 1.4 waves); 2048 x 65536 (bfloat16, top-p) 339 (41; instructions of two
+// passes, 56 thousand a row, then the draws).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
