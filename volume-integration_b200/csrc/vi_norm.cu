@@ -12,7 +12,7 @@
 // neighbouring pixels and whose warps share the channels.  Rows that no block can hold are read again for each step.
 // The weights' gradients are summed in registers over a persistent block's rows, then over blocks in order.
 // Sums of pairs and products of pairs are one instruction each.  2073600 x 64 in bfloat16: images 105 us forward (81 at the copy
-// rate) and 250 backward (122), rows 120 and 189; 32768 x 4096 in float16: 146 (82) and 207 (123), where the latency of
+// rate) and 250 backward (122), rows 120 and 189; 32768 x 4096 in float16: 128 (82) and 207 (123), where the latency of
 // a block's sums is the bound.
 #include <algorithm>
 #include <atomic>
@@ -882,6 +882,7 @@ void norm_call(Call& c, bool backward) {
   if (wide(VEC, false)) {
     if (!backward) {
       if (rows_lanes<T, VEC, 1, 4, false>(c, n) || rows_lanes<T, VEC, 2, 2, false>(c, n) || rows_lanes<T, VEC, 4, 1, false>(c, n) ||
+          (n > 256 && rows_block<T, VEC, 4, false>(c, n)) ||  // fewer warps to add up (32768 x 4096: 146 us with 2, 128)
           rows_block<T, VEC, 2, false>(c, n) || rows_block<T, VEC, 4, false>(c, n))
         return;
     } else {  // sums of 16 columns a lane at most, in registers
