@@ -443,8 +443,8 @@ int vi_linear_act_int8(int dtype, int activation, const vi_matrix* x, const floa
  * Labels drawn from rows of logits.  With w_v = exp((z_v - max z) / temperature) and the candidates in the order of falling
  * z (ties: lowest index first): top_k (0: off) keeps the first top_k; top_p (1 or more: off) those of them in front
  * of which lies less than top_p of their mass (the first always); min_p (0: off) those with w >= min_p.  label_m is the first
- * index at which the sum of the kept w, in index order, exceeds u_m times their sum (u_m in [0, 1), float32; from 1 on the last
- * one kept).  temperature 0: the first of the largest.  A row whose logits are all -inf, or hold a NaN, has label -1; a +inf takes all
+ * index at which the sum of the kept w, in index order, exceeds u_m times their sum (u_m in [0, 1), float32; below 0 it is 0, from
+ * 1 on the answer is the last one kept).  temperature 0: the first of the largest.  A row whose logits are all -inf, or hold a NaN, has label -1; a +inf takes all
  * mass (several share it).  Each setting is one value, or an array of one per row where its array is not NULL (there a
  * temperature of 0 or less is 0, one that is NaN gives -1, a top_k under 1 is off, a top_p of 0 or less keeps the first).
  * Weights and sums are 64 bits wide.

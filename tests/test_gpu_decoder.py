@@ -174,6 +174,21 @@ def test_layer_norm_single_gradients(order, K):
         hl.assert_within(("dx", "dweight", "dbias")[which], got, want[1 + which])
 
 
+@pytest.mark.parametrize("order,K", [("rows", 40), ("image", 40), ("rows", 1000)])
+def test_layer_norm_with_a_bias_alone(order, K):
+    heads = _heads()
+    x, w, b, dy = _norm_inputs(50, K, F32, order, order, "both", 19)
+    one = torch.ones_like(w)
+    want = dl.layer_norm(x, one, b, 1e-5, dy)
+    x.requires_grad_(True), b.requires_grad_(True)
+    y = heads.layer_norm(x, None, b)
+    dx, db = torch.autograd.grad(y, (x, b), dy)
+    for name, got, ref in (("y", y, want[0]), ("dx", dx, want[1]), ("dbias", db, want[3])):
+        hl.assert_within(name, got, ref)
+    (db2,) = torch.autograd.grad(heads.layer_norm(x.detach(), None, b), (b,), dy)
+    assert torch.equal(db, db2)
+
+
 def test_layer_norm_gradients_against_differences():
     # the loss along a random direction, central differences of the kernel's own float32 results.  The step h makes
     # an error of h^2 / 6 times the third derivative along it (about 1 here: under 1e-3 of a slope of size sqrt(MK)), and the
@@ -434,6 +449,10 @@ def test_sample_labels_ends_of_u_and_ties(V):
     for settings in (dict(), dict(top_k=2), dict(top_k=V // 2 + 1), dict(top_p=0.6), dict(top_k=V // 2 + 1, top_p=0.55),
                      dict(min_p=0.3)):
         _labels(z, u, **settings)
+    for V_u, u_same in ((-3.0, 0.0), (NAN, 0.0)):  # under 0, or no number: 0
+        low = _heads().sample_labels(z, torch.full_like(u, V_u), top_k=2)
+        assert torch.equal(low, _heads().sample_labels(z, torch.full_like(u, u_same), top_k=2))
+        assert torch.equal(_heads().sample_labels(z, torch.full_like(u, V_u)), _heads().sample_labels(z, torch.full_like(u, u_same)))
     z[:] = 0.25  # all equal: the front of the order is the front of the row
     got = _labels(z, u, top_k=2)
     assert int(got.max()) <= 1
