@@ -17,7 +17,7 @@
 // of the mass) that no other label can be kept.
 //
 // 640000 x 150 (float16 image, min-p) takes 71 us (31 at the copy rate; instructions bound it); 1024 x 30011 (float32, top-k, top-p,
-// min-p) 74 (19; the chains of bisections and the passes' 1.4 waves); 2048 x 65536 (bfloat16, top-p) 339 (41; instructions of two
+// min-p) 74 (19; the chains of bisections and the passes' 1.7 waves); 2048 x 65536 (bfloat16, top-p) 326 (41; instructions of two
 // passes, 56 thousand a row, then the draws).
 #include <algorithm>
 #include <atomic>
@@ -1156,7 +1156,7 @@ __device__ __noinline__ int whole_row(Team<W>& team, LongShared<W>& sh, const Ro
 }
 
 template <int W, typename T, int MODE>
-__global__ void __launch_bounds__(32 * W, W == 8 ? 5 : 2) sample_long_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(32 * W, W == 8 ? 4 : 2) sample_long_kernel(const __grid_constant__ SampleArgs a) {
   using O = Order<T>;
   __shared__ LongShared<W> sh;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, V = a.V;
@@ -1592,7 +1592,7 @@ cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
     b.list_bytes = list_bytes(W);
     const auto both = [&](auto mode) {
       constexpr int MODE = decltype(mode)::value;
-      const cudaError_t rc = run(sample_long_kernel<W, T, MODE>, a.M, 32 * W, W == 8 ? 5 : 2);
+      const cudaError_t rc = run(sample_long_kernel<W, T, MODE>, a.M, 32 * W, W == 8 ? 4 : 2);
       return rc == cudaSuccess ? run(sample_held_kernel<W, T, MODE>, a.M, 32 * W, W == 8 ? 16 : 2) : rc;
     };
     return a.z.cs == 1 ? both(std::integral_constant<int, kVectors>()) : both(std::integral_constant<int, kStrided>());
