@@ -1,0 +1,85 @@
+"""GPU tests of what layer_norm, linear_act_int8 and sample_labels do at their edges: what a kernel keeps between its
+passes, settings at the ends of their ranges, logits far from zero, waits that run out in a part of a warp."""
+import ctypes
+
+import pytest
+import torch
+
+import decoder_lib as dl
+import heads_abi as ha
+import heads_lib as hl
+from test_decoder_cpu import Sampling
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+TYPES = dict(argvalues=[F32, F16, BF16], ids=["f32", "f16", "bf16"])
+INF = float("inf")
+
+
+def _heads():
+    from volume_integration import heads
+    return heads
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+# ---- candidates of long rows ----
+NOTE = 96       # bytes that sample_labels notes a row in its scratch: a double, two floats, the state, 16 counts, padding
+KEPT = 512      # candidates a warp keeps
+
+
+def _candidates(z, u, **settings):
+    """(labels, [M, W] counts, [M, W, KEPT] places) of a call with a scratch of the test's own."""
+    lib, p = ha.load(), ctypes.c_void_p
+    lib.vi_sample_labels_scratch_bytes.argtypes = [ctypes.c_int, ctypes.POINTER(ha.Matrix), ctypes.POINTER(Sampling)]
+    lib.vi_sample_labels_scratch_bytes.restype = ctypes.c_uint64
+    lib.vi_sample_labels.argtypes = [ctypes.c_int, ctypes.POINTER(ha.Matrix), p, ctypes.POINTER(Sampling), p, p,
+                                     ctypes.c_uint64, p]
+    M = z.shape[0]
+    warps = 16 if M <= torch.cuda.get_device_properties(0).multi_processor_count else 8
+    s = Sampling(**{**dict(temperature=1.0, top_p=1.0, min_p=0.0, top_k=0), **settings})
+    n = lib.vi_sample_labels_scratch_bytes(ha.DTYPE[z.dtype], ha.matrix(z), ctypes.byref(s))
+    lists = warps * KEPT * 4
+    assert n >= M * (NOTE + lists)
+    scratch = torch.zeros(n, device="cuda", dtype=torch.uint8)
+    label = torch.empty(M, device="cuda", dtype=torch.int64)
+    assert lib.vi_sample_labels(ha.DTYPE[z.dtype], ha.matrix(z), p(u.data_ptr()), ctypes.byref(s), p(label.data_ptr()),
+                                p(scratch.data_ptr()), n, p(torch.cuda.current_stream().cuda_stream)) == 0, lib.vi_last_error()
+    notes = scratch[:M * NOTE].view(torch.int32).reshape(M, NOTE // 4)
+    assert int(notes[:, 4].min()) >= 0 and int(notes[:, 4].max()) <= 2  # the state: the layout is the one read here
+    return label, notes[:, 5:5 + warps], scratch[M * NOTE:M * (NOTE + lists)].view(torch.int32).reshape(M, warps, KEPT)
+
+
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("M,V,order", [(200, 9000, "image"), (200, 9001, "rows"), (3, 50257, "rows"), (3, 50257, "image")])
+def test_candidates_of_long_rows_are_labels_of_the_row(M, V, order, dt):
+    # the last warp's part of these rows holds fewer labels than it keeps candidates; a floor under a peak, clipped and flat
+    # logits put the sample's tail into one value, so that no guess leaves anything out
+    g = _gen(V)
+    u = torch.rand(M, generator=g, device="cuda")
+    peak = torch.zeros(M, V, device="cuda")
+    peak[:, 5] = 9.0
+    clipped = torch.randn(M, V, generator=g, device="cuda").clamp(-0.5, 0.5) * 40
+    masked = torch.randn(M, V, generator=g, device="cuda")
+    masked[:, 100:] = -INF
+    kinds = [peak, clipped, torch.full((M, V), 0.25, device="cuda"), masked]
+    for kind in kinds:
+        z = kind.t().contiguous().t() if order == "image" else kind
+        z = z.to(dt) if order == "image" else z.to(dt).contiguous()
+        assert (z.stride(0) == 1) == (order == "image")
+        first = torch.zeros(M, device="cuda", dtype=torch.int64)
+        if order == "rows":  # places are counted from the 16 bytes' boundary in front of a row
+            first = (z.data_ptr() + torch.arange(M, device="cuda") * z.stride(0) * z.element_size()) % 16 // z.element_size()
+        for settings in (dict(top_p=0.9), dict(top_p=0.999, temperature=1.9), dict(top_k=V - 1), dict(top_k=50),
+                         dict(min_p=1e-30), dict(min_p=0.5), dict(temperature=0.0), dict(min_p=1e-30, temperature=1e4)):
+            label, counts, places = _candidates(z, u, **settings)
+            kept = torch.arange(KEPT, device="cuda") < counts[:, :, None]
+            low, high = first[:, None, None], first[:, None, None] + V
+            outside = kept & ((places < low) | (places >= high))
+            assert not bool(outside.any()), (settings, int(outside.sum()))
+            assert int(counts.sum(1).max()) <= V, settings
+            assert torch.equal(label[:3].cpu(), dl.sample(z[:3], u[:3], **settings)), settings

@@ -21,6 +21,7 @@
 // passes, 56 thousand a row, then the draws).
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <cstdlib>
 #include <type_traits>
@@ -1290,6 +1291,9 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : 2) sample_long_kernel(con
       else pass(std::false_type(), std::true_type(), std::true_type(), INFINITY);
       team.ahead(sum, before, all);
     }
+    // The type's lowest finite value, and the least guess: a place behind the row's ends holds -inf, as does a label that cannot
+    // be kept, and neither is a candidate (a list of places that hold no label would be read past the row).
+    constexpr float kLowest = sizeof(T) == 4 ? -FLT_MAX : std::is_same<T, __half>::value ? -65504.0f : -0x1.fep127f;
     float tail = 0.75f;  // top-p: of the share that is not kept, what may lie under the guess
     int tries = 2;
     while (workable && list) {
@@ -1340,15 +1344,16 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : 2) sample_long_kernel(con
       } else if (!greedy) {
         guess = ref + (float)(log2_min_p(a, s) / s.scale) * (1.0f + 1e-5f) - 1e-6f * fabsf(ref);
       }
+      guess = fmaxf(guess, kLowest);
       n = 0;
       if (top_p) pass(std::true_type(), std::false_type(), std::false_type(), guess);
       else pass(std::true_type(), std::true_type(), std::false_type(), guess);
-      if (!top_p || --tries == 0) break;
+      if (!top_p || --tries == 0 || guess == kLowest) break;
       // more of the tail, if what is held is not enough
       __syncwarp();
       double m = 0.0;
       for (int i = lane; i < min(n, kListWarp); i += 32) m += exp2_fast((r.at(candidates[i]) - ref) * scale);
-      if (team.sum(m) > s.p * all * (1.0 + 1e-5) || guess == -INFINITY) break;
+      if (team.sum(m) > s.p * all * (1.0 + 1e-5)) break;
       tail = 0.3f;
     }
     const uint32_t top = team.most(best != best || s.t != s.t ? kAll : O::of(best));
