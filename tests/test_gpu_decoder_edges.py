@@ -83,3 +83,35 @@ def test_candidates_of_long_rows_are_labels_of_the_row(M, V, order, dt):
             assert not bool(outside.any()), (settings, int(outside.sum()))
             assert int(counts.sum(1).max()) <= V, settings
             assert torch.equal(label[:3].cpu(), dl.sample(z[:3], u[:3], **settings)), settings
+
+
+# ---- logits far from zero ----
+def _u_at_borders(z, t, p, g):
+    """For each row a u just behind the start of a kept label's share, by the definition with top-p alone."""
+    z = z.double().cpu()
+    us = []
+    for row in z:
+        w = torch.exp((row - row.max()) / t)
+        order = torch.sort(row, descending=True, stable=True).indices
+        before = w[order].cumsum(0) - w[order]
+        n = max(1, int((before < p * w.sum()).sum()))
+        kept = torch.sort(order[:n]).values
+        run = w[kept].cumsum(0)
+        at = int(torch.randint(n // 2, n, (1,), generator=g))
+        us.append(torch.tensor(float((run[at] - w[kept[at]]) / run[-1]) + 2e-7).float())
+    return torch.stack(us).cuda()
+
+
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("shift,t", [(30.0, 0.1), (100.0, 0.5), (1000.0, 1.0), (1000.0, 0.1), (-1000.0, 0.1), (8000.0, 0.5)])
+def test_top_p_of_long_rows_far_from_zero(shift, t, dt):
+    # in float32 thousands of labels are kept, each about 1e-4 of the mass: a mass that is off by more than the kernel allows
+    # for keeps another number of them, and every border moves
+    g, cpu = _gen(int(shift) % 97), torch.Generator().manual_seed(int(shift) % 89)
+    M, V, p = 100, 9000, 0.7
+    step = {F32: 0.0, F16: 2.0 ** -10, BF16: 2.0 ** -7}[dt] * abs(shift)  # spread over some of the type's steps
+    z = (shift + max(t, step) * torch.randn(M, V, generator=g, device="cuda")).to(dt)
+    u = _u_at_borders(z, t, p, cpu)
+    got = _heads().sample_labels(z, u, temperature=t, top_p=p)
+    want = dl.sample(z, u, temperature=t, top_p=p)
+    assert torch.equal(got.cpu(), want), int((got.cpu() != want).sum())

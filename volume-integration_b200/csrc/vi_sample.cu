@@ -810,7 +810,7 @@ struct LongShared {
 // What the passes over a row leave for the draw.
 enum { kDone, kFromList, kWhole };
 struct RowNote {
-  double all;       // mass beside exp2(ref scale)
+  double all;       // mass beside exp2 of ref scale, as rounded to float32
   float best, ref;
   int state;
   int n[16];        // candidates of each warp
@@ -1194,7 +1194,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : 2) sample_long_kernel(con
     ref = O::value(max(team.most(O::of(ref)), O::of(-INFINITY)));
     const bool workable = plain_scale(s, ref) || (greedy && fabsf(ref) < INFINITY);
 
-    const float ref_scaled = ref * scale;  // its rounding is a factor of all weights alike
+    const float ref_scaled = __fmul_rn(ref, scale);  // its rounding is a factor of all weights alike, up to 0.3% (plain_scale)
 
     // one pass over the row, for sums of the weights beside 2^(ref scale), or for the labels from `guess` on
     float best = -INFINITY;
@@ -1352,7 +1352,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : 2) sample_long_kernel(con
       // more of the tail, if what is held is not enough
       __syncwarp();
       double m = 0.0;
-      for (int i = lane; i < min(n, kListWarp); i += 32) m += exp2_fast((r.at(candidates[i]) - ref) * scale);
+      for (int i = lane; i < min(n, kListWarp); i += 32) m += exp2_fast(fmaf(r.at(candidates[i]), scale, -ref_scaled));
       if (team.sum(m) > s.p * all * (1.0 + 1e-5)) break;
       tail = 0.3f;
     }
@@ -1465,7 +1465,9 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : 1) sample_held_kernel(con
       }
       double all = -1.0, slack = 0.0;  // all: the row's mass, known to the slack
       if (top_p) {
-        const double far = fmax(0.0, (double)(best - note.ref) * s.scale), up = exp2((double)(note.ref - best) * (double)(float)s.scale);
+        // the passes' weights are beside 2^ref_scaled, as rounded there; here they are beside the largest's
+        const float scale = (float)s.scale, ref_scaled = __fmul_rn(note.ref, scale);
+        const double far = fmax(0.0, (double)(best - note.ref) * s.scale), up = exp2((double)ref_scaled - (double)best * (double)scale);
         all = note.all * up;
         slack = 0.5 * all * (a.margin + far * a.margin_far);
         if (!(far < 8.0)) all = INFINITY;  // the sum in float32 counts on a sample that comes near the largest
