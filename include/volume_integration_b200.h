@@ -446,7 +446,8 @@ int vi_linear_act_int8(int dtype, int activation, const vi_matrix* x, const floa
  * index at which the sum of the kept w, in index order, exceeds u_m times their sum (u_m in [0, 1), float32; below 0 it is 0, from
  * 1 on the answer is the last one kept).  temperature 0: the first of the largest.  A row whose logits are all -inf, or hold a NaN, has label -1; a +inf takes all
  * mass (several share it).  Each setting is one value, or an array of one per row where its array is not NULL (there a
- * temperature of 0 or less is 0, one that is NaN gives -1, a top_k under 1 is off, a top_p of 0 or less keeps the first).
+ * temperature of 0 or less is 0, one that is NaN gives -1, a top_k under 1 is off, a top_p of 0 or less keeps the first, a
+ * min_p above 1 is 1, which keeps the largest, one under 0 is off; a top_p or min_p that is NaN is off).
  * Weights and sums are 64 bits wide.
  */
 typedef struct vi_sampling {

@@ -115,3 +115,24 @@ def test_top_p_of_long_rows_far_from_zero(shift, t, dt):
     got = _heads().sample_labels(z, u, temperature=t, top_p=p)
     want = dl.sample(z, u, temperature=t, top_p=p)
     assert torch.equal(got.cpu(), want), int((got.cpu() != want).sum())
+
+
+# ---- settings at the ends of their ranges ----
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("V,order", [(20, "rows"), (40, "image"), (400, "image"), (3000, "rows"), (9000, "rows"), (9000, "image")])
+def test_settings_by_row_outside_their_ranges(V, order, dt):
+    # a min_p above 1 keeps the largest, as 1 does; top_p and min_p that are no numbers, and a negative min_p, are off
+    nan = float("nan")
+    g = _gen(V)
+    M = 48
+    z = hl.matrix(M, V, dt, g, order, scale=3.0)
+    z[7, [3, V - 1]] = z[7].max() + 1  # two largest
+    u = torch.rand(M, generator=g, device="cuda")
+    m = torch.tensor([1.0, 1.5, 2.0, 1e30, INF, nan, -1.0, 7.0, 0.0, 0.3, -INF, 1 + 2.0 ** -23], device="cuda").repeat(4)
+    p = torch.tensor([nan, 0.9, 1.5, INF, nan, 0.0, -1.0, -INF], device="cuda").repeat(6)
+    means = m.nan_to_num(nan=0.0, posinf=1.0).clamp(0, 1)
+    for extra in (dict(), dict(temperature=0.5), dict(top_k=9), dict(top_p=0.8)):
+        got = _heads().sample_labels(z, u, min_p=m, **extra)
+        assert torch.equal(got.cpu(), dl.sample(z, u, min_p=means, **extra)), extra
+    got = _heads().sample_labels(z, u, top_p=p, min_p=0.01)
+    assert torch.equal(got.cpu(), dl.sample(z, u, top_p=p.nan_to_num(nan=1.0), min_p=0.01))

@@ -88,6 +88,7 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int64_t row) 
   s.t = a.temperature ? (double)a.temperature[row] : a.temperature_all;
   s.p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
   s.m = a.min_p ? (double)a.min_p[row] : a.min_p_all;
+  if (s.m > 1.0) s.m = 1.0;  // a row's own: the largest is always kept
   s.k = a.top_k ? a.top_k[row] : a.top_k_all;
   s.u = fmax((double)a.u[row], 0.0);  // under 0, or a NaN: the first one kept
   s.scale = a.temperature ? kLog2e64 / s.t : a.scale_all;

@@ -259,9 +259,10 @@ def sample_labels(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     ``temperature`` 0 takes the first of the largest.
 
     Each setting is a number, or a tensor [...] with one value a row (top_k int64, the others float32; a row's
-    temperature of 0 or less is 0, a top_k under 1 is off, a top_p of 0 or less keeps the first).  Logits of -inf
-    are never drawn; a row without any other, or with a NaN, answers -1; +inf takes all mass.  Weights and sums are
-    64 bits wide, so the answer is the definition's but where u falls within about 1e-10 of a border.
+    temperature of 0 or less is 0, one that is NaN answers -1, a top_k under 1 is off, a top_p of 0 or less keeps the
+    first, a min_p above 1 is 1; a top_p or min_p that is NaN is off).  Logits of -inf are never drawn; a row without
+    any other, or with a NaN, answers -1; +inf takes all mass.  Weights and sums are 64 bits wide, so the answer is the
+    definition's but where u falls within about 1e-10 of a border.
     """
     what = "sample_labels"
     if logits.dim() < 1 or logits.shape[-1] < 1:
