@@ -136,3 +136,29 @@ def test_settings_by_row_outside_their_ranges(V, order, dt):
         assert torch.equal(got.cpu(), dl.sample(z, u, min_p=means, **extra)), extra
     got = _heads().sample_labels(z, u, top_p=p, min_p=0.01)
     assert torch.equal(got.cpu(), dl.sample(z, u, top_p=p.nan_to_num(nan=1.0), min_p=0.01))
+
+
+# ---- waits that run out ----
+def test_a_wait_that_runs_out_for_one_lane_ends_the_block(monkeypatch):
+    # every copy arrives, but one lane's wait counts as run out: its warp, or block, gives up as one, and the status word says so
+    heads, g = _heads(), _gen(43)
+    w = heads.quantize_rows(hl.matrix(64, 64, F32, g))
+    u = torch.rand(70000, generator=g, device="cuda")
+    calls = []
+    for dt in (F16, BF16):
+        for order in ("rows", "image"):
+            x = hl.matrix(70000, 64, dt, g, order)
+            calls.append(lambda x=x: heads.linear_act_int8(x, w, residual=x, activation="gelu"))
+    for dt in (F32, F16, BF16):
+        z = hl.matrix(70000, 21, dt, g, "image")
+        calls.append(lambda z=z: heads.sample_labels(z, u, min_p=0.02))
+    before = [call() for call in calls]
+    assert heads.device_status() == 0
+    monkeypatch.setenv("VI_HEADS_TEST_TIMEOUT", "2")
+    for call in calls:
+        call()
+        assert heads.device_status(reset=True) == 8
+    monkeypatch.delenv("VI_HEADS_TEST_TIMEOUT")
+    for call, want in zip(calls, before):
+        assert torch.equal(call(), want)
+    assert heads.device_status() == 0

@@ -200,9 +200,9 @@ struct SampleArgs {
   double scale_all, log2_min_p_all, cut_all;  // set by the launcher: log2(e) / temperature_all; their quotient
   void* scratch;             // sample_scratch() bytes
   int64_t list_at, list_bytes;  // set by the launcher: where the rows' candidates lie in it
-  uint32_t* status;          // set by the launcher: the word of the heads' timeouts; how long a wait lasts; a testing hook
-  int64_t wait_limit;
-  int withhold;
+  uint32_t* status;          // set by the launcher: the word of the heads' timeouts; how long a wait lasts; testing hooks (the
+  int64_t wait_limit;        // first copy is never issued; one thread's wait counts as run out)
+  int withhold, lapse;
   float margin;              // set by the launcher: how near to a border float32 does not decide, of the whole sum
   float margin_far;          // set by the launcher: more of it by octaves between the guessed and the true largest
 };

@@ -33,7 +33,8 @@ struct FusedArgs {
   int K, N, image;
   uint32_t idesc;
   int64_t wait_limit;  // cycles
-  int withhold;        // testing hook: the first load is never issued
+  int withhold;        // testing hooks: the first load is never issued;
+  int lapse;           // one lane's wait counts as run out
   uint32_t* status;
   Epilogue e;
 };
@@ -88,7 +89,9 @@ __global__ void __launch_bounds__(Fused<T>::kThreads, 1) int8_fused_kernel(const
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, i++) {
       const uint32_t base = smem_u32(smem) + (i & 1) * S::kStage, x = smem_u32(smem + S::kX) + xs * S::kXBytes;
       // the last product that read this stage has ended, and with it the epilogue of four tiles ago
-      if (!mbar_wait(xfull + 8 * xs, xphase, dead, a.wait_limit) || !mbar_wait(aempty + 8 * (i & 1), (i / 2 & 1) ^ 1, dead, a.wait_limit)) break;
+      bool on = mbar_wait(xfull + 8 * xs, xphase, dead, a.wait_limit) && mbar_wait(aempty + 8 * (i & 1), (i / 2 & 1) ^ 1, dead, a.wait_limit);
+      if (a.lapse && lane == 5) on = false, *dead = 1;
+      if (!__all_sync(0xffffffffu, on)) break;  // the lanes leave together: what follows exchanges between them
       if (a.image) {  // a lane: two neighbouring pixels, half of the channels
         const int pair_row = first + lane % 16 * 2, k0 = lane / 16 * (kFusedK / 2);
         const uint32_t own = x + pair_row * 2 + k0 * (S::kRows * 2);
@@ -341,7 +344,8 @@ int launch_int8_fused(int dtype, int64_t M, const View& x, const Operand& B, con
   a.idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kFusedN >> 3) << 17) | ((128u >> 4) << 24);
   const char* test = getenv("VI_HEADS_TEST_TIMEOUT");
   a.withhold = test && test[0] == '1';
-  a.wait_limit = a.withhold ? 1 << 20 : kWaitLimit;
+  a.lapse = test && test[0] == '2';
+  a.wait_limit = a.withhold || a.lapse ? 1 << 20 : kWaitLimit;
   a.status = status_word();
   a.e = e;
   if (!a.status) return set_error(VI_ERR_CUDA, "heads: the status word has no address");

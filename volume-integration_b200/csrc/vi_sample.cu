@@ -652,7 +652,9 @@ __global__ void __launch_bounds__(kTileThreads) sample_tiles_kernel(const __grid
       mbar_expect(bar, a.V * kTileThreads * 4);
       tma_load<false>(smem_u32(words), &map, bar, (int)(tile * kTileThreads * PX), 0, 0);
     }
-    if (!mbar_wait(bar, phase, dead, a.wait_limit)) break;
+    bool on = mbar_wait(bar, phase, dead, a.wait_limit);
+    if (a.lapse && tid == 37) on = false, *dead = 1;
+    if (!__syncthreads_and(on)) break;  // the block leaves together: what follows exchanges between lanes, and has a barrier
     const int64_t row = (tile * kTileThreads + tid) * PX;
     uint32_t again = 0;  // pixels that float32 does not decide
     float best[PX];
@@ -1560,7 +1562,8 @@ cudaError_t launch(const SampleArgs& a, int sms, cudaStream_t s) {
       b.status = status_word();
       const char* test = getenv("VI_HEADS_TEST_TIMEOUT");
       b.withhold = test && test[0] == '1';
-      b.wait_limit = b.withhold ? 1 << 20 : kWaitLimit;
+      b.lapse = test && test[0] == '2';
+      b.wait_limit = b.withhold || b.lapse ? 1 << 20 : kWaitLimit;
       if (fn && b.status &&
           fn(&map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(a.z.p), dims, strides, box,
              unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
