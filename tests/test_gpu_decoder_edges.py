@@ -162,3 +162,40 @@ def test_a_wait_that_runs_out_for_one_lane_ends_the_block(monkeypatch):
     for call, want in zip(calls, before):
         assert torch.equal(call(), want)
     assert heads.device_status() == 0
+
+
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("M,V,order", [(3000, 400, "image"), (3001, 1000, "image"), (3000, 33, "image"), (300, 500, "rows")])
+def test_min_p_of_1_draws_among_the_largest(M, V, order, dt):
+    g = _gen(V)
+    z = hl.matrix(M, V, dt, g, order, scale=3.0)
+    top = z.amax(1)
+    z[::3, V // 2] = top[::3]                                     # two largest
+    z[1::3, 7] = torch.nextafter(top[1::3].float(), top[1::3].float() - 1).to(dt)  # float32: the next one below
+    u = torch.rand(M, generator=g, device="cuda")
+    for t, m in ((1.0, 1.0), (3.0, 1.0), (1.0, 1 - 2.0 ** -24), (1.0, 1 - 2e-7), (0.5, 1 - 1e-6), (1.0, 1 - 1e-5), (1.0, 1 - 4e-5)):
+        got = _heads().sample_labels(z, u, temperature=t, min_p=m)
+        assert torch.equal(got.cpu(), dl.sample(z, u, temperature=t, min_p=m)), (t, m)
+
+
+@pytest.mark.parametrize("dt", **TYPES)
+def test_min_p_of_1_takes_no_longer_than_less(dt):
+    # an image of 257 to 1024 labels: its largest logits, whose weight is 1, are no cause for doing a pixel again in 64 bits
+    # (10 to 17 times as long)
+    heads, g = _heads(), _gen(44)
+    z = hl.matrix(100000, 400, dt, g, "image", scale=3.0)
+    u = torch.rand(100000, generator=g, device="cuda")
+
+    def fastest(min_p):
+        times = []
+        for _ in range(8):
+            ends = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+            ends[0].record()
+            heads.sample_labels(z, u, min_p=min_p)
+            ends[1].record()
+            torch.cuda.synchronize()
+            times.append(ends[0].elapsed_time(ends[1]))
+        return min(times)
+
+    usual = fastest(0.5)
+    assert fastest(1.0) <= 3 * usual and fastest(1 - 1e-5) <= 3 * usual

@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kImageThreads) sample_image_kernel(const __gri
     uint32_t again = 0;  // pixels that float32 does not decide
     if (here) {
       const T* p = (const T*)a.z.p + row * a.z.rs;
-      float best[PX], scale[PX], least[PX];
+      float best[PX], scale[PX], least[PX], reach[PX];  // reach: how near to least float32 does not decide
       bool first[PX];  // temperature 0
 #pragma unroll
       for (int j = 0; j < PX; j++) best[j] = -INFINITY;
@@ -524,6 +524,11 @@ __global__ void __launch_bounds__(kImageThreads) sample_image_kernel(const __gri
         }
         scale[j] = (float)s[j].scale;
         least[j] = (float)s[j].m;
+        // The largest's weight, which is 1 exactly, is not in doubt.  Weights next to it are off by 2^-22 alone, as their
+        // exponents are next to 0.  A min_p of 1 keeps the largest only: a scale that leaves no other weight at 1.
+        reach[j] = 3e-5f * least[j];
+        if (1.0f - least[j] > 1e-6f) reach[j] = fminf(reach[j], 1.0f - least[j]);
+        if (s[j].m >= 1.0) scale[j] = FLT_MAX, reach[j] = 0.0f;
       }
       if (firsts) {
         int at[PX];
@@ -544,7 +549,7 @@ __global__ void __launch_bounds__(kImageThreads) sample_image_kernel(const __gri
         bool doubt[PX] = {};
         const auto weight = [&](float z, int j) {
           const float x = exp2_fast((z - best[j]) * scale[j]);
-          doubt[j] |= fabsf(x - least[j]) < 3e-5f * least[j];
+          doubt[j] |= fabsf(x - least[j]) < reach[j];
           return x < least[j] ? 0.0f : x;
         };
         for (int c = 0; c < kPieces; c++) {
