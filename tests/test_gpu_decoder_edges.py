@@ -199,3 +199,20 @@ def test_min_p_of_1_takes_no_longer_than_less(dt):
 
     usual = fastest(0.5)
     assert fastest(1.0) <= 3 * usual and fastest(1 - 1e-5) <= 3 * usual
+
+
+# ---- launches ----
+@pytest.mark.parametrize("M,K,launches", [(4, 5000, 3), (4, 4000, 2), (9, 5000, 3), (9, 48, 3)])
+def test_linear_act_int8_copies_unaligned_weights_once(M, K, launches):
+    # weights whose rows do not lie 16 bytes apart are copied by one launch; beside it: up to 8 rows of up to 4096 features are
+    # one, else the rows' quantising and the product
+    heads, g, lib = _heads(), _gen(K), ha.load()
+    lib.vi_kernel_launches.restype = ctypes.c_uint64
+    x = hl.matrix(M, K, BF16, g)
+    q, s = heads.quantize_rows(hl.matrix(70, K, F32, g))
+    odd = torch.empty(70, K + 1, device="cuda", dtype=torch.int8)[:, :K]
+    odd.copy_(q)
+    before = lib.vi_kernel_launches()
+    y = heads.linear_act_int8(x, (odd, s))
+    assert lib.vi_kernel_launches() - before == launches
+    assert torch.equal(y, heads.linear_act_int8(x, (q, s)))

@@ -1185,16 +1185,12 @@ int int8_forward(Run& r, int dtype, int act, const vi_matrix* x, const float* x_
   e.out = view(y);
   e.col_scale = w_scale;
   e.row_scale = x_scale;
-  if (!x_scale && M <= 8) {
-    const size_t mark = r.cur;
+  if (!x_scale && int8_few(M, K)) {
     if (int rc = operand8(r, w, B)) return rc;
-    if (int8_few(M, K, B)) {
-      if (r.dry) return VI_OK;
-      const cudaError_t rc = launch_int8_few(dtype, M, view(x), B, e, r.s);
-      r.launches++;
-      return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
-    }
-    r.release(mark);
+    if (r.dry) return VI_OK;
+    const cudaError_t rc = launch_int8_few(dtype, M, view(x), B, e, r.s);
+    r.launches++;
+    return rc == cudaSuccess ? VI_OK : set_error(VI_ERR_CUDA, cudaGetErrorString(rc));
   }
   if (!x_scale && int8_fused(dtype, M, N, K, view(x))) {
     if (int rc = operand8(r, w, B)) return rc;

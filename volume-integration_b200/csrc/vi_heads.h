@@ -180,7 +180,7 @@ struct QuantArgs {
 };
 cudaError_t launch_quantize(int dtype, const QuantArgs& a, int sms, cudaStream_t s);
 // kEpiInt8's product for up to 8 float rows, quantised on the way (vi_quant.cu); w's rows lie a multiple of 16 bytes apart.
-bool int8_few(int64_t M, int64_t K, const Operand& w);
+bool int8_few(int64_t M, int64_t K);
 cudaError_t launch_int8_few(int dtype, int64_t M, const View& x, const Operand& w, const Epilogue& e, cudaStream_t s);
 // Copies [rows, k] 8-bit integers of any strides to rows `ld` apart.
 cudaError_t launch_pack8(const View& src, int64_t rows, int64_t k, int8_t* dst, int64_t ld, cudaStream_t s);

@@ -383,9 +383,7 @@ cudaError_t launch_quantize(int dtype, const QuantArgs& a, int sms, cudaStream_t
   else c.run<__nv_bfloat16>();
   return cudaPeekAtLastError();
 }
-bool int8_few(int64_t M, int64_t K, const Operand& w) {
-  return M <= kFewRows && K <= kFewTerms && (uintptr_t)w.p % 16 == 0 && w.ld % 16 == 0;
-}
+bool int8_few(int64_t M, int64_t K) { return M <= kFewRows && K <= kFewTerms; }
 cudaError_t launch_int8_few(int dtype, int64_t M, const View& x, const Operand& w, const Epilogue& e, cudaStream_t s) {
   FewArgs a{(int)M, (int)w.rows, (int)w.k, e.act, x, e.res, e.out, (const int8_t*)w.p, w.ld, e.col_scale, e.bias};
   const unsigned blocks = (unsigned)ceil_div(w.rows, kThreads / 32 * kFewColumns);
