@@ -216,3 +216,31 @@ def test_linear_act_int8_copies_unaligned_weights_once(M, K, launches):
     y = heads.linear_act_int8(x, (odd, s))
     assert lib.vi_kernel_launches() - before == launches
     assert torch.equal(y, heads.linear_act_int8(x, (q, s)))
+
+
+def test_quantize_rows_of_images_from_several_threads():
+    # calls of a C host's threads that need different amounts of shared memory, at once
+    import threading
+    lib, p, g = ha.load(), ctypes.c_void_p, _gen(47)
+    lib.vi_quantize_rows.argtypes = [ctypes.c_int, ctypes.POINTER(ha.Matrix), ctypes.POINTER(ha.Matrix), p, p]
+    sizes, out, failed = (2600, 1000, 2600, 1200), [], []
+    for K in sizes:
+        x = hl.matrix(100, K, BF16, g, "image")
+        out.append((x, torch.zeros(100, (K + 15) // 16 * 16, device="cuda", dtype=torch.int8)[:, :K], torch.zeros(100, device="cuda")))
+    torch.cuda.synchronize()
+
+    def calls(x, q, scale):
+        for _ in range(3000):
+            if lib.vi_quantize_rows(2, ha.matrix(x), ha.matrix(q), p(scale.data_ptr()), None):
+                failed.append(lib.vi_last_error())
+
+    threads = [threading.Thread(target=calls, args=o) for o in out]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, (len(failed), failed[0])
+    for x, q, scale in out:
+        wq, ws = dl.quantize(x)
+        assert torch.equal(q, wq) and torch.equal(scale, ws)

@@ -341,9 +341,11 @@ struct Call {
   bool image() {
     const int warps = (int)std::min<int64_t>(16, ceil_div(ceil_div(a.K, 4), R / 4));
     const size_t smem = (size_t)32 * VP * ((ceil_div(a.K, 4) | 1) + 2 * warps) * 4;
-    if (smem > 200 * 1024) return false;
+    constexpr int kMost = 200 * 1024;
+    if (smem > kMost) return false;
     auto* kernel = quantize_image_kernel<T, VP, R, LONG>;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    // the most that any call asks for, as another thread's call may need more than this one
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) {
       cudaGetLastError();
       return false;
     }
