@@ -244,3 +244,14 @@ def test_quantize_rows_of_images_from_several_threads():
     for x, q, scale in out:
         wq, ws = dl.quantize(x)
         assert torch.equal(q, wq) and torch.equal(scale, ws)
+
+
+# ---- scales ----
+@pytest.mark.parametrize("power", [-140, -96, -95, -80, -1, 0, 126, 127])
+def test_scales_are_the_rounded_quotients_of_every_significand(power):
+    x = torch.arange(1 << 23, 1 << 24, dtype=torch.int64).double().mul(2.0 ** -23).mul(2.0 ** power)
+    x = x[x <= torch.finfo(F32).max].float()  # under 2^-126 some are rounded: still values of the type
+    # rounded twice, which is as once: no quotient by 127 lies within 1 / 254 of a step of float32's halves but on them
+    want = (x.double() / 127).float()
+    _, scale = _heads().quantize_rows(x.cuda().unsqueeze(1))
+    assert torch.equal(scale.cpu(), want)

@@ -20,7 +20,11 @@ struct Scale {
   // of the largest magnitude's bits
   __device__ __forceinline__ explicit Scale(uint32_t top) {
     const float x = __uint_as_float(top);
-    if (top >= 0x10000000u && top < 0x7f000000u) {  // within normal numbers a rounded reciprocal and one correction divide exactly
+    // Division by a constant as P. Markstein published it (IBM J. Res. Dev. 34, 1990): with r the rounded reciprocal and q within one
+    // last place of x / 127, the rest x - 127 q is exact in one fused operation and q + r rest is the rounded quotient.  r is
+    // off by 2^-28 of itself and x r is rounded once more, so q is within one last place.  The bounds keep every step among
+    // normal numbers, the rest (down to 2^-24 of x) too.
+    if (top >= 0x10000000u && top < 0x7f000000u) {
       constexpr float r = 1.0f / 127.0f;
       const float q = x * r;
       s = fmaf(fmaf(-127.0f, q, x), r, q);
