@@ -12,9 +12,9 @@ namespace {
 
 // ---- few features: quantised on the way into the product ----
 // Up to 64 features and 64 channels of 16-bit types are bound by memory and by the epilogue, and a pass that quantises would
-// write and read the features once more (2M x 64 -> 64 with gelu and a residual: 284 us + 235 apart).  Here one warp
-// copies 256 rows of x at a time into shared memory (316 us in all: the latency of 26 warps at 72 registers), eight find their scales and write the tensor core's operand, two products
-// of 128 rows follow, and 8 warps run the epilogue.
+// write and read the features once more (2M x 64 -> 64 with gelu and a residual: 284 us + 235 apart).  Here one warp copies 256
+// rows of x at a time into shared memory, eight find their scales and write the tensor core's operand, two products of 128 rows
+// follow, and 16 warps run the epilogue: 317 us in all, the latency of 26 warps at 72 registers.
 constexpr int kFusedK = 64, kFusedN = 64;
 template <typename T>
 struct Fused {
@@ -28,7 +28,6 @@ struct Fused {
   static_assert(kSmem <= 227 * 1024, "shared memory of a block");
 };
 struct FusedArgs {
-  View x;
   int64_t M;
   int K, N, image;
   uint32_t idesc;
@@ -217,51 +216,44 @@ __global__ void __launch_bounds__(Fused<T>::kThreads, 1) int8_fused_kernel(const
     int i = 0;
     bool on = true;
     for (int64_t t = blockIdx.x; t < tiles && on; t += gridDim.x, i++) {
-      {
-        const int half = warp / 8;
-        const int row = half * 128 + quad * 32;
-        const int64_t m0 = t * S::kRows + row;
-        const bool some = m0 < a.M && c < a.N;
-        const Place here{(int)m0, c, (int)min((int64_t)32, a.M - m0), min(32, a.N - c)};
-        Row<T> extra, y;
-        int way = kNone;
-        if (some && e.res.p) way = load_tile<T>(extra, e.res, res_access, st, lane, here);  // asked for before the product is waited for
-        {
-          on = mbar_wait(sfull + 8 * (i & 3), i / 4 & 1, dead, a.wait_limit) && mbar_wait(tfull + 8 * (i & 1), i / 2 & 1, dead, a.wait_limit);
-          on = __all_sync(0xffffffffu, on);
-          if (!on) break;
-          fence_after();
-        }
-        if (some) {
-          const float row_scale = scales[(i & 3) * S::kRows + row + lane];
-          const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + (i & 1) * 128 + half * 64 + c;
-          if (e.res.p) own_row<T>(extra, way, st, lane);
+      const int half = warp / 8, row = half * 128 + quad * 32;
+      const int64_t m0 = t * S::kRows + row;
+      const bool some = m0 < a.M && c < a.N;
+      const Place here{(int)m0, c, (int)min((int64_t)32, a.M - m0), min(32, a.N - c)};
+      Row<T> extra, y;
+      int way = kNone;
+      if (some && e.res.p) way = load_tile<T>(extra, e.res, res_access, st, lane, here);  // asked for before the product is waited for
+      on = mbar_wait(sfull + 8 * (i & 3), i / 4 & 1, dead, a.wait_limit) && mbar_wait(tfull + 8 * (i & 1), i / 2 & 1, dead, a.wait_limit);
+      on = __all_sync(0xffffffffu, on);
+      if (!on) break;
+      fence_after();
+      if (some) {
+        const float row_scale = scales[(i & 3) * S::kRows + row + lane];
+        const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + (i & 1) * 128 + half * 64 + c;
+        if (e.res.p) own_row<T>(extra, way, st, lane);
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            float2 v[8];
-            tmem_load16(src + h * 16, (float*)v);
-            tmem_wait_load();
-            scale_sums(bias_slot + 128 + h * 64, row_scale, v);
-            if (e.bias) add_bias<16>(bias_slot + h * 64, v);
+        for (int h = 0; h < 2; h++) {
+          float2 v[8];
+          tmem_load16(src + h * 16, (float*)v);
+          tmem_wait_load();
+          scale_sums(bias_slot + 128 + h * 64, row_scale, v);
+          if (e.bias) add_bias<16>(bias_slot + h * 64, v);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-              float2 w, d;
-              activate<ACT, false, false>(v[j], w, d);
-              v[j] = ACT == VI_ACT_RELU ? relu_signed_zero<T>(w) : w;
-              if (e.res.p) v[j] = __fadd2_rn(v[j], get_pair(extra, h * 8 + j));
-              set_pair(y, h * 8 + j, v[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) asm volatile("" : "+r"(y.w[h * 8 + j]));
+          for (int j = 0; j < 8; j++) {
+            float2 w, d;
+            activate<ACT, false, false>(v[j], w, d);
+            v[j] = ACT == VI_ACT_RELU ? relu_signed_zero<T>(w) : w;
+            if (e.res.p) v[j] = __fadd2_rn(v[j], get_pair(extra, h * 8 + j));
+            set_pair(y, h * 8 + j, v[j]);
           }
+#pragma unroll
+          for (int j = 0; j < 8; j++) asm volatile("" : "+r"(y.w[h * 8 + j]));
         }
-        {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(tempty + 8 * (i & 1));
-        }
-        if (some) store_tile(y, e.out, out_access, st, lane, here);
       }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tempty + 8 * (i & 1));
+      if (some) store_tile(y, e.out, out_access, st, lane, here);
     }
   }
   __syncwarp();
@@ -336,7 +328,6 @@ int launch_int8_fused(int dtype, int64_t M, const View& x, const Operand& B, con
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return set_error(VI_ERR_CUDA, "heads: a tensor map could not be encoded");
   FusedArgs a{};
-  a.x = x;
   a.M = M;
   a.K = (int)B.k;
   a.N = (int)B.rows;

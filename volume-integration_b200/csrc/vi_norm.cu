@@ -757,16 +757,6 @@ struct Call {
   template <auto kernel>
   void run(int threads, size_t smem, int64_t units, int lanes, int per) {
     static std::atomic<int> known[33];  // blocks per SM by warps a block (shared memory differs little)
-    static std::atomic<uint64_t> large;  // devices on which the kernel may have more than 48 KB
-    if (smem > 48 * 1024) {
-      int dev = 0;
-      cudaGetDevice(&dev);
-      const uint64_t bit = 1ull << (dev & 63);
-      if (dev >= 64 || !(large.load(std::memory_order_relaxed) & bit)) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) cudaGetLastError();
-        else if (dev < 64) large.fetch_or(bit, std::memory_order_relaxed);
-      }
-    }
     int n = known[threads / 32].load(std::memory_order_relaxed);
     if (n <= 0) {
       if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) == cudaSuccess && n > 0)
