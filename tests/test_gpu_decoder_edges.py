@@ -255,3 +255,21 @@ def test_scales_are_the_rounded_quotients_of_every_significand(power):
     want = (x.double() / 127).float()
     _, scale = _heads().quantize_rows(x.cuda().unsqueeze(1))
     assert torch.equal(scale.cpu(), want)
+
+
+# ---- draws at the ends of u ----
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("M,V,order", [(40, 21, "rows"), (300, 100, "image"), (300, 300, "image"), (40, 3000, "rows"),
+                                       (40, 20000, "rows"), (200, 50001, "rows"), (40, 20000, "image")])
+def test_u_of_0_draws_the_first_label_with_weight(M, V, order, dt):
+    # however little it weighs beside the ones behind it
+    g = _gen(V)
+    z = hl.matrix(M, V, dt, g, order, scale=30.0)
+    z[::2, :V // 3] = -INF
+    u = torch.zeros(M, device="cuda")
+    for t in (1.0, 0.7, 3.0):
+        w = torch.exp((z.double() - z.double().amax(1, keepdim=True)) / t)
+        want = (w > 2.0 ** -999).to(torch.uint8).argmax(1)  # the kernel's least weight is 2^-1000
+        for settings in (dict(), dict(top_p=1.0), dict(min_p=0.0, top_k=2 * V)):
+            got = _heads().sample_labels(z, u, temperature=t, **settings)
+            assert torch.equal(got, want), (t, settings, int((got != want).sum()))

@@ -1076,8 +1076,9 @@ __device__ __noinline__ int whole_row(Team<W>& team, LongShared<W>& sh, const Ro
   // the warp whose part holds the draw (u of 1 and more: every warp, for its last label)
   uint32_t hit = 0, last = 0;
   if (mine > 0.0 && ((before <= want && before + mine > want) || !(s.u < 1.0))) {
-    const double f0 = before + run - m1 - m0, f1 = before + run - m1;  // in front of the lane's groups
-    const uint32_t holds = __ballot_sync(kAll, (f1 > want && m0 > 0.0) || (before + run > want && m1 > 0.0));
+    // in front of the lane's groups: sums of what lies there alone, so that in front of the first label with weight there is 0
+    const double others = __shfl_up_sync(kAll, run, 1), f0 = before + (lane ? others : 0.0), f1 = f0 + m0;
+    const uint32_t holds = __ballot_sync(kAll, (f1 > want && m0 > 0.0) || (f1 + m1 > want && m1 > 0.0));
     const uint32_t some_mass = __ballot_sync(kAll, m0 + m1 > 0.0);
     const int l = holds ? __ffs(holds) - 1 : 31 - __clz(some_mass);
     for (int half = 0; half < 2 && !hit; half++) {
