@@ -273,3 +273,21 @@ def test_u_of_0_draws_the_first_label_with_weight(M, V, order, dt):
         for settings in (dict(), dict(top_p=1.0), dict(min_p=0.0, top_k=2 * V)):
             got = _heads().sample_labels(z, u, temperature=t, **settings)
             assert torch.equal(got, want), (t, settings, int((got != want).sum()))
+
+
+@pytest.mark.parametrize("dt", **TYPES)
+@pytest.mark.parametrize("V,order", [(20, "rows"), (40, "image"), (400, "image"), (3000, "rows"), (9000, "rows"), (9000, "image")])
+def test_infinite_logits_take_all_mass_at_any_temperature(V, order, dt):
+    g = _gen(V)
+    M = 64
+    z = hl.matrix(M, V, dt, g, order, scale=3.0)
+    where = torch.randint(1, V, (M, 2), generator=g, device="cuda")
+    z.scatter_(1, where, INF)
+    u = torch.rand(M, generator=g, device="cuda")
+    u[:2], u[2] = 0.0, 1 - 2.0 ** -24
+    first, second = where.amin(1), where.amax(1)
+    want = torch.where((u < 0.5) | (first == second), first, second)
+    for t in (0.5, 1e6, 1e35, INF, torch.full((M,), INF, device="cuda")):
+        for settings in (dict(), dict(top_k=5), dict(top_p=0.999), dict(min_p=0.2), dict(top_k=V - 1, top_p=1.0)):
+            got = _heads().sample_labels(z, u, temperature=t, **settings)
+            assert torch.equal(got, want), (t if isinstance(t, float) else "rows", settings, int((got != want).sum()))

@@ -52,8 +52,8 @@ struct Order {
   }
 };
 
-// 2^x for x <= 0, to 1e-14 of it (0 below 2^-1000): 2^x = 2^k e^(f ln 2) with k whole and |f| <= 1/2, by the
-// exponential's series to the 12th power.
+// 2^x for x <= 0, to 1e-14 of it (0 below 2^-1000, and where x is no number: an infinite distance to the largest at an infinite
+// temperature): 2^x = 2^k e^(f ln 2) with k whole and |f| <= 1/2, by the exponential's series to the 12th power.
 __device__ __forceinline__ double pow2_64(double x) {
   constexpr double l = 0.693147180559945309417232121458;
   constexpr double c[13] = {1.0,
@@ -73,7 +73,7 @@ __device__ __forceinline__ double pow2_64(double x) {
   double p = c[12];
 #pragma unroll
   for (int i = 11; i >= 0; i--) p = fma(p, f, c[i]);
-  return x < -1000.0 ? 0.0 : __hiloint2double(__double2hiint(p) + (__double2loint(m) << 20), __double2loint(p));
+  return x >= -1000.0 ? __hiloint2double(__double2hiint(p) + (__double2loint(m) << 20), __double2loint(p)) : 0.0;
 }
 
 constexpr double kLog2e64 = 1.44269504088896340735992468100;
