@@ -1222,6 +1222,8 @@ int int8_forward(Run& r, int dtype, int act, const vi_matrix* x, const float* x_
     std::swap(e.row_scale, e.col_scale);
     std::swap(A, B);
   }
+  // The float products' costs of tiles serve: within 6% of the best width of 64, 128 and 256 at 14 of 15 sizes from 100 x 4096 ->
+  // 4096 to 65536 x 1024 -> 1024 and 2073600 x 96 -> 96; 14% at 65 channels of an image.
   p.bn = tile_width(dtype == VI_F32 ? VI_BF16 : dtype, kEpiInt8, A.rows, B.rows, 1, r.sms);
   return launch_int8_gemm(dtype, A, B, p, e, r.sms, r.s);
 }

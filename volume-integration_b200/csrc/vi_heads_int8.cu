@@ -2,7 +2,7 @@
 //
 // Mathematics.  x_mk is about s_m q_mk and w_nk about t_n p_nk with whole q and p in [-127, 127]; the sum over k of
 // q p is exact in 32 bits (under 2^17 terms), and y = act(s_m t_n sum + b_n) + res is rounded once to the type.
-// 32768 x 1024 -> 4096 with relu: 153 us, 1.8 * 10^15 operations a second; the float16 product 237.
+// 32768 x 1024 -> 4096 with relu, x quantised before: 156 us at 1965 MHz, 1.8 * 10^15 operations a second; the float16 layer 229.
 #include "vi_heads_gemm.cuh"
 #include "vi_quant.cuh"
 
@@ -309,7 +309,9 @@ cudaError_t run_act(int bn, const CUtensorMap& ma, const CUtensorMap& mb, const 
 
 }  // namespace
 
-// Few features and channels of 16-bit types, and rows enough that their bytes count, where bulk copies reach them.
+// Few features and channels of 16-bit types, and rows enough that their bytes count, where bulk copies reach them.  bfloat16
+// 64 -> 64 with gelu and a residual, image (rows): 524288 pixels 92 us (88) here, 150 (102) apart; 32768 16 (16), 27 (19); below, this
+// kernel would save up to 8 us of a call that is launches mostly: 8192 pixels 14 (14), 23 (16).
 bool int8_fused(int dtype, int64_t M, int64_t N, int64_t K, const View& x) {
   if (dtype == VI_F32 || K > kFusedK || N > kFusedN || M < 32768) return false;
   if ((uintptr_t)x.p % 16) return false;

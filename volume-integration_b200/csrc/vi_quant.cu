@@ -1,8 +1,8 @@
 // Rows of 8-bit integers with a scale each.
 //
 // Mathematics.  s = f32(max_k |x_k| / 127), q_k = x_k / s rounded to the nearest whole number, ties to even: |q| <= 127.
-// The rounding is that of the exact quotient: x times the rounded 1 / s decides it, but near halves, where a division in
-// 64 bits does.  A row of zeros has s = 0 and q = 0; one that holds an infinity or a NaN has s = NaN and q = 0, so
+// The rounding is that of the exact quotient: x times the rounded 1 / s decides it, but near halves, where the exact rest
+// x - q s does.  A row of zeros has s = 0 and q = 0; one that holds an infinity or a NaN has s = NaN and q = 0, so
 // that what is made of it is NaN.
 //
 // One pass over x, held in registers between the maximum and the rounding; memory bounds long rows (32768 x 1024 in float16: 25 us,

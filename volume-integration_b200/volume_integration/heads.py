@@ -126,8 +126,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last axis, in one pass.
 
     x: [..., K]; weight, bias: [K], either may be None; var is the mean of
-    (x - mean)^2.  Returns x's shape and type, in x's memory order, rounded once.  Statistics and
-    all sums are float32; each row's are kept for the backward (12 bytes a row).  A row's
+    (x - mean)^2.  Returns x's shape and type, rounded once, in x's memory order where its rows lie evenly
+    spaced (a batch of images does not: row by row then).  Statistics and all sums are float32; each row's are kept for the backward (12 bytes a row).  A row's
     NaN or infinity stays in its row, in the result and in x's gradient.
     """
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -188,6 +188,10 @@ def linear_act_int8(x, weight, bias=None, residual=None, activation="none", dtyp
     (x's).  K is less than 2^17: sums are exact, then scaled in float32, and results are rounded once.  Rows or channels whose scale is
     NaN come out as NaN.  For display: there is no backward, and inputs that require gradients are refused
     where they are recorded.
+
+    It pays where sums are long and outputs many (32768 x 1024 -> 4096 in float16: 180 us, linear_act 229), where several
+    layers of 512 features and more read one pair, and for float32 x.  16-bit layers of up to 512 features take longer than in linear_act, as
+    finding the scales costs a pass over x (1920 x 1080 x 64 -> 64: 324 us, linear_act 209).
     """
     what = "linear_act_int8"
     wq, ws = _check_pair(weight, what, "weight")
@@ -261,8 +265,11 @@ def sample_labels(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     Each setting is a number, or a tensor [...] with one value a row (top_k int64, the others float32; a row's
     temperature of 0 or less is 0, one that is NaN answers -1, a top_k under 1 is off, a top_p of 0 or less keeps the
     first, a min_p above 1 is 1; a top_p or min_p that is NaN is off).  Logits of -inf are never drawn; a row without
-    any other, or with a NaN, answers -1; +inf takes all mass.  Weights and sums are 64 bits wide, so the answer is the
-    definition's but where u falls within about 1e-10 of a border.
+    any other, or with a NaN, answers -1; +inf takes all mass.  Weights (from 2^-1000 on) and sums are 64 bits wide
+    where they decide, so the answer is the definition's but where u falls within about 1e-10 of a border.
+
+    Fast on images (channel-first logits) of up to 256 labels without top_k and top_p; with one of them an image is read
+    with strides (800 x 800 x 150 in float16: 78 us with min_p, 2 ms with top_p).
     """
     what = "sample_labels"
     if logits.dim() < 1 or logits.shape[-1] < 1:
